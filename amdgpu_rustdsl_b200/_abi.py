@@ -83,6 +83,28 @@ class Problem(C.Structure):
     ]
 
 
+class Kv4CacheArgs(C.Structure):
+    """fmha_kv4_cache of include/fmha_kv4_abi.h."""
+    _fields_ = [("pool", C.c_void_p), ("table", C.c_void_p), ("lengths", C.c_void_p), ("pages", C.c_uint64), ("B", C.c_uint32), ("HK", C.c_uint32), ("page", C.c_uint32),
+                ("table_width", C.c_uint32)]
+
+
+class Kv4Rows(C.Structure):
+    """fmha_kv4_rows: strides in elements."""
+    _fields_ = [("data", C.c_void_p), ("stride_b", C.c_int64), ("stride_s", C.c_int64), ("stride_h", C.c_int64)]
+
+
+class Kv4AttendArgs(C.Structure):
+    _fields_ = [("q", Kv4Rows), ("out", C.c_void_p), ("counts", C.c_void_p), ("lse", C.c_void_p), ("weights", C.c_void_p), ("weights_in", C.c_void_p),
+                ("workspace", C.c_void_p), ("workspace_bytes", C.c_uint64), ("weights_width", C.c_uint64), ("S", C.c_uint32), ("H", C.c_uint32), ("causal", C.c_uint32),
+                ("scale", C.c_float)]
+
+
+class Kv4EvictArgs(C.Structure):
+    _fields_ = [("weights", C.c_void_p), ("kept", C.c_void_p), ("weights_out", C.c_void_p), ("weights_width", C.c_uint64), ("weights_out_width", C.c_uint64),
+                ("keep", C.c_uint32), ("recent", C.c_uint32), ("first", C.c_uint32)]
+
+
 assert C.sizeof(AttnArgs) == 656 and C.sizeof(KvSplitArgs) == 648 and C.sizeof(CombineArgs) == 36
 assert AttnArgs.ext_ptr_peer_plan.offset == 0x38 and KvSplitArgs.ext_ptr_peer_plan.offset == 0x38
 assert AttnArgs.s_seq_len.offset == 0x60 and AttnArgs.ptr_q_descale.offset == 0x200 and AttnArgs.abi_tail.offset == 0x280
@@ -159,6 +181,17 @@ def load():
     lib.fmha_mxfp8_mma_issue_ceiling.argtypes = [C.c_int, C.c_int, C.c_void_p, C.POINTER(C.c_float)]
     lib.fmha_mxfp8_selftest_bounded_wait.restype = C.c_int
     lib.fmha_mxfp8_selftest_bounded_wait.argtypes = [C.c_uint32, C.c_void_p, C.POINTER(C.c_uint32), C.POINTER(C.c_float)]
+    cache, rows, err = C.POINTER(Kv4CacheArgs), C.POINTER(Kv4Rows), [C.c_void_p, C.c_char_p, C.c_size_t]
+    lib.fmha_kv4_append.restype = C.c_int
+    lib.fmha_kv4_append.argtypes = [cache, rows, rows, C.c_uint32, C.c_void_p] + err
+    lib.fmha_kv4_read.restype = C.c_int
+    lib.fmha_kv4_read.argtypes = [cache, rows, rows, C.c_uint32, C.c_int, C.c_void_p] + err
+    lib.fmha_kv4_attend_workspace.restype = C.c_uint64
+    lib.fmha_kv4_attend_workspace.argtypes = [cache, C.POINTER(Kv4AttendArgs)]
+    lib.fmha_kv4_attend.restype = C.c_int
+    lib.fmha_kv4_attend.argtypes = [cache, C.POINTER(Kv4AttendArgs)] + err
+    lib.fmha_kv4_evict.restype = C.c_int
+    lib.fmha_kv4_evict.argtypes = [cache, cache, C.POINTER(Kv4EvictArgs)] + err
     _lib = lib
     return lib
 
@@ -169,6 +202,10 @@ EXPORTS = (
     "fmha_mxfp8_mma_issue_ceiling", "fmha_mxfp8_selftest_bounded_wait", "fmha_mxfp8_kvsplit_static_scratch", "fmha_mxfp8_quantize_qk", "fmha_mxfp8_quantize_v", "fmha_mxfp8_combine_f32", "fmha_mxfp8_peer_alloc", "fmha_mxfp8_peer_open", "fmha_mxfp8_peer_close", "fmha_mxfp8_peer_free",
     "fmha_mxfp8_peer_plan_build", "fmha_mxfp8_combine_scatter", "fmha_mxfp8_copy_async", "fmha_mxfp8_peer_barrier",
 )
+
+
+# include/fmha_kv4_abi.h
+KV4_EXPORTS = ("fmha_kv4_append", "fmha_kv4_read", "fmha_kv4_attend_workspace", "fmha_kv4_attend", "fmha_kv4_evict")
 
 
 class ContractError(ValueError):

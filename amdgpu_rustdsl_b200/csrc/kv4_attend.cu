@@ -1,0 +1,693 @@
+// Attention of few query rows over the 4-bit cache: decode, drafts of a few tokens, and (32 rows of a KV head at a time) any number of rows.
+//
+// Work. An item is one sequence and KV head (and row tile); its tokens are cut in tiles of 128. All tiles of all items, in order, are dealt out in equal runs to the
+// CTAs, from the lengths on the device: a batch of ragged sequences keeps every CTA busy for the same time, one long sequence as well. An item that more than one CTA
+// worked on is put together from f32 partials by the combine kernel.
+//
+// A warp takes 32 tokens of a tile, 4352 bytes, which copies of whole page records (cp.async.bulk) bring to a ring of its own in shared memory, and computes both
+// products transposed, so that the tokens are the rows of the matrix instruction and the few query rows its 8 columns:
+//   S^T [16 tokens x 8 rows] = K [16 x 128] Q^T      K's codes become f16 by the conversion instruction, two per byte; the E8M0 factor of a token's 32 elements
+//                                                     multiplies the two products' sum in f32
+//   O^T [128 x 8 rows] += V^T [128 x 16 tokens] P^T  P goes from S^T's layout to the operand's by an 8 x 8 transpose between lanes; V's factors multiply P
+// Q goes in as f16 with a power of two per row taken out, which is exact for bf16 elements down to 2^-30 of the row's largest.
+//
+// Softmax in base 2 with a running reference per row. P V wants P times V's factor in f16: the reference M follows s + e, e the exponent of the token's largest V
+// factor (kept within what f32 sums of 2^(s - M) bear), so that P 2^e is at most 2^4 however large V is; the four factors of a token relative to 2^e are exact
+// in f16 down to 2^-34. M moves when a value exceeds it by more than 2^4, by a vote of the warp; the sums and O are rescaled then.
+#include "kv4.cuh"
+#include "ptx_sm100.cuh"
+
+#include <atomic>
+
+namespace b200mx {
+
+namespace {
+
+using namespace kv4;
+
+constexpr unsigned kWarps = 4, kThreads = kWarps * 32;
+constexpr unsigned kUnit = 32;                    // tokens of a warp at a time
+constexpr unsigned kTile = kWarps * kUnit;
+constexpr unsigned kUnitBytes = kUnit * FMHA_KV4_TOKEN_BYTES;
+constexpr unsigned kCtasPerSm = 4;
+constexpr float kLowest = -1e30f;                 // the reference of a row that has seen nothing
+constexpr float kSlack = 4.0f;
+// The exponent e that a token's V factors are taken relative to: within what f32 sums of 2^(s - M), which lie between 2^-kHighE and 2^(4 - kLowE) a token, bear. The
+// factors go in times 2^kUp, which the division by the sums takes out again: f16 has more room below 1 than above, and P 2^e is at most 2^4
+constexpr int kLowE = -100, kHighE = 124, kUp = 10;
+constexpr float kDown = 1.0f / (1 << kUp);
+constexpr float kLn2 = 0.69314718055994531f, kLog2e = 1.44269504088896341f;
+
+// What a unit's 32 lanes work out for its tokens, one lane a token
+struct TokenFactors {
+    float4 k[kUnit];               // 2^(E - 127) of the four K blocks
+    float2 v[kUnit];               // e, 2^-e
+    uint16_t r[kUnit / 2][4][2];   // [token pair][block][token of the pair]: V's factor over 2^(e - kUp), f16
+};
+
+template <unsigned kStages>
+struct alignas(128) WarpShared {
+    uint8_t ring[kStages][kUnitBytes];
+    TokenFactors f;
+};
+
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
+}
+
+__device__ __forceinline__ uint32_t tiles_of(const Kv4View& c, uint32_t b) { return (length_of(c, b) + kTile - 1u) / kTile; }
+
+// Sum of tiles over the sequences below `upto`, and over all, times `per` (heads x row tiles). All threads of the CTA.
+struct Sums {
+    unsigned long long below, all;
+};
+__device__ __forceinline__ Sums sum_tiles(const Kv4View& c, uint32_t upto, uint32_t per, unsigned long long (*part)[2]) {
+    unsigned long long below = 0, all = 0;
+    for (uint32_t b = threadIdx.x; b < c.B; b += kThreads) {
+        const uint32_t t = tiles_of(c, b);
+        all += t;
+        if (b < upto) below += t;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        below += __shfl_xor_sync(0xFFFFFFFFu, below, o);
+        all += __shfl_xor_sync(0xFFFFFFFFu, all, o);
+    }
+    if ((threadIdx.x & 31u) == 0u) part[threadIdx.x >> 5][0] = below, part[threadIdx.x >> 5][1] = all;
+    __syncthreads();
+    below = all = 0;
+#pragma unroll
+    for (unsigned w = 0; w < kWarps; ++w) below += part[w][0], all += part[w][1];
+    __syncthreads();
+    return {below * per, all * per};
+}
+
+// The CTAs that share `all` tiles: run w is [w * all / n, (w + 1) * all / n)
+__device__ __forceinline__ uint32_t workers(unsigned long long all, uint32_t grid) { return static_cast<uint32_t>(all < grid ? all : grid); }
+__device__ __forceinline__ unsigned long long run_begin(unsigned long long all, uint32_t n, uint32_t w) { return all * w / n; }
+__device__ __forceinline__ uint32_t worker_at(unsigned long long all, uint32_t n, unsigned long long tile) { return static_cast<uint32_t>(((tile + 1ull) * n - 1ull) / all); }
+
+// Query rows of an item as the matrix instruction's operand: rows gid of each of NT groups of eight, elements 32 blk + 8 tig .. + 7 of each block
+template <int NT>
+struct QueryRows {
+    uint32_t q[NT][4][4];   // [group][block][element pair]
+    float factor[NT][2];    // of the columns 2 tig, 2 tig + 1: scale * log2(e) * the power of two taken out
+    uint32_t limit[NT][2];  // tokens that the columns see
+};
+template <int NT>
+__device__ __forceinline__ void load_rows(QueryRows<NT>& x, const Kv4AttendParams& p, uint32_t b, uint32_t head, uint32_t row0, uint32_t length, uint32_t n) {
+    const unsigned lane = threadIdx.x & 31u, gid = lane >> 2, tig = lane & 3u;
+    const uint32_t rows = p.S * p.group;
+#pragma unroll
+    for (int g = 0; g < NT; ++g) {
+        const uint32_t row = row0 + 8u * g + gid, i = row / p.group;
+        const bool live = row < rows && i < n;
+        uint4 raw[4];
+        uint32_t amax = 0;
+#pragma unroll
+        for (int blk = 0; blk < 4; ++blk) {
+            raw[blk] = make_uint4(0u, 0u, 0u, 0u);
+            if (live) raw[blk] = ld_v4(p.q.data + b * p.q.stride_b + i * p.q.stride_s + (head * p.group + row % p.group) * p.q.stride_h + 64u * blk + 16u * tig);
+            const uint32_t w[4] = {raw[blk].x, raw[blk].y, raw[blk].z, raw[blk].w};
+#pragma unroll
+            for (int k = 0; k < 4; ++k) amax = max(amax, max((w[k] << 16) & 0x7FFFFFFFu, w[k] & 0x7FFF0000u));
+        }
+        amax = max(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, 1));
+        amax = max(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, 2));
+        // the largest element gets the exponent 14; rows of zeros, subnormals, Inf or NaN keep a factor of 1 or the largest there is
+        int field = static_cast<int>(amax >> 23);
+        if (field == 255 || amax == 0u) field = 141;
+        if (field < 15) field = 15;   // 2^(141 - field) stays normal
+        const float down = __uint_as_float(static_cast<uint32_t>(268 - field) << 23);   // 2^(14 - (field - 127))
+        const float back = __uint_as_float(static_cast<uint32_t>(field - 14) << 23);
+#pragma unroll
+        for (int blk = 0; blk < 4; ++blk) {
+            const uint32_t w[4] = {raw[blk].x, raw[blk].y, raw[blk].z, raw[blk].w};
+#pragma unroll
+            for (int k = 0; k < 4; ++k) x.q[g][blk][k] = pack_f16x2(__uint_as_float(w[k] << 16) * down, __uint_as_float(w[k] & 0xFFFF0000u) * down);
+        }
+        const uint32_t lim = !live ? 0u : p.causal ? length - n + i + 1u : length;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const int src = static_cast<int>(2u * tig + j) * 4;   // a lane that holds that row
+            x.factor[g][j] = __shfl_sync(0xFFFFFFFFu, back, src) * p.scale_log2;
+            x.limit[g][j] = __shfl_sync(0xFFFFFFFFu, lim, src);
+        }
+    }
+}
+
+// S^T of 16 tokens: the K codes at `codes` (row-major, 64 bytes a token), factors f[0 .. 15]
+template <int NT>
+__device__ __forceinline__ void scores(float (&s)[NT][4], const uint8_t* codes, const float4* f, const QueryRows<NT>& x) {
+    const unsigned lane = threadIdx.x & 31u, gid = lane >> 2, tig = lane & 3u;
+    const uint4 top = *reinterpret_cast<const uint4*>(codes + 64u * gid + 16u * tig), bot = *reinterpret_cast<const uint4*>(codes + 64u * (gid + 8u) + 16u * tig);
+    const float4 ft = f[gid], fb = f[gid + 8u];
+    const float zero[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int blk = 0; blk < 4; ++blk) {
+        const uint32_t t0 = blk < 2 ? top.x : top.y, t1 = blk < 2 ? top.z : top.w, b0 = blk < 2 ? bot.x : bot.y, b1 = blk < 2 ? bot.z : bot.w;
+        uint32_t a[8];
+        if (blk & 1) {
+            a[0] = e2m1x2_to_f16x2<2>(t0), a[1] = e2m1x2_to_f16x2<2>(b0), a[2] = e2m1x2_to_f16x2<3>(t0), a[3] = e2m1x2_to_f16x2<3>(b0);
+            a[4] = e2m1x2_to_f16x2<2>(t1), a[5] = e2m1x2_to_f16x2<2>(b1), a[6] = e2m1x2_to_f16x2<3>(t1), a[7] = e2m1x2_to_f16x2<3>(b1);
+        } else {
+            a[0] = e2m1x2_to_f16x2<0>(t0), a[1] = e2m1x2_to_f16x2<0>(b0), a[2] = e2m1x2_to_f16x2<1>(t0), a[3] = e2m1x2_to_f16x2<1>(b0);
+            a[4] = e2m1x2_to_f16x2<0>(t1), a[5] = e2m1x2_to_f16x2<0>(b1), a[6] = e2m1x2_to_f16x2<1>(t1), a[7] = e2m1x2_to_f16x2<1>(b1);
+        }
+        const float st = blk == 0 ? ft.x : blk == 1 ? ft.y : blk == 2 ? ft.z : ft.w, sb = blk == 0 ? fb.x : blk == 1 ? fb.y : blk == 2 ? fb.z : fb.w;
+#pragma unroll
+        for (int g = 0; g < NT; ++g) {
+            float d[4];
+            mma_f16(d, a[0], a[1], a[2], a[3], x.q[g][blk][0], x.q[g][blk][1], zero);
+            mma_f16(d, a[4], a[5], a[6], a[7], x.q[g][blk][2], x.q[g][blk][3], d);
+            if (blk == 0) {
+                s[g][0] = d[0] * st, s[g][1] = d[1] * st, s[g][2] = d[2] * sb, s[g][3] = d[3] * sb;
+            } else {
+                s[g][0] = fmaf(d[0], st, s[g][0]), s[g][1] = fmaf(d[1], st, s[g][1]), s[g][2] = fmaf(d[2], sb, s[g][2]), s[g][3] = fmaf(d[3], sb, s[g][3]);
+            }
+        }
+    }
+}
+
+// One lane a token: its factors, from the unit's scale bytes. A token behind the length weighs nothing, one in a page outside the pool is NaN.
+__device__ __forceinline__ void token_factors(TokenFactors& f, uint32_t kw, uint32_t vw, bool live, bool lost) {
+    const unsigned t = threadIdx.x & 31u;
+    float4 k = make_float4(scale_f32(kw, 0), scale_f32(kw, 1), scale_f32(kw, 2), scale_f32(kw, 3));
+    if (lost) k = make_float4(__uint_as_float(0x7FC00000u), 0.0f, 0.0f, 0.0f);
+    f.k[t] = k;
+    const uint32_t e0 = vw & 0xFFu, e1 = (vw >> 8) & 0xFFu, e2 = (vw >> 16) & 0xFFu, e3 = vw >> 24;
+    int e = static_cast<int>(max(max(e0, e1), max(e2, e3))) - 127;
+    e = min(max(e, kLowE), kHighE);
+    if (!live) e = 0;
+    f.v[t] = make_float2(static_cast<float>(e), __uint_as_float(static_cast<uint32_t>(127 - e) << 23));
+    const uint32_t eb[4] = {e0, e1, e2, e3};
+#pragma unroll
+    for (int b = 0; b < 4; ++b) {
+        const int d = static_cast<int>(eb[b]) - 127 - e + kUp;   // at most 11 (E <= 252)
+        uint32_t h = d >= -14 ? static_cast<uint32_t>(d + 15) << 10 : d >= -24 ? 1u << (d + 24) : 0u;
+        if (eb[b] == 0u || !live) h = 0u;
+        if (eb[b] == 255u && live) h = 0x7E00u;
+        f.r[t >> 1][b][t & 1u] = static_cast<uint16_t>(h);
+    }
+}
+
+template <int NT, unsigned kStages>
+struct alignas(128) CtaShared {
+    WarpShared<kStages> warp[kWarps];
+    float m[kWarps][8 * NT], l[kWarps][8 * NT];
+    unsigned long long part[kWarps][2];
+    unsigned long long bars[kWarps][kStages];
+    unsigned long long rem;
+    uint32_t seq, failed;
+};
+
+// Partials of CTA w: two slots (0: an item that an earlier CTA began, 1: one that a later CTA goes on with) of rows x (128 O, then M and l behind all rows)
+__device__ __forceinline__ float* slot_of(float* ws, uint32_t w, uint32_t slot, uint32_t rows) { return ws + (static_cast<size_t>(w) * 2u + slot) * rows * 130u; }
+
+template <int NT, unsigned kStages>
+__global__ void __launch_bounds__(kThreads) kv4_attend_kernel(const __grid_constant__ Kv4AttendParams p, uint32_t row_tiles) {
+    extern __shared__ __align__(128) uint8_t smem_raw[];
+    CtaShared<NT, kStages>& sh = *reinterpret_cast<CtaShared<NT, kStages>*>(smem_raw);
+    const unsigned lane = threadIdx.x & 31u, warp = threadIdx.x >> 5, gid = lane >> 2, tig = lane & 3u;
+    WarpShared<kStages>& mine = sh.warp[warp];
+    const uint32_t bar0 = sm100::smem_u32(&sh.bars[warp][0]);
+    if (lane == 0u) {
+        for (unsigned i = 0; i < kStages; ++i) sm100::mbar_init(bar0 + 8u * i, 1u);
+        sm100::fence_mbar_init();
+    }
+    if (threadIdx.x == 0u) sh.failed = 0u;
+    pdl_launch();
+    pdl_wait();
+    __syncthreads();
+    const uint32_t per = p.c.HK * row_tiles;
+    const unsigned long long all = sum_tiles(p.c, 0u, per, sh.part).all;
+    const uint32_t n_work = workers(all, gridDim.x);
+    if (blockIdx.x >= n_work) return;
+    unsigned long long pos = run_begin(all, n_work, blockIdx.x);
+    const unsigned long long end = run_begin(all, n_work, blockIdx.x + 1u);
+    // the sequence that tile `pos` is in
+    if (warp == 0u) {
+        unsigned long long before = 0;
+        for (uint32_t b0 = 0; b0 < p.c.B; b0 += 32u) {
+            const unsigned long long t = b0 + lane < p.c.B ? 1ull * tiles_of(p.c, b0 + lane) * per : 0ull;
+            unsigned long long s = t;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const unsigned long long a = __shfl_up_sync(0xFFFFFFFFu, s, o);
+                if (lane >= static_cast<unsigned>(o)) s += a;
+            }
+            const unsigned hit = __ballot_sync(0xFFFFFFFFu, before + s > pos);
+            if (hit != 0u) {
+                if (lane == static_cast<unsigned>(__ffs(hit)) - 1u) sh.seq = b0 + lane, sh.rem = pos - (before + s - t);
+                break;
+            }
+            before += __shfl_sync(0xFFFFFFFFu, s, 31);
+        }
+    }
+    __syncthreads();
+    uint32_t b = sh.seq;
+    unsigned long long in_seq = sh.rem;
+    uint32_t phase_bits = 0;   // parity of each stage's next wait
+    const uint32_t page = 1u << p.c.page_log2, piece = min(page, kUnit), pieces = kUnit / piece;   // a unit is `pieces` records of `piece` tokens in the ring
+
+    while (pos < end) {
+        const uint32_t length = length_of(p.c, b), tiles = (length + kTile - 1u) / kTile;
+        if (in_seq >= 1ull * tiles * per) {   // also where a sequence has none
+            in_seq -= 1ull * tiles * per;
+            ++b;
+            continue;
+        }
+        const uint32_t item = static_cast<uint32_t>(in_seq / tiles), first = static_cast<uint32_t>(in_seq % tiles);
+        const uint32_t head = item / row_tiles, row0 = (item % row_tiles) * 8u * NT;
+        const uint32_t n_tiles = static_cast<uint32_t>(min(static_cast<unsigned long long>(tiles - first), end - pos));
+        const uint32_t n_rows = count_of(p.counts, b, p.S, length);
+        QueryRows<NT> x;
+        load_rows<NT>(x, p, b, head, row0, length, n_rows);
+        uint32_t low = 0xFFFFFFFFu;   // tokens that every live column sees
+#pragma unroll
+        for (int g = 0; g < NT; ++g) {
+#pragma unroll
+            for (int j = 0; j < 2; ++j) low = min(low, x.limit[g][j] == 0u ? 0xFFFFFFFFu : x.limit[g][j]);
+        }
+        low = min(low, __shfl_xor_sync(0xFFFFFFFFu, low, 1));
+        low = min(low, __shfl_xor_sync(0xFFFFFFFFu, low, 2));
+        low = min(low, length);
+
+        float o[NT][8][4], m[NT][2], l[NT][2];
+#pragma unroll
+        for (int g = 0; g < NT; ++g) {
+            m[g][0] = m[g][1] = kLowest;
+            l[g][0] = l[g][1] = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) o[g][i][0] = o[g][i][1] = o[g][i][2] = o[g][i][3] = 0.0f;
+        }
+        const uint32_t t_first = first * kTile + warp * kUnit;
+        const uint32_t units = t_first >= length ? 0u : min(n_tiles, (length - t_first + kTile - 1u) / kTile);
+        // pages of the unit that is copied next, looked up one unit ahead; lane 0 issues
+        long long ids[2];
+        auto look_up = [&](uint32_t u) {
+            const uint32_t t = t_first + u * kTile;
+            ids[0] = u < units ? page_of(p.c, b, t) : -1;
+            ids[1] = pieces > 1u && u < units && t + piece < length ? page_of(p.c, b, t + piece) : -1;
+        };
+        auto issue = [&](uint32_t u) {
+            if (u >= units) return;
+            const uint32_t st = u % kStages, bar = bar0 + 8u * st, t = t_first + u * kTile;
+            const uint32_t dst = sm100::smem_u32(mine.ring[st]);
+            if (lane == 0u) {
+                uint32_t bytes = 0;
+                for (uint32_t i = 0; i < pieces; ++i) bytes += ids[i] >= 0 ? piece * FMHA_KV4_TOKEN_BYTES : 0u;
+                sm100::mbar_arrive_expect_tx(bar, bytes);
+                for (uint32_t i = 0; i < pieces; ++i) {
+                    if (ids[i] < 0) continue;
+                    const uint8_t* rec = record_of(p.c, ids[i], head);
+                    const uint32_t to = dst + i * piece * FMHA_KV4_TOKEN_BYTES;
+                    if (page <= kUnit) {
+                        bulk_load(to, rec, piece * FMHA_KV4_TOKEN_BYTES, bar);
+                    } else {   // 32 tokens out of a longer page: its four parts
+                        const uint32_t slot = t & (page - 1u);
+                        bulk_load(to, rec + 64u * slot, 64u * kUnit, bar);
+                        bulk_load(to + 64u * kUnit, rec + 64u * (page + slot), 64u * kUnit, bar);
+                        bulk_load(to + 128u * kUnit, rec + 128u * page + 4u * slot, 4u * kUnit, bar);
+                        bulk_load(to + 132u * kUnit, rec + 132u * page + 4u * slot, 4u * kUnit, bar);
+                    }
+                }
+            }
+        };
+        // whether the pages of a unit's two halves are of the pool, for the units in flight (bits 2 st, 2 st + 1)
+        uint32_t have = 0;
+        auto note = [&](uint32_t u) {
+            const uint32_t st = u % kStages;
+            have &= ~(3u << (2u * st));
+            have |= ((ids[0] >= 0 ? 1u : 0u) | ((pieces > 1u ? ids[1] : ids[0]) >= 0 ? 2u : 0u)) << (2u * st);
+        };
+        look_up(0);
+#pragma unroll
+        for (unsigned u = 0; u < kStages - 1u; ++u) {
+            issue(u);
+            note(u);
+            look_up(u + 1u);
+        }
+        bool ok = true;
+        for (uint32_t u = 0; u < units; ++u) {
+            issue(u + kStages - 1u);
+            note(u + kStages - 1u);
+            look_up(u + kStages);
+            const uint32_t st = u % kStages, tok0 = t_first + u * kTile;
+            if (!sm100::mbar_wait(bar0 + 8u * st, (phase_bits >> st) & 1u, &sh.failed)) {
+                ok = false;
+                break;
+            }
+            phase_bits ^= 1u << st;
+            const uint8_t* raw = mine.ring[st];
+            {
+                const uint32_t rec = lane / piece, in = lane % piece;
+                const uint8_t* at = raw + rec * piece * FMHA_KV4_TOKEN_BYTES + 4u * in;
+                const bool lost = ((have >> (2u * st + (lane >> 4))) & 1u) == 0u;
+                token_factors(mine.f, *reinterpret_cast<const uint32_t*>(at + 128u * piece), *reinterpret_cast<const uint32_t*>(at + 132u * piece), tok0 + lane < length && !lost, lost);
+            }
+            __syncwarp();
+            float s[2][NT][4];
+#pragma unroll
+            for (int gr = 0; gr < 2; ++gr) {
+                const uint8_t* codes = raw + (pieces > 1u ? gr * 16u * FMHA_KV4_TOKEN_BYTES : gr * 1024u);
+                scores<NT>(s[gr], codes, mine.f.k + 16 * gr, x);
+            }
+            const bool edge = tok0 + kUnit > low;
+            bool over = false;
+            float2 fv[2][2];
+#pragma unroll
+            for (int gr = 0; gr < 2; ++gr) {
+                fv[gr][0] = mine.f.v[16 * gr + gid], fv[gr][1] = mine.f.v[16 * gr + 8 + gid];
+#pragma unroll
+                for (int g = 0; g < NT; ++g) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        s[gr][g][i] = fmaf(s[gr][g][i], x.factor[g][i & 1], fv[gr][i >> 1].x);
+                        if (edge && tok0 + 16u * gr + 8u * (i >> 1) + gid >= x.limit[g][i & 1]) s[gr][g][i] = -INFINITY;
+                        over |= s[gr][g][i] > m[g][i & 1] + kSlack;
+                    }
+                }
+            }
+            if (__any_sync(0xFFFFFFFFu, over)) {
+#pragma unroll
+                for (int g = 0; g < NT; ++g) {
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        float top = fmaxf(fmaxf(s[0][g][j], s[0][g][2 + j]), fmaxf(s[1][g][j], s[1][g][2 + j]));
+                        top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 4));
+                        top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 8));
+                        top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 16));
+                        top = fmaxf(top, m[g][j]);
+                        const float f = ex2(m[g][j] - top);
+                        m[g][j] = top;
+                        l[g][j] *= f;
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) o[g][i][j] *= f, o[g][i][2 + j] *= f;
+                    }
+                }
+            }
+#pragma unroll
+            for (int gr = 0; gr < 2; ++gr) {
+                uint32_t pt[NT][2];
+#pragma unroll
+                for (int g = 0; g < NT; ++g) {
+                    float e[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        e[i] = ex2(s[gr][g][i] - m[g][i & 1]);
+                        l[g][i & 1] = fmaf(e[i], fv[gr][i >> 1].y, l[g][i & 1]);
+                    }
+                    pt[g][0] = transpose_8x8(pack_f16x2(e[0], e[1]));
+                    pt[g][1] = transpose_8x8(pack_f16x2(e[2], e[3]));
+                }
+                const uint8_t* codes = raw + (pieces > 1u ? gr * 16u * FMHA_KV4_TOKEN_BYTES + 1024u : 2048u + gr * 1024u) + 8u * gid;
+                const uint2 w0 = *reinterpret_cast<const uint2*>(codes + 64u * (2u * tig)), w1 = *reinterpret_cast<const uint2*>(codes + 64u * (2u * tig + 1u));
+                const uint2 w2 = *reinterpret_cast<const uint2*>(codes + 64u * (2u * tig + 8u)), w3 = *reinterpret_cast<const uint2*>(codes + 64u * (2u * tig + 9u));
+                const uint4 ra = *reinterpret_cast<const uint4*>(&mine.f.r[8 * gr + tig][0][0]), rb = *reinterpret_cast<const uint4*>(&mine.f.r[8 * gr + 4 + tig][0][0]);
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    const uint32_t x0 = half ? w0.y : w0.x, x1 = half ? w1.y : w1.x, x2 = half ? w2.y : w2.x, x3 = half ? w3.y : w3.x;
+                    // bytes of (first token, second token) of a pair: even elements, odd elements
+                    const uint32_t ev0 = (x0 & 0x0F0F0F0Fu) | ((x1 << 4) & 0xF0F0F0F0u), od0 = ((x0 >> 4) & 0x0F0F0F0Fu) | (x1 & 0xF0F0F0F0u);
+                    const uint32_t ev1 = (x2 & 0x0F0F0F0Fu) | ((x3 << 4) & 0xF0F0F0F0u), od1 = ((x2 >> 4) & 0x0F0F0F0Fu) | (x3 & 0xF0F0F0F0u);
+#pragma unroll
+                    for (int bb = 0; bb < 2; ++bb) {
+                        const int blk = 2 * half + bb;
+                        const uint32_t r0 = blk == 0 ? ra.x : blk == 1 ? ra.y : blk == 2 ? ra.z : ra.w, r1 = blk == 0 ? rb.x : blk == 1 ? rb.y : blk == 2 ? rb.z : rb.w;
+                        uint32_t a[8];
+                        if (bb) {
+                            a[0] = e2m1x2_to_f16x2<2>(ev0), a[1] = e2m1x2_to_f16x2<2>(od0), a[2] = e2m1x2_to_f16x2<2>(ev1), a[3] = e2m1x2_to_f16x2<2>(od1);
+                            a[4] = e2m1x2_to_f16x2<3>(ev0), a[5] = e2m1x2_to_f16x2<3>(od0), a[6] = e2m1x2_to_f16x2<3>(ev1), a[7] = e2m1x2_to_f16x2<3>(od1);
+                        } else {
+                            a[0] = e2m1x2_to_f16x2<0>(ev0), a[1] = e2m1x2_to_f16x2<0>(od0), a[2] = e2m1x2_to_f16x2<0>(ev1), a[3] = e2m1x2_to_f16x2<0>(od1);
+                            a[4] = e2m1x2_to_f16x2<1>(ev0), a[5] = e2m1x2_to_f16x2<1>(od0), a[6] = e2m1x2_to_f16x2<1>(ev1), a[7] = e2m1x2_to_f16x2<1>(od1);
+                        }
+#pragma unroll
+                        for (int g = 0; g < NT; ++g) {
+                            uint32_t p0 = mul_f16x2(pt[g][0], r0), p1 = mul_f16x2(pt[g][1], r1);
+                            if (edge) {   // a weight of 0 hides what it multiplies, NaN too
+                                p0 = (pt[g][0] & 0x7FFFu ? p0 & 0xFFFFu : 0u) | (pt[g][0] & 0x7FFF0000u ? p0 & 0xFFFF0000u : 0u);
+                                p1 = (pt[g][1] & 0x7FFFu ? p1 & 0xFFFFu : 0u) | (pt[g][1] & 0x7FFF0000u ? p1 & 0xFFFF0000u : 0u);
+                            }
+                            mma_f16(o[g][2 * blk], a[0], a[1], a[2], a[3], p0, p1, o[g][2 * blk]);
+                            mma_f16(o[g][2 * blk + 1], a[4], a[5], a[6], a[7], p0, p1, o[g][2 * blk + 1]);
+                        }
+                    }
+                }
+            }
+            __syncwarp();   // the stage and the factors are free again
+        }
+        if (!ok) {
+            if (lane == 0u) atomicOr(p.status, 1u);
+        }
+
+        // the warps' sums of the item come together
+#pragma unroll
+        for (int g = 0; g < NT; ++g) {
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                l[g][j] += __shfl_xor_sync(0xFFFFFFFFu, l[g][j], 4);
+                l[g][j] += __shfl_xor_sync(0xFFFFFFFFu, l[g][j], 8);
+                l[g][j] += __shfl_xor_sync(0xFFFFFFFFu, l[g][j], 16);
+                if (gid == 0u) sh.m[warp][8 * g + 2 * tig + j] = m[g][j], sh.l[warp][8 * g + 2 * tig + j] = l[g][j];
+            }
+        }
+        __syncthreads();
+        if (sh.failed != 0u) return;   // (the same for all: it was raised in front of the barrier)
+        const bool whole = first == 0u && n_tiles == tiles;
+        const uint32_t slot = first == 0u ? 1u : 0u;
+        float* part = slot_of(p.ws, blockIdx.x, slot, 8u * NT);
+#pragma unroll
+        for (int g = 0; g < NT; ++g) {
+            float* mine_o = reinterpret_cast<float*>(mine.ring[0]);   // [8 rows][128], the ring is empty
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const int row = 8 * g + 2 * static_cast<int>(tig) + j;
+                float top = fmaxf(fmaxf(sh.m[0][row], sh.m[1][row]), fmaxf(sh.m[2][row], sh.m[3][row]));
+                const float f = ex2(m[g][j] - top);
+#pragma unroll
+                for (int blk = 0; blk < 4; ++blk) {
+                    *reinterpret_cast<float4*>(mine_o + (2u * tig + j) * 128u + 32u * blk + 4u * gid) =
+                        make_float4(o[g][2 * blk][j] * f, o[g][2 * blk][2 + j] * f, o[g][2 * blk + 1][j] * f, o[g][2 * blk + 1][2 + j] * f);
+                }
+            }
+            __syncthreads();
+            {
+                const uint32_t r = threadIdx.x >> 4, d = (threadIdx.x & 15u) * 8u, row = row0 + 8u * g + r;
+                float top = fmaxf(fmaxf(sh.m[0][8 * g + r], sh.m[1][8 * g + r]), fmaxf(sh.m[2][8 * g + r], sh.m[3][8 * g + r]));
+                float total = 0.0f, acc[8];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) acc[k] = 0.0f;
+#pragma unroll
+                for (unsigned w = 0; w < kWarps; ++w) {
+                    total = fmaf(sh.l[w][8 * g + r], ex2(sh.m[w][8 * g + r] - top), total);
+                    const float4* src = reinterpret_cast<const float4*>(reinterpret_cast<const float*>(sh.warp[w].ring[0]) + r * 128u + d);
+                    const float4 a = src[0], c = src[1];
+                    acc[0] += a.x, acc[1] += a.y, acc[2] += a.z, acc[3] += a.w, acc[4] += c.x, acc[5] += c.y, acc[6] += c.z, acc[7] += c.w;
+                }
+                if (row < p.S * p.group) {
+                    if (whole) {
+                        if (row / p.group >= n_rows) top = kLowest;   // a row that stands for nothing
+                        const uint32_t i = row / p.group, h = head * p.group + row % p.group;
+                        const float inv = top == kLowest ? 0.0f : kDown / total;
+                        *reinterpret_cast<uint4*>(p.out + ((static_cast<size_t>(b) * p.S + i) * p.H + h) * 128u + d) =
+                            make_uint4(pack_bf16x2(acc[0] * inv, acc[1] * inv), pack_bf16x2(acc[2] * inv, acc[3] * inv), pack_bf16x2(acc[4] * inv, acc[5] * inv), pack_bf16x2(acc[6] * inv, acc[7] * inv));
+                        if (p.lse != nullptr && d == 0u) p.lse[(static_cast<size_t>(b) * p.H + h) * p.S + i] = top == kLowest ? -INFINITY : (top + lg2(total)) * kLn2;
+                    } else {
+                        float* at = part + (8u * g + r) * 128u + d;
+                        *reinterpret_cast<float4*>(at) = make_float4(acc[0], acc[1], acc[2], acc[3]);
+                        *reinterpret_cast<float4*>(at + 4) = make_float4(acc[4], acc[5], acc[6], acc[7]);
+                        if (d == 0u) *reinterpret_cast<float2*>(part + 8u * NT * 128u + (8u * g + r) * 2u) = make_float2(top, total);
+                    }
+                }
+            }
+            __syncthreads();
+        }
+        // what the generic proxy read and wrote in the ring is behind the next copies into it
+        sm100::fence_proxy_async_smem();
+        pos += n_tiles;
+        in_seq += n_tiles;
+    }
+}
+
+// One CTA a query row: rows that see nothing, and items that more than one CTA worked on
+template <int NT>
+__global__ void __launch_bounds__(kThreads) kv4_combine_kernel(const __grid_constant__ Kv4AttendParams p, uint32_t row_tiles, uint32_t attend_grid) {
+    __shared__ unsigned long long part[kWarps][2];
+    __shared__ float sm_m[kWarps], sm_l[kWarps];
+    __shared__ float4 sm_o[kWarps][32];
+    pdl_launch();
+    pdl_wait();
+    const uint32_t rows = p.S * p.group, row = blockIdx.x % rows, bh = blockIdx.x / rows, head = bh % p.c.HK, b = bh / p.c.HK;
+    const uint32_t per = p.c.HK * row_tiles;
+    const Sums sums = sum_tiles(p.c, b, per, part);
+    const uint32_t tiles = tiles_of(p.c, b), item = head * row_tiles + row / (8u * NT);
+    const unsigned long long t0 = sums.below + 1ull * item * tiles, t1 = t0 + tiles;
+    uint32_t from = 0, to = 0;   // the CTAs that hold parts, to - from + 1 of them
+    uint32_t n_work = 1;
+    if (tiles > 0u) {
+        n_work = workers(sums.all, attend_grid);
+        from = worker_at(sums.all, n_work, t0);
+        to = worker_at(sums.all, n_work, t1 - 1ull);
+        if (from == to) return;
+    }
+    const bool sees = row / p.group < count_of(p.counts, b, p.S, length_of(p.c, b));
+    const unsigned lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
+    float m = kLowest, l = 0.0f;
+    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (tiles > 0u && sees) {
+        const uint32_t r = row % (8u * NT);
+        for (uint32_t w = from + warp; w <= to; w += kWarps) {
+            const float* src = slot_of(p.ws, w, w == from ? 1u : 0u, 8u * NT);
+            const float pm = ld_f32(src + 8u * NT * 128u + 2u * r), pl = ld_f32(src + 8u * NT * 128u + 2u * r + 1u);
+            const uint4 raw = ld_v4(src + r * 128u + 4u * lane);
+            const float top = fmaxf(m, pm), a = ex2(m - top), c = ex2(pm - top);
+            m = top;
+            l = fmaf(l, a, pl * c);
+            o.x = fmaf(o.x, a, __uint_as_float(raw.x) * c), o.y = fmaf(o.y, a, __uint_as_float(raw.y) * c);
+            o.z = fmaf(o.z, a, __uint_as_float(raw.z) * c), o.w = fmaf(o.w, a, __uint_as_float(raw.w) * c);
+        }
+    }
+    if (lane == 0u) sm_m[warp] = m, sm_l[warp] = l;
+    sm_o[warp][lane] = o;
+    __syncthreads();
+    if (warp != 0u) return;
+    const float top = fmaxf(fmaxf(sm_m[0], sm_m[1]), fmaxf(sm_m[2], sm_m[3]));
+    l = 0.0f;
+    o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+    for (unsigned w = 0; w < kWarps; ++w) {
+        const float f = ex2(sm_m[w] - top);
+        const float4 c = sm_o[w][lane];
+        l = fmaf(sm_l[w], f, l);
+        o.x = fmaf(c.x, f, o.x), o.y = fmaf(c.y, f, o.y), o.z = fmaf(c.z, f, o.z), o.w = fmaf(c.w, f, o.w);
+    }
+    const float inv = top == kLowest ? 0.0f : kDown / l;
+    const uint32_t i = row / p.group, h = head * p.group + row % p.group;
+    *reinterpret_cast<uint2*>(p.out + ((static_cast<size_t>(b) * p.S + i) * p.H + h) * 128u + 4u * lane) = make_uint2(pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv));
+    if (p.lse != nullptr && lane == 0u) p.lse[(static_cast<size_t>(b) * p.H + h) * p.S + i] = top == kLowest ? -INFINITY : (top + lg2(l)) * kLn2;
+}
+
+// The attention weights that the cached tokens received: p = 2^(s - lse), summed over the rows and the group's heads. A warp has 32 tokens and goes over all rows, in
+// order, so that the sums are the same every time.
+__global__ void __launch_bounds__(kThreads) kv4_weigh_kernel(const __grid_constant__ Kv4AttendParams p, uint32_t tiles) {
+    __shared__ __align__(16) float4 factors[kWarps][kUnit];
+    __shared__ __align__(16) uint8_t codes[kWarps][kUnit * 64u];
+    pdl_launch();
+    pdl_wait();
+    const unsigned lane = threadIdx.x & 31u, warp = threadIdx.x >> 5, gid = lane >> 2, tig = lane & 3u;
+    const uint32_t bh = blockIdx.x / tiles, head = bh % p.c.HK, b = bh / p.c.HK, tok0 = (blockIdx.x % tiles * kWarps + warp) * kUnit;
+    const uint32_t length = length_of(p.c, b), n = count_of(p.counts, b, p.S, length), page = 1u << p.c.page_log2;
+    if (tok0 >= length) return;
+    {
+        // a lane brings its token's 64 bytes and factors
+        const uint32_t t = tok0 + lane;
+        const long long id = t < length ? page_of(p.c, b, t) : -1;
+        float4 k = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (id >= 0) {
+            const uint8_t* rec = record_of(p.c, id, head);
+            const uint32_t slot = t & (page - 1u), kw = ld_u32(rec + 128u * page + 4u * slot);
+            k = make_float4(scale_f32(kw, 0), scale_f32(kw, 1), scale_f32(kw, 2), scale_f32(kw, 3));
+#pragma unroll
+            for (int i = 0; i < 4; ++i) *reinterpret_cast<uint4*>(&codes[warp][64u * lane + 16u * i]) = ld_v4(rec + 64u * slot + 16u * i);
+        } else {
+            k.x = __uint_as_float(0x7FC00000u);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) *reinterpret_cast<uint4*>(&codes[warp][64u * lane + 16u * i]) = make_uint4(0u, 0u, 0u, 0u);
+        }
+        factors[warp][lane] = k;
+    }
+    __syncwarp();
+    float sum[2][2] = {{0.0f, 0.0f}, {0.0f, 0.0f}};
+    const uint32_t rows = n * p.group;
+    for (uint32_t row0 = 0; row0 < rows; row0 += 8u) {
+        if (p.causal && length - n + (row0 + 7u) / p.group < tok0) continue;   // (uniform: no row of the eight sees the tokens)
+        QueryRows<1> x;
+        load_rows<1>(x, p, b, head, row0, length, n);
+        float lse2[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const uint32_t row = row0 + 2u * tig + j;
+            lse2[j] = row < rows ? ld_f32(p.lse + (static_cast<size_t>(b) * p.H + head * p.group + row % p.group) * p.S + row / p.group) * kLog2e : 0.0f;
+        }
+#pragma unroll
+        for (int gr = 0; gr < 2; ++gr) {
+            float s[1][4];
+            scores<1>(s, &codes[warp][1024u * gr], &factors[warp][16 * gr], x);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const bool seen = tok0 + 16u * gr + 8u * (i >> 1) + gid < x.limit[0][i & 1];
+                const float w = ex2(fmaf(s[0][i], x.factor[0][i & 1], -lse2[i & 1]));
+                sum[gr][i >> 1] += seen ? w : 0.0f;
+            }
+        }
+    }
+#pragma unroll
+    for (int gr = 0; gr < 2; ++gr) {
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            float v = sum[gr][k];
+            v += __shfl_xor_sync(0xFFFFFFFFu, v, 1);
+            v += __shfl_xor_sync(0xFFFFFFFFu, v, 2);
+            const uint32_t t = tok0 + 16u * gr + 8u * k + gid;
+            if (tig == 0u && t < length) {
+                const size_t at = static_cast<size_t>(bh) * p.weights_width + t;
+                const bool old = p.weights_in != nullptr && (!p.causal || t < length - n);
+                p.weights[at] = (old ? ld_f32(p.weights_in + at) : 0.0f) + v;
+            }
+        }
+    }
+}
+
+constexpr unsigned kStages1 = 3;
+constexpr uint32_t kMaxGroups = 4;   // groups of eight rows that an item holds at most
+
+uint32_t groups_of(uint32_t rows) { return rows <= 8u ? 1u : rows <= 16u ? 2u : kMaxGroups; }
+
+uint32_t attend_grid(const Kv4View& c, uint32_t row_tiles) {
+    const unsigned long long tiles = ((static_cast<unsigned long long>(c.table_width) << c.page_log2) + kTile - 1u) / kTile;
+    const unsigned long long most = tiles * c.B * c.HK * row_tiles, full = static_cast<unsigned long long>(kCtasPerSm) * static_cast<unsigned long long>(current_sm_count());
+    return static_cast<uint32_t>(most < full ? (most ? most : 1ull) : full);
+}
+
+template <int NT>
+cudaError_t launch_rows(const Kv4AttendParams& p, uint32_t row_tiles, cudaStream_t stream) {
+    const uint32_t grid = attend_grid(p.c, row_tiles);
+    const size_t smem = sizeof(CtaShared<NT, kStages1>);
+    static std::atomic<bool> set[64];
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (dev < 0 || dev >= 64 || !set[dev].load(std::memory_order_relaxed)) {
+        e = cudaFuncSetAttribute(kv4_attend_kernel<NT, kStages1>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+        if (e != cudaSuccess) return e;
+        if (dev >= 0 && dev < 64) set[dev].store(true, std::memory_order_relaxed);
+    }
+    e = kv4_launch(kv4_attend_kernel<NT, kStages1>, dim3(grid), kThreads, smem, stream, p, row_tiles);
+    if (e != cudaSuccess) return e;
+    return kv4_launch(kv4_combine_kernel<NT>, dim3(p.c.B * p.c.HK * p.S * p.group), kThreads, 0, stream, p, row_tiles, grid);
+}
+
+uint64_t partial_bytes(const Kv4View& c, uint32_t rows) {
+    const uint32_t nt = groups_of(rows), row_tiles = (rows + 8u * nt - 1u) / (8u * nt);
+    return static_cast<uint64_t>(attend_grid(c, row_tiles)) * 2u * 8u * nt * 130u * 4u;
+}
+
+}  // namespace
+
+uint64_t kv4_attend_workspace(const Kv4View& c, uint32_t S, uint32_t H, bool weights, bool lse) {
+    return partial_bytes(c, S * (H / c.HK)) + (weights && !lse ? static_cast<uint64_t>(c.B) * S * H * 4u : 0u);
+}
+
+cudaError_t launch_kv4_attend(const Kv4AttendParams& params, cudaStream_t stream) {
+    Kv4AttendParams p = params;
+    const uint32_t rows = p.S * p.group, nt = groups_of(rows), row_tiles = (rows + 8u * nt - 1u) / (8u * nt);
+    if (p.weights != nullptr && p.lse == nullptr) p.lse = p.ws + partial_bytes(p.c, rows) / 4u;   // the weights go by the rows' log-sum-exps
+    cudaError_t e = nt == 1u ? launch_rows<1>(p, row_tiles, stream) : nt == 2u ? launch_rows<2>(p, row_tiles, stream) : launch_rows<4>(p, row_tiles, stream);
+    if (e != cudaSuccess || p.weights == nullptr) return e;
+    const uint32_t tiles = ((p.c.table_width << p.c.page_log2) + kTile - 1u) / kTile;
+    return kv4_launch(kv4_weigh_kernel, dim3(tiles * p.c.B * p.c.HK), kThreads, 0, stream, p, tiles);
+}
+
+}  // namespace b200mx

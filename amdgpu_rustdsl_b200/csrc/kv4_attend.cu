@@ -40,10 +40,14 @@ constexpr float kLn2 = 0.69314718055994531f, kLog2e = 1.44269504088896341f;
 
 // What a unit's 32 lanes work out for its tokens, one lane a token
 struct TokenFactors {
-    float4 k[kUnit];               // 2^(E - 127) of the four K blocks
-    float2 v[kUnit];               // e, 2^-e
-    uint16_t r[kUnit / 2][4][2];   // [token pair][block][token of the pair]: V's factor over 2^(e - kUp), f16
+    float4 k[kUnit];           // 2^(E - 127) of the four K blocks
+    float2 v[kUnit];           // e, 2^-e
+    uint32_t r[kUnit / 2][4];  // [token pair][block]: V's factors over 2^(e - kUp), f16, of the pair's tokens in the operand's order
 };
+
+// Row r of the matrix instructions' token operands is token row_token(r) of its eight: neighbours in a pair (rows 2 j, 2 j + 1) stay neighbours, and the first tokens of the four
+// pairs, which one load of V codes reads, are two even and two odd ones: their 64-byte rows then meet in the banks in twos, not in fours.
+__device__ __forceinline__ uint32_t row_token(uint32_t r) { return r ^ ((r >> 1) & 1u); }
 
 template <unsigned kStages>
 struct alignas(128) WarpShared {
@@ -140,8 +144,9 @@ __device__ __forceinline__ void load_rows(QueryRows<NT>& x, const Kv4AttendParam
 template <int NT>
 __device__ __forceinline__ void scores(float (&s)[NT][4], const uint8_t* codes, const float4* f, const QueryRows<NT>& x) {
     const unsigned lane = threadIdx.x & 31u, gid = lane >> 2, tig = lane & 3u;
-    const uint4 top = *reinterpret_cast<const uint4*>(codes + 64u * gid + 16u * tig), bot = *reinterpret_cast<const uint4*>(codes + 64u * (gid + 8u) + 16u * tig);
-    const float4 ft = f[gid], fb = f[gid + 8u];
+    const uint32_t row = row_token(gid);
+    const uint4 top = *reinterpret_cast<const uint4*>(codes + 64u * row + 16u * tig), bot = *reinterpret_cast<const uint4*>(codes + 64u * (row + 8u) + 16u * tig);
+    const float4 ft = f[row], fb = f[row + 8u];
     const float zero[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int blk = 0; blk < 4; ++blk) {
@@ -169,26 +174,27 @@ __device__ __forceinline__ void scores(float (&s)[NT][4], const uint8_t* codes, 
     }
 }
 
-// One lane a token: its factors, from the unit's scale bytes. A token behind the length weighs nothing, one in a page outside the pool is NaN.
-__device__ __forceinline__ void token_factors(TokenFactors& f, uint32_t kw, uint32_t vw, bool live, bool lost) {
+// One lane a token: its factors, from the unit's scale bytes. A token behind the length is masked later; its V factors have to be finite.
+__device__ __forceinline__ void token_factors(TokenFactors& f, uint32_t kw, uint32_t vw, bool live) {
     const unsigned t = threadIdx.x & 31u;
-    float4 k = make_float4(scale_f32(kw, 0), scale_f32(kw, 1), scale_f32(kw, 2), scale_f32(kw, 3));
-    if (lost) k = make_float4(__uint_as_float(0x7FC00000u), 0.0f, 0.0f, 0.0f);
-    f.k[t] = k;
-    const uint32_t e0 = vw & 0xFFu, e1 = (vw >> 8) & 0xFFu, e2 = (vw >> 16) & 0xFFu, e3 = vw >> 24;
-    int e = static_cast<int>(max(max(e0, e1), max(e2, e3))) - 127;
-    e = min(max(e, kLowE), kHighE);
-    if (!live) e = 0;
+    f.k[t] = make_float4(scale_f32(kw, 0), scale_f32(kw, 1), scale_f32(kw, 2), scale_f32(kw, 3));
+    if (!live) vw = 0x7F7F7F7Fu;
+    const int e0 = vw & 0xFFu, e1 = (vw >> 8) & 0xFFu, e2 = (vw >> 16) & 0xFFu, e3 = vw >> 24;
+    const int top = max(max(e0, e1), max(e2, e3)), e = min(max(top - 127, kLowE), kHighE);
     f.v[t] = make_float2(static_cast<float>(e), __uint_as_float(static_cast<uint32_t>(127 - e) << 23));
-    const uint32_t eb[4] = {e0, e1, e2, e3};
-#pragma unroll
-    for (int b = 0; b < 4; ++b) {
-        const int d = static_cast<int>(eb[b]) - 127 - e + kUp;   // at most 11 (E <= 252)
-        uint32_t h = d >= -14 ? static_cast<uint32_t>(d + 15) << 10 : d >= -24 ? 1u << (d + 24) : 0u;
-        if (eb[b] == 0u || !live) h = 0u;
-        if (eb[b] == 255u && live) h = 0x7E00u;
-        f.r[t >> 1][b][t & 1u] = static_cast<uint16_t>(h);
+    // as f32 exponents (E <= 252 leaves them below f16's largest), rounded to f16, which knows subnormals
+    float r0 = __uint_as_float(static_cast<uint32_t>(max(e0 - e + kUp, 0)) << 23), r1 = __uint_as_float(static_cast<uint32_t>(max(e1 - e + kUp, 0)) << 23);
+    float r2 = __uint_as_float(static_cast<uint32_t>(max(e2 - e + kUp, 0)) << 23), r3 = __uint_as_float(static_cast<uint32_t>(max(e3 - e + kUp, 0)) << 23);
+    if (top == 255) {
+        const float nan = __uint_as_float(0x7FC00000u);
+        r0 = e0 == 255 ? nan : r0, r1 = e1 == 255 ? nan : r1, r2 = e2 == 255 ? nan : r2, r3 = e3 == 255 ? nan : r3;
     }
+    // an even lane takes blocks 0 and 1 of its pair, the odd one 2 and 3; pairs whose operand rows are the other way round are stored so
+    const uint32_t r01 = pack_f16x2(r0, r1), r23 = pack_f16x2(r2, r3);
+    const bool odd = t & 1u, flip = (t >> 1) & 1u;
+    const uint32_t mine = odd ? r23 : r01, got = __shfl_xor_sync(0xFFFFFFFFu, odd ? r01 : r23, 1);
+    const uint32_t first = odd != flip ? got : mine, second = odd != flip ? mine : got;
+    *reinterpret_cast<uint2*>(&f.r[t >> 1][odd ? 2 : 0]) = make_uint2(__byte_perm(first, second, 0x5410), __byte_perm(first, second, 0x7632));
 }
 
 template <int NT, unsigned kStages>
@@ -204,8 +210,125 @@ struct alignas(128) CtaShared {
 // Partials of CTA w: two slots (0: an item that an earlier CTA began, 1: one that a later CTA goes on with) of rows x (128 O, then M and l behind all rows)
 __device__ __forceinline__ float* slot_of(float* ws, uint32_t w, uint32_t slot, uint32_t rows) { return ws + (static_cast<size_t>(w) * 2u + slot) * rows * 130u; }
 
+// What stands in for a page that the pool does not have: codes of 0, scales of 255, so that everything in it is NaN
+template <int kPage>
+struct LostPage {
+    uint8_t bytes[FMHA_KV4_TOKEN_BYTES * kPage];
+    constexpr LostPage() : bytes{} {
+        for (int i = 128 * kPage; i < 136 * kPage; ++i) bytes[i] = 0xFF;
+    }
+};
+struct LostPages {
+    alignas(16) LostPage<16> p16;
+    alignas(16) LostPage<32> p32;
+    alignas(16) LostPage<64> p64;
+    alignas(16) LostPage<128> p128;
+};
+__device__ const LostPages kNowhere;
+
+// 32 tokens: scores, softmax, and their part of O
+template <int NT, bool kEdge>
+__device__ __forceinline__ void attend_unit(float (&o)[NT][8][4], float (&m)[NT][2], float (&l)[NT][2], const QueryRows<NT>& x, const uint8_t* k_codes, const uint8_t* v_codes, uint32_t granule,
+                                            const TokenFactors& f, uint32_t tok0) {
+    const unsigned lane = threadIdx.x & 31u, gid = lane >> 2, tig = lane & 3u;
+    const uint32_t row = row_token(gid);
+    float s[2][NT][4];
+    float2 fv[2][2];
+#pragma unroll
+    for (int gr = 0; gr < 2; ++gr) {
+        scores<NT>(s[gr], k_codes + gr * granule, f.k + 16 * gr, x);
+        fv[gr][0] = f.v[16 * gr + row], fv[gr][1] = f.v[16 * gr + 8 + row];
+#pragma unroll
+        for (int g = 0; g < NT; ++g) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                s[gr][g][i] = fmaf(s[gr][g][i], x.factor[g][i & 1], fv[gr][i >> 1].x);
+                if (kEdge && tok0 + 16u * gr + 8u * (i >> 1) + row >= x.limit[g][i & 1]) s[gr][g][i] = -INFINITY;
+            }
+        }
+    }
+    bool over = false;
+    float top[NT][2];
+#pragma unroll
+    for (int g = 0; g < NT; ++g) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            top[g][j] = fmaxf(fmaxf(s[0][g][j], s[0][g][2 + j]), fmaxf(s[1][g][j], s[1][g][2 + j]));
+            over |= top[g][j] > m[g][j] + kSlack;
+        }
+    }
+    if (__any_sync(0xFFFFFFFFu, over)) {
+#pragma unroll
+        for (int g = 0; g < NT; ++g) {
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                float t = top[g][j];
+                t = fmaxf(t, __shfl_xor_sync(0xFFFFFFFFu, t, 4));
+                t = fmaxf(t, __shfl_xor_sync(0xFFFFFFFFu, t, 8));
+                t = fmaxf(t, __shfl_xor_sync(0xFFFFFFFFu, t, 16));
+                t = fmaxf(t, m[g][j]);
+                const float c = ex2(m[g][j] - t);
+                m[g][j] = t;
+                l[g][j] *= c;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) o[g][i][j] *= c, o[g][i][2 + j] *= c;
+            }
+        }
+    }
+    const uint32_t t0 = row_token(2u * tig), t1 = t0 ^ 1u;
+#pragma unroll
+    for (int gr = 0; gr < 2; ++gr) {
+        uint32_t pt[NT][2];
+#pragma unroll
+        for (int g = 0; g < NT; ++g) {
+            float e[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                e[i] = ex2(s[gr][g][i] - m[g][i & 1]);
+                l[g][i & 1] = fmaf(e[i], fv[gr][i >> 1].y, l[g][i & 1]);
+            }
+            pt[g][0] = transpose_8x8(pack_f16x2(e[0], e[1]));
+            pt[g][1] = transpose_8x8(pack_f16x2(e[2], e[3]));
+        }
+        const uint8_t* codes = v_codes + gr * granule + 8u * gid;
+        const uint2 w0 = *reinterpret_cast<const uint2*>(codes + 64u * t0), w1 = *reinterpret_cast<const uint2*>(codes + 64u * t1);
+        const uint2 w2 = *reinterpret_cast<const uint2*>(codes + 64u * (t0 + 8u)), w3 = *reinterpret_cast<const uint2*>(codes + 64u * (t1 + 8u));
+        const uint4 ra = *reinterpret_cast<const uint4*>(f.r[8 * gr + tig]), rb = *reinterpret_cast<const uint4*>(f.r[8 * gr + 4 + tig]);
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            const uint32_t x0 = half ? w0.y : w0.x, x1 = half ? w1.y : w1.x, x2 = half ? w2.y : w2.x, x3 = half ? w3.y : w3.x;
+            // bytes of (first token, second token) of a pair: even elements, odd elements
+            const uint32_t ev0 = (x0 & 0x0F0F0F0Fu) | ((x1 << 4) & 0xF0F0F0F0u), od0 = ((x0 >> 4) & 0x0F0F0F0Fu) | (x1 & 0xF0F0F0F0u);
+            const uint32_t ev1 = (x2 & 0x0F0F0F0Fu) | ((x3 << 4) & 0xF0F0F0F0u), od1 = ((x2 >> 4) & 0x0F0F0F0Fu) | (x3 & 0xF0F0F0F0u);
+#pragma unroll
+            for (int bb = 0; bb < 2; ++bb) {
+                const int blk = 2 * half + bb;
+                const uint32_t r0 = blk == 0 ? ra.x : blk == 1 ? ra.y : blk == 2 ? ra.z : ra.w, r1 = blk == 0 ? rb.x : blk == 1 ? rb.y : blk == 2 ? rb.z : rb.w;
+                uint32_t a[8];
+                if (bb) {
+                    a[0] = e2m1x2_to_f16x2<2>(ev0), a[1] = e2m1x2_to_f16x2<2>(od0), a[2] = e2m1x2_to_f16x2<2>(ev1), a[3] = e2m1x2_to_f16x2<2>(od1);
+                    a[4] = e2m1x2_to_f16x2<3>(ev0), a[5] = e2m1x2_to_f16x2<3>(od0), a[6] = e2m1x2_to_f16x2<3>(ev1), a[7] = e2m1x2_to_f16x2<3>(od1);
+                } else {
+                    a[0] = e2m1x2_to_f16x2<0>(ev0), a[1] = e2m1x2_to_f16x2<0>(od0), a[2] = e2m1x2_to_f16x2<0>(ev1), a[3] = e2m1x2_to_f16x2<0>(od1);
+                    a[4] = e2m1x2_to_f16x2<1>(ev0), a[5] = e2m1x2_to_f16x2<1>(od0), a[6] = e2m1x2_to_f16x2<1>(ev1), a[7] = e2m1x2_to_f16x2<1>(od1);
+                }
+#pragma unroll
+                for (int g = 0; g < NT; ++g) {
+                    uint32_t p0 = mul_f16x2(pt[g][0], r0), p1 = mul_f16x2(pt[g][1], r1);
+                    if (kEdge) {   // a weight of 0 hides what it multiplies, NaN too
+                        p0 = (pt[g][0] & 0x7FFFu ? p0 & 0xFFFFu : 0u) | (pt[g][0] & 0x7FFF0000u ? p0 & 0xFFFF0000u : 0u);
+                        p1 = (pt[g][1] & 0x7FFFu ? p1 & 0xFFFFu : 0u) | (pt[g][1] & 0x7FFF0000u ? p1 & 0xFFFF0000u : 0u);
+                    }
+                    mma_f16(o[g][2 * blk], a[0], a[1], a[2], a[3], p0, p1, o[g][2 * blk]);
+                    mma_f16(o[g][2 * blk + 1], a[4], a[5], a[6], a[7], p0, p1, o[g][2 * blk + 1]);
+                }
+            }
+        }
+    }
+}
+
 template <int NT, unsigned kStages>
-__global__ void __launch_bounds__(kThreads) kv4_attend_kernel(const __grid_constant__ Kv4AttendParams p, uint32_t row_tiles) {
+__global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : NT == 2 ? 3 : 2) kv4_attend_kernel(const __grid_constant__ Kv4AttendParams p, uint32_t row_tiles) {
     extern __shared__ __align__(128) uint8_t smem_raw[];
     CtaShared<NT, kStages>& sh = *reinterpret_cast<CtaShared<NT, kStages>*>(smem_raw);
     const unsigned lane = threadIdx.x & 31u, warp = threadIdx.x >> 5, gid = lane >> 2, tig = lane & 3u;
@@ -248,7 +371,12 @@ __global__ void __launch_bounds__(kThreads) kv4_attend_kernel(const __grid_const
     uint32_t b = sh.seq;
     unsigned long long in_seq = sh.rem;
     uint32_t phase_bits = 0;   // parity of each stage's next wait
-    const uint32_t page = 1u << p.c.page_log2, piece = min(page, kUnit), pieces = kUnit / piece;   // a unit is `pieces` records of `piece` tokens in the ring
+    // in the ring a unit is one record of 32 tokens, or two of 16
+    const uint32_t page = 1u << p.c.page_log2, pieces = page == 16u ? 2u : 1u, pages = static_cast<uint32_t>(p.c.pages), page_bytes = static_cast<uint32_t>(p.c.page_bytes);
+    const uint32_t granule = pieces > 1u ? kUnitBytes / 2u : 16u * 64u, v_codes = pieces > 1u ? 1024u : 2048u, v_scales = pieces > 1u ? 64u : 128u;
+    const uint32_t scales_at = pieces > 1u ? (lane >> 4) * (kUnitBytes / 2u) + 2048u + 4u * (lane & 15u) : 4096u + 4u * lane;
+    const uint8_t* nowhere = page == 16u ? kNowhere.p16.bytes : page == 32u ? kNowhere.p32.bytes : page == 64u ? kNowhere.p64.bytes : kNowhere.p128.bytes;
+    const uint32_t ring0 = sm100::smem_u32(mine.ring[0]);
 
     while (pos < end) {
         const uint32_t length = length_of(p.c, b), tiles = (length + kTile - 1u) / kTile;
@@ -284,157 +412,65 @@ __global__ void __launch_bounds__(kThreads) kv4_attend_kernel(const __grid_const
         const uint32_t t_first = first * kTile + warp * kUnit;
         const uint32_t units = t_first >= length ? 0u : min(n_tiles, (length - t_first + kTile - 1u) / kTile);
         // pages of the unit that is copied next, looked up one unit ahead; lane 0 issues
-        long long ids[2];
+        const int32_t* row_of_table = p.c.table + static_cast<size_t>(b) * p.c.table_width;
+        const uint8_t* heads = p.c.pool + (static_cast<size_t>(head) * FMHA_KV4_TOKEN_BYTES << p.c.page_log2);
+        int id0 = 0, id1 = 0;
         auto look_up = [&](uint32_t u) {
             const uint32_t t = t_first + u * kTile;
-            ids[0] = u < units ? page_of(p.c, b, t) : -1;
-            ids[1] = pieces > 1u && u < units && t + piece < length ? page_of(p.c, b, t + piece) : -1;
+            if (u < units) {
+                id0 = ld_i32(row_of_table + (t >> p.c.page_log2));
+                if (pieces > 1u && t + 16u < length) id1 = ld_i32(row_of_table + (t >> 4) + 1u);
+            }
+        };
+        auto record = [&](int id) {
+            return static_cast<uint32_t>(id) < pages ? heads + static_cast<uint64_t>(static_cast<uint32_t>(id)) * page_bytes : nowhere;
         };
         auto issue = [&](uint32_t u) {
-            if (u >= units) return;
-            const uint32_t st = u % kStages, bar = bar0 + 8u * st, t = t_first + u * kTile;
-            const uint32_t dst = sm100::smem_u32(mine.ring[st]);
-            if (lane == 0u) {
-                uint32_t bytes = 0;
-                for (uint32_t i = 0; i < pieces; ++i) bytes += ids[i] >= 0 ? piece * FMHA_KV4_TOKEN_BYTES : 0u;
-                sm100::mbar_arrive_expect_tx(bar, bytes);
-                for (uint32_t i = 0; i < pieces; ++i) {
-                    if (ids[i] < 0) continue;
-                    const uint8_t* rec = record_of(p.c, ids[i], head);
-                    const uint32_t to = dst + i * piece * FMHA_KV4_TOKEN_BYTES;
-                    if (page <= kUnit) {
-                        bulk_load(to, rec, piece * FMHA_KV4_TOKEN_BYTES, bar);
+            if (u < units && lane == 0u) {
+                const uint32_t st = u % kStages, bar = bar0 + 8u * st, t = t_first + u * kTile, dst = ring0 + st * kUnitBytes;
+                const uint8_t* rec = record(id0);
+                if (pieces > 1u) {
+                    const bool two = t + 16u < length;
+                    sm100::mbar_arrive_expect_tx(bar, two ? kUnitBytes : kUnitBytes / 2u);
+                    bulk_load(dst, rec, kUnitBytes / 2u, bar);
+                    if (two) bulk_load(dst + kUnitBytes / 2u, record(id1), kUnitBytes / 2u, bar);
+                } else {
+                    sm100::mbar_arrive_expect_tx(bar, kUnitBytes);
+                    if (page == kUnit) {
+                        bulk_load(dst, rec, kUnitBytes, bar);
                     } else {   // 32 tokens out of a longer page: its four parts
                         const uint32_t slot = t & (page - 1u);
-                        bulk_load(to, rec + 64u * slot, 64u * kUnit, bar);
-                        bulk_load(to + 64u * kUnit, rec + 64u * (page + slot), 64u * kUnit, bar);
-                        bulk_load(to + 128u * kUnit, rec + 128u * page + 4u * slot, 4u * kUnit, bar);
-                        bulk_load(to + 132u * kUnit, rec + 132u * page + 4u * slot, 4u * kUnit, bar);
+                        bulk_load(dst, rec + 64u * slot, 64u * kUnit, bar);
+                        bulk_load(dst + 64u * kUnit, rec + 64u * (page + slot), 64u * kUnit, bar);
+                        bulk_load(dst + 128u * kUnit, rec + 128u * page + 4u * slot, 4u * kUnit, bar);
+                        bulk_load(dst + 132u * kUnit, rec + 132u * page + 4u * slot, 4u * kUnit, bar);
                     }
                 }
             }
-        };
-        // whether the pages of a unit's two halves are of the pool, for the units in flight (bits 2 st, 2 st + 1)
-        uint32_t have = 0;
-        auto note = [&](uint32_t u) {
-            const uint32_t st = u % kStages;
-            have &= ~(3u << (2u * st));
-            have |= ((ids[0] >= 0 ? 1u : 0u) | ((pieces > 1u ? ids[1] : ids[0]) >= 0 ? 2u : 0u)) << (2u * st);
         };
         look_up(0);
 #pragma unroll
         for (unsigned u = 0; u < kStages - 1u; ++u) {
             issue(u);
-            note(u);
             look_up(u + 1u);
         }
         bool ok = true;
-        for (uint32_t u = 0; u < units; ++u) {
+        for (uint32_t u = 0, st = 0; u < units; ++u, st = st + 1u == kStages ? 0u : st + 1u) {
             issue(u + kStages - 1u);
-            note(u + kStages - 1u);
             look_up(u + kStages);
-            const uint32_t st = u % kStages, tok0 = t_first + u * kTile;
+            const uint32_t tok0 = t_first + u * kTile;
             if (!sm100::mbar_wait(bar0 + 8u * st, (phase_bits >> st) & 1u, &sh.failed)) {
                 ok = false;
                 break;
             }
             phase_bits ^= 1u << st;
-            const uint8_t* raw = mine.ring[st];
-            {
-                const uint32_t rec = lane / piece, in = lane % piece;
-                const uint8_t* at = raw + rec * piece * FMHA_KV4_TOKEN_BYTES + 4u * in;
-                const bool lost = ((have >> (2u * st + (lane >> 4))) & 1u) == 0u;
-                token_factors(mine.f, *reinterpret_cast<const uint32_t*>(at + 128u * piece), *reinterpret_cast<const uint32_t*>(at + 132u * piece), tok0 + lane < length && !lost, lost);
-            }
+            const uint8_t* raw = mine.ring[0] + st * kUnitBytes;
+            token_factors(mine.f, *reinterpret_cast<const uint32_t*>(raw + scales_at), *reinterpret_cast<const uint32_t*>(raw + scales_at + v_scales), tok0 + lane < length);
             __syncwarp();
-            float s[2][NT][4];
-#pragma unroll
-            for (int gr = 0; gr < 2; ++gr) {
-                const uint8_t* codes = raw + (pieces > 1u ? gr * 16u * FMHA_KV4_TOKEN_BYTES : gr * 1024u);
-                scores<NT>(s[gr], codes, mine.f.k + 16 * gr, x);
-            }
-            const bool edge = tok0 + kUnit > low;
-            bool over = false;
-            float2 fv[2][2];
-#pragma unroll
-            for (int gr = 0; gr < 2; ++gr) {
-                fv[gr][0] = mine.f.v[16 * gr + gid], fv[gr][1] = mine.f.v[16 * gr + 8 + gid];
-#pragma unroll
-                for (int g = 0; g < NT; ++g) {
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        s[gr][g][i] = fmaf(s[gr][g][i], x.factor[g][i & 1], fv[gr][i >> 1].x);
-                        if (edge && tok0 + 16u * gr + 8u * (i >> 1) + gid >= x.limit[g][i & 1]) s[gr][g][i] = -INFINITY;
-                        over |= s[gr][g][i] > m[g][i & 1] + kSlack;
-                    }
-                }
-            }
-            if (__any_sync(0xFFFFFFFFu, over)) {
-#pragma unroll
-                for (int g = 0; g < NT; ++g) {
-#pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        float top = fmaxf(fmaxf(s[0][g][j], s[0][g][2 + j]), fmaxf(s[1][g][j], s[1][g][2 + j]));
-                        top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 4));
-                        top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 8));
-                        top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 16));
-                        top = fmaxf(top, m[g][j]);
-                        const float f = ex2(m[g][j] - top);
-                        m[g][j] = top;
-                        l[g][j] *= f;
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) o[g][i][j] *= f, o[g][i][2 + j] *= f;
-                    }
-                }
-            }
-#pragma unroll
-            for (int gr = 0; gr < 2; ++gr) {
-                uint32_t pt[NT][2];
-#pragma unroll
-                for (int g = 0; g < NT; ++g) {
-                    float e[4];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        e[i] = ex2(s[gr][g][i] - m[g][i & 1]);
-                        l[g][i & 1] = fmaf(e[i], fv[gr][i >> 1].y, l[g][i & 1]);
-                    }
-                    pt[g][0] = transpose_8x8(pack_f16x2(e[0], e[1]));
-                    pt[g][1] = transpose_8x8(pack_f16x2(e[2], e[3]));
-                }
-                const uint8_t* codes = raw + (pieces > 1u ? gr * 16u * FMHA_KV4_TOKEN_BYTES + 1024u : 2048u + gr * 1024u) + 8u * gid;
-                const uint2 w0 = *reinterpret_cast<const uint2*>(codes + 64u * (2u * tig)), w1 = *reinterpret_cast<const uint2*>(codes + 64u * (2u * tig + 1u));
-                const uint2 w2 = *reinterpret_cast<const uint2*>(codes + 64u * (2u * tig + 8u)), w3 = *reinterpret_cast<const uint2*>(codes + 64u * (2u * tig + 9u));
-                const uint4 ra = *reinterpret_cast<const uint4*>(&mine.f.r[8 * gr + tig][0][0]), rb = *reinterpret_cast<const uint4*>(&mine.f.r[8 * gr + 4 + tig][0][0]);
-#pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    const uint32_t x0 = half ? w0.y : w0.x, x1 = half ? w1.y : w1.x, x2 = half ? w2.y : w2.x, x3 = half ? w3.y : w3.x;
-                    // bytes of (first token, second token) of a pair: even elements, odd elements
-                    const uint32_t ev0 = (x0 & 0x0F0F0F0Fu) | ((x1 << 4) & 0xF0F0F0F0u), od0 = ((x0 >> 4) & 0x0F0F0F0Fu) | (x1 & 0xF0F0F0F0u);
-                    const uint32_t ev1 = (x2 & 0x0F0F0F0Fu) | ((x3 << 4) & 0xF0F0F0F0u), od1 = ((x2 >> 4) & 0x0F0F0F0Fu) | (x3 & 0xF0F0F0F0u);
-#pragma unroll
-                    for (int bb = 0; bb < 2; ++bb) {
-                        const int blk = 2 * half + bb;
-                        const uint32_t r0 = blk == 0 ? ra.x : blk == 1 ? ra.y : blk == 2 ? ra.z : ra.w, r1 = blk == 0 ? rb.x : blk == 1 ? rb.y : blk == 2 ? rb.z : rb.w;
-                        uint32_t a[8];
-                        if (bb) {
-                            a[0] = e2m1x2_to_f16x2<2>(ev0), a[1] = e2m1x2_to_f16x2<2>(od0), a[2] = e2m1x2_to_f16x2<2>(ev1), a[3] = e2m1x2_to_f16x2<2>(od1);
-                            a[4] = e2m1x2_to_f16x2<3>(ev0), a[5] = e2m1x2_to_f16x2<3>(od0), a[6] = e2m1x2_to_f16x2<3>(ev1), a[7] = e2m1x2_to_f16x2<3>(od1);
-                        } else {
-                            a[0] = e2m1x2_to_f16x2<0>(ev0), a[1] = e2m1x2_to_f16x2<0>(od0), a[2] = e2m1x2_to_f16x2<0>(ev1), a[3] = e2m1x2_to_f16x2<0>(od1);
-                            a[4] = e2m1x2_to_f16x2<1>(ev0), a[5] = e2m1x2_to_f16x2<1>(od0), a[6] = e2m1x2_to_f16x2<1>(ev1), a[7] = e2m1x2_to_f16x2<1>(od1);
-                        }
-#pragma unroll
-                        for (int g = 0; g < NT; ++g) {
-                            uint32_t p0 = mul_f16x2(pt[g][0], r0), p1 = mul_f16x2(pt[g][1], r1);
-                            if (edge) {   // a weight of 0 hides what it multiplies, NaN too
-                                p0 = (pt[g][0] & 0x7FFFu ? p0 & 0xFFFFu : 0u) | (pt[g][0] & 0x7FFF0000u ? p0 & 0xFFFF0000u : 0u);
-                                p1 = (pt[g][1] & 0x7FFFu ? p1 & 0xFFFFu : 0u) | (pt[g][1] & 0x7FFF0000u ? p1 & 0xFFFF0000u : 0u);
-                            }
-                            mma_f16(o[g][2 * blk], a[0], a[1], a[2], a[3], p0, p1, o[g][2 * blk]);
-                            mma_f16(o[g][2 * blk + 1], a[4], a[5], a[6], a[7], p0, p1, o[g][2 * blk + 1]);
-                        }
-                    }
-                }
+            if (tok0 + kUnit <= low) {
+                attend_unit<NT, false>(o, m, l, x, raw, raw + v_codes, granule, mine.f, tok0);
+            } else {
+                attend_unit<NT, true>(o, m, l, x, raw, raw + v_codes, granule, mine.f, tok0);
             }
             __syncwarp();   // the stage and the factors are free again
         }
@@ -617,7 +653,7 @@ __global__ void __launch_bounds__(kThreads) kv4_weigh_kernel(const __grid_consta
             scores<1>(s, &codes[warp][1024u * gr], &factors[warp][16 * gr], x);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const bool seen = tok0 + 16u * gr + 8u * (i >> 1) + gid < x.limit[0][i & 1];
+                const bool seen = tok0 + 16u * gr + 8u * (i >> 1) + row_token(gid) < x.limit[0][i & 1];
                 const float w = ex2(fmaf(s[0][i], x.factor[0][i & 1], -lse2[i & 1]));
                 sum[gr][i >> 1] += seen ? w : 0.0f;
             }
@@ -630,7 +666,7 @@ __global__ void __launch_bounds__(kThreads) kv4_weigh_kernel(const __grid_consta
             float v = sum[gr][k];
             v += __shfl_xor_sync(0xFFFFFFFFu, v, 1);
             v += __shfl_xor_sync(0xFFFFFFFFu, v, 2);
-            const uint32_t t = tok0 + 16u * gr + 8u * k + gid;
+            const uint32_t t = tok0 + 16u * gr + 8u * k + row_token(gid);
             if (tig == 0u && t < length) {
                 const size_t at = static_cast<size_t>(bh) * p.weights_width + t;
                 const bool old = p.weights_in != nullptr && (!p.causal || t < length - n);

@@ -15,6 +15,7 @@
 // factor (kept within what f32 sums of 2^(s - M) bear), so that P 2^e is at most 2^4 however large V is; the four factors of a token relative to 2^e are exact
 // in f16 down to 2^-34. M moves when a value exceeds it by more than 2^4, by a vote of the warp; the sums and O are rescaled then.
 #include "kv4.cuh"
+#include "kv4_schedule.cuh"
 #include "ptx_sm100.cuh"
 
 #include <atomic>
@@ -28,14 +29,10 @@ using namespace kv4;
 constexpr unsigned kWarps = 4, kThreads = kWarps * 32;
 constexpr unsigned kUnit = 32;                    // tokens of a warp at a time
 constexpr unsigned kTile = kWarps * kUnit;
+static_assert(kTile == kStepTokens, "a step is a tile");
 constexpr unsigned kUnitBytes = kUnit * FMHA_KV4_TOKEN_BYTES;
 constexpr unsigned kCtasPerSm = 4;
-constexpr float kLowest = -1e30f;                 // the reference of a row that has seen nothing
 constexpr float kSlack = 4.0f;
-// The exponent e that a token's V factors are taken relative to: within what f32 sums of 2^(s - M), which lie between 2^-kHighE and 2^(4 - kLowE) a token, bear. The
-// factors go in times 2^kUp, which the division by the sums takes out again: f16 has more room below 1 than above, and P 2^e is at most 2^4
-constexpr int kLowE = -100, kHighE = 124, kUp = 10;
-constexpr float kDown = 1.0f / (1 << kUp);
 constexpr float kLn2 = 0.69314718055994531f, kLog2e = 1.44269504088896341f;
 
 // What a unit's 32 lanes work out for its tokens, one lane a token
@@ -58,38 +55,6 @@ struct alignas(128) WarpShared {
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
 }
-
-__device__ __forceinline__ uint32_t tiles_of(const Kv4View& c, uint32_t b) { return (length_of(c, b) + kTile - 1u) / kTile; }
-
-// Sum of tiles over the sequences below `upto`, and over all, times `per` (heads x row tiles). All threads of the CTA.
-struct Sums {
-    unsigned long long below, all;
-};
-__device__ __forceinline__ Sums sum_tiles(const Kv4View& c, uint32_t upto, uint32_t per, unsigned long long (*part)[2]) {
-    unsigned long long below = 0, all = 0;
-    for (uint32_t b = threadIdx.x; b < c.B; b += kThreads) {
-        const uint32_t t = tiles_of(c, b);
-        all += t;
-        if (b < upto) below += t;
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        below += __shfl_xor_sync(0xFFFFFFFFu, below, o);
-        all += __shfl_xor_sync(0xFFFFFFFFu, all, o);
-    }
-    if ((threadIdx.x & 31u) == 0u) part[threadIdx.x >> 5][0] = below, part[threadIdx.x >> 5][1] = all;
-    __syncthreads();
-    below = all = 0;
-#pragma unroll
-    for (unsigned w = 0; w < kWarps; ++w) below += part[w][0], all += part[w][1];
-    __syncthreads();
-    return {below * per, all * per};
-}
-
-// The CTAs that share `all` tiles: run w is [w * all / n, (w + 1) * all / n)
-__device__ __forceinline__ uint32_t workers(unsigned long long all, uint32_t grid) { return static_cast<uint32_t>(all < grid ? all : grid); }
-__device__ __forceinline__ unsigned long long run_begin(unsigned long long all, uint32_t n, uint32_t w) { return all * w / n; }
-__device__ __forceinline__ uint32_t worker_at(unsigned long long all, uint32_t n, unsigned long long tile) { return static_cast<uint32_t>(((tile + 1ull) * n - 1ull) / all); }
 
 // Query rows of an item as the matrix instruction's operand: rows gid of each of NT groups of eight, elements 32 blk + 8 tig .. + 7 of each block
 template <int NT>
@@ -179,20 +144,11 @@ __device__ __forceinline__ void token_factors(TokenFactors& f, uint32_t kw, uint
     const unsigned t = threadIdx.x & 31u;
     f.k[t] = make_float4(scale_f32(kw, 0), scale_f32(kw, 1), scale_f32(kw, 2), scale_f32(kw, 3));
     if (!live) vw = 0x7F7F7F7Fu;
-    const int e0 = vw & 0xFFu, e1 = (vw >> 8) & 0xFFu, e2 = (vw >> 16) & 0xFFu, e3 = vw >> 24;
-    const int top = max(max(e0, e1), max(e2, e3)), e = min(max(top - 127, kLowE), kHighE);
-    f.v[t] = make_float2(static_cast<float>(e), __uint_as_float(static_cast<uint32_t>(127 - e) << 23));
-    // as f32 exponents (E <= 252 leaves them below f16's largest), rounded to f16, which knows subnormals
-    float r0 = __uint_as_float(static_cast<uint32_t>(max(e0 - e + kUp, 0)) << 23), r1 = __uint_as_float(static_cast<uint32_t>(max(e1 - e + kUp, 0)) << 23);
-    float r2 = __uint_as_float(static_cast<uint32_t>(max(e2 - e + kUp, 0)) << 23), r3 = __uint_as_float(static_cast<uint32_t>(max(e3 - e + kUp, 0)) << 23);
-    if (top == 255) {
-        const float nan = __uint_as_float(0x7FC00000u);
-        r0 = e0 == 255 ? nan : r0, r1 = e1 == 255 ? nan : r1, r2 = e2 == 255 ? nan : r2, r3 = e3 == 255 ? nan : r3;
-    }
+    const ValueFactors vf = value_factors(vw);
+    f.v[t] = make_float2(vf.e, vf.inv);
     // an even lane takes blocks 0 and 1 of its pair, the odd one 2 and 3; pairs whose operand rows are the other way round are stored so
-    const uint32_t r01 = pack_f16x2(r0, r1), r23 = pack_f16x2(r2, r3);
     const bool odd = t & 1u, flip = (t >> 1) & 1u;
-    const uint32_t mine = odd ? r23 : r01, got = __shfl_xor_sync(0xFFFFFFFFu, odd ? r01 : r23, 1);
+    const uint32_t mine = odd ? vf.r23 : vf.r01, got = __shfl_xor_sync(0xFFFFFFFFu, odd ? vf.r01 : vf.r23, 1);
     const uint32_t first = odd != flip ? got : mine, second = odd != flip ? mine : got;
     *reinterpret_cast<uint2*>(&f.r[t >> 1][odd ? 2 : 0]) = make_uint2(__byte_perm(first, second, 0x5410), __byte_perm(first, second, 0x7632));
 }
@@ -201,14 +157,10 @@ template <int NT, unsigned kStages>
 struct alignas(128) CtaShared {
     WarpShared<kStages> warp[kWarps];
     float m[kWarps][8 * NT], l[kWarps][8 * NT];
-    unsigned long long part[kWarps][2];
+    Sums part[kWarps];
     unsigned long long bars[kWarps][kStages];
-    unsigned long long rem;
-    uint32_t seq, failed;
+    uint32_t failed;
 };
-
-// Partials of CTA w: two slots (0: an item that an earlier CTA began, 1: one that a later CTA goes on with) of rows x (128 O, then M and l behind all rows)
-__device__ __forceinline__ float* slot_of(float* ws, uint32_t w, uint32_t slot, uint32_t rows) { return ws + (static_cast<size_t>(w) * 2u + slot) * rows * 130u; }
 
 // What stands in for a page that the pool does not have: codes of 0, scales of 255, so that everything in it is NaN
 template <int kPage>
@@ -342,34 +294,13 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : NT == 2 ? 3 : 2) kv4_a
     pdl_launch();
     pdl_wait();
     __syncthreads();
-    const uint32_t per = p.c.HK * row_tiles;
-    const unsigned long long all = sum_tiles(p.c, 0u, per, sh.part).all;
+    const Deal deal{8u * NT, row_tiles};
+    const unsigned long long all = sum_steps(p, deal, 0u, sh.part).all;
     const uint32_t n_work = workers(all, gridDim.x);
     if (blockIdx.x >= n_work) return;
-    unsigned long long pos = run_begin(all, n_work, blockIdx.x);
-    const unsigned long long end = run_begin(all, n_work, blockIdx.x + 1u);
-    // the sequence that tile `pos` is in
-    if (warp == 0u) {
-        unsigned long long before = 0;
-        for (uint32_t b0 = 0; b0 < p.c.B; b0 += 32u) {
-            const unsigned long long t = b0 + lane < p.c.B ? 1ull * tiles_of(p.c, b0 + lane) * per : 0ull;
-            unsigned long long s = t;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const unsigned long long a = __shfl_up_sync(0xFFFFFFFFu, s, o);
-                if (lane >= static_cast<unsigned>(o)) s += a;
-            }
-            const unsigned hit = __ballot_sync(0xFFFFFFFFu, before + s > pos);
-            if (hit != 0u) {
-                if (lane == static_cast<unsigned>(__ffs(hit)) - 1u) sh.seq = b0 + lane, sh.rem = pos - (before + s - t);
-                break;
-            }
-            before += __shfl_sync(0xFFFFFFFFu, s, 31);
-        }
-    }
-    __syncthreads();
-    uint32_t b = sh.seq;
-    unsigned long long in_seq = sh.rem;
+    const unsigned long long begin = run_begin(all, n_work, blockIdx.x);
+    unsigned long long left = run_begin(all, n_work, blockIdx.x + 1u) - begin;
+    Place at = find_step(p, deal, begin);
     uint32_t phase_bits = 0;   // parity of each stage's next wait
     // in the ring a unit is one record of 32 tokens, or two of 16
     const uint32_t page = 1u << p.c.page_log2, pieces = page == 16u ? 2u : 1u, pages = static_cast<uint32_t>(p.c.pages), page_bytes = static_cast<uint32_t>(p.c.page_bytes);
@@ -378,17 +309,10 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : NT == 2 ? 3 : 2) kv4_a
     const uint8_t* nowhere = page == 16u ? kNowhere.p16.bytes : page == 32u ? kNowhere.p32.bytes : page == 64u ? kNowhere.p64.bytes : kNowhere.p128.bytes;
     const uint32_t ring0 = sm100::smem_u32(mine.ring[0]);
 
-    while (pos < end) {
-        const uint32_t length = length_of(p.c, b), tiles = (length + kTile - 1u) / kTile;
-        if (in_seq >= 1ull * tiles * per) {   // also where a sequence has none
-            in_seq -= 1ull * tiles * per;
-            ++b;
-            continue;
-        }
-        const uint32_t item = static_cast<uint32_t>(in_seq / tiles), first = static_cast<uint32_t>(in_seq % tiles);
-        const uint32_t head = item / row_tiles, row0 = (item % row_tiles) * 8u * NT;
-        const uint32_t n_tiles = static_cast<uint32_t>(min(static_cast<unsigned long long>(tiles - first), end - pos));
-        const uint32_t n_rows = count_of(p.counts, b, p.S, length);
+    while (left > 0ull) {
+        const Segment seg = next_segment(p, deal, at, left);
+        const uint32_t b = seg.b, head = seg.head, row0 = seg.row0, first = seg.first, n_tiles = seg.steps;
+        const uint32_t length = length_of(p.c, b), n_rows = count_of(p.counts, b, p.S, length);
         QueryRows<NT> x;
         load_rows<NT>(x, p, b, head, row0, length, n_rows);
         uint32_t low = 0xFFFFFFFFu;   // tokens that every live column sees
@@ -491,7 +415,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : NT == 2 ? 3 : 2) kv4_a
         }
         __syncthreads();
         if (sh.failed != 0u) return;   // (the same for all: it was raised in front of the barrier)
-        const bool whole = first == 0u && n_tiles == tiles;
+        const bool whole = n_tiles == seg.of;
         const uint32_t slot = first == 0u ? 1u : 0u;
         float* part = slot_of(p.ws, blockIdx.x, slot, 8u * NT);
 #pragma unroll
@@ -511,7 +435,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : NT == 2 ? 3 : 2) kv4_a
             __syncthreads();
             {
                 const uint32_t r = threadIdx.x >> 4, d = (threadIdx.x & 15u) * 8u, row = row0 + 8u * g + r;
-                float top = fmaxf(fmaxf(sh.m[0][8 * g + r], sh.m[1][8 * g + r]), fmaxf(sh.m[2][8 * g + r], sh.m[3][8 * g + r]));
+                const float top = fmaxf(fmaxf(sh.m[0][8 * g + r], sh.m[1][8 * g + r]), fmaxf(sh.m[2][8 * g + r], sh.m[3][8 * g + r]));
                 float total = 0.0f, acc[8];
 #pragma unroll
                 for (int k = 0; k < 8; ++k) acc[k] = 0.0f;
@@ -524,16 +448,16 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : NT == 2 ? 3 : 2) kv4_a
                 }
                 if (row < p.S * p.group) {
                     if (whole) {
-                        if (row / p.group >= n_rows) top = kLowest;   // a row that stands for nothing
+                        const bool none = total == 0.0f || row / p.group >= n_rows;   // sees nothing, or stands for nothing
                         const uint32_t i = row / p.group, h = head * p.group + row % p.group;
-                        const float inv = top == kLowest ? 0.0f : kDown / total;
+                        const float inv = kDown / total;
                         *reinterpret_cast<uint4*>(p.out + ((static_cast<size_t>(b) * p.S + i) * p.H + h) * 128u + d) =
-                            make_uint4(pack_bf16x2(acc[0] * inv, acc[1] * inv), pack_bf16x2(acc[2] * inv, acc[3] * inv), pack_bf16x2(acc[4] * inv, acc[5] * inv), pack_bf16x2(acc[6] * inv, acc[7] * inv));
-                        if (p.lse != nullptr && d == 0u) p.lse[(static_cast<size_t>(b) * p.H + h) * p.S + i] = top == kLowest ? -INFINITY : (top + lg2(total)) * kLn2;
+                            none ? make_uint4(0u, 0u, 0u, 0u) : make_uint4(pack_bf16x2(acc[0] * inv, acc[1] * inv), pack_bf16x2(acc[2] * inv, acc[3] * inv), pack_bf16x2(acc[4] * inv, acc[5] * inv), pack_bf16x2(acc[6] * inv, acc[7] * inv));
+                        if (p.lse != nullptr && d == 0u) p.lse[(static_cast<size_t>(b) * p.H + h) * p.S + i] = none ? -INFINITY : (top + lg2(total)) * kLn2;
                     } else {
                         float* at = part + (8u * g + r) * 128u + d;
-                        *reinterpret_cast<float4*>(at) = make_float4(acc[0], acc[1], acc[2], acc[3]);
-                        *reinterpret_cast<float4*>(at + 4) = make_float4(acc[4], acc[5], acc[6], acc[7]);
+                        *reinterpret_cast<float4*>(at) = make_float4(acc[0] * kDown, acc[1] * kDown, acc[2] * kDown, acc[3] * kDown);
+                        *reinterpret_cast<float4*>(at + 4) = make_float4(acc[4] * kDown, acc[5] * kDown, acc[6] * kDown, acc[7] * kDown);
                         if (d == 0u) *reinterpret_cast<float2*>(part + 8u * NT * 128u + (8u * g + r) * 2u) = make_float2(top, total);
                     }
                 }
@@ -542,28 +466,24 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : NT == 2 ? 3 : 2) kv4_a
         }
         // what the generic proxy read and wrote in the ring is behind the next copies into it
         sm100::fence_proxy_async_smem();
-        pos += n_tiles;
-        in_seq += n_tiles;
     }
 }
 
 // One CTA a query row: rows that see nothing, and items that more than one CTA worked on
-template <int NT>
-__global__ void __launch_bounds__(kThreads) kv4_combine_kernel(const __grid_constant__ Kv4AttendParams p, uint32_t row_tiles, uint32_t attend_grid) {
-    __shared__ unsigned long long part[kWarps][2];
+__global__ void __launch_bounds__(kThreads) kv4_combine_kernel(const __grid_constant__ Kv4AttendParams p, Deal deal, uint32_t attend_grid) {
+    __shared__ Sums part[kWarps];
     __shared__ float sm_m[kWarps], sm_l[kWarps];
     __shared__ float4 sm_o[kWarps][32];
     pdl_launch();
     pdl_wait();
     const uint32_t rows = p.S * p.group, row = blockIdx.x % rows, bh = blockIdx.x / rows, head = bh % p.c.HK, b = bh / p.c.HK;
-    const uint32_t per = p.c.HK * row_tiles;
-    const Sums sums = sum_tiles(p.c, b, per, part);
-    const uint32_t tiles = tiles_of(p.c, b), item = head * row_tiles + row / (8u * NT);
-    const unsigned long long t0 = sums.below + 1ull * item * tiles, t1 = t0 + tiles;
+    const uint32_t entry = b * deal.row_tiles + row / deal.rows;
+    const Sums sums = sum_steps(p, deal, entry, part);
+    const uint32_t steps = steps_of(p, deal, entry);
     uint32_t from = 0, to = 0;   // the CTAs that hold parts, to - from + 1 of them
-    uint32_t n_work = 1;
-    if (tiles > 0u) {
-        n_work = workers(sums.all, attend_grid);
+    if (steps > 0u) {
+        const unsigned long long t0 = sums.below + 1ull * head * steps, t1 = t0 + steps;
+        const uint32_t n_work = workers(sums.all, attend_grid);
         from = worker_at(sums.all, n_work, t0);
         to = worker_at(sums.all, n_work, t1 - 1ull);
         if (from == to) return;
@@ -572,11 +492,11 @@ __global__ void __launch_bounds__(kThreads) kv4_combine_kernel(const __grid_cons
     const unsigned lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
     float m = kLowest, l = 0.0f;
     float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    if (tiles > 0u && sees) {
-        const uint32_t r = row % (8u * NT);
+    if (steps > 0u && sees) {
+        const uint32_t r = row % deal.rows;
         for (uint32_t w = from + warp; w <= to; w += kWarps) {
-            const float* src = slot_of(p.ws, w, w == from ? 1u : 0u, 8u * NT);
-            const float pm = ld_f32(src + 8u * NT * 128u + 2u * r), pl = ld_f32(src + 8u * NT * 128u + 2u * r + 1u);
+            const float* src = slot_of(p.ws, w, w == from ? 1u : 0u, deal.rows);
+            const float pm = ld_f32(src + deal.rows * 128u + 2u * r), pl = ld_f32(src + deal.rows * 128u + 2u * r + 1u);
             const uint4 raw = ld_v4(src + r * 128u + 4u * lane);
             const float top = fmaxf(m, pm), a = ex2(m - top), c = ex2(pm - top);
             m = top;
@@ -599,10 +519,11 @@ __global__ void __launch_bounds__(kThreads) kv4_combine_kernel(const __grid_cons
         l = fmaf(sm_l[w], f, l);
         o.x = fmaf(c.x, f, o.x), o.y = fmaf(c.y, f, o.y), o.z = fmaf(c.z, f, o.z), o.w = fmaf(c.w, f, o.w);
     }
-    const float inv = top == kLowest ? 0.0f : kDown / l;
+    const bool none = l == 0.0f;
+    const float inv = none ? 0.0f : 1.0f / l;
     const uint32_t i = row / p.group, h = head * p.group + row % p.group;
     *reinterpret_cast<uint2*>(p.out + ((static_cast<size_t>(b) * p.S + i) * p.H + h) * 128u + 4u * lane) = make_uint2(pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv));
-    if (p.lse != nullptr && lane == 0u) p.lse[(static_cast<size_t>(b) * p.H + h) * p.S + i] = top == kLowest ? -INFINITY : (top + lg2(l)) * kLn2;
+    if (p.lse != nullptr && lane == 0u) p.lse[(static_cast<size_t>(b) * p.H + h) * p.S + i] = none ? -INFINITY : (top + lg2(l)) * kLn2;
 }
 
 // The attention weights that the cached tokens received: p = 2^(s - lse), summed over the rows and the group's heads. A warp has 32 tokens and goes over all rows, in
@@ -677,9 +598,9 @@ __global__ void __launch_bounds__(kThreads) kv4_weigh_kernel(const __grid_consta
 }
 
 constexpr unsigned kStages1 = 3;
-constexpr uint32_t kMaxGroups = 4;   // groups of eight rows that an item holds at most
+constexpr uint32_t kMostFew = 32;   // rows of a KV head from which on the tensor cores' tiles of 128 rows take over
 
-uint32_t groups_of(uint32_t rows) { return rows <= 8u ? 1u : rows <= 16u ? 2u : kMaxGroups; }
+uint32_t groups_of(uint32_t rows) { return rows <= 8u ? 1u : rows <= 16u ? 2u : 4u; }
 
 uint32_t attend_grid(const Kv4View& c, uint32_t row_tiles) {
     const unsigned long long tiles = ((static_cast<unsigned long long>(c.table_width) << c.page_log2) + kTile - 1u) / kTile;
@@ -702,12 +623,19 @@ cudaError_t launch_rows(const Kv4AttendParams& p, uint32_t row_tiles, cudaStream
     }
     e = kv4_launch(kv4_attend_kernel<NT, kStages1>, dim3(grid), kThreads, smem, stream, p, row_tiles);
     if (e != cudaSuccess) return e;
-    return kv4_launch(kv4_combine_kernel<NT>, dim3(p.c.B * p.c.HK * p.S * p.group), kThreads, 0, stream, p, row_tiles, grid);
+    return kv4_launch(kv4_combine_kernel, dim3(p.c.B * p.c.HK * p.S * p.group), kThreads, 0, stream, p, Deal{8u * NT, row_tiles}, grid);
 }
 
 uint64_t partial_bytes(const Kv4View& c, uint32_t rows) {
-    const uint32_t nt = groups_of(rows), row_tiles = (rows + 8u * nt - 1u) / (8u * nt);
-    return static_cast<uint64_t>(attend_grid(c, row_tiles)) * 2u * 8u * nt * 130u * 4u;
+    if (rows > kMostFew) return kv4_partial_bytes(kv4_prefill_grid(), kv4_prefill_rows());
+    return kv4_partial_bytes(attend_grid(c, 1u), 8u * groups_of(rows));
+}
+
+cudaError_t launch_many(const Kv4AttendParams& p, cudaStream_t stream) {
+    const uint32_t rows = p.S * p.group, row_tiles = (rows + kv4_prefill_rows() - 1u) / kv4_prefill_rows();
+    const cudaError_t e = launch_kv4_prefill(p, row_tiles, stream);
+    if (e != cudaSuccess) return e;
+    return kv4_launch(kv4_combine_kernel, dim3(p.c.B * p.c.HK * rows), kThreads, 0, stream, p, Deal{kv4_prefill_rows(), row_tiles}, kv4_prefill_grid());
 }
 
 }  // namespace
@@ -718,9 +646,9 @@ uint64_t kv4_attend_workspace(const Kv4View& c, uint32_t S, uint32_t H, bool wei
 
 cudaError_t launch_kv4_attend(const Kv4AttendParams& params, cudaStream_t stream) {
     Kv4AttendParams p = params;
-    const uint32_t rows = p.S * p.group, nt = groups_of(rows), row_tiles = (rows + 8u * nt - 1u) / (8u * nt);
+    const uint32_t rows = p.S * p.group, nt = groups_of(rows);
     if (p.weights != nullptr && p.lse == nullptr) p.lse = p.ws + partial_bytes(p.c, rows) / 4u;   // the weights go by the rows' log-sum-exps
-    cudaError_t e = nt == 1u ? launch_rows<1>(p, row_tiles, stream) : nt == 2u ? launch_rows<2>(p, row_tiles, stream) : launch_rows<4>(p, row_tiles, stream);
+    cudaError_t e = rows > kMostFew ? launch_many(p, stream) : nt == 1u ? launch_rows<1>(p, 1u, stream) : nt == 2u ? launch_rows<2>(p, 1u, stream) : launch_rows<4>(p, 1u, stream);
     if (e != cudaSuccess || p.weights == nullptr) return e;
     const uint32_t tiles = ((p.c.table_width << p.c.page_log2) + kTile - 1u) / kTile;
     return kv4_launch(kv4_weigh_kernel, dim3(tiles * p.c.B * p.c.HK), kThreads, 0, stream, p, tiles);

@@ -1,0 +1,491 @@
+// Attention of many query rows over the 4-bit cache: prompts and chunks of them, on the tcgen05 tensor cores.
+//
+//   S = Q K^T,  P = 2^(c S + e - m),  O += P V',  l += sum P 2^-e,  out = O / l,   c = scale * log2(e), m a running reference per row,
+//
+// e the exponent of a token's largest V factor and V' = V 2^-e: P and V' are f16, K and Q bf16, where a code times its factor is exact.
+//
+// A CTA has 256 query rows of one KV head (rows of the sequence and of the head's group packed, whatever the group's size) as two tiles of 128 and goes over the tokens
+// 128 at a time. Per step four warps turn the step's K and V codes into 16-bit operands in shared memory, once for both tiles; one
+// thread issues the products, S from shared memory, P V with P from tensor memory; and two groups of four warps do the softmax, one tile each, a thread a row, so that
+// the tensor cores work on one tile while the other's softmax runs. P overwrites S in tensor memory. m moves only when a row's maximum exceeds it by 2^8, so O is
+// hardly ever rescaled.
+//
+// Steps are dealt out to one CTA per SM as kv4_schedule.cuh says; items that several CTAs worked on go through f32 partials and the combine kernel.
+#include "kv4.cuh"
+#include "kv4_schedule.cuh"
+#include "ptx_sm100.cuh"
+
+#include <atomic>
+
+namespace b200mx {
+
+namespace {
+
+using namespace kv4;
+using namespace sm100;
+
+constexpr uint32_t kTileRows = 128, kItemRows = 256, kStages = 2;
+// Slots of e and 2^-e, by step. The converters write those of step j + 4 behind the scores of step j + 2, which are behind the P of step j + 1 of the tiles that go on
+constexpr uint32_t kFactorSlots = 4;
+constexpr uint32_t kAtomBytes = 128u * 128u, kTileBytes = 2u * kAtomBytes;   // 128 rows x 64 elements with 128-byte swizzle; two of them a tile
+constexpr uint32_t kThreads = 512;
+// Warps 0-3 and 4-7: softmax of tile 0 and 1; 8-11: codes to bf16; 12: products. The pools of setmaxnreg come out of the launch's 128 registers a thread.
+constexpr int kSoftmaxRegs = 176, kConvertRegs = 112, kIssueRegs = 48;
+static_assert(8 * kSoftmaxRegs + 4 * kConvertRegs + 4 * kIssueRegs <= 16 * 128, "register shares");
+constexpr uint32_t kColS = 0, kColO = 256;   // S (and P in its first half) of tile q at 128 q, O at 256 + 128 q
+constexpr float kSlack = 8.0f;
+constexpr float kLn2 = 0.69314718055994531f;
+
+enum Bar : uint32_t { kKFull = 0, kKEmpty = 2, kVFull = 4, kVEmpty = 6, kSFull = 8, kPFull = 10, kODone = 12, kOFree = 14, kQFull = 16, kQEmpty = 17, kDrained = 18, kEFull = 19, kBars = 19 + kFactorSlots };
+
+struct Shared {
+    uint8_t q[2][kTileBytes], k[kStages][kTileBytes], v[kStages][kTileBytes];
+    float e[kFactorSlots][128], inv[kFactorSlots][128];
+    unsigned long long bars[kBars];
+    Sums part[kThreads / 32];
+    uint32_t tmem, failed, not_drained;
+};
+
+// a = a x + c, b = b x + d in one instruction
+__device__ __forceinline__ void fma2(uint32_t& a, uint32_t& b, float x, float c, float d) {
+    unsigned long long p, q, r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(p) : "r"(a), "r"(b));
+    asm("mov.b64 %0, {%1, %1};" : "=l"(q) : "f"(x));
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(c), "f"(d));
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(p) : "l"(p), "l"(q), "l"(r));
+    asm("mov.b64 {%0, %1}, %2;" : "=r"(a), "=r"(b) : "l"(p));
+}
+// a += x u, b += y w in one instruction
+__device__ __forceinline__ void accumulate2(float& a, float& b, float x, float y, float u, float w) {
+    unsigned long long p, q, r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(p) : "f"(a), "f"(b));
+    asm("mov.b64 %0, {%1, %2};" : "=l"(q) : "f"(x), "f"(y));
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(u), "f"(w));
+    asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(p) : "l"(q), "l"(r));
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(p));
+}
+__device__ __forceinline__ void add2(float& a, float& b, float x, float y) {
+    unsigned long long p, q;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(p) : "f"(a), "f"(b));
+    asm("mov.b64 %0, {%1, %2};" : "=l"(q) : "f"(x), "f"(y));
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(p) : "l"(p), "l"(q));
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(p));
+}
+
+// steps of tile q of a segment's item: those that its last live row sees
+__device__ __forceinline__ uint32_t tile_steps(const Kv4AttendParams& p, const Segment& s, uint32_t q, uint32_t length, uint32_t n) {
+    const uint32_t r0 = s.row0 + q * kTileRows;
+    if (r0 >= n * p.group) return 0u;
+    const uint32_t last = (min(r0 + kTileRows, n * p.group) - 1u) / p.group;
+    const uint32_t of = ((p.causal ? length - n + last + 1u : length) + kStepTokens - 1u) / kStepTokens;
+    return of <= s.first ? 0u : min(s.steps, of - s.first);
+}
+
+// 8 elements of a block, two bytes of codes in `half` (0, 1) of each word, times the block's factor, as bf16
+__device__ __forceinline__ uint4 to_bf16(uint32_t lo, uint32_t hi, bool half, float f) {
+    const float2 a = f16x2_to_f32(half ? e2m1x2_to_f16x2<2>(lo) : e2m1x2_to_f16x2<0>(lo)), b = f16x2_to_f32(half ? e2m1x2_to_f16x2<3>(lo) : e2m1x2_to_f16x2<1>(lo));
+    const float2 c = f16x2_to_f32(half ? e2m1x2_to_f16x2<2>(hi) : e2m1x2_to_f16x2<0>(hi)), d = f16x2_to_f32(half ? e2m1x2_to_f16x2<3>(hi) : e2m1x2_to_f16x2<1>(hi));
+    return make_uint4(pack_bf16x2(a.x * f, a.y * f), pack_bf16x2(b.x * f, b.y * f), pack_bf16x2(c.x * f, c.y * f), pack_bf16x2(d.x * f, d.y * f));
+}
+// the same in f16, `f` twice the block's factor
+__device__ __forceinline__ uint4 to_f16(uint32_t lo, uint32_t hi, bool half, uint32_t f) {
+    return make_uint4(mul_f16x2(half ? e2m1x2_to_f16x2<2>(lo) : e2m1x2_to_f16x2<0>(lo), f), mul_f16x2(half ? e2m1x2_to_f16x2<3>(lo) : e2m1x2_to_f16x2<1>(lo), f),
+                      mul_f16x2(half ? e2m1x2_to_f16x2<2>(hi) : e2m1x2_to_f16x2<0>(hi), f), mul_f16x2(half ? e2m1x2_to_f16x2<3>(hi) : e2m1x2_to_f16x2<1>(hi), f));
+}
+__device__ __forceinline__ uint4 convert(uint32_t lo, uint32_t hi, bool half, float f) { return to_bf16(lo, hi, half, f); }
+__device__ __forceinline__ uint4 convert(uint32_t lo, uint32_t hi, bool half, uint32_t f) { return to_f16(lo, hi, half, f); }
+// A token's 64 code bytes to its row of a tile
+template <typename F>
+__device__ __forceinline__ void store_row(uint8_t* tile, uint32_t row, const uint4 (&codes)[4], const F (&f)[4]) {
+    uint8_t* at = tile + row * 128u;
+#pragma unroll
+    for (uint32_t j = 0; j < 4; ++j) {
+#pragma unroll
+        for (uint32_t b = 0; b < 4; ++b) {
+            const uint4 x = convert(b < 2 ? codes[j].x : codes[j].y, b < 2 ? codes[j].z : codes[j].w, b & 1u, f[b]);
+            *reinterpret_cast<uint4*>(at + (b >> 1) * kAtomBytes + (((4u * (b & 1u) + j) ^ (row & 7u)) << 4)) = x;
+        }
+    }
+}
+
+__global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_constant__ Kv4AttendParams p, uint32_t row_tiles) {
+    extern __shared__ uint8_t smem_raw[];
+    Shared& sh = *reinterpret_cast<Shared*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023u) & ~static_cast<uintptr_t>(1023u));
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
+    const uint32_t bars = smem_u32(sh.bars);
+    auto bar = [&](uint32_t i) { return bars + 8u * i; };
+    if (threadIdx.x == 0u) {
+        for (uint32_t i = 0; i < 2; ++i) {
+            mbar_init(bar(kKFull + i), 128u), mbar_init(bar(kVFull + i), 128u);
+            mbar_init(bar(kKEmpty + i), 1u), mbar_init(bar(kVEmpty + i), 1u), mbar_init(bar(kSFull + i), 1u), mbar_init(bar(kODone + i), 1u);
+            mbar_init(bar(kPFull + i), 4u), mbar_init(bar(kOFree + i), 4u);
+        }
+        for (uint32_t i = 0; i < kFactorSlots; ++i) mbar_init(bar(kEFull + i), 4u);
+        mbar_init(bar(kQFull), 128u), mbar_init(bar(kQEmpty), 1u), mbar_init(bar(kDrained), 1u);
+        fence_mbar_init();
+        sh.failed = sh.not_drained = 0u;
+    }
+    if (warp == 12u) tmem_alloc(smem_u32(&sh.tmem), 512u);
+    tc_fence_before_sync();
+    __syncthreads();
+    tc_fence_after_sync();
+    const uint32_t tmem = sh.tmem;
+    pdl_launch();
+    pdl_wait();
+    const Deal deal{kItemRows, row_tiles};
+    const unsigned long long all = sum_steps(p, deal, 0u, sh.part).all;
+    const uint32_t n_work = workers(all, gridDim.x);
+    volatile uint32_t* failed = &sh.failed;
+    if (blockIdx.x < n_work) {
+        const unsigned long long begin = run_begin(all, n_work, blockIdx.x);
+        unsigned long long left = run_begin(all, n_work, blockIdx.x + 1u) - begin;
+        Place at = find_step(p, deal, begin);
+        if (warp < 8u) {
+            asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
+            const uint32_t q = warp >> 2, r = threadIdx.x & 127u, lanes = (warp & 3u) << 21;   // 32 TMEM lanes per warp, in bits 16 and up
+            const uint32_t t_s = tmem + lanes + kColS + 128u * q, t_o = tmem + lanes + kColO + 128u * q;
+            const float c = p.scale_log2;
+            uint32_t s_phase = 0, o_phase = 0, step0 = 0;   // step0: steps in front of the segment
+            bool ok = true;
+            while (left > 0ull && ok) {
+                const Segment seg = next_segment(p, deal, at, left);
+                const uint32_t length = length_of(p.c, seg.b), n = count_of(p.counts, seg.b, p.S, length);
+                const uint32_t steps = tile_steps(p, seg, q, length, n), row = seg.row0 + q * kTileRows + r, i = row / p.group;
+                const bool exists = row < p.S * p.group, live = exists && i < n;
+                const uint32_t limit = !live ? 0u : p.causal ? length - n + i + 1u : length;
+                float m = kLowest, l = 0.0f;
+                for (uint32_t j = 0; j < steps; ++j) {
+                    if (!mbar_wait(bar(kSFull + q), s_phase, failed)) {
+                        ok = false;
+                        break;
+                    }
+                    s_phase ^= 1u;
+                    // (not the K tile's barrier: while a group is still storing the rows of the segment before, that one may already be two steps on)
+                    if (!mbar_wait(bar(kEFull + (step0 + j) % kFactorSlots), (step0 + j) / kFactorSlots & 1u, failed)) {
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after_sync();
+                    const float4* e4 = reinterpret_cast<const float4*>(sh.e[(step0 + j) % kFactorSlots]);
+                    const float4* inv4 = reinterpret_cast<const float4*>(sh.inv[(step0 + j) % kFactorSlots]);
+                    uint32_t s[4][32];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) tmem_ld32(t_s + 32u * k, s[k]);
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        reg_fence32(s[k]);
+#pragma unroll
+                        for (int x = 0; x < 32; x += 4) {
+                            const float4 e = e4[8 * k + x / 4];
+                            fma2(s[k][x], s[k][x + 1], c, e.x, e.y);
+                            fma2(s[k][x + 2], s[k][x + 3], c, e.z, e.w);
+                        }
+                    }
+                    const uint32_t tok0 = (seg.first + j) * kStepTokens;
+                    if (__any_sync(0xFFFFFFFFu, tok0 + kStepTokens > limit)) {
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+#pragma unroll
+                            for (int x = 0; x < 32; ++x) {
+                                if (tok0 + 32u * k + x >= limit) s[k][x] = 0xFF800000u;
+                            }
+                        }
+                    }
+                    float top[4];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        top[k] = fmaxf(__uint_as_float(s[k][0]), __uint_as_float(s[k][1]));
+#pragma unroll
+                        for (int x = 2; x < 32; x += 2) top[k] = fmaxf(top[k], fmaxf(__uint_as_float(s[k][x]), __uint_as_float(s[k][x + 1])));
+                    }
+                    const float most = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+                    const bool over = most > m + kSlack;
+                    if (__any_sync(0xFFFFFFFFu, over)) {
+                        const float next = over ? most : m, f = ex2(m - next);
+                        m = next;
+                        l *= f;
+                        if (j > 0u) {   // the product before this one is done: S came behind it
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) {
+                                uint32_t o[32];
+                                tmem_ld32(t_o + 32u * k, o);
+                                tmem_wait_ld();
+                                reg_fence32(o);
+#pragma unroll
+                                for (int x = 0; x < 32; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * f);
+                                tmem_st32(t_o + 32u * k, o);
+                            }
+                            tmem_wait_st();
+                        }
+                    }
+                    float l0 = 0.0f, l1 = 0.0f;
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        uint32_t pw[16];
+#pragma unroll
+                        for (int x = 0; x < 8; ++x) {
+                            const float4 inv = inv4[8 * k + x];
+#pragma unroll
+                            for (int y = 0; y < 2; ++y) {
+                                float a = __uint_as_float(s[k][4 * x + 2 * y]), b = __uint_as_float(s[k][4 * x + 2 * y + 1]);
+                                add2(a, b, -m, -m);
+                                a = ex2(a), b = ex2(b);
+                                accumulate2(l0, l1, a, b, y ? inv.z : inv.x, y ? inv.w : inv.y);
+                                pw[2 * x + y] = pack_f16x2(a, b);
+                            }
+                        }
+                        tmem_st16(t_s + 16u * k, pw);
+                    }
+                    l += l0 + l1;
+                    tmem_wait_st();
+                    tc_fence_before_sync();
+                    __syncwarp();
+                    if (lane == 0u) mbar_arrive(bar(kPFull + q));
+                }
+                if (!ok) break;
+                step0 += seg.steps;
+                const bool whole = seg.steps == seg.of;
+                const uint32_t h = seg.head * p.group + row % p.group;
+                float* part = slot_of(p.ws, blockIdx.x, seg.first == 0u ? 1u : 0u, kItemRows) + (q * kTileRows + r) * 128u;
+                __nv_bfloat16* out = p.out + ((static_cast<size_t>(seg.b) * p.S + i) * p.H + h) * 128u;
+                const bool none = l == 0.0f;   // NaN is something
+                const float inv = none ? 0.0f : kDown / l;
+                if (steps > 0u) {
+                    if (!mbar_wait(bar(kODone + q), o_phase, failed)) {
+                        ok = false;
+                        break;
+                    }
+                    o_phase ^= 1u;
+                    tc_fence_after_sync();
+                }
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    uint32_t o[32];
+                    if (steps > 0u) {
+                        tmem_ld32(t_o + 32u * k, o);
+                        tmem_wait_ld();
+                        reg_fence32(o);
+                    } else {
+#pragma unroll
+                        for (int x = 0; x < 32; ++x) o[x] = 0u;
+                    }
+                    if (k == 3 && steps > 0u) {
+                        tc_fence_before_sync();
+                        __syncwarp();
+                        if (lane == 0u) mbar_arrive(bar(kOFree + q));
+                    }
+                    if (!exists) continue;
+                    if (whole) {
+#pragma unroll
+                        for (int x = 0; x < 32; x += 8) {
+                            uint4 w;
+                            w.x = pack_bf16x2(__uint_as_float(o[x]) * inv, __uint_as_float(o[x + 1]) * inv), w.y = pack_bf16x2(__uint_as_float(o[x + 2]) * inv, __uint_as_float(o[x + 3]) * inv);
+                            w.z = pack_bf16x2(__uint_as_float(o[x + 4]) * inv, __uint_as_float(o[x + 5]) * inv), w.w = pack_bf16x2(__uint_as_float(o[x + 6]) * inv, __uint_as_float(o[x + 7]) * inv);
+                            if (none) w = make_uint4(0u, 0u, 0u, 0u);
+                            *reinterpret_cast<uint4*>(out + 32 * k + x) = w;
+                        }
+                    } else if (live) {
+#pragma unroll
+                        for (int x = 0; x < 32; x += 4) *reinterpret_cast<float4*>(part + 32 * k + x) = make_float4(__uint_as_float(o[x]) * kDown, __uint_as_float(o[x + 1]) * kDown, __uint_as_float(o[x + 2]) * kDown, __uint_as_float(o[x + 3]) * kDown);
+                    }
+                }
+                if (whole) {
+                    if (exists && p.lse != nullptr) p.lse[(static_cast<size_t>(seg.b) * p.H + h) * p.S + i] = none ? -INFINITY : (m + lg2(l)) * kLn2;
+                } else if (live) {
+                    *reinterpret_cast<float2*>(slot_of(p.ws, blockIdx.x, seg.first == 0u ? 1u : 0u, kItemRows) + kItemRows * 128u + 2u * (q * kTileRows + r)) = make_float2(m, l);
+                }
+            }
+        } else if (warp < 12u) {
+            asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kConvertRegs));
+            const uint32_t r = threadIdx.x & 127u, page = 1u << p.c.page_log2;
+            uint32_t step = 0, q_count = 0;   // steps and segments so far
+            bool ok = true;
+            while (left > 0ull && ok) {
+                const Segment seg = next_segment(p, deal, at, left);
+                const uint32_t length = length_of(p.c, seg.b), n = count_of(p.counts, seg.b, p.S, length);
+                uint4 k[4], v[4];
+                uint32_t ks = 0, vs = 0;
+                bool lost = false, empty = true;
+                auto fetch = [&](uint32_t j) {
+                    const uint32_t t = (seg.first + j) * kStepTokens + r;
+                    empty = j >= seg.steps || t >= length;
+                    if (empty) return;
+                    const long long id = page_of(p.c, seg.b, t);
+                    lost = id < 0;
+                    if (lost) return;
+                    const uint8_t* rec = record_of(p.c, id, seg.head);
+                    const uint32_t slot = t & (page - 1u);
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) k[x] = ld_v4(rec + 64u * slot + 16u * x), v[x] = ld_v4(rec + 64u * (page + slot) + 16u * x);
+                    ks = ld_u32(rec + 128u * page + 4u * slot), vs = ld_u32(rec + 132u * page + 4u * slot);
+                };
+                fetch(0);
+                // the query rows: 16 threads a row, 16 bytes each
+                if (!mbar_wait(bar(kQEmpty), (q_count + 1u) & 1u, failed)) {
+                    ok = false;
+                    break;
+                }
+                ++q_count;
+#pragma unroll 1
+                for (uint32_t x0 = 0; x0 < 32u; x0 += 8u) {
+                    uint4 raw[8];
+#pragma unroll
+                    for (uint32_t x = 0; x < 8u; ++x) {
+                        const uint32_t e = (x0 + x) * 128u + r, row = seg.row0 + (e >> 4), i = row / p.group;
+                        raw[x] = make_uint4(0u, 0u, 0u, 0u);
+                        if (i < n) raw[x] = ld_v4(p.q.data + seg.b * p.q.stride_b + i * p.q.stride_s + (seg.head * p.group + row % p.group) * p.q.stride_h + 16u * (e & 15u));
+                    }
+#pragma unroll
+                    for (uint32_t x = 0; x < 8u; ++x) {
+                        const uint32_t e = (x0 + x) * 128u + r, row = e >> 4, chunk = e & 15u;
+                        *reinterpret_cast<uint4*>(sh.q[row >> 7] + (chunk >> 3) * kAtomBytes + (row & 127u) * 128u + (((chunk & 7u) ^ (row & 7u)) << 4)) = raw[x];
+                    }
+                }
+                fence_proxy_async_smem();
+                mbar_arrive(bar(kQFull));
+                for (uint32_t j = 0; j < seg.steps; ++j, ++step) {
+                    const uint32_t st = step % kStages, parity = (step / kStages + 1u) & 1u;
+                    // A token behind the length must not bring NaN into P V; one that is lost, or whose V is NaN, makes the rows that see it NaN by its scores
+                    float fk[4];
+                    uint32_t fv[4];
+                    const ValueFactors f = value_factors(empty || lost ? 0x7F7F7F7Fu : vs);
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) fk[x] = scale_f32(ks, x);
+                    fv[0] = __byte_perm(f.r01, 0u, 0x1010), fv[1] = __byte_perm(f.r01, 0u, 0x3232), fv[2] = __byte_perm(f.r23, 0u, 0x1010), fv[3] = __byte_perm(f.r23, 0u, 0x3232);
+                    if (empty || lost) {
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) k[x] = v[x] = make_uint4(0u, 0u, 0u, 0u);
+                    }
+                    if (empty || lost || f.broken) {
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) fk[x] = empty ? 0.0f : __uint_as_float(0x7FC00000u), fv[x] = 0u;
+                    }
+                    if (!mbar_wait(bar(kKEmpty + st), parity, failed)) {
+                        ok = false;
+                        break;
+                    }
+                    sh.e[step % kFactorSlots][r] = f.e, sh.inv[step % kFactorSlots][r] = f.inv;
+                    __syncwarp();
+                    if (lane == 0u) mbar_arrive(bar(kEFull + step % kFactorSlots));
+                    store_row(sh.k[st], r, k, fk);
+                    fence_proxy_async_smem();
+                    mbar_arrive(bar(kKFull + st));
+                    if (!mbar_wait(bar(kVEmpty + st), parity, failed)) {
+                        ok = false;
+                        break;
+                    }
+                    store_row(sh.v[st], r, v, fv);
+                    fence_proxy_async_smem();
+                    mbar_arrive(bar(kVFull + st));
+                    lost = false, ks = vs = 0u;
+                    fetch(j + 1u);
+                }
+            }
+        } else {
+            asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kIssueRegs));
+            if (warp == 12u) {
+                const uint32_t id_s = idesc_16bit(true, 128, 128, 0, 0), id_o = idesc_16bit(false, 128, 128, 0, 1);
+                const uint64_t dq = make_smem_desc(smem_u32(sh.q[0]), 16, 1024, kSwizzle128B), dk = make_smem_desc(smem_u32(sh.k[0]), 16, 1024, kSwizzle128B);
+                const uint64_t dv = make_smem_desc(smem_u32(sh.v[0]), kAtomBytes, 1024, kSwizzle128B);
+                uint32_t step = 0, q_count = 0, p_phase[2] = {0u, 0u}, o_count[2] = {0u, 0u};
+                auto scores = [&](uint32_t q, uint32_t st) {
+                    if (elect_one_sync()) {
+#pragma unroll
+                        for (uint32_t x = 0; x < 8u; ++x) {
+                            const uint32_t off = ((x >> 2) * kAtomBytes + (x & 3u) * 32u) >> 4;
+                            mma_f16_ss(tmem + kColS + 128u * q, dq + (q * kTileBytes >> 4) + off, dk + (st * kTileBytes >> 4) + off, id_s, x > 0u ? 1u : 0u);
+                        }
+                        tc_commit(bar(kSFull + q));
+                    }
+                    __syncwarp();
+                };
+                auto outputs = [&](uint32_t q, uint32_t st, bool first, bool last) {
+                    if (elect_one_sync()) {
+#pragma unroll
+                        for (uint32_t x = 0; x < 8u; ++x)
+                            mma_f16_ts(tmem + kColO + 128u * q, tmem + kColS + 128u * q + 8u * x, dv + ((st * kTileBytes + x * 2048u) >> 4), id_o, (!first || x > 0u) ? 1u : 0u);
+                        if (last) tc_commit(bar(kODone + q));
+                    }
+                    __syncwarp();
+                };
+                auto commit = [&](uint32_t b) {
+                    if (elect_one_sync()) tc_commit(b);
+                    __syncwarp();
+                };
+                bool ok = true;
+                auto wait = [&](uint32_t b, uint32_t parity) {
+                    if (ok && !mbar_wait(b, parity, failed)) ok = false;
+                    return ok;
+                };
+                while (left > 0ull && ok) {
+                    const Segment seg = next_segment(p, deal, at, left);
+                    const uint32_t length = length_of(p.c, seg.b), n = count_of(p.counts, seg.b, p.S, length);
+                    const uint32_t steps[2] = {tile_steps(p, seg, 0u, length, n), tile_steps(p, seg, 1u, length, n)};
+                    if (!wait(bar(kQFull), q_count & 1u)) break;
+                    ++q_count;
+                    if (!wait(bar(kKFull + step % kStages), step / kStages & 1u)) break;
+                    tc_fence_after_sync();
+                    if (steps[0] > 0u) scores(0u, step % kStages);
+                    if (steps[1] > 0u) scores(1u, step % kStages);
+                    commit(bar(kKEmpty + step % kStages));
+                    if (seg.steps == 1u) commit(bar(kQEmpty));
+                    for (uint32_t j = 0; j < seg.steps; ++j, ++step) {
+                        const uint32_t st = step % kStages, next = (step + 1u) % kStages;
+                        const bool more = j + 1u < seg.steps;
+                        if (!wait(bar(kVFull + st), step / kStages & 1u)) break;
+                        if (more && !wait(bar(kKFull + next), (step + 1u) / kStages & 1u)) break;
+#pragma unroll
+                        for (uint32_t q = 0; q < 2u; ++q) {
+                            if (j < steps[q]) {
+                                if (j == 0u) wait(bar(kOFree + q), (o_count[q]++ + 1u) & 1u);
+                                if (!wait(bar(kPFull + q), p_phase[q])) break;
+                                p_phase[q] ^= 1u;
+                                tc_fence_after_sync();
+                                outputs(q, st, j == 0u, j + 1u == steps[q]);
+                            }
+                            if (q == 1u) commit(bar(kVEmpty + st));
+                            if (more && j + 1u < steps[q]) scores(q, next);
+                        }
+                        if (!ok) break;
+                        if (more) commit(bar(kKEmpty + next));
+                        if (j + 2u == seg.steps) commit(bar(kQEmpty));
+                    }
+                }
+                if (!ok) {   // whatever was issued has to be over before the tensor memory goes back
+                    commit(bar(kDrained));
+                    (void)mbar_wait(bar(kDrained), 0u, &sh.not_drained);
+                }
+            }
+        }
+    }
+    tc_fence_before_sync();
+    __syncthreads();
+    if (threadIdx.x == 0u && sh.failed != 0u) atomicOr(p.status, 1u);
+    if (warp == 12u) {
+        tc_fence_after_sync();
+        tmem_dealloc(tmem, 512u);
+    }
+}
+
+}  // namespace
+
+uint32_t kv4_prefill_grid() { return static_cast<uint32_t>(current_sm_count()); }
+uint32_t kv4_prefill_rows() { return kItemRows; }
+
+cudaError_t launch_kv4_prefill(const Kv4AttendParams& p, uint32_t row_tiles, cudaStream_t stream) {
+    constexpr size_t smem = sizeof(Shared) + 1024u;
+    static_assert(smem <= 227u * 1024u, "shared memory of a CTA");
+    static std::atomic<bool> set[64];
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (dev < 0 || dev >= 64 || !set[dev].load(std::memory_order_relaxed)) {
+        e = cudaFuncSetAttribute(kv4_prefill_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+        if (e != cudaSuccess) return e;
+        if (dev >= 0 && dev < 64) set[dev].store(true, std::memory_order_relaxed);
+    }
+    return kv4_launch(kv4_prefill_kernel, dim3(kv4_prefill_grid()), kThreads, smem, stream, p, row_tiles);
+}
+
+}  // namespace b200mx

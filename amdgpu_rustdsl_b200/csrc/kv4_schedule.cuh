@@ -1,0 +1,109 @@
+// How the attention kernels of the 4-bit cache share their work, worked out on the device from the lengths.
+//
+// An entry is a sequence and one of its row tiles (`rows` query rows of a KV head); an item is an entry and a KV head, heads fastest. An item has as many steps as there
+// are tiles of 128 tokens that its rows see. All steps of all items, in order, are dealt out in equal runs to the CTAs.
+#pragma once
+#include "kv4.cuh"
+
+namespace b200mx {
+namespace kv4 {
+
+constexpr uint32_t kStepTokens = 128;
+
+struct Deal {
+    uint32_t rows, row_tiles;   // of an item, of a sequence
+};
+
+__device__ __forceinline__ uint32_t steps_of(const Kv4AttendParams& p, const Deal& d, uint32_t entry) {
+    const uint32_t b = entry / d.row_tiles, row0 = (entry - b * d.row_tiles) * d.rows, length = length_of(p.c, b), n = count_of(p.counts, b, p.S, length);
+    if (row0 >= n * p.group) return 0u;
+    const uint32_t last = (min(row0 + d.rows, n * p.group) - 1u) / p.group;
+    return ((p.causal ? length - n + last + 1u : length) + kStepTokens - 1u) / kStepTokens;
+}
+
+struct Sums {
+    unsigned long long below, all;
+};
+// Steps of the entries below `upto`, and of all, times the heads. All threads of the CTA; `part` has an element per warp.
+__device__ __forceinline__ Sums sum_steps(const Kv4AttendParams& p, const Deal& d, uint32_t upto, Sums* part) {
+    unsigned long long below = 0, all = 0;
+    for (uint32_t e = threadIdx.x; e < p.c.B * d.row_tiles; e += blockDim.x) {
+        const uint32_t t = steps_of(p, d, e);
+        all += t;
+        if (e < upto) below += t;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        below += __shfl_xor_sync(0xFFFFFFFFu, below, o);
+        all += __shfl_xor_sync(0xFFFFFFFFu, all, o);
+    }
+    if ((threadIdx.x & 31u) == 0u) part[threadIdx.x >> 5] = {below, all};
+    __syncthreads();
+    below = all = 0;
+    for (unsigned w = 0; w < blockDim.x / 32u; ++w) below += part[w].below, all += part[w].all;
+    __syncthreads();
+    return {below * p.c.HK, all * p.c.HK};
+}
+
+// CTA w of n has the steps [run_begin(w), run_begin(w + 1)) of `all`; worker_at is the one that has a step
+__device__ __forceinline__ uint32_t workers(unsigned long long all, uint32_t grid) { return static_cast<uint32_t>(all < grid ? all : grid); }
+__device__ __forceinline__ unsigned long long run_begin(unsigned long long all, uint32_t n, uint32_t w) { return all * w / n; }
+__device__ __forceinline__ uint32_t worker_at(unsigned long long all, uint32_t n, unsigned long long step) { return static_cast<uint32_t>(((step + 1ull) * n - 1ull) / all); }
+
+// The entry that step `pos` belongs to and the step's number within it, for all lanes of a warp
+struct Place {
+    uint32_t entry;
+    unsigned long long in;   // step within the entry's items
+};
+__device__ __forceinline__ Place find_step(const Kv4AttendParams& p, const Deal& d, unsigned long long pos) {
+    const unsigned lane = threadIdx.x & 31u;
+    const uint32_t entries = p.c.B * d.row_tiles;
+    unsigned long long before = 0;
+    for (uint32_t e0 = 0; e0 < entries; e0 += 32u) {
+        const unsigned long long t = e0 + lane < entries ? 1ull * steps_of(p, d, e0 + lane) * p.c.HK : 0ull;
+        unsigned long long s = t;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const unsigned long long a = __shfl_up_sync(0xFFFFFFFFu, s, o);
+            if (lane >= static_cast<unsigned>(o)) s += a;
+        }
+        const unsigned hit = __ballot_sync(0xFFFFFFFFu, before + s > pos);
+        if (hit != 0u) {
+            const int at = __ffs(hit) - 1;
+            return {e0 + static_cast<uint32_t>(at), pos - (before + __shfl_sync(0xFFFFFFFFu, s - t, at))};
+        }
+        before += __shfl_sync(0xFFFFFFFFu, s, 31);
+    }
+    return {entries, 0ull};
+}
+
+// A run of steps of one item
+struct Segment {
+    uint32_t b, head, row0;         // the item
+    uint32_t first, steps, of;      // steps first .. first + steps - 1 of `of`
+};
+// The segment at the head of a CTA's run of `left` steps; moves on behind it
+__device__ __forceinline__ Segment next_segment(const Kv4AttendParams& p, const Deal& d, Place& at, unsigned long long& left) {
+    uint32_t of = steps_of(p, d, at.entry);
+    while (at.in >= 1ull * of * p.c.HK) {   // also where an entry has none
+        at.in -= 1ull * of * p.c.HK;
+        of = steps_of(p, d, ++at.entry);
+    }
+    Segment s;
+    s.b = at.entry / d.row_tiles, s.row0 = (at.entry - s.b * d.row_tiles) * d.rows;
+    s.head = static_cast<uint32_t>(at.in / of), s.first = static_cast<uint32_t>(at.in - 1ull * s.head * of), s.of = of;
+    s.steps = static_cast<uint32_t>(min(static_cast<unsigned long long>(of - s.first), left));
+    at.in += s.steps;
+    left -= s.steps;
+    return s;
+}
+
+// Partials of CTA w: two slots (0: an item that an earlier CTA began, 1: one that a later CTA goes on with), each `rows` x 128 f32 of O, in front of `rows` pairs of M (base 2) and l
+__device__ __forceinline__ float* slot_of(float* ws, uint32_t w, uint32_t slot, uint32_t rows) { return ws + (static_cast<size_t>(w) * 2u + slot) * rows * 130u; }
+constexpr float kLowest = -1e30f;   // M of a row that has seen nothing
+
+}  // namespace kv4
+
+inline uint64_t kv4_partial_bytes(uint32_t grid, uint32_t rows) { return static_cast<uint64_t>(grid) * 2u * rows * 130u * 4u; }
+
+}  // namespace b200mx

@@ -14,6 +14,15 @@ from tests import kv4_reference as R
 pytestmark = pytest.mark.gpu
 
 
+@pytest.fixture(autouse=True)
+def no_wait_ran_out():
+    """No kernel gave up a wait (the status word is the process's: earlier tests' kernels count too)."""
+    from amdgpu_rustdsl_b200 import device_status
+    before = device_status()
+    yield
+    assert device_status() == before
+
+
 def make_cache(lengths, HK, page, seed=0, width=None, extra=3, k_gain=None, v_gain=None, garbage=0xFF):
     """A cache with normal keys and values; pages in random order; unused pages and tokens behind the lengths hold `garbage` bytes (0xFF: NaN scales)."""
     from amdgpu_rustdsl_b200 import Kv4Cache
@@ -341,6 +350,20 @@ def test_many_tiles_against_a_plain_product():
                     assert ((out[b, :, h].double() - ref).abs() <= room).all()
                     assert ((lse[b, h].double() - ref_lse).abs() <= off).all()
                 assert ((w[b, hk, :L].double() - mass).abs() <= 2 * off * mass + 1e-30).all()
+
+
+def test_back_to_back_calls_give_the_same():
+    """Many launches without a wait between them, of work that is cut between CTAs in the middle of items: none stalls, all give the same bits."""
+    from amdgpu_rustdsl_b200 import fmha_fwd_kv4
+    cache = make_cache([3000, 1500], 2, 64, seed=15)
+    for S in (1, 4, 100, 300):
+        q = queries(2, S, 8)
+        first, out = torch.empty_like(q), torch.empty_like(q)
+        fmha_fwd_kv4(q, cache, first)
+        for _ in range(200):
+            fmha_fwd_kv4(q, cache, out)
+        torch.cuda.synchronize()
+        assert torch.equal(out, first)
 
 
 def test_append_rounds_every_bf16_value_as_the_definition_does():

@@ -171,26 +171,26 @@ __device__ __forceinline__ uint32_t mul_f16x2(uint32_t a, uint32_t b) {
     asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
     return r;
 }
-// Softmax of rows that multiply V in f16. V's four factors of a token are taken relative to 2^e, e the exponent of the largest, kept within what f32 sums of 2^(s - M)
-// bear (they lie between 2^-kHighE and 2^(8 - kLowE) a token when M follows s + e). The factors go in times 2^kUp, which the division by the sums takes out again: f16 has
-// more room below 1 than above.
+// Softmax of rows that multiply V in f16. V's factors of a group of tokens that are worked on together are taken relative to 2^e, e the exponent of the group's largest, kept
+// within what f32 sums of 2^(s - M) bear (they lie between 2^-kHighE and 2^(8 - kLowE) a token when M follows s + e). The factors go in times 2^kUp, which the division
+// by the sums takes out again: f16 has more room below 1 than above, and factors are exact down to 2^-34 of the group's largest.
 constexpr int kLowE = -100, kHighE = 124, kUp = 10;
 constexpr float kDown = 1.0f / (1 << kUp);
+// the largest of a token's four scale bytes
+__device__ __forceinline__ uint32_t largest_byte(uint32_t word) { return max(max(word & 0xFFu, (word >> 8) & 0xFFu), max((word >> 16) & 0xFFu, word >> 24)); }
+__device__ __forceinline__ int group_exponent(uint32_t largest) { return min(max(static_cast<int>(largest) - 127, kLowE), kHighE); }
 struct ValueFactors {
-    float e, inv;        // e and 2^-e
-    uint32_t r01, r23;   // 2^(E - 127 - e + kUp) of the blocks, f16 (E <= 252 leaves them below its largest)
-    bool broken;         // a block is NaN
+    uint32_t r01, r23;   // 2^(E - 127 - e + kUp) of the blocks, f16 (E <= 252 leaves them below its largest); NaN for 255
 };
-__device__ __forceinline__ ValueFactors value_factors(uint32_t word) {
-    const int e0 = word & 0xFFu, e1 = (word >> 8) & 0xFFu, e2 = (word >> 16) & 0xFFu, e3 = word >> 24;
-    const int top = max(max(e0, e1), max(e2, e3)), e = min(max(top - 127, kLowE), kHighE);
-    float r0 = __uint_as_float(static_cast<uint32_t>(max(e0 - e + kUp, 0)) << 23), r1 = __uint_as_float(static_cast<uint32_t>(max(e1 - e + kUp, 0)) << 23);
-    float r2 = __uint_as_float(static_cast<uint32_t>(max(e2 - e + kUp, 0)) << 23), r3 = __uint_as_float(static_cast<uint32_t>(max(e3 - e + kUp, 0)) << 23);
-    if (top == 255) {
+__device__ __forceinline__ ValueFactors value_factors(uint32_t word, uint32_t largest, int e) {
+    const int e0 = word & 0xFFu, e1 = (word >> 8) & 0xFFu, e2 = (word >> 16) & 0xFFu, e3 = word >> 24, up = kUp - e;
+    float r0 = __uint_as_float(static_cast<uint32_t>(max(e0 + up, 0)) << 23), r1 = __uint_as_float(static_cast<uint32_t>(max(e1 + up, 0)) << 23);
+    float r2 = __uint_as_float(static_cast<uint32_t>(max(e2 + up, 0)) << 23), r3 = __uint_as_float(static_cast<uint32_t>(max(e3 + up, 0)) << 23);
+    if (largest == 255u) {
         const float nan = __uint_as_float(0x7FC00000u);
         r0 = e0 == 255 ? nan : r0, r1 = e1 == 255 ? nan : r1, r2 = e2 == 255 ? nan : r2, r3 = e3 == 255 ? nan : r3;
     }
-    return {static_cast<float>(e), __uint_as_float(static_cast<uint32_t>(127 - e) << 23), pack_f16x2(r0, r1), pack_f16x2(r2, r3), top == 255};
+    return {pack_f16x2(r0, r1), pack_f16x2(r2, r3)};
 }
 __device__ __forceinline__ uint32_t transpose_8x8(uint32_t a) {
     uint32_t r;

@@ -99,6 +99,9 @@ int fmha_kv4_attend(const fmha_kv4_cache* cache, const fmha_kv4_attend_args* a, 
     if (a->S == 0u) return 0;
     if (static_cast<uint64_t>(p.c.B) * a->S * a->H > kMostRows) return refuse(err, cap, "attend: more than 2^30 query rows");
     const uint64_t tokens = static_cast<uint64_t>(p.c.table_width) << p.c.page_log2;
+    // the kernels deal out steps of 128 tokens and 256 rows at most, counted in 32 bits
+    const uint64_t row_tiles = (static_cast<uint64_t>(a->S) * (a->H / p.c.HK) + 255u) / 256u;
+    if (((tokens + 127u) / 128u) * p.c.B * p.c.HK > 0xFFFFFFFFull / row_tiles) return refuse(err, cap, "attend: more than 2^32 steps of 128 tokens and 256 query rows");
     if (a->weights != nullptr && a->weights_width < tokens) return refuse(err, cap, "attend: weights must have room for the %llu tokens of the table", static_cast<unsigned long long>(tokens));
     if (a->weights == nullptr && a->weights_in != nullptr) return refuse(err, cap, "attend: weights_in without weights");
     if (a->weights != nullptr && static_cast<uint64_t>(p.c.B) * p.c.HK * ((tokens + 127u) / 128u) > kMostRows) return refuse(err, cap, "attend: more than 2^37 cached tokens x heads with weights");

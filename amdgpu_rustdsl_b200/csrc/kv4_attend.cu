@@ -11,9 +11,8 @@
 //   O^T [128 x 8 rows] += V^T [128 x 16 tokens] P^T  P goes from S^T's layout to the operand's by an 8 x 8 transpose between lanes; V's factors multiply P
 // Q goes in as f16 with a power of two per row taken out, which is exact for bf16 elements down to 2^-30 of the row's largest.
 //
-// Softmax in base 2 with a running reference per row. P V wants P times V's factor in f16: the reference M follows s + e, e the exponent of the token's largest V
-// factor (kept within what f32 sums of 2^(s - M) bear), so that P 2^e is at most 2^4 however large V is; the four factors of a token relative to 2^e are exact
-// in f16 down to 2^-34. M moves when a value exceeds it by more than 2^4, by a vote of the warp; the sums and O are rescaled then.
+// Softmax in base 2 with a running reference per row. P V wants P times V's factor in f16: the reference M follows s + e, e the exponent of the largest V factor of
+// the 32 tokens, so that P 2^e is at most 2^4 however large V is; the factors relative to 2^e are exact in f16 down to 2^-34. M moves when a value exceeds it by more than 2^4, by a vote of the warp; the sums and O are rescaled then.
 #include "kv4.cuh"
 #include "kv4_schedule.cuh"
 #include "ptx_sm100.cuh"
@@ -38,7 +37,6 @@ constexpr float kLn2 = 0.69314718055994531f, kLog2e = 1.44269504088896341f;
 // What a unit's 32 lanes work out for its tokens, one lane a token
 struct TokenFactors {
     float4 k[kUnit];           // 2^(E - 127) of the four K blocks
-    float2 v[kUnit];           // e, 2^-e
     uint32_t r[kUnit / 2][4];  // [token pair][block]: V's factors over 2^(e - kUp), f16, of the pair's tokens in the operand's order
 };
 
@@ -139,18 +137,20 @@ __device__ __forceinline__ void scores(float (&s)[NT][4], const uint8_t* codes, 
     }
 }
 
-// One lane a token: its factors, from the unit's scale bytes. A token behind the length is masked later; its V factors have to be finite.
-__device__ __forceinline__ void token_factors(TokenFactors& f, uint32_t kw, uint32_t vw, bool live) {
+// One lane a token: its factors, from the unit's scale bytes; e of the unit. A token behind the length is masked later; its V factors have to be finite.
+__device__ __forceinline__ int token_factors(TokenFactors& f, uint32_t kw, uint32_t vw, bool live) {
     const unsigned t = threadIdx.x & 31u;
     f.k[t] = make_float4(scale_f32(kw, 0), scale_f32(kw, 1), scale_f32(kw, 2), scale_f32(kw, 3));
-    if (!live) vw = 0x7F7F7F7Fu;
-    const ValueFactors vf = value_factors(vw);
-    f.v[t] = make_float2(vf.e, vf.inv);
+    if (!live) vw = 0u;
+    const uint32_t largest = largest_byte(vw);
+    const int e = group_exponent(__reduce_max_sync(0xFFFFFFFFu, largest == 255u ? 0u : largest));
+    const ValueFactors vf = value_factors(vw, largest, e);
     // an even lane takes blocks 0 and 1 of its pair, the odd one 2 and 3; pairs whose operand rows are the other way round are stored so
     const bool odd = t & 1u, flip = (t >> 1) & 1u;
     const uint32_t mine = odd ? vf.r23 : vf.r01, got = __shfl_xor_sync(0xFFFFFFFFu, odd ? vf.r01 : vf.r23, 1);
     const uint32_t first = odd != flip ? got : mine, second = odd != flip ? mine : got;
     *reinterpret_cast<uint2*>(&f.r[t >> 1][odd ? 2 : 0]) = make_uint2(__byte_perm(first, second, 0x5410), __byte_perm(first, second, 0x7632));
+    return e;
 }
 
 template <int NT, unsigned kStages>
@@ -181,20 +181,18 @@ __device__ const LostPages kNowhere;
 // 32 tokens: scores, softmax, and their part of O
 template <int NT, bool kEdge>
 __device__ __forceinline__ void attend_unit(float (&o)[NT][8][4], float (&m)[NT][2], float (&l)[NT][2], const QueryRows<NT>& x, const uint8_t* k_codes, const uint8_t* v_codes, uint32_t granule,
-                                            const TokenFactors& f, uint32_t tok0) {
+                                            const TokenFactors& f, int e, uint32_t tok0) {
     const unsigned lane = threadIdx.x & 31u, gid = lane >> 2, tig = lane & 3u;
     const uint32_t row = row_token(gid);
     float s[2][NT][4];
-    float2 fv[2][2];
+    const float ef = static_cast<float>(e), inv = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
 #pragma unroll
     for (int gr = 0; gr < 2; ++gr) {
         scores<NT>(s[gr], k_codes + gr * granule, f.k + 16 * gr, x);
-        fv[gr][0] = f.v[16 * gr + row], fv[gr][1] = f.v[16 * gr + 8 + row];
 #pragma unroll
         for (int g = 0; g < NT; ++g) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                s[gr][g][i] = fmaf(s[gr][g][i], x.factor[g][i & 1], fv[gr][i >> 1].x);
                 if (kEdge && tok0 + 16u * gr + 8u * (i >> 1) + row >= x.limit[g][i & 1]) s[gr][g][i] = -INFINITY;
             }
         }
@@ -205,7 +203,7 @@ __device__ __forceinline__ void attend_unit(float (&o)[NT][8][4], float (&m)[NT]
     for (int g = 0; g < NT; ++g) {
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-            top[g][j] = fmaxf(fmaxf(s[0][g][j], s[0][g][2 + j]), fmaxf(s[1][g][j], s[1][g][2 + j]));
+            top[g][j] = fmaf(fmaxf(fmaxf(s[0][g][j], s[0][g][2 + j]), fmaxf(s[1][g][j], s[1][g][2 + j])), x.factor[g][j], ef);
             over |= top[g][j] > m[g][j] + kSlack;
         }
     }
@@ -228,19 +226,22 @@ __device__ __forceinline__ void attend_unit(float (&o)[NT][8][4], float (&m)[NT]
         }
     }
     const uint32_t t0 = row_token(2u * tig), t1 = t0 ^ 1u;
+    float sum[NT][2];
+#pragma unroll
+    for (int g = 0; g < NT; ++g) sum[g][0] = sum[g][1] = 0.0f;
 #pragma unroll
     for (int gr = 0; gr < 2; ++gr) {
         uint32_t pt[NT][2];
 #pragma unroll
         for (int g = 0; g < NT; ++g) {
-            float e[4];
+            float w[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                e[i] = ex2(s[gr][g][i] - m[g][i & 1]);
-                l[g][i & 1] = fmaf(e[i], fv[gr][i >> 1].y, l[g][i & 1]);
+                w[i] = ex2(fmaf(s[gr][g][i], x.factor[g][i & 1], ef - m[g][i & 1]));
+                sum[g][i & 1] += w[i];
             }
-            pt[g][0] = transpose_8x8(pack_f16x2(e[0], e[1]));
-            pt[g][1] = transpose_8x8(pack_f16x2(e[2], e[3]));
+            pt[g][0] = transpose_8x8(pack_f16x2(w[0], w[1]));
+            pt[g][1] = transpose_8x8(pack_f16x2(w[2], w[3]));
         }
         const uint8_t* codes = v_codes + gr * granule + 8u * gid;
         const uint2 w0 = *reinterpret_cast<const uint2*>(codes + 64u * t0), w1 = *reinterpret_cast<const uint2*>(codes + 64u * t1);
@@ -277,6 +278,8 @@ __device__ __forceinline__ void attend_unit(float (&o)[NT][8][4], float (&m)[NT]
             }
         }
     }
+#pragma unroll
+    for (int g = 0; g < NT; ++g) l[g][0] = fmaf(sum[g][0], inv, l[g][0]), l[g][1] = fmaf(sum[g][1], inv, l[g][1]);
 }
 
 template <int NT, unsigned kStages>
@@ -295,11 +298,11 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : NT == 2 ? 3 : 2) kv4_a
     pdl_wait();
     __syncthreads();
     const Deal deal{8u * NT, row_tiles};
-    const unsigned long long all = sum_steps(p, deal, 0u, sh.part).all;
+    const uint32_t all = sum_steps(p, deal, 0u, sh.part).all;
     const uint32_t n_work = workers(all, gridDim.x);
     if (blockIdx.x >= n_work) return;
-    const unsigned long long begin = run_begin(all, n_work, blockIdx.x);
-    unsigned long long left = run_begin(all, n_work, blockIdx.x + 1u) - begin;
+    const uint32_t begin = run_begin(all, n_work, blockIdx.x);
+    uint32_t left = run_begin(all, n_work, blockIdx.x + 1u) - begin;
     Place at = find_step(p, deal, begin);
     uint32_t phase_bits = 0;   // parity of each stage's next wait
     // in the ring a unit is one record of 32 tokens, or two of 16
@@ -309,7 +312,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : NT == 2 ? 3 : 2) kv4_a
     const uint8_t* nowhere = page == 16u ? kNowhere.p16.bytes : page == 32u ? kNowhere.p32.bytes : page == 64u ? kNowhere.p64.bytes : kNowhere.p128.bytes;
     const uint32_t ring0 = sm100::smem_u32(mine.ring[0]);
 
-    while (left > 0ull) {
+    while (left > 0u) {
         const Segment seg = next_segment(p, deal, at, left);
         const uint32_t b = seg.b, head = seg.head, row0 = seg.row0, first = seg.first, n_tiles = seg.steps;
         const uint32_t length = length_of(p.c, b), n_rows = count_of(p.counts, b, p.S, length);
@@ -389,12 +392,12 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : NT == 2 ? 3 : 2) kv4_a
             }
             phase_bits ^= 1u << st;
             const uint8_t* raw = mine.ring[0] + st * kUnitBytes;
-            token_factors(mine.f, *reinterpret_cast<const uint32_t*>(raw + scales_at), *reinterpret_cast<const uint32_t*>(raw + scales_at + v_scales), tok0 + lane < length);
+            const int e = token_factors(mine.f, *reinterpret_cast<const uint32_t*>(raw + scales_at), *reinterpret_cast<const uint32_t*>(raw + scales_at + v_scales), tok0 + lane < length);
             __syncwarp();
             if (tok0 + kUnit <= low) {
-                attend_unit<NT, false>(o, m, l, x, raw, raw + v_codes, granule, mine.f, tok0);
+                attend_unit<NT, false>(o, m, l, x, raw, raw + v_codes, granule, mine.f, e, tok0);
             } else {
-                attend_unit<NT, true>(o, m, l, x, raw, raw + v_codes, granule, mine.f, tok0);
+                attend_unit<NT, true>(o, m, l, x, raw, raw + v_codes, granule, mine.f, e, tok0);
             }
             __syncwarp();   // the stage and the factors are free again
         }
@@ -482,10 +485,10 @@ __global__ void __launch_bounds__(kThreads) kv4_combine_kernel(const __grid_cons
     const uint32_t steps = steps_of(p, deal, entry);
     uint32_t from = 0, to = 0;   // the CTAs that hold parts, to - from + 1 of them
     if (steps > 0u) {
-        const unsigned long long t0 = sums.below + 1ull * head * steps, t1 = t0 + steps;
+        const uint32_t t0 = sums.below + head * steps, t1 = t0 + steps;
         const uint32_t n_work = workers(sums.all, attend_grid);
         from = worker_at(sums.all, n_work, t0);
-        to = worker_at(sums.all, n_work, t1 - 1ull);
+        to = worker_at(sums.all, n_work, t1 - 1u);
         if (from == to) return;
     }
     const bool sees = row / p.group < count_of(p.counts, b, p.S, length_of(p.c, b));

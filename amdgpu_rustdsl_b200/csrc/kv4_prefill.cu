@@ -2,7 +2,8 @@
 //
 //   S = Q K^T,  P = 2^(c S + e - m),  O += P V',  l += sum P 2^-e,  out = O / l,   c = scale * log2(e), m a running reference per row,
 //
-// e the exponent of a token's largest V factor and V' = V 2^-e: P and V' are f16, K and Q bf16, where a code times its factor is exact.
+// e the exponent of the largest V factor of the step's tokens and V' = V 2^-e: P and V' are f16 (V' is exact down to 2^-34 of the step's largest), K and Q bf16, where a
+// code times its factor is exact.
 //
 // A CTA has 256 query rows of one KV head (rows of the sequence and of the head's group packed, whatever the group's size) as two tiles of 128 and goes over the tokens
 // 128 at a time. Per step four warps turn the step's K and V codes into 16-bit operands in shared memory, once for both tiles; one
@@ -25,12 +26,12 @@ using namespace kv4;
 using namespace sm100;
 
 constexpr uint32_t kTileRows = 128, kItemRows = 256, kStages = 2;
-// Slots of e and 2^-e, by step. The converters write those of step j + 4 behind the scores of step j + 2, which are behind the P of step j + 1 of the tiles that go on
+// Slots of e, by step. The converters write those of step j + 4 behind the scores of step j + 2, which are behind the P of step j + 1 of the tiles that go on
 constexpr uint32_t kFactorSlots = 4;
 constexpr uint32_t kAtomBytes = 128u * 128u, kTileBytes = 2u * kAtomBytes;   // 128 rows x 64 elements with 128-byte swizzle; two of them a tile
 constexpr uint32_t kThreads = 512;
 // Warps 0-3 and 4-7: softmax of tile 0 and 1; 8-11: codes to bf16; 12: products. The pools of setmaxnreg come out of the launch's 128 registers a thread.
-constexpr int kSoftmaxRegs = 176, kConvertRegs = 112, kIssueRegs = 48;
+constexpr int kSoftmaxRegs = 176, kConvertRegs = 104, kIssueRegs = 56;
 static_assert(8 * kSoftmaxRegs + 4 * kConvertRegs + 4 * kIssueRegs <= 16 * 128, "register shares");
 constexpr uint32_t kColS = 0, kColO = 256;   // S (and P in its first half) of tile q at 128 q, O at 256 + 128 q
 constexpr float kSlack = 8.0f;
@@ -40,29 +41,20 @@ enum Bar : uint32_t { kKFull = 0, kKEmpty = 2, kVFull = 4, kVEmpty = 6, kSFull =
 
 struct Shared {
     uint8_t q[2][kTileBytes], k[kStages][kTileBytes], v[kStages][kTileBytes];
-    float e[kFactorSlots][128], inv[kFactorSlots][128];
+    uint4 e[kFactorSlots];   // the largest scale byte of V that each of the converting warps met
     unsigned long long bars[kBars];
     Sums part[kThreads / 32];
     uint32_t tmem, failed, not_drained;
 };
 
-// a = a x + c, b = b x + d in one instruction
-__device__ __forceinline__ void fma2(uint32_t& a, uint32_t& b, float x, float c, float d) {
+// a = a x + c, b = b x + c in one instruction
+__device__ __forceinline__ void fma2(uint32_t& a, uint32_t& b, float x, float c) {
     unsigned long long p, q, r;
     asm("mov.b64 %0, {%1, %2};" : "=l"(p) : "r"(a), "r"(b));
     asm("mov.b64 %0, {%1, %1};" : "=l"(q) : "f"(x));
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(c), "f"(d));
+    asm("mov.b64 %0, {%1, %1};" : "=l"(r) : "f"(c));
     asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(p) : "l"(p), "l"(q), "l"(r));
     asm("mov.b64 {%0, %1}, %2;" : "=r"(a), "=r"(b) : "l"(p));
-}
-// a += x u, b += y w in one instruction
-__device__ __forceinline__ void accumulate2(float& a, float& b, float x, float y, float u, float w) {
-    unsigned long long p, q, r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(p) : "f"(a), "f"(b));
-    asm("mov.b64 %0, {%1, %2};" : "=l"(q) : "f"(x), "f"(y));
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(u), "f"(w));
-    asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(p) : "l"(q), "l"(r));
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(p));
 }
 __device__ __forceinline__ void add2(float& a, float& b, float x, float y) {
     unsigned long long p, q;
@@ -129,16 +121,16 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
     tc_fence_before_sync();
     __syncthreads();
     tc_fence_after_sync();
-    const uint32_t tmem = sh.tmem;
+    const uint32_t tmem = __shfl_sync(0xFFFFFFFFu, sh.tmem, 0);
     pdl_launch();
     pdl_wait();
     const Deal deal{kItemRows, row_tiles};
-    const unsigned long long all = sum_steps(p, deal, 0u, sh.part).all;
+    const uint32_t all = sum_steps(p, deal, 0u, sh.part).all;
     const uint32_t n_work = workers(all, gridDim.x);
     volatile uint32_t* failed = &sh.failed;
     if (blockIdx.x < n_work) {
-        const unsigned long long begin = run_begin(all, n_work, blockIdx.x);
-        unsigned long long left = run_begin(all, n_work, blockIdx.x + 1u) - begin;
+        const uint32_t begin = run_begin(all, n_work, blockIdx.x);
+        uint32_t left = run_begin(all, n_work, blockIdx.x + 1u) - begin;
         Place at = find_step(p, deal, begin);
         if (warp < 8u) {
             asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
@@ -147,7 +139,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
             const float c = p.scale_log2;
             uint32_t s_phase = 0, o_phase = 0, step0 = 0;   // step0: steps in front of the segment
             bool ok = true;
-            while (left > 0ull && ok) {
+            while (left > 0u && ok) {
                 const Segment seg = next_segment(p, deal, at, left);
                 const uint32_t length = length_of(p.c, seg.b), n = count_of(p.counts, seg.b, p.S, length);
                 const uint32_t steps = tile_steps(p, seg, q, length, n), row = seg.row0 + q * kTileRows + r, i = row / p.group;
@@ -166,22 +158,14 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
                         break;
                     }
                     tc_fence_after_sync();
-                    const float4* e4 = reinterpret_cast<const float4*>(sh.e[(step0 + j) % kFactorSlots]);
-                    const float4* inv4 = reinterpret_cast<const float4*>(sh.inv[(step0 + j) % kFactorSlots]);
+                    const uint4 most4 = sh.e[(step0 + j) % kFactorSlots];
+                    const int e = group_exponent(max(max(most4.x, most4.y), max(most4.z, most4.w)));
                     uint32_t s[4][32];
 #pragma unroll
                     for (int k = 0; k < 4; ++k) tmem_ld32(t_s + 32u * k, s[k]);
                     tmem_wait_ld();
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        reg_fence32(s[k]);
-#pragma unroll
-                        for (int x = 0; x < 32; x += 4) {
-                            const float4 e = e4[8 * k + x / 4];
-                            fma2(s[k][x], s[k][x + 1], c, e.x, e.y);
-                            fma2(s[k][x + 2], s[k][x + 3], c, e.z, e.w);
-                        }
-                    }
+                    for (int k = 0; k < 4; ++k) reg_fence32(s[k]);
                     const uint32_t tok0 = (seg.first + j) * kStepTokens;
                     if (__any_sync(0xFFFFFFFFu, tok0 + kStepTokens > limit)) {
 #pragma unroll
@@ -199,7 +183,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
 #pragma unroll
                         for (int x = 2; x < 32; x += 2) top[k] = fmaxf(top[k], fmaxf(__uint_as_float(s[k][x]), __uint_as_float(s[k][x + 1])));
                     }
-                    const float most = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+                    const float most = fmaf(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])), c, static_cast<float>(e));
                     const bool over = most > m + kSlack;
                     if (__any_sync(0xFFFFFFFFu, over)) {
                         const float next = over ? most : m, f = ex2(m - next);
@@ -207,37 +191,34 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
                         l *= f;
                         if (j > 0u) {   // the product before this one is done: S came behind it
 #pragma unroll
-                            for (int k = 0; k < 4; ++k) {
-                                uint32_t o[32];
-                                tmem_ld32(t_o + 32u * k, o);
+                            for (int k = 0; k < 8; ++k) {
+                                uint32_t o[16];
+                                tmem_ld16(t_o + 16u * k, o);
                                 tmem_wait_ld();
-                                reg_fence32(o);
+                                reg_fence16(o);
 #pragma unroll
-                                for (int x = 0; x < 32; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * f);
-                                tmem_st32(t_o + 32u * k, o);
+                                for (int x = 0; x < 16; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * f);
+                                tmem_st16(t_o + 16u * k, o);
                             }
                             tmem_wait_st();
                         }
                     }
+                    const float shift = static_cast<float>(e) - m;
                     float l0 = 0.0f, l1 = 0.0f;
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
                         uint32_t pw[16];
 #pragma unroll
-                        for (int x = 0; x < 8; ++x) {
-                            const float4 inv = inv4[8 * k + x];
-#pragma unroll
-                            for (int y = 0; y < 2; ++y) {
-                                float a = __uint_as_float(s[k][4 * x + 2 * y]), b = __uint_as_float(s[k][4 * x + 2 * y + 1]);
-                                add2(a, b, -m, -m);
-                                a = ex2(a), b = ex2(b);
-                                accumulate2(l0, l1, a, b, y ? inv.z : inv.x, y ? inv.w : inv.y);
-                                pw[2 * x + y] = pack_f16x2(a, b);
-                            }
+                        for (int x = 0; x < 16; ++x) {
+                            uint32_t a = s[k][2 * x], b = s[k][2 * x + 1];
+                            fma2(a, b, c, shift);
+                            const float ea = ex2(__uint_as_float(a)), eb = ex2(__uint_as_float(b));
+                            add2(l0, l1, ea, eb);
+                            pw[x] = pack_f16x2(ea, eb);
                         }
                         tmem_st16(t_s + 16u * k, pw);
                     }
-                    l += l0 + l1;
+                    l = fmaf(l0 + l1, __uint_as_float(static_cast<uint32_t>(127 - e) << 23), l);
                     tmem_wait_st();
                     tc_fence_before_sync();
                     __syncwarp();
@@ -301,7 +282,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
             const uint32_t r = threadIdx.x & 127u, page = 1u << p.c.page_log2;
             uint32_t step = 0, q_count = 0;   // steps and segments so far
             bool ok = true;
-            while (left > 0ull && ok) {
+            while (left > 0u && ok) {
                 const Segment seg = next_segment(p, deal, at, left);
                 const uint32_t length = length_of(p.c, seg.b), n = count_of(p.counts, seg.b, p.S, length);
                 uint4 k[4], v[4];
@@ -349,7 +330,12 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
                     // A token behind the length must not bring NaN into P V; one that is lost, or whose V is NaN, makes the rows that see it NaN by its scores
                     float fk[4];
                     uint32_t fv[4];
-                    const ValueFactors f = value_factors(empty || lost ? 0x7F7F7F7Fu : vs);
+                    const uint32_t largest = empty || lost ? 0u : largest_byte(vs), met = __reduce_max_sync(0xFFFFFFFFu, largest == 255u ? 0u : largest);
+                    if (lane == 0u) reinterpret_cast<uint32_t*>(&sh.e[step % kFactorSlots])[warp & 3u] = met;
+                    named_bar_sync(1u, 128u);
+                    const uint4 most4 = sh.e[step % kFactorSlots];
+                    const ValueFactors f = value_factors(vs, largest, group_exponent(max(max(most4.x, most4.y), max(most4.z, most4.w))));
+                    const bool broken = largest == 255u;
 #pragma unroll
                     for (int x = 0; x < 4; ++x) fk[x] = scale_f32(ks, x);
                     fv[0] = __byte_perm(f.r01, 0u, 0x1010), fv[1] = __byte_perm(f.r01, 0u, 0x3232), fv[2] = __byte_perm(f.r23, 0u, 0x1010), fv[3] = __byte_perm(f.r23, 0u, 0x3232);
@@ -357,7 +343,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
 #pragma unroll
                         for (int x = 0; x < 4; ++x) k[x] = v[x] = make_uint4(0u, 0u, 0u, 0u);
                     }
-                    if (empty || lost || f.broken) {
+                    if (empty || lost || broken) {
 #pragma unroll
                         for (int x = 0; x < 4; ++x) fk[x] = empty ? 0.0f : __uint_as_float(0x7FC00000u), fv[x] = 0u;
                     }
@@ -365,8 +351,6 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
                         ok = false;
                         break;
                     }
-                    sh.e[step % kFactorSlots][r] = f.e, sh.inv[step % kFactorSlots][r] = f.inv;
-                    __syncwarp();
                     if (lane == 0u) mbar_arrive(bar(kEFull + step % kFactorSlots));
                     store_row(sh.k[st], r, k, fk);
                     fence_proxy_async_smem();
@@ -418,10 +402,12 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
                     if (ok && !mbar_wait(b, parity, failed)) ok = false;
                     return ok;
                 };
-                while (left > 0ull && ok) {
+                while (left > 0u && ok) {
                     const Segment seg = next_segment(p, deal, at, left);
                     const uint32_t length = length_of(p.c, seg.b), n = count_of(p.counts, seg.b, p.S, length);
-                    const uint32_t steps[2] = {tile_steps(p, seg, 0u, length, n), tile_steps(p, seg, 1u, length, n)};
+                    // (the same in all lanes; said so, it lets the compiler keep what the products take in uniform registers)
+                    const uint32_t steps[2] = {__shfl_sync(0xFFFFFFFFu, tile_steps(p, seg, 0u, length, n), 0), __shfl_sync(0xFFFFFFFFu, tile_steps(p, seg, 1u, length, n), 0)};
+                    const uint32_t seg_steps = __shfl_sync(0xFFFFFFFFu, seg.steps, 0);
                     if (!wait(bar(kQFull), q_count & 1u)) break;
                     ++q_count;
                     if (!wait(bar(kKFull + step % kStages), step / kStages & 1u)) break;
@@ -429,10 +415,10 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
                     if (steps[0] > 0u) scores(0u, step % kStages);
                     if (steps[1] > 0u) scores(1u, step % kStages);
                     commit(bar(kKEmpty + step % kStages));
-                    if (seg.steps == 1u) commit(bar(kQEmpty));
-                    for (uint32_t j = 0; j < seg.steps; ++j, ++step) {
+                    if (seg_steps == 1u) commit(bar(kQEmpty));
+                    for (uint32_t j = 0; j < seg_steps; ++j, ++step) {
                         const uint32_t st = step % kStages, next = (step + 1u) % kStages;
-                        const bool more = j + 1u < seg.steps;
+                        const bool more = j + 1u < seg_steps;
                         if (!wait(bar(kVFull + st), step / kStages & 1u)) break;
                         if (more && !wait(bar(kKFull + next), (step + 1u) / kStages & 1u)) break;
 #pragma unroll
@@ -449,7 +435,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
                         }
                         if (!ok) break;
                         if (more) commit(bar(kKEmpty + next));
-                        if (j + 2u == seg.steps) commit(bar(kQEmpty));
+                        if (j + 2u == seg_steps) commit(bar(kQEmpty));
                     }
                 }
                 if (!ok) {   // whatever was issued has to be over before the tensor memory goes back

@@ -22,11 +22,11 @@ __device__ __forceinline__ uint32_t steps_of(const Kv4AttendParams& p, const Dea
 }
 
 struct Sums {
-    unsigned long long below, all;
+    uint32_t below, all;
 };
-// Steps of the entries below `upto`, and of all, times the heads. All threads of the CTA; `part` has an element per warp.
+// Steps of the entries below `upto`, and of all, times the heads (the host has checked that they stay below 2^32). All threads of the CTA; `part` has an element per warp.
 __device__ __forceinline__ Sums sum_steps(const Kv4AttendParams& p, const Deal& d, uint32_t upto, Sums* part) {
-    unsigned long long below = 0, all = 0;
+    uint32_t below = 0, all = 0;
     for (uint32_t e = threadIdx.x; e < p.c.B * d.row_tiles; e += blockDim.x) {
         const uint32_t t = steps_of(p, d, e);
         all += t;
@@ -46,25 +46,25 @@ __device__ __forceinline__ Sums sum_steps(const Kv4AttendParams& p, const Deal& 
 }
 
 // CTA w of n has the steps [run_begin(w), run_begin(w + 1)) of `all`; worker_at is the one that has a step
-__device__ __forceinline__ uint32_t workers(unsigned long long all, uint32_t grid) { return static_cast<uint32_t>(all < grid ? all : grid); }
-__device__ __forceinline__ unsigned long long run_begin(unsigned long long all, uint32_t n, uint32_t w) { return all * w / n; }
-__device__ __forceinline__ uint32_t worker_at(unsigned long long all, uint32_t n, unsigned long long step) { return static_cast<uint32_t>(((step + 1ull) * n - 1ull) / all); }
+__device__ __forceinline__ uint32_t workers(uint32_t all, uint32_t grid) { return min(all, grid); }
+__device__ __forceinline__ uint32_t run_begin(uint32_t all, uint32_t n, uint32_t w) { return static_cast<uint32_t>(1ull * all * w / n); }
+__device__ __forceinline__ uint32_t worker_at(uint32_t all, uint32_t n, uint32_t step) { return static_cast<uint32_t>(((step + 1ull) * n - 1ull) / all); }
 
 // The entry that step `pos` belongs to and the step's number within it, for all lanes of a warp
 struct Place {
     uint32_t entry;
-    unsigned long long in;   // step within the entry's items
+    uint32_t in;   // step within the entry's items
 };
-__device__ __forceinline__ Place find_step(const Kv4AttendParams& p, const Deal& d, unsigned long long pos) {
+__device__ __forceinline__ Place find_step(const Kv4AttendParams& p, const Deal& d, uint32_t pos) {
     const unsigned lane = threadIdx.x & 31u;
     const uint32_t entries = p.c.B * d.row_tiles;
-    unsigned long long before = 0;
+    uint32_t before = 0;
     for (uint32_t e0 = 0; e0 < entries; e0 += 32u) {
-        const unsigned long long t = e0 + lane < entries ? 1ull * steps_of(p, d, e0 + lane) * p.c.HK : 0ull;
-        unsigned long long s = t;
+        const uint32_t t = e0 + lane < entries ? steps_of(p, d, e0 + lane) * p.c.HK : 0u;
+        uint32_t s = t;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const unsigned long long a = __shfl_up_sync(0xFFFFFFFFu, s, o);
+            const uint32_t a = __shfl_up_sync(0xFFFFFFFFu, s, o);
             if (lane >= static_cast<unsigned>(o)) s += a;
         }
         const unsigned hit = __ballot_sync(0xFFFFFFFFu, before + s > pos);
@@ -74,7 +74,7 @@ __device__ __forceinline__ Place find_step(const Kv4AttendParams& p, const Deal&
         }
         before += __shfl_sync(0xFFFFFFFFu, s, 31);
     }
-    return {entries, 0ull};
+    return {entries, 0u};
 }
 
 // A run of steps of one item
@@ -83,16 +83,16 @@ struct Segment {
     uint32_t first, steps, of;      // steps first .. first + steps - 1 of `of`
 };
 // The segment at the head of a CTA's run of `left` steps; moves on behind it
-__device__ __forceinline__ Segment next_segment(const Kv4AttendParams& p, const Deal& d, Place& at, unsigned long long& left) {
+__device__ __forceinline__ Segment next_segment(const Kv4AttendParams& p, const Deal& d, Place& at, uint32_t& left) {
     uint32_t of = steps_of(p, d, at.entry);
-    while (at.in >= 1ull * of * p.c.HK) {   // also where an entry has none
-        at.in -= 1ull * of * p.c.HK;
+    while (at.in >= of * p.c.HK) {   // also where an entry has none
+        at.in -= of * p.c.HK;
         of = steps_of(p, d, ++at.entry);
     }
     Segment s;
     s.b = at.entry / d.row_tiles, s.row0 = (at.entry - s.b * d.row_tiles) * d.rows;
-    s.head = static_cast<uint32_t>(at.in / of), s.first = static_cast<uint32_t>(at.in - 1ull * s.head * of), s.of = of;
-    s.steps = static_cast<uint32_t>(min(static_cast<unsigned long long>(of - s.first), left));
+    s.head = at.in / of, s.first = at.in - s.head * of, s.of = of;
+    s.steps = min(of - s.first, left);
     at.in += s.steps;
     left -= s.steps;
     return s;

@@ -179,6 +179,13 @@ constexpr float kDown = 1.0f / (1 << kUp);
 // the largest of a token's four scale bytes
 __device__ __forceinline__ uint32_t largest_byte(uint32_t word) { return max(max(word & 0xFFu, (word >> 8) & 0xFFu), max((word >> 16) & 0xFFu, word >> 24)); }
 __device__ __forceinline__ int group_exponent(uint32_t largest) { return min(max(static_cast<int>(largest) - 127, kLowE), kHighE); }
+// A query row in f16: the factor that brings its largest element (f32 bits of its size) to the exponent 14, and what undoes it. Rows of zeros or with Inf or NaN keep 1.
+__device__ __forceinline__ float2 row_factors(uint32_t largest) {
+    int field = static_cast<int>(largest >> 23);
+    if (field == 255 || largest == 0u) field = 141;
+    if (field < 15) field = 15;   // both stay normal
+    return make_float2(__uint_as_float(static_cast<uint32_t>(268 - field) << 23), __uint_as_float(static_cast<uint32_t>(field - 14) << 23));
+}
 struct ValueFactors {
     uint32_t r01, r23;   // 2^(E - 127 - e + kUp) of the blocks, f16 (E <= 252 leaves them below its largest); NaN for 255
 };

@@ -32,6 +32,7 @@ static_assert(kTile == kStepTokens, "a step is a tile");
 constexpr unsigned kUnitBytes = kUnit * FMHA_KV4_TOKEN_BYTES;
 constexpr unsigned kCtasPerSm = 4;
 constexpr float kSlack = 4.0f;
+constexpr float kLeast = 1e-37f;                  // of a row's factor: times a masked score it is still -inf
 constexpr float kLn2 = 0.69314718055994531f, kLog2e = 1.44269504088896341f;
 
 // What a unit's 32 lanes work out for its tokens, one lane a token
@@ -81,23 +82,18 @@ __device__ __forceinline__ void load_rows(QueryRows<NT>& x, const Kv4AttendParam
         }
         amax = max(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, 1));
         amax = max(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, 2));
-        // the largest element gets the exponent 14; rows of zeros, subnormals, Inf or NaN keep a factor of 1 or the largest there is
-        int field = static_cast<int>(amax >> 23);
-        if (field == 255 || amax == 0u) field = 141;
-        if (field < 15) field = 15;   // 2^(141 - field) stays normal
-        const float down = __uint_as_float(static_cast<uint32_t>(268 - field) << 23);   // 2^(14 - (field - 127))
-        const float back = __uint_as_float(static_cast<uint32_t>(field - 14) << 23);
+        const float2 f = row_factors(amax);
 #pragma unroll
         for (int blk = 0; blk < 4; ++blk) {
             const uint32_t w[4] = {raw[blk].x, raw[blk].y, raw[blk].z, raw[blk].w};
 #pragma unroll
-            for (int k = 0; k < 4; ++k) x.q[g][blk][k] = pack_f16x2(__uint_as_float(w[k] << 16) * down, __uint_as_float(w[k] & 0xFFFF0000u) * down);
+            for (int k = 0; k < 4; ++k) x.q[g][blk][k] = pack_f16x2(__uint_as_float(w[k] << 16) * f.x, __uint_as_float(w[k] & 0xFFFF0000u) * f.x);
         }
         const uint32_t lim = !live ? 0u : p.causal ? length - n + i + 1u : length;
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
             const int src = static_cast<int>(2u * tig + j) * 4;   // a lane that holds that row
-            x.factor[g][j] = __shfl_sync(0xFFFFFFFFu, back, src) * p.scale_log2;
+            x.factor[g][j] = fmaxf(__shfl_sync(0xFFFFFFFFu, f.y, src) * p.scale_log2, kLeast);
             x.limit[g][j] = __shfl_sync(0xFFFFFFFFu, lim, src);
         }
     }
@@ -300,9 +296,12 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : NT == 2 ? 3 : 2) kv4_a
     const Deal deal{8u * NT, row_tiles};
     const uint32_t all = sum_steps(p, deal, 0u, sh.part).all;
     const uint32_t n_work = workers(all, gridDim.x);
+    clear_empty_entries(p, deal);
+    if (threadIdx.x == 0u) begun_by(p.ws, blockIdx.x)->last = blockIdx.x;
     if (blockIdx.x >= n_work) return;
     const uint32_t begin = run_begin(all, n_work, blockIdx.x);
-    uint32_t left = run_begin(all, n_work, blockIdx.x + 1u) - begin;
+    const uint32_t end = run_begin(all, n_work, blockIdx.x + 1u);
+    uint32_t left = end - begin;
     Place at = find_step(p, deal, begin);
     uint32_t phase_bits = 0;   // parity of each stage's next wait
     // in the ring a unit is one record of 32 tokens, or two of 16
@@ -313,7 +312,9 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : NT == 2 ? 3 : 2) kv4_a
     const uint32_t ring0 = sm100::smem_u32(mine.ring[0]);
 
     while (left > 0u) {
+        const uint32_t pos = end - left;
         const Segment seg = next_segment(p, deal, at, left);
+        if (threadIdx.x == 0u && seg.first == 0u && seg.steps < seg.of) *begun_by(p.ws, blockIdx.x) = {seg.b, seg.head, seg.row0, worker_at(all, n_work, pos + seg.of - 1u)};
         const uint32_t b = seg.b, head = seg.head, row0 = seg.row0, first = seg.first, n_tiles = seg.steps;
         const uint32_t length = length_of(p.c, b), n_rows = count_of(p.counts, b, p.S, length);
         QueryRows<NT> x;
@@ -420,7 +421,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : NT == 2 ? 3 : 2) kv4_a
         if (sh.failed != 0u) return;   // (the same for all: it was raised in front of the barrier)
         const bool whole = n_tiles == seg.of;
         const uint32_t slot = first == 0u ? 1u : 0u;
-        float* part = slot_of(p.ws, blockIdx.x, slot, 8u * NT);
+        float* part = slot_of(p.ws, gridDim.x, blockIdx.x, slot, 8u * NT);
 #pragma unroll
         for (int g = 0; g < NT; ++g) {
             float* mine_o = reinterpret_cast<float*>(mine.ring[0]);   // [8 rows][128], the ring is empty
@@ -472,61 +473,66 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : NT == 2 ? 3 : 2) kv4_a
     }
 }
 
-// One CTA a query row: rows that see nothing, and items that more than one CTA worked on
-__global__ void __launch_bounds__(kThreads) kv4_combine_kernel(const __grid_constant__ Kv4AttendParams p, Deal deal, uint32_t attend_grid) {
-    __shared__ Sums part[kWarps];
+// Puts the items together that more than one CTA of a launch worked on; blockIdx.x is the CTA that began one. kFewRows: a CTA has one row, its warps the parts in turn; else a warp has
+// a row and all of its parts. Four parts are in flight at a time.
+template <bool kFewRows>
+__global__ void __launch_bounds__(kThreads) kv4_combine_kernel(const __grid_constant__ Kv4AttendParams p, uint32_t rows) {
     __shared__ float sm_m[kWarps], sm_l[kWarps];
     __shared__ float4 sm_o[kWarps][32];
     pdl_launch();
     pdl_wait();
-    const uint32_t rows = p.S * p.group, row = blockIdx.x % rows, bh = blockIdx.x / rows, head = bh % p.c.HK, b = bh / p.c.HK;
-    const uint32_t entry = b * deal.row_tiles + row / deal.rows;
-    const Sums sums = sum_steps(p, deal, entry, part);
-    const uint32_t steps = steps_of(p, deal, entry);
-    uint32_t from = 0, to = 0;   // the CTAs that hold parts, to - from + 1 of them
-    if (steps > 0u) {
-        const uint32_t t0 = sums.below + head * steps, t1 = t0 + steps;
-        const uint32_t n_work = workers(sums.all, attend_grid);
-        from = worker_at(sums.all, n_work, t0);
-        to = worker_at(sums.all, n_work, t1 - 1u);
-        if (from == to) return;
-    }
-    const bool sees = row / p.group < count_of(p.counts, b, p.S, length_of(p.c, b));
     const unsigned lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
+    const uint32_t r = kFewRows ? blockIdx.y : blockIdx.y * kWarps + warp;
+    const uint4 begun = ld_v4(begun_by(p.ws, blockIdx.x));
+    const uint32_t b = begun.x, head = begun.y, row = begun.z + r, last = begun.w;
+    if (last == blockIdx.x || row >= p.S * p.group) return;   // (the same in all warps where they meet below)
+    const uint32_t i = row / p.group, h = head * p.group + row % p.group;
+    const bool sees = i < count_of(p.counts, b, p.S, length_of(p.c, b));
+    constexpr uint32_t kStride = kFewRows ? kWarps : 1u;
     float m = kLowest, l = 0.0f;
     float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    if (steps > 0u && sees) {
-        const uint32_t r = row % deal.rows;
-        for (uint32_t w = from + warp; w <= to; w += kWarps) {
-            const float* src = slot_of(p.ws, w, w == from ? 1u : 0u, deal.rows);
-            const float pm = ld_f32(src + deal.rows * 128u + 2u * r), pl = ld_f32(src + deal.rows * 128u + 2u * r + 1u);
-            const uint4 raw = ld_v4(src + r * 128u + 4u * lane);
-            const float top = fmaxf(m, pm), a = ex2(m - top), c = ex2(pm - top);
+    for (uint32_t w0 = blockIdx.x + (kFewRows ? warp : 0u); sees && w0 <= last; w0 += 4u * kStride) {
+        float pm[4], pl[4];
+        uint4 raw[4];
+#pragma unroll
+        for (uint32_t k = 0; k < 4u; ++k) {
+            const uint32_t w = w0 + k * kStride;
+            pm[k] = kLowest, pl[k] = 0.0f, raw[k] = make_uint4(0u, 0u, 0u, 0u);
+            if (w <= last) {
+                const float* src = slot_of(p.ws, gridDim.x, w, w == blockIdx.x ? 1u : 0u, rows);
+                pm[k] = ld_f32(src + rows * 128u + 2u * r), pl[k] = ld_f32(src + rows * 128u + 2u * r + 1u);
+                raw[k] = ld_v4(src + r * 128u + 4u * lane);
+            }
+        }
+#pragma unroll
+        for (uint32_t k = 0; k < 4u; ++k) {
+            const float top = fmaxf(m, pm[k]), a = ex2(m - top), c = ex2(pm[k] - top);
             m = top;
-            l = fmaf(l, a, pl * c);
-            o.x = fmaf(o.x, a, __uint_as_float(raw.x) * c), o.y = fmaf(o.y, a, __uint_as_float(raw.y) * c);
-            o.z = fmaf(o.z, a, __uint_as_float(raw.z) * c), o.w = fmaf(o.w, a, __uint_as_float(raw.w) * c);
+            l = fmaf(l, a, pl[k] * c);
+            o.x = fmaf(o.x, a, __uint_as_float(raw[k].x) * c), o.y = fmaf(o.y, a, __uint_as_float(raw[k].y) * c);
+            o.z = fmaf(o.z, a, __uint_as_float(raw[k].z) * c), o.w = fmaf(o.w, a, __uint_as_float(raw[k].w) * c);
         }
     }
-    if (lane == 0u) sm_m[warp] = m, sm_l[warp] = l;
-    sm_o[warp][lane] = o;
-    __syncthreads();
-    if (warp != 0u) return;
-    const float top = fmaxf(fmaxf(sm_m[0], sm_m[1]), fmaxf(sm_m[2], sm_m[3]));
-    l = 0.0f;
-    o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (kFewRows) {
+        if (lane == 0u) sm_m[warp] = m, sm_l[warp] = l;
+        sm_o[warp][lane] = o;
+        __syncthreads();
+        if (warp != 0u) return;
+        m = fmaxf(fmaxf(sm_m[0], sm_m[1]), fmaxf(sm_m[2], sm_m[3]));
+        l = 0.0f;
+        o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-    for (unsigned w = 0; w < kWarps; ++w) {
-        const float f = ex2(sm_m[w] - top);
-        const float4 c = sm_o[w][lane];
-        l = fmaf(sm_l[w], f, l);
-        o.x = fmaf(c.x, f, o.x), o.y = fmaf(c.y, f, o.y), o.z = fmaf(c.z, f, o.z), o.w = fmaf(c.w, f, o.w);
+        for (unsigned w = 0; w < kWarps; ++w) {
+            const float f = ex2(sm_m[w] - m);
+            const float4 c = sm_o[w][lane];
+            l = fmaf(sm_l[w], f, l);
+            o.x = fmaf(c.x, f, o.x), o.y = fmaf(c.y, f, o.y), o.z = fmaf(c.z, f, o.z), o.w = fmaf(c.w, f, o.w);
+        }
     }
     const bool none = l == 0.0f;
     const float inv = none ? 0.0f : 1.0f / l;
-    const uint32_t i = row / p.group, h = head * p.group + row % p.group;
     *reinterpret_cast<uint2*>(p.out + ((static_cast<size_t>(b) * p.S + i) * p.H + h) * 128u + 4u * lane) = make_uint2(pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv));
-    if (p.lse != nullptr && lane == 0u) p.lse[(static_cast<size_t>(b) * p.H + h) * p.S + i] = none ? -INFINITY : (top + lg2(l)) * kLn2;
+    if (p.lse != nullptr && lane == 0u) p.lse[(static_cast<size_t>(b) * p.H + h) * p.S + i] = none ? -INFINITY : (m + lg2(l)) * kLn2;
 }
 
 // The attention weights that the cached tokens received: p = 2^(s - lse), summed over the rows and the group's heads. A warp has 32 tokens and goes over all rows, in
@@ -626,7 +632,7 @@ cudaError_t launch_rows(const Kv4AttendParams& p, uint32_t row_tiles, cudaStream
     }
     e = kv4_launch(kv4_attend_kernel<NT, kStages1>, dim3(grid), kThreads, smem, stream, p, row_tiles);
     if (e != cudaSuccess) return e;
-    return kv4_launch(kv4_combine_kernel, dim3(p.c.B * p.c.HK * p.S * p.group), kThreads, 0, stream, p, Deal{8u * NT, row_tiles}, grid);
+    return kv4_launch(kv4_combine_kernel<true>, dim3(grid, p.S * p.group < 8u * NT ? p.S * p.group : 8u * NT), kThreads, 0, stream, p, 8u * NT);
 }
 
 uint64_t partial_bytes(const Kv4View& c, uint32_t rows) {
@@ -638,7 +644,8 @@ cudaError_t launch_many(const Kv4AttendParams& p, cudaStream_t stream) {
     const uint32_t rows = p.S * p.group, row_tiles = (rows + kv4_prefill_rows() - 1u) / kv4_prefill_rows();
     const cudaError_t e = launch_kv4_prefill(p, row_tiles, stream);
     if (e != cudaSuccess) return e;
-    return kv4_launch(kv4_combine_kernel, dim3(p.c.B * p.c.HK * rows), kThreads, 0, stream, p, Deal{kv4_prefill_rows(), row_tiles}, kv4_prefill_grid());
+    const uint32_t most = rows < kv4_prefill_rows() ? rows : kv4_prefill_rows();
+    return kv4_launch(kv4_combine_kernel<false>, dim3(kv4_prefill_grid(), (most + kWarps - 1u) / kWarps), kThreads, 0, stream, p, kv4_prefill_rows());
 }
 
 }  // namespace

@@ -1,15 +1,15 @@
 // Attention of many query rows over the 4-bit cache: prompts and chunks of them, on the tcgen05 tensor cores.
 //
-//   S = Q K^T,  P = 2^(c S + e - m),  O += P V',  l += sum P 2^-e,  out = O / l,   c = scale * log2(e), m a running reference per row,
+//   S = Q K'^T,  P = 2^(c S + e - m),  O += P V',  l += sum P 2^-e,  out = O / l,   c = scale * log2(e) * what was taken out of Q and K, m a running reference per row
 //
-// e the exponent of the largest V factor of the step's tokens and V' = V 2^-e: P and V' are f16 (V' is exact down to 2^-34 of the step's largest), K and Q bf16, where a
-// code times its factor is exact.
+// All operands are f16: Q with a power of two per row taken out, K' and V' relative to the largest factor of the step's 128 tokens, all exact down to 2^-30 of the row's
+// or the step's largest.
 //
 // A CTA has 256 query rows of one KV head (rows of the sequence and of the head's group packed, whatever the group's size) as two tiles of 128 and goes over the tokens
-// 128 at a time. Per step four warps turn the step's K and V codes into 16-bit operands in shared memory, once for both tiles; one
-// thread issues the products, S from shared memory, P V with P from tensor memory; and two groups of four warps do the softmax, one tile each, a thread a row, so that
-// the tensor cores work on one tile while the other's softmax runs. P overwrites S in tensor memory. m moves only when a row's maximum exceeds it by 2^8, so O is
-// hardly ever rescaled.
+// 128 at a time. Per step four warps turn the step's K and V codes into f16 in shared memory, once for both tiles; one thread issues the products, S from shared
+// memory, P V with P from tensor memory; and two groups of four warps do the softmax, one tile each, a thread a row, so that the tensor cores work on one tile while the
+// other's softmax runs. P overwrites S in tensor memory and goes over in two halves of 64 tokens, the first while the second is still being computed. m moves only
+// when a row's maximum exceeds it by 2^8, so O is hardly ever rescaled.
 //
 // Steps are dealt out to one CTA per SM as kv4_schedule.cuh says; items that several CTAs worked on go through f32 partials and the combine kernel.
 #include "kv4.cuh"
@@ -17,6 +17,7 @@
 #include "ptx_sm100.cuh"
 
 #include <atomic>
+#include <cstddef>
 
 namespace b200mx {
 
@@ -25,23 +26,26 @@ namespace {
 using namespace kv4;
 using namespace sm100;
 
-constexpr uint32_t kTileRows = 128, kItemRows = 256, kStages = 2;
-// Slots of e, by step. The converters write those of step j + 4 behind the scores of step j + 2, which are behind the P of step j + 1 of the tiles that go on
+constexpr uint32_t kTileRows = 128, kItemRows = 256, kStages = 2, kHalf = 64;
+// Slots of the steps' exponents. The converters write those of step j + 4 behind the scores of step j + 2, which are behind the P of step j + 1 of the tiles that go on
 constexpr uint32_t kFactorSlots = 4;
 constexpr uint32_t kAtomBytes = 128u * 128u, kTileBytes = 2u * kAtomBytes;   // 128 rows x 64 elements with 128-byte swizzle; two of them a tile
 constexpr uint32_t kThreads = 512;
-// Warps 0-3 and 4-7: softmax of tile 0 and 1; 8-11: codes to bf16; 12: products. The pools of setmaxnreg come out of the launch's 128 registers a thread.
+// Warps 0-3 and 4-7: softmax of tile 0 and 1; 8-11: codes to f16; 12 and 13: products of tile 0 and 1. The pools of setmaxnreg come out of the launch's 128 registers a thread.
 constexpr int kSoftmaxRegs = 176, kConvertRegs = 104, kIssueRegs = 56;
 static_assert(8 * kSoftmaxRegs + 4 * kConvertRegs + 4 * kIssueRegs <= 16 * 128, "register shares");
-constexpr uint32_t kColS = 0, kColO = 256;   // S (and P in its first half) of tile q at 128 q, O at 256 + 128 q
+constexpr uint32_t kColS = 0, kColO = 256;   // S of tile q (P in its first half) at 128 q, O at 256 + 128 q
 constexpr float kSlack = 8.0f;
+constexpr float kLeast = 1e-37f;   // times a masked score it is still -inf
 constexpr float kLn2 = 0.69314718055994531f;
 
-enum Bar : uint32_t { kKFull = 0, kKEmpty = 2, kVFull = 4, kVEmpty = 6, kSFull = 8, kPFull = 10, kODone = 12, kOFree = 14, kQFull = 16, kQEmpty = 17, kDrained = 18, kEFull = 19, kBars = 19 + kFactorSlots };
+// barriers; kPFull by 2 q + half
+enum Bar : uint32_t { kKFull = 0, kKEmpty = 2, kVFull = 4, kVEmpty = 6, kSFull = 8, kODone = 10, kPFull = 12, kOFree = 16, kQFull = 18, kQEmpty = 20, kDrained = 21, kEFull = 23, kBars = 23 + kFactorSlots };
 
 struct Shared {
     uint8_t q[2][kTileBytes], k[kStages][kTileBytes], v[kStages][kTileBytes];
-    uint4 e[kFactorSlots];   // the largest scale byte of V that each of the converting warps met
+    uint4 most[kFactorSlots][2];   // the largest scale byte of K and of V that each of the converting warps met
+    float q_factor[2][kItemRows];  // the powers of two that were taken out of the rows, of even and of odd segments
     unsigned long long bars[kBars];
     Sums part[kThreads / 32];
     uint32_t tmem, failed, not_drained;
@@ -73,28 +77,20 @@ __device__ __forceinline__ uint32_t tile_steps(const Kv4AttendParams& p, const S
     return of <= s.first ? 0u : min(s.steps, of - s.first);
 }
 
-// 8 elements of a block, two bytes of codes in `half` (0, 1) of each word, times the block's factor, as bf16
-__device__ __forceinline__ uint4 to_bf16(uint32_t lo, uint32_t hi, bool half, float f) {
-    const float2 a = f16x2_to_f32(half ? e2m1x2_to_f16x2<2>(lo) : e2m1x2_to_f16x2<0>(lo)), b = f16x2_to_f32(half ? e2m1x2_to_f16x2<3>(lo) : e2m1x2_to_f16x2<1>(lo));
-    const float2 c = f16x2_to_f32(half ? e2m1x2_to_f16x2<2>(hi) : e2m1x2_to_f16x2<0>(hi)), d = f16x2_to_f32(half ? e2m1x2_to_f16x2<3>(hi) : e2m1x2_to_f16x2<1>(hi));
-    return make_uint4(pack_bf16x2(a.x * f, a.y * f), pack_bf16x2(b.x * f, b.y * f), pack_bf16x2(c.x * f, c.y * f), pack_bf16x2(d.x * f, d.y * f));
-}
-// the same in f16, `f` twice the block's factor
+// 8 elements of a block, two bytes of codes in `half` (0, 1) of each word, times the block's factor (twice in f), as f16
 __device__ __forceinline__ uint4 to_f16(uint32_t lo, uint32_t hi, bool half, uint32_t f) {
     return make_uint4(mul_f16x2(half ? e2m1x2_to_f16x2<2>(lo) : e2m1x2_to_f16x2<0>(lo), f), mul_f16x2(half ? e2m1x2_to_f16x2<3>(lo) : e2m1x2_to_f16x2<1>(lo), f),
                       mul_f16x2(half ? e2m1x2_to_f16x2<2>(hi) : e2m1x2_to_f16x2<0>(hi), f), mul_f16x2(half ? e2m1x2_to_f16x2<3>(hi) : e2m1x2_to_f16x2<1>(hi), f));
 }
-__device__ __forceinline__ uint4 convert(uint32_t lo, uint32_t hi, bool half, float f) { return to_bf16(lo, hi, half, f); }
-__device__ __forceinline__ uint4 convert(uint32_t lo, uint32_t hi, bool half, uint32_t f) { return to_f16(lo, hi, half, f); }
 // A token's 64 code bytes to its row of a tile
-template <typename F>
-__device__ __forceinline__ void store_row(uint8_t* tile, uint32_t row, const uint4 (&codes)[4], const F (&f)[4]) {
+__device__ __forceinline__ void store_row(uint8_t* tile, uint32_t row, const uint4 (&codes)[4], const ValueFactors& factors) {
     uint8_t* at = tile + row * 128u;
+    const uint32_t f[4] = {__byte_perm(factors.r01, 0u, 0x1010), __byte_perm(factors.r01, 0u, 0x3232), __byte_perm(factors.r23, 0u, 0x1010), __byte_perm(factors.r23, 0u, 0x3232)};
 #pragma unroll
     for (uint32_t j = 0; j < 4; ++j) {
 #pragma unroll
         for (uint32_t b = 0; b < 4; ++b) {
-            const uint4 x = convert(b < 2 ? codes[j].x : codes[j].y, b < 2 ? codes[j].z : codes[j].w, b & 1u, f[b]);
+            const uint4 x = to_f16(b < 2 ? codes[j].x : codes[j].y, b < 2 ? codes[j].z : codes[j].w, b & 1u, f[b]);
             *reinterpret_cast<uint4*>(at + (b >> 1) * kAtomBytes + (((4u * (b & 1u) + j) ^ (row & 7u)) << 4)) = x;
         }
     }
@@ -109,11 +105,12 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
     if (threadIdx.x == 0u) {
         for (uint32_t i = 0; i < 2; ++i) {
             mbar_init(bar(kKFull + i), 128u), mbar_init(bar(kVFull + i), 128u);
-            mbar_init(bar(kKEmpty + i), 1u), mbar_init(bar(kVEmpty + i), 1u), mbar_init(bar(kSFull + i), 1u), mbar_init(bar(kODone + i), 1u);
-            mbar_init(bar(kPFull + i), 4u), mbar_init(bar(kOFree + i), 4u);
+            mbar_init(bar(kKEmpty + i), 2u), mbar_init(bar(kVEmpty + i), 2u), mbar_init(bar(kOFree + i), 4u);
+            mbar_init(bar(kSFull + i), 1u), mbar_init(bar(kODone + i), 1u);
         }
+        for (uint32_t i = 0; i < 4; ++i) mbar_init(bar(kPFull + i), 4u);
         for (uint32_t i = 0; i < kFactorSlots; ++i) mbar_init(bar(kEFull + i), 4u);
-        mbar_init(bar(kQFull), 128u), mbar_init(bar(kQEmpty), 1u), mbar_init(bar(kDrained), 1u);
+        mbar_init(bar(kQFull), 128u), mbar_init(bar(kQFull + 1u), 128u), mbar_init(bar(kQEmpty), 2u), mbar_init(bar(kDrained), 1u), mbar_init(bar(kDrained + 1u), 1u);
         fence_mbar_init();
         sh.failed = sh.not_drained = 0u;
     }
@@ -128,38 +125,43 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
     const uint32_t all = sum_steps(p, deal, 0u, sh.part).all;
     const uint32_t n_work = workers(all, gridDim.x);
     volatile uint32_t* failed = &sh.failed;
+    clear_empty_entries(p, deal);
+    if (threadIdx.x == 0u) begun_by(p.ws, blockIdx.x)->last = blockIdx.x;
     if (blockIdx.x < n_work) {
         const uint32_t begin = run_begin(all, n_work, blockIdx.x);
-        uint32_t left = run_begin(all, n_work, blockIdx.x + 1u) - begin;
+        const uint32_t end = run_begin(all, n_work, blockIdx.x + 1u);
+        uint32_t left = end - begin;
         Place at = find_step(p, deal, begin);
         if (warp < 8u) {
             asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
             const uint32_t q = warp >> 2, r = threadIdx.x & 127u, lanes = (warp & 3u) << 21;   // 32 TMEM lanes per warp, in bits 16 and up
             const uint32_t t_s = tmem + lanes + kColS + 128u * q, t_o = tmem + lanes + kColO + 128u * q;
-            const float c = p.scale_log2;
-            uint32_t s_phase = 0, o_phase = 0, step0 = 0;   // step0: steps in front of the segment
+            uint32_t s_phase = 0, o_phase = 0, step0 = 0, segment = 0;   // step0, segment: steps and segments in front of this one
             bool ok = true;
-            while (left > 0u && ok) {
+            for (; left > 0u && ok; ++segment) {
+                const uint32_t pos = end - left;
                 const Segment seg = next_segment(p, deal, at, left);
+                if (threadIdx.x == 0u && seg.first == 0u && seg.steps < seg.of) *begun_by(p.ws, blockIdx.x) = {seg.b, seg.head, seg.row0, worker_at(all, n_work, pos + seg.of - 1u)};
                 const uint32_t length = length_of(p.c, seg.b), n = count_of(p.counts, seg.b, p.S, length);
                 const uint32_t steps = tile_steps(p, seg, q, length, n), row = seg.row0 + q * kTileRows + r, i = row / p.group;
                 const bool exists = row < p.S * p.group, live = exists && i < n;
                 const uint32_t limit = !live ? 0u : p.causal ? length - n + i + 1u : length;
-                float m = kLowest, l = 0.0f;
-                for (uint32_t j = 0; j < steps; ++j) {
-                    if (!mbar_wait(bar(kSFull + q), s_phase, failed)) {
-                        ok = false;
-                        break;
-                    }
-                    s_phase ^= 1u;
+                float m = kLowest, l = 0.0f, c_row = 0.0f;
+                if (steps > 0u) {   // (slots of their own for even and odd segments: while this group stores the rows of the one before, the next but one cannot have come)
+                    ok = mbar_wait(bar(kQFull + (segment & 1u)), segment >> 1 & 1u, failed);
+                    c_row = p.scale_log2 * sh.q_factor[segment & 1u][q * kTileRows + r];
+                }
+                for (uint32_t j = 0; j < steps && ok; ++j) {
                     // (not the K tile's barrier: while a group is still storing the rows of the segment before, that one may already be two steps on)
-                    if (!mbar_wait(bar(kEFull + (step0 + j) % kFactorSlots), (step0 + j) / kFactorSlots & 1u, failed)) {
-                        ok = false;
-                        break;
-                    }
+                    const uint32_t slot = (step0 + j) % kFactorSlots;
+                    ok = mbar_wait(bar(kEFull + slot), (step0 + j) / kFactorSlots & 1u, failed);
+                    const uint4 mk = sh.most[slot][0], mv = sh.most[slot][1];
+                    const int ek = group_exponent(max(max(mk.x, mk.y), max(mk.z, mk.w))), e = group_exponent(max(max(mv.x, mv.y), max(mv.z, mv.w)));
+                    const float c = fmaxf(c_row * __uint_as_float(static_cast<uint32_t>(127 + ek - kUp) << 23), kLeast), ef = static_cast<float>(e);
+                    ok = ok && mbar_wait(bar(kSFull + q), s_phase, failed);
+                    if (!ok) break;
+                    s_phase ^= 1u;
                     tc_fence_after_sync();
-                    const uint4 most4 = sh.e[(step0 + j) % kFactorSlots];
-                    const int e = group_exponent(max(max(most4.x, most4.y), max(most4.z, most4.w)));
                     uint32_t s[4][32];
 #pragma unroll
                     for (int k = 0; k < 4; ++k) tmem_ld32(t_s + 32u * k, s[k]);
@@ -183,15 +185,15 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
 #pragma unroll
                         for (int x = 2; x < 32; x += 2) top[k] = fmaxf(top[k], fmaxf(__uint_as_float(s[k][x]), __uint_as_float(s[k][x + 1])));
                     }
-                    const float most = fmaf(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])), c, static_cast<float>(e));
+                    const float most = fmaf(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])), c, ef);
                     const bool over = most > m + kSlack;
                     if (__any_sync(0xFFFFFFFFu, over)) {
                         const float next = over ? most : m, f = ex2(m - next);
                         m = next;
                         l *= f;
-                        if (j > 0u) {   // the product before this one is done: S came behind it
-#pragma unroll
-                            for (int k = 0; k < 8; ++k) {
+                        if (j > 0u) {   // the product before this one is over: S came behind it
+#pragma unroll 1
+                            for (uint32_t k = 0; k < 8u; ++k) {
                                 uint32_t o[16];
                                 tmem_ld16(t_o + 16u * k, o);
                                 tmem_wait_ld();
@@ -203,7 +205,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
                             tmem_wait_st();
                         }
                     }
-                    const float shift = static_cast<float>(e) - m;
+                    const float shift = ef - m;
                     float l0 = 0.0f, l1 = 0.0f;
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
@@ -217,26 +219,26 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
                             pw[x] = pack_f16x2(ea, eb);
                         }
                         tmem_st16(t_s + 16u * k, pw);
+                        if (k & 1) {
+                            tmem_wait_st();
+                            tc_fence_before_sync();
+                            __syncwarp();
+                            if (lane == 0u) mbar_arrive(bar(kPFull + 2u * q + (k >> 1)));
+                        }
                     }
                     l = fmaf(l0 + l1, __uint_as_float(static_cast<uint32_t>(127 - e) << 23), l);
-                    tmem_wait_st();
-                    tc_fence_before_sync();
-                    __syncwarp();
-                    if (lane == 0u) mbar_arrive(bar(kPFull + q));
                 }
                 if (!ok) break;
                 step0 += seg.steps;
                 const bool whole = seg.steps == seg.of;
                 const uint32_t h = seg.head * p.group + row % p.group;
-                float* part = slot_of(p.ws, blockIdx.x, seg.first == 0u ? 1u : 0u, kItemRows) + (q * kTileRows + r) * 128u;
+                float* part = slot_of(p.ws, gridDim.x, blockIdx.x, seg.first == 0u ? 1u : 0u, kItemRows) + (q * kTileRows + r) * 128u;
                 __nv_bfloat16* out = p.out + ((static_cast<size_t>(seg.b) * p.S + i) * p.H + h) * 128u;
                 const bool none = l == 0.0f;   // NaN is something
                 const float inv = none ? 0.0f : kDown / l;
                 if (steps > 0u) {
-                    if (!mbar_wait(bar(kODone + q), o_phase, failed)) {
-                        ok = false;
-                        break;
-                    }
+                    ok = mbar_wait(bar(kODone + q), o_phase, failed);
+                    if (!ok) break;
                     o_phase ^= 1u;
                     tc_fence_after_sync();
                 }
@@ -274,42 +276,44 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
                 if (whole) {
                     if (exists && p.lse != nullptr) p.lse[(static_cast<size_t>(seg.b) * p.H + h) * p.S + i] = none ? -INFINITY : (m + lg2(l)) * kLn2;
                 } else if (live) {
-                    *reinterpret_cast<float2*>(slot_of(p.ws, blockIdx.x, seg.first == 0u ? 1u : 0u, kItemRows) + kItemRows * 128u + 2u * (q * kTileRows + r)) = make_float2(m, l);
+                    *reinterpret_cast<float2*>(slot_of(p.ws, gridDim.x, blockIdx.x, seg.first == 0u ? 1u : 0u, kItemRows) + kItemRows * 128u + 2u * (q * kTileRows + r)) = make_float2(m, l);
                 }
             }
         } else if (warp < 12u) {
             asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kConvertRegs));
             const uint32_t r = threadIdx.x & 127u, page = 1u << p.c.page_log2;
-            uint32_t step = 0, q_count = 0;   // steps and segments so far
+            uint32_t step = 0, segment = 0;   // so far
             bool ok = true;
-            while (left > 0u && ok) {
+            for (; left > 0u && ok; ++segment) {
                 const Segment seg = next_segment(p, deal, at, left);
                 const uint32_t length = length_of(p.c, seg.b), n = count_of(p.counts, seg.b, p.S, length);
+                // the token of this thread in step j: its page, looked up a step ahead of its bytes
+                long long page_ahead = -1;
+                auto look_up = [&](uint32_t j) {
+                    const uint32_t t = (seg.first + j) * kStepTokens + r;
+                    if (j < seg.steps && t < length) page_ahead = page_of(p.c, seg.b, t);
+                };
                 uint4 k[4], v[4];
                 uint32_t ks = 0, vs = 0;
                 bool lost = false, empty = true;
-                auto fetch = [&](uint32_t j) {
+                auto fetch = [&](uint32_t j, bool values) {
                     const uint32_t t = (seg.first + j) * kStepTokens + r;
-                    empty = j >= seg.steps || t >= length;
-                    if (empty) return;
-                    const long long id = page_of(p.c, seg.b, t);
-                    lost = id < 0;
-                    if (lost) return;
-                    const uint8_t* rec = record_of(p.c, id, seg.head);
+                    if (j >= seg.steps || t >= length || page_ahead < 0) return;
+                    const uint8_t* rec = record_of(p.c, page_ahead, seg.head);
                     const uint32_t slot = t & (page - 1u);
+                    if (values) {
 #pragma unroll
-                    for (int x = 0; x < 4; ++x) k[x] = ld_v4(rec + 64u * slot + 16u * x), v[x] = ld_v4(rec + 64u * (page + slot) + 16u * x);
-                    ks = ld_u32(rec + 128u * page + 4u * slot), vs = ld_u32(rec + 132u * page + 4u * slot);
+                        for (int x = 0; x < 4; ++x) v[x] = ld_v4(rec + 64u * (page + slot) + 16u * x);
+                    } else {
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) k[x] = ld_v4(rec + 64u * slot + 16u * x);
+                        ks = ld_u32(rec + 128u * page + 4u * slot), vs = ld_u32(rec + 132u * page + 4u * slot);
+                    }
                 };
-                fetch(0);
                 // the query rows: 16 threads a row, 16 bytes each
-                if (!mbar_wait(bar(kQEmpty), (q_count + 1u) & 1u, failed)) {
-                    ok = false;
-                    break;
-                }
-                ++q_count;
+                ok = mbar_wait(bar(kQEmpty), (segment + 1u) & 1u, failed);
 #pragma unroll 1
-                for (uint32_t x0 = 0; x0 < 32u; x0 += 8u) {
+                for (uint32_t x0 = 0; x0 < 32u && ok; x0 += 8u) {
                     uint4 raw[8];
 #pragma unroll
                     for (uint32_t x = 0; x < 8u; ++x) {
@@ -320,128 +324,140 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
 #pragma unroll
                     for (uint32_t x = 0; x < 8u; ++x) {
                         const uint32_t e = (x0 + x) * 128u + r, row = e >> 4, chunk = e & 15u;
-                        *reinterpret_cast<uint4*>(sh.q[row >> 7] + (chunk >> 3) * kAtomBytes + (row & 127u) * 128u + (((chunk & 7u) ^ (row & 7u)) << 4)) = raw[x];
+                        uint32_t w[4] = {raw[x].x, raw[x].y, raw[x].z, raw[x].w}, amax = 0;
+#pragma unroll
+                        for (int y = 0; y < 4; ++y) amax = max(amax, max((w[y] << 16) & 0x7FFFFFFFu, w[y] & 0x7FFF0000u));
+#pragma unroll
+                        for (int y = 1; y < 16; y <<= 1) amax = max(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, y));
+                        const float2 f = row_factors(amax);
+#pragma unroll
+                        for (int y = 0; y < 4; ++y) w[y] = pack_f16x2(__uint_as_float(w[y] << 16) * f.x, __uint_as_float(w[y] & 0xFFFF0000u) * f.x);
+                        *reinterpret_cast<uint4*>(sh.q[row >> 7] + (chunk >> 3) * kAtomBytes + (row & 127u) * 128u + (((chunk & 7u) ^ (row & 7u)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+                        if (chunk == 0u) sh.q_factor[segment & 1u][row] = f.y;
                     }
                 }
                 fence_proxy_async_smem();
-                mbar_arrive(bar(kQFull));
+                mbar_arrive(bar(kQFull + (segment & 1u)));
+                look_up(0u);
+                empty = seg.first * kStepTokens + r >= length, lost = page_ahead < 0;
+                fetch(0u, false);
+                fetch(0u, true);
+                look_up(1u);
                 for (uint32_t j = 0; j < seg.steps; ++j, ++step) {
-                    const uint32_t st = step % kStages, parity = (step / kStages + 1u) & 1u;
+                    const uint32_t st = step % kStages, parity = (step / kStages + 1u) & 1u, slot = step % kFactorSlots;
                     // A token behind the length must not bring NaN into P V; one that is lost, or whose V is NaN, makes the rows that see it NaN by its scores
-                    float fk[4];
-                    uint32_t fv[4];
-                    const uint32_t largest = empty || lost ? 0u : largest_byte(vs), met = __reduce_max_sync(0xFFFFFFFFu, largest == 255u ? 0u : largest);
-                    if (lane == 0u) reinterpret_cast<uint32_t*>(&sh.e[step % kFactorSlots])[warp & 3u] = met;
-                    named_bar_sync(1u, 128u);
-                    const uint4 most4 = sh.e[step % kFactorSlots];
-                    const ValueFactors f = value_factors(vs, largest, group_exponent(max(max(most4.x, most4.y), max(most4.z, most4.w))));
-                    const bool broken = largest == 255u;
-#pragma unroll
-                    for (int x = 0; x < 4; ++x) fk[x] = scale_f32(ks, x);
-                    fv[0] = __byte_perm(f.r01, 0u, 0x1010), fv[1] = __byte_perm(f.r01, 0u, 0x3232), fv[2] = __byte_perm(f.r23, 0u, 0x1010), fv[3] = __byte_perm(f.r23, 0u, 0x3232);
-                    if (empty || lost) {
-#pragma unroll
-                        for (int x = 0; x < 4; ++x) k[x] = v[x] = make_uint4(0u, 0u, 0u, 0u);
+                    const uint32_t top_k = empty || lost ? 0u : largest_byte(ks), top_v = empty || lost ? 0u : largest_byte(vs);
+                    const uint32_t met_k = __reduce_max_sync(0xFFFFFFFFu, top_k == 255u ? 0u : top_k), met_v = __reduce_max_sync(0xFFFFFFFFu, top_v == 255u ? 0u : top_v);
+                    if (lane == 0u) reinterpret_cast<uint32_t*>(&sh.most[slot][0])[warp & 3u] = met_k, reinterpret_cast<uint32_t*>(&sh.most[slot][1])[warp & 3u] = met_v;
+                    // (also where a wait has run out in one of the four warps: they leave together)
+                    ok = named_bar_all(1u, 128u, ok);
+                    if (!ok) break;
+                    if (lane == 0u) mbar_arrive(bar(kEFull + slot));
+                    const uint4 mk = sh.most[slot][0], mv = sh.most[slot][1];
+                    ValueFactors fk = value_factors(ks, top_k, group_exponent(max(max(mk.x, mk.y), max(mk.z, mk.w))));
+                    ValueFactors fv = value_factors(vs, top_v, group_exponent(max(max(mv.x, mv.y), max(mv.z, mv.w))));
+                    if (empty || lost || top_v == 255u) {
+                        fk.r01 = fk.r23 = empty ? 0u : 0x7E007E00u, fv.r01 = fv.r23 = 0u;   // (the codes are whatever they were: finite)
                     }
-                    if (empty || lost || broken) {
-#pragma unroll
-                        for (int x = 0; x < 4; ++x) fk[x] = empty ? 0.0f : __uint_as_float(0x7FC00000u), fv[x] = 0u;
+                    ok = mbar_wait(bar(kKEmpty + st), parity, failed);
+                    if (ok) {
+                        store_row(sh.k[st], r, k, fk);
+                        fence_proxy_async_smem();
+                        mbar_arrive(bar(kKFull + st));
                     }
-                    if (!mbar_wait(bar(kKEmpty + st), parity, failed)) {
-                        ok = false;
-                        break;
+                    empty = j + 1u >= seg.steps || (seg.first + j + 1u) * kStepTokens + r >= length, lost = page_ahead < 0;
+                    fetch(j + 1u, false);
+                    ok = ok && mbar_wait(bar(kVEmpty + st), parity, failed);
+                    if (ok) {
+                        store_row(sh.v[st], r, v, fv);
+                        fence_proxy_async_smem();
+                        mbar_arrive(bar(kVFull + st));
                     }
-                    if (lane == 0u) mbar_arrive(bar(kEFull + step % kFactorSlots));
-                    store_row(sh.k[st], r, k, fk);
-                    fence_proxy_async_smem();
-                    mbar_arrive(bar(kKFull + st));
-                    if (!mbar_wait(bar(kVEmpty + st), parity, failed)) {
-                        ok = false;
-                        break;
-                    }
-                    store_row(sh.v[st], r, v, fv);
-                    fence_proxy_async_smem();
-                    mbar_arrive(bar(kVFull + st));
-                    lost = false, ks = vs = 0u;
-                    fetch(j + 1u);
+                    fetch(j + 1u, true);
+                    look_up(j + 2u);
                 }
             }
         } else {
             asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kIssueRegs));
-            if (warp == 12u) {
-                const uint32_t id_s = idesc_16bit(true, 128, 128, 0, 0), id_o = idesc_16bit(false, 128, 128, 0, 1);
-                const uint64_t dq = make_smem_desc(smem_u32(sh.q[0]), 16, 1024, kSwizzle128B), dk = make_smem_desc(smem_u32(sh.k[0]), 16, 1024, kSwizzle128B);
-                const uint64_t dv = make_smem_desc(smem_u32(sh.v[0]), kAtomBytes, 1024, kSwizzle128B);
-                uint32_t step = 0, q_count = 0, p_phase[2] = {0u, 0u}, o_count[2] = {0u, 0u};
-                auto scores = [&](uint32_t q, uint32_t st) {
-                    if (elect_one_sync()) {
-#pragma unroll
-                        for (uint32_t x = 0; x < 8u; ++x) {
-                            const uint32_t off = ((x >> 2) * kAtomBytes + (x & 3u) * 32u) >> 4;
-                            mma_f16_ss(tmem + kColS + 128u * q, dq + (q * kTileBytes >> 4) + off, dk + (st * kTileBytes >> 4) + off, id_s, x > 0u ? 1u : 0u);
-                        }
-                        tc_commit(bar(kSFull + q));
-                    }
-                    __syncwarp();
-                };
-                auto outputs = [&](uint32_t q, uint32_t st, bool first, bool last) {
-                    if (elect_one_sync()) {
-#pragma unroll
-                        for (uint32_t x = 0; x < 8u; ++x)
-                            mma_f16_ts(tmem + kColO + 128u * q, tmem + kColS + 128u * q + 8u * x, dv + ((st * kTileBytes + x * 2048u) >> 4), id_o, (!first || x > 0u) ? 1u : 0u);
-                        if (last) tc_commit(bar(kODone + q));
-                    }
-                    __syncwarp();
+            if (warp < 14u) {
+                // All of this runs on values that are the same in the warp's 32 lanes. The compiler has to see that (they come out of votes and reductions, which have uniform
+                // results): the products' operands then stay in uniform registers and take few instructions to issue. A warp per tile: the two take turns with the tensor cores,
+                // and neither's waits hold the other's products up.
+                auto uniform = [](uint32_t x) { return __reduce_max_sync(0xFFFFFFFFu, x); };
+                const uint32_t q = uniform(warp - 12u), t_s = uniform(tmem) + kColS + 128u * q, t_o = uniform(tmem) + kColO + 128u * q;
+                constexpr uint32_t id_s = idesc_16bit(false, 128, 128, 0, 0), id_o = idesc_16bit(false, 128, 128, 0, 1);
+                const uint64_t d_k = make_smem_desc(smem_u32(sh.q[0]), 16, 1024, kSwizzle128B), d_v = make_smem_desc(smem_u32(sh.v[0]), kAtomBytes, 1024, kSwizzle128B);
+                const uint32_t k_hi = static_cast<uint32_t>(d_k >> 32), v_hi = static_cast<uint32_t>(d_v >> 32);
+                const uint32_t q_lo = uniform(static_cast<uint32_t>(d_k)) + (q * kTileBytes >> 4), k_lo = uniform(static_cast<uint32_t>(d_k)) + (2u * kTileBytes >> 4), v_lo = uniform(static_cast<uint32_t>(d_v));
+                static_assert(offsetof(Shared, k) == 2u * kTileBytes, "K behind Q");
+                uint32_t step = 0, segment = 0, p_phase = 0, o_phase = 1;
+                bool ok = true;
+                auto wait = [&](uint32_t b, uint32_t parity) {
+                    ok = ok && __all_sync(0xFFFFFFFFu, mbar_wait(b, parity, failed));
+                    return ok;
                 };
                 auto commit = [&](uint32_t b) {
                     if (elect_one_sync()) tc_commit(b);
-                    __syncwarp();
                 };
-                bool ok = true;
-                auto wait = [&](uint32_t b, uint32_t parity) {
-                    if (ok && !mbar_wait(b, parity, failed)) ok = false;
-                    return ok;
+                auto scores = [&](uint32_t st) {
+                    if (elect_one_sync()) {
+                        const uint32_t b = k_lo + (st * kTileBytes >> 4);
+#pragma unroll
+                        for (uint32_t x = 0; x < 8u; ++x) {
+                            const uint32_t off = ((x >> 2) * kAtomBytes + (x & 3u) * 32u) >> 4;
+                            mma_f16_ss(t_s, q_lo + off, k_hi, b + off, k_hi, id_s, x > 0u ? 1u : 0u);
+                        }
+                        tc_commit(bar(kSFull + q));
+                    }
                 };
-                while (left > 0u && ok) {
+                for (; uniform(left) > 0u && ok; ++segment) {
                     const Segment seg = next_segment(p, deal, at, left);
                     const uint32_t length = length_of(p.c, seg.b), n = count_of(p.counts, seg.b, p.S, length);
-                    // (the same in all lanes; said so, it lets the compiler keep what the products take in uniform registers)
-                    const uint32_t steps[2] = {__shfl_sync(0xFFFFFFFFu, tile_steps(p, seg, 0u, length, n), 0), __shfl_sync(0xFFFFFFFFu, tile_steps(p, seg, 1u, length, n), 0)};
-                    const uint32_t seg_steps = __shfl_sync(0xFFFFFFFFu, seg.steps, 0);
-                    if (!wait(bar(kQFull), q_count & 1u)) break;
-                    ++q_count;
+                    const uint32_t steps = uniform(tile_steps(p, seg, q, length, n)), seg_steps = uniform(seg.steps);
+                    if (!wait(bar(kQFull + (segment & 1u)), segment >> 1 & 1u)) break;
                     if (!wait(bar(kKFull + step % kStages), step / kStages & 1u)) break;
                     tc_fence_after_sync();
-                    if (steps[0] > 0u) scores(0u, step % kStages);
-                    if (steps[1] > 0u) scores(1u, step % kStages);
+                    if (steps > 0u) {
+                        scores(step % kStages);   // overwrites P of the step before, behind its products
+                        if (!wait(bar(kOFree + q), o_phase)) break;
+                        o_phase ^= 1u;
+                    }
                     commit(bar(kKEmpty + step % kStages));
                     if (seg_steps == 1u) commit(bar(kQEmpty));
                     for (uint32_t j = 0; j < seg_steps; ++j, ++step) {
                         const uint32_t st = step % kStages, next = (step + 1u) % kStages;
                         const bool more = j + 1u < seg_steps;
                         if (!wait(bar(kVFull + st), step / kStages & 1u)) break;
-                        if (more && !wait(bar(kKFull + next), (step + 1u) / kStages & 1u)) break;
+                        if (j < steps) {
 #pragma unroll
-                        for (uint32_t q = 0; q < 2u; ++q) {
-                            if (j < steps[q]) {
-                                if (j == 0u) wait(bar(kOFree + q), (o_count[q]++ + 1u) & 1u);
-                                if (!wait(bar(kPFull + q), p_phase[q])) break;
-                                p_phase[q] ^= 1u;
+                            for (uint32_t h = 0; h < 2u; ++h) {
+                                if (!wait(bar(kPFull + 2u * q + h), p_phase)) break;
                                 tc_fence_after_sync();
-                                outputs(q, st, j == 0u, j + 1u == steps[q]);
+                                if (elect_one_sync()) {
+                                    const uint32_t b = v_lo + ((st * kTileBytes + h * kHalf * 128u) >> 4);
+#pragma unroll
+                                    for (uint32_t x = 0; x < 4u; ++x) mma_f16_ts(t_o, t_s + 32u * h + 8u * x, b + (x * 2048u >> 4), v_hi, id_o, (j > 0u || h + x > 0u) ? 1u : 0u);
+                                    if (h == 1u && j + 1u == steps) tc_commit(bar(kODone + q));
+                                }
                             }
-                            if (q == 1u) commit(bar(kVEmpty + st));
-                            if (more && j + 1u < steps[q]) scores(q, next);
+                            p_phase ^= 1u;
                         }
                         if (!ok) break;
-                        if (more) commit(bar(kKEmpty + next));
+                        commit(bar(kVEmpty + st));
+                        if (more) {
+                            if (!wait(bar(kKFull + next), (step + 1u) / kStages & 1u)) break;
+                            tc_fence_after_sync();
+                            if (j + 1u < steps) scores(next);
+                            commit(bar(kKEmpty + next));
+                        }
                         if (j + 2u == seg_steps) commit(bar(kQEmpty));
                     }
                 }
                 if (!ok) {   // whatever was issued has to be over before the tensor memory goes back
-                    commit(bar(kDrained));
-                    (void)mbar_wait(bar(kDrained), 0u, &sh.not_drained);
+                    commit(bar(kDrained + q));
+                    (void)mbar_wait(bar(kDrained + q), 0u, &sh.not_drained);
                 }
+                __syncwarp();
             }
         }
     }

@@ -98,12 +98,30 @@ __device__ __forceinline__ Segment next_segment(const Kv4AttendParams& p, const 
     return s;
 }
 
-// Partials of CTA w: two slots (0: an item that an earlier CTA began, 1: one that a later CTA goes on with), each `rows` x 128 f32 of O, in front of `rows` pairs of M (base 2) and l
-__device__ __forceinline__ float* slot_of(float* ws, uint32_t w, uint32_t slot, uint32_t rows) { return ws + (static_cast<size_t>(w) * 2u + slot) * rows * 130u; }
+// The workspace of a launch of `grid` CTAs: an entry per CTA that says which item the CTA began and others went on with, behind them the CTAs' partials: two slots (0: an item
+// that an earlier CTA began, 1: one that a later CTA goes on with), each `rows` x 128 f32 of O in front of `rows` pairs of M (base 2) and l
+struct Begun {
+    uint32_t b, head, row0, last;   // the last CTA that has a part; the CTA itself: there is no such item
+};
+__device__ __forceinline__ Begun* begun_by(float* ws, uint32_t w) { return reinterpret_cast<Begun*>(ws) + w; }
+__device__ __forceinline__ float* slot_of(float* ws, uint32_t grid, uint32_t w, uint32_t slot, uint32_t rows) { return ws + 4u * grid + (static_cast<size_t>(w) * 2u + slot) * rows * 130u; }
 constexpr float kLowest = -1e30f;   // M of a row that has seen nothing
+
+// Entries that no CTA has steps of: their rows see nothing. All threads of the grid.
+__device__ __forceinline__ void clear_empty_entries(const Kv4AttendParams& p, const Deal& d) {
+    for (uint32_t e = blockIdx.x; e < p.c.B * d.row_tiles; e += gridDim.x) {
+        if (steps_of(p, d, e) != 0u) continue;
+        const uint32_t b = e / d.row_tiles, row0 = (e - b * d.row_tiles) * d.rows, rows = min(d.rows, p.S * p.group - row0);
+        for (uint32_t x = threadIdx.x; x < rows * p.c.HK * 16u; x += blockDim.x) {
+            const uint32_t part = x & 15u, row = row0 + (x >> 4) % rows, head = (x >> 4) / rows, i = row / p.group, h = head * p.group + row % p.group;
+            *reinterpret_cast<uint4*>(p.out + ((static_cast<size_t>(b) * p.S + i) * p.H + h) * 128u + 8u * part) = make_uint4(0u, 0u, 0u, 0u);
+            if (part == 0u && p.lse != nullptr) p.lse[(static_cast<size_t>(b) * p.H + h) * p.S + i] = -INFINITY;
+        }
+    }
+}
 
 }  // namespace kv4
 
-inline uint64_t kv4_partial_bytes(uint32_t grid, uint32_t rows) { return static_cast<uint64_t>(grid) * 2u * rows * 130u * 4u; }
+inline uint64_t kv4_partial_bytes(uint32_t grid, uint32_t rows) { return static_cast<uint64_t>(grid) * (16u + 2u * rows * 130u * 4u); }
 
 }  // namespace b200mx

@@ -69,6 +69,7 @@ int fmha_kv4_append(const fmha_kv4_cache* cache, const fmha_kv4_rows* k, const f
     if (int r = rows_of(k, "append: k", rk, err, cap)) return r;
     if (int r = rows_of(v, "append: v", rv, err, cap)) return r;
     if (S == 0u) return 0;
+    if (static_cast<uint64_t>(c.B) * S * c.HK > kMostRows) return refuse(err, cap, "append: more than 2^30 rows");
     return done(b200mx::launch_kv4_append(c, rk, rv, S, counts, static_cast<cudaStream_t>(stream)), err, cap);
 }
 
@@ -80,6 +81,7 @@ int fmha_kv4_read(const fmha_kv4_cache* cache, const fmha_kv4_rows* k, const fmh
     if (int r = rows_of(v, "read: v", rv, err, cap)) return r;
     if (!last && counts != nullptr) return refuse(err, cap, "read: counts go with the newest tokens only");
     if (S == 0u) return 0;
+    if (static_cast<uint64_t>(c.B) * S * c.HK > kMostRows) return refuse(err, cap, "read: more than 2^30 rows");
     return done(b200mx::launch_kv4_read(c, rk, rv, S, last != 0, counts, static_cast<cudaStream_t>(stream)), err, cap);
 }
 

@@ -30,6 +30,7 @@ struct Kv4AttendParams {
     float* weights;
     const float* weights_in;
     float* ws;
+    float* scores;      // null, or [B][HK][tokens of the table][rows of a KV head, even]: what the weights are made of
     unsigned long long weights_width;
     uint32_t S, H, group, causal;
     float scale_log2;   // scale * log2(e)
@@ -50,6 +51,8 @@ cudaError_t launch_kv4_append(const Kv4View& c, const Kv4Rows& k, const Kv4Rows&
 cudaError_t launch_kv4_read(const Kv4View& c, const Kv4Rows& k, const Kv4Rows& v, uint32_t S, bool last, const int32_t* counts, cudaStream_t stream);
 uint64_t kv4_attend_workspace(const Kv4View& c, uint32_t S, uint32_t H, bool weights, bool lse);
 cudaError_t launch_kv4_attend(const Kv4AttendParams& p, cudaStream_t stream);
+// kv4_weigh.cu: the attention weights, from p.lse and, if there, p.scores
+cudaError_t launch_kv4_weigh(const Kv4AttendParams& p, cudaStream_t stream);
 // kv4_prefill.cu: one CTA per SM, items of kv4_prefill_rows() query rows, partials in p.ws as the decode kernels leave them
 uint32_t kv4_prefill_grid();
 uint32_t kv4_prefill_rows();

@@ -1,18 +1,19 @@
-// Attention of few query rows over the 4-bit cache: decode, drafts of a few tokens, and (32 rows of a KV head at a time) any number of rows.
+// Attention of few query rows over the 4-bit cache: decode, and drafts of a few tokens, up to 32 rows of a KV head (kv4_prefill.cu has more).
 //
-// Work. An item is one sequence and KV head (and row tile); its tokens are cut in tiles of 128. All tiles of all items, in order, are dealt out in equal runs to the
-// CTAs, from the lengths on the device: a batch of ragged sequences keeps every CTA busy for the same time, one long sequence as well. An item that more than one CTA
-// worked on is put together from f32 partials by the combine kernel.
+// Work. An item is one sequence and KV head; its tokens are cut in tiles of 128. All tiles of all items, in order, are dealt out in equal runs to the CTAs, from the
+// lengths on the device: a batch of ragged sequences keeps every CTA busy for the same time, one long sequence as well. An item that more than one CTA worked on is put
+// together from f32 partials by the combine kernel.
 //
-// A warp takes 32 tokens of a tile, 4352 bytes, which copies of whole page records (cp.async.bulk) bring to a ring of its own in shared memory, and computes both
-// products transposed, so that the tokens are the rows of the matrix instruction and the few query rows its 8 columns:
+// Copies of whole page records (cp.async.bulk) bring a tile, 17408 bytes, to a ring of three in shared memory; the warps take turns in issuing them. A warp takes 32 of
+// the tile's tokens and computes both products transposed, so that the tokens are the rows of the matrix instruction and the few query rows its 8 columns:
 //   S^T [16 tokens x 8 rows] = K [16 x 128] Q^T      K's codes become f16 by the conversion instruction, two per byte; the E8M0 factor of a token's 32 elements
 //                                                     multiplies the two products' sum in f32
 //   O^T [128 x 8 rows] += V^T [128 x 16 tokens] P^T  P goes from S^T's layout to the operand's by an 8 x 8 transpose between lanes; V's factors multiply P
 // Q goes in as f16 with a power of two per row taken out, which is exact for bf16 elements down to 2^-30 of the row's largest.
 //
 // Softmax in base 2 with a running reference per row. P V wants P times V's factor in f16: the reference M follows s + e, e the exponent of the largest V factor of
-// the 32 tokens, so that P 2^e is at most 2^4 however large V is; the factors relative to 2^e are exact in f16 down to 2^-34. M moves when a value exceeds it by more than 2^4, by a vote of the warp; the sums and O are rescaled then.
+// the 32 tokens, so that P 2^e is at most 2^4 however large V is; the factors relative to 2^e are exact in f16 down to 2^-34. M moves when a value exceeds it by more
+// than 2^4, by a vote of the warp; the sums and O are rescaled then.
 #include "kv4.cuh"
 #include "kv4_schedule.cuh"
 #include "ptx_sm100.cuh"
@@ -29,11 +30,10 @@ constexpr unsigned kWarps = 4, kThreads = kWarps * 32;
 constexpr unsigned kUnit = 32;                    // tokens of a warp at a time
 constexpr unsigned kTile = kWarps * kUnit;
 static_assert(kTile == kStepTokens, "a step is a tile");
-constexpr unsigned kUnitBytes = kUnit * FMHA_KV4_TOKEN_BYTES;
-constexpr unsigned kCtasPerSm = 4;
+constexpr unsigned kStages = 3, kTileBytes = kTile * FMHA_KV4_TOKEN_BYTES;
 constexpr float kSlack = 4.0f;
 constexpr float kLeast = 1e-37f;                  // of a row's factor: times a masked score it is still -inf
-constexpr float kLn2 = 0.69314718055994531f, kLog2e = 1.44269504088896341f;
+constexpr float kLn2 = 0.69314718055994531f;
 
 // What a unit's 32 lanes work out for its tokens, one lane a token
 struct TokenFactors {
@@ -45,25 +45,21 @@ struct TokenFactors {
 // pairs, which one load of V codes reads, are two even and two odd ones: their 64-byte rows then meet in the banks in twos, not in fours.
 __device__ __forceinline__ uint32_t row_token(uint32_t r) { return r ^ ((r >> 1) & 1u); }
 
-template <unsigned kStages>
-struct alignas(128) WarpShared {
-    uint8_t ring[kStages][kUnitBytes];
-    TokenFactors f;
-};
-
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
 }
 
-// Query rows of an item as the matrix instruction's operand: rows gid of each of NT groups of eight, elements 32 blk + 8 tig .. + 7 of each block
+// Query rows of an item as the matrix instruction's operand: rows gid of each of NT groups of eight, elements 32 blk + 8 tig .. + 7 of each block. Two and more groups keep
+// the elements in shared memory (a lane reads back what it would hold): the registers are O's.
 template <int NT>
 struct QueryRows {
-    uint32_t q[NT][4][4];   // [group][block][element pair]
-    float factor[NT][2];    // of the columns 2 tig, 2 tig + 1: scale * log2(e) * the power of two taken out
-    uint32_t limit[NT][2];  // tokens that the columns see
+    static constexpr bool kShared = NT >= 2;
+    uint4 q[kShared ? 1 : NT][4];   // [group][block]
+    float factor[NT][2];            // of the columns 2 tig, 2 tig + 1: scale * log2(e) * the power of two taken out
+    uint32_t limit[NT][2];          // tokens that the columns see
 };
 template <int NT>
-__device__ __forceinline__ void load_rows(QueryRows<NT>& x, const Kv4AttendParams& p, uint32_t b, uint32_t head, uint32_t row0, uint32_t length, uint32_t n) {
+__device__ __forceinline__ void load_rows(QueryRows<NT>& x, uint4* q_shared, const Kv4AttendParams& p, uint32_t b, uint32_t head, uint32_t row0, uint32_t length, uint32_t n) {
     const unsigned lane = threadIdx.x & 31u, gid = lane >> 2, tig = lane & 3u;
     const uint32_t rows = p.S * p.group;
 #pragma unroll
@@ -85,9 +81,12 @@ __device__ __forceinline__ void load_rows(QueryRows<NT>& x, const Kv4AttendParam
         const float2 f = row_factors(amax);
 #pragma unroll
         for (int blk = 0; blk < 4; ++blk) {
-            const uint32_t w[4] = {raw[blk].x, raw[blk].y, raw[blk].z, raw[blk].w};
+            uint32_t w[4] = {raw[blk].x, raw[blk].y, raw[blk].z, raw[blk].w};
 #pragma unroll
-            for (int k = 0; k < 4; ++k) x.q[g][blk][k] = pack_f16x2(__uint_as_float(w[k] << 16) * f.x, __uint_as_float(w[k] & 0xFFFF0000u) * f.x);
+            for (int k = 0; k < 4; ++k) w[k] = pack_f16x2(__uint_as_float(w[k] << 16) * f.x, __uint_as_float(w[k] & 0xFFFF0000u) * f.x);
+            const uint4 packed = make_uint4(w[0], w[1], w[2], w[3]);
+            if (QueryRows<NT>::kShared) q_shared[(g * 4 + blk) * 32 + lane] = packed;   // (all warps write the same)
+            else x.q[QueryRows<NT>::kShared ? 0 : g][blk] = packed;
         }
         const uint32_t lim = !live ? 0u : p.causal ? length - n + i + 1u : length;
 #pragma unroll
@@ -97,37 +96,50 @@ __device__ __forceinline__ void load_rows(QueryRows<NT>& x, const Kv4AttendParam
             x.limit[g][j] = __shfl_sync(0xFFFFFFFFu, lim, src);
         }
     }
+    if (QueryRows<NT>::kShared) __syncwarp();
 }
 
-// S^T of 16 tokens: the K codes at `codes` (row-major, 64 bytes a token), factors f[0 .. 15]
+// S^T of 32 tokens: the K codes at `codes` (row-major, 64 bytes a token), the second 16 tokens `granule` bytes on, factors f[0 .. 31]
 template <int NT>
-__device__ __forceinline__ void scores(float (&s)[NT][4], const uint8_t* codes, const float4* f, const QueryRows<NT>& x) {
+__device__ __forceinline__ void scores(float (&s)[2][NT][4], const uint8_t* codes, uint32_t granule, const float4* f, const QueryRows<NT>& x, const uint4* q_shared) {
     const unsigned lane = threadIdx.x & 31u, gid = lane >> 2, tig = lane & 3u;
-    const uint32_t row = row_token(gid);
-    const uint4 top = *reinterpret_cast<const uint4*>(codes + 64u * row + 16u * tig), bot = *reinterpret_cast<const uint4*>(codes + 64u * (row + 8u) + 16u * tig);
-    const float4 ft = f[row], fb = f[row + 8u];
     const float zero[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    const uint32_t row = row_token(gid);
+    uint4 top[2], bot[2];
+#pragma unroll
+    for (int gr = 0; gr < 2; ++gr) {
+        top[gr] = *reinterpret_cast<const uint4*>(codes + gr * granule + 64u * row + 16u * tig);
+        bot[gr] = *reinterpret_cast<const uint4*>(codes + gr * granule + 64u * (row + 8u) + 16u * tig);
+    }
 #pragma unroll
     for (int blk = 0; blk < 4; ++blk) {
-        const uint32_t t0 = blk < 2 ? top.x : top.y, t1 = blk < 2 ? top.z : top.w, b0 = blk < 2 ? bot.x : bot.y, b1 = blk < 2 ? bot.z : bot.w;
-        uint32_t a[8];
-        if (blk & 1) {
-            a[0] = e2m1x2_to_f16x2<2>(t0), a[1] = e2m1x2_to_f16x2<2>(b0), a[2] = e2m1x2_to_f16x2<3>(t0), a[3] = e2m1x2_to_f16x2<3>(b0);
-            a[4] = e2m1x2_to_f16x2<2>(t1), a[5] = e2m1x2_to_f16x2<2>(b1), a[6] = e2m1x2_to_f16x2<3>(t1), a[7] = e2m1x2_to_f16x2<3>(b1);
-        } else {
-            a[0] = e2m1x2_to_f16x2<0>(t0), a[1] = e2m1x2_to_f16x2<0>(b0), a[2] = e2m1x2_to_f16x2<1>(t0), a[3] = e2m1x2_to_f16x2<1>(b0);
-            a[4] = e2m1x2_to_f16x2<0>(t1), a[5] = e2m1x2_to_f16x2<0>(b1), a[6] = e2m1x2_to_f16x2<1>(t1), a[7] = e2m1x2_to_f16x2<1>(b1);
-        }
-        const float st = blk == 0 ? ft.x : blk == 1 ? ft.y : blk == 2 ? ft.z : ft.w, sb = blk == 0 ? fb.x : blk == 1 ? fb.y : blk == 2 ? fb.z : fb.w;
+        uint4 q[NT];
 #pragma unroll
-        for (int g = 0; g < NT; ++g) {
-            float d[4];
-            mma_f16(d, a[0], a[1], a[2], a[3], x.q[g][blk][0], x.q[g][blk][1], zero);
-            mma_f16(d, a[4], a[5], a[6], a[7], x.q[g][blk][2], x.q[g][blk][3], d);
-            if (blk == 0) {
-                s[g][0] = d[0] * st, s[g][1] = d[1] * st, s[g][2] = d[2] * sb, s[g][3] = d[3] * sb;
+        for (int g = 0; g < NT; ++g) q[g] = QueryRows<NT>::kShared ? q_shared[(g * 4 + blk) * 32 + lane] : x.q[QueryRows<NT>::kShared ? 0 : g][blk];
+#pragma unroll
+        for (int gr = 0; gr < 2; ++gr) {
+            const uint32_t t0 = blk < 2 ? top[gr].x : top[gr].y, t1 = blk < 2 ? top[gr].z : top[gr].w, b0 = blk < 2 ? bot[gr].x : bot[gr].y, b1 = blk < 2 ? bot[gr].z : bot[gr].w;
+            uint32_t a[8];
+            if (blk & 1) {
+                a[0] = e2m1x2_to_f16x2<2>(t0), a[1] = e2m1x2_to_f16x2<2>(b0), a[2] = e2m1x2_to_f16x2<3>(t0), a[3] = e2m1x2_to_f16x2<3>(b0);
+                a[4] = e2m1x2_to_f16x2<2>(t1), a[5] = e2m1x2_to_f16x2<2>(b1), a[6] = e2m1x2_to_f16x2<3>(t1), a[7] = e2m1x2_to_f16x2<3>(b1);
             } else {
-                s[g][0] = fmaf(d[0], st, s[g][0]), s[g][1] = fmaf(d[1], st, s[g][1]), s[g][2] = fmaf(d[2], sb, s[g][2]), s[g][3] = fmaf(d[3], sb, s[g][3]);
+                a[0] = e2m1x2_to_f16x2<0>(t0), a[1] = e2m1x2_to_f16x2<0>(b0), a[2] = e2m1x2_to_f16x2<1>(t0), a[3] = e2m1x2_to_f16x2<1>(b0);
+                a[4] = e2m1x2_to_f16x2<0>(t1), a[5] = e2m1x2_to_f16x2<0>(b1), a[6] = e2m1x2_to_f16x2<1>(t1), a[7] = e2m1x2_to_f16x2<1>(b1);
+            }
+            const float *ft = reinterpret_cast<const float*>(f + 16 * gr + row), *fb = reinterpret_cast<const float*>(f + 16 * gr + row + 8u);
+            const float st = ft[blk], sb = fb[blk];
+#pragma unroll
+            for (int g = 0; g < NT; ++g) {
+                float d[4];
+                mma_f16(d, a[0], a[1], a[2], a[3], q[g].x, q[g].y, zero);
+                mma_f16(d, a[4], a[5], a[6], a[7], q[g].z, q[g].w, d);
+                if (blk == 0) {
+                    s[gr][g][0] = d[0] * st, s[gr][g][1] = d[1] * st, s[gr][g][2] = d[2] * sb, s[gr][g][3] = d[3] * sb;
+                } else {
+                    s[gr][g][0] = fmaf(d[0], st, s[gr][g][0]), s[gr][g][1] = fmaf(d[1], st, s[gr][g][1]);
+                    s[gr][g][2] = fmaf(d[2], sb, s[gr][g][2]), s[gr][g][3] = fmaf(d[3], sb, s[gr][g][3]);
+                }
             }
         }
     }
@@ -149,12 +161,14 @@ __device__ __forceinline__ int token_factors(TokenFactors& f, uint32_t kw, uint3
     return e;
 }
 
-template <int NT, unsigned kStages>
+template <int NT>
 struct alignas(128) CtaShared {
-    WarpShared<kStages> warp[kWarps];
+    uint8_t ring[kStages][kTileBytes];
+    TokenFactors f[kWarps];
+    uint4 q[QueryRows<NT>::kShared ? NT * 4 * 32 : 1];
     float m[kWarps][8 * NT], l[kWarps][8 * NT];
     Sums part[kWarps];
-    unsigned long long bars[kWarps][kStages];
+    unsigned long long full[kStages], empty[kStages];
     uint32_t failed;
 };
 
@@ -177,19 +191,30 @@ __device__ const LostPages kNowhere;
 // 32 tokens: scores, softmax, and their part of O
 template <int NT, bool kEdge>
 __device__ __forceinline__ void attend_unit(float (&o)[NT][8][4], float (&m)[NT][2], float (&l)[NT][2], const QueryRows<NT>& x, const uint8_t* k_codes, const uint8_t* v_codes, uint32_t granule,
-                                            const TokenFactors& f, int e, uint32_t tok0) {
+                                            const TokenFactors& f, int e, uint32_t tok0, const uint4* q_shared, float* kept_scores, uint32_t kept_rows, uint32_t length) {
     const unsigned lane = threadIdx.x & 31u, gid = lane >> 2, tig = lane & 3u;
     const uint32_t row = row_token(gid);
     float s[2][NT][4];
+    scores<NT>(s, k_codes, granule, f.k, x, q_shared);
     const float ef = static_cast<float>(e), inv = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
 #pragma unroll
     for (int gr = 0; gr < 2; ++gr) {
-        scores<NT>(s[gr], k_codes + gr * granule, f.k + 16 * gr, x);
 #pragma unroll
         for (int g = 0; g < NT; ++g) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 if (kEdge && tok0 + 16u * gr + 8u * (i >> 1) + row >= x.limit[g][i & 1]) s[gr][g][i] = -INFINITY;
+            }
+        }
+    }
+    if (NT == 1 && kept_scores != nullptr && 2u * tig < kept_rows) {   // for the attention weights: scores in base 2, [token][rows]
+#pragma unroll
+        for (int gr = 0; gr < 2; ++gr) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const uint32_t t = 16u * gr + 8u * i + row;
+                if (kEdge && tok0 + t >= length) continue;
+                *reinterpret_cast<float2*>(kept_scores + t * kept_rows + 2u * tig) = make_float2(s[gr][0][2 * i] * x.factor[0][0], s[gr][0][2 * i + 1] * x.factor[0][1]);
             }
         }
     }
@@ -278,38 +303,37 @@ __device__ __forceinline__ void attend_unit(float (&o)[NT][8][4], float (&m)[NT]
     for (int g = 0; g < NT; ++g) l[g][0] = fmaf(sum[g][0], inv, l[g][0]), l[g][1] = fmaf(sum[g][1], inv, l[g][1]);
 }
 
-template <int NT, unsigned kStages>
-__global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : NT == 2 ? 3 : 2) kv4_attend_kernel(const __grid_constant__ Kv4AttendParams p, uint32_t row_tiles) {
+template <int NT>
+__global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : NT == 2 ? 3 : 2) kv4_attend_kernel(const __grid_constant__ Kv4AttendParams p) {
     extern __shared__ __align__(128) uint8_t smem_raw[];
-    CtaShared<NT, kStages>& sh = *reinterpret_cast<CtaShared<NT, kStages>*>(smem_raw);
+    CtaShared<NT>& sh = *reinterpret_cast<CtaShared<NT>*>(smem_raw);
     const unsigned lane = threadIdx.x & 31u, warp = threadIdx.x >> 5, gid = lane >> 2, tig = lane & 3u;
-    WarpShared<kStages>& mine = sh.warp[warp];
-    const uint32_t bar0 = sm100::smem_u32(&sh.bars[warp][0]);
-    if (lane == 0u) {
-        for (unsigned i = 0; i < kStages; ++i) sm100::mbar_init(bar0 + 8u * i, 1u);
+    const uint32_t full0 = sm100::smem_u32(sh.full), empty0 = sm100::smem_u32(sh.empty), ring0 = sm100::smem_u32(sh.ring[0]);
+    if (threadIdx.x == 0u) {
+        for (unsigned i = 0; i < kStages; ++i) sm100::mbar_init(full0 + 8u * i, 1u), sm100::mbar_init(empty0 + 8u * i, kWarps);
         sm100::fence_mbar_init();
+        sh.failed = 0u;
     }
-    if (threadIdx.x == 0u) sh.failed = 0u;
     pdl_launch();
     pdl_wait();
     __syncthreads();
-    const Deal deal{8u * NT, row_tiles};
+    const Deal deal{8u * NT, 1u};
     const uint32_t all = sum_steps(p, deal, 0u, sh.part).all;
     const uint32_t n_work = workers(all, gridDim.x);
     clear_empty_entries(p, deal);
     if (threadIdx.x == 0u) begun_by(p.ws, blockIdx.x)->last = blockIdx.x;
     if (blockIdx.x >= n_work) return;
-    const uint32_t begin = run_begin(all, n_work, blockIdx.x);
-    const uint32_t end = run_begin(all, n_work, blockIdx.x + 1u);
+    const uint32_t begin = run_begin(all, n_work, blockIdx.x), end = run_begin(all, n_work, blockIdx.x + 1u);
     uint32_t left = end - begin;
     Place at = find_step(p, deal, begin);
-    uint32_t phase_bits = 0;   // parity of each stage's next wait
-    // in the ring a unit is one record of 32 tokens, or two of 16
-    const uint32_t page = 1u << p.c.page_log2, pieces = page == 16u ? 2u : 1u, pages = static_cast<uint32_t>(p.c.pages), page_bytes = static_cast<uint32_t>(p.c.page_bytes);
-    const uint32_t granule = pieces > 1u ? kUnitBytes / 2u : 16u * 64u, v_codes = pieces > 1u ? 1024u : 2048u, v_scales = pieces > 1u ? 64u : 128u;
-    const uint32_t scales_at = pieces > 1u ? (lane >> 4) * (kUnitBytes / 2u) + 2048u + 4u * (lane & 15u) : 4096u + 4u * lane;
+    // where this warp's 32 tokens of a tile lie in a stage: their K codes (the second 16 `granule` bytes on), from there to the V codes, and a lane's scales
+    const uint32_t page = 1u << p.c.page_log2, record_bytes = FMHA_KV4_TOKEN_BYTES << p.c.page_log2, pages = static_cast<uint32_t>(p.c.pages), page_bytes = static_cast<uint32_t>(p.c.page_bytes);
+    const uint32_t in_tile = warp * kUnit, unit_at = (in_tile >> p.c.page_log2) * record_bytes + (in_tile & (page - 1u)) * 64u;
+    const uint32_t granule = page == 16u ? record_bytes : 1024u, v_codes = 64u * page;
+    const uint32_t my_token = in_tile + lane, scales_at = (my_token >> p.c.page_log2) * record_bytes + 128u * page + (my_token & (page - 1u)) * 4u, v_scales = 4u * page;
     const uint8_t* nowhere = page == 16u ? kNowhere.p16.bytes : page == 32u ? kNowhere.p32.bytes : page == 64u ? kNowhere.p64.bytes : kNowhere.p128.bytes;
-    const uint32_t ring0 = sm100::smem_u32(mine.ring[0]);
+    const uint32_t kept_rows = (p.S * p.group + 1u) & ~1u;
+    uint32_t tile = 0;   // of this CTA so far: stage tile % kStages, phase tile / kStages of its barriers
 
     while (left > 0u) {
         const uint32_t pos = end - left;
@@ -317,17 +341,38 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : NT == 2 ? 3 : 2) kv4_a
         if (threadIdx.x == 0u && seg.first == 0u && seg.steps < seg.of) *begun_by(p.ws, blockIdx.x) = {seg.b, seg.head, seg.row0, worker_at(all, n_work, pos + seg.of - 1u)};
         const uint32_t b = seg.b, head = seg.head, row0 = seg.row0, first = seg.first, n_tiles = seg.steps;
         const uint32_t length = length_of(p.c, b), n_rows = count_of(p.counts, b, p.S, length);
+        const int32_t* row_of_table = p.c.table + static_cast<size_t>(b) * p.c.table_width;
+        const uint8_t* heads = p.c.pool + static_cast<size_t>(head) * record_bytes;
+        // The copies of tile i of the segment: lane r brings the tile's r-th record; its page was looked up when the warp last had its turn
+        int id = 0;
+        auto look_up = [&](uint32_t i) {
+            const uint32_t t = (first + i) * kTile + lane * page;
+            if (i < n_tiles && lane * page < kTile && t < length) id = ld_i32(row_of_table + (t >> p.c.page_log2));
+        };
+        auto issue = [&](uint32_t i) {
+            const uint32_t stage = (tile + i) % kStages, t = (first + i) * kTile, records = min(max(kTile >> p.c.page_log2, 1u), (length - t + page - 1u) >> p.c.page_log2);
+            if (lane == 0u) sm100::mbar_arrive_expect_tx(full0 + 8u * stage, records * record_bytes);
+            __syncwarp();
+            if (lane < records) {
+                const uint8_t* rec = static_cast<uint32_t>(id) < pages ? heads + static_cast<uint64_t>(static_cast<uint32_t>(id)) * page_bytes : nowhere;
+                bulk_load(ring0 + stage * kTileBytes + lane * record_bytes, rec, record_bytes, full0 + 8u * stage);
+            }
+        };
+        // warp w issues the tiles w, w + 4, ...; at the start of a segment the ring is empty
+        look_up(warp);
+        if (warp < kStages - 1u && warp < n_tiles) {
+            issue(warp);
+            look_up(warp + kWarps);
+        }
         QueryRows<NT> x;
-        load_rows<NT>(x, p, b, head, row0, length, n_rows);
+        load_rows<NT>(x, sh.q, p, b, head, row0, length, n_rows);
         uint32_t low = 0xFFFFFFFFu;   // tokens that every live column sees
 #pragma unroll
         for (int g = 0; g < NT; ++g) {
 #pragma unroll
             for (int j = 0; j < 2; ++j) low = min(low, x.limit[g][j] == 0u ? 0xFFFFFFFFu : x.limit[g][j]);
         }
-        low = min(low, __shfl_xor_sync(0xFFFFFFFFu, low, 1));
-        low = min(low, __shfl_xor_sync(0xFFFFFFFFu, low, 2));
-        low = min(low, length);
+        low = min(__reduce_min_sync(0xFFFFFFFFu, low), length);
 
         float o[NT][8][4], m[NT][2], l[NT][2];
 #pragma unroll
@@ -337,71 +382,40 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : NT == 2 ? 3 : 2) kv4_a
 #pragma unroll
             for (int i = 0; i < 8; ++i) o[g][i][0] = o[g][i][1] = o[g][i][2] = o[g][i][3] = 0.0f;
         }
-        const uint32_t t_first = first * kTile + warp * kUnit;
-        const uint32_t units = t_first >= length ? 0u : min(n_tiles, (length - t_first + kTile - 1u) / kTile);
-        // pages of the unit that is copied next, looked up one unit ahead; lane 0 issues
-        const int32_t* row_of_table = p.c.table + static_cast<size_t>(b) * p.c.table_width;
-        const uint8_t* heads = p.c.pool + (static_cast<size_t>(head) * FMHA_KV4_TOKEN_BYTES << p.c.page_log2);
-        int id0 = 0, id1 = 0;
-        auto look_up = [&](uint32_t u) {
-            const uint32_t t = t_first + u * kTile;
-            if (u < units) {
-                id0 = ld_i32(row_of_table + (t >> p.c.page_log2));
-                if (pieces > 1u && t + 16u < length) id1 = ld_i32(row_of_table + (t >> 4) + 1u);
-            }
-        };
-        auto record = [&](int id) {
-            return static_cast<uint32_t>(id) < pages ? heads + static_cast<uint64_t>(static_cast<uint32_t>(id)) * page_bytes : nowhere;
-        };
-        auto issue = [&](uint32_t u) {
-            if (u < units && lane == 0u) {
-                const uint32_t st = u % kStages, bar = bar0 + 8u * st, t = t_first + u * kTile, dst = ring0 + st * kUnitBytes;
-                const uint8_t* rec = record(id0);
-                if (pieces > 1u) {
-                    const bool two = t + 16u < length;
-                    sm100::mbar_arrive_expect_tx(bar, two ? kUnitBytes : kUnitBytes / 2u);
-                    bulk_load(dst, rec, kUnitBytes / 2u, bar);
-                    if (two) bulk_load(dst + kUnitBytes / 2u, record(id1), kUnitBytes / 2u, bar);
-                } else {
-                    sm100::mbar_arrive_expect_tx(bar, kUnitBytes);
-                    if (page == kUnit) {
-                        bulk_load(dst, rec, kUnitBytes, bar);
-                    } else {   // 32 tokens out of a longer page: its four parts
-                        const uint32_t slot = t & (page - 1u);
-                        bulk_load(dst, rec + 64u * slot, 64u * kUnit, bar);
-                        bulk_load(dst + 64u * kUnit, rec + 64u * (page + slot), 64u * kUnit, bar);
-                        bulk_load(dst + 128u * kUnit, rec + 128u * page + 4u * slot, 4u * kUnit, bar);
-                        bulk_load(dst + 132u * kUnit, rec + 132u * page + 4u * slot, 4u * kUnit, bar);
-                    }
-                }
-            }
-        };
-        look_up(0);
-#pragma unroll
-        for (unsigned u = 0; u < kStages - 1u; ++u) {
-            issue(u);
-            look_up(u + 1u);
-        }
         bool ok = true;
-        for (uint32_t u = 0, st = 0; u < units; ++u, st = st + 1u == kStages ? 0u : st + 1u) {
-            issue(u + kStages - 1u);
-            look_up(u + kStages);
-            const uint32_t tok0 = t_first + u * kTile;
-            if (!sm100::mbar_wait(bar0 + 8u * st, (phase_bits >> st) & 1u, &sh.failed)) {
+        for (uint32_t i = 0; i < n_tiles; ++i) {
+            const uint32_t stage = (tile + i) % kStages, parity = ((tile + i) / kStages) & 1u, tok0 = (first + i) * kTile + in_tile;
+            if (!sm100::mbar_wait(full0 + 8u * stage, parity, &sh.failed)) {
                 ok = false;
                 break;
             }
-            phase_bits ^= 1u << st;
-            const uint8_t* raw = mine.ring[0] + st * kUnitBytes;
-            const int e = token_factors(mine.f, *reinterpret_cast<const uint32_t*>(raw + scales_at), *reinterpret_cast<const uint32_t*>(raw + scales_at + v_scales), tok0 + lane < length);
-            __syncwarp();
-            if (tok0 + kUnit <= low) {
-                attend_unit<NT, false>(o, m, l, x, raw, raw + v_codes, granule, mine.f, e, tok0);
-            } else {
-                attend_unit<NT, true>(o, m, l, x, raw, raw + v_codes, granule, mine.f, e, tok0);
+            if (tok0 < length) {
+                const uint8_t* raw = sh.ring[stage];
+                const int e = token_factors(sh.f[warp], *reinterpret_cast<const uint32_t*>(raw + scales_at), *reinterpret_cast<const uint32_t*>(raw + scales_at + v_scales), tok0 + lane < length);
+                __syncwarp();
+                const uint8_t* codes = raw + unit_at;
+                float* kept = p.scores == nullptr ? nullptr : p.scores + ((static_cast<size_t>(b) * p.c.HK + head) * (static_cast<size_t>(p.c.table_width) << p.c.page_log2) + tok0) * kept_rows;
+                if (tok0 + kUnit <= low) {
+                    attend_unit<NT, false>(o, m, l, x, codes, codes + v_codes, granule, sh.f[warp], e, tok0, sh.q, kept, kept_rows, length);
+                } else {
+                    attend_unit<NT, true>(o, m, l, x, codes, codes + v_codes, granule, sh.f[warp], e, tok0, sh.q, kept, kept_rows, length);
+                }
             }
-            __syncwarp();   // the stage and the factors are free again
+            __syncwarp();   // this warp is done with the stage and its factors
+            if (lane == 0u) sm100::mbar_arrive(empty0 + 8u * stage);
+            // its turn to bring the tile after the next, into the stage of the tile before this one
+            const uint32_t ahead = i + kStages - 1u;
+            if (ahead % kWarps == warp && ahead < n_tiles) {
+                const uint32_t before = tile + ahead;   // (the stage's last tile but one phase)
+                if (before >= kStages && !sm100::mbar_wait(empty0 + 8u * (before % kStages), (before / kStages - 1u) & 1u, &sh.failed)) {
+                    ok = false;
+                    break;
+                }
+                issue(ahead);
+                look_up(ahead + kWarps);
+            }
         }
+        tile += n_tiles;
         if (!ok) {
             if (lane == 0u) atomicOr(p.status, 1u);
         }
@@ -424,7 +438,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : NT == 2 ? 3 : 2) kv4_a
         float* part = slot_of(p.ws, gridDim.x, blockIdx.x, slot, 8u * NT);
 #pragma unroll
         for (int g = 0; g < NT; ++g) {
-            float* mine_o = reinterpret_cast<float*>(mine.ring[0]);   // [8 rows][128], the ring is empty
+            float* mine_o = reinterpret_cast<float*>(sh.ring[0]) + warp * 1024u;   // [8 rows][128], the ring is empty
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
                 const int row = 8 * g + 2 * static_cast<int>(tig) + j;
@@ -446,7 +460,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : NT == 2 ? 3 : 2) kv4_a
 #pragma unroll
                 for (unsigned w = 0; w < kWarps; ++w) {
                     total = fmaf(sh.l[w][8 * g + r], ex2(sh.m[w][8 * g + r] - top), total);
-                    const float4* src = reinterpret_cast<const float4*>(reinterpret_cast<const float*>(sh.warp[w].ring[0]) + r * 128u + d);
+                    const float4* src = reinterpret_cast<const float4*>(reinterpret_cast<const float*>(sh.ring[0]) + w * 1024u + r * 128u + d);
                     const float4 a = src[0], c = src[1];
                     acc[0] += a.x, acc[1] += a.y, acc[2] += a.z, acc[3] += a.w, acc[4] += c.x, acc[5] += c.y, acc[6] += c.z, acc[7] += c.w;
                 }
@@ -535,133 +549,70 @@ __global__ void __launch_bounds__(kThreads) kv4_combine_kernel(const __grid_cons
     if (p.lse != nullptr && lane == 0u) p.lse[(static_cast<size_t>(b) * p.H + h) * p.S + i] = none ? -INFINITY : (m + lg2(l)) * kLn2;
 }
 
-// The attention weights that the cached tokens received: p = 2^(s - lse), summed over the rows and the group's heads. A warp has 32 tokens and goes over all rows, in
-// order, so that the sums are the same every time.
-__global__ void __launch_bounds__(kThreads) kv4_weigh_kernel(const __grid_constant__ Kv4AttendParams p, uint32_t tiles) {
-    __shared__ __align__(16) float4 factors[kWarps][kUnit];
-    __shared__ __align__(16) uint8_t codes[kWarps][kUnit * 64u];
-    pdl_launch();
-    pdl_wait();
-    const unsigned lane = threadIdx.x & 31u, warp = threadIdx.x >> 5, gid = lane >> 2, tig = lane & 3u;
-    const uint32_t bh = blockIdx.x / tiles, head = bh % p.c.HK, b = bh / p.c.HK, tok0 = (blockIdx.x % tiles * kWarps + warp) * kUnit;
-    const uint32_t length = length_of(p.c, b), n = count_of(p.counts, b, p.S, length), page = 1u << p.c.page_log2;
-    if (tok0 >= length) return;
-    {
-        // a lane brings its token's 64 bytes and factors
-        const uint32_t t = tok0 + lane;
-        const long long id = t < length ? page_of(p.c, b, t) : -1;
-        float4 k = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        if (id >= 0) {
-            const uint8_t* rec = record_of(p.c, id, head);
-            const uint32_t slot = t & (page - 1u), kw = ld_u32(rec + 128u * page + 4u * slot);
-            k = make_float4(scale_f32(kw, 0), scale_f32(kw, 1), scale_f32(kw, 2), scale_f32(kw, 3));
-#pragma unroll
-            for (int i = 0; i < 4; ++i) *reinterpret_cast<uint4*>(&codes[warp][64u * lane + 16u * i]) = ld_v4(rec + 64u * slot + 16u * i);
-        } else {
-            k.x = __uint_as_float(0x7FC00000u);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) *reinterpret_cast<uint4*>(&codes[warp][64u * lane + 16u * i]) = make_uint4(0u, 0u, 0u, 0u);
-        }
-        factors[warp][lane] = k;
-    }
-    __syncwarp();
-    float sum[2][2] = {{0.0f, 0.0f}, {0.0f, 0.0f}};
-    const uint32_t rows = n * p.group;
-    for (uint32_t row0 = 0; row0 < rows; row0 += 8u) {
-        if (p.causal && length - n + (row0 + 7u) / p.group < tok0) continue;   // (uniform: no row of the eight sees the tokens)
-        QueryRows<1> x;
-        load_rows<1>(x, p, b, head, row0, length, n);
-        float lse2[2];
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            const uint32_t row = row0 + 2u * tig + j;
-            lse2[j] = row < rows ? ld_f32(p.lse + (static_cast<size_t>(b) * p.H + head * p.group + row % p.group) * p.S + row / p.group) * kLog2e : 0.0f;
-        }
-#pragma unroll
-        for (int gr = 0; gr < 2; ++gr) {
-            float s[1][4];
-            scores<1>(s, &codes[warp][1024u * gr], &factors[warp][16 * gr], x);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const bool seen = tok0 + 16u * gr + 8u * (i >> 1) + row_token(gid) < x.limit[0][i & 1];
-                const float w = ex2(fmaf(s[0][i], x.factor[0][i & 1], -lse2[i & 1]));
-                sum[gr][i >> 1] += seen ? w : 0.0f;
-            }
-        }
-    }
-#pragma unroll
-    for (int gr = 0; gr < 2; ++gr) {
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            float v = sum[gr][k];
-            v += __shfl_xor_sync(0xFFFFFFFFu, v, 1);
-            v += __shfl_xor_sync(0xFFFFFFFFu, v, 2);
-            const uint32_t t = tok0 + 16u * gr + 8u * k + row_token(gid);
-            if (tig == 0u && t < length) {
-                const size_t at = static_cast<size_t>(bh) * p.weights_width + t;
-                const bool old = p.weights_in != nullptr && (!p.causal || t < length - n);
-                p.weights[at] = (old ? ld_f32(p.weights_in + at) : 0.0f) + v;
-            }
-        }
-    }
-}
-
-constexpr unsigned kStages1 = 3;
 constexpr uint32_t kMostFew = 32;   // rows of a KV head from which on the tensor cores' tiles of 128 rows take over
 
-uint32_t groups_of(uint32_t rows) { return rows <= 8u ? 1u : rows <= 16u ? 2u : 4u; }
+uint32_t groups_of(uint32_t rows) { return (rows + 7u) / 8u; }
 
-uint32_t attend_grid(const Kv4View& c, uint32_t row_tiles) {
-    const unsigned long long tiles = ((static_cast<unsigned long long>(c.table_width) << c.page_log2) + kTile - 1u) / kTile;
-    const unsigned long long most = tiles * c.B * c.HK * row_tiles, full = static_cast<unsigned long long>(kCtasPerSm) * static_cast<unsigned long long>(current_sm_count());
+uint32_t attend_grid(const Kv4View& c, uint32_t groups) {
+    const unsigned long long tiles = ((static_cast<unsigned long long>(c.table_width) << c.page_log2) + kTile - 1u) / kTile, per_sm = groups == 1u ? 4u : groups == 2u ? 3u : 2u;
+    const unsigned long long most = tiles * c.B * c.HK, full = per_sm * static_cast<unsigned long long>(current_sm_count());
     return static_cast<uint32_t>(most < full ? (most ? most : 1ull) : full);
 }
 
 template <int NT>
-cudaError_t launch_rows(const Kv4AttendParams& p, uint32_t row_tiles, cudaStream_t stream) {
-    const uint32_t grid = attend_grid(p.c, row_tiles);
-    const size_t smem = sizeof(CtaShared<NT, kStages1>);
+cudaError_t launch_rows(const Kv4AttendParams& p, cudaStream_t stream) {
+    const uint32_t grid = attend_grid(p.c, NT), rows = p.S * p.group;
+    const size_t smem = sizeof(CtaShared<NT>);
     static std::atomic<bool> set[64];
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
     if (dev < 0 || dev >= 64 || !set[dev].load(std::memory_order_relaxed)) {
-        e = cudaFuncSetAttribute(kv4_attend_kernel<NT, kStages1>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+        e = cudaFuncSetAttribute(kv4_attend_kernel<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
         if (e != cudaSuccess) return e;
         if (dev >= 0 && dev < 64) set[dev].store(true, std::memory_order_relaxed);
     }
-    e = kv4_launch(kv4_attend_kernel<NT, kStages1>, dim3(grid), kThreads, smem, stream, p, row_tiles);
+    e = kv4_launch(kv4_attend_kernel<NT>, dim3(grid), kThreads, smem, stream, p);
     if (e != cudaSuccess) return e;
-    return kv4_launch(kv4_combine_kernel<true>, dim3(grid, p.S * p.group < 8u * NT ? p.S * p.group : 8u * NT), kThreads, 0, stream, p, 8u * NT);
+    return kv4_launch(kv4_combine_kernel<true>, dim3(grid, rows < 8u * NT ? rows : 8u * NT), kThreads, 0, stream, p, 8u * NT);
+}
+
+cudaError_t launch_many(const Kv4AttendParams& p, cudaStream_t stream) {
+    const uint32_t rows = p.S * p.group, per = kv4_prefill_rows(), row_tiles = (rows + per - 1u) / per, most = rows < per ? rows : per;
+    const cudaError_t e = launch_kv4_prefill(p, row_tiles, stream);
+    if (e != cudaSuccess) return e;
+    return kv4_launch(kv4_combine_kernel<false>, dim3(kv4_prefill_grid(), (most + kWarps - 1u) / kWarps), kThreads, 0, stream, p, per);
 }
 
 uint64_t partial_bytes(const Kv4View& c, uint32_t rows) {
     if (rows > kMostFew) return kv4_partial_bytes(kv4_prefill_grid(), kv4_prefill_rows());
-    return kv4_partial_bytes(attend_grid(c, 1u), 8u * groups_of(rows));
+    return kv4_partial_bytes(attend_grid(c, groups_of(rows)), 8u * groups_of(rows));
 }
-
-cudaError_t launch_many(const Kv4AttendParams& p, cudaStream_t stream) {
-    const uint32_t rows = p.S * p.group, row_tiles = (rows + kv4_prefill_rows() - 1u) / kv4_prefill_rows();
-    const cudaError_t e = launch_kv4_prefill(p, row_tiles, stream);
-    if (e != cudaSuccess) return e;
-    const uint32_t most = rows < kv4_prefill_rows() ? rows : kv4_prefill_rows();
-    return kv4_launch(kv4_combine_kernel<false>, dim3(kv4_prefill_grid(), (most + kWarps - 1u) / kWarps), kThreads, 0, stream, p, kv4_prefill_rows());
+uint64_t lse_bytes(const Kv4View& c, uint32_t S, uint32_t H) { return (static_cast<uint64_t>(c.B) * S * H * 4u + 15u) & ~15ull; }
+// Up to 8 rows leave their scores for the weights, at 4 bytes a row and token; with more it costs less to compute them again
+uint64_t score_bytes(const Kv4View& c, uint32_t rows) {
+    return rows > 8u ? 0u : (static_cast<uint64_t>(c.B) * c.HK * c.table_width << c.page_log2) * ((rows + 1u) & ~1u) * 4u;
 }
 
 }  // namespace
 
 uint64_t kv4_attend_workspace(const Kv4View& c, uint32_t S, uint32_t H, bool weights, bool lse) {
-    return partial_bytes(c, S * (H / c.HK)) + (weights && !lse ? static_cast<uint64_t>(c.B) * S * H * 4u : 0u);
+    const uint32_t rows = S * (H / c.HK);
+    return partial_bytes(c, rows) + (weights ? score_bytes(c, rows) + (lse ? 0u : lse_bytes(c, S, H)) : 0u);
 }
 
 cudaError_t launch_kv4_attend(const Kv4AttendParams& params, cudaStream_t stream) {
     Kv4AttendParams p = params;
-    const uint32_t rows = p.S * p.group, nt = groups_of(rows);
-    if (p.weights != nullptr && p.lse == nullptr) p.lse = p.ws + partial_bytes(p.c, rows) / 4u;   // the weights go by the rows' log-sum-exps
-    cudaError_t e = rows > kMostFew ? launch_many(p, stream) : nt == 1u ? launch_rows<1>(p, 1u, stream) : nt == 2u ? launch_rows<2>(p, 1u, stream) : launch_rows<4>(p, 1u, stream);
-    if (e != cudaSuccess || p.weights == nullptr) return e;
-    const uint32_t tiles = ((p.c.table_width << p.c.page_log2) + kTile - 1u) / kTile;
-    return kv4_launch(kv4_weigh_kernel, dim3(tiles * p.c.B * p.c.HK), kThreads, 0, stream, p, tiles);
+    const uint32_t rows = p.S * p.group;
+    p.scores = nullptr;
+    if (p.weights != nullptr) {   // the weights go by the rows' log-sum-exps
+        uint8_t* more = reinterpret_cast<uint8_t*>(p.ws) + partial_bytes(p.c, rows);
+        if (rows <= 8u) p.scores = reinterpret_cast<float*>(more);
+        if (p.lse == nullptr) p.lse = reinterpret_cast<float*>(more + score_bytes(p.c, rows));
+    }
+    const uint32_t groups = groups_of(rows);
+    const cudaError_t e = rows > kMostFew ? launch_many(p, stream) : groups == 1u ? launch_rows<1>(p, stream) : groups == 2u ? launch_rows<2>(p, stream) : groups == 3u ? launch_rows<3>(p, stream) : launch_rows<4>(p, stream);
+    return e != cudaSuccess || p.weights == nullptr ? e : launch_kv4_weigh(p, stream);
 }
 
 }  // namespace b200mx

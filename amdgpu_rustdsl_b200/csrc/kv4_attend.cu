@@ -30,7 +30,9 @@ constexpr unsigned kWarps = 4, kThreads = kWarps * 32;
 constexpr unsigned kUnit = 32;                    // tokens of a warp at a time
 constexpr unsigned kTile = kWarps * kUnit;
 static_assert(kTile == kStepTokens, "a step is a tile");
-constexpr unsigned kStages = 3, kTileBytes = kTile * FMHA_KV4_TOKEN_BYTES;
+constexpr unsigned kStages = 3;                    // (a segment's first kStages - 1 tiles are brought by a warp each)
+static_assert(kStages - 1 <= kWarps, "a warp for each of the first tiles");
+constexpr unsigned kTileBytes = kTile * FMHA_KV4_TOKEN_BYTES;
 constexpr float kSlack = 4.0f;
 constexpr float kLeast = 1e-37f;                  // of a row's factor: times a masked score it is still -inf
 constexpr float kLn2 = 0.69314718055994531f;
@@ -333,7 +335,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : NT == 2 ? 3 : 2) kv4_a
     const uint32_t my_token = in_tile + lane, scales_at = (my_token >> p.c.page_log2) * record_bytes + 128u * page + (my_token & (page - 1u)) * 4u, v_scales = 4u * page;
     const uint8_t* nowhere = page == 16u ? kNowhere.p16.bytes : page == 32u ? kNowhere.p32.bytes : page == 64u ? kNowhere.p64.bytes : kNowhere.p128.bytes;
     const uint32_t kept_rows = (p.S * p.group + 1u) & ~1u;
-    uint32_t tile = 0;   // of this CTA so far: stage tile % kStages, phase tile / kStages of its barriers
+    uint32_t stage = 0, phase = 0, filled = 0;   // of the next tile: its stage and the parity of the stage's barriers; tiles so far
 
     while (left > 0u) {
         const uint32_t pos = end - left;
@@ -349,19 +351,19 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : NT == 2 ? 3 : 2) kv4_a
             const uint32_t t = (first + i) * kTile + lane * page;
             if (i < n_tiles && lane * page < kTile && t < length) id = ld_i32(row_of_table + (t >> p.c.page_log2));
         };
-        auto issue = [&](uint32_t i) {
-            const uint32_t stage = (tile + i) % kStages, t = (first + i) * kTile, records = min(max(kTile >> p.c.page_log2, 1u), (length - t + page - 1u) >> p.c.page_log2);
-            if (lane == 0u) sm100::mbar_arrive_expect_tx(full0 + 8u * stage, records * record_bytes);
+        auto issue = [&](uint32_t i, uint32_t into) {
+            const uint32_t t = (first + i) * kTile, records = min(max(kTile >> p.c.page_log2, 1u), (length - t + page - 1u) >> p.c.page_log2);
+            if (lane == 0u) sm100::mbar_arrive_expect_tx(full0 + 8u * into, records * record_bytes);
             __syncwarp();
             if (lane < records) {
                 const uint8_t* rec = static_cast<uint32_t>(id) < pages ? heads + static_cast<uint64_t>(static_cast<uint32_t>(id)) * page_bytes : nowhere;
-                bulk_load(ring0 + stage * kTileBytes + lane * record_bytes, rec, record_bytes, full0 + 8u * stage);
+                bulk_load(ring0 + into * kTileBytes + lane * record_bytes, rec, record_bytes, full0 + 8u * into);
             }
         };
         // warp w issues the tiles w, w + 4, ...; at the start of a segment the ring is empty
         look_up(warp);
         if (warp < kStages - 1u && warp < n_tiles) {
-            issue(warp);
+            issue(warp, (stage + warp) % kStages);
             look_up(warp + kWarps);
         }
         QueryRows<NT> x;
@@ -382,10 +384,11 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : NT == 2 ? 3 : 2) kv4_a
 #pragma unroll
             for (int i = 0; i < 8; ++i) o[g][i][0] = o[g][i][1] = o[g][i][2] = o[g][i][3] = 0.0f;
         }
+        float* kept = p.scores == nullptr ? nullptr : p.scores + ((static_cast<size_t>(b) * p.c.HK + head) * (static_cast<size_t>(p.c.table_width) << p.c.page_log2) + first * kTile + in_tile) * kept_rows;
         bool ok = true;
-        for (uint32_t i = 0; i < n_tiles; ++i) {
-            const uint32_t stage = (tile + i) % kStages, parity = ((tile + i) / kStages) & 1u, tok0 = (first + i) * kTile + in_tile;
-            if (!sm100::mbar_wait(full0 + 8u * stage, parity, &sh.failed)) {
+        uint32_t tok0 = first * kTile + in_tile, my_turn = (warp + 2u * kWarps - (kStages - 1u)) % kWarps;   // tiles until this warp brings one
+        for (uint32_t i = 0; i < n_tiles; ++i, tok0 += kTile) {
+            if (!sm100::mbar_wait(full0 + 8u * stage, phase, &sh.failed)) {
                 ok = false;
                 break;
             }
@@ -394,28 +397,31 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : NT == 2 ? 3 : 2) kv4_a
                 const int e = token_factors(sh.f[warp], *reinterpret_cast<const uint32_t*>(raw + scales_at), *reinterpret_cast<const uint32_t*>(raw + scales_at + v_scales), tok0 + lane < length);
                 __syncwarp();
                 const uint8_t* codes = raw + unit_at;
-                float* kept = p.scores == nullptr ? nullptr : p.scores + ((static_cast<size_t>(b) * p.c.HK + head) * (static_cast<size_t>(p.c.table_width) << p.c.page_log2) + tok0) * kept_rows;
                 if (tok0 + kUnit <= low) {
-                    attend_unit<NT, false>(o, m, l, x, codes, codes + v_codes, granule, sh.f[warp], e, tok0, sh.q, kept, kept_rows, length);
+                    attend_unit<NT, false>(o, m, l, x, codes, codes + v_codes, granule, sh.f[warp], e, tok0, sh.q, kept == nullptr ? nullptr : kept + i * kTile * kept_rows, kept_rows, length);
                 } else {
-                    attend_unit<NT, true>(o, m, l, x, codes, codes + v_codes, granule, sh.f[warp], e, tok0, sh.q, kept, kept_rows, length);
+                    attend_unit<NT, true>(o, m, l, x, codes, codes + v_codes, granule, sh.f[warp], e, tok0, sh.q, kept == nullptr ? nullptr : kept + i * kTile * kept_rows, kept_rows, length);
                 }
             }
             __syncwarp();   // this warp is done with the stage and its factors
             if (lane == 0u) sm100::mbar_arrive(empty0 + 8u * stage);
-            // its turn to bring the tile after the next, into the stage of the tile before this one
-            const uint32_t ahead = i + kStages - 1u;
-            if (ahead % kWarps == warp && ahead < n_tiles) {
-                const uint32_t before = tile + ahead;   // (the stage's last tile but one phase)
-                if (before >= kStages && !sm100::mbar_wait(empty0 + 8u * (before % kStages), (before / kStages - 1u) & 1u, &sh.failed)) {
-                    ok = false;
-                    break;
+            // its turn to bring the tile kStages - 1 tiles on, into the stage of the tile before this one
+            const uint32_t ahead = i + kStages - 1u, into = stage == 0u ? kStages - 1u : stage - 1u;
+            if (my_turn-- == 0u) {
+                my_turn = kWarps - 1u;
+                if (ahead < n_tiles) {
+                    // (the tile before this one has the phase before this stage's, or this stage's where it lies behind it; a stage's first tile finds it empty)
+                    if (filled + i > 0u && !sm100::mbar_wait(empty0 + 8u * into, stage == 0u ? phase ^ 1u : phase, &sh.failed)) {
+                        ok = false;
+                        break;
+                    }
+                    issue(ahead, into);
+                    look_up(ahead + kWarps);
                 }
-                issue(ahead);
-                look_up(ahead + kWarps);
             }
+            if (++stage == kStages) stage = 0u, phase ^= 1u;
         }
-        tile += n_tiles;
+        filled += n_tiles;
         if (!ok) {
             if (lane == 0u) atomicOr(p.status, 1u);
         }

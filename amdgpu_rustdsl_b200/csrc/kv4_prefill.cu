@@ -40,12 +40,11 @@ constexpr float kLeast = 1e-37f;   // times a masked score it is still -inf
 constexpr float kLn2 = 0.69314718055994531f;
 
 // barriers; kPFull by 2 q + half
-enum Bar : uint32_t { kKFull = 0, kKEmpty = 2, kVFull = 4, kVEmpty = 6, kSFull = 8, kODone = 10, kPFull = 12, kOFree = 16, kQFull = 18, kQEmpty = 20, kDrained = 21, kEFull = 23, kBars = 23 + kFactorSlots };
+enum Bar : uint32_t { kKFull = 0, kKEmpty = 2, kVFull = 4, kVEmpty = 6, kSFull = 8, kODone = 10, kPFull = 12, kOFree = 16, kQFull = 18, kQEmpty = 20, kTurn = 22, kDrained = 24, kEFull = 26, kBars = 26 + kFactorSlots };
 
 struct Shared {
     uint8_t q[2][kTileBytes], k[kStages][kTileBytes], v[kStages][kTileBytes];
     uint4 most[kFactorSlots][2];   // the largest scale byte of K and of V that each of the converting warps met
-    float q_factor[2][kItemRows];  // the powers of two that were taken out of the rows, of even and of odd segments
     unsigned long long bars[kBars];
     Sums part[kThreads / 32];
     uint32_t tmem, failed, not_drained;
@@ -106,11 +105,12 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
         for (uint32_t i = 0; i < 2; ++i) {
             mbar_init(bar(kKFull + i), 128u), mbar_init(bar(kVFull + i), 128u);
             mbar_init(bar(kKEmpty + i), 2u), mbar_init(bar(kVEmpty + i), 2u), mbar_init(bar(kOFree + i), 4u);
-            mbar_init(bar(kSFull + i), 1u), mbar_init(bar(kODone + i), 1u);
+            mbar_init(bar(kSFull + i), 1u), mbar_init(bar(kODone + i), 1u), mbar_init(bar(kQFull + i), 4u), mbar_init(bar(kQEmpty + i), 1u);
+            mbar_init(bar(kTurn + i), 1u), mbar_init(bar(kDrained + i), 1u);
         }
         for (uint32_t i = 0; i < 4; ++i) mbar_init(bar(kPFull + i), 4u);
         for (uint32_t i = 0; i < kFactorSlots; ++i) mbar_init(bar(kEFull + i), 4u);
-        mbar_init(bar(kQFull), 128u), mbar_init(bar(kQFull + 1u), 128u), mbar_init(bar(kQEmpty), 2u), mbar_init(bar(kDrained), 1u), mbar_init(bar(kDrained + 1u), 1u);
+        
         fence_mbar_init();
         sh.failed = sh.not_drained = 0u;
     }
@@ -136,20 +136,54 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
             asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
             const uint32_t q = warp >> 2, r = threadIdx.x & 127u, lanes = (warp & 3u) << 21;   // 32 TMEM lanes per warp, in bits 16 and up
             const uint32_t t_s = tmem + lanes + kColS + 128u * q, t_o = tmem + lanes + kColO + 128u * q;
-            uint32_t s_phase = 0, o_phase = 0, step0 = 0, segment = 0;   // step0, segment: steps and segments in front of this one
+            uint32_t s_phase = 0, o_phase = 0, q_phase = 1, step0 = 0;   // step0: steps in front of the segment
             bool ok = true;
-            for (; left > 0u && ok; ++segment) {
-                const uint32_t pos = end - left;
-                const Segment seg = next_segment(p, deal, at, left);
+            // The query rows, a thread its own: asked for while the last products of the segment before are under way, kept in registers over its epilogue
+            uint4 raw[16];
+            auto ask_rows = [&](const Segment& seg, uint32_t n) {
+                const uint32_t row = seg.row0 + q * kTileRows + r, i = row / p.group;
+                const uint8_t* src = p.q.data + seg.b * p.q.stride_b + i * p.q.stride_s + (seg.head * p.group + row % p.group) * p.q.stride_h;
+#pragma unroll
+                for (int x = 0; x < 16; ++x) raw[x] = i < n ? ld_v4(src + 16 * x) : make_uint4(0u, 0u, 0u, 0u);
+            };
+            Segment seg;
+            uint32_t pos, length, n;
+            auto next = [&]() {
+                pos = end - left;
+                seg = next_segment(p, deal, at, left);
+                length = length_of(p.c, seg.b), n = count_of(p.counts, seg.b, p.S, length);
+                ask_rows(seg, n);
+            };
+            next();
+            for (bool more = true; more && ok;) {
                 if (threadIdx.x == 0u && seg.first == 0u && seg.steps < seg.of) *begun_by(p.ws, blockIdx.x) = {seg.b, seg.head, seg.row0, worker_at(all, n_work, pos + seg.of - 1u)};
-                const uint32_t length = length_of(p.c, seg.b), n = count_of(p.counts, seg.b, p.S, length);
                 const uint32_t steps = tile_steps(p, seg, q, length, n), row = seg.row0 + q * kTileRows + r, i = row / p.group;
                 const bool exists = row < p.S * p.group, live = exists && i < n;
                 const uint32_t limit = !live ? 0u : p.causal ? length - n + i + 1u : length;
-                float m = kLowest, l = 0.0f, c_row = 0.0f;
-                if (steps > 0u) {   // (slots of their own for even and odd segments: while this group stores the rows of the one before, the next but one cannot have come)
-                    ok = mbar_wait(bar(kQFull + (segment & 1u)), segment >> 1 & 1u, failed);
-                    c_row = p.scale_log2 * sh.q_factor[segment & 1u][q * kTileRows + r];
+                float m = kLowest, l = 0.0f, c_row;
+                {
+                    uint32_t amax = 0;
+#pragma unroll
+                    for (int x = 0; x < 16; ++x) {
+                        const uint32_t w[4] = {raw[x].x, raw[x].y, raw[x].z, raw[x].w};
+#pragma unroll
+                        for (int y = 0; y < 4; ++y) amax = max(amax, max((w[y] << 16) & 0x7FFFFFFFu, w[y] & 0x7FFF0000u));
+                    }
+                    const float2 f = row_factors(amax);
+                    c_row = p.scale_log2 * f.y;
+                    ok = mbar_wait(bar(kQEmpty + q), q_phase, failed);   // S of the segment before is done with its rows
+                    if (!ok) break;
+                    q_phase ^= 1u;
+#pragma unroll
+                    for (uint32_t x = 0; x < 16u; ++x) {
+                        uint32_t w[4] = {raw[x].x, raw[x].y, raw[x].z, raw[x].w};
+#pragma unroll
+                        for (int y = 0; y < 4; ++y) w[y] = pack_f16x2(__uint_as_float(w[y] << 16) * f.x, __uint_as_float(w[y] & 0xFFFF0000u) * f.x);
+                        *reinterpret_cast<uint4*>(sh.q[q] + (x >> 3) * kAtomBytes + r * 128u + (((x & 7u) ^ (r & 7u)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+                    }
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0u) mbar_arrive(bar(kQFull + q));
                 }
                 for (uint32_t j = 0; j < steps && ok; ++j) {
                     // (not the K tile's barrier: while a group is still storing the rows of the segment before, that one may already be two steps on)
@@ -230,10 +264,13 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
                 }
                 if (!ok) break;
                 step0 += seg.steps;
-                const bool whole = seg.steps == seg.of;
-                const uint32_t h = seg.head * p.group + row % p.group;
-                float* part = slot_of(p.ws, gridDim.x, blockIdx.x, seg.first == 0u ? 1u : 0u, kItemRows) + (q * kTileRows + r) * 128u;
-                __nv_bfloat16* out = p.out + ((static_cast<size_t>(seg.b) * p.S + i) * p.H + h) * 128u;
+                const Segment done = seg;
+                more = left > 0u;
+                if (more) next();
+                const bool whole = done.steps == done.of;
+                const uint32_t h = done.head * p.group + row % p.group;
+                float* part = slot_of(p.ws, gridDim.x, blockIdx.x, done.first == 0u ? 1u : 0u, kItemRows) + (q * kTileRows + r) * 128u;
+                __nv_bfloat16* out = p.out + ((static_cast<size_t>(done.b) * p.S + i) * p.H + h) * 128u;
                 const bool none = l == 0.0f;   // NaN is something
                 const float inv = none ? 0.0f : kDown / l;
                 if (steps > 0u) {
@@ -274,17 +311,17 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
                     }
                 }
                 if (whole) {
-                    if (exists && p.lse != nullptr) p.lse[(static_cast<size_t>(seg.b) * p.H + h) * p.S + i] = none ? -INFINITY : (m + lg2(l)) * kLn2;
+                    if (exists && p.lse != nullptr) p.lse[(static_cast<size_t>(done.b) * p.H + h) * p.S + i] = none ? -INFINITY : (m + lg2(l)) * kLn2;
                 } else if (live) {
-                    *reinterpret_cast<float2*>(slot_of(p.ws, gridDim.x, blockIdx.x, seg.first == 0u ? 1u : 0u, kItemRows) + kItemRows * 128u + 2u * (q * kTileRows + r)) = make_float2(m, l);
+                    *reinterpret_cast<float2*>(slot_of(p.ws, gridDim.x, blockIdx.x, done.first == 0u ? 1u : 0u, kItemRows) + kItemRows * 128u + 2u * (q * kTileRows + r)) = make_float2(m, l);
                 }
             }
         } else if (warp < 12u) {
             asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kConvertRegs));
             const uint32_t r = threadIdx.x & 127u, page = 1u << p.c.page_log2;
-            uint32_t step = 0, segment = 0;   // so far
+            uint32_t step = 0;   // so far
             bool ok = true;
-            for (; left > 0u && ok; ++segment) {
+            while (left > 0u && ok) {
                 const Segment seg = next_segment(p, deal, at, left);
                 const uint32_t length = length_of(p.c, seg.b), n = count_of(p.counts, seg.b, p.S, length);
                 // the token of this thread in step j: its page, looked up a step ahead of its bytes
@@ -310,34 +347,6 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
                         ks = ld_u32(rec + 128u * page + 4u * slot), vs = ld_u32(rec + 132u * page + 4u * slot);
                     }
                 };
-                // the query rows: 16 threads a row, 16 bytes each
-                ok = mbar_wait(bar(kQEmpty), (segment + 1u) & 1u, failed);
-#pragma unroll 1
-                for (uint32_t x0 = 0; x0 < 32u && ok; x0 += 8u) {
-                    uint4 raw[8];
-#pragma unroll
-                    for (uint32_t x = 0; x < 8u; ++x) {
-                        const uint32_t e = (x0 + x) * 128u + r, row = seg.row0 + (e >> 4), i = row / p.group;
-                        raw[x] = make_uint4(0u, 0u, 0u, 0u);
-                        if (i < n) raw[x] = ld_v4(p.q.data + seg.b * p.q.stride_b + i * p.q.stride_s + (seg.head * p.group + row % p.group) * p.q.stride_h + 16u * (e & 15u));
-                    }
-#pragma unroll
-                    for (uint32_t x = 0; x < 8u; ++x) {
-                        const uint32_t e = (x0 + x) * 128u + r, row = e >> 4, chunk = e & 15u;
-                        uint32_t w[4] = {raw[x].x, raw[x].y, raw[x].z, raw[x].w}, amax = 0;
-#pragma unroll
-                        for (int y = 0; y < 4; ++y) amax = max(amax, max((w[y] << 16) & 0x7FFFFFFFu, w[y] & 0x7FFF0000u));
-#pragma unroll
-                        for (int y = 1; y < 16; y <<= 1) amax = max(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, y));
-                        const float2 f = row_factors(amax);
-#pragma unroll
-                        for (int y = 0; y < 4; ++y) w[y] = pack_f16x2(__uint_as_float(w[y] << 16) * f.x, __uint_as_float(w[y] & 0xFFFF0000u) * f.x);
-                        *reinterpret_cast<uint4*>(sh.q[row >> 7] + (chunk >> 3) * kAtomBytes + (row & 127u) * 128u + (((chunk & 7u) ^ (row & 7u)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
-                        if (chunk == 0u) sh.q_factor[segment & 1u][row] = f.y;
-                    }
-                }
-                fence_proxy_async_smem();
-                mbar_arrive(bar(kQFull + (segment & 1u)));
                 look_up(0u);
                 empty = seg.first * kStepTokens + r >= length, lost = page_ahead < 0;
                 fetch(0u, false);
@@ -390,7 +399,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
                 const uint32_t k_hi = static_cast<uint32_t>(d_k >> 32), v_hi = static_cast<uint32_t>(d_v >> 32);
                 const uint32_t q_lo = uniform(static_cast<uint32_t>(d_k)) + (q * kTileBytes >> 4), k_lo = uniform(static_cast<uint32_t>(d_k)) + (2u * kTileBytes >> 4), v_lo = uniform(static_cast<uint32_t>(d_v));
                 static_assert(offsetof(Shared, k) == 2u * kTileBytes, "K behind Q");
-                uint32_t step = 0, segment = 0, p_phase = 0, o_phase = 1;
+                uint32_t step = 0, q_phase = 0, turn = q ^ 1u, p_phase = 0, o_phase = 1;   // (tile 0 goes first)
                 bool ok = true;
                 auto wait = [&](uint32_t b, uint32_t parity) {
                     ok = ok && __all_sync(0xFFFFFFFFu, mbar_wait(b, parity, failed));
@@ -410,11 +419,12 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
                         tc_commit(bar(kSFull + q));
                     }
                 };
-                for (; uniform(left) > 0u && ok; ++segment) {
+                while (uniform(left) > 0u && ok) {
                     const Segment seg = next_segment(p, deal, at, left);
                     const uint32_t length = length_of(p.c, seg.b), n = count_of(p.counts, seg.b, p.S, length);
                     const uint32_t steps = uniform(tile_steps(p, seg, q, length, n)), seg_steps = uniform(seg.steps);
-                    if (!wait(bar(kQFull + (segment & 1u)), segment >> 1 & 1u)) break;
+                    if (!wait(bar(kQFull + q), q_phase)) break;
+                    q_phase ^= 1u;
                     if (!wait(bar(kKFull + step % kStages), step / kStages & 1u)) break;
                     tc_fence_after_sync();
                     if (steps > 0u) {
@@ -423,11 +433,14 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
                         o_phase ^= 1u;
                     }
                     commit(bar(kKEmpty + step % kStages));
-                    if (seg_steps == 1u) commit(bar(kQEmpty));
+                    if (seg_steps == 1u) commit(bar(kQEmpty + q));
                     for (uint32_t j = 0; j < seg_steps; ++j, ++step) {
                         const uint32_t st = step % kStages, next = (step + 1u) % kStages;
                         const bool more = j + 1u < seg_steps;
                         if (!wait(bar(kVFull + st), step / kStages & 1u)) break;
+                        // The tiles take turns, so that one's products run under the other's softmax: without, both do the same at the same time
+                        if (!wait(bar(kTurn + q), turn)) break;
+                        turn ^= 1u;
                         if (j < steps) {
 #pragma unroll
                             for (uint32_t h = 0; h < 2u; ++h) {
@@ -450,7 +463,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
                             if (j + 1u < steps) scores(next);
                             commit(bar(kKEmpty + next));
                         }
-                        if (j + 2u == seg_steps) commit(bar(kQEmpty));
+                        if (lane == 0u) mbar_arrive(bar(kTurn + (q ^ 1u)));
+                        if (j + 2u == seg_steps) commit(bar(kQEmpty + q));
                     }
                 }
                 if (!ok) {   // whatever was issued has to be over before the tensor memory goes back

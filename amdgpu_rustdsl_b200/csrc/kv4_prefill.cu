@@ -154,8 +154,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
                 length = length_of(p.c, seg.b), n = count_of(p.counts, seg.b, p.S, length);
                 ask_rows(seg, n);
             };
-            next();
-            for (bool more = true; more && ok;) {
+            bool more = true;
+            for (bool started = false; more && ok; started = true) {
+                if (!started) next();
                 if (threadIdx.x == 0u && seg.first == 0u && seg.steps < seg.of) *begun_by(p.ws, blockIdx.x) = {seg.b, seg.head, seg.row0, worker_at(all, n_work, pos + seg.of - 1u)};
                 const uint32_t steps = tile_steps(p, seg, q, length, n), row = seg.row0 + q * kTileRows + r, i = row / p.group;
                 const bool exists = row < p.S * p.group, live = exists && i < n;
@@ -243,16 +244,15 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
                     float l0 = 0.0f, l1 = 0.0f;
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
-                        uint32_t pw[16];
 #pragma unroll
                         for (int x = 0; x < 16; ++x) {
                             uint32_t a = s[k][2 * x], b = s[k][2 * x + 1];
                             fma2(a, b, c, shift);
                             const float ea = ex2(__uint_as_float(a)), eb = ex2(__uint_as_float(b));
                             add2(l0, l1, ea, eb);
-                            pw[x] = pack_f16x2(ea, eb);
+                            s[k][x] = pack_f16x2(ea, eb);   // (behind what it overwrites)
                         }
-                        tmem_st16(t_s + 16u * k, pw);
+                        tmem_st16_of32(t_s + 16u * k, s[k]);
                         if (k & 1) {
                             tmem_wait_st();
                             tc_fence_before_sync();
@@ -266,7 +266,12 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
                 step0 += seg.steps;
                 const Segment done = seg;
                 more = left > 0u;
-                if (more) next();
+                if (more) {
+                    next();
+                } else {   // (assigned either way: nothing of the old rows stays in registers for it)
+#pragma unroll
+                    for (int x = 0; x < 16; ++x) raw[x] = make_uint4(0u, 0u, 0u, 0u);
+                }
                 const bool whole = done.steps == done.of;
                 const uint32_t h = done.head * p.group + row % p.group;
                 float* part = slot_of(p.ws, gridDim.x, blockIdx.x, done.first == 0u ? 1u : 0u, kItemRows) + (q * kTileRows + r) * 128u;
@@ -279,18 +284,18 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
                     o_phase ^= 1u;
                     tc_fence_after_sync();
                 }
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    uint32_t o[32];
+#pragma unroll 1
+                for (uint32_t k = 0; k < 8u; ++k) {
+                    uint32_t o[16];
                     if (steps > 0u) {
-                        tmem_ld32(t_o + 32u * k, o);
+                        tmem_ld16(t_o + 16u * k, o);
                         tmem_wait_ld();
-                        reg_fence32(o);
+                        reg_fence16(o);
                     } else {
 #pragma unroll
-                        for (int x = 0; x < 32; ++x) o[x] = 0u;
+                        for (int x = 0; x < 16; ++x) o[x] = 0u;
                     }
-                    if (k == 3 && steps > 0u) {
+                    if (k == 7u && steps > 0u) {
                         tc_fence_before_sync();
                         __syncwarp();
                         if (lane == 0u) mbar_arrive(bar(kOFree + q));
@@ -298,16 +303,16 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
                     if (!exists) continue;
                     if (whole) {
 #pragma unroll
-                        for (int x = 0; x < 32; x += 8) {
+                        for (int x = 0; x < 16; x += 8) {
                             uint4 w;
                             w.x = pack_bf16x2(__uint_as_float(o[x]) * inv, __uint_as_float(o[x + 1]) * inv), w.y = pack_bf16x2(__uint_as_float(o[x + 2]) * inv, __uint_as_float(o[x + 3]) * inv);
                             w.z = pack_bf16x2(__uint_as_float(o[x + 4]) * inv, __uint_as_float(o[x + 5]) * inv), w.w = pack_bf16x2(__uint_as_float(o[x + 6]) * inv, __uint_as_float(o[x + 7]) * inv);
                             if (none) w = make_uint4(0u, 0u, 0u, 0u);
-                            *reinterpret_cast<uint4*>(out + 32 * k + x) = w;
+                            *reinterpret_cast<uint4*>(out + 16u * k + x) = w;
                         }
                     } else if (live) {
 #pragma unroll
-                        for (int x = 0; x < 32; x += 4) *reinterpret_cast<float4*>(part + 32 * k + x) = make_float4(__uint_as_float(o[x]) * kDown, __uint_as_float(o[x + 1]) * kDown, __uint_as_float(o[x + 2]) * kDown, __uint_as_float(o[x + 3]) * kDown);
+                        for (int x = 0; x < 16; x += 4) *reinterpret_cast<float4*>(part + 16u * k + x) = make_float4(__uint_as_float(o[x]) * kDown, __uint_as_float(o[x + 1]) * kDown, __uint_as_float(o[x + 2]) * kDown, __uint_as_float(o[x + 3]) * kDown);
                     }
                 }
                 if (whole) {

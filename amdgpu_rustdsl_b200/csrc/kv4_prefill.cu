@@ -136,56 +136,56 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
             asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
             const uint32_t q = warp >> 2, r = threadIdx.x & 127u, lanes = (warp & 3u) << 21;   // 32 TMEM lanes per warp, in bits 16 and up
             const uint32_t t_s = tmem + lanes + kColS + 128u * q, t_o = tmem + lanes + kColO + 128u * q;
-            uint32_t s_phase = 0, o_phase = 0, q_phase = 1, step0 = 0;   // step0: steps in front of the segment
+            uint32_t s_phase = 0, o_phase = 0, q_phase = 0, step0 = 0;   // step0: steps in front of the segment
             bool ok = true;
-            // The query rows, a thread its own: asked for while the last products of the segment before are under way, kept in registers over its epilogue
+            // The query rows: asked for while the last products of the segment before are under way, kept in registers over its epilogue. A warp has the rows of its threads, two
+            // of them with a load: lane l brings 16 bytes (8 elements, number l mod 16) of row 2 x + l / 16
             uint4 raw[16];
-            auto ask_rows = [&](const Segment& seg, uint32_t n) {
-                const uint32_t row = seg.row0 + q * kTileRows + r, i = row / p.group;
-                const uint8_t* src = p.q.data + seg.b * p.q.stride_b + i * p.q.stride_s + (seg.head * p.group + row % p.group) * p.q.stride_h;
-#pragma unroll
-                for (int x = 0; x < 16; ++x) raw[x] = i < n ? ld_v4(src + 16 * x) : make_uint4(0u, 0u, 0u, 0u);
-            };
             Segment seg;
             uint32_t pos, length, n;
             auto next = [&]() {
                 pos = end - left;
                 seg = next_segment(p, deal, at, left);
                 length = length_of(p.c, seg.b), n = count_of(p.counts, seg.b, p.S, length);
-                ask_rows(seg, n);
+                const uint32_t row = seg.row0 + q * kTileRows + (r & 96u) + (lane >> 4);
+                uint32_t i = row / p.group, h = row - i * p.group;
+                const uint8_t* src = p.q.data + seg.b * p.q.stride_b + seg.head * p.group * p.q.stride_h + 16u * (lane & 15u);
+#pragma unroll
+                for (int x = 0; x < 16; ++x) {
+                    raw[x] = i < n ? ld_v4(src + i * p.q.stride_s + h * p.q.stride_h) : make_uint4(0u, 0u, 0u, 0u);
+                    for (h += 2u; h >= p.group; h -= p.group) ++i;
+                }
             };
+            uint8_t* mine = sh.q[q] + (r >> 5) * (kTileBytes / 4u);   // a quarter of the rows' place, where this warp turns its part of O round, between two segments
             bool more = true;
-            for (bool started = false; more && ok; started = true) {
+            for (bool started = false; more; started = true) {
                 if (!started) next();
+                // the tile's four warps are done with the place of the rows; also where a wait has run out in one of them: they leave together
+                ok = named_bar_all(2u + q, 128u, ok);
+                if (!ok) break;
                 if (threadIdx.x == 0u && seg.first == 0u && seg.steps < seg.of) *begun_by(p.ws, blockIdx.x) = {seg.b, seg.head, seg.row0, worker_at(all, n_work, pos + seg.of - 1u)};
                 const uint32_t steps = tile_steps(p, seg, q, length, n), row = seg.row0 + q * kTileRows + r, i = row / p.group;
                 const bool exists = row < p.S * p.group, live = exists && i < n;
                 const uint32_t limit = !live ? 0u : p.causal ? length - n + i + 1u : length;
-                float m = kLowest, l = 0.0f, c_row;
-                {
-                    uint32_t amax = 0;
+                float m = kLowest, l = 0.0f, c_row = 0.0f;
 #pragma unroll
-                    for (int x = 0; x < 16; ++x) {
-                        const uint32_t w[4] = {raw[x].x, raw[x].y, raw[x].z, raw[x].w};
+                for (uint32_t x = 0; x < 16u; ++x) {
+                    uint32_t w[4] = {raw[x].x, raw[x].y, raw[x].z, raw[x].w}, amax = 0;
 #pragma unroll
-                        for (int y = 0; y < 4; ++y) amax = max(amax, max((w[y] << 16) & 0x7FFFFFFFu, w[y] & 0x7FFF0000u));
-                    }
+                    for (int y = 0; y < 4; ++y) amax = max(amax, max((w[y] << 16) & 0x7FFFFFFFu, w[y] & 0x7FFF0000u));
+#pragma unroll
+                    for (int y = 1; y < 16; y <<= 1) amax = max(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, y));
                     const float2 f = row_factors(amax);
-                    c_row = p.scale_log2 * f.y;
-                    ok = mbar_wait(bar(kQEmpty + q), q_phase, failed);   // S of the segment before is done with its rows
-                    if (!ok) break;
-                    q_phase ^= 1u;
+                    const float back = __shfl_sync(0xFFFFFFFFu, f.y, (lane & 1u) << 4);   // of row 2 x + lane mod 2
+                    if (lane >> 1 == x) c_row = p.scale_log2 * back;
 #pragma unroll
-                    for (uint32_t x = 0; x < 16u; ++x) {
-                        uint32_t w[4] = {raw[x].x, raw[x].y, raw[x].z, raw[x].w};
-#pragma unroll
-                        for (int y = 0; y < 4; ++y) w[y] = pack_f16x2(__uint_as_float(w[y] << 16) * f.x, __uint_as_float(w[y] & 0xFFFF0000u) * f.x);
-                        *reinterpret_cast<uint4*>(sh.q[q] + (x >> 3) * kAtomBytes + r * 128u + (((x & 7u) ^ (r & 7u)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
-                    }
-                    fence_proxy_async_smem();
-                    __syncwarp();
-                    if (lane == 0u) mbar_arrive(bar(kQFull + q));
+                    for (int y = 0; y < 4; ++y) w[y] = pack_f16x2(__uint_as_float(w[y] << 16) * f.x, __uint_as_float(w[y] & 0xFFFF0000u) * f.x);
+                    const uint32_t to = (r & 96u) + 2u * x + (lane >> 4), chunk = lane & 15u;
+                    *reinterpret_cast<uint4*>(sh.q[q] + (chunk >> 3) * kAtomBytes + to * 128u + (((chunk & 7u) ^ (to & 7u)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
                 }
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0u) mbar_arrive(bar(kQFull + q));
                 for (uint32_t j = 0; j < steps && ok; ++j) {
                     // (not the K tile's barrier: while a group is still storing the rows of the segment before, that one may already be two steps on)
                     const uint32_t slot = (step0 + j) % kFactorSlots;
@@ -262,7 +262,6 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
                     }
                     l = fmaf(l0 + l1, __uint_as_float(static_cast<uint32_t>(127 - e) << 23), l);
                 }
-                if (!ok) break;
                 step0 += seg.steps;
                 const Segment done = seg;
                 more = left > 0u;
@@ -272,53 +271,67 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
 #pragma unroll
                     for (int x = 0; x < 16; ++x) raw[x] = make_uint4(0u, 0u, 0u, 0u);
                 }
-                const bool whole = done.steps == done.of;
-                const uint32_t h = done.head * p.group + row % p.group;
-                float* part = slot_of(p.ws, gridDim.x, blockIdx.x, done.first == 0u ? 1u : 0u, kItemRows) + (q * kTileRows + r) * 128u;
-                __nv_bfloat16* out = p.out + ((static_cast<size_t>(done.b) * p.S + i) * p.H + h) * 128u;
-                const bool none = l == 0.0f;   // NaN is something
-                const float inv = none ? 0.0f : kDown / l;
+                ok = ok && mbar_wait(bar(kQEmpty + q), q_phase, failed);   // S is done with the rows
+                q_phase ^= 1u;
                 if (steps > 0u) {
-                    ok = mbar_wait(bar(kODone + q), o_phase, failed);
-                    if (!ok) break;
+                    ok = ok && mbar_wait(bar(kODone + q), o_phase, failed);
                     o_phase ^= 1u;
                     tc_fence_after_sync();
                 }
+                if (!ok) continue;
+                const bool whole = done.steps == done.of, none = l == 0.0f;   // NaN is something
+                const uint32_t h = done.head * p.group + row % p.group;
+                const float factor = whole ? (none ? 0.0f : kDown / l) : kDown;
+                const uint32_t at_row = exists ? (done.b * p.S + i) * p.H + h : 0xFFFFFFFFu;   // of out, in rows
+                float* slot = slot_of(p.ws, gridDim.x, blockIdx.x, done.first == 0u ? 1u : 0u, kItemRows);
+                // O by 64 columns: a thread writes its row's to shared memory, and the warp stores whole pieces of rows
 #pragma unroll 1
-                for (uint32_t k = 0; k < 8u; ++k) {
-                    uint32_t o[16];
-                    if (steps > 0u) {
-                        tmem_ld16(t_o + 16u * k, o);
-                        tmem_wait_ld();
-                        reg_fence16(o);
-                    } else {
+                for (uint32_t c = 0; c < 2u; ++c) {
 #pragma unroll
-                        for (int x = 0; x < 16; ++x) o[x] = 0u;
+                    for (uint32_t k = 0; k < 4u; ++k) {
+                        uint32_t o[16];
+                        if (steps > 0u) {
+                            tmem_ld16(t_o + 64u * c + 16u * k, o);
+                            tmem_wait_ld();
+                            reg_fence16(o);
+                        } else {
+#pragma unroll
+                            for (int x = 0; x < 16; ++x) o[x] = 0u;
+                        }
+#pragma unroll
+                        for (uint32_t x = 0; x < 4u; ++x) {
+                            float4 v = make_float4(__uint_as_float(o[4 * x]) * factor, __uint_as_float(o[4 * x + 1]) * factor, __uint_as_float(o[4 * x + 2]) * factor, __uint_as_float(o[4 * x + 3]) * factor);
+                            if (none) v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                            *reinterpret_cast<float4*>(mine + lane * 256u + (((4u * k + x) ^ (lane & 15u)) << 4)) = v;
+                        }
                     }
-                    if (k == 7u && steps > 0u) {
+                    if (c == 1u && steps > 0u) {
                         tc_fence_before_sync();
                         __syncwarp();
                         if (lane == 0u) mbar_arrive(bar(kOFree + q));
                     }
-                    if (!exists) continue;
+                    __syncwarp();
                     if (whole) {
-#pragma unroll
-                        for (int x = 0; x < 16; x += 8) {
-                            uint4 w;
-                            w.x = pack_bf16x2(__uint_as_float(o[x]) * inv, __uint_as_float(o[x + 1]) * inv), w.y = pack_bf16x2(__uint_as_float(o[x + 2]) * inv, __uint_as_float(o[x + 3]) * inv);
-                            w.z = pack_bf16x2(__uint_as_float(o[x + 4]) * inv, __uint_as_float(o[x + 5]) * inv), w.w = pack_bf16x2(__uint_as_float(o[x + 6]) * inv, __uint_as_float(o[x + 7]) * inv);
-                            if (none) w = make_uint4(0u, 0u, 0u, 0u);
-                            *reinterpret_cast<uint4*>(out + 16u * k + x) = w;
+#pragma unroll 4
+                        for (uint32_t x = 0; x < 8u; ++x) {   // four rows of 64 bf16 at a time
+                            const uint32_t from = 4u * x + (lane >> 3), piece = lane & 7u, to = __shfl_sync(0xFFFFFFFFu, at_row, from);
+                            const float4 u = *reinterpret_cast<const float4*>(mine + from * 256u + (((2u * piece) ^ (from & 15u)) << 4)), v = *reinterpret_cast<const float4*>(mine + from * 256u + (((2u * piece + 1u) ^ (from & 15u)) << 4));
+                            if (to != 0xFFFFFFFFu)
+                                *reinterpret_cast<uint4*>(p.out + static_cast<size_t>(to) * 128u + 64u * c + 8u * piece) = make_uint4(pack_bf16x2(u.x, u.y), pack_bf16x2(u.z, u.w), pack_bf16x2(v.x, v.y), pack_bf16x2(v.z, v.w));
                         }
-                    } else if (live) {
-#pragma unroll
-                        for (int x = 0; x < 16; x += 4) *reinterpret_cast<float4*>(part + 16u * k + x) = make_float4(__uint_as_float(o[x]) * kDown, __uint_as_float(o[x + 1]) * kDown, __uint_as_float(o[x + 2]) * kDown, __uint_as_float(o[x + 3]) * kDown);
+                    } else {
+#pragma unroll 4
+                        for (uint32_t x = 0; x < 16u; ++x) {   // two rows of 64 f32 at a time
+                            const uint32_t from = 2u * x + (lane >> 4), piece = lane & 15u;
+                            *reinterpret_cast<float4*>(slot + (q * kTileRows + (r & 96u) + from) * 128u + 64u * c + 4u * piece) = *reinterpret_cast<const float4*>(mine + from * 256u + ((piece ^ (from & 15u)) << 4));
+                        }
                     }
+                    __syncwarp();
                 }
                 if (whole) {
                     if (exists && p.lse != nullptr) p.lse[(static_cast<size_t>(done.b) * p.H + h) * p.S + i] = none ? -INFINITY : (m + lg2(l)) * kLn2;
                 } else if (live) {
-                    *reinterpret_cast<float2*>(slot_of(p.ws, gridDim.x, blockIdx.x, done.first == 0u ? 1u : 0u, kItemRows) + kItemRows * 128u + 2u * (q * kTileRows + r)) = make_float2(m, l);
+                    *reinterpret_cast<float2*>(slot + kItemRows * 128u + 2u * (q * kTileRows + r)) = make_float2(m, l);
                 }
             }
         } else if (warp < 12u) {

@@ -47,6 +47,10 @@ struct Shared {
     uint4 most[kFactorSlots][2];   // the largest scale byte of K and of V that each of the converting warps met
     unsigned long long bars[kBars];
     Sums part[kThreads / 32];
+    struct Plan {
+        Segment seg;
+        uint32_t pos, length, n;
+    } plan[8];                     // of a softmax warp's next segment
     uint32_t tmem, failed, not_drained;
 };
 
@@ -141,12 +145,16 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
             // The query rows: asked for while the last products of the segment before are under way, kept in registers over its epilogue. A warp has the rows of its threads, two
             // of them with a load: lane l brings 16 bytes (8 elements, number l mod 16) of row 2 x + l / 16
             uint4 raw[16];
-            Segment seg;
-            uint32_t pos, length, n;
-            auto next = [&]() {
-                pos = end - left;
-                seg = next_segment(p, deal, at, left);
-                length = length_of(p.c, seg.b), n = count_of(p.counts, seg.b, p.S, length);
+            // Where the next segment is, is worked out while the first scores of this one are computed; the rows are asked for at its end
+            auto plan_next = [&]() {
+                Shared::Plan x;
+                x.pos = end - left;
+                x.seg = next_segment(p, deal, at, left);
+                x.length = length_of(p.c, x.seg.b), x.n = count_of(p.counts, x.seg.b, p.S, x.length);
+                if (lane == 0u) sh.plan[warp] = x;
+                __syncwarp();
+            };
+            auto ask_rows = [&](const Segment& seg, uint32_t n) {
                 const uint32_t row = seg.row0 + q * kTileRows + (r & 96u) + (lane >> 4);
                 uint32_t i = row / p.group, h = row - i * p.group;
                 const uint8_t* src = p.q.data + seg.b * p.q.stride_b + seg.head * p.group * p.q.stride_h + 16u * (lane & 15u);
@@ -156,10 +164,13 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
                     for (h += 2u; h >= p.group; h -= p.group) ++i;
                 }
             };
+            plan_next();
+            Shared::Plan now = sh.plan[warp];
+            ask_rows(now.seg, now.n);
             uint8_t* mine = sh.q[q] + (r >> 5) * (kTileBytes / 4u);   // a quarter of the rows' place, where this warp turns its part of O round, between two segments
-            bool more = true;
-            for (bool started = false; more; started = true) {
-                if (!started) next();
+            for (bool more = true; more;) {
+                const Segment seg = now.seg;
+                const uint32_t pos = now.pos, length = now.length, n = now.n;
                 // the tile's four warps are done with the place of the rows; also where a wait has run out in one of them: they leave together
                 ok = named_bar_all(2u + q, 128u, ok);
                 if (!ok) break;
@@ -168,24 +179,38 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
                 const bool exists = row < p.S * p.group, live = exists && i < n;
                 const uint32_t limit = !live ? 0u : p.causal ? length - n + i + 1u : length;
                 float m = kLowest, l = 0.0f, c_row = 0.0f;
+                {
+                    uint32_t amax[8];   // sizes as bf16 bits, of rows 2 x and 2 x + 1 of pairs of loads in the halves
 #pragma unroll
-                for (uint32_t x = 0; x < 16u; ++x) {
-                    uint32_t w[4] = {raw[x].x, raw[x].y, raw[x].z, raw[x].w}, amax = 0;
+                    for (int x = 0; x < 8; ++x) {
+                        auto largest = [](const uint4& v) {
+                            const uint32_t m = __vmaxu2(__vmaxu2(v.x & 0x7FFF7FFFu, v.y & 0x7FFF7FFFu), __vmaxu2(v.z & 0x7FFF7FFFu, v.w & 0x7FFF7FFFu));
+                            return max(m & 0xFFFFu, m >> 16);
+                        };
+                        amax[x] = largest(raw[2 * x]) | largest(raw[2 * x + 1]) << 16;
+                    }
 #pragma unroll
-                    for (int y = 0; y < 4; ++y) amax = max(amax, max((w[y] << 16) & 0x7FFFFFFFu, w[y] & 0x7FFF0000u));
+                    for (int y = 1; y < 16; y <<= 1) {
 #pragma unroll
-                    for (int y = 1; y < 16; y <<= 1) amax = max(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, y));
-                    const float2 f = row_factors(amax);
-                    const float back = __shfl_sync(0xFFFFFFFFu, f.y, (lane & 1u) << 4);   // of row 2 x + lane mod 2
-                    if (lane >> 1 == x) c_row = p.scale_log2 * back;
+                        for (int x = 0; x < 8; ++x) amax[x] = __vmaxu2(amax[x], __shfl_xor_sync(0xFFFFFFFFu, amax[x], y));
+                    }
 #pragma unroll
-                    for (int y = 0; y < 4; ++y) w[y] = pack_f16x2(__uint_as_float(w[y] << 16) * f.x, __uint_as_float(w[y] & 0xFFFF0000u) * f.x);
-                    const uint32_t to = (r & 96u) + 2u * x + (lane >> 4), chunk = lane & 15u;
-                    *reinterpret_cast<uint4*>(sh.q[q] + (chunk >> 3) * kAtomBytes + to * 128u + (((chunk & 7u) ^ (to & 7u)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+                    for (uint32_t x = 0; x < 16u; ++x) {
+                        uint32_t w[4] = {raw[x].x, raw[x].y, raw[x].z, raw[x].w};
+                        const float2 f = row_factors(x & 1u ? amax[x / 2] & 0xFFFF0000u : amax[x / 2] << 16);
+                        const float back = __shfl_sync(0xFFFFFFFFu, f.y, (lane & 1u) << 4);   // of row 2 x + lane mod 2
+                        if (lane >> 1 == x) c_row = p.scale_log2 * back;
+#pragma unroll
+                        for (int y = 0; y < 4; ++y) w[y] = pack_f16x2(__uint_as_float(w[y] << 16) * f.x, __uint_as_float(w[y] & 0xFFFF0000u) * f.x);
+                        const uint32_t to = (r & 96u) + 2u * x + (lane >> 4), chunk = lane & 15u;
+                        *reinterpret_cast<uint4*>(sh.q[q] + (chunk >> 3) * kAtomBytes + to * 128u + (((chunk & 7u) ^ (to & 7u)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+                    }
                 }
                 fence_proxy_async_smem();
                 __syncwarp();
                 if (lane == 0u) mbar_arrive(bar(kQFull + q));
+                more = left > 0u;
+                if (more) plan_next();
                 for (uint32_t j = 0; j < steps && ok; ++j) {
                     // (not the K tile's barrier: while a group is still storing the rows of the segment before, that one may already be two steps on)
                     const uint32_t slot = (step0 + j) % kFactorSlots;
@@ -264,9 +289,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
                 }
                 step0 += seg.steps;
                 const Segment done = seg;
-                more = left > 0u;
                 if (more) {
-                    next();
+                    now = sh.plan[warp];
+                    ask_rows(now.seg, now.n);
                 } else {   // (assigned either way: nothing of the old rows stays in registers for it)
 #pragma unroll
                     for (int x = 0; x < 16; ++x) raw[x] = make_uint4(0u, 0u, 0u, 0u);
@@ -288,21 +313,21 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
 #pragma unroll 1
                 for (uint32_t c = 0; c < 2u; ++c) {
 #pragma unroll
-                    for (uint32_t k = 0; k < 4u; ++k) {
-                        uint32_t o[16];
+                    for (uint32_t k = 0; k < 2u; ++k) {
+                        uint32_t o[32];
                         if (steps > 0u) {
-                            tmem_ld16(t_o + 64u * c + 16u * k, o);
+                            tmem_ld32(t_o + 64u * c + 32u * k, o);
                             tmem_wait_ld();
-                            reg_fence16(o);
+                            reg_fence32(o);
                         } else {
 #pragma unroll
-                            for (int x = 0; x < 16; ++x) o[x] = 0u;
+                            for (int x = 0; x < 32; ++x) o[x] = 0u;
                         }
 #pragma unroll
-                        for (uint32_t x = 0; x < 4u; ++x) {
+                        for (uint32_t x = 0; x < 8u; ++x) {
                             float4 v = make_float4(__uint_as_float(o[4 * x]) * factor, __uint_as_float(o[4 * x + 1]) * factor, __uint_as_float(o[4 * x + 2]) * factor, __uint_as_float(o[4 * x + 3]) * factor);
                             if (none) v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                            *reinterpret_cast<float4*>(mine + lane * 256u + (((4u * k + x) ^ (lane & 15u)) << 4)) = v;
+                            *reinterpret_cast<float4*>(mine + lane * 256u + (((8u * k + x) ^ (lane & 15u)) << 4)) = v;
                         }
                     }
                     if (c == 1u && steps > 0u) {

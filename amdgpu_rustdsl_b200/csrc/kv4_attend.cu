@@ -323,7 +323,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : NT == 2 ? 3 : 2) kv4_a
     const uint32_t all = sum_steps(p, deal, 0u, sh.part).all;
     const uint32_t n_work = workers(all, gridDim.x);
     clear_empty_entries(p, deal);
-    if (threadIdx.x == 0u) begun_by(p.ws, blockIdx.x)->last = blockIdx.x;
+    if (threadIdx.x == 0u) begin_nothing(p, deal);
     if (blockIdx.x >= n_work) return;
     const uint32_t begin = run_begin(all, n_work, blockIdx.x), end = run_begin(all, n_work, blockIdx.x + 1u);
     uint32_t left = end - begin;
@@ -340,7 +340,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : NT == 2 ? 3 : 2) kv4_a
     while (left > 0u) {
         const uint32_t pos = end - left;
         const Segment seg = next_segment(p, deal, at, left);
-        if (threadIdx.x == 0u && seg.first == 0u && seg.steps < seg.of) *begun_by(p.ws, blockIdx.x) = {seg.b, seg.head, seg.row0, worker_at(all, n_work, pos + seg.of - 1u)};
+        if (threadIdx.x == 0u) begin_item(p, deal, seg, pos, all, n_work);
         const uint32_t b = seg.b, head = seg.head, row0 = seg.row0, first = seg.first, n_tiles = seg.steps;
         const uint32_t length = length_of(p.c, b), n_rows = count_of(p.counts, b, p.S, length);
         const int32_t* row_of_table = p.c.table + static_cast<size_t>(b) * p.c.table_width;
@@ -493,25 +493,27 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : NT == 2 ? 3 : 2) kv4_a
     }
 }
 
-// Puts the items together that more than one CTA of a launch worked on; blockIdx.x is the CTA that began one. kFewRows: a CTA has one row, its warps the parts in turn; else a warp has
-// a row and all of its parts. Four parts are in flight at a time.
-template <bool kFewRows>
-__global__ void __launch_bounds__(kThreads) kv4_combine_kernel(const __grid_constant__ Kv4AttendParams p, uint32_t rows) {
-    __shared__ float sm_m[kWarps], sm_l[kWarps];
-    __shared__ float4 sm_o[kWarps][32];
+// Puts the items together that more than one CTA of a launch worked on: blockIdx.x is an entry of the workspace, parts come from a launch of `grid` CTAs. kTogether: a CTA of so many
+// warps has one row, its warps the parts in turn; 0: a warp has a row and all of its parts. Four parts are in flight at a time. (The CTAs take little shared memory on
+// purpose: with 8 KB in place of 2 the attention kernel behind this one took 272 us in place of 236, 64
+// sequences of 16384 tokens.)
+template <uint32_t kTogether>
+__global__ void __launch_bounds__(kTogether ? 32 * kTogether : 256) kv4_combine_kernel(const __grid_constant__ Kv4AttendParams p, uint32_t rows, uint32_t row_tiles, uint32_t grid) {
+    __shared__ float sm_m[kTogether ? kTogether : 1u], sm_l[kTogether ? kTogether : 1u];
+    __shared__ float4 sm_o[kTogether ? 4 : 1][32];
     pdl_launch();
     pdl_wait();
-    const unsigned lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
-    const uint32_t r = kFewRows ? blockIdx.y : blockIdx.y * kWarps + warp;
-    const uint4 begun = ld_v4(begun_by(p.ws, blockIdx.x));
-    const uint32_t b = begun.x, head = begun.y, row = begun.z + r, last = begun.w;
-    if (last == blockIdx.x || row >= p.S * p.group) return;   // (the same in all warps where they meet below)
+    const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
+    const uint32_t r = kTogether ? blockIdx.y : blockIdx.y * (blockDim.x >> 5) + warp;
+    const uint4 begun = ld_v4(begun_at(p.ws, blockIdx.x));
+    const uint32_t entry = begun.x / p.c.HK, head = begun.x - entry * p.c.HK, b = entry / row_tiles, row = (entry - b * row_tiles) * rows + r, from = begun.y, last = begun.z;
+    if (last == from || row >= p.S * p.group) return;   // (the same in all warps where they meet below)
     const uint32_t i = row / p.group, h = head * p.group + row % p.group;
     const bool sees = i < count_of(p.counts, b, p.S, length_of(p.c, b));
-    constexpr uint32_t kStride = kFewRows ? kWarps : 1u;
+    constexpr uint32_t kStride = kTogether ? kTogether : 1u;
     float m = kLowest, l = 0.0f;
     float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    for (uint32_t w0 = blockIdx.x + (kFewRows ? warp : 0u); sees && w0 <= last; w0 += 4u * kStride) {
+    for (uint32_t w0 = from + (kTogether ? warp : 0u); sees && w0 <= last; w0 += 4u * kStride) {
         float pm[4], pl[4];
         uint4 raw[4];
 #pragma unroll
@@ -519,7 +521,7 @@ __global__ void __launch_bounds__(kThreads) kv4_combine_kernel(const __grid_cons
             const uint32_t w = w0 + k * kStride;
             pm[k] = kLowest, pl[k] = 0.0f, raw[k] = make_uint4(0u, 0u, 0u, 0u);
             if (w <= last) {
-                const float* src = slot_of(p.ws, gridDim.x, w, w == blockIdx.x ? 1u : 0u, rows);
+                const float* src = slot_of(p.ws, grid, w, w == from ? 1u : 0u, rows);
                 pm[k] = ld_f32(src + rows * 128u + 2u * r), pl[k] = ld_f32(src + rows * 128u + 2u * r + 1u);
                 raw[k] = ld_v4(src + r * 128u + 4u * lane);
             }
@@ -533,21 +535,34 @@ __global__ void __launch_bounds__(kThreads) kv4_combine_kernel(const __grid_cons
             o.z = fmaf(o.z, a, __uint_as_float(raw[k].z) * c), o.w = fmaf(o.w, a, __uint_as_float(raw[k].w) * c);
         }
     }
-    if (kFewRows) {
+    if constexpr (kTogether != 0u) {   // four warps at a time hand over what they have
         if (lane == 0u) sm_m[warp] = m, sm_l[warp] = l;
-        sm_o[warp][lane] = o;
+        if (warp < 4u) sm_o[warp][lane] = o;
         __syncthreads();
-        if (warp != 0u) return;
-        m = fmaxf(fmaxf(sm_m[0], sm_m[1]), fmaxf(sm_m[2], sm_m[3]));
+        m = sm_m[0];
+#pragma unroll
+        for (uint32_t w = 1; w < kTogether; ++w) m = fmaxf(m, sm_m[w]);
+        const float4 mine = o;
         l = 0.0f;
         o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-        for (unsigned w = 0; w < kWarps; ++w) {
-            const float f = ex2(sm_m[w] - m);
-            const float4 c = sm_o[w][lane];
-            l = fmaf(sm_l[w], f, l);
-            o.x = fmaf(c.x, f, o.x), o.y = fmaf(c.y, f, o.y), o.z = fmaf(c.z, f, o.z), o.w = fmaf(c.w, f, o.w);
+        for (uint32_t w0 = 0; w0 < kTogether; w0 += 4u) {
+            if (w0 > 0u) {
+                __syncthreads();
+                if (warp - w0 < 4u) sm_o[warp - w0][lane] = mine;
+                __syncthreads();
+            }
+            if (warp == 0u) {
+#pragma unroll
+                for (uint32_t w = 0; w < 4u; ++w) {
+                    const float f = ex2(sm_m[w0 + w] - m);
+                    const float4 c = sm_o[w][lane];
+                    l = fmaf(sm_l[w0 + w], f, l);
+                    o.x = fmaf(c.x, f, o.x), o.y = fmaf(c.y, f, o.y), o.z = fmaf(c.z, f, o.z), o.w = fmaf(c.w, f, o.w);
+                }
+            }
         }
+        if (warp != 0u) return;
     }
     const bool none = l == 0.0f;
     const float inv = none ? 0.0f : 1.0f / l;
@@ -580,14 +595,17 @@ cudaError_t launch_rows(const Kv4AttendParams& p, cudaStream_t stream) {
     }
     e = kv4_launch(kv4_attend_kernel<NT>, dim3(grid), kThreads, smem, stream, p);
     if (e != cudaSuccess) return e;
-    return kv4_launch(kv4_combine_kernel<true>, dim3(grid, rows < 8u * NT ? rows : 8u * NT), kThreads, 0, stream, p, 8u * NT);
+    // 4 warps have 16 parts in flight; where an item has more on average, 16 warps (5 rows over 65536 tokens, 74 parts: 28.4 us in place of 31)
+    const uint32_t entries = begun_entries(p.c, 1u, grid), some = rows < 8u * NT ? rows : 8u * NT;
+    if (grid / entries > 16u) return kv4_launch(kv4_combine_kernel<16>, dim3(entries, some), 512u, 0, stream, p, 8u * NT, 1u, grid);
+    return kv4_launch(kv4_combine_kernel<4>, dim3(entries, some), 128u, 0, stream, p, 8u * NT, 1u, grid);
 }
 
 cudaError_t launch_many(const Kv4AttendParams& p, cudaStream_t stream) {
     const uint32_t rows = p.S * p.group, per = kv4_prefill_rows(), row_tiles = (rows + per - 1u) / per, most = rows < per ? rows : per;
     const cudaError_t e = launch_kv4_prefill(p, row_tiles, stream);
     if (e != cudaSuccess) return e;
-    return kv4_launch(kv4_combine_kernel<false>, dim3(kv4_prefill_grid(), (most + kWarps - 1u) / kWarps), kThreads, 0, stream, p, per);
+    return kv4_launch(kv4_combine_kernel<0>, dim3(begun_entries(p.c, row_tiles, kv4_prefill_grid()), (most + 7u) / 8u), 256u, 0, stream, p, per, row_tiles, kv4_prefill_grid());
 }
 
 uint64_t partial_bytes(const Kv4View& c, uint32_t rows) {

@@ -130,7 +130,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
     const uint32_t n_work = workers(all, gridDim.x);
     volatile uint32_t* failed = &sh.failed;
     clear_empty_entries(p, deal);
-    if (threadIdx.x == 0u) begun_by(p.ws, blockIdx.x)->last = blockIdx.x;
+    if (threadIdx.x == 0u) begin_nothing(p, deal);
     if (blockIdx.x < n_work) {
         const uint32_t begin = run_begin(all, n_work, blockIdx.x);
         const uint32_t end = run_begin(all, n_work, blockIdx.x + 1u);
@@ -174,7 +174,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
                 // the tile's four warps are done with the place of the rows; also where a wait has run out in one of them: they leave together
                 ok = named_bar_all(2u + q, 128u, ok);
                 if (!ok) break;
-                if (threadIdx.x == 0u && seg.first == 0u && seg.steps < seg.of) *begun_by(p.ws, blockIdx.x) = {seg.b, seg.head, seg.row0, worker_at(all, n_work, pos + seg.of - 1u)};
+                if (threadIdx.x == 0u) begin_item(p, deal, seg, pos, all, n_work);
                 const uint32_t steps = tile_steps(p, seg, q, length, n), row = seg.row0 + q * kTileRows + r, i = row / p.group;
                 const bool exists = row < p.S * p.group, live = exists && i < n;
                 const uint32_t limit = !live ? 0u : p.causal ? length - n + i + 1u : length;

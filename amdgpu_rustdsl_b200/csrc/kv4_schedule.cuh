@@ -98,19 +98,36 @@ __device__ __forceinline__ Segment next_segment(const Kv4AttendParams& p, const 
     return s;
 }
 
-// The workspace of a launch of `grid` CTAs: an entry per CTA that says which item the CTA began and others went on with, behind them the CTAs' partials: two slots (0: an item
-// that an earlier CTA began, 1: one that a later CTA goes on with), each `rows` x 128 f32 of O in front of `rows` pairs of M (base 2) and l
+// The workspace of a launch of `grid` CTAs: entries that say which CTAs worked on an item, one per item, or where there are more items than a quarter of the CTAs one per CTA for the item that it
+// began and others went on with; behind room for `grid` of them the CTAs' partials: two slots (0: an item that an earlier CTA began, 1: one that a later CTA goes on with), each
+// `rows` x 128 f32 of O in front of `rows` pairs of M (base 2) and l
 struct Begun {
-    uint32_t b, head, row0, last;   // the last CTA that has a part; the CTA itself: there is no such item
+    uint32_t item, first, last, unused;   // the first and the last CTA that have a part; the same: there is nothing to put together
 };
-__device__ __forceinline__ Begun* begun_by(float* ws, uint32_t w) { return reinterpret_cast<Begun*>(ws) + w; }
+// (4 items of 74 parts each: 28 us with the item's entries, 36 with an entry and a row of idle CTAs for each of the 296 CTAs; 192 items of up to 7 parts among 592 CTAs: 72.6 and 69.7)
+__host__ __device__ __forceinline__ bool begun_by_item(const Kv4View& c, uint32_t row_tiles, uint32_t grid) { return 4ull * c.B * c.HK * row_tiles <= grid; }
+__host__ __device__ __forceinline__ uint32_t begun_entries(const Kv4View& c, uint32_t row_tiles, uint32_t grid) { return begun_by_item(c, row_tiles, grid) ? c.B * c.HK * row_tiles : grid; }
+__device__ __forceinline__ Begun* begun_at(float* ws, uint32_t x) { return reinterpret_cast<Begun*>(ws) + x; }
+// by one thread of a CTA: at its start, and for each segment
+__device__ __forceinline__ void begin_nothing(const Kv4AttendParams& p, const Deal& d) {
+    if (!begun_by_item(p.c, d.row_tiles, gridDim.x)) *begun_at(p.ws, blockIdx.x) = {0u, blockIdx.x, blockIdx.x, 0u};
+}
+__device__ __forceinline__ void begin_item(const Kv4AttendParams& p, const Deal& d, const Segment& s, uint32_t pos, uint32_t all, uint32_t n_work) {
+    if (s.first != 0u) return;
+    const uint32_t item = (s.b * d.row_tiles + s.row0 / d.rows) * p.c.HK + s.head, last = s.steps == s.of ? blockIdx.x : worker_at(all, n_work, pos + s.of - 1u);
+    const bool by_item = begun_by_item(p.c, d.row_tiles, gridDim.x);
+    if (by_item || last != blockIdx.x) *begun_at(p.ws, by_item ? item : blockIdx.x) = {item, blockIdx.x, last, 0u};
+}
 __device__ __forceinline__ float* slot_of(float* ws, uint32_t grid, uint32_t w, uint32_t slot, uint32_t rows) { return ws + 4u * grid + (static_cast<size_t>(w) * 2u + slot) * rows * 130u; }
 constexpr float kLowest = -1e30f;   // M of a row that has seen nothing
 
-// Entries that no CTA has steps of: their rows see nothing. All threads of the grid.
+// Sequences' row tiles that no CTA has steps of: their rows see nothing. All threads of the grid.
 __device__ __forceinline__ void clear_empty_entries(const Kv4AttendParams& p, const Deal& d) {
     for (uint32_t e = blockIdx.x; e < p.c.B * d.row_tiles; e += gridDim.x) {
         if (steps_of(p, d, e) != 0u) continue;
+        if (begun_by_item(p.c, d.row_tiles, gridDim.x)) {
+            for (uint32_t h = threadIdx.x; h < p.c.HK; h += blockDim.x) *begun_at(p.ws, e * p.c.HK + h) = {0u, 0u, 0u, 0u};
+        }
         const uint32_t b = e / d.row_tiles, row0 = (e - b * d.row_tiles) * d.rows, rows = min(d.rows, p.S * p.group - row0);
         for (uint32_t x = threadIdx.x; x < rows * p.c.HK * 16u; x += blockDim.x) {
             const uint32_t part = x & 15u, row = row0 + (x >> 4) % rows, head = (x >> 4) / rows, i = row / p.group, h = head * p.group + row % p.group;

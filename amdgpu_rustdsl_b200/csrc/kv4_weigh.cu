@@ -2,9 +2,10 @@
 // known. The sums run over the rows in order, a token's all in one warp: the same bits every time.
 //
 // With up to 8 rows the attention kernel has left the scores (a token's all in one 8- to 32-byte piece), and a thread adds up a token's. With more rows S^T = K Q^T is computed
-// again, a warp for 32 tokens whose K codes it converts once, against blocks of 64 rows that the CTA converts into shared memory in the operand's layout; that is bound
-// by the matrix instructions (8 per 16 tokens and 8 rows).
+// again, a warp for 32 tokens whose K it converts once (to bf16, which a code times its factor is exactly), against blocks of 64 rows that all warps of the CTA use. The rows
+// come as they are, by asynchronous copies into the operand's layout, a block ahead. That is bound by the matrix instructions (8 per 16 tokens and 8 rows).
 #include "kv4.cuh"
+#include "ptx_sm100.cuh"
 
 namespace b200mx {
 
@@ -12,8 +13,9 @@ namespace {
 
 using namespace kv4;
 
-constexpr uint32_t kWarps = 4, kThreads = 32 * kWarps, kUnit = 32, kTile = kWarps * kUnit, kBlock = 64;   // kBlock: rows at a time
-constexpr float kLog2e = 1.44269504088896341f, kLeast = 1e-37f;
+constexpr uint32_t kWarps = 8, kThreads = 32 * kWarps, kUnit = 32, kTile = kWarps * kUnit, kBlock = 64;   // kBlock: rows at a time
+static_assert(kBlock == 8 * kWarps, "a warp brings 8 rows");
+constexpr float kLog2e = 1.44269504088896341f;
 
 __device__ __forceinline__ void store_weight(const Kv4AttendParams& p, uint32_t bh, uint32_t t, uint32_t length, uint32_t n, float v) {
     const size_t at = static_cast<size_t>(bh) * p.weights_width + t;
@@ -49,10 +51,16 @@ __global__ void __launch_bounds__(256) kv4_add_scores_kernel(const __grid_consta
 }
 
 struct Shared {
-    uint4 q[kBlock / 8][4][32];      // [group of 8 rows][block of elements][lane]: the operand's elements
-    float factor[kBlock], lse[kBlock];
-    uint32_t limit[kBlock];
+    uint4 q[2][kBlock / 8][4][32];   // [buffer][group of 8 rows][block of elements][lane]: the operand's elements
+    float lse[2][kBlock];
+    uint32_t limit[2][kBlock];
 };
+
+// two elements in f16, times f, in bf16
+__device__ __forceinline__ uint32_t times(uint32_t two, float f) {
+    const float2 x = f16x2_to_f32(two);
+    return pack_bf16x2(x.x * f, x.y * f);
+}
 
 __global__ void __launch_bounds__(kThreads) kv4_weigh_kernel(const __grid_constant__ Kv4AttendParams p, uint32_t tiles) {
     __shared__ Shared sh;
@@ -62,10 +70,24 @@ __global__ void __launch_bounds__(kThreads) kv4_weigh_kernel(const __grid_consta
     const uint32_t bh = blockIdx.x / tiles, head = bh % p.c.HK, b = bh / p.c.HK, tile0 = (blockIdx.x - bh * tiles) * kTile, tok0 = tile0 + warp * kUnit;
     const uint32_t length = length_of(p.c, b), n = count_of(p.counts, b, p.S, length), page = 1u << p.c.page_log2, rows = n * p.group;
     if (tile0 >= length) return;   // (the same for the CTA)
-    // A lane's share of the K operand, 16 tokens at a time: the elements 32 blk + 8 tig .. + 7 of the tokens gid and gid + 8, times the block's factor over the token's largest, and
-    // what is left out, 2^(e - kUp), to multiply the scores with
+    // rows that see none of the tile are left out: with a causal mask the first that sees a token of it is token tile0 itself
+    const uint32_t first = p.causal && tile0 > length - n ? (tile0 - (length - n)) * p.group / kBlock * kBlock : 0u;
+    // a warp brings 8 rows: lane (gid, tig) the elements 32 blk + 8 tig .. + 7 of row gid. Rows behind the last become zeros that see nothing.
+    auto bring = [&](uint32_t row0, uint32_t into) {
+        if (row0 >= rows) return;
+        const uint32_t r = 8u * warp + gid, row = row0 + r, i = row / p.group, h = head * p.group + row - i * p.group;
+        const bool live = row < rows;
+        const uint8_t* from = live ? p.q.data + b * p.q.stride_b + i * p.q.stride_s + h * p.q.stride_h + 16u * tig : p.q.data;
+#pragma unroll
+        for (uint32_t blk = 0; blk < 4u; ++blk) sm100::cp_async_16(sm100::smem_u32(&sh.q[into][warp][blk][lane]), from + (live ? 64u * blk : 0u), live ? 16u : 0u);
+        if (tig == 0u) {
+            sm100::cp_async_4(sm100::smem_u32(&sh.lse[into][r]), live ? p.lse + (static_cast<size_t>(b) * p.H + h) * p.S + i : p.lse, live ? 4u : 0u);
+            sh.limit[into][r] = !live ? 0u : p.causal ? length - n + i + 1u : length;
+        }
+    };
+    bring(first, 0u);
+    // A lane's share of the K operand, 16 tokens at a time: the elements 32 blk + 8 tig .. + 7 of the tokens gid and gid + 8
     uint32_t k[2][4][8];
-    float back[2][2];
 #pragma unroll
     for (int gr = 0; gr < 2; ++gr) {
 #pragma unroll
@@ -78,80 +100,46 @@ __global__ void __launch_bounds__(kThreads) kv4_weigh_kernel(const __grid_consta
                 const uint8_t* rec = record_of(p.c, id, head);
                 codes = ld_v4(rec + 64u * (t & (page - 1u)) + 16u * tig), scales = ld_u32(rec + 128u * page + 4u * (t & (page - 1u)));
             }
-            const uint32_t largest = largest_byte(scales);
-            const int e = group_exponent(largest == 255u ? 127u : largest);
-            const ValueFactors f = value_factors(scales, largest, e);
-            back[gr][half] = __uint_as_float(static_cast<uint32_t>(127 + e - kUp) << 23);
-            const uint32_t fs[4] = {__byte_perm(f.r01, 0u, 0x1010), __byte_perm(f.r01, 0u, 0x3232), __byte_perm(f.r23, 0u, 0x1010), __byte_perm(f.r23, 0u, 0x3232)};
 #pragma unroll
             for (int blk = 0; blk < 4; ++blk) {
-                const uint32_t w0 = blk < 2 ? codes.x : codes.y, w1 = blk < 2 ? codes.z : codes.w;
-                k[gr][blk][half] = mul_f16x2(blk & 1 ? e2m1x2_to_f16x2<2>(w0) : e2m1x2_to_f16x2<0>(w0), fs[blk]);
-                k[gr][blk][2 + half] = mul_f16x2(blk & 1 ? e2m1x2_to_f16x2<3>(w0) : e2m1x2_to_f16x2<1>(w0), fs[blk]);
-                k[gr][blk][4 + half] = mul_f16x2(blk & 1 ? e2m1x2_to_f16x2<2>(w1) : e2m1x2_to_f16x2<0>(w1), fs[blk]);
-                k[gr][blk][6 + half] = mul_f16x2(blk & 1 ? e2m1x2_to_f16x2<3>(w1) : e2m1x2_to_f16x2<1>(w1), fs[blk]);
+                const uint32_t w0 = blk < 2 ? codes.x : codes.y, w1 = blk < 2 ? codes.z : codes.w, scale = scales >> (8 * blk) & 0xFFu;
+                const float f = scale == 255u ? __uint_as_float(0x7FC00000u) : __uint_as_float(scale << 23);
+                k[gr][blk][half] = times(blk & 1 ? e2m1x2_to_f16x2<2>(w0) : e2m1x2_to_f16x2<0>(w0), f);
+                k[gr][blk][2 + half] = times(blk & 1 ? e2m1x2_to_f16x2<3>(w0) : e2m1x2_to_f16x2<1>(w0), f);
+                k[gr][blk][4 + half] = times(blk & 1 ? e2m1x2_to_f16x2<2>(w1) : e2m1x2_to_f16x2<0>(w1), f);
+                k[gr][blk][6 + half] = times(blk & 1 ? e2m1x2_to_f16x2<3>(w1) : e2m1x2_to_f16x2<1>(w1), f);
             }
         }
     }
     float sum[2][2] = {{0.0f, 0.0f}, {0.0f, 0.0f}};
-    // rows that see none of the tile are left out: with a causal mask the first that sees a token of it is token tile0 itself
-    const uint32_t first = p.causal && tile0 > length - n ? (tile0 - (length - n)) * p.group / kBlock * kBlock : 0u;
-    for (uint32_t row0 = first; row0 < rows; row0 += kBlock) {
-        __syncthreads();   // the block before is used up
-        // a warp brings 16 rows: lane (gid, tig) the elements 32 blk + 8 tig .. + 7 of row gid of two groups
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-            const uint32_t g = 2u * warp + x, r = 8u * g + gid, row = row0 + r, i = row / p.group, h = head * p.group + row % p.group;
-            const bool live = row < rows;
-            uint4 raw[4];
-            uint32_t amax = 0;
-#pragma unroll
-            for (int blk = 0; blk < 4; ++blk) {
-                raw[blk] = make_uint4(0u, 0u, 0u, 0u);
-                if (live) raw[blk] = ld_v4(p.q.data + b * p.q.stride_b + i * p.q.stride_s + h * p.q.stride_h + 64u * blk + 16u * tig);
-                const uint32_t w[4] = {raw[blk].x, raw[blk].y, raw[blk].z, raw[blk].w};
-#pragma unroll
-                for (int y = 0; y < 4; ++y) amax = max(amax, max((w[y] << 16) & 0x7FFFFFFFu, w[y] & 0x7FFF0000u));
-            }
-            amax = max(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, 1));
-            amax = max(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, 2));
-            const float2 f = row_factors(amax);
-#pragma unroll
-            for (int blk = 0; blk < 4; ++blk) {
-                uint32_t w[4] = {raw[blk].x, raw[blk].y, raw[blk].z, raw[blk].w};
-#pragma unroll
-                for (int y = 0; y < 4; ++y) w[y] = pack_f16x2(__uint_as_float(w[y] << 16) * f.x, __uint_as_float(w[y] & 0xFFFF0000u) * f.x);
-                sh.q[g][blk][lane] = make_uint4(w[0], w[1], w[2], w[3]);
-            }
-            if (tig == 0u) {
-                sh.factor[r] = fmaxf(f.y * p.scale_log2, kLeast);
-                sh.lse[r] = live ? ld_f32(p.lse + (static_cast<size_t>(b) * p.H + h) * p.S + i) * kLog2e : 0.0f;
-                sh.limit[r] = !live ? 0u : p.causal ? length - n + i + 1u : length;
-            }
-        }
-        __syncthreads();
+    uint32_t from = 0;
+    for (uint32_t row0 = first; row0 < rows; row0 += kBlock, from ^= 1u) {
+        sm100::cp_async_wait_all();
+        __syncthreads();   // the block is there, and all are done with the one before
+        bring(row0 + kBlock, from ^ 1u);
         if (tok0 >= length) continue;
         const uint32_t groups = min(kBlock, rows - row0 + 7u) / 8u;
         for (uint32_t g = 0; g < groups; ++g) {
             float d[2][4] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
 #pragma unroll
             for (int blk = 0; blk < 4; ++blk) {
-                const uint4 q = sh.q[g][blk][lane];
+                const uint4 q = sh.q[from][g][blk][lane];
 #pragma unroll
                 for (int gr = 0; gr < 2; ++gr) {
-                    mma_f16(d[gr], k[gr][blk][0], k[gr][blk][1], k[gr][blk][2], k[gr][blk][3], q.x, q.y, d[gr]);
-                    mma_f16(d[gr], k[gr][blk][4], k[gr][blk][5], k[gr][blk][6], k[gr][blk][7], q.z, q.w, d[gr]);
+                    mma_bf16(d[gr], k[gr][blk][0], k[gr][blk][1], k[gr][blk][2], k[gr][blk][3], q.x, q.y, d[gr]);
+                    mma_bf16(d[gr], k[gr][blk][4], k[gr][blk][5], k[gr][blk][6], k[gr][blk][7], q.z, q.w, d[gr]);
                 }
             }
-            const float2 factor = *reinterpret_cast<const float2*>(&sh.factor[8u * g + 2u * tig]), lse = *reinterpret_cast<const float2*>(&sh.lse[8u * g + 2u * tig]);
-            const uint2 limit = *reinterpret_cast<const uint2*>(&sh.limit[8u * g + 2u * tig]);
+            float2 lse = *reinterpret_cast<const float2*>(&sh.lse[from][8u * g + 2u * tig]);
+            const uint2 limit = *reinterpret_cast<const uint2*>(&sh.limit[from][8u * g + 2u * tig]);
+            lse.x *= kLog2e, lse.y *= kLog2e;
 #pragma unroll
             for (int gr = 0; gr < 2; ++gr) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const uint32_t t = tok0 + 16u * gr + 8u * (i >> 1) + gid;
-                    const float w = ex2(fmaf(d[gr][i] * back[gr][i >> 1], i & 1 ? factor.y : factor.x, -(i & 1 ? lse.y : lse.x)));
-                    sum[gr][i >> 1] += t < (i & 1 ? limit.y : limit.x) ? w : 0.0f;
+                    const float w = ex2(fmaf(d[gr][i], p.scale_log2, -(i & 1 ? lse.y : lse.x)));
+                    if (t < (i & 1 ? limit.y : limit.x)) sum[gr][i >> 1] += w;
                 }
             }
         }

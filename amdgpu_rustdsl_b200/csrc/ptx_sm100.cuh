@@ -174,10 +174,13 @@ __device__ __forceinline__ bool elect_one_sync() {
     return pred != 0;
 }
 
-// ----------------------------------------------------------------------------------------------- 4-byte asynchronous copies
-// global -> shared (generic proxy); with `bytes` 0 nothing is read and the word becomes 0
+// ----------------------------------------------------------------------------------------------- 4- and 16-byte asynchronous copies
+// global -> shared (generic proxy); with `bytes` 0 nothing is read and the words become 0
 __device__ __forceinline__ void cp_async_4(uint32_t dst, const void* src, uint32_t bytes) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_async_16(uint32_t dst, const void* src, uint32_t bytes) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
 // one arrival on `bar` (already in its count) when this thread's copies so far have landed
 __device__ __forceinline__ void cp_async_arrive(uint32_t bar) { asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory"); }

@@ -225,11 +225,12 @@ __global__ void __launch_bounds__(256) kv4_move_kernel(const __grid_constant__ K
 }  // namespace
 
 cudaError_t launch_kv4_evict(const Kv4EvictParams& p, cudaStream_t stream) {
-    // CTAs of a (sequence, head): as many as fill the machine, two an SM, or as the longest sequence needs to keep its keys in registers
+    // CTAs of a (sequence, head): as many as there are SMs for (8 items of 16384 tokens: 23.1 us with 8, 27.9 with the 2 that hold the keys; 128 items of 4096 tokens: 44.0 with 1,
+    // 46.0 with 2), or as the longest sequence needs to keep its keys in registers (256 items of 16384 tokens: 166 us with 2, 174 with 1 that reads them again)
     const uint64_t tokens = static_cast<uint64_t>(p.from.table_width) << p.from.page_log2;
     const uint32_t items = p.from.B * p.from.HK, sms = static_cast<uint32_t>(current_sm_count());
     uint32_t ctas = 1;
-    while (ctas < kMostCtas && (items * ctas * 2u <= 2u * sms || tokens > static_cast<uint64_t>(ctas) * kHeld * kThreads)) ctas *= 2u;
+    while (ctas < kMostCtas && (items * ctas * 2u <= sms || tokens > static_cast<uint64_t>(ctas) * kHeld * kThreads)) ctas *= 2u;
     while (ctas > 1u && tokens < static_cast<uint64_t>(ctas) * 256u) ctas /= 2u;   // (no runs of less than 256 tokens)
     const bool held = tokens <= static_cast<uint64_t>(ctas) * kHeld * kThreads;
     cudaLaunchConfig_t cfg = {};

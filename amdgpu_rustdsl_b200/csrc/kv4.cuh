@@ -174,6 +174,11 @@ __device__ __forceinline__ uint32_t mul_f16x2(uint32_t a, uint32_t b) {
     asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
     return r;
 }
+__device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
 // Softmax of rows that multiply V in f16. V's factors of a group of tokens that are worked on together are taken relative to 2^e, e the exponent of the group's largest, kept
 // within what f32 sums of 2^(s - M) bear (they lie between 2^-kHighE and 2^(8 - kLowE) a token when M follows s + e). The factors go in times 2^kUp, which the division
 // by the sums takes out again: f16 has more room below 1 than above, and factors are exact down to 2^-34 of the group's largest.

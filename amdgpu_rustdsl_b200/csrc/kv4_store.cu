@@ -36,34 +36,30 @@ __device__ __forceinline__ uint2 row_and_head(const StoreParams& p, uint32_t r) 
 __device__ __forceinline__ void append_row(const uint4 raw, uint8_t* record, uint32_t page, uint32_t slot, bool is_v) {
     const unsigned part = threadIdx.x & 15u, blk = part >> 2, tig = part & 3u;
     const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
-    // the block's largest magnitude, as the bits of an f32 (ordered as integers; Inf and NaN come out on top)
-    uint32_t amax = 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) amax = max(amax, max((w[i] << 16) & 0x7FFFFFFFu, w[i] & 0x7FFF0000u));
-    amax = max(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, 1));
-    amax = max(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, 2));
-    const uint32_t field = amax >> 23;
+    // the block's largest magnitude, as bf16 bits (ordered as integers; Inf and NaN come out on top)
+    uint32_t amax = __vmaxu2(__vmaxu2(w[0] & 0x7FFF7FFFu, w[1] & 0x7FFF7FFFu), __vmaxu2(w[2] & 0x7FFF7FFFu, w[3] & 0x7FFF7FFFu));
+    amax = __vmaxu2(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, 1));
+    amax = __vmaxu2(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, 2));
+    const uint32_t field = max(amax >> 23, amax >> 7 & 255u);
     const bool broken = field == 255u;
     const uint32_t e = broken ? 255u : (field < 3u ? 1u : field - 2u);
-    // x * 2^(127 - E), exact up to what rounds to a code of 0 anyway; 127 - E lies in [-125, 126]
-    const float up = broken ? 0.0f : __uint_as_float((254u - e) << 23);
+    // x * 2^(127 - E) in bf16, exact up to what rounds to a code of 0 anyway; 127 - E lies in [-125, 126]
+    const uint32_t up = ((254u - e) << 7) * 0x10001u;
     uint32_t code[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) code[i] = broken ? 0u : f32x2_to_e2m1x2(__fmul_rn(__uint_as_float(w[i] << 16), up), __fmul_rn(__uint_as_float(w[i] & 0xFFFF0000u), up));
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t x = mul_bf16x2(w[i], up);
+        code[i] = f32x2_to_e2m1x2(__uint_as_float(x << 16), __uint_as_float(x & 0xFFFF0000u));
+    }
     // elements 32 blk + 8 tig ..: bytes 0, 1 belong to group g = 2 tig, bytes 2, 3 to group 2 tig + 1; a group's bytes 2 blk, 2 blk + 1. Lanes of an even and an
     // odd block swap halves, so that each holds a word of one group: lane (blk, tig) word 4 tig + 2 (blk & 1) + (blk >> 1)
-    const uint32_t lo = code[0] | (code[1] << 8), hi = code[2] | (code[3] << 8);
-    const bool odd = blk & 1u;
-    const uint32_t got = __shfl_xor_sync(0xFFFFFFFFu, odd ? lo : hi, 4);
-    const uint32_t word = odd ? (got | (hi << 16)) : (lo | (got << 16));
-    // the row's four scale bytes
-    uint32_t scales = e << (8u * blk);
-    scales |= __shfl_xor_sync(0xFFFFFFFFu, scales, 4);
-    scales |= __shfl_xor_sync(0xFFFFFFFFu, scales, 8);
+    uint32_t word = __byte_perm(__byte_perm(code[0], code[1], 0x0040), __byte_perm(code[2], code[3], 0x0040), 0x5410);
+    if (broken) word = 0u;
+    word = __byte_perm(word, __shfl_xor_sync(0xFFFFFFFFu, word, 4), blk & 1u ? 0x3276 : 0x5410);
     if (record != nullptr) {
         uint8_t* codes = record + (is_v ? 64u * page : 0u) + 64u * slot;
         *reinterpret_cast<uint32_t*>(codes + 4u * (4u * tig + 2u * (blk & 1u) + (blk >> 1))) = word;
-        if (part == 0u) *reinterpret_cast<uint32_t*>(record + (is_v ? 132u : 128u) * page + 4u * slot) = scales;
+        if (tig == 0u) record[(is_v ? 132u : 128u) * page + 4u * slot + blk] = static_cast<uint8_t>(e);
     }
 }
 
@@ -100,14 +96,21 @@ __global__ void __launch_bounds__(256) kv4_append_kernel(const __grid_constant__
     }
 }
 
-// 8 elements of a row: two bytes each of the two groups of this lane, and the block's factor
-__device__ __forceinline__ uint4 values_of(uint32_t word, float scale) {
-    const float2 a = f16x2_to_f32(e2m1x2_to_f16x2<0>(word)), b = f16x2_to_f32(e2m1x2_to_f16x2<1>(word));
-    const float2 c = f16x2_to_f32(e2m1x2_to_f16x2<2>(word)), d = f16x2_to_f32(e2m1x2_to_f16x2<3>(word));
-    return make_uint4(pack_bf16x2(a.x * scale, a.y * scale), pack_bf16x2(b.x * scale, b.y * scale), pack_bf16x2(c.x * scale, c.y * scale), pack_bf16x2(d.x * scale, d.y * scale));
+// a pair of codes as f16 times the block's factor (twice in `scale`), in bf16
+__device__ __forceinline__ uint32_t value_pair(uint32_t two, unsigned long long scale) {
+    const float2 x = f16x2_to_f32(two);
+    unsigned long long y;
+    float lo, hi;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(y) : "f"(x.x), "f"(x.y));
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(y) : "l"(y), "l"(scale));
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(y));
+    return pack_bf16x2(lo, hi);
 }
-__device__ __forceinline__ uint32_t two_groups(const uint8_t* p) {
-    return *reinterpret_cast<const volatile uint16_t*>(p) | (static_cast<uint32_t>(*reinterpret_cast<const volatile uint16_t*>(p + 8)) << 16);
+// 8 elements of a row
+__device__ __forceinline__ uint4 values_of(uint32_t word, float scale) {
+    unsigned long long both;
+    asm("mov.b64 %0, {%1, %1};" : "=l"(both) : "f"(scale));
+    return make_uint4(value_pair(e2m1x2_to_f16x2<0>(word), both), value_pair(e2m1x2_to_f16x2<1>(word), both), value_pair(e2m1x2_to_f16x2<2>(word), both), value_pair(e2m1x2_to_f16x2<3>(word), both));
 }
 
 __global__ void __launch_bounds__(256) kv4_read_kernel(const __grid_constant__ StoreParams p) {
@@ -131,14 +134,16 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(const __grid_constant__ S
             word[k][0] = word[k][1] = sc[k][0] = sc[k][1] = 0u;
             if (id[k] >= 0) {
                 const uint32_t slot = (t0 + at[k].x) & (page - 1u);
-                const uint8_t *record = record_of(p.c, id[k], at[k].y), *codes = record + 64u * slot + 16u * tig + 2u * blk, *scales = record + 128u * page + 4u * slot;
-                word[k][0] = two_groups(codes), word[k][1] = two_groups(codes + 64u * page);
+                const uint8_t *record = record_of(p.c, id[k], at[k].y), *codes = record + 64u * slot + 4u * (4u * tig + 2u * (blk & 1u) + (blk >> 1)), *scales = record + 128u * page + 4u * slot;
+                word[k][0] = ld_u32(codes), word[k][1] = ld_u32(codes + 64u * page);
                 sc[k][0] = ld_u32(scales), sc[k][1] = ld_u32(scales + 4u * page);
             }
         }
 #pragma unroll
         for (int k = 0; k < kRows; ++k) {
             const uint32_t r = first + 16u * k;
+#pragma unroll
+            for (int x = 0; x < 2; ++x) word[k][x] = __byte_perm(word[k][x], __shfl_xor_sync(0xFFFFFFFFu, word[k][x], 4), blk & 1u ? 0x3276 : 0x5410);   // (as in append_row)
             if (r >= p.rows) continue;
             const bool lost = id[k] < 0 && r < rows;
 #pragma unroll

@@ -14,6 +14,11 @@
 // Softmax in base 2 with a running reference per row. P V wants P times V's factor in f16: the reference M follows s + e, e the exponent of the largest V factor of
 // the 32 tokens, so that P 2^e is at most 2^4 however large V is; the factors relative to 2^e are exact in f16 down to 2^-34. M moves when a value exceeds it by more
 // than 2^4, by a vote of the warp; the sums and O are rescaled then.
+//
+// With one group of 8 columns the instruction stream is the bound, not the bytes: 64 sequences x 8 heads of 16384 tokens take 236 us, 4.8 TB/s of the 6.5 that a copy reaches; 594
+// instructions per 32 tokens of a warp (301 of them conversions, packing and logic, a pipe at half rate), issued in 55 % of the cycles. Four CTAs an SM are what the registers
+// allow; three of them took 226 us there but 71 in place of 68 on ragged sequences in pages of 16, five and six with two stages 470 to 610 (spills).
+// Groups of 8 rows more cost their products and softmax: 32 rows over 16 x 4096 tokens 65 us, against 100 with the tiles of 128 rows.
 #include "kv4.cuh"
 #include "kv4_schedule.cuh"
 #include "ptx_sm100.cuh"
@@ -495,8 +500,8 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : NT == 2 ? 3 : 2) kv4_a
 
 // Puts the items together that more than one CTA of a launch worked on: blockIdx.x is an entry of the workspace, parts come from a launch of `grid` CTAs. kTogether: a CTA of so many
 // warps has one row, its warps the parts in turn; 0: a warp has a row and all of its parts. Four parts are in flight at a time. (The CTAs take little shared memory on
-// purpose: with 8 KB in place of 2 the attention kernel behind this one took 272 us in place of 236, 64
-// sequences of 16384 tokens.)
+// purpose: with 8 KB in place of 2 the attention kernel behind this one took 272 us in place of
+// 236, 64 sequences of 16384 tokens.)
 template <uint32_t kTogether>
 __global__ void __launch_bounds__(kTogether ? 32 * kTogether : 256) kv4_combine_kernel(const __grid_constant__ Kv4AttendParams p, uint32_t rows, uint32_t row_tiles, uint32_t grid) {
     __shared__ float sm_m[kTogether ? kTogether : 1u], sm_l[kTogether ? kTogether : 1u];
@@ -570,7 +575,9 @@ __global__ void __launch_bounds__(kTogether ? 32 * kTogether : 256) kv4_combine_
     if (p.lse != nullptr && lane == 0u) p.lse[(static_cast<size_t>(b) * p.H + h) * p.S + i] = none ? -INFINITY : (m + lg2(l)) * kLn2;
 }
 
-constexpr uint32_t kMostFew = 32;   // rows of a KV head from which on the tensor cores' tiles of 128 rows take over
+// Rows of a KV head up to which this kernel is taken; more go to the tensor cores' tiles of 128 rows. 16 sequences of 4096 tokens: 20 rows 49 us here and 100 there, 32 rows 65 and 100;
+// one of 65536: 28 and 66, 34 and 67. (The registers end at 32: two passes over the cache would cost as much as the tiles do from about 48 rows on.)
+constexpr uint32_t kMostFew = 32;
 
 uint32_t groups_of(uint32_t rows) { return (rows + 7u) / 8u; }
 
@@ -595,7 +602,7 @@ cudaError_t launch_rows(const Kv4AttendParams& p, cudaStream_t stream) {
     }
     e = kv4_launch(kv4_attend_kernel<NT>, dim3(grid), kThreads, smem, stream, p);
     if (e != cudaSuccess) return e;
-    // 4 warps have 16 parts in flight; where an item has more on average, 16 warps (5 rows over 65536 tokens, 74 parts: 28.4 us in place of 31)
+    // 4 warps have 16 parts in flight; where an item has more on average, 16 warps (5 rows over 65536 tokens, 74 parts: 28 us in place of 36)
     const uint32_t entries = begun_entries(p.c, 1u, grid), some = rows < 8u * NT ? rows : 8u * NT;
     if (grid / entries > 16u) return kv4_launch(kv4_combine_kernel<16>, dim3(entries, some), 512u, 0, stream, p, 8u * NT, 1u, grid);
     return kv4_launch(kv4_combine_kernel<4>, dim3(entries, some), 128u, 0, stream, p, 8u * NT, 1u, grid);
@@ -613,7 +620,8 @@ uint64_t partial_bytes(const Kv4View& c, uint32_t rows) {
     return kv4_partial_bytes(attend_grid(c, groups_of(rows)), 8u * groups_of(rows));
 }
 uint64_t lse_bytes(const Kv4View& c, uint32_t S, uint32_t H) { return (static_cast<uint64_t>(c.B) * S * H * 4u + 15u) & ~15ull; }
-// Up to 8 rows leave their scores for the weights, at 4 bytes a row and token; with more it costs less to compute them again
+// Up to 8 rows leave their scores for the weights, at 4 bytes a row and token (16 sequences of 4096 tokens: 4 rows 38 us, 69 where they are computed again; 8 rows 42 and 71). More rows
+// would fill the memory with scores, 4 bytes against the 17 of a token's K and V per row in the group; they are computed again.
 uint64_t score_bytes(const Kv4View& c, uint32_t rows) {
     return rows > 8u ? 0u : (static_cast<uint64_t>(c.B) * c.HK * c.table_width << c.page_log2) * ((rows + 1u) & ~1u) * 4u;
 }

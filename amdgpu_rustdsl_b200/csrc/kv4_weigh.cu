@@ -3,7 +3,9 @@
 //
 // With up to 8 rows the attention kernel has left the scores (a token's all in one 8- to 32-byte piece), and a thread adds up a token's. With more rows S^T = K Q^T is computed
 // again, a warp for 32 tokens whose K it converts once (to bf16, which a code times its factor is exactly), against blocks of 64 rows that all warps of the CTA use. The rows
-// come as they are, by asynchronous copies into the operand's layout, a block ahead. That is bound by the matrix instructions (8 per 16 tokens and 8 rows).
+// come as they are, by asynchronous copies into the operand's layout, a block ahead. That is bound by the matrix instructions (8 per 16 tokens and 8 rows): 400 rows
+// over four ragged sequences of up to 4001 tokens, 8 heads, 32 us where the instructions' rate gives about 15 and two uneven rounds of CTAs twice that; 46 us before the rows
+// were copied as they are, 35 with CTAs of half the tokens.
 #include "kv4.cuh"
 #include "ptx_sm100.cuh"
 

@@ -8,7 +8,7 @@
  *   [ 64 * page  K codes | 64 * page  V codes | 4 * page  K scales | 4 * page  V scales ]
  *
  * A token's 128 elements of K (or V) are OCP MXFP4: 64 bytes of e2m1 codes and four E8M0 scales, one per 32 elements; value = code * 2^(scale - 127).
- * Scale 255 makes the block's elements NaN, scale 0 makes them zero. Byte 8 g + 2 b + r of the 64 holds the elements 32 b + 4 g + 2 r (low nibble)
+ * Scale 255 with codes of 0, as append writes it, makes the block's elements NaN, scale 0 makes them zero. Byte 8 g + 2 b + r of the 64 holds the elements 32 b + 4 g + 2 r (low nibble)
  * and 32 b + 4 g + 2 r + 1: with it a lane of the matrix instructions' operand layouts finds its elements of all four blocks side by side, for K
  * (16 bytes) and for V (8 bytes) alike, and a token's bytes are its own, so that appending one token never rewrites a neighbour's byte.
  *
@@ -63,6 +63,8 @@ int fmha_kv4_read(const fmha_kv4_cache* cache, const fmha_kv4_rows* k, const fmh
  *   weights: NULL or f32 [B][HK][weights_width]: weights[b][kv][t] = old + (sum of the softmax weights of token t over the rows and the query heads of the
  *     KV head), for t < length; nothing is written behind the length. old = weights_in[b][kv][t] (same width; may be the same array), 0 where weights_in is
  *     NULL and, with `causal`, for the n newest tokens. Sums in a fixed order: the same bits every time.
+ *   Ranges: the products run in f16 against powers of two that are taken out, so that any scale goes. What is exact is a query row's elements down to 2^-30 of its largest,
+ *     V's down to 2^-33 of the largest scale among 32 neighbouring tokens (128 with more than 32 query rows of a KV head, then K's as well); smaller ones count as less.
  *   workspace: fmha_kv4_attend_workspace() bytes of device memory, 16-byte aligned; scratch, no initial contents.
  */
 typedef struct fmha_kv4_attend_args {

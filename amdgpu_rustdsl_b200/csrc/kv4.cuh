@@ -184,6 +184,8 @@ __device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
 // by the sums takes out again: f16 has more room below 1 than above, and factors are exact down to 2^-34 of the group's largest.
 constexpr int kLowE = -100, kHighE = 124, kUp = 10;
 constexpr float kDown = 1.0f / (1 << kUp);
+// 0xFF in the place of the scale bytes that stand for NaN
+__device__ __forceinline__ uint32_t nan_bytes(uint32_t word) { return __vcmpeq4(word, 0xFFFFFFFFu); }
 // the largest of a token's four scale bytes
 __device__ __forceinline__ uint32_t largest_byte(uint32_t word) { return max(max(word & 0xFFu, (word >> 8) & 0xFFu), max((word >> 16) & 0xFFu, word >> 24)); }
 __device__ __forceinline__ int group_exponent(uint32_t largest) { return min(max(static_cast<int>(largest) - 127, kLowE), kHighE); }

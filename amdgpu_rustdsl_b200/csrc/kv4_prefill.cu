@@ -35,6 +35,9 @@ using namespace sm100;
 constexpr uint32_t kTileRows = 128, kItemRows = 256, kStages = 2, kHalf = 64;
 // Slots of the steps' exponents. The converters write those of step j + 4 behind the scores of step j + 2, which are behind the P of step j + 1 of the tiles that go on
 constexpr uint32_t kFactorSlots = 4;
+// Slots of the segments' blocks of NaN. The converters begin segment n behind its step's third forerunner, whose scores both issuing warps have issued: these are in segment n - 3 at least,
+// and an issuing warp begins a segment when its tile's softmax has stored the one before
+constexpr uint32_t kNanSlots = 4;
 constexpr uint32_t kAtomBytes = 128u * 128u, kTileBytes = 2u * kAtomBytes;   // 128 rows x 64 elements with 128-byte swizzle; two of them a tile
 constexpr uint32_t kThreads = 512;
 // Warps 0-3 and 4-7: softmax of tile 0 and 1; 8-11: codes to f16; 12 and 13: products of tile 0 and 1. The pools of setmaxnreg come out of the launch's 128 registers a thread.
@@ -51,12 +54,14 @@ enum Bar : uint32_t { kKFull = 0, kKEmpty = 2, kVFull = 4, kVEmpty = 6, kSFull =
 struct Shared {
     uint8_t q[2][kTileBytes], k[kStages][kTileBytes], v[kStages][kTileBytes];
     uint4 most[kFactorSlots][2];   // the largest scale byte of K and of V that each of the converting warps met
+    uint4 nan_from[kNanSlots][4];  // of a segment and a converting warp: the first token that has NaN in each block of its V, all ones where none has
     unsigned long long bars[kBars];
     Sums part[kThreads / 32];
     struct Plan {
         Segment seg;
-        uint32_t pos, length, n;
+        uint32_t pos, length, n, number;   // (segments are counted from 1)
     } plan[8];                     // of a softmax warp's next segment
+    uint32_t converting[4];        // number of a converting warp's segment
     uint32_t tmem, failed, not_drained;
 };
 
@@ -105,6 +110,16 @@ __device__ __forceinline__ void store_row(uint8_t* tile, uint32_t row, const uin
     }
 }
 
+// The first of a warp's 32 tokens, from token `from` on, with NaN in a block of its V (0xFF in that byte of `nan`), where none before had it
+__device__ __forceinline__ void note_nan(uint4& first, uint32_t nan, uint32_t from) {
+    uint32_t* at = reinterpret_cast<uint32_t*>(&first);
+#pragma unroll 1
+    for (uint32_t x = 0; x < 4u; ++x) {
+        const uint32_t has = __ballot_sync(0xFFFFFFFFu, (nan >> (8u * x) & 1u) != 0u);
+        if ((threadIdx.x & 31u) == 0u && has != 0u && at[x] == 0xFFFFFFFFu) at[x] = from + static_cast<uint32_t>(__ffs(static_cast<int>(has))) - 1u;
+    }
+}
+
 __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_constant__ Kv4AttendParams p, uint32_t row_tiles) {
     extern __shared__ uint8_t smem_raw[];
     Shared& sh = *reinterpret_cast<Shared*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023u) & ~static_cast<uintptr_t>(1023u));
@@ -123,6 +138,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
         
         fence_mbar_init();
         sh.failed = sh.not_drained = 0u;
+        for (uint32_t i = 0; i < 8; ++i) sh.plan[i].number = sh.converting[i & 3u] = 0u;
     }
     if (warp == 12u) tmem_alloc(smem_u32(&sh.tmem), 512u);
     tc_fence_before_sync();
@@ -157,7 +173,10 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
                 x.pos = end - left;
                 x.seg = next_segment(p, deal, at, left);
                 x.length = length_of(p.c, x.seg.b), x.n = count_of(p.counts, x.seg.b, p.S, x.length);
-                if (lane == 0u) sh.plan[warp] = x;
+                if (lane == 0u) {
+                    x.number = sh.plan[warp].number + 1u;
+                    sh.plan[warp] = x;
+                }
                 __syncwarp();
             };
             auto ask_rows = [&](const Segment& seg, uint32_t n) {
@@ -182,8 +201,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
                 if (!ok) break;
                 if (threadIdx.x == 0u) begin_item(p, deal, seg, pos, all, n_work);
                 const uint32_t steps = tile_steps(p, seg, q, length, n), row = seg.row0 + q * kTileRows + r, i = row / p.group;
-                const bool exists = row < p.S * p.group, live = exists && i < n;
-                const uint32_t limit = !live ? 0u : p.causal ? length - n + i + 1u : length;
+                const bool exists = row < p.S * p.group;
+                const uint32_t limit = !exists || i >= n ? 0u : p.causal ? length - n + i + 1u : length;
                 float m = kLowest, l = 0.0f, c_row = 0.0f;
                 {
                     uint32_t amax[8];   // sizes as bf16 bits, of rows 2 x and 2 x + 1 of pairs of loads in the halves
@@ -313,6 +332,16 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
                 const bool whole = done.steps == done.of, none = l == 0.0f;   // NaN is something
                 const uint32_t h = done.head * p.group + row % p.group;
                 const float factor = whole ? (none ? 0.0f : kDown / l) : kDown;
+                // Blocks of V's NaN went into the product as 0, where NaN would meet the weights of 0 of rows that do not see it. A row sees the tokens in front of its limit.
+                uint32_t nan_blocks = 0;
+                if (steps > 0u) {
+                    const uint32_t number = sh.plan[warp].number - (more ? 1u : 0u);   // (the plan is already the next segment's)
+#pragma unroll
+                    for (uint32_t w = 0; w < 4u; ++w) {
+                        const uint4 from = sh.nan_from[number % kNanSlots][w];
+                        nan_blocks |= (from.x < limit ? 1u : 0u) | (from.y < limit ? 2u : 0u) | (from.z < limit ? 4u : 0u) | (from.w < limit ? 8u : 0u);
+                    }
+                }
                 const uint32_t at_row = exists ? (done.b * p.S + i) * p.H + h : 0xFFFFFFFFu;   // of out, in rows
                 float* slot = slot_of(p.ws, gridDim.x, blockIdx.x, done.first == 0u ? 1u : 0u, kItemRows);
                 // O by 64 columns: a thread writes its row's to shared memory, and the warp stores whole pieces of rows
@@ -321,6 +350,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
 #pragma unroll
                     for (uint32_t k = 0; k < 2u; ++k) {
                         uint32_t o[32];
+                        const float f = nan_blocks >> (2u * c + k) & 1u ? __uint_as_float(0x7FC00000u) : factor;
                         if (steps > 0u) {
                             tmem_ld32(t_o + 64u * c + 32u * k, o);
                             tmem_wait_ld();
@@ -331,7 +361,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
                         }
 #pragma unroll
                         for (uint32_t x = 0; x < 8u; ++x) {
-                            float4 v = make_float4(__uint_as_float(o[4 * x]) * factor, __uint_as_float(o[4 * x + 1]) * factor, __uint_as_float(o[4 * x + 2]) * factor, __uint_as_float(o[4 * x + 3]) * factor);
+                            float4 v = make_float4(__uint_as_float(o[4 * x]) * f, __uint_as_float(o[4 * x + 1]) * f, __uint_as_float(o[4 * x + 2]) * f, __uint_as_float(o[4 * x + 3]) * f);
                             if (none) v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
                             *reinterpret_cast<float4*>(mine + lane * 256u + (((8u * k + x) ^ (lane & 15u)) << 4)) = v;
                         }
@@ -361,7 +391,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
                 }
                 if (whole) {
                     if (exists && p.lse != nullptr) p.lse[(static_cast<size_t>(done.b) * p.H + h) * p.S + i] = none ? -INFINITY : (m + lg2(l)) * kLn2;
-                } else if (live) {
+                } else if (limit != 0u) {
                     *reinterpret_cast<float2*>(slot + kItemRows * 128u + 2u * (q * kTileRows + r)) = make_float2(m, l);
                 }
             }
@@ -372,6 +402,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
             bool ok = true;
             while (left > 0u && ok) {
                 const Segment seg = next_segment(p, deal, at, left);
+                if (lane == 0u) sh.nan_from[++sh.converting[warp & 3u] % kNanSlots][warp & 3u] = make_uint4(0xFFFFFFFFu, 0xFFFFFFFFu, 0xFFFFFFFFu, 0xFFFFFFFFu);
                 const uint32_t length = length_of(p.c, seg.b), n = count_of(p.counts, seg.b, p.S, length);
                 // the token of this thread in step j: its page, looked up a step ahead of its bytes
                 long long page_ahead = -1;
@@ -403,9 +434,15 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
                 look_up(1u);
                 for (uint32_t j = 0; j < seg.steps; ++j, ++step) {
                     const uint32_t st = step % kStages, parity = (step / kStages + 1u) & 1u, slot = step % kFactorSlots;
-                    // A token behind the length must not bring NaN into P V; one that is lost, or whose V is NaN, makes the rows that see it NaN by its scores
-                    const uint32_t top_k = empty || lost ? 0u : largest_byte(ks), top_v = empty || lost ? 0u : largest_byte(vs);
-                    const uint32_t met_k = __reduce_max_sync(0xFFFFFFFFu, top_k == 255u ? 0u : top_k), met_v = __reduce_max_sync(0xFFFFFFFFu, top_v == 255u ? 0u : top_v);
+                    // A token behind the length must not bring NaN into P V; one that is lost makes the rows that see it NaN by its scores
+                    const uint32_t top_k = empty || lost ? 0u : largest_byte(ks), met_k = __reduce_max_sync(0xFFFFFFFFu, top_k == 255u ? 0u : top_k);
+                    uint32_t top_v = empty || lost ? 0u : largest_byte(vs), met_v = __reduce_max_sync(0xFFFFFFFFu, top_v);
+                    if (met_v == 255u) {   // NaN in V: the first token of each block is noted, and its scale becomes 0
+                        const uint32_t nan = empty || lost ? 0u : nan_bytes(vs);
+                        note_nan(sh.nan_from[sh.converting[warp & 3u] % kNanSlots][warp & 3u], nan, (seg.first + j) * kStepTokens + (r & 96u));
+                        vs &= ~nan;
+                        top_v = empty || lost ? 0u : largest_byte(vs), met_v = __reduce_max_sync(0xFFFFFFFFu, top_v);
+                    }
                     if (lane == 0u) reinterpret_cast<uint32_t*>(&sh.most[slot][0])[warp & 3u] = met_k, reinterpret_cast<uint32_t*>(&sh.most[slot][1])[warp & 3u] = met_v;
                     // (also where a wait has run out in one of the four warps: they leave together)
                     ok = named_bar_all(1u, 128u, ok);
@@ -414,7 +451,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
                     const uint4 mk = sh.most[slot][0], mv = sh.most[slot][1];
                     ValueFactors fk = value_factors(ks, top_k, group_exponent(max(max(mk.x, mk.y), max(mk.z, mk.w))));
                     ValueFactors fv = value_factors(vs, top_v, group_exponent(max(max(mv.x, mv.y), max(mv.z, mv.w))));
-                    if (empty || lost || top_v == 255u) {
+                    if (empty || lost) {
                         fk.r01 = fk.r23 = empty ? 0u : 0x7E007E00u, fv.r01 = fv.r23 = 0u;   // (the codes are whatever they were: finite)
                     }
                     ok = mbar_wait(bar(kKEmpty + st), parity, failed);

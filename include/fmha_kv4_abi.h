@@ -63,6 +63,7 @@ int fmha_kv4_read(const fmha_kv4_cache* cache, const fmha_kv4_rows* k, const fmh
  *   weights: NULL or f32 [B][HK][weights_width]: weights[b][kv][t] = old + (sum of the softmax weights of token t over the rows and the query heads of the
  *     KV head), for t < length; nothing is written behind the length. old = weights_in[b][kv][t] (same width; may be the same array), 0 where weights_in is
  *     NULL and, with `causal`, for the n newest tokens. Sums in a fixed order: the same bits every time.
+ *   NaN: a block of V that is NaN makes its 32 elements NaN in the rows that see the token, whatever the weight, and nothing else; NaN in K makes all of these rows NaN.
  *   Ranges: the products run in f16 against powers of two that are taken out, so that any scale goes. What is exact is a query row's elements down to 2^-30 of its largest,
  *     V's down to 2^-33 of the largest scale among 32 neighbouring tokens (128 with more than 32 query rows of a KV head, then K's as well); smaller ones count as less.
  *   workspace: fmha_kv4_attend_workspace() bytes of device memory, 16-byte aligned; scratch, no initial contents.

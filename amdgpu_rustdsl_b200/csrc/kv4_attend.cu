@@ -158,7 +158,9 @@ __device__ __forceinline__ int token_factors(TokenFactors& f, uint32_t kw, uint3
     f.k[t] = make_float4(scale_f32(kw, 0), scale_f32(kw, 1), scale_f32(kw, 2), scale_f32(kw, 3));
     if (!live) vw = 0u;
     const uint32_t largest = largest_byte(vw);
-    const int e = group_exponent(__reduce_max_sync(0xFFFFFFFFu, largest == 255u ? 0u : largest));
+    uint32_t met = largest;
+    if (largest == 255u) met = largest_byte(vw & ~nan_bytes(vw));   // (a token's other blocks count)
+    const int e = group_exponent(__reduce_max_sync(0xFFFFFFFFu, met));
     const ValueFactors vf = value_factors(vw, largest, e);
     // an even lane takes blocks 0 and 1 of its pair, the odd one 2 and 3; pairs whose operand rows are the other way round are stored so
     const bool odd = t & 1u, flip = (t >> 1) & 1u;

@@ -79,3 +79,9 @@ def test_a_block_of_a_token(S, group, page, causal):
 def test_where_items_are_cut_between_ctas(S, group):
     """A long sequence whose partial results are put together, rows that stand for nothing beside it."""
     check([3001, 600], 1, group, S, 64, [(0, 0, 1500, 1, 1.0), (0, 0, 2998, 2, 1.0), (1, 0, 599, 0, 1.0)], True, counts=[S, min(S, 3)])
+
+
+@pytest.mark.parametrize("S,group,page", SHAPES)
+def test_the_blocks_beside_it_may_be_larger_than_everything_around(S, group, page):
+    """What is left of the token counts with its own scales: alone among 32 and 128 tokens, and 2^20 times what the tokens beside it hold."""
+    check([129, 33, 200], 2, group, S, page, [(0, 0, 128, 2, 1.0), (1, 1, 32, 0, 1.0), (2, 0, 77, 1, 2.0 ** 20), (2, 1, 199, 3, 2.0 ** 20)], True)

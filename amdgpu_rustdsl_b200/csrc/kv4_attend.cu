@@ -40,6 +40,7 @@ static_assert(kStages - 1 <= kWarps, "a warp for each of the first tiles");
 constexpr unsigned kTileBytes = kTile * FMHA_KV4_TOKEN_BYTES;
 constexpr float kSlack = 4.0f;
 constexpr float kLeast = 1e-37f;                  // of a row's factor: times a masked score it is still -inf
+constexpr float kVanishes = 2.98023223876953125e-8f;   // 2^-25: becomes 0 in f16
 constexpr float kLn2 = 0.69314718055994531f;
 
 // What a unit's 32 lanes work out for its tokens, one lane a token
@@ -269,6 +270,7 @@ __device__ __forceinline__ void attend_unit(float (&o)[NT][8][4], float (&m)[NT]
             for (int i = 0; i < 4; ++i) {
                 w[i] = ex2(fmaf(s[gr][g][i], x.factor[g][i & 1], ef - m[g][i & 1]));
                 sum[g][i & 1] += w[i];
+                if (kEdge && w[i] <= kVanishes && s[gr][g][i] != -INFINITY) w[i] = -0.0f;   // seen all the same: 0 is for masked tokens
             }
             pt[g][0] = transpose_8x8(pack_f16x2(w[0], w[1]));
             pt[g][1] = transpose_8x8(pack_f16x2(w[2], w[3]));
@@ -298,9 +300,9 @@ __device__ __forceinline__ void attend_unit(float (&o)[NT][8][4], float (&m)[NT]
 #pragma unroll
                 for (int g = 0; g < NT; ++g) {
                     uint32_t p0 = mul_f16x2(pt[g][0], r0), p1 = mul_f16x2(pt[g][1], r1);
-                    if (kEdge) {   // a weight of 0 hides what it multiplies, NaN too
-                        p0 = (pt[g][0] & 0x7FFFu ? p0 & 0xFFFFu : 0u) | (pt[g][0] & 0x7FFF0000u ? p0 & 0xFFFF0000u : 0u);
-                        p1 = (pt[g][1] & 0x7FFFu ? p1 & 0xFFFFu : 0u) | (pt[g][1] & 0x7FFF0000u ? p1 & 0xFFFF0000u : 0u);
+                    if (kEdge) {   // a weight of 0 (not -0) hides what it multiplies, NaN too
+                        p0 = (pt[g][0] & 0xFFFFu ? p0 & 0xFFFFu : 0u) | (pt[g][0] & 0xFFFF0000u ? p0 & 0xFFFF0000u : 0u);
+                        p1 = (pt[g][1] & 0xFFFFu ? p1 & 0xFFFFu : 0u) | (pt[g][1] & 0xFFFF0000u ? p1 & 0xFFFF0000u : 0u);
                     }
                     mma_f16(o[g][2 * blk], a[0], a[1], a[2], a[3], p0, p1, o[g][2 * blk]);
                     mma_f16(o[g][2 * blk + 1], a[4], a[5], a[6], a[7], p0, p1, o[g][2 * blk + 1]);

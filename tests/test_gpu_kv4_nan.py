@@ -85,3 +85,28 @@ def test_where_items_are_cut_between_ctas(S, group):
 def test_the_blocks_beside_it_may_be_larger_than_everything_around(S, group, page):
     """What is left of the token counts with its own scales: alone among 32 and 128 tokens, and 2^20 times what the tokens beside it hold."""
     check([129, 33, 200], 2, group, S, page, [(0, 0, 128, 2, 1.0), (1, 1, 32, 0, 1.0), (2, 0, 77, 1, 2.0 ** 20), (2, 1, 199, 3, 2.0 ** 20)], True)
+
+
+@pytest.mark.parametrize("S", [1, 5, 40])
+def test_a_weight_too_small_for_16_bits_still_meets_nan(S):
+    """One key has all the weight; the token with NaN, four behind it among the last, partly masked tokens, is seen with a weight far below 2^-25."""
+    from amdgpu_rustdsl_b200 import fmha_fwd_kv4
+    cache = make_cache([40], 1, 16, seed=61)
+    q = queries(1, S, 1, gain=0.0)
+    q[0] = q[0, 0]
+    codes, scales, _ = R.encode((q[0, 0, 0].float() * 32).bfloat16().cpu()[None])
+    c, s = R.record(cache.pool, int(cache.table[0, 2]), 0, 0)
+    c[1], s[1] = codes[0].cuda(), scales[0].cuda()
+    x = torch.randn(128, generator=torch.Generator().manual_seed(3))
+    x[40] = math.nan
+    put_v(cache, 0, 37, 0, x)
+    k, _ = R.tokens(cache.pool.cpu(), cache.table[0].tolist(), 0, 40)
+    score = k @ q[0, 0, 0].cpu().double() / math.sqrt(128)
+    assert score[37] - score[33] < -40   # (e^-40 < 2^-57)
+    out = torch.empty_like(q)
+    fmha_fwd_kv4(q, cache, out)
+    for i in range(S):
+        bad = torch.isnan(out[0, i, 0]).cpu()
+        expect = torch.zeros(128, dtype=torch.bool)
+        expect[32:64] = 40 - S + i >= 37
+        assert torch.equal(bad, expect), i

@@ -1,4 +1,4 @@
-"""The 4-bit cache where a CTA has much to do: rings that are refilled many times. Against 64 bits on the GPU.
+"""The 4-bit cache where a CTA has much to do: rings that are refilled many times, selections of many rounds. Against 64 bits on the GPU.
 
 Tolerances. A score is off by at most 128 * 2^-24 of the sum of its products' sizes, exp2 and log2 by 2^-21 (`off`). A sum over L tokens in f32 is off by L * 2^-24 of
 the sum of its terms' sizes at most. An output has two such scores and sums, weights rounded to f16 (2^-11; below 2^-24 of the row's largest product they vanish,
@@ -65,3 +65,56 @@ def test_many_tiles_a_cta(S, group, page, causal):
             room = 2 * (p * (off + L * 2.0 ** -24)[:, None]).sum(0) + 2.0 ** -20 * (mass + old) + 1e-30
             got = weights[b, hk].double()
             assert ((got[:L] - mass - old).abs() <= room).all() and (got[L:] == -7.0).all(), (b, hk)
+
+
+def check_evict(lengths, HK, page, keep, recent, first, weights, width=None):
+    """Positions by a stable sort, weights and values gathered from them."""
+    from amdgpu_rustdsl_b200 import Kv4Cache, kv4_evict, kv4_pool, kv4_read
+    B, per = len(lengths), -(-keep // page)
+    cache, k, v = filled(lengths, HK, page, keep, width)
+    weights = weights(B, HK, cache.capacity)
+    into = Kv4Cache(kv4_pool(B * per, HK, page), torch.randperm(B * per, device="cuda").int().view(B, per), torch.full((B,), -1, dtype=torch.int32, device="cuda"))
+    kept, out = torch.full((B, HK, keep), -9, dtype=torch.int32, device="cuda"), torch.full((B, HK, keep), -9.0, device="cuda")
+    kv4_evict(cache, weights, into, keep=keep, recent=recent, first=first, kept=kept, weights_out=out)
+    new_k, new_v = (torch.empty(B, keep, HK, 128, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    kv4_read(into, new_k, new_v)
+    assert into.lengths.tolist() == [min(n, keep) for n in lengths]
+    for b, L in enumerate(lengths):
+        for h in range(HK):
+            stay = torch.arange(min(L, keep), device="cuda")
+            if L > keep:
+                some = weights[b, h, first:L - recent] + 0.0   # (zeros of either sign are equal)
+                order = torch.sort(some.cpu(), descending=True, stable=True).indices[:keep - first - recent].cuda() + first
+                stay = torch.cat([torch.arange(first, device="cuda"), order.sort().values, torch.arange(L - recent, L, device="cuda")])
+            n = len(stay)
+            assert torch.equal(kept[b, h, :n].long(), stay) and (kept[b, h, n:] == -1).all(), (b, h)
+            assert torch.equal(out[b, h, :n].view(torch.int32), weights[b, h, stay].view(torch.int32)) and (out[b, h, n:] == -9).all()
+            assert torch.equal(new_k[b, :n, h], k[b, stay, h]) and torch.equal(new_v[b, :n, h], v[b, stay, h]), (b, h)
+
+
+def few_values(B, HK, n):
+    """Many equal weights, so that the cut lies among equals that every round and CTA has some of."""
+    return torch.randint(0, 6, (B, HK, n), generator=torch.Generator(device="cuda").manual_seed(n), device="cuda").float()
+
+
+def long_tailed(B, HK, n):
+    g = torch.Generator(device="cuda").manual_seed(n + 1)
+    w = torch.exp2(torch.randn(B, HK, n, generator=g, device="cuda") * 3) * (torch.rand(B, HK, n, generator=g, device="cuda") > 0.1)
+    w[:, :, ::977], w[:, :, 5::1993], w[:, :, 7::1501] = math.nan, -math.inf, math.inf
+    return w
+
+
+@pytest.mark.parametrize("weights", [few_values, long_tailed])
+@pytest.mark.parametrize("lengths,HK,page,keep,recent,first,width", [
+    # one CTA a head, 8 to 16 rounds of 512 tokens
+    ([4096, 8000, 8191, 4097, 5003, 7168, 512, 513, 1, 0, 6000, 8192, 7777, 4608, 4607, 3000], 8, 64, 1024, 128, 4, None),
+    ([8192, 6001, 5000], 64, 32, 4900, 0, 0, None),
+    # 8 CTAs a head, 13 rounds each, and sequences of which some CTAs have a round or none
+    ([50001, 4000, 37], 8, 128, 6250, 500, 16, None),
+    ([65536, 65535], 2, 128, 30000, 1, 1, None),
+    # tables of more than 65536 tokens: keys that are read again, with one round a CTA and with up to 37
+    ([3000, 66000, 5], 2, 128, 1000, 10, 3, 520),
+    ([150000, 70001], 2, 64, 40000, 0, 0, None),
+])
+def test_evictions_of_many_rounds(lengths, HK, page, keep, recent, first, width, weights):
+    check_evict(lengths, HK, page, keep, recent, first, weights, width)

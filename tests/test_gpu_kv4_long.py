@@ -29,9 +29,9 @@ def filled(lengths, HK, page, seed, width=None):
     return cache, k, v
 
 
-# rows of a KV head from one group of eight to four, pages of every size; lengths off the tiles of 128, and enough of them for a dozen tiles a CTA
+# rows of a KV head from one group of eight to four, and for the tensor cores' tiles; pages of every size; lengths off the tiles of 128, and enough of them for a dozen tiles a CTA
 @pytest.mark.parametrize("S,group,page,causal", [(1, 4, 16, True), (1, 8, 128, True), (2, 4, 32, False), (3, 4, 16, True), (4, 4, 128, True), (5, 4, 64, True), (3, 8, 16, False), (8, 4, 16, True),
-                                                 (2, 16, 128, True), (12, 4, 32, True)])
+                                                 (2, 16, 128, True), (12, 4, 32, True), (70, 4, 64, True), (9, 5, 16, False)])
 def test_many_tiles_a_cta(S, group, page, causal):
     from amdgpu_rustdsl_b200 import fmha_fwd_kv4
     lengths, HK = [8001, 7937, 8063, 8000, 7000, 8064, 5555, 8050, 8033, 8011, 7999, 8003, 6003, 8039, 8040, 7777], 8

@@ -10,15 +10,17 @@ raises the lengths, appends the new tokens and attends:
     kv4_evict(cache, w, smaller, keep=1024, recent=128)                       # when the pages run out
 
 PyTorch owns memory and streams only; every call goes to the sm_100a kernels behind the C ABI of ``include/fmha_kv4_abi.h``. Calls run on torch's current stream of
-the cache's device (or ``stream``, a raw handle) and do not wait for it. Wrong arguments raise ``ValueError``.
+the cache's device (or ``stream``, a raw handle) and do not wait for it. Scratch memory is kept per stream; several threads may make calls on one. Wrong arguments raise
+``ValueError``.
 """
 from __future__ import annotations
 
 import ctypes as C
 import math
+import threading
 
 from . import _abi
-from .ops import _raw_stream, _ws
+from .ops import _raw_stream, _ws, _ws_lock
 
 D = 128
 TOKEN_BYTES = 136   # a token's K and V of one KV head: 2 x (64 code bytes + 4 scale bytes)
@@ -91,22 +93,29 @@ def _f32(who, name, x, cache, at_least):
     return x.data_ptr()
 
 
-_errors = C.create_string_buffer(256)
+class _Errors(threading.local):
+    """A thread's buffer for the library's messages."""
+
+    def __init__(self):
+        self.text = C.create_string_buffer(256)
+
+
+_errors = _Errors()
 
 
 def _check(who, rc):
     if rc > 0:
-        raise ValueError(f"{who}: {_errors.value.decode()}")
+        raise ValueError(f"{who}: {_errors.text.value.decode()}")
     if rc < 0:
-        raise RuntimeError(f"{who} failed with code {rc}: {_errors.value.decode()}")
+        raise RuntimeError(f"{who} failed with code {rc}: {_errors.text.value.decode()}")
 
 
 def _call(torch, cache, stream, fn, *args):
     """fn(*args, stream, err, cap) with the cache's device current."""
     if torch.cuda.current_device() == (cache.device.index or 0):
-        return fn(*args, stream, _errors, 256)
+        return fn(*args, stream, _errors.text, 256)
     with torch.cuda.device(cache.device):
-        return fn(*args, stream, _errors, 256)
+        return fn(*args, stream, _errors.text, 256)
 
 
 def kv4_append(cache, k, v, *, counts=None, stream=None):
@@ -175,9 +184,10 @@ def fmha_fwd_kv4(q, cache, out, *, causal=True, counts=None, scale=None, lse=Non
         raise ValueError("fmha_fwd_kv4: weights_in without weights")
     raw = stream if stream is not None else _raw_stream(torch, cache.device)
     nbytes = lib.fmha_kv4_attend_workspace(cache.c, a)
-    ws = _ws("kv4", nbytes, cache.device, raw)
-    a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
-    rc = _call(torch, cache, raw, lib.fmha_kv4_attend, cache.c, a)
+    with _ws_lock(cache.device, raw):
+        ws = _ws("kv4", nbytes, cache.device, raw)
+        a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
+        rc = _call(torch, cache, raw, lib.fmha_kv4_attend, cache.c, a)
     if rc:
         _check("fmha_fwd_kv4", rc)
 
@@ -201,9 +211,14 @@ def kv4_evict(cache, weights, into, *, keep, recent=0, first=0, kept=None, weigh
     if keep < 1 or recent < 0 or first < 0:
         raise ValueError("kv4_evict: keep must be positive, recent and first not negative")
     raw = stream if stream is not None else _raw_stream(torch, cache.device)
-    a.kept = _i32("kv4_evict", "kept", kept, cache, (cache.B, cache.HK, keep)) or _ws("kv4_kept", 4 * cache.B * cache.HK * keep, cache.device, raw).data_ptr()
+    a.kept = _i32("kv4_evict", "kept", kept, cache, (cache.B, cache.HK, keep))
     if weights_out is not None:
         a.weights_out, a.weights_out_width = _f32("kv4_evict", "weights_out", weights_out, cache, keep), weights_out.shape[2]
-    rc = _call(torch, cache, raw, lib.fmha_kv4_evict, cache.c, into.c, a)
+    if kept is not None:
+        rc = _call(torch, cache, raw, lib.fmha_kv4_evict, cache.c, into.c, a)
+    else:
+        with _ws_lock(cache.device, raw):
+            a.kept = _ws("kv4_kept", 4 * cache.B * cache.HK * keep, cache.device, raw).data_ptr()
+            rc = _call(torch, cache, raw, lib.fmha_kv4_evict, cache.c, into.c, a)
     if rc:
         _check("kv4_evict", rc)

@@ -6,8 +6,10 @@ PyTorch is used only as the owner of device memory and streams; every launch goe
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 import math
+import threading
 
 from . import _abi
 from ._abi import COMBINE8H, KVSPLIT, PATH_IDS, PATH_NAMES, T128, VS128, ContractError
@@ -31,6 +33,17 @@ _workspace = {}
 def _ws_key(name, device, stream):
     """Workspaces are per (device, stream): stream handle 0 (the default stream) exists on every device."""
     return (name, device.index if device.index is not None else -1, int(stream))
+
+
+_ws_locks = {}
+
+
+def _ws_lock(device, stream):
+    """Held from the moment a call takes a stream's workspaces until its last kernel is enqueued. Kernels of one stream run in order, so that calls take turns with the
+    workspaces as long as all kernels of one are enqueued before those of the next: without the lock another thread's could come between a split and its combine."""
+    key = (device.index, int(stream))
+    lock = _ws_locks.get(key)
+    return lock if lock is not None else _ws_locks.setdefault(key, threading.RLock())
 
 
 # Calls already made, by their tensors' addresses, shapes and options: the kernels, filled argument blocks and grids they came to. A call
@@ -127,19 +140,13 @@ def fmha_fwd_mxfp8(q, k, v, q_scale, k_scale, v_scale, out, *, path="auto", spli
            None if v_blockscale is None else v_blockscale.data_ptr(), None if lse is None else lse.data_ptr(), dev.index)
     hit = _calls.get(key)
     if hit is not None and hit[0] == _ws_generation and q.is_contiguous() and k.is_contiguous() and v.is_contiguous() and out.is_contiguous():
-        raw = raw_stream
-        if torch.cuda.current_device() == (dev.index or 0):
-            for kernel, args, grid in hit[1]:
-                rc = lib.fmha_mxfp8_launch(kernel, C.byref(args), grid, C.c_void_p(raw))
-                if rc:
-                    raise RuntimeError(f"fmha_mxfp8_launch({lib.fmha_mxfp8_kernel_name(kernel).decode()}) failed with code {rc}")
-        else:
-            with torch.cuda.device(dev):
-                for kernel, args, grid in hit[1]:
-                    rc = lib.fmha_mxfp8_launch(kernel, C.byref(args), grid, C.c_void_p(raw))
-                    if rc:
-                        raise RuntimeError(f"fmha_mxfp8_launch({lib.fmha_mxfp8_kernel_name(kernel).decode()}) failed with code {rc}")
-        return hit[2]
+        if hit[3] is None:
+            _replay(torch, lib, dev, hit[1], raw_stream)
+            return hit[2]
+        with hit[3]:
+            if hit[0] == _ws_generation:   # (another thread may have replaced the workspaces meanwhile)
+                _replay(torch, lib, dev, hit[1], raw_stream)
+                return hit[2]
     B, S, H, d = q.shape
     _, SK, HK, dk = k.shape
     if d != D or dk != D or HK == 0 or H % HK or (H // HK) & (H // HK - 1) or H // HK > 16:
@@ -173,16 +180,32 @@ def fmha_fwd_mxfp8(q, k, v, q_scale, k_scale, v_scale, out, *, path="auto", spli
         splits = splits or 4
     record = []
     args = (lib, q, k, v, q_scale, k_scale, v_scale, out, path, splits, raw_stream, check, flags, v_blockscale, lse, B, S, H, SK, HK, record)
+    lock = _ws_lock(dev, raw_stream) if path == "kvsplit" else None
     # (no function is defined in here for _on_device: what it would refer to could not be plain locals, which cost a remembered call 0.7 us)
+    with lock or _no_lock:
+        if torch.cuda.current_device() == (dev.index or 0):
+            ran = _launch_dispatched(unsplit and path == "kvsplit", *args)
+        else:
+            with torch.cuda.device(dev):
+                ran = _launch_dispatched(unsplit and path == "kvsplit", *args)
+        if len(_calls) >= 256:
+            _calls.clear()
+        _calls[key] = (_ws_generation, record, ran, lock)   # the key holds the stream: the split path's workspaces belong to one
+    return ran
+
+
+_no_lock = contextlib.nullcontext()
+
+
+def _replay(torch, lib, dev, launches, stream):
     if torch.cuda.current_device() == (dev.index or 0):
-        ran = _launch_dispatched(unsplit and path == "kvsplit", *args)
+        for kernel, args, grid in launches:
+            rc = lib.fmha_mxfp8_launch(kernel, C.byref(args), grid, C.c_void_p(stream))
+            if rc:
+                raise RuntimeError(f"fmha_mxfp8_launch({lib.fmha_mxfp8_kernel_name(kernel).decode()}) failed with code {rc}")
     else:
         with torch.cuda.device(dev):
-            ran = _launch_dispatched(unsplit and path == "kvsplit", *args)
-    if len(_calls) >= 256:
-        _calls.clear()
-    _calls[key] = (_ws_generation, record, ran)   # the key holds the stream: the split path's workspaces belong to one
-    return ran
+            _replay(torch, lib, dev, launches, stream)
 
 
 def _raw_stream(torch, dev):

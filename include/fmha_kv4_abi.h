@@ -12,7 +12,9 @@
  * and 32 b + 4 g + 2 r + 1: with it a lane of the matrix instructions' operand layouts finds its elements of all four blocks side by side, for K
  * (16 bytes) and for V (8 bytes) alike, and a token's bytes are its own, so that appending one token never rewrites a neighbour's byte.
  *
- * Every call is enqueued on `stream`, allocates nothing and waits for nothing. Lengths, counts and page numbers are read on the device: a length
+ * Every call is enqueued on `stream`, allocates nothing and waits for nothing. attend and evict enqueue several kernels, which hand on to one another what they leave in the
+ * scratch memory they are given (`workspace`, `kept`): two calls may share it only if all kernels of one are enqueued, on the same stream, before those of the other, not from two
+ * threads at a time. Lengths, counts and page numbers are read on the device: a length
  * above table_width * page or below 0 is cut to that range, a page number outside the pool is never followed (append drops the token, the others see
  * NaN in its place).
  *

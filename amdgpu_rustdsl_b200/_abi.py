@@ -181,6 +181,8 @@ def load():
     lib.fmha_mxfp8_mma_issue_ceiling.argtypes = [C.c_int, C.c_int, C.c_void_p, C.POINTER(C.c_float)]
     lib.fmha_mxfp8_selftest_bounded_wait.restype = C.c_int
     lib.fmha_mxfp8_selftest_bounded_wait.argtypes = [C.c_uint32, C.c_void_p, C.POINTER(C.c_uint32), C.POINTER(C.c_float)]
+    lib.cudaStreamIsCapturing.restype = C.c_int   # of the CUDA runtime that the library is linked with
+    lib.cudaStreamIsCapturing.argtypes = [C.c_void_p, C.POINTER(C.c_int)]
     cache, rows, err = C.POINTER(Kv4CacheArgs), C.POINTER(Kv4Rows), [C.c_void_p, C.c_char_p, C.c_size_t]
     lib.fmha_kv4_append.restype = C.c_int
     lib.fmha_kv4_append.argtypes = [cache, rows, rows, C.c_uint32, C.c_void_p] + err

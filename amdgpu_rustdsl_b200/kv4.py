@@ -10,8 +10,8 @@ raises the lengths, appends the new tokens and attends:
     kv4_evict(cache, w, smaller, keep=1024, recent=128)                       # when the pages run out
 
 PyTorch owns memory and streams only; every call goes to the sm_100a kernels behind the C ABI of ``include/fmha_kv4_abi.h``. Calls run on torch's current stream of
-the cache's device (or ``stream``, a raw handle) and do not wait for it. Scratch memory is kept per stream; several threads may make calls on one. Wrong arguments raise
-``ValueError``.
+the cache's device (or ``stream``, a raw handle) and do not wait for it. Scratch memory is kept per stream; several threads may make calls on one. In a graph that ``torch.cuda.graph`` captures
+it is the graph's own. Wrong arguments raise ``ValueError``.
 """
 from __future__ import annotations
 
@@ -218,7 +218,8 @@ def kv4_evict(cache, weights, into, *, keep, recent=0, first=0, kept=None, weigh
         rc = _call(torch, cache, raw, lib.fmha_kv4_evict, cache.c, into.c, a)
     else:
         with _ws_lock(cache.device, raw):
-            a.kept = _ws("kv4_kept", 4 * cache.B * cache.HK * keep, cache.device, raw).data_ptr()
+            scratch = _ws("kv4_kept", 4 * cache.B * cache.HK * keep, cache.device, raw)
+            a.kept = scratch.data_ptr()
             rc = _call(torch, cache, raw, lib.fmha_kv4_evict, cache.c, into.c, a)
     if rc:
         _check("kv4_evict", rc)

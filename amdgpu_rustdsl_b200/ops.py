@@ -53,23 +53,38 @@ _calls = {}
 _ws_generation = 0
 
 
+def _capturing(stream):
+    """Whether a graph is being captured from the stream. (The default stream's handle is 0; it cannot be captured.)"""
+    if not stream:
+        return False
+    status = C.c_int(0)
+    rc = _abi.load().cudaStreamIsCapturing(stream, C.byref(status))
+    if rc:
+        raise RuntimeError(f"the stream's capture status is not to be had: cudaError {rc}")
+    return status.value != 0
+
+
 def _ws(name, nbytes, device, stream, zero=False):
-    """Grow-only per-device, per-stream workspace for the KV-split partials (the reference's ``_ws``, ops.py:72-85, which frees the old
-    buffer with a synchronising ``hipFree``). Here the old buffer goes back to torch's caching allocator, which only orders its reuse
-    against torch's own current stream: a split or combine still running on ``stream`` is therefore waited for first."""
+    """Grow-only per-device, per-stream workspace (the reference's ``_ws``, ops.py:72-85, which frees the old buffer with a synchronising
+    ``hipFree``). Here buffers are made and given back on the stream that uses them, where torch's caching allocator orders what they are used for next. The caller holds on to
+    the buffer until its kernels are enqueued.
+
+    While a graph is captured from the stream, a call gets a buffer of its own, which torch takes from the graph's memory: the graph's replays write to it as long as the graph
+    lives, whatever becomes of the stream's buffer, and on whatever stream they run. ``zero``: cleared once; its users leave it cleared."""
     import torch
     key = _ws_key(name, device, stream)
-    buf = _workspace.get(key)
-    if buf is None or buf.numel() < nbytes:
-        global _ws_generation
-        _ws_generation += 1   # remembered calls hold the old buffers' addresses
-        if buf is not None:
-            (torch.cuda.ExternalStream(int(stream), device=device) if stream else torch.cuda.default_stream(device)).synchronize()
-        if zero:   # cleared once; its users leave it cleared. The fill runs on torch's current stream: it must be done before `stream` uses it
-            buf = _workspace[key] = torch.zeros(nbytes, dtype=torch.uint8, device=device)
-            torch.cuda.current_stream(device).synchronize()
+    buf, captured = _workspace.get(key), _capturing(stream)
+    if captured or buf is None or buf.numel() < nbytes:
+        make = torch.zeros if zero else torch.empty
+        if stream == _raw_stream(torch, device):
+            buf = make(nbytes, dtype=torch.uint8, device=device)
         else:
-            buf = _workspace[key] = torch.empty(nbytes, dtype=torch.uint8, device=device)
+            with torch.cuda.stream(torch.cuda.ExternalStream(int(stream), device=device) if stream else torch.cuda.default_stream(device)):
+                buf = make(nbytes, dtype=torch.uint8, device=device)
+        if not captured:
+            global _ws_generation
+            _ws_generation += 1   # remembered calls hold the old buffers' addresses
+            _workspace[key] = buf
     return buf
 
 
@@ -144,7 +159,7 @@ def fmha_fwd_mxfp8(q, k, v, q_scale, k_scale, v_scale, out, *, path="auto", spli
             _replay(torch, lib, dev, hit[1], raw_stream)
             return hit[2]
         with hit[3]:
-            if hit[0] == _ws_generation:   # (another thread may have replaced the workspaces meanwhile)
+            if hit[0] == _ws_generation and not _capturing(raw_stream):   # (another thread may have replaced the workspaces meanwhile)
                 _replay(torch, lib, dev, hit[1], raw_stream)
                 return hit[2]
     B, S, H, d = q.shape
@@ -188,9 +203,10 @@ def fmha_fwd_mxfp8(q, k, v, q_scale, k_scale, v_scale, out, *, path="auto", spli
         else:
             with torch.cuda.device(dev):
                 ran = _launch_dispatched(unsplit and path == "kvsplit", *args)
-        if len(_calls) >= 256:
-            _calls.clear()
-        _calls[key] = (_ws_generation, record, ran, lock)   # the key holds the stream: the split path's workspaces belong to one
+        if lock is None or not _capturing(raw_stream):
+            if len(_calls) >= 256:
+                _calls.clear()
+            _calls[key] = (_ws_generation, record, ran, lock)   # the key holds the stream: the split path's workspaces belong to one
     return ran
 
 
@@ -252,7 +268,8 @@ def _launch_path(lib, q, k, v, q_scale, k_scale, v_scale, out, path, splits, str
     a.ptr_ohat, a.ptr_lse, a.kvs_splits, a.kvs_rows_total = ohat.data_ptr(), lse_ws.data_ptr(), splits, rows_total
     sizes.ptr_ohat, sizes.ptr_lse = splits * rows_total * D * 4, splits * rows_total * 4
     if flags & _abi.FLAG_FUSED_COMBINE:
-        a.ext_ptr_fused_counters = _ws("fused_counters", 4 * B * H * math.ceil(S / 128), q.device, stream, zero=True).data_ptr()
+        counters = _ws("fused_counters", 4 * B * H * math.ceil(S / 128), q.device, stream, zero=True)
+        a.ext_ptr_fused_counters = counters.data_ptr()
     _check_launch(lib, KVSPLIT, a, sizes, _abi.grid3(math.ceil(S / 256), H, B * splits), syms, stream, check, record)
     if flags & _abi.FLAG_FUSED_COMBINE:
         return path, splits

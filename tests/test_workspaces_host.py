@@ -1,4 +1,5 @@
-"""The workspaces that the Python entries keep per stream, with the library and the GPU replaced by stand-ins: no call's kernels come between those of another."""
+"""The workspaces that the Python entries keep per stream, with the library and the GPU replaced by stand-ins: no call's kernels come between those of another, and no graph
+holds a buffer that may be replaced."""
 import ctypes as C
 import threading
 import time
@@ -136,3 +137,111 @@ def test_messages_of_several_threads_do_not_mix(no_gpu, monkeypatch):
             with pytest.raises(ValueError, match=f"{i + 1} rows"):
                 kv4.kv4_append(cache, x, x)
     in_threads(work)
+
+
+class Captured:
+    """A library whose streams are being captured or not, and the scratch memory that its calls were given."""
+
+    def __init__(self):
+        self.capturing, self.scratch, self.bytes = False, [], 64
+
+    def cudaStreamIsCapturing(self, stream, status):
+        C.cast(status, C.POINTER(C.c_int))[0] = int(self.capturing)
+        return 0
+
+    def fmha_kv4_attend_workspace(self, cache, a):
+        return self.bytes
+
+    def fmha_kv4_attend(self, cache, a, stream, err, cap):
+        self.scratch.append(a.workspace)
+        return 0
+
+    def fmha_mxfp8_launch(self, kernel, args, grid, stream):
+        if kernel == _abi.KVSPLIT:
+            self.scratch.append(args._obj.ptr_ohat)
+        return 0
+
+
+@pytest.fixture
+def captured(no_gpu, monkeypatch):
+    lib = Captured()
+    monkeypatch.setattr(_abi, "load", lambda: lib)
+    for module in (ops, kv4):
+        monkeypatch.setattr(module, "_raw_stream", lambda torch, dev: 77)   # a stream that is not the default one
+    keep = []   # nothing is freed, so that equal addresses are equal buffers
+
+    def empty(*a, **k):
+        keep.append(torch.zeros(*a, **k))
+        return keep[-1]
+    monkeypatch.setattr(torch, "empty", empty)
+    return lib
+
+
+def test_a_captured_attention_call_has_scratch_memory_of_its_own(captured):
+    cache, q = a_cache(), torch.zeros(1, 1, 1, 128, dtype=torch.bfloat16)
+
+    def call():
+        kv4.fmha_fwd_kv4(q, cache, torch.zeros_like(q))
+        return captured.scratch[-1]
+    kept = call()
+    assert call() == kept
+    captured.capturing = True
+    first, second = call(), call()
+    assert len({kept, first, second}) == 3
+    captured.capturing = False
+    assert call() == kept       # neither of the graph's buffers stays the stream's
+    captured.bytes = 1 << 20
+    assert call() not in (kept, first, second)
+
+
+def test_a_captured_split_is_not_remembered_and_replays_none(captured):
+    class Tensor:
+        def __init__(self, x):
+            self.x, self.is_cuda = x, True
+
+        def __getattr__(self, name):
+            return getattr(self.x, name)
+    q, kv = (Tensor(torch.zeros(1, n, 1, 128, dtype=torch.uint8)) for n in (128, 1024))
+    out, scales = Tensor(torch.zeros(1, 128, 1, 128, dtype=torch.bfloat16)), Tensor(torch.zeros(1 << 16, dtype=torch.uint8))
+
+    def call():
+        ops.fmha_fwd_mxfp8(q, kv, kv, scales, scales, scales, out, path="kvsplit", splits=4, check=False)
+        return captured.scratch[-1]
+    captured.capturing = True
+    first = call()
+    assert not ops._calls and call() != first
+    captured.capturing = False
+    kept = call()
+    assert kept != first and call() == kept and len(ops._calls) == 1
+    captured.capturing = True
+    assert call() not in (kept, first)
+    captured.capturing = False
+    assert call() == kept
+
+
+def test_buffers_are_made_on_the_stream_that_uses_them(captured, monkeypatch):
+    """A buffer for another stream than torch's current one comes from that stream's part of the allocator, which orders its next use."""
+    entered = []
+
+    class Stream:
+        def __init__(self, handle, device=None):
+            self.handle = handle
+
+    class On:
+        def __init__(self, stream):
+            self.stream = stream
+
+        def __enter__(self):
+            entered.append(self.stream.handle)
+
+        def __exit__(self, *a):
+            entered.append("out")
+    monkeypatch.setattr(torch.cuda, "ExternalStream", Stream)
+    monkeypatch.setattr(torch.cuda, "stream", On)
+    cache, q = a_cache(), torch.zeros(1, 1, 1, 128, dtype=torch.bfloat16)
+    kv4.fmha_fwd_kv4(q, cache, torch.zeros_like(q))
+    assert entered == []
+    kv4.fmha_fwd_kv4(q, cache, torch.zeros_like(q), stream=99)
+    assert entered == [99, "out"]
+    kv4.fmha_fwd_kv4(q, cache, torch.zeros_like(q), stream=99)
+    assert entered == [99, "out"]

@@ -30,6 +30,12 @@ int done(cudaError_t e, char* err, size_t cap) {
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
+// whether two ranges of bytes have any in common
+bool overlap(const void* a, uint64_t a_bytes, const void* b, uint64_t b_bytes) {
+    const uint64_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+    return x < y + b_bytes && y < x + a_bytes;
+}
+
 // kernels keep row numbers in 32 bits and grids in 31
 constexpr uint64_t kMostRows = 1ull << 30;
 
@@ -135,6 +141,9 @@ int fmha_kv4_evict(const fmha_kv4_cache* cache, const fmha_kv4_cache* into, cons
     if (a->keep == 0u || a->keep > room) return refuse(err, cap, "evict: keep must be 1 to the %llu tokens that into has room for", static_cast<unsigned long long>(room));
     if (static_cast<uint64_t>(a->recent) + a->first > a->keep) return refuse(err, cap, "evict: first + recent must not exceed keep");
     if (a->weights_out != nullptr && a->weights_out_width < a->keep) return refuse(err, cap, "evict: weights_out must have room for keep tokens");
+    const uint64_t heads = static_cast<uint64_t>(p.from.B) * p.from.HK;
+    if (a->weights_out != nullptr && overlap(a->weights, 4u * heads * a->weights_width, a->weights_out, 4u * heads * a->weights_out_width))
+        return refuse(err, cap, "evict: weights_out must not share memory with weights");
     p.weights = a->weights, p.kept = a->kept, p.weights_out = a->weights_out;
     p.weights_width = a->weights_width, p.weights_out_width = a->weights_out_width;
     p.keep = a->keep, p.recent = a->recent, p.first = a->first;

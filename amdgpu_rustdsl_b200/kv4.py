@@ -199,7 +199,8 @@ def kv4_evict(cache, weights, into, *, keep, recent=0, first=0, kept=None, weigh
     The first ``first`` and the last ``recent`` tokens stay, and of the others those with the greatest ``weights`` (f32 [B, HK, capacity or more], as ``fmha_fwd_kv4``
     accumulates them); among equals the earlier ones, and NaN counts as more than any number. Different heads keep different tokens.
     kept         int32 [B, HK, keep]: the positions that stayed, ascending, -1 behind them
-    weights_out  f32 [B, HK, keep or more]: their weights, for the next eviction; nothing is written behind the new length
+    weights_out  f32 [B, HK, keep or more]: their weights, for the next eviction; nothing is written behind the new length. Another tensor than ``weights``, whose
+                 memory it must not share.
     """
     import torch
     lib = _abi.load()

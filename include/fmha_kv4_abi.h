@@ -91,7 +91,8 @@ int fmha_kv4_attend(const fmha_kv4_cache* cache, const fmha_kv4_attend_args* arg
  *   tokens 0, 1, ... of `into`, whose lengths become min(length, keep). `into` has the same B, HK and page, room for `keep` tokens, and its pages must not be
  *   pages that `cache` reads (the pool may be the same).
  *   weights f32 [B][HK][weights_width]. kept: int32 [B][HK][keep], the positions that stayed, -1 behind them (scratch that must be there).
- *   weights_out: NULL or f32 [B][HK][weights_out_width], the weights of the tokens that stayed; nothing is written behind the new length.
+ *   weights_out: NULL or f32 [B][HK][weights_out_width], the weights of the tokens that stayed; nothing is written behind the new length. It must not share memory
+ *   with `weights` (the copies run in no order).
  */
 typedef struct fmha_kv4_evict_args {
     const float* weights;

@@ -111,11 +111,19 @@ int fmha_kv4_attend(const fmha_kv4_cache* cache, const fmha_kv4_attend_args* a, 
     const uint64_t row_tiles = (static_cast<uint64_t>(a->S) * (a->H / p.c.HK) + 255u) / 256u;
     if (((tokens + 127u) / 128u) * p.c.B * p.c.HK > 0xFFFFFFFFull / row_tiles) return refuse(err, cap, "attend: more than 2^32 steps of 128 tokens and 256 query rows");
     if (a->weights != nullptr && a->weights_width < tokens) return refuse(err, cap, "attend: weights must have room for the %llu tokens of the table", static_cast<unsigned long long>(tokens));
+    const uint64_t weights_bytes = 4u * static_cast<uint64_t>(p.c.B) * p.c.HK * a->weights_width;
+    if (a->weights != nullptr && a->weights_in != nullptr && a->weights_in != a->weights && overlap(a->weights, weights_bytes, a->weights_in, weights_bytes))
+        return refuse(err, cap, "attend: weights_in must be weights or share no memory with it");
     if (a->weights == nullptr && a->weights_in != nullptr) return refuse(err, cap, "attend: weights_in without weights");
     if (a->weights != nullptr && static_cast<uint64_t>(p.c.B) * p.c.HK * ((tokens + 127u) / 128u) > kMostRows) return refuse(err, cap, "attend: more than 2^37 cached tokens x heads with weights");
     if (!(a->scale > 0.0f) || a->scale > 3.0e38f) return refuse(err, cap, "attend: scale must be a positive number");
     if (a->workspace == nullptr || !aligned16(a->workspace) || a->workspace_bytes < fmha_kv4_attend_workspace(cache, a))
         return refuse(err, cap, "attend: the workspace must be 16-byte aligned and hold fmha_kv4_attend_workspace() bytes");
+    if (a->out == a->q.data) {   // a row's elements are read before it is written, by whoever writes it; the weights of many rows go by the queries again
+        const int64_t row = 128, rows = row * a->H, all = rows * a->S;
+        if ((a->H > 1u && a->q.stride_h != row) || (a->S > 1u && a->q.stride_s != rows) || (p.c.B > 1u && a->q.stride_b != all)) return refuse(err, cap, "attend: out may be q only where q is packed as out is");
+        if (a->weights != nullptr && a->S * (a->H / p.c.HK) > 8u) return refuse(err, cap, "attend: out may not be q where the weights of more than 8 rows of a KV head are asked for");
+    }
     p.out = static_cast<__nv_bfloat16*>(a->out);
     p.counts = a->counts;
     p.lse = a->lse;

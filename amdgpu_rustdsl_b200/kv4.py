@@ -152,12 +152,13 @@ def kv4_read(cache, k, v, *, last=False, counts=None, stream=None):
 def fmha_fwd_kv4(q, cache, out, *, causal=True, counts=None, scale=None, lse=None, weights=None, weights_in=None, stream=None):
     """Attention over the cache: ``out = softmax(scale q k^T) v``, q bf16 [B, S, H, 128] (strided), out bf16 [B, S, H, 128] (packed), H = 1 to 16 times the KV heads.
 
+    out         shares no memory with q; or it is q, packed, without ``weights`` or with at most 8 rows (S times H / HK) of a KV head
     causal      the rows are the sequences' newest tokens (``counts`` as in ``kv4_append``): row i of n sees the tokens up to ``lengths[b] - n + i``. Without it every row
                 sees all tokens. Rows beyond n, and rows that see nothing, are zeros.
     scale       1 / sqrt(128) where not given
     lse         f32 [B, H, S]: natural log-sum-exps, -inf for rows that see nothing
     weights     f32 [B, HK, capacity or more]: for each token t below the length, the softmax weight that it received from the rows and the query heads of its KV head,
-                plus ``weights_in`` there (the same shape, may be the same tensor) where given; with ``causal`` the n newest tokens start from nothing. Nothing is
+                plus ``weights_in`` there (the same shape; the same tensor, or one that shares no memory with it) where given; with ``causal`` the n newest tokens start from nothing. Nothing is
                 written behind the length. The sums are the same bits every time.
     """
     import torch

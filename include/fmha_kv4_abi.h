@@ -63,7 +63,7 @@ int fmha_kv4_read(const fmha_kv4_cache* cache, const fmha_kv4_rows* k, const fmh
  *   H / HK from 1 to 16. Rows from n on, and rows that see no token, get zeros (log-sum-exp -inf).
  *   lse: NULL or f32 [B][H][S], natural.
  *   weights: NULL or f32 [B][HK][weights_width]: weights[b][kv][t] = old + (sum of the softmax weights of token t over the rows and the query heads of the
- *     KV head), for t < length; nothing is written behind the length. old = weights_in[b][kv][t] (same width; may be the same array), 0 where weights_in is
+ *     KV head), for t < length; nothing is written behind the length. old = weights_in[b][kv][t] (same width; the same array, or one that shares no memory with it), 0 where weights_in is
  *     NULL and, with `causal`, for the n newest tokens. Sums in a fixed order: the same bits every time.
  *   NaN: a block of V that is NaN makes its 32 elements NaN in the rows that see the token, whatever the weight, and nothing else; NaN in K makes all of these rows NaN.
  *   Ranges: the products run in f16 against powers of two that are taken out, so that any scale goes. What is exact is a query row's elements down to 2^-30 of its largest,
@@ -72,7 +72,7 @@ int fmha_kv4_read(const fmha_kv4_cache* cache, const fmha_kv4_rows* k, const fmh
  */
 typedef struct fmha_kv4_attend_args {
     fmha_kv4_rows q;        /* [B][S][H][128] */
-    void* out;              /* bf16 [B][S][H][128], packed, 16-byte aligned */
+    void* out;              /* bf16 [B][S][H][128], packed, 16-byte aligned; shares no memory with q, or is q, packed, without weights or with up to 8 rows of a KV head */
     const int32_t* counts;
     float* lse;
     float* weights;

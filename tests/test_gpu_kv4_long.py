@@ -118,3 +118,17 @@ def long_tailed(B, HK, n):
 ])
 def test_evictions_of_many_rounds(lengths, HK, page, keep, recent, first, width, weights):
     check_evict(lengths, HK, page, keep, recent, first, weights, width)
+
+
+@pytest.mark.parametrize("S,weights", [(1, True), (2, True), (3, False), (8, False), (70, False)])
+def test_attention_in_place(S, weights):
+    """out may be q, cut items and sequences without tokens among them."""
+    from amdgpu_rustdsl_b200 import fmha_fwd_kv4
+    cache, _, _ = filled([5000, 1, 3001, 777], 2, 32, S)
+    cache.lengths[1] = 0
+    g = torch.Generator(device="cuda").manual_seed(S)
+    q = torch.randn(4, S, 8, 128, generator=g, device="cuda").bfloat16()
+    out, w, v = torch.full_like(q, math.nan), *(torch.zeros(4, 2, cache.capacity, device="cuda") for _ in range(2))
+    fmha_fwd_kv4(q, cache, out, weights=w if weights else None)
+    fmha_fwd_kv4(q, cache, q, weights=v if weights else None)
+    assert torch.equal(q, out) and torch.equal(w, v)

@@ -56,8 +56,8 @@ int view_of(const fmha_kv4_cache* c, const char* name, Kv4View& v, char* err, si
     return 0;
 }
 
-int rows_of(const fmha_kv4_rows* x, const char* name, Kv4Rows& r, char* err, size_t cap) {
-    if (x == nullptr || x->data == nullptr) return refuse(err, cap, "%s must be given", name);
+int rows_of(const fmha_kv4_rows* x, uint32_t S, const char* name, Kv4Rows& r, char* err, size_t cap) {
+    if (x == nullptr || (x->data == nullptr && S != 0u)) return refuse(err, cap, "%s must be given", name);   // (no rows have no address)
     if (!aligned16(x->data) || ((x->stride_b | x->stride_s | x->stride_h) & 7) != 0) return refuse(err, cap, "%s: pointer and strides must be multiples of 16 bytes", name);
     r.data = static_cast<uint8_t*>(x->data);
     r.stride_b = 2 * x->stride_b, r.stride_s = 2 * x->stride_s, r.stride_h = 2 * x->stride_h;
@@ -72,8 +72,8 @@ int fmha_kv4_append(const fmha_kv4_cache* cache, const fmha_kv4_rows* k, const f
     Kv4View c;
     Kv4Rows rk, rv;
     if (int r = view_of(cache, "append", c, err, cap)) return r;
-    if (int r = rows_of(k, "append: k", rk, err, cap)) return r;
-    if (int r = rows_of(v, "append: v", rv, err, cap)) return r;
+    if (int r = rows_of(k, S, "append: k", rk, err, cap)) return r;
+    if (int r = rows_of(v, S, "append: v", rv, err, cap)) return r;
     if (S == 0u) return 0;
     if (static_cast<uint64_t>(c.B) * S * c.HK > kMostRows) return refuse(err, cap, "append: more than 2^30 rows");
     return done(b200mx::launch_kv4_append(c, rk, rv, S, counts, static_cast<cudaStream_t>(stream)), err, cap);
@@ -83,8 +83,8 @@ int fmha_kv4_read(const fmha_kv4_cache* cache, const fmha_kv4_rows* k, const fmh
     Kv4View c;
     Kv4Rows rk, rv;
     if (int r = view_of(cache, "read", c, err, cap)) return r;
-    if (int r = rows_of(k, "read: k", rk, err, cap)) return r;
-    if (int r = rows_of(v, "read: v", rv, err, cap)) return r;
+    if (int r = rows_of(k, S, "read: k", rk, err, cap)) return r;
+    if (int r = rows_of(v, S, "read: v", rv, err, cap)) return r;
     if (!last && counts != nullptr) return refuse(err, cap, "read: counts go with the newest tokens only");
     if (S == 0u) return 0;
     if (static_cast<uint64_t>(c.B) * S * c.HK > kMostRows) return refuse(err, cap, "read: more than 2^30 rows");
@@ -101,14 +101,14 @@ int fmha_kv4_attend(const fmha_kv4_cache* cache, const fmha_kv4_attend_args* a, 
     b200mx::Kv4AttendParams p = {};
     if (a == nullptr) return refuse(err, cap, "attend: no arguments");
     if (int r = view_of(cache, "attend", p.c, err, cap)) return r;
-    if (int r = rows_of(&a->q, "attend: q", p.q, err, cap)) return r;
+    if (int r = rows_of(&a->q, a->S, "attend: q", p.q, err, cap)) return r;
     if (a->H == 0u || a->H % p.c.HK != 0u || a->H / p.c.HK > 16u) return refuse(err, cap, "attend: H must be 1 to 16 times the KV heads (H %u, HK %u)", a->H, p.c.HK);
-    if (a->out == nullptr || !aligned16(a->out)) return refuse(err, cap, "attend: out must be given and 16-byte aligned");
-    if (a->S == 0u) return 0;
+    if ((a->out == nullptr && a->S != 0u) || !aligned16(a->out)) return refuse(err, cap, "attend: out must be given and 16-byte aligned");
+    if (a->S == 0u && (a->weights == nullptr || a->weights == a->weights_in)) return 0;
     if (static_cast<uint64_t>(p.c.B) * a->S * a->H > kMostRows) return refuse(err, cap, "attend: more than 2^30 query rows");
     const uint64_t tokens = static_cast<uint64_t>(p.c.table_width) << p.c.page_log2;
     // the kernels deal out steps of 128 tokens and 256 rows at most, counted in 32 bits
-    const uint64_t row_tiles = (static_cast<uint64_t>(a->S) * (a->H / p.c.HK) + 255u) / 256u;
+    const uint64_t row_tiles = a->S == 0u ? 1u : (static_cast<uint64_t>(a->S) * (a->H / p.c.HK) + 255u) / 256u;
     if (((tokens + 127u) / 128u) * p.c.B * p.c.HK > 0xFFFFFFFFull / row_tiles) return refuse(err, cap, "attend: more than 2^32 steps of 128 tokens and 256 query rows");
     if (a->weights != nullptr && a->weights_width < tokens) return refuse(err, cap, "attend: weights must have room for the %llu tokens of the table", static_cast<unsigned long long>(tokens));
     const uint64_t weights_bytes = 4u * static_cast<uint64_t>(p.c.B) * p.c.HK * a->weights_width;
@@ -119,7 +119,7 @@ int fmha_kv4_attend(const fmha_kv4_cache* cache, const fmha_kv4_attend_args* a, 
     if (!(a->scale > 0.0f) || a->scale > 3.0e38f) return refuse(err, cap, "attend: scale must be a positive number");
     if (a->workspace == nullptr || !aligned16(a->workspace) || a->workspace_bytes < fmha_kv4_attend_workspace(cache, a))
         return refuse(err, cap, "attend: the workspace must be 16-byte aligned and hold fmha_kv4_attend_workspace() bytes");
-    if (a->out == a->q.data) {   // a row's elements are read before it is written, by whoever writes it; the weights of many rows go by the queries again
+    if (a->out == a->q.data && a->S != 0u) {   // a row's elements are read before it is written, by whoever writes it; the weights of many rows go by the queries again
         const int64_t row = 128, rows = row * a->H, all = rows * a->S;
         if ((a->H > 1u && a->q.stride_h != row) || (a->S > 1u && a->q.stride_s != rows) || (p.c.B > 1u && a->q.stride_b != all)) return refuse(err, cap, "attend: out may be q only where q is packed as out is");
         if (a->weights != nullptr && a->S * (a->H / p.c.HK) > 8u) return refuse(err, cap, "attend: out may not be q where the weights of more than 8 rows of a KV head are asked for");
@@ -133,7 +133,7 @@ int fmha_kv4_attend(const fmha_kv4_cache* cache, const fmha_kv4_attend_args* a, 
     p.scale_log2 = a->scale * 1.44269504088896341f;
     p.status = b200mx::device_status_word();
     if (p.status == nullptr) return -static_cast<int>(cudaErrorInvalidSymbol);
-    return done(b200mx::launch_kv4_attend(p, static_cast<cudaStream_t>(stream)), err, cap);
+    return done(a->S == 0u ? b200mx::launch_kv4_weigh(p, static_cast<cudaStream_t>(stream)) : b200mx::launch_kv4_attend(p, static_cast<cudaStream_t>(stream)), err, cap);
 }
 
 int fmha_kv4_evict(const fmha_kv4_cache* cache, const fmha_kv4_cache* into, const fmha_kv4_evict_args* a, void* stream, char* err, size_t cap) {

@@ -48,7 +48,7 @@ typedef struct fmha_kv4_rows {
 
 /*
  * The S rows of a sequence are its newest tokens: with n = counts[b] (cut to min(S, length); counts NULL: n = min(S, length)) row i < n stands for token
- * length - n + i, and rows from n on for nothing.
+ * length - n + i, and rows from n on for nothing. S may be 0 (and the rows' pointers then NULL): there is nothing to do but to carry weights_in over to weights.
  *
  * append: rounds K and V rows [B][S][HK] into the cache's tokens (lengths have been raised by the caller). scale = clamp(floor(log2 amax) - 2 + 127,
  *   1, 252), code = e2m1, nearest, ties to even, saturating at 6; a block that holds Inf or NaN becomes NaN.

@@ -73,6 +73,8 @@ def _rows(who, name, x, cache, S=None, heads=None):
     ptr = x.data_ptr()
     if x.device != cache.device or sd != 1 or (sb | ss | sh) & 7 or ptr & 15:
         raise ValueError(f"{who}: {name} must be on the cache's device, its last dimension dense, its start and its strides multiples of 16 bytes")
+    if shape[1] > 0x7FFFFFFF:   # (a stride of 0 makes as many rows as you like; the library counts them in 32 bits)
+        raise ValueError(f"{who}: {name} has {shape[1]} rows, more than 2^31")
     return _abi.Kv4Rows(ptr, sb, ss, sh)
 
 
@@ -209,9 +211,9 @@ def kv4_evict(cache, weights, into, *, keep, recent=0, first=0, kept=None, weigh
     if into.device != cache.device:
         raise ValueError("kv4_evict: into must be on the cache's device")
     a.weights, a.weights_width = _f32("kv4_evict", "weights", weights, cache, cache.capacity), weights.shape[2]
+    if not 1 <= keep <= into.capacity or recent < 0 or first < 0 or first + recent > keep:   # (here, in numbers of any size: the struct's have 32 bits)
+        raise ValueError(f"kv4_evict: keep must be 1 to the {into.capacity} tokens that into has room for, recent and first not negative and no more than keep together")
     a.keep, a.recent, a.first = keep, recent, first
-    if keep < 1 or recent < 0 or first < 0:
-        raise ValueError("kv4_evict: keep must be positive, recent and first not negative")
     raw = stream if stream is not None else _raw_stream(torch, cache.device)
     a.kept = _i32("kv4_evict", "kept", kept, cache, (cache.B, cache.HK, keep))
     if weights_out is not None:

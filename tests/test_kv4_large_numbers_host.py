@@ -1,0 +1,35 @@
+"""Numbers that do not fit the fields and registers they go into are refused, not cut."""
+import ctypes as C
+import types
+
+import pytest
+import torch
+
+from tests.test_kv4_host import FAKE, _cache, _rows
+from tests.test_workspaces_host import a_cache, no_gpu  # noqa: F401
+
+
+def calls_nothing(*a):
+    raise AssertionError("a call went out")
+
+
+@pytest.fixture
+def no_library(no_gpu, monkeypatch):  # noqa: F811
+    from amdgpu_rustdsl_b200 import _abi
+    lib = types.SimpleNamespace(fmha_kv4_evict=calls_nothing, fmha_kv4_append=calls_nothing, fmha_kv4_read=calls_nothing)
+    monkeypatch.setattr(_abi, "load", lambda: lib)
+
+
+@pytest.mark.parametrize("change", [dict(recent=1 << 32), dict(first=1 << 32), dict(keep=(1 << 32) + 16), dict(keep=65), dict(keep=1 << 31), dict(recent=(1 << 32) - 8, first=16), dict(recent=10, first=7)])
+def test_evictions(no_library, change):
+    from amdgpu_rustdsl_b200 import kv4
+    with pytest.raises(ValueError, match="keep must be"):
+        kv4.kv4_evict(a_cache(), torch.zeros(1, 1, 64), a_cache(), **{"keep": 16, **change})
+
+
+def test_rows_of_a_stride_of_0(no_library):
+    from amdgpu_rustdsl_b200 import kv4
+    x = torch.zeros(1, 1, 1, 128, dtype=torch.bfloat16).expand(1, 1 << 32, 1, 128)
+    for call in (kv4.kv4_append, kv4.kv4_read):
+        with pytest.raises(ValueError, match="more than 2"):
+            call(a_cache(), x, x)

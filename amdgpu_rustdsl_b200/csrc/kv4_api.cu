@@ -46,6 +46,7 @@ int view_of(const fmha_kv4_cache* c, const char* name, Kv4View& v, char* err, si
     if (!aligned16(c->pool)) return refuse(err, cap, "%s: the pool must be 16-byte aligned", name);
     if (c->pages > 0x7FFFFFFFull || static_cast<uint64_t>(c->B) * c->HK > kMostRows || static_cast<uint64_t>(c->table_width) * c->page > 0x7FFFFFFFull)
         return refuse(err, cap, "%s: more than 2^31 pages or tokens of a sequence, or 2^30 sequences x heads", name);
+    if (static_cast<uint64_t>(c->HK) * FMHA_KV4_TOKEN_BYTES * c->page > 0xFFFFFFFFull) return refuse(err, cap, "%s: pages of 4 GiB and more", name);   // (the decode kernel holds their size in 32 bits)
     v.pool = static_cast<uint8_t*>(c->pool);
     v.table = c->table;
     v.lengths = c->lengths;

@@ -33,3 +33,15 @@ def test_rows_of_a_stride_of_0(no_library):
     for call in (kv4.kv4_append, kv4.kv4_read):
         with pytest.raises(ValueError, match="more than 2"):
             call(a_cache(), x, x)
+
+
+def test_pages_of_4_gib(abi):
+    """Pages of 128 tokens with the most heads that 32 bits hold pass this check (and stop at the next), those with one more do not."""
+    lib, err, rows = abi.load(), C.create_string_buffer(256), _rows(abi)
+    most = (2 ** 32 - 1) // (136 * 128)
+    for heads, message in ((most + 1, "4 GiB"), (1 << 29, "4 GiB"), (most, "must be given")):
+        cache = _cache(abi, HK=heads, B=1, page=128)
+        assert lib.fmha_kv4_append(cache, abi.Kv4Rows(None, 8, 8, 8), rows, 3, None, None, err, 256) == 6 and message in err.value.decode()
+        if heads > most:
+            assert lib.fmha_kv4_attend(cache, abi.Kv4AttendArgs(q=rows, out=FAKE, S=3, H=heads, scale=1.0), None, err, 256) == 6 and message in err.value.decode()
+            assert lib.fmha_kv4_evict(cache, cache, abi.Kv4EvictArgs(), None, err, 256) == 6 and message in err.value.decode()

@@ -117,7 +117,7 @@ int fmha_kv4_attend(const fmha_kv4_cache* cache, const fmha_kv4_attend_args* a, 
         return refuse(err, cap, "attend: weights_in must be weights or share no memory with it");
     if (a->weights == nullptr && a->weights_in != nullptr) return refuse(err, cap, "attend: weights_in without weights");
     if (a->weights != nullptr && static_cast<uint64_t>(p.c.B) * p.c.HK * ((tokens + 127u) / 128u) > kMostRows) return refuse(err, cap, "attend: more than 2^37 cached tokens x heads with weights");
-    if (!(a->scale > 0.0f) || a->scale > 3.0e38f) return refuse(err, cap, "attend: scale must be a positive number");
+    if (!(a->scale > 0.0f) || a->scale > 2.3e38f) return refuse(err, cap, "attend: scale must be a positive number");
     if (a->workspace == nullptr || !aligned16(a->workspace) || a->workspace_bytes < fmha_kv4_attend_workspace(cache, a))
         return refuse(err, cap, "attend: the workspace must be 16-byte aligned and hold fmha_kv4_attend_workspace() bytes");
     if (a->out == a->q.data && a->S != 0u) {   // a row's elements are read before it is written, by whoever writes it; the weights of many rows go by the queries again

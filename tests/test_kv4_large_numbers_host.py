@@ -45,3 +45,12 @@ def test_pages_of_4_gib(abi):
         if heads > most:
             assert lib.fmha_kv4_attend(cache, abi.Kv4AttendArgs(q=rows, out=FAKE, S=3, H=heads, scale=1.0), None, err, 256) == 6 and message in err.value.decode()
             assert lib.fmha_kv4_evict(cache, cache, abi.Kv4EvictArgs(), None, err, 256) == 6 and message in err.value.decode()
+
+
+@pytest.mark.parametrize("scale", [2.4e38, 3.3e38])
+def test_scales_that_overflow_in_base_2(abi, scale):
+    lib, err = abi.load(), C.create_string_buffer(256)
+    a = abi.Kv4AttendArgs(q=_rows(abi), out=8 * FAKE, S=3, H=4, scale=scale, workspace=FAKE, workspace_bytes=1)
+    assert lib.fmha_kv4_attend(_cache(abi), a, None, err, 256) == 6 and "scale must be" in err.value.decode()
+    a.scale = 2.2e38
+    assert lib.fmha_kv4_attend(_cache(abi), a, None, err, 256) == 6 and "workspace" in err.value.decode()

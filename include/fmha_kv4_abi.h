@@ -66,8 +66,11 @@ int fmha_kv4_read(const fmha_kv4_cache* cache, const fmha_kv4_rows* k, const fmh
  *     KV head), for t < length; nothing is written behind the length. old = weights_in[b][kv][t] (same width; the same array, or one that shares no memory with it), 0 where weights_in is
  *     NULL and, with `causal`, for the n newest tokens. Sums in a fixed order: the same bits every time.
  *   NaN: a block of V that is NaN makes its 32 elements NaN in the rows that see the token, whatever the weight, and nothing else; NaN in K makes all of these rows NaN.
- *   Ranges: the products run in f16 against powers of two that are taken out, so that any scale goes. What is exact is a query row's elements down to 2^-30 of its largest,
- *     V's down to 2^-33 of the largest scale among 32 neighbouring tokens (128 with more than 32 query rows of a KV head, then K's as well); smaller ones count as less.
+ *   Ranges: the products run in f16 against powers of two that are taken out. What is exact is a query row's elements down to 2^-30 of its largest, V's down to 2^-33 of the largest
+ *     scale among 32 neighbouring tokens (128 with more than 32 query rows of a KV head, then K's as well); smaller ones count as less. Keys have to stay below 2^100, scores below 2^90
+ *     in size, and with `weights` of more than 8 rows of a KV head the products q . k, without the scale, within f32.
+ *     In front of V the softmax weights are rounded to f16, in their sum (log-sum-exp, `weights`) they are not. A token whose weight times V's scale is less than 2^-25 of the row's largest such
+ *     product leaves nothing in out, at most 1.5 * 2^-25 of that product each: 0.3 % of it if 65536 tokens are all that small.
  *   workspace: fmha_kv4_attend_workspace() bytes of device memory, 16-byte aligned; scratch, no initial contents.
  */
 typedef struct fmha_kv4_attend_args {

@@ -281,13 +281,17 @@ def _launch_path(lib, q, k, v, q_scale, k_scale, v_scale, out, path, splits, str
 
 
 def reset_workspaces():
-    """Drops the cached KV-split workspaces (partials, log-sum-exps, the fused merge's counters) after a synchronise; the next call makes new ones."""
+    """Drops the cached workspaces (partials, log-sum-exps, the fused merge's counters, those of the 4-bit cache) after a synchronise; the next call makes new ones. Waits for
+    calls that other threads are making."""
     import torch
     global _ws_generation
-    torch.cuda.synchronize()
-    _workspace.clear()
-    _calls.clear()
-    _ws_generation += 1
+    with contextlib.ExitStack() as held:
+        for lock in list(_ws_locks.values()):
+            held.enter_context(lock)
+        torch.cuda.synchronize()
+        _workspace.clear()
+        _calls.clear()
+        _ws_generation += 1
 
 
 def device_status() -> int:

@@ -245,3 +245,27 @@ def test_buffers_are_made_on_the_stream_that_uses_them(captured, monkeypatch):
     assert entered == [99, "out"]
     kv4.fmha_fwd_kv4(q, cache, torch.zeros_like(q), stream=99)
     assert entered == [99, "out"]
+
+
+def test_workspaces_are_not_dropped_under_a_call(no_gpu, monkeypatch):
+    """reset_workspaces from another thread comes behind the call that holds a buffer."""
+    lib, events, inside = TwoKernels(), [], threading.Event()
+
+    def attend(cache, a, stream, err, cap):
+        inside.set()
+        time.sleep(0.05)
+        events.append("enqueued")
+        return 0
+    lib.fmha_kv4_attend = attend
+    monkeypatch.setattr(_abi, "load", lambda: lib)
+    monkeypatch.setattr(torch.cuda, "synchronize", lambda: events.append("dropped"))
+
+    def call():
+        q = torch.zeros(1, 1, 1, 128, dtype=torch.bfloat16)
+        kv4.fmha_fwd_kv4(q, a_cache(), torch.empty_like(q))
+
+    def reset():
+        inside.wait(5)
+        ops.reset_workspaces()
+    in_threads(lambda i: reset() if i else call(), 2)
+    assert events == ["enqueued", "dropped"]

@@ -15,9 +15,10 @@
 // the 32 tokens, so that P 2^e is at most 2^4 however large V is; the factors relative to 2^e are exact in f16 down to 2^-34. M moves when a value exceeds it by more
 // than 2^4, by a vote of the warp; the sums and O are rescaled then.
 //
-// With one group of 8 columns the instruction stream is the bound, not the bytes: 64 sequences x 8 heads of 16384 tokens take 236 us, 4.8 TB/s of the 6.5 that a copy reaches; 594
-// instructions per 32 tokens of a warp (301 of them conversions, packing and logic, a pipe at half rate), issued in 55 % of the cycles. Four CTAs an SM are what the registers
-// allow; three of them took 226 us there but 71 in place of 68 on ragged sequences in pages of 16, five and six with two stages 470 to 610 (spills).
+// With one group of 8 columns the bound is latency, not the bytes and no pipe: 64 sequences x 8 heads of 16384 tokens take 237 to 257 us by box, 4.4 to 4.8 TB/s of the 6.5 that a copy reaches; 594
+// instructions per 32 tokens of a warp (301 of them conversions, packing and logic, a pipe at half rate that is busy 56 % of the time), issued in 56 % of the cycles by 16 warps an SM. Four CTAs an SM
+// are what the registers allow; three of them took 226 us where four took 236, but 71 in place of 68 on ragged sequences in pages of 16, five and six with two stages 470 to 610 (spills). The kernels
+// taken spill too: 68 and 80 bytes stored and loaded with one group, 84 and 124, 60 and 92, 292 and 424 with two, three and four.
 // Groups of 8 rows more cost their products and softmax: 32 rows over 16 x 4096 tokens 65 us, against 100 with the tiles of 128 rows.
 #include "kv4.cuh"
 #include "kv4_schedule.cuh"

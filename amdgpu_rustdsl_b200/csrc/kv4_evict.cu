@@ -5,7 +5,8 @@
 // above that key stay, and of those equal to it the earliest. Their places follow from ballots and counts in token order; a second
 // kernel copies the 136 bytes of each token that stays.
 //
-// The selection is bound by latency: the loads, and four exchanges of the cluster (1 to 2 us each). The keys stay in registers (16 a thread) where
+// The selection is bound by latency: the loads, four dependent rounds of histogram, barriers and scan (37 % of the issue slots with one CTA a head), and where a head has several CTAs an exchange of
+// the cluster in each (1 to 2 us). The keys stay in registers (16 a thread) where
 // the runs are short enough; else they are read again from L2 for every pass. 512 threads, so that two CTAs share an SM: with 1024, one a SM, 24 clusters of 8 took two rounds.
 // 16 x 8 heads of 4096 tokens to 1024: selection 15 us, copy 12; 3 x 8 heads of 50001 tokens to 6250: 22 and 11.
 #include "kv4.cuh"

@@ -13,7 +13,7 @@
 //
 // Bounds: a step of 256 rows and 128 tokens takes about 3750 clocks, of which the tensor cores work 2048 and the exponentials need as many; a tile's scores, softmax and product
 // follow one another, since the 512 columns of tensor memory are O and one S of both tiles. A CTA's change from one item to the next costs about 16000 clocks more. 4096 rows
-// over 8192 tokens, 32 heads on 8: 438 us = 0.94 PFLOP/s, 0.58 of the measured bf16 rate; 512 rows over 16384, 16 heads on 4: 90 us. Slower: scores in halves of 64 tokens (801 us
+// over 8192 tokens, 32 heads on 8: 445 us = 0.93 PFLOP/s, 0.57 of the measured bf16 rate; 512 rows over 16384, 16 heads on 4: 91 us, 27.4 steps a CTA. Spills: 296 bytes stored, 596 loaded. Slower: scores in halves of 64 tokens (801 us
 // when this took 746), two threads a row (594, then 473), part of the exponentials as polynomials (483, then 463), no turns of the tiles (558), P in one piece (457, then 447),
 // K in bf16 (458, with the query rows by asynchronous copies).
 //

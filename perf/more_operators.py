@@ -187,10 +187,10 @@ def _blocks(pool, page):
 
 
 def _scale_of(largest):
-    """The smallest power of two that brings `largest` to 448 or less, from 2^-100 to 2^119."""
+    """The smallest power of two that brings `largest` to 448 or less, from 2^-90 to 2^119."""
     mantissa, exponent = torch.frexp(largest)
-    e = torch.where(largest == 0, -100, exponent - 9 + (mantissa > LARGEST / 512).int())
-    return torch.ldexp(torch.ones_like(largest), e.clamp(-100, 119).int())
+    e = torch.where(largest == 0, -90, exponent - 9 + (mantissa > LARGEST / 512).int())
+    return torch.ldexp(torch.ones_like(largest), e.clamp(-90, 119).int())
 
 
 def _round(x, scale):
@@ -539,7 +539,7 @@ def _exact_append(case, s):
             for i, name in enumerate(("k", "v")):
                 x = s[name][b, :n, h].double()
                 blocks = torch.cat([torch.zeros(old, D, device="cuda", dtype=torch.float64), x, torch.zeros(fill, D, device="cuda", dtype=torch.float64)]).view(-1, BLOCK * D)
-                scale = torch.pow(2.0, torch.ceil(torch.log2(blocks.abs().amax(1).clamp(min=LARGEST * 2.0 ** -100) / LARGEST)))
+                scale = torch.pow(2.0, torch.ceil(torch.log2(blocks.abs().amax(1).clamp(min=LARGEST * 2.0 ** -90) / LARGEST)))
                 if old:
                     scale[0] = torch.maximum(scale[0], held[2 + i][0])
                 out[name][b, :n, h] = (_nearest_64(blocks / scale[:, None]) * scale[:, None]).view(-1, D)[old:old + n]

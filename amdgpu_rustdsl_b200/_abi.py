@@ -105,6 +105,24 @@ class Kv4EvictArgs(C.Structure):
                 ("keep", C.c_uint32), ("recent", C.c_uint32), ("first", C.c_uint32)]
 
 
+class Kv8AttendArgs(C.Structure):
+    _fields_ = [("q", Kv4Rows), ("out", C.c_void_p), ("counts", C.c_void_p), ("lse", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_uint64),
+                ("S", C.c_uint32), ("H", C.c_uint32), ("causal", C.c_uint32), ("scale", C.c_float)]
+
+
+class RopeArgs(C.Structure):
+    """fmha_rope_args"""
+    _fields_ = [("x", Kv4Rows), ("x_out", Kv4Rows), ("y", Kv4Rows), ("y_out", Kv4Rows), ("turns", C.c_void_p), ("positions", C.c_void_p),
+                ("positions_stride_b", C.c_int64), ("positions_stride_s", C.c_int64), ("positions_64", C.c_uint32), ("B", C.c_uint32), ("S", C.c_uint32),
+                ("heads_x", C.c_uint32), ("heads_y", C.c_uint32), ("head_dim", C.c_uint32), ("rotary", C.c_uint32), ("type", C.c_uint32),
+                ("interleaved", C.c_uint32), ("backward", C.c_uint32), ("factor", C.c_float)]
+
+
+class PagesArgs(C.Structure):
+    """fmha_pages"""
+    _fields_ = [("free", C.c_void_p), ("table", C.c_void_p), ("lengths", C.c_void_p), ("pages", C.c_uint32), ("B", C.c_uint32), ("page", C.c_uint32), ("table_width", C.c_uint32)]
+
+
 assert C.sizeof(AttnArgs) == 656 and C.sizeof(KvSplitArgs) == 648 and C.sizeof(CombineArgs) == 36
 assert AttnArgs.ext_ptr_peer_plan.offset == 0x38 and KvSplitArgs.ext_ptr_peer_plan.offset == 0x38
 assert AttnArgs.s_seq_len.offset == 0x60 and AttnArgs.ptr_q_descale.offset == 0x200 and AttnArgs.abi_tail.offset == 0x280
@@ -194,6 +212,20 @@ def load():
     lib.fmha_kv4_attend.argtypes = [cache, C.POINTER(Kv4AttendArgs)] + err
     lib.fmha_kv4_evict.restype = C.c_int
     lib.fmha_kv4_evict.argtypes = [cache, cache, C.POINTER(Kv4EvictArgs)] + err
+    lib.fmha_kv8_append.restype = C.c_int
+    lib.fmha_kv8_append.argtypes = [cache, rows, rows, C.c_uint32, C.c_void_p] + err
+    lib.fmha_kv8_read.restype = C.c_int
+    lib.fmha_kv8_read.argtypes = [cache, rows, rows, C.c_uint32, C.c_int, C.c_void_p] + err
+    lib.fmha_kv8_attend_workspace.restype = C.c_uint64
+    lib.fmha_kv8_attend_workspace.argtypes = [cache, C.POINTER(Kv8AttendArgs)]
+    lib.fmha_kv8_attend.restype = C.c_int
+    lib.fmha_kv8_attend.argtypes = [cache, C.POINTER(Kv8AttendArgs)] + err
+    lib.fmha_rope_rotate.restype = C.c_int
+    lib.fmha_rope_rotate.argtypes = [C.POINTER(RopeArgs)] + err
+    lib.fmha_pages_take.restype = C.c_int
+    lib.fmha_pages_take.argtypes = [C.POINTER(PagesArgs), C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_uint32] + err
+    lib.fmha_pages_cut.restype = C.c_int
+    lib.fmha_pages_cut.argtypes = [C.POINTER(PagesArgs), C.c_void_p] + err
     _lib = lib
     return lib
 
@@ -208,6 +240,10 @@ EXPORTS = (
 
 # include/fmha_kv4_abi.h
 KV4_EXPORTS = ("fmha_kv4_append", "fmha_kv4_read", "fmha_kv4_attend_workspace", "fmha_kv4_attend", "fmha_kv4_evict")
+# include/fmha_kv8_abi.h, fmha_rope_abi.h, fmha_pages_abi.h
+KV8_EXPORTS = ("fmha_kv8_append", "fmha_kv8_read", "fmha_kv8_attend_workspace", "fmha_kv8_attend")
+ROPE_EXPORTS = ("fmha_rope_rotate",)
+PAGES_EXPORTS = ("fmha_pages_take", "fmha_pages_cut")
 
 
 class ContractError(ValueError):

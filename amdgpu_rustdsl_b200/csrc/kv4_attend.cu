@@ -580,6 +580,22 @@ __global__ void __launch_bounds__(kTogether ? 32 * kTogether : 256) kv4_combine_
     if (p.lse != nullptr && lane == 0u) p.lse[(static_cast<size_t>(b) * p.H + h) * p.S + i] = none ? -INFINITY : (m + lg2(l)) * kLn2;
 }
 
+}  // namespace
+
+// what a launch of `grid` CTAs with items of `slots` rows (8 to 32, one row tile a sequence) or of `per` rows left in p.ws
+cudaError_t launch_combine_few(const Kv4AttendParams& p, uint32_t slots, uint32_t grid, cudaStream_t stream) {
+    // 4 warps have 16 parts in flight; where an item has more on average, 16 warps (5 rows over 65536 tokens, 74 parts: 28 us in place of 36)
+    const uint32_t rows = p.S * p.group, entries = begun_entries(p.c, 1u, grid), some = rows < slots ? rows : slots;
+    if (grid / entries > 16u) return kv4_launch(kv4_combine_kernel<16>, dim3(entries, some), 512u, 0, stream, p, slots, 1u, grid);
+    return kv4_launch(kv4_combine_kernel<4>, dim3(entries, some), 128u, 0, stream, p, slots, 1u, grid);
+}
+cudaError_t launch_combine_many(const Kv4AttendParams& p, uint32_t per, uint32_t row_tiles, uint32_t grid, cudaStream_t stream) {
+    const uint32_t rows = p.S * p.group, most = rows < per ? rows : per;
+    return kv4_launch(kv4_combine_kernel<0>, dim3(begun_entries(p.c, row_tiles, grid), (most + 7u) / 8u), 256u, 0, stream, p, per, row_tiles, grid);
+}
+
+namespace {
+
 // Rows of a KV head up to which this kernel is taken; more go to the tensor cores' tiles of 128 rows. 16 sequences of 4096 tokens: 20 rows 49 us here and 100 there, 32 rows 65 and 100;
 // one of 65536: 28 and 66, 34 and 67. (The registers end at 32: two passes over the cache would cost as much as the tiles do from about 48 rows on.)
 constexpr uint32_t kMostFew = 32;
@@ -594,7 +610,7 @@ uint32_t attend_grid(const Kv4View& c, uint32_t groups) {
 
 template <int NT>
 cudaError_t launch_rows(const Kv4AttendParams& p, cudaStream_t stream) {
-    const uint32_t grid = attend_grid(p.c, NT), rows = p.S * p.group;
+    const uint32_t grid = attend_grid(p.c, NT);
     const size_t smem = sizeof(CtaShared<NT>);
     static std::atomic<bool> set[64];
     int dev = 0;
@@ -606,18 +622,13 @@ cudaError_t launch_rows(const Kv4AttendParams& p, cudaStream_t stream) {
         if (dev >= 0 && dev < 64) set[dev].store(true, std::memory_order_relaxed);
     }
     e = kv4_launch(kv4_attend_kernel<NT>, dim3(grid), kThreads, smem, stream, p);
-    if (e != cudaSuccess) return e;
-    // 4 warps have 16 parts in flight; where an item has more on average, 16 warps (5 rows over 65536 tokens, 74 parts: 28 us in place of 36)
-    const uint32_t entries = begun_entries(p.c, 1u, grid), some = rows < 8u * NT ? rows : 8u * NT;
-    if (grid / entries > 16u) return kv4_launch(kv4_combine_kernel<16>, dim3(entries, some), 512u, 0, stream, p, 8u * NT, 1u, grid);
-    return kv4_launch(kv4_combine_kernel<4>, dim3(entries, some), 128u, 0, stream, p, 8u * NT, 1u, grid);
+    return e != cudaSuccess ? e : launch_combine_few(p, 8u * NT, grid, stream);
 }
 
 cudaError_t launch_many(const Kv4AttendParams& p, cudaStream_t stream) {
-    const uint32_t rows = p.S * p.group, per = kv4_prefill_rows(), row_tiles = (rows + per - 1u) / per, most = rows < per ? rows : per;
+    const uint32_t rows = p.S * p.group, per = kv4_prefill_rows(), row_tiles = (rows + per - 1u) / per;
     const cudaError_t e = launch_kv4_prefill(p, row_tiles, stream);
-    if (e != cudaSuccess) return e;
-    return kv4_launch(kv4_combine_kernel<0>, dim3(begun_entries(p.c, row_tiles, kv4_prefill_grid()), (most + 7u) / 8u), 256u, 0, stream, p, per, row_tiles, kv4_prefill_grid());
+    return e != cudaSuccess ? e : launch_combine_many(p, per, row_tiles, kv4_prefill_grid(), stream);
 }
 
 uint64_t partial_bytes(const Kv4View& c, uint32_t rows) {

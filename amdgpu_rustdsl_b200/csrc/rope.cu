@@ -1,0 +1,317 @@
+// Rotary positions (include/fmha_rope_abi.h): pairs of a row's elements are turned by position * frequency.
+//
+// A CTA has one to four tokens. Its threads first work out the tokens' sines and cosines, one pair each, into shared memory: the phase is position * frequency in 64-bit integers, whole
+// turns fall out at the top, and the quarter turn is taken off before the rest becomes f32. Then a thread keeps those of the pairs that it has in every head and goes over the token's
+// heads, 16 bytes of both halves of a head (or of neighbours) at a time, four heads in flight.
+// Bound by bytes: each row once in and once out; with one token a sequence by the launch and one trip to memory.
+#include "../../include/fmha_rope_abi.h"
+#include "cache_args.cuh"
+
+#include <cuda_fp16.h>
+
+namespace b200mx {
+
+namespace {
+
+constexpr uint32_t kThreads = 256, kMostTokens = 4, kMostPairs = FMHA_ROPE_MAX_HEAD_DIM / 2;
+
+struct Rows {
+    const uint8_t* in;
+    uint8_t* out;
+    long long in_b, in_s, in_h, out_b, out_s, out_h;   // bytes
+};
+
+struct RopeParams {
+    Rows x, y;
+    const unsigned long long* turns;
+    const void* positions;
+    long long positions_b, positions_s;
+    uint32_t S, tokens, heads_x, heads, head_dim, n;
+    uint32_t per_cta;      // tokens
+    uint32_t rotate, items;   // pieces of a row that are turned, and with those that are only copied
+    bool positions_64, backward, interleaved;
+    float factor;
+};
+
+// cos and sin of 2 pi phase / 2^64, the phase without whole turns
+__device__ __forceinline__ float2 turn(unsigned long long phase) {
+    const unsigned long long quarter = (phase + (1ull << 61)) >> 62;             // nearest quarter turn
+    const long long rest = static_cast<long long>(phase - (quarter << 62));      // within an eighth of a turn of it
+    float s, c;
+    sincospif(__ll2float_rn(rest) * 1.0842021724855044e-19f, &s, &c);            // 2^-63
+    if (quarter & 1ull) {
+        const float t = s;
+        s = c, c = -t;
+    }
+    return quarter & 2ull ? make_float2(-c, -s) : make_float2(c, s);
+}
+
+template <typename T> __device__ __forceinline__ float to_f32(T x);
+template <> __device__ __forceinline__ float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
+template <> __device__ __forceinline__ float to_f32(__half x) { return __half2float(x); }
+template <> __device__ __forceinline__ float to_f32(float x) { return x; }
+template <typename T> __device__ __forceinline__ T of_f32(float x);
+template <> __device__ __forceinline__ __nv_bfloat16 of_f32(float x) { return __float2bfloat16_rn(x); }
+template <> __device__ __forceinline__ __half of_f32(float x) { return __float2half_rn(x); }
+template <> __device__ __forceinline__ float of_f32(float x) { return x; }
+
+template <typename T, int N>
+struct alignas(sizeof(T) * N) Piece {
+    T at[N];
+};
+// (volatile: behind the wait for the grid before)
+template <typename T, int N>
+__device__ __forceinline__ Piece<T, N> load(const uint8_t* p) {
+    constexpr int kBytes = sizeof(T) * N;
+    union {
+        Piece<T, N> piece;
+        uint32_t w[kBytes >= 4 ? kBytes / 4 : 1];
+        uint16_t h;
+    } u;
+    if constexpr (kBytes == 16) asm volatile("ld.global.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(u.w[0]), "=r"(u.w[1]), "=r"(u.w[2]), "=r"(u.w[3]) : "l"(p));
+    if constexpr (kBytes == 8) asm volatile("ld.global.v2.u32 {%0, %1}, [%2];" : "=r"(u.w[0]), "=r"(u.w[1]) : "l"(p));
+    if constexpr (kBytes == 4) asm volatile("ld.global.u32 %0, [%1];" : "=r"(u.w[0]) : "l"(p));
+    if constexpr (kBytes == 2) asm volatile("ld.global.u16 %0, [%1];" : "=h"(u.h) : "l"(p));
+    return u.piece;
+}
+
+// N elements of T at a time. N = 1 takes both layouts, a pair's elements one by one.
+template <typename T, int N, bool kNeighbours>
+__global__ void __launch_bounds__(kThreads) rope_kernel(const __grid_constant__ RopeParams p) {
+    __shared__ float2 table[kMostTokens * kMostPairs];
+    kv4::pdl_launch();
+    kv4::pdl_wait();
+    const uint32_t token0 = blockIdx.x * p.per_cta, tokens = min(p.per_cta, p.tokens - token0);
+    for (uint32_t k = threadIdx.x; k < tokens * p.n; k += kThreads) {
+        const uint32_t token = token0 + k / p.n, i = k % p.n, b = token / p.S, s = token - b * p.S;
+        const long long at = b * p.positions_b + s * p.positions_s;
+        long long position;
+        if (p.positions_64) asm volatile("ld.global.s64 %0, [%1];" : "=l"(position) : "l"(static_cast<const long long*>(p.positions) + at));
+        else position = kv4::ld_i32(static_cast<const int32_t*>(p.positions) + at);
+        unsigned long long turns;
+        asm volatile("ld.global.u64 %0, [%1];" : "=l"(turns) : "l"(p.turns + i));
+        float2 t = turn(static_cast<unsigned long long>(position) * turns);
+        t.x *= p.factor, t.y *= p.backward ? -p.factor : p.factor;
+        table[k] = t;
+    }
+    __syncthreads();
+    // groups of `items` threads: one item each, tokens and heads dealt out to the groups
+    const uint32_t groups = p.items < kThreads ? kThreads / p.items : 1u, group = p.items < kThreads ? threadIdx.x / p.items : 0u;
+    const uint32_t sharing = groups / p.per_cta > 0u ? groups / p.per_cta : 1u;   // groups (of all CTAs of this token: times the grid's second dimension) that share a token
+    if (group >= sharing * p.per_cta) return;
+    const uint32_t mine = group % p.per_cta;   // (the token; there are at least as many groups as tokens)
+    if (mine >= tokens) return;
+    const uint32_t token = token0 + mine, b = token / p.S, s = token - b * p.S;
+    const uint32_t first = blockIdx.y * sharing + group / p.per_cta, stride = gridDim.y * sharing;
+    constexpr bool kScalar = N == 1;
+    constexpr uint32_t kPairs = kScalar ? 1 : kNeighbours ? N / 2 : N;
+    for (uint32_t item = p.items < kThreads ? threadIdx.x - group * p.items : threadIdx.x; item < p.items; item += p.items < kThreads ? p.items : kThreads) {
+        const bool turned = item < p.rotate;
+        // byte offsets within a row of the item's elements, and of their partners
+        const uint32_t from = turned ? (kScalar && p.interleaved ? 2u * item : item * N) : 2u * p.n + (item - p.rotate) * N;
+        const uint32_t at = from * static_cast<uint32_t>(sizeof(T)), partner = (kScalar && p.interleaved ? from + 1u : from + p.n) * static_cast<uint32_t>(sizeof(T));
+        const bool two = turned && !kNeighbours;
+        float2 t[kPairs];
+#pragma unroll
+        for (uint32_t i = 0; i < kPairs; ++i) t[i] = turned ? table[mine * p.n + item * kPairs + i] : make_float2(1.0f, 0.0f);
+        const uint8_t* in_x = p.x.in + b * p.x.in_b + s * p.x.in_s + at;
+        const uint8_t* in_y = p.y.in + b * p.y.in_b + s * p.y.in_s + at;
+        uint8_t* out_x = p.x.out + b * p.x.out_b + s * p.x.out_s + at;
+        uint8_t* out_y = p.y.out + b * p.y.out_b + s * p.y.out_s + at;
+        constexpr int kFlight = 4;
+        for (uint32_t h0 = first; h0 < p.heads; h0 += kFlight * stride) {
+            Piece<T, N> a[kFlight], c[kFlight];
+#pragma unroll
+            for (int k = 0; k < kFlight; ++k) {
+                const uint32_t h = h0 + k * stride;
+                if (h >= p.heads) continue;
+                const uint8_t* src = h < p.heads_x ? in_x + h * p.x.in_h : in_y + (h - p.heads_x) * p.y.in_h;
+                a[k] = load<T, N>(src);
+                if (two) c[k] = load<T, N>(src + (partner - at));
+            }
+#pragma unroll
+            for (int k = 0; k < kFlight; ++k) {
+                const uint32_t h = h0 + k * stride;
+                if (h >= p.heads) continue;
+                uint8_t* dst = h < p.heads_x ? out_x + h * p.x.out_h : out_y + (h - p.heads_x) * p.y.out_h;
+                if (turned) {
+                    if constexpr (kNeighbours) {
+#pragma unroll
+                        for (uint32_t i = 0; i < kPairs; ++i) {
+                            const float u = to_f32(a[k].at[2 * i]), v = to_f32(a[k].at[2 * i + 1]);
+                            a[k].at[2 * i] = of_f32<T>(fmaf(u, t[i].x, -(v * t[i].y)));
+                            a[k].at[2 * i + 1] = of_f32<T>(fmaf(u, t[i].y, v * t[i].x));
+                        }
+                    } else {
+#pragma unroll
+                        for (uint32_t i = 0; i < kPairs; ++i) {
+                            const float u = to_f32(a[k].at[i]), v = to_f32(c[k].at[i]);
+                            a[k].at[i] = of_f32<T>(fmaf(u, t[i].x, -(v * t[i].y)));
+                            c[k].at[i] = of_f32<T>(fmaf(u, t[i].y, v * t[i].x));
+                        }
+                        *reinterpret_cast<Piece<T, N>*>(dst + (partner - at)) = c[k];
+                    }
+                }
+                *reinterpret_cast<Piece<T, N>*>(dst) = a[k];
+            }
+        }
+    }
+}
+
+template <typename T, int N, bool kNeighbours>
+cudaError_t launch(RopeParams p, bool copies, cudaStream_t stream) {
+    p.rotate = N == 1 ? p.n : kNeighbours ? 2u * p.n / N : p.n / N;
+    p.items = p.rotate + (copies ? (p.head_dim - 2u * p.n) / N : 0u);
+    const uint32_t groups = p.items < kThreads ? kThreads / p.items : 1u, sms = static_cast<uint32_t>(current_sm_count());
+    // Four tokens a CTA share its sines; with few tokens one each, their heads dealt out over up to four CTAs
+    p.per_cta = p.tokens >= 16u * sms ? (groups < kMostTokens ? groups : kMostTokens) : 1u;
+    const uint32_t ctas = (p.tokens + p.per_cta - 1u) / p.per_cta, sharing = groups / p.per_cta > 0u ? groups / p.per_cta : 1u;
+    uint32_t split = 1;
+    while (split < 4u && 2u * split * ctas <= 2u * sms && 2u * split * sharing <= p.heads) split *= 2u;
+    return kv4_launch(rope_kernel<T, N, kNeighbours>, dim3(ctas, split), kThreads, 0, stream, p);
+}
+
+template <typename T, int N>
+cudaError_t launch_layout(const RopeParams& p, bool copies, cudaStream_t stream) {
+    if constexpr (N == 1) return launch<T, 1, false>(p, copies, stream);
+    else return p.interleaved ? launch<T, N, true>(p, copies, stream) : launch<T, N, false>(p, copies, stream);
+}
+// `unit`: the most elements that all rows and parts of rows are multiples of
+template <typename T>
+cudaError_t launch_type(const RopeParams& p, uint32_t unit, bool copies, cudaStream_t stream) {
+    if constexpr (sizeof(T) == 2) {
+        if (unit >= 8u) return launch_layout<T, 8>(p, copies, stream);
+    }
+    if (unit >= 4u) return launch_layout<T, 4>(p, copies, stream);
+    if (unit >= 2u) return launch_layout<T, 2>(p, copies, stream);
+    return launch_layout<T, 1>(p, copies, stream);
+}
+
+}  // namespace
+}  // namespace b200mx
+
+namespace {
+
+using b200mx::RopeParams;
+using b200mx::Rows;
+
+struct Extent {
+    uint64_t begin, end;   // bytes
+};
+Extent extent_of(const fmha_rope_rows& r, const fmha_rope_args& a, uint32_t heads, uint64_t size) {
+    const uint64_t begin = reinterpret_cast<uintptr_t>(r.data);
+    return {begin, begin + size * ((a.B - 1u) * static_cast<uint64_t>(r.stride_b) + (a.S - 1u) * static_cast<uint64_t>(r.stride_s) + (heads - 1u) * static_cast<uint64_t>(r.stride_h) + a.head_dim)};
+}
+// whether no element stands twice: each dimension's stride, in their order, is as long as what lies within it
+bool distinct(const fmha_rope_rows& r, const fmha_rope_args& a, uint32_t heads) {
+    struct {
+        uint64_t stride, size;
+    } d[3] = {{static_cast<uint64_t>(r.stride_b), a.B}, {static_cast<uint64_t>(r.stride_s), a.S}, {static_cast<uint64_t>(r.stride_h), heads}};
+    for (int i = 0; i < 2; ++i) {
+        for (int j = 0; j < 2 - i; ++j) {
+            if (d[j].stride > d[j + 1].stride) {
+                const auto t = d[j];
+                d[j] = d[j + 1], d[j + 1] = t;
+            }
+        }
+    }
+    uint64_t inner = a.head_dim;
+    for (int i = 0; i < 3; ++i) {
+        if (d[i].size == 1u) continue;
+        if (d[i].stride < inner) return false;
+        inner = d[i].stride * (d[i].size - 1u) + inner;
+    }
+    return true;
+}
+// Whether two tensors' elements are kept apart, as far as it shows: they lie behind one another, or they are heads of the same tokens' rows that do
+bool apart(const fmha_rope_rows& r, uint32_t r_heads, const fmha_rope_rows& q, uint32_t q_heads, const fmha_rope_args& a, uint64_t size) {
+    const Extent x = extent_of(r, a, r_heads, size), y = extent_of(q, a, q_heads, size);
+    if (x.end <= y.begin || y.end <= x.begin) return true;
+    if ((a.B > 1u && r.stride_b != q.stride_b) || (a.S > 1u && r.stride_s != q.stride_s)) return false;
+    const bool first = x.begin < y.begin;
+    const uint64_t ahead = first ? y.begin - x.begin : x.begin - y.begin;
+    const uint64_t front = size * ((first ? r_heads - 1u : q_heads - 1u) * static_cast<uint64_t>(first ? r.stride_h : q.stride_h) + a.head_dim);
+    const uint64_t back = size * ((first ? q_heads - 1u : r_heads - 1u) * static_cast<uint64_t>(first ? q.stride_h : r.stride_h) + a.head_dim);
+    // the token's part in front ends where the other begins, and that ends in front of the next token's
+    uint64_t next = ~0ull;
+    if (a.S > 1u) next = size * static_cast<uint64_t>(r.stride_s);
+    if (a.B > 1u && size * static_cast<uint64_t>(r.stride_b) < next) next = size * static_cast<uint64_t>(r.stride_b);
+    return ahead >= front && ahead + back <= next;
+}
+
+int check_rows(const fmha_rope_rows& r, const fmha_rope_args& a, uint32_t heads, uint64_t size, const char* name, char* err, size_t cap) {
+    if (r.data == nullptr) return refuse(err, cap, "rope: %s must be given", name);
+    if (reinterpret_cast<uintptr_t>(r.data) % size != 0) return refuse(err, cap, "rope: %s must be aligned as its elements are", name);
+    if (r.stride_b < 0 || r.stride_s < 0 || r.stride_h < 0) return refuse(err, cap, "rope: %s has negative strides", name);
+    const int64_t most = 1ll << 56;
+    const auto fits = [&](int64_t stride, uint64_t n) { return n <= 1u || static_cast<uint64_t>(stride) <= static_cast<uint64_t>(most) / n; };
+    if (!fits(r.stride_b, a.B) || !fits(r.stride_s, a.S) || !fits(r.stride_h, heads)) return refuse(err, cap, "rope: %s is larger than any memory", name);
+    return 0;
+}
+
+// strides that dimensions of one element have are of no matter
+void clear_strides(fmha_rope_rows& r, const fmha_rope_args& a, uint32_t heads) {
+    if (a.B == 1u) r.stride_b = 0;
+    if (a.S == 1u) r.stride_s = 0;
+    if (heads <= 1u) r.stride_h = 0;
+}
+
+}  // namespace
+
+extern "C" int fmha_rope_rotate(const fmha_rope_args* args, void* stream, char* err, size_t cap) {
+    if (args == nullptr) return refuse(err, cap, "rope: no arguments");
+    fmha_rope_args a = *args;
+    if (a.type > FMHA_ROPE_F32) return refuse(err, cap, "rope: type must be bf16, f16 or f32");
+    if (a.head_dim == 0u || a.head_dim > FMHA_ROPE_MAX_HEAD_DIM || a.rotary < 2u || a.rotary % 2u != 0u || a.rotary > a.head_dim)
+        return refuse(err, cap, "rope: heads have up to %u elements, of which an even number is turned (%u of %u)", FMHA_ROPE_MAX_HEAD_DIM, a.rotary, a.head_dim);
+    if (!(a.factor > 0.0f) || a.factor > 3.0e38f) return refuse(err, cap, "rope: factor must be a positive number");
+    if (a.heads_x == 0u) return refuse(err, cap, "rope: x has no heads");
+    if (a.turns == nullptr || (reinterpret_cast<uintptr_t>(a.turns) & 7u) != 0) return refuse(err, cap, "rope: turns must be given and aligned");
+    if (a.B == 0u || a.S == 0u) return 0;
+    const uint64_t size = a.type == FMHA_ROPE_F32 ? 4u : 2u;
+    if (a.positions == nullptr || reinterpret_cast<uintptr_t>(a.positions) % (a.positions_64 ? 8u : 4u) != 0) return refuse(err, cap, "rope: positions must be given and aligned");
+    if (static_cast<uint64_t>(a.B) * a.S > kMostRows || static_cast<uint64_t>(a.heads_x) + a.heads_y > kMostRows || static_cast<uint64_t>(a.B) * a.S * (static_cast<uint64_t>(a.heads_x) + a.heads_y) > (1ull << 40))
+        return refuse(err, cap, "rope: more than 2^30 tokens, or 2^40 rows");
+    clear_strides(a.x, a, a.heads_x), clear_strides(a.x_out, a, a.heads_x), clear_strides(a.y, a, a.heads_y), clear_strides(a.y_out, a, a.heads_y);
+    if (int r = check_rows(a.x, a, a.heads_x, size, "x", err, cap)) return r;
+    if (int r = check_rows(a.x_out, a, a.heads_x, size, "x_out", err, cap)) return r;
+    const auto same = [](const fmha_rope_rows& r, const fmha_rope_rows& q) { return r.data == q.data && r.stride_b == q.stride_b && r.stride_s == q.stride_s && r.stride_h == q.stride_h; };
+    if (!distinct(a.x_out, a, a.heads_x)) return refuse(err, cap, "rope: elements of x_out share memory");
+    if (!same(a.x, a.x_out) && !apart(a.x, a.heads_x, a.x_out, a.heads_x, a, size)) return refuse(err, cap, "rope: x_out must be x or share no memory with it");
+    bool copies = !same(a.x, a.x_out);
+    if (a.heads_y != 0u) {
+        if (int r = check_rows(a.y, a, a.heads_y, size, "y", err, cap)) return r;
+        if (int r = check_rows(a.y_out, a, a.heads_y, size, "y_out", err, cap)) return r;
+        if (!distinct(a.y_out, a, a.heads_y)) return refuse(err, cap, "rope: elements of y_out share memory");
+        if (!same(a.y, a.y_out) && !apart(a.y, a.heads_y, a.y_out, a.heads_y, a, size)) return refuse(err, cap, "rope: y_out must be y or share no memory with it");
+        if (!apart(a.x_out, a.heads_x, a.y_out, a.heads_y, a, size) || !apart(a.x_out, a.heads_x, a.y, a.heads_y, a, size) || !apart(a.x, a.heads_x, a.y_out, a.heads_y, a, size))
+            return refuse(err, cap, "rope: an output must not share memory with the other input or output");
+        copies |= !same(a.y, a.y_out);
+    }
+    RopeParams p = {};
+    const auto rows = [&](const fmha_rope_rows& in, const fmha_rope_rows& out) {
+        const long long z = static_cast<long long>(size);
+        return Rows{static_cast<const uint8_t*>(in.data), static_cast<uint8_t*>(out.data), z * in.stride_b, z * in.stride_s, z * in.stride_h, z * out.stride_b, z * out.stride_s, z * out.stride_h};
+    };
+    p.x = rows(a.x, a.x_out);
+    p.y = a.heads_y != 0u ? rows(a.y, a.y_out) : p.x;
+    p.turns = reinterpret_cast<const unsigned long long*>(a.turns);
+    p.positions = a.positions, p.positions_b = a.positions_stride_b, p.positions_s = a.positions_stride_s, p.positions_64 = a.positions_64 != 0u;
+    p.S = a.S, p.tokens = a.B * a.S, p.heads_x = a.heads_x, p.heads = a.heads_x + a.heads_y, p.head_dim = a.head_dim, p.n = a.rotary / 2u;
+    p.backward = a.backward != 0u, p.interleaved = a.interleaved != 0u, p.factor = a.factor;
+    // the widest access that everything is a multiple of
+    uint32_t unit = 16u / static_cast<uint32_t>(size);
+    const auto limit = [&](uint64_t bytes) {
+        while (unit > 1u && bytes % (unit * size) != 0u) unit /= 2u;
+    };
+    for (const fmha_rope_rows* r : {&a.x, &a.x_out, &a.y, &a.y_out}) {
+        if (r == &a.y && a.heads_y == 0u) break;
+        limit(reinterpret_cast<uintptr_t>(r->data)), limit(size * r->stride_b), limit(size * r->stride_s), limit(size * r->stride_h);
+    }
+    limit(size * (p.interleaved ? 2u * p.n : p.n));
+    if (copies) limit(size * (p.head_dim - 2u * p.n));
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    return done(a.type == FMHA_ROPE_BF16 ? b200mx::launch_type<__nv_bfloat16>(p, unit, copies, st) : a.type == FMHA_ROPE_F16 ? b200mx::launch_type<__half>(p, unit, copies, st)
+                                                                                                                      : b200mx::launch_type<float>(p, unit, copies, st),
+                err, cap);
+}

@@ -35,7 +35,30 @@ def kv4_pool(pages, kv_heads, page=64, device="cuda"):
     return torch.zeros((pages, kv_heads, TOKEN_BYTES * page), dtype=torch.uint8, device=device)
 
 
-class Kv4Cache:
+class PagedCache:
+    """Views of the caller's pool, table and lengths as the C struct: what the caches of 4 and of 8 bits have in common."""
+    __slots__ = ("pool", "table", "lengths", "page", "B", "HK", "capacity", "device", "c")
+    TOKEN_BYTES = 0   # of a token and KV head
+
+    def __init__(self, pool, table, lengths):
+        import torch
+        who, token = type(self).__name__, self.TOKEN_BYTES
+        if pool.dtype != torch.uint8 or pool.dim() != 3 or pool.shape[2] % token or pool.shape[2] // token not in PAGE_SIZES:
+            raise ValueError(f"{who}: pool must be uint8 [pages, KV heads, {token} * page] with pages of 16, 32, 64 or 128 tokens")
+        if table.dtype != torch.int32 or table.dim() != 2 or lengths.dtype != torch.int32 or tuple(lengths.shape) != (table.shape[0],):
+            raise ValueError(f"{who}: table must be int32 [B, width] and lengths int32 [B]")
+        for name, t in (("pool", pool), ("table", table), ("lengths", lengths)):
+            if not t.is_cuda or t.device != pool.device or not t.is_contiguous() or t.numel() == 0:
+                raise ValueError(f"{who}: {name} must be a contiguous CUDA tensor on the pool's device with something in it")
+        if pool.data_ptr() % 16:
+            raise ValueError(f"{who}: pool must start on a 16-byte boundary")
+        self.pool, self.table, self.lengths, self.device = pool, table, lengths, pool.device
+        self.page, self.HK, self.B = pool.shape[2] // token, pool.shape[1], table.shape[0]
+        self.capacity = table.shape[1] * self.page   # tokens that a sequence has room for
+        self.c = _abi.Kv4CacheArgs(pool.data_ptr(), table.data_ptr(), lengths.data_ptr(), pool.shape[0], self.B, self.HK, self.page, table.shape[1])
+
+
+class Kv4Cache(PagedCache):
     """A paged cache of MXFP4 keys and values: views of the caller's tensors, nothing of its own.
 
     pool     uint8 [pages, HK, 136 * page], page 16, 32, 64 or 128 (``kv4_pool``)
@@ -44,23 +67,8 @@ class Kv4Cache:
 
     The tensors may be written between calls (on the stream of the calls), not replaced.
     """
-    __slots__ = ("pool", "table", "lengths", "page", "B", "HK", "capacity", "device", "c")
-
-    def __init__(self, pool, table, lengths):
-        import torch
-        if pool.dtype != torch.uint8 or pool.dim() != 3 or pool.shape[2] % TOKEN_BYTES or pool.shape[2] // TOKEN_BYTES not in PAGE_SIZES:
-            raise ValueError("Kv4Cache: pool must be uint8 [pages, KV heads, 136 * page] with pages of 16, 32, 64 or 128 tokens")
-        if table.dtype != torch.int32 or table.dim() != 2 or lengths.dtype != torch.int32 or tuple(lengths.shape) != (table.shape[0],):
-            raise ValueError("Kv4Cache: table must be int32 [B, width] and lengths int32 [B]")
-        for name, t in (("pool", pool), ("table", table), ("lengths", lengths)):
-            if not t.is_cuda or t.device != pool.device or not t.is_contiguous() or t.numel() == 0:
-                raise ValueError(f"Kv4Cache: {name} must be a contiguous CUDA tensor on the pool's device with something in it")
-        if pool.data_ptr() % 16:
-            raise ValueError("Kv4Cache: pool must start on a 16-byte boundary")
-        self.pool, self.table, self.lengths, self.device = pool, table, lengths, pool.device
-        self.page, self.HK, self.B = pool.shape[2] // TOKEN_BYTES, pool.shape[1], table.shape[0]
-        self.capacity = table.shape[1] * self.page   # tokens that a sequence has room for
-        self.c = _abi.Kv4CacheArgs(pool.data_ptr(), table.data_ptr(), lengths.data_ptr(), pool.shape[0], self.B, self.HK, self.page, table.shape[1])
+    __slots__ = ()
+    TOKEN_BYTES = TOKEN_BYTES
 
 
 def _rows(who, name, x, cache, S=None, heads=None):

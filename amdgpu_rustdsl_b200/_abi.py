@@ -223,7 +223,7 @@ def load():
     lib.fmha_rope_rotate.restype = C.c_int
     lib.fmha_rope_rotate.argtypes = [C.POINTER(RopeArgs)] + err
     lib.fmha_pages_take.restype = C.c_int
-    lib.fmha_pages_take.argtypes = [C.POINTER(PagesArgs), C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_uint32] + err
+    lib.fmha_pages_take.argtypes = [C.POINTER(PagesArgs), C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_void_p, C.c_void_p, C.c_uint32] + err
     lib.fmha_pages_cut.restype = C.c_int
     lib.fmha_pages_cut.argtypes = [C.POINTER(PagesArgs), C.c_void_p] + err
     _lib = lib

@@ -16,9 +16,11 @@ struct PagesParams {
     int32_t *free, *table, *lengths;
     uint32_t pages, B, page_log2, table_width;
     const int32_t* asked;   // counts, or what to keep
-    int32_t *granted, *positions, *starts;
+    int32_t *granted, *starts;
+    void* positions;
     long long* slots;
     uint32_t S;
+    bool positions_64;
 };
 
 // cached nowhere on the SM: other CTAs write it in the same launch
@@ -155,7 +157,11 @@ __global__ void __launch_bounds__(kThreads) pages_take_kernel(const __grid_const
         for (uint32_t r = share(rows, blockIdx.x) + threadIdx.x; r < end; r += kThreads) {
             const uint32_t b = r / p.S, i = r - b * p.S, x = b - range.begin, t = sm_length[x] + i;
             const bool live = i < sm_granted[x];
-            if (p.positions != nullptr) p.positions[r] = live ? static_cast<int32_t>(t) : -1;
+            if (p.positions != nullptr) {
+                const int position = live ? static_cast<int32_t>(t) : -1;
+                if (p.positions_64) static_cast<long long*>(p.positions)[r] = position;
+                else static_cast<int32_t*>(p.positions)[r] = position;
+            }
             if (p.slots != nullptr) {
                 long long slot = -1;
                 if (live) {
@@ -260,7 +266,7 @@ uint32_t grid_of(uint32_t B, uint64_t rows) {
 
 extern "C" {
 
-int fmha_pages_take(const fmha_pages* pages, const int32_t* counts, int32_t* granted, int32_t* positions, int64_t* slots, int32_t* starts, uint32_t S, void* stream, char* err, size_t cap) {
+int fmha_pages_take(const fmha_pages* pages, const int32_t* counts, int32_t* granted, void* positions, int positions_64, int64_t* slots, int32_t* starts, uint32_t S, void* stream, char* err, size_t cap) {
     PagesParams p = {};
     if (int r = params_of(pages, "take", p, err, cap)) return r;
     if (counts == nullptr || granted == nullptr) return refuse(err, cap, "take: counts and granted must be given");
@@ -268,10 +274,10 @@ int fmha_pages_take(const fmha_pages* pages, const int32_t* counts, int32_t* gra
     const bool maps = positions != nullptr || slots != nullptr;
     if (maps && static_cast<uint64_t>(p.B) * S > kMostRows) return refuse(err, cap, "take: more than 2^30 rows");
     const uint64_t rows = maps ? static_cast<uint64_t>(p.B) * S : 0u;
-    const Span s[] = {{granted, 4ull * p.B, "granted"}, {positions, 4u * rows, "positions"}, {slots, 8u * rows, "slots"}, {starts, 4ull * (p.B + 1ull), "starts"}, {counts, 4ull * p.B, "counts"},
+    const Span s[] = {{granted, 4ull * p.B, "granted"}, {positions, (positions_64 ? 8u : 4u) * rows, "positions"}, {slots, 8u * rows, "slots"}, {starts, 4ull * (p.B + 1ull), "starts"}, {counts, 4ull * p.B, "counts"},
                       {p.free, 4ull * (p.pages + 4ull), "the stack"}, {p.table, 4ull * p.B * p.table_width, "the table"}, {p.lengths, 4ull * p.B, "the lengths"}};
     if (int r = check_apart(s, 8, 7, "take", err, cap)) return r;
-    p.asked = counts, p.granted = granted, p.positions = positions, p.slots = reinterpret_cast<long long*>(slots), p.starts = starts, p.S = S;
+    p.asked = counts, p.granted = granted, p.positions = positions, p.positions_64 = positions_64 != 0, p.slots = reinterpret_cast<long long*>(slots), p.starts = starts, p.S = S;
     return done(b200mx::kv4_launch(b200mx::pages_take_kernel, dim3(grid_of(p.B, rows)), b200mx::kThreads, 0, static_cast<cudaStream_t>(stream), p), err, cap);
 }
 

@@ -75,16 +75,48 @@ __device__ __forceinline__ Piece<T, N> load(const uint8_t* p) {
     return u.piece;
 }
 
+constexpr uint32_t kFlight = 4;   // heads of a thread at a time
+
 // N elements of T at a time. N = 1 takes both layouts, a pair's elements one by one.
 template <typename T, int N, bool kNeighbours>
-__global__ void __launch_bounds__(kThreads) rope_kernel(const __grid_constant__ RopeParams p) {
+__global__ void __launch_bounds__(kThreads, 3) rope_kernel(const __grid_constant__ RopeParams p) {
     __shared__ float2 table[kMostTokens * kMostPairs];
     kv4::pdl_launch();
     kv4::pdl_wait();
     const uint32_t token0 = blockIdx.x * p.per_cta, tokens = min(p.per_cta, p.tokens - token0);
+    // groups of `items` threads: one item each, tokens and heads dealt out to the groups
+    const uint32_t groups = p.items < kThreads ? kThreads / p.items : 1u, group = p.items < kThreads ? threadIdx.x / p.items : 0u;
+    const uint32_t sharing = groups / p.per_cta;   // groups that share a token, of each CTA along the grid's second dimension
+    const uint32_t mine = group % p.per_cta, stride = gridDim.y * sharing;
+    const bool active = group < sharing * p.per_cta && mine < tokens;
+    const uint32_t token = token0 + (active ? mine : 0u), b = token / p.S, s = token - b * p.S;
+    const uint32_t first = blockIdx.y * sharing + group / p.per_cta;
+    constexpr bool kScalar = N == 1;
+    constexpr uint32_t kPairs = kScalar ? 1 : kNeighbours ? N / 2 : N;
+    const uint32_t item0 = p.items < kThreads ? threadIdx.x - group * p.items : threadIdx.x, item_step = p.items < kThreads ? p.items : kThreads;
+    const uint8_t *in_x = p.x.in + b * p.x.in_b + s * p.x.in_s, *in_y = p.y.in + b * p.y.in_b + s * p.y.in_s;
+    uint8_t *out_x = p.x.out + b * p.x.out_b + s * p.x.out_s, *out_y = p.y.out + b * p.y.out_b + s * p.y.out_s;
+    // byte offsets within a row of an item's elements, and of their partners
+    const auto turned = [&](uint32_t item) { return item < p.rotate; };
+    const auto offset = [&](uint32_t item) {
+        return (turned(item) ? (kScalar && p.interleaved ? 2u * item : item * N) : 2u * p.n + (item - p.rotate) * N) * static_cast<uint32_t>(sizeof(T));
+    };
+    const uint32_t partner = (kScalar && p.interleaved ? 1u : p.n) * static_cast<uint32_t>(sizeof(T));
+    Piece<T, N> a[kFlight], c[kFlight];
+    const auto fetch = [&](uint32_t item, uint32_t h0) {
+#pragma unroll
+        for (uint32_t k = 0; k < kFlight; ++k) {
+            const uint32_t h = h0 + k * stride;
+            if (h >= p.heads) continue;
+            const uint8_t* src = (h < p.heads_x ? in_x + h * p.x.in_h : in_y + (h - p.heads_x) * p.y.in_h) + offset(item);
+            a[k] = load<T, N>(src);
+            if (!kNeighbours && turned(item)) c[k] = load<T, N>(src + partner);
+        }
+    };
+    if (active && item0 < p.items) fetch(item0, first);   // under way while the sines are worked out
     for (uint32_t k = threadIdx.x; k < tokens * p.n; k += kThreads) {
-        const uint32_t token = token0 + k / p.n, i = k % p.n, b = token / p.S, s = token - b * p.S;
-        const long long at = b * p.positions_b + s * p.positions_s;
+        const uint32_t at_token = token0 + k / p.n, i = k % p.n, at_b = at_token / p.S, at_s = at_token - at_b * p.S;
+        const long long at = at_b * p.positions_b + at_s * p.positions_s;
         long long position;
         if (p.positions_64) asm volatile("ld.global.s64 %0, [%1];" : "=l"(position) : "l"(static_cast<const long long*>(p.positions) + at));
         else position = kv4::ld_i32(static_cast<const int32_t*>(p.positions) + at);
@@ -95,62 +127,28 @@ __global__ void __launch_bounds__(kThreads) rope_kernel(const __grid_constant__ 
         table[k] = t;
     }
     __syncthreads();
-    // groups of `items` threads: one item each, tokens and heads dealt out to the groups
-    const uint32_t groups = p.items < kThreads ? kThreads / p.items : 1u, group = p.items < kThreads ? threadIdx.x / p.items : 0u;
-    const uint32_t sharing = groups / p.per_cta > 0u ? groups / p.per_cta : 1u;   // groups (of all CTAs of this token: times the grid's second dimension) that share a token
-    if (group >= sharing * p.per_cta) return;
-    const uint32_t mine = group % p.per_cta;   // (the token; there are at least as many groups as tokens)
-    if (mine >= tokens) return;
-    const uint32_t token = token0 + mine, b = token / p.S, s = token - b * p.S;
-    const uint32_t first = blockIdx.y * sharing + group / p.per_cta, stride = gridDim.y * sharing;
-    constexpr bool kScalar = N == 1;
-    constexpr uint32_t kPairs = kScalar ? 1 : kNeighbours ? N / 2 : N;
-    for (uint32_t item = p.items < kThreads ? threadIdx.x - group * p.items : threadIdx.x; item < p.items; item += p.items < kThreads ? p.items : kThreads) {
-        const bool turned = item < p.rotate;
-        // byte offsets within a row of the item's elements, and of their partners
-        const uint32_t from = turned ? (kScalar && p.interleaved ? 2u * item : item * N) : 2u * p.n + (item - p.rotate) * N;
-        const uint32_t at = from * static_cast<uint32_t>(sizeof(T)), partner = (kScalar && p.interleaved ? from + 1u : from + p.n) * static_cast<uint32_t>(sizeof(T));
-        const bool two = turned && !kNeighbours;
+    if (!active) return;
+    for (uint32_t item = item0; item < p.items; item += item_step) {
         float2 t[kPairs];
 #pragma unroll
-        for (uint32_t i = 0; i < kPairs; ++i) t[i] = turned ? table[mine * p.n + item * kPairs + i] : make_float2(1.0f, 0.0f);
-        const uint8_t* in_x = p.x.in + b * p.x.in_b + s * p.x.in_s + at;
-        const uint8_t* in_y = p.y.in + b * p.y.in_b + s * p.y.in_s + at;
-        uint8_t* out_x = p.x.out + b * p.x.out_b + s * p.x.out_s + at;
-        uint8_t* out_y = p.y.out + b * p.y.out_b + s * p.y.out_s + at;
-        constexpr int kFlight = 4;
+        for (uint32_t i = 0; i < kPairs; ++i) t[i] = turned(item) ? table[mine * p.n + item * kPairs + i] : make_float2(1.0f, 0.0f);
         for (uint32_t h0 = first; h0 < p.heads; h0 += kFlight * stride) {
-            Piece<T, N> a[kFlight], c[kFlight];
+            if (item != item0 || h0 != first) fetch(item, h0);
 #pragma unroll
-            for (int k = 0; k < kFlight; ++k) {
+            for (uint32_t k = 0; k < kFlight; ++k) {
                 const uint32_t h = h0 + k * stride;
                 if (h >= p.heads) continue;
-                const uint8_t* src = h < p.heads_x ? in_x + h * p.x.in_h : in_y + (h - p.heads_x) * p.y.in_h;
-                a[k] = load<T, N>(src);
-                if (two) c[k] = load<T, N>(src + (partner - at));
-            }
+                uint8_t* dst = (h < p.heads_x ? out_x + h * p.x.out_h : out_y + (h - p.heads_x) * p.y.out_h) + offset(item);
+                if (turned(item)) {
 #pragma unroll
-            for (int k = 0; k < kFlight; ++k) {
-                const uint32_t h = h0 + k * stride;
-                if (h >= p.heads) continue;
-                uint8_t* dst = h < p.heads_x ? out_x + h * p.x.out_h : out_y + (h - p.heads_x) * p.y.out_h;
-                if (turned) {
-                    if constexpr (kNeighbours) {
-#pragma unroll
-                        for (uint32_t i = 0; i < kPairs; ++i) {
-                            const float u = to_f32(a[k].at[2 * i]), v = to_f32(a[k].at[2 * i + 1]);
-                            a[k].at[2 * i] = of_f32<T>(fmaf(u, t[i].x, -(v * t[i].y)));
-                            a[k].at[2 * i + 1] = of_f32<T>(fmaf(u, t[i].y, v * t[i].x));
-                        }
-                    } else {
-#pragma unroll
-                        for (uint32_t i = 0; i < kPairs; ++i) {
-                            const float u = to_f32(a[k].at[i]), v = to_f32(c[k].at[i]);
-                            a[k].at[i] = of_f32<T>(fmaf(u, t[i].x, -(v * t[i].y)));
-                            c[k].at[i] = of_f32<T>(fmaf(u, t[i].y, v * t[i].x));
-                        }
-                        *reinterpret_cast<Piece<T, N>*>(dst + (partner - at)) = c[k];
+                    for (uint32_t i = 0; i < kPairs; ++i) {
+                        T& first_of = kNeighbours ? a[k].at[2 * i] : a[k].at[i];
+                        T& second_of = kNeighbours ? a[k].at[2 * i + 1] : c[k].at[i];
+                        const float u = to_f32(first_of), v = to_f32(second_of);
+                        first_of = of_f32<T>(fmaf(u, t[i].x, -(v * t[i].y)));
+                        second_of = of_f32<T>(fmaf(u, t[i].y, v * t[i].x));
                     }
+                    if (!kNeighbours) *reinterpret_cast<Piece<T, N>*>(dst + partner) = c[k];
                 }
                 *reinterpret_cast<Piece<T, N>*>(dst) = a[k];
             }
@@ -163,9 +161,16 @@ cudaError_t launch(RopeParams p, bool copies, cudaStream_t stream) {
     p.rotate = N == 1 ? p.n : kNeighbours ? 2u * p.n / N : p.n / N;
     p.items = p.rotate + (copies ? (p.head_dim - 2u * p.n) / N : 0u);
     const uint32_t groups = p.items < kThreads ? kThreads / p.items : 1u, sms = static_cast<uint32_t>(current_sm_count());
-    // Four tokens a CTA share its sines; with few tokens one each, their heads dealt out over up to four CTAs
-    p.per_cta = p.tokens >= 16u * sms ? (groups < kMostTokens ? groups : kMostTokens) : 1u;
-    const uint32_t ctas = (p.tokens + p.per_cta - 1u) / p.per_cta, sharing = groups / p.per_cta > 0u ? groups / p.per_cta : 1u;
+    // With many tokens as many of them a CTA, up to four, as give the most heads a thread in one round of loads; with few one each, their heads dealt out over up to four CTAs
+    p.per_cta = 1u;
+    if (p.tokens >= 16u * sms) {
+        uint32_t best = 0;
+        for (uint32_t t = 1; t <= kMostTokens && t <= groups; ++t) {
+            const uint32_t rounds = (p.heads + groups / t * kFlight - 1u) / (groups / t * kFlight), busy = t * p.heads * 1024u / (rounds * kFlight);
+            if (busy > best) best = busy, p.per_cta = t;
+        }
+    }
+    const uint32_t ctas = (p.tokens + p.per_cta - 1u) / p.per_cta, sharing = groups / p.per_cta;
     uint32_t split = 1;
     while (split < 4u && 2u * split * ctas <= 2u * sms && 2u * split * sharing <= p.heads) split *= 2u;
     return kv4_launch(rope_kernel<T, N, kNeighbours>, dim3(ctas, split), kThreads, 0, stream, p);

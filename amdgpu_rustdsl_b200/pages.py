@@ -39,7 +39,7 @@ def pages_take(free, cache, counts, granted, *, positions=None, slots=None, star
     in front of it are more than are free.
 
     granted    int32 [B]: counts[b] or 0; what ``kv8_append`` and the attention take as ``counts``
-    positions  int32 [B, S]: of row i < granted[b] the token it becomes, the length before plus i; -1 in other rows
+    positions  int32 or int64 [B, S]: of row i < granted[b] the token it becomes, the length before plus i; -1 in other rows
     slots      int64 [B, S]: page number times tokens of a page, plus the place within it, of that token; -1 in other rows
     starts     int32 [B + 1]: the sums of granted in front of each sequence, and of all
     """
@@ -50,11 +50,11 @@ def pages_take(free, cache, counts, granted, *, positions=None, slots=None, star
         raise ValueError("pages_take: counts and granted must be given")
     n, g = _i32("pages_take", "counts", counts, cache, (cache.B,)), _i32("pages_take", "granted", granted, cache, (cache.B,))
     S = 0
-    for name, x, dtype in (("positions", positions, torch.int32), ("slots", slots, torch.int64)):
+    for name, x, kinds in (("positions", positions, (torch.int32, torch.int64)), ("slots", slots, (torch.int64,))):
         if x is None:
             continue
-        if x.dtype != dtype or x.dim() != 2 or x.shape[0] != cache.B or (S and x.shape[1] != S) or x.device != cache.device or not x.is_contiguous():
-            raise ValueError(f"pages_take: {name} must be a contiguous {dtype} tensor [{cache.B}, S] on the cache's device, positions and slots with the same S")
+        if x.dtype not in kinds or x.dim() != 2 or x.shape[0] != cache.B or (S and x.shape[1] != S) or x.device != cache.device or not x.is_contiguous():
+            raise ValueError(f"pages_take: {name} must be a contiguous {" or ".join(map(str, kinds))} tensor [{cache.B}, S] on the cache's device, positions and slots with the same S")
         S = x.shape[1]
     if S > 0x7FFFFFFF:
         raise ValueError(f"pages_take: {S} rows, more than 2^31")
@@ -62,7 +62,7 @@ def pages_take(free, cache, counts, granted, *, positions=None, slots=None, star
         raise ValueError("pages_take: positions and slots must have the same S")
     s = _i32("pages_take", "starts", starts, cache, (cache.B + 1,))
     raw = stream if stream is not None else _raw_stream(torch, cache.device)
-    rc = _call(torch, cache, raw, lib.fmha_pages_take, p, n, g, None if positions is None else positions.data_ptr(), None if slots is None else slots.data_ptr(), s, S)
+    rc = _call(torch, cache, raw, lib.fmha_pages_take, p, n, g, None if positions is None else positions.data_ptr(), positions is not None and positions.dtype == torch.int64, None if slots is None else slots.data_ptr(), s, S)
     if rc:
         _check("pages_take", rc)
 

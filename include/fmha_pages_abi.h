@@ -29,14 +29,14 @@ typedef struct fmha_pages {
  * take: sequence b asks for counts[b] new tokens (below 0: none). It needs the pages that length + counts[b] tokens take and it does not have; sequences are served in order. One is
  *   granted all of its tokens, or none where its table has no room for them, or where it needs pages and the pages needed by it and the sequences in front of it (those without room
  *   aside) are more than are free. granted[b] = counts[b] or 0; the new pages go from the stack to the table, in order; lengths[b] grows by granted[b].
- *   positions: NULL or int32 [B][S]: of row i < granted[b] the token it becomes, length (before) + i; -1 in other rows.
+ *   positions: NULL or int32 [B][S] (int64 with positions_64): of row i < granted[b] the token it becomes, length (before) + i; -1 in other rows.
  *   slots: NULL or int64 [B][S]: page * (tokens of a page) + place within the page of that token; -1 in other rows and where the table names no page.
  *   starts: NULL or int32 [B + 1]: sums of granted in front of each sequence, and of all.
  *   granted, positions, slots and starts share no memory with counts, the stack, the table, the lengths or one another.
  * cut: lengths[b] becomes min(length, max(keep[b], 0)); pages without tokens go back to the stack, their table entries become -1. The last sequence's last page goes onto it first: a cut
  *   to the lengths before a take leaves stack, table and lengths as they were before it. Pages that the stack has no room for are dropped. keep shares no memory with the others.
  */
-int fmha_pages_take(const fmha_pages* p, const int32_t* counts, int32_t* granted, int32_t* positions, int64_t* slots, int32_t* starts, uint32_t S, void* stream, char* err, size_t cap);
+int fmha_pages_take(const fmha_pages* p, const int32_t* counts, int32_t* granted, void* positions, int positions_64, int64_t* slots, int32_t* starts, uint32_t S, void* stream, char* err, size_t cap);
 int fmha_pages_cut(const fmha_pages* p, const int32_t* keep, void* stream, char* err, size_t cap);
 
 #ifdef __cplusplus

@@ -70,11 +70,11 @@ class State:
         free, table, lengths = self.lists
         return self.free.tolist() == free and self.cache.table.tolist() == table and self.cache.lengths.tolist() == lengths
 
-    def take(self, counts, S, **without):
+    def take(self, counts, S, positions=torch.int32, **without):
         from amdgpu_rustdsl_b200 import pages_take
         B = self.cache.B
-        out = dict(positions=torch.full((B, S), -9, dtype=torch.int32, device="cuda"), slots=torch.full((B, S), -9, dtype=torch.int64, device="cuda"), starts=torch.full((B + 1,), -9, dtype=torch.int32, device="cuda"))
-        out = {k: None if k in without else v for k, v in out.items()}
+        out = dict(positions=torch.full((B, S), -9, dtype=positions or torch.int32, device="cuda"), slots=torch.full((B, S), -9, dtype=torch.int64, device="cuda"), starts=torch.full((B + 1,), -9, dtype=torch.int32, device="cuda"))
+        out = {k: None if k in without or positions is None and k == "positions" else v for k, v in out.items()}
         granted = torch.full((B,), -9, dtype=torch.int32, device="cuda")
         pages_take(self.free, self.cache, torch.tensor(counts, dtype=torch.int32, device="cuda"), granted, **out)
         want = plain_take(*self.lists, counts, self.page, S)
@@ -101,7 +101,7 @@ def test_tokens_come_and_go(page, bits):
     for step in range(25):
         most = [1, 4, 3 * page, 1, 0][step % 5]
         counts = torch.randint(0, most + 1, (5,), generator=g).tolist()
-        s.take(counts, max(1, most))
+        s.take(counts, max(1, most), torch.int64 if step % 2 else torch.int32)
         if step % 3 == 2:
             s.cut([max(0, n - int(torch.randint(0, 5, (1,), generator=g))) for n in s.lists[2]])
         if step % 7 == 6:
@@ -133,7 +133,7 @@ def test_batches_of_all_sizes_and_back(B, S, page, L):
 
 
 def test_outputs_that_nobody_asks_for():
-    for without in (dict(positions=1), dict(slots=1), dict(starts=1), dict(positions=1, slots=1, starts=1)):
+    for without in (dict(positions=None), dict(slots=1), dict(starts=1), dict(positions=None, slots=1, starts=1), dict(positions=torch.int64), dict(positions=torch.int64, slots=1)):
         State([20, 3, 0], 16, 8, 9).take([30, 1, 17], 40, **without)
 
 
@@ -159,7 +159,6 @@ def test_graphs_and_other_streams():
     s = State([10, 40, 16], 16, 6, 7)
     counts, granted = torch.tensor([9, 9, 1], dtype=torch.int32, device="cuda"), torch.empty(3, dtype=torch.int32, device="cuda")
     positions = torch.empty(3, 9, dtype=torch.int32, device="cuda")
-    before = s.free.clone(), s.cache.table.clone(), s.cache.lengths.clone()
     keep = s.cache.lengths.clone()
     graph = torch.cuda.CUDAGraph()
     torch.cuda.synchronize()
@@ -174,7 +173,8 @@ def test_graphs_and_other_streams():
     torch.cuda.synchronize()
     pages_cut(s.free, s.cache, keep, stream=side.cuda_stream)
     side.synchronize()
-    assert all(torch.equal(a, b) for a, b in zip(before, (s.free, s.cache.table, s.cache.lengths)))
+    plain_cut(*s.lists, [10, 40, 16], 16)   # (three takes handed pages out in turns: they go back in another order)
+    assert s.same()
 
 
 def test_refusals_of_the_python_entry():
@@ -185,7 +185,7 @@ def test_refusals_of_the_python_entry():
     for call, message in (
             (lambda: pages_take(s.free.long(), s.cache, counts, granted), "int32"), (lambda: pages_take(s.free.cpu(), s.cache, counts, granted), "device"), (lambda: pages_take(s.free[:4], s.cache, counts, granted), "pages"),
             (lambda: pages_take(s.free, s.cache, None, granted), "counts"), (lambda: pages_take(s.free, s.cache, counts, None), "granted"), (lambda: pages_take(s.free, s.cache, i32(3), granted), "counts"),
-            (lambda: pages_take(s.free, s.cache, counts, counts), "share memory"), (lambda: pages_take(s.free, s.cache, counts, granted, positions=i32(3, 2)), "positions"),
+            (lambda: pages_take(s.free, s.cache, counts, counts), "share memory"), (lambda: pages_take(s.free, s.cache, counts, granted, positions=i32(3, 2)), "positions"), (lambda: pages_take(s.free, s.cache, counts, granted, positions=i32(2, 2).float()), "positions"),
             (lambda: pages_take(s.free, s.cache, counts, granted, slots=i32(2, 2)), "slots"), (lambda: pages_take(s.free, s.cache, counts, granted, positions=i32(2, 3), slots=i32(2, 2).long()), "slots"),
             (lambda: pages_take(s.free, s.cache, counts, granted, positions=i32(2, 0), slots=i32(2, 2).long()), "same S"), (lambda: pages_take(s.free, s.cache, counts, granted, starts=i32(2)), "starts"),
             (lambda: pages_cut(s.free, s.cache, None), "keep"), (lambda: pages_cut(s.free, s.cache, i32(3)), "keep"), (lambda: pages_cut(s.free, s.cache, s.cache.lengths), "share memory")):

@@ -14,9 +14,9 @@ def _pages(abi, **change):
     return p
 
 
-def _take(abi, p, counts=4 * FAKE, granted=5 * FAKE, positions=6 * FAKE, slots=7 * FAKE, starts=8 * FAKE, S=3):
+def _take(abi, p, counts=4 * FAKE, granted=5 * FAKE, positions=6 * FAKE, slots=7 * FAKE, starts=8 * FAKE, S=3, wide=0):
     err = C.create_string_buffer(256)
-    return abi.load().fmha_pages_take(p, counts, granted, positions, slots, starts, S, None, err, 256), err.value.decode()
+    return abi.load().fmha_pages_take(p, counts, granted, positions, wide, slots, starts, S, None, err, 256), err.value.decode()
 
 
 def _cut(abi, p, keep=4 * FAKE):
@@ -35,7 +35,7 @@ def test_bad_pages_are_refused(abi, change, message):
 
 @pytest.mark.parametrize("change,message", [({"counts": None}, "must be given"), ({"granted": None}, "must be given"), ({"granted": 4 * FAKE}, "granted must not share"), ({"positions": 5 * FAKE + 8}, "granted must not share"),
                                             ({"slots": 6 * FAKE + 40}, "positions must not share"), ({"starts": 7 * FAKE + 90}, "slots must not share"), ({"starts": 4 * FAKE + 8}, "counts"),
-                                            ({"positions": FAKE + 400}, "the stack"), ({"slots": 2 * FAKE + 100}, "the table"), ({"starts": 3 * FAKE + 12}, "the lengths"), ({"S": 1 << 29}, "2^30")])
+                                            ({"positions": FAKE + 400}, "the stack"), ({"slots": 2 * FAKE + 100}, "the table"), ({"starts": 3 * FAKE + 12}, "the lengths"), ({"S": 1 << 29}, "2^30"), ({"slots": 6 * FAKE + 48, "wide": 1}, "positions must not share")])
 def test_bad_takes_are_refused(abi, change, message):
     rc, err = _take(abi, _pages(abi), **change)
     assert rc == 6 and message in err, err

@@ -10,22 +10,27 @@ namespace kv4 {
 
 constexpr uint32_t kStepTokens = 128;
 
-struct Deal {
+// (steps of kTokens: what the text above says of 128 tokens holds for them)
+template <uint32_t kTokens>
+struct DealOf {
     uint32_t rows, row_tiles;   // of an item, of a sequence
 };
+using Deal = DealOf<kStepTokens>;
 
-__device__ __forceinline__ uint32_t steps_of(const Kv4AttendParams& p, const Deal& d, uint32_t entry) {
+template <uint32_t kTokens>
+__device__ __forceinline__ uint32_t steps_of(const Kv4AttendParams& p, const DealOf<kTokens>& d, uint32_t entry) {
     const uint32_t b = entry / d.row_tiles, row0 = (entry - b * d.row_tiles) * d.rows, length = length_of(p.c, b), n = count_of(p.counts, b, p.S, length);
     if (row0 >= n * p.group) return 0u;
     const uint32_t last = (min(row0 + d.rows, n * p.group) - 1u) / p.group;
-    return ((p.causal ? length - n + last + 1u : length) + kStepTokens - 1u) / kStepTokens;
+    return ((p.causal ? length - n + last + 1u : length) + kTokens - 1u) / kTokens;
 }
 
 struct Sums {
     uint32_t below, all;
 };
 // Steps of the entries below `upto`, and of all, times the heads (the host has checked that they stay below 2^32). All threads of the CTA; `part` has an element per warp.
-__device__ __forceinline__ Sums sum_steps(const Kv4AttendParams& p, const Deal& d, uint32_t upto, Sums* part) {
+template <uint32_t kTokens>
+__device__ __forceinline__ Sums sum_steps(const Kv4AttendParams& p, const DealOf<kTokens>& d, uint32_t upto, Sums* part) {
     uint32_t below = 0, all = 0;
     for (uint32_t e = threadIdx.x; e < p.c.B * d.row_tiles; e += blockDim.x) {
         const uint32_t t = steps_of(p, d, e);
@@ -55,7 +60,8 @@ struct Place {
     uint32_t entry;
     uint32_t in;   // step within the entry's items
 };
-__device__ __forceinline__ Place find_step(const Kv4AttendParams& p, const Deal& d, uint32_t pos) {
+template <uint32_t kTokens>
+__device__ __forceinline__ Place find_step(const Kv4AttendParams& p, const DealOf<kTokens>& d, uint32_t pos) {
     const unsigned lane = threadIdx.x & 31u;
     const uint32_t entries = p.c.B * d.row_tiles;
     uint32_t before = 0;
@@ -83,7 +89,8 @@ struct Segment {
     uint32_t first, steps, of;      // steps first .. first + steps - 1 of `of`
 };
 // The segment at the head of a CTA's run of `left` steps; moves on behind it
-__device__ __forceinline__ Segment next_segment(const Kv4AttendParams& p, const Deal& d, Place& at, uint32_t& left) {
+template <uint32_t kTokens>
+__device__ __forceinline__ Segment next_segment(const Kv4AttendParams& p, const DealOf<kTokens>& d, Place& at, uint32_t& left) {
     uint32_t of = steps_of(p, d, at.entry);
     while (at.in >= of * p.c.HK) {   // also where an entry has none
         at.in -= of * p.c.HK;
@@ -109,10 +116,12 @@ __host__ __device__ __forceinline__ bool begun_by_item(const Kv4View& c, uint32_
 __host__ __device__ __forceinline__ uint32_t begun_entries(const Kv4View& c, uint32_t row_tiles, uint32_t grid) { return begun_by_item(c, row_tiles, grid) ? c.B * c.HK * row_tiles : grid; }
 __device__ __forceinline__ Begun* begun_at(float* ws, uint32_t x) { return reinterpret_cast<Begun*>(ws) + x; }
 // by one thread of a CTA: at its start, and for each segment
-__device__ __forceinline__ void begin_nothing(const Kv4AttendParams& p, const Deal& d) {
+template <uint32_t kTokens>
+__device__ __forceinline__ void begin_nothing(const Kv4AttendParams& p, const DealOf<kTokens>& d) {
     if (!begun_by_item(p.c, d.row_tiles, gridDim.x)) *begun_at(p.ws, blockIdx.x) = {0u, blockIdx.x, blockIdx.x, 0u};
 }
-__device__ __forceinline__ void begin_item(const Kv4AttendParams& p, const Deal& d, const Segment& s, uint32_t pos, uint32_t all, uint32_t n_work) {
+template <uint32_t kTokens>
+__device__ __forceinline__ void begin_item(const Kv4AttendParams& p, const DealOf<kTokens>& d, const Segment& s, uint32_t pos, uint32_t all, uint32_t n_work) {
     if (s.first != 0u) return;
     const uint32_t item = (s.b * d.row_tiles + s.row0 / d.rows) * p.c.HK + s.head, last = s.steps == s.of ? blockIdx.x : worker_at(all, n_work, pos + s.of - 1u);
     const bool by_item = begun_by_item(p.c, d.row_tiles, gridDim.x);
@@ -122,7 +131,8 @@ __device__ __forceinline__ float* slot_of(float* ws, uint32_t grid, uint32_t w, 
 constexpr float kLowest = -1e30f;   // M of a row that has seen nothing
 
 // Sequences' row tiles that no CTA has steps of: their rows see nothing. All threads of the grid.
-__device__ __forceinline__ void clear_empty_entries(const Kv4AttendParams& p, const Deal& d) {
+template <uint32_t kTokens>
+__device__ __forceinline__ void clear_empty_entries(const Kv4AttendParams& p, const DealOf<kTokens>& d) {
     for (uint32_t e = blockIdx.x; e < p.c.B * d.row_tiles; e += gridDim.x) {
         if (steps_of(p, d, e) != 0u) continue;
         if (begun_by_item(p.c, d.row_tiles, gridDim.x)) {

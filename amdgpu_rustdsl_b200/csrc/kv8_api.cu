@@ -52,9 +52,9 @@ int fmha_kv8_attend(const fmha_kv8_cache* cache, const fmha_kv8_attend_args* a, 
     if ((a->out == nullptr && a->S != 0u) || !aligned16(a->out)) return refuse(err, cap, "attend: out must be given and 16-byte aligned");
     if (a->S == 0u) return 0;
     if (static_cast<uint64_t>(p.c.B) * a->S * a->H > kMostRows) return refuse(err, cap, "attend: more than 2^30 query rows");
-    // the kernels deal out steps of 128 tokens and 256 rows at most, counted in 32 bits
+    // the kernels deal out steps of 80 tokens and 256 rows at least, counted in 32 bits
     const uint64_t tokens = static_cast<uint64_t>(p.c.table_width) << p.c.page_log2, row_tiles = (static_cast<uint64_t>(a->S) * (a->H / p.c.HK) + 255u) / 256u;
-    if (((tokens + 127u) / 128u) * p.c.B * p.c.HK > 0xFFFFFFFFull / row_tiles) return refuse(err, cap, "attend: more than 2^32 steps of 128 tokens and 256 query rows");
+    if (((tokens + 79u) / 80u) * p.c.B * p.c.HK > 0xFFFFFFFFull / row_tiles) return refuse(err, cap, "attend: more than 2^32 steps of 80 tokens and 256 query rows");
     if (!(a->scale > 0.0f) || a->scale > 2.3e38f) return refuse(err, cap, "attend: scale must be a positive number");
     if (a->workspace == nullptr || !aligned16(a->workspace) || a->workspace_bytes < fmha_kv8_attend_workspace(cache, a))
         return refuse(err, cap, "attend: the workspace must be 16-byte aligned and hold fmha_kv8_attend_workspace() bytes");

@@ -6,10 +6,10 @@
 // Q is f16 with a power of two per row taken out, exact down to 2^-30 of the row's largest.
 //
 // A CTA has 256 query rows of one KV head (rows of the sequence and of the head's group packed, whatever the group's size) as two tiles of 128 and goes over the tokens
-// 128 at a time. Per step four warps turn the step's K and V codes into f16 in shared memory, once for both tiles; one thread a tile issues the products, S from shared
-// memory, P V with P from tensor memory; and two groups of four warps do the softmax, one tile each, a thread a row, so that the tensor cores work on one tile while the
-// other's softmax runs. P overwrites S in tensor memory and goes over in two halves of 64 tokens, the first while the second is still being computed. m moves only
-// when a row's maximum exceeds it by 2^(kUp + kSlack), so O is hardly ever rescaled.
+// 80 at a time, five blocks: that is what makes a tile's O (128 columns), scores (80) and weights (40) fit half of tensor memory side by side, so that the next step's scores are computed
+// while the softmax works on this step's. Per step one warp brings the codes (cp.async.bulk), four warps turn them into f16 in shared memory, once for both tiles, a thread a tile issues
+// the products, S from shared memory, P V with P from tensor memory, and two groups of four warps do the softmax, one tile each, a thread a row. m moves only when a row's maximum
+// exceeds it by 2^(kUp + kSlack), so O is hardly ever rescaled.
 //
 // Steps are dealt out to one CTA per SM as kv4_schedule.cuh says; items that several CTAs worked on go through f32 partials and the combine kernel.
 #include "kv4_schedule.cuh"
@@ -26,36 +26,48 @@ namespace {
 using namespace kv8;
 using namespace sm100;
 
-constexpr uint32_t kTileRows = 128, kItemRows = 256, kStages = 2, kHalf = 64;
-// Slots of the steps' scales. The converters write those of step j + 4 behind the scores of step j + 2, which are behind the P of step j + 1 of the tiles that go on
-constexpr uint32_t kFactorSlots = 4;
-// Slots of the segments' first tokens with NaN in V. The converters begin segment n behind its step's third forerunner, whose scores both issuing warps have issued: these are in segment n - 3 at least,
-// and an issuing warp begins a segment when its tile's softmax has stored the one before
-constexpr uint32_t kNanSlots = 4;
-constexpr uint32_t kAtomBytes = 128u * 128u, kTileBytes = 2u * kAtomBytes;   // 128 rows x 64 elements with 128-byte swizzle; two of them a tile
+constexpr uint32_t kTileRows = 128, kItemRows = 256, kStep = 80, kBlocks = kStep / kBlockTokens, kStages = 3, kRawStages = 2;
+// Slots of the steps' scales. Those of step j are written when its codes have come, for which those of step j - 2 must have been taken: behind the scores of step j - 5 (three stages of K)
+// and so behind the softmax's reads of the scores of step j - 6
+constexpr uint32_t kScaleSlots = 8;
+// Slots of the segments. Segment n is published, and its first token with NaN in V noted, when the codes of a step of segment n - 3 at least have been taken, behind the products of one of
+// segment n - 6, and so behind the end of segment n - 7
+constexpr uint32_t kSegmentSlots = 8;
+constexpr uint32_t kQAtom = 128u * 128u, kTileBytes = 2u * kQAtom;   // 128 rows x 64 elements with 128-byte swizzle; two of them a tile of query rows
+constexpr uint32_t kAtomBytes = kStep * 128u, kStepBytes = 2u * kAtomBytes;   // the same of a step's K or V
 constexpr uint32_t kThreads = 512;
-// Warps 0-3 and 4-7: softmax of tile 0 and 1; 8-11: codes to f16; 12 and 13: products of tile 0 and 1. The pools of setmaxnreg come out of the launch's 128 registers a thread.
-constexpr int kSoftmaxRegs = 176, kConvertRegs = 112, kIssueRegs = 48;
+// Warps 0-3 and 4-7: softmax of tile 0 and 1; 8-11: codes to f16; 12 and 13: products of tile 0 and 1; 14: copies; 15: scales. The pools of setmaxnreg come out of the launch's 128
+// registers a thread.
+constexpr uint32_t kIssueWarp = 12, kCopyWarp = 14;
+constexpr int kSoftmaxRegs = 168, kConvertRegs = 96, kIssueRegs = 80;
 static_assert(8 * kSoftmaxRegs + 4 * kConvertRegs + 4 * kIssueRegs <= 16 * 128, "register shares");
-constexpr uint32_t kColS = 0, kColO = 256;   // S of tile q (P in its first half) at 128 q, O at 256 + 128 q
+constexpr uint32_t kColP = 80, kColO = 128, kColTile = 256;   // of a tile's 256 columns: S, P, O
 constexpr float kUpF = 6.0f, kSlack = 8.0f;   // (f16 has more room above 1 than a weight needs)
 constexpr float kLeast = 1e-37f;   // times a masked score it is still -inf
 constexpr float kLn2 = 0.69314718055994531f;
 
 // barriers; kPFull by 2 q + half
-enum Bar : uint32_t { kKFull = 0, kKEmpty = 2, kVFull = 4, kVEmpty = 6, kSFull = 8, kODone = 10, kPFull = 12, kOFree = 16, kQFull = 18, kQEmpty = 20, kTurn = 22, kDrained = 24, kEFull = 26, kBars = 26 + kFactorSlots };
+enum Bar : uint32_t {
+    kKFull = 0, kKEmpty = kKFull + kStages, kVFull = kKEmpty + kStages, kVEmpty = kVFull + kStages,   // by stage
+    kRawFull = kVEmpty + kStages, kRawEmpty = kRawFull + kRawStages,
+    kSFull = kRawEmpty + kRawStages, kSFree = kSFull + 2, kPFull = kSFree + 2, kPFree = kPFull + 2, kOFree = kPFree + 2, kQFull = kOFree + 2, kQEmpty = kQFull + 2, kDrained = kQEmpty + 2,   // by tile
+    kScales = kDrained + 2, kSegment = kScales + kScaleSlots, kBars = kSegment + kSegmentSlots
+};
 
 struct Shared {
-    uint8_t q[2][kTileBytes], k[kStages][kTileBytes], v[kStages][kTileBytes];
-    float2 scales[kFactorSlots][kStepTokens / kBlockTokens];   // of K and V
-    uint32_t nan_from[kNanSlots][4];   // of a segment and a converting warp: the first token that has NaN in its V, all ones where none has
+    uint8_t q[2][kTileBytes], k[kStages][kStepBytes], v[kStages][kStepBytes];
+    uint8_t raw_k[kRawStages][kBlocks][kVCodes], raw_v[kRawStages][kBlocks][kMeta - kVCodes];   // a step's codes as they come
+    uint4 meta[kRawStages][kBlocks];   // and its scales and masks
+    uint32_t plain[kScaleSlots];       // whether every token of a step has numbers
+    alignas(16) float scales[kScaleSlots][3][8];   // of a step's blocks: scale of K, exponent e of V's, 2^-e
+    uint32_t nan_from[kSegmentSlots];  // of a segment: the first token that has NaN in its V, all ones where none has
     unsigned long long bars[kBars];
     Sums part[kThreads / 32];
     struct Plan {
         Segment seg;
-        uint32_t pos, length, n, number;   // (segments are counted from 1)
-    } plan[8];                     // of a softmax warp's next segment
-    uint32_t converting[4];        // number of a converting warp's segment
+        uint32_t length, n, left;      // left: steps of the CTA's run behind the segment
+        uint32_t steps[2];             // of the two tiles: those that their last live rows see
+    } plan[kSegmentSlots];
     uint32_t tmem, failed, not_drained;
 };
 
@@ -81,10 +93,35 @@ __device__ __forceinline__ uint32_t tile_steps(const Kv8AttendParams& p, const S
     const uint32_t r0 = s.row0 + q * kTileRows;
     if (r0 >= n * p.group) return 0u;
     const uint32_t last = (min(r0 + kTileRows, n * p.group) - 1u) / p.group;
-    const uint32_t of = ((p.causal ? length - n + last + 1u : length) + kStepTokens - 1u) / kStepTokens;
+    const uint32_t of = ((p.causal ? length - n + last + 1u : length) + kStep - 1u) / kStep;
     return of <= s.first ? 0u : min(s.steps, of - s.first);
 }
 
+// the larger of three
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t* r) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]) : "memory");
+}
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
+}
+// waits for two barriers; where both are there already, in the time that one takes
+__device__ __forceinline__ bool mbar_wait2(uint32_t a, uint32_t a_parity, uint32_t b, uint32_t b_parity, volatile uint32_t* abort_flag) {
+    uint32_t first, second;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%2], %3;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 q, [%4], %5;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\tselp.u32 %1, 1, 0, q;\n\t}"
+        : "=r"(first), "=r"(second)
+        : "r"(a), "r"(a_parity), "r"(b), "r"(b_parity)
+        : "memory");
+    return (first != 0u || mbar_wait(a, a_parity, abort_flag)) && (second != 0u || mbar_wait(b, b_parity, abort_flag));
+}
 // eight codes as f16
 __device__ __forceinline__ uint4 to_f16(uint32_t lo, uint32_t hi) { return make_uint4(e4m3x2_lo(lo), e4m3x2_hi(lo), e4m3x2_lo(hi), e4m3x2_hi(hi)); }
 __device__ __forceinline__ uint4* piece_at(uint8_t* tile, uint32_t row, uint32_t piece) {   // 8 elements of a row of a tile
@@ -98,27 +135,25 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
     const uint32_t bars = smem_u32(sh.bars);
     auto bar = [&](uint32_t i) { return bars + 8u * i; };
     if (threadIdx.x == 0u) {
+        for (uint32_t i = 0; i < kStages; ++i) mbar_init(bar(kKFull + i), 128u), mbar_init(bar(kVFull + i), 128u), mbar_init(bar(kKEmpty + i), 2u), mbar_init(bar(kVEmpty + i), 2u);
+        for (uint32_t i = 0; i < kRawStages; ++i) mbar_init(bar(kRawFull + i), 1u), mbar_init(bar(kRawEmpty + i), 4u);
         for (uint32_t i = 0; i < 2; ++i) {
-            mbar_init(bar(kKFull + i), 128u), mbar_init(bar(kVFull + i), 128u);
-            mbar_init(bar(kKEmpty + i), 2u), mbar_init(bar(kVEmpty + i), 2u), mbar_init(bar(kOFree + i), 4u);
-            mbar_init(bar(kSFull + i), 1u), mbar_init(bar(kODone + i), 1u), mbar_init(bar(kQFull + i), 4u), mbar_init(bar(kQEmpty + i), 1u);
-            mbar_init(bar(kTurn + i), 1u), mbar_init(bar(kDrained + i), 1u);
+            mbar_init(bar(kSFull + i), 1u), mbar_init(bar(kSFree + i), 4u), mbar_init(bar(kPFull + i), 4u), mbar_init(bar(kPFree + i), 1u), mbar_init(bar(kOFree + i), 4u);
+            mbar_init(bar(kQFull + i), 4u), mbar_init(bar(kQEmpty + i), 1u), mbar_init(bar(kDrained + i), 1u);
         }
-        for (uint32_t i = 0; i < 4; ++i) mbar_init(bar(kPFull + i), 4u);
-        for (uint32_t i = 0; i < kFactorSlots; ++i) mbar_init(bar(kEFull + i), 4u);
-        
+        for (uint32_t i = 0; i < kScaleSlots; ++i) mbar_init(bar(kScales + i), 1u);
+        for (uint32_t i = 0; i < kSegmentSlots; ++i) mbar_init(bar(kSegment + i), 1u);
         fence_mbar_init();
         sh.failed = sh.not_drained = 0u;
-        for (uint32_t i = 0; i < 8; ++i) sh.plan[i].number = sh.converting[i & 3u] = 0u;
     }
-    if (warp == 12u) tmem_alloc(smem_u32(&sh.tmem), 512u);
+    if (warp == kIssueWarp) tmem_alloc(smem_u32(&sh.tmem), 512u);
     tc_fence_before_sync();
     __syncthreads();
     tc_fence_after_sync();
     const uint32_t tmem = __shfl_sync(0xFFFFFFFFu, sh.tmem, 0);
     pdl_launch();
     pdl_wait();
-    const Deal deal{kItemRows, row_tiles};
+    const DealOf<kStep> deal{kItemRows, row_tiles};
     const uint32_t all = sum_steps(p, deal, 0u, sh.part).all;
     const uint32_t n_work = workers(all, gridDim.x);
     volatile uint32_t* failed = &sh.failed;
@@ -127,128 +162,125 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
     if (blockIdx.x < n_work) {
         const uint32_t begin = run_begin(all, n_work, blockIdx.x);
         const uint32_t end = run_begin(all, n_work, blockIdx.x + 1u);
-        uint32_t left = end - begin;
-        Place at = find_step(p, deal, begin);
+        uint32_t number = 0;   // of the role's segment
+        // the next segment, once the copying warp has published it; all lanes. False: a wait has run out
+        const auto next_plan = [&](Shared::Plan& x) {
+            const uint32_t slot = number % kSegmentSlots;
+            if (!__all_sync(0xFFFFFFFFu, mbar_wait(bar(kSegment + slot), number / kSegmentSlots & 1u, failed))) return false;
+            x = sh.plan[slot];
+            ++number;
+            return true;
+        };
         if (warp < 8u) {
             asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
             const uint32_t q = warp >> 2, r = threadIdx.x & 127u, lanes = (warp & 3u) << 21;   // 32 TMEM lanes per warp, in bits 16 and up
-            const uint32_t t_s = tmem + lanes + kColS + 128u * q, t_o = tmem + lanes + kColO + 128u * q;
-            uint32_t s_phase = 0, o_phase = 0, q_phase = 0, step0 = 0;   // step0: steps in front of the segment
+            const uint32_t t_s = tmem + lanes + kColTile * q, t_p = t_s + kColP, t_o = t_s + kColO;
+            uint32_t s_phase = 0, p_phase = 0, q_phase = 0, step0 = 0;   // step0: steps in front of the segment
             bool ok = true;
-            // The query rows: asked for while the last products of the segment before are under way, kept in registers over its epilogue. A warp has the rows of its threads, two
-            // of them with a load: lane l brings 16 bytes (8 elements, number l mod 16) of row 2 x + l / 16
-            uint4 raw[16];
-            // Where the next segment is, is worked out while the first scores of this one are computed; the rows are asked for at its end
-            auto plan_next = [&]() {
-                Shared::Plan x;
-                x.pos = end - left;
-                x.seg = next_segment(p, deal, at, left);
-                x.length = length_of(p.c, x.seg.b), x.n = count_of(p.counts, x.seg.b, p.S, x.length);
-                if (lane == 0u) {
-                    x.number = sh.plan[warp].number + 1u;
-                    sh.plan[warp] = x;
+            // The query rows, fetched into L2 when the segment is published: they go to their place as they come, once the scores of the segment before are done with its rows, and become f16 there, a
+            // thread its row's, so that the next scores are computed while that segment's last product runs and its O is stored. c_row: what the thread's row was multiplied by, taken out
+            auto load_rows = [&](const Segment& seg, uint32_t n, float& c_row) {
+                if (!__all_sync(0xFFFFFFFFu, mbar_wait(bar(kQEmpty + q), q_phase ^ 1u, failed))) return false;
+                q_phase ^= 1u;
+                const uint32_t row = seg.row0 + q * kTileRows + r, i = row / p.group, chunk = lane & 15u;
+                const uint8_t* src = p.q.data + seg.b * p.q.stride_b + i * p.q.stride_s + (seg.head * p.group + row - i * p.group) * p.q.stride_h;
+                const unsigned long long mine = i < n ? reinterpret_cast<unsigned long long>(src) : 0ull;
+#pragma unroll 4
+                for (uint32_t x = 0; x < 16u; ++x) {   // two rows at a time, a lane 16 bytes
+                    const uint32_t from = 2u * x + (lane >> 4), to = (r & 96u) + from;
+                    const unsigned long long at_row = __shfl_sync(0xFFFFFFFFu, mine, from);
+                    cp_async_16(smem_u32(sh.q[q] + (chunk >> 3) * kQAtom + to * 128u + (((chunk & 7u) ^ (to & 7u)) << 4)),
+                                at_row != 0ull ? reinterpret_cast<const uint8_t*>(at_row) + 16u * chunk : p.q.data, at_row != 0ull ? 16u : 0u);
                 }
+                cp_async_wait_all();
                 __syncwarp();
-            };
-            auto ask_rows = [&](const Segment& seg, uint32_t n) {
-                const uint32_t row = seg.row0 + q * kTileRows + (r & 96u) + (lane >> 4);
-                uint32_t i = row / p.group, h = row - i * p.group;
-                const uint8_t* src = p.q.data + seg.b * p.q.stride_b + seg.head * p.group * p.q.stride_h + 16u * (lane & 15u);
-#pragma unroll
-                for (int x = 0; x < 16; ++x) {
-                    raw[x] = i < n ? ld_v4(src + i * p.q.stride_s + h * p.q.stride_h) : make_uint4(0u, 0u, 0u, 0u);
-                    for (h += 2u; h >= p.group; h -= p.group) ++i;
+                uint4* const place = reinterpret_cast<uint4*>(sh.q[q] + r * 128u);
+                uint32_t top = 0;   // sizes as bf16 bits
+#pragma unroll 8
+                for (uint32_t x = 0; x < 16u; ++x) {
+                    const uint4 v = place[(x >> 3) * (kQAtom / 16u) + ((x & 7u) ^ (r & 7u))];
+                    top = __vmaxu2(top, __vmaxu2(__vmaxu2(v.x & 0x7FFF7FFFu, v.y & 0x7FFF7FFFu), __vmaxu2(v.z & 0x7FFF7FFFu, v.w & 0x7FFF7FFFu)));
                 }
-            };
-            plan_next();
-            Shared::Plan now = sh.plan[warp];
-            ask_rows(now.seg, now.n);
-            uint8_t* mine = sh.q[q] + (r >> 5) * (kTileBytes / 4u);   // a quarter of the rows' place, where this warp turns its part of O round, between two segments
-            for (bool more = true; more;) {
-                const Segment seg = now.seg;
-                const uint32_t pos = now.pos, length = now.length, n = now.n;
-                // the tile's four warps are done with the place of the rows; also where a wait has run out in one of them: they leave together
-                ok = named_bar_all(2u + q, 128u, ok);
-                if (!ok) break;
-                if (threadIdx.x == 0u) begin_item(p, deal, seg, pos, all, n_work);
-                const uint32_t steps = tile_steps(p, seg, q, length, n), row = seg.row0 + q * kTileRows + r, i = row / p.group;
-                const bool exists = row < p.S * p.group;
-                const uint32_t limit = !exists || i >= n ? 0u : p.causal ? length - n + i + 1u : length;
-                float m = kLowest, l = 0.0f, c_row = 0.0f;
-                {
-                    uint32_t amax[8];   // sizes as bf16 bits, of rows 2 x and 2 x + 1 of pairs of loads in the halves
+                const float2 f = row_factors(max(top << 16, top & 0xFFFF0000u));
+                c_row = p.scale_log2 * f.y;
+#pragma unroll 4
+                for (uint32_t x = 0; x < 16u; ++x) {
+                    uint4* at_piece = place + (x >> 3) * (kQAtom / 16u) + ((x & 7u) ^ (r & 7u));
+                    const uint4 v = *at_piece;
+                    uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-                    for (int x = 0; x < 8; ++x) {
-                        auto largest = [](const uint4& v) {
-                            const uint32_t m = __vmaxu2(__vmaxu2(v.x & 0x7FFF7FFFu, v.y & 0x7FFF7FFFu), __vmaxu2(v.z & 0x7FFF7FFFu, v.w & 0x7FFF7FFFu));
-                            return max(m & 0xFFFFu, m >> 16);
-                        };
-                        amax[x] = largest(raw[2 * x]) | largest(raw[2 * x + 1]) << 16;
-                    }
-#pragma unroll
-                    for (int y = 1; y < 16; y <<= 1) {
-#pragma unroll
-                        for (int x = 0; x < 8; ++x) amax[x] = __vmaxu2(amax[x], __shfl_xor_sync(0xFFFFFFFFu, amax[x], y));
-                    }
-#pragma unroll
-                    for (uint32_t x = 0; x < 16u; ++x) {
-                        uint32_t w[4] = {raw[x].x, raw[x].y, raw[x].z, raw[x].w};
-                        const float2 f = row_factors(x & 1u ? amax[x / 2] & 0xFFFF0000u : amax[x / 2] << 16);
-                        const float back = __shfl_sync(0xFFFFFFFFu, f.y, (lane & 1u) << 4);   // of row 2 x + lane mod 2
-                        if (lane >> 1 == x) c_row = p.scale_log2 * back;
-#pragma unroll
-                        for (int y = 0; y < 4; ++y) w[y] = pack_f16x2(__uint_as_float(w[y] << 16) * f.x, __uint_as_float(w[y] & 0xFFFF0000u) * f.x);
-                        const uint32_t to = (r & 96u) + 2u * x + (lane >> 4), chunk = lane & 15u;
-                        *reinterpret_cast<uint4*>(sh.q[q] + (chunk >> 3) * kAtomBytes + to * 128u + (((chunk & 7u) ^ (to & 7u)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
-                    }
+                    for (int y = 0; y < 4; ++y) w[y] = pack_f16x2(__uint_as_float(w[y] << 16) * f.x, __uint_as_float(w[y] & 0xFFFF0000u) * f.x);
+                    *at_piece = make_uint4(w[0], w[1], w[2], w[3]);
                 }
                 fence_proxy_async_smem();
                 __syncwarp();
                 if (lane == 0u) mbar_arrive(bar(kQFull + q));
-                more = left > 0u;
-                if (more) plan_next();
+                return true;
+            };
+            float c_row = 0.0f;
+            Shared::Plan now;
+            ok = next_plan(now) && load_rows(now.seg, now.n, c_row);
+            for (bool more = true; more && ok;) {
+                const Segment seg = now.seg;
+                const uint32_t length = now.length, n = now.n, nan_slot = (number - 1u) % kSegmentSlots;
+                more = now.left > 0u;
+                const uint32_t steps = q != 0u ? now.steps[1] : now.steps[0], row = seg.row0 + q * kTileRows + r, i = row / p.group;
+                const bool exists = row < p.S * p.group;
+                const uint32_t limit = !exists || i >= n ? 0u : p.causal ? length - n + i + 1u : length;
+                float m = kLowest, l = 0.0f;
                 for (uint32_t j = 0; j < steps && ok; ++j) {
                     // (not the K tile's barrier: while a group is still storing the rows of the segment before, that one may already be two steps on)
-                    const uint32_t slot = (step0 + j) % kFactorSlots;
-                    ok = mbar_wait(bar(kEFull + slot), (step0 + j) / kFactorSlots & 1u, failed);
-                    const float2* scales = sh.scales[slot];
-                    ok = ok && mbar_wait(bar(kSFull + q), s_phase, failed);
+                    const uint32_t slot = (step0 + j) % kScaleSlots;
+                    ok = __all_sync(0xFFFFFFFFu, mbar_wait2(bar(kScales + slot), (step0 + j) / kScaleSlots & 1u, bar(kSFull + q), s_phase, failed));
                     if (!ok) break;
                     s_phase ^= 1u;
                     tc_fence_after_sync();
-                    uint32_t s[4][32];
+                    uint32_t s[kStep];
+                    tmem_ld32(t_s, *reinterpret_cast<uint32_t(*)[32]>(s));
+                    tmem_ld32(t_s + 32u, *reinterpret_cast<uint32_t(*)[32]>(s + 32));
+                    tmem_ld16(t_s + 64u, *reinterpret_cast<uint32_t(*)[16]>(s + 64));
+                    float c[kBlocks], shift[kBlocks], back[kBlocks];
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) tmem_ld32(t_s + 32u * k, s[k]);
+                    for (int k = 0; k < static_cast<int>(kBlocks); ++k) c[k] = fmaxf(c_row * sh.scales[slot][0][k], kLeast), shift[k] = sh.scales[slot][1][k], back[k] = sh.scales[slot][2][k];
                     tmem_wait_ld();
+                    reg_fence32(*reinterpret_cast<uint32_t(*)[32]>(s)), reg_fence32(*reinterpret_cast<uint32_t(*)[32]>(s + 32)), reg_fence16(*reinterpret_cast<uint32_t(*)[16]>(s + 64));
+                    tc_fence_before_sync();
+                    __syncwarp();
+                    if (lane == 0u) mbar_arrive(bar(kSFree + q));   // the next scores may overwrite these
+                    const int seen = static_cast<int>(limit) - static_cast<int>((seg.first + j) * kStep);
+                    if (__any_sync(0xFFFFFFFFu, seen < static_cast<int>(kStep))) {
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) reg_fence32(s[k]);
-                    const uint32_t tok0 = (seg.first + j) * kStepTokens;
-                    if (__any_sync(0xFFFFFFFFu, tok0 + kStepTokens > limit)) {
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) {
-#pragma unroll
-                            for (int x = 0; x < 32; ++x) {
-                                if (tok0 + 32u * k + x >= limit) s[k][x] = 0xFF800000u;
-                            }
+                        for (int y = 0; y < static_cast<int>(kStep); ++y) {
+                            if (y >= seen) s[y] = 0xFF800000u;
                         }
                     }
                     float most = -INFINITY;
 #pragma unroll
-                    for (int k = 0; k < 8; ++k) {   // a block of 16 tokens
-                        const uint32_t* x = s[k >> 1] + 16 * (k & 1);
-                        float top[2] = {__uint_as_float(x[0]), __uint_as_float(x[1])};
+                    for (int k = 0; k < static_cast<int>(kBlocks); ++k) {
+                        const uint32_t* y = s + 16 * k;
+                        float top = fmaxf(__uint_as_float(y[0]), __uint_as_float(y[1])), more = fmaxf(__uint_as_float(y[2]), __uint_as_float(y[3]));
 #pragma unroll
-                        for (int y = 2; y < 16; y += 2) top[0] = fmaxf(top[0], __uint_as_float(x[y])), top[1] = fmaxf(top[1], __uint_as_float(x[y + 1]));
-                        const float2 of = scales[k];
-                        most = fmaxf(most, fmaf(fmaxf(top[0], top[1]), fmaxf(c_row * of.x, kLeast), static_cast<float>(exponent_of(__float_as_uint(of.y)))));
+                        for (int z = 4; z < 16; z += 4) top = max3(top, __uint_as_float(y[z]), __uint_as_float(y[z + 1])), more = max3(more, __uint_as_float(y[z + 2]), __uint_as_float(y[z + 3]));
+                        most = fmaxf(most, fmaf(fmaxf(top, more), c[k], shift[k]));
                     }
                     most -= kUpF;
                     const bool over = most > m + kSlack;
+                    // once the product of the step before is over, O may be rescaled and P overwritten
+                    bool waited = j == 0u;
+                    const auto wait_product = [&]() {
+                        if (!waited) {
+                            ok = __all_sync(0xFFFFFFFFu, mbar_wait(bar(kPFree + q), p_phase, failed));
+                            p_phase ^= 1u;
+                            tc_fence_after_sync();
+                        }
+                        waited = true;
+                    };
                     if (__any_sync(0xFFFFFFFFu, over)) {
+                        wait_product();
                         const float next = over ? most : m, f = ex2(m - next);
                         m = next;
                         l *= f;
-                        if (j > 0u) {   // the product before this one is over: S came behind it
+                        if (j > 0u) {
 #pragma unroll 1
                             for (uint32_t k = 0; k < 8u; ++k) {
                                 uint32_t o[16];
@@ -263,209 +295,174 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
                         }
                     }
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) {
+                    for (int k = 0; k < static_cast<int>(kBlocks); ++k) {
+                        const float down = shift[k] - m;
+                        float l0 = 0.0f, l1 = 0.0f;
 #pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            const float2 of = scales[2 * k + h];
-                            const int e = exponent_of(__float_as_uint(of.y));
-                            const float c = fmaxf(c_row * of.x, kLeast), shift = static_cast<float>(e) - m;
-                            float l0 = 0.0f, l1 = 0.0f;
-#pragma unroll
-                            for (int x = 8 * h; x < 8 * h + 8; ++x) {
-                                uint32_t a = s[k][2 * x], b = s[k][2 * x + 1];
-                                fma2(a, b, c, shift);
-                                const float ea = ex2(__uint_as_float(a)), eb = ex2(__uint_as_float(b));
-                                add2(l0, l1, ea, eb);
-                                s[k][x] = pack_f16x2(ea, eb);   // (behind what it overwrites)
-                            }
-                            l = fmaf(l0 + l1, power_of(-e), l);
+                        for (int z = 0; z < 8; ++z) {
+                            uint32_t a = s[16 * k + 2 * z], b = s[16 * k + 2 * z + 1];
+                            fma2(a, b, c[k], down);
+                            const float ea = ex2(__uint_as_float(a)), eb = ex2(__uint_as_float(b));
+                            add2(l0, l1, ea, eb);
+                            s[16 * k + z] = pack_f16x2(ea, eb);   // (behind what it overwrites)
                         }
-                        tmem_st16_of32(t_s + 16u * k, s[k]);
-                        if (k & 1) {
-                            tmem_wait_st();
-                            tc_fence_before_sync();
-                            __syncwarp();
-                            if (lane == 0u) mbar_arrive(bar(kPFull + 2u * q + (k >> 1)));
-                        }
+                        l = fmaf(l0 + l1, back[k], l);
                     }
+                    wait_product();
+#pragma unroll
+                    for (int k = 0; k < static_cast<int>(kBlocks); ++k) tmem_st8(t_p + 8u * k, s + 16 * k);
+                    tmem_wait_st();
+                    tc_fence_before_sync();
+                    __syncwarp();
+                    if (lane == 0u) mbar_arrive(bar(kPFull + q));
                 }
                 step0 += seg.steps;
-                const Segment done = seg;
-                if (more) {
-                    now = sh.plan[warp];
-                    ask_rows(now.seg, now.n);
-                } else {   // (assigned either way: nothing of the old rows stays in registers for it)
-#pragma unroll
-                    for (int x = 0; x < 16; ++x) raw[x] = make_uint4(0u, 0u, 0u, 0u);
-                }
-                ok = ok && mbar_wait(bar(kQEmpty + q), q_phase, failed);   // S is done with the rows
-                q_phase ^= 1u;
+                if (!ok) break;
+                if (more) ok = next_plan(now) && load_rows(now.seg, now.n, c_row);   // (the next segment's scores start while this one's O is stored)
                 if (steps > 0u) {
-                    ok = ok && mbar_wait(bar(kODone + q), o_phase, failed);
-                    o_phase ^= 1u;
+                    ok = ok && __all_sync(0xFFFFFFFFu, mbar_wait(bar(kPFree + q), p_phase, failed));
+                    p_phase ^= 1u;
                     tc_fence_after_sync();
                 }
-                if (!ok) continue;
-                const bool whole = done.steps == done.of, none = l == 0.0f;   // NaN is something
-                const uint32_t h = done.head * p.group + row % p.group;
-                float factor = whole ? (none ? 0.0f : 1.0f / l) : 1.0f;
+                if (!ok) break;
+                const bool whole = seg.steps == seg.of, none = l == 0.0f;   // NaN is something
+                const uint32_t h = seg.head * p.group + row % p.group;
+                float factor = none ? 0.0f : whole ? 1.0f / l : 1.0f;
                 // NaN of V went into the product as 0, where it would meet the weights of 0 of rows that do not see it. A row sees the tokens in front of its limit.
-                if (steps > 0u) {
-                    const uint32_t number = sh.plan[warp].number - (more ? 1u : 0u);   // (the plan is already the next segment's)
-#pragma unroll
-                    for (uint32_t w = 0; w < 4u; ++w) {
-                        if (sh.nan_from[number % kNanSlots][w] < limit) factor = __uint_as_float(0x7FC00000u);
-                    }
-                }
-                const uint32_t at_row = exists ? (done.b * p.S + i) * p.H + h : 0xFFFFFFFFu;   // of out, in rows
-                float* slot = slot_of(p.ws, gridDim.x, blockIdx.x, done.first == 0u ? 1u : 0u, kItemRows);
-                // O by 64 columns: a thread writes its row's to shared memory, and the warp stores whole pieces of rows
+                if (steps > 0u && sh.nan_from[nan_slot] < limit) factor = __uint_as_float(0x7FC00000u);
+                __nv_bfloat16* out = p.out + ((static_cast<size_t>(seg.b) * p.S + i) * p.H + h) * 128u;
+                float* slot = slot_of(p.ws, gridDim.x, blockIdx.x, seg.first == 0u ? 1u : 0u, kItemRows);
+                float* part = slot + (q * kTileRows + r) * 128u;
 #pragma unroll 1
-                for (uint32_t c = 0; c < 2u; ++c) {
-#pragma unroll
-                    for (uint32_t k = 0; k < 2u; ++k) {
-                        uint32_t o[32];
-                        if (steps > 0u) {
-                            tmem_ld32(t_o + 64u * c + 32u * k, o);
-                            tmem_wait_ld();
-                            reg_fence32(o);
-                        } else {
-#pragma unroll
-                            for (int x = 0; x < 32; ++x) o[x] = 0u;
-                        }
-#pragma unroll
-                        for (uint32_t x = 0; x < 8u; ++x) {
-                            float4 v = make_float4(__uint_as_float(o[4 * x]) * factor, __uint_as_float(o[4 * x + 1]) * factor, __uint_as_float(o[4 * x + 2]) * factor, __uint_as_float(o[4 * x + 3]) * factor);
-                            if (none) v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                            *reinterpret_cast<float4*>(mine + lane * 256u + (((8u * k + x) ^ (lane & 15u)) << 4)) = v;
+                for (uint32_t c = 0; c < 4u; ++c) {   // 32 columns at a time, a thread its row's
+                    uint32_t o[32];
+                    if (steps > 0u) {
+                        tmem_ld32(t_o + 32u * c, o);
+                        tmem_wait_ld();
+                        reg_fence32(o);
+                        if (c == 3u) {
+                            tc_fence_before_sync();
+                            __syncwarp();
+                            if (lane == 0u) mbar_arrive(bar(kOFree + q));
                         }
                     }
-                    if (c == 1u && steps > 0u) {
-                        tc_fence_before_sync();
-                        __syncwarp();
-                        if (lane == 0u) mbar_arrive(bar(kOFree + q));
-                    }
-                    __syncwarp();
+#pragma unroll
+                    for (int x = 0; x < 32; ++x) o[x] = steps == 0u || none ? 0u : __float_as_uint(__uint_as_float(o[x]) * factor);
                     if (whole) {
-#pragma unroll 4
-                        for (uint32_t x = 0; x < 8u; ++x) {   // four rows of 64 bf16 at a time
-                            const uint32_t from = 4u * x + (lane >> 3), piece = lane & 7u, to = __shfl_sync(0xFFFFFFFFu, at_row, from);
-                            const float4 u = *reinterpret_cast<const float4*>(mine + from * 256u + (((2u * piece) ^ (from & 15u)) << 4)), v = *reinterpret_cast<const float4*>(mine + from * 256u + (((2u * piece + 1u) ^ (from & 15u)) << 4));
-                            if (to != 0xFFFFFFFFu)
-                                *reinterpret_cast<uint4*>(p.out + static_cast<size_t>(to) * 128u + 64u * c + 8u * piece) = make_uint4(pack_bf16x2(u.x, u.y), pack_bf16x2(u.z, u.w), pack_bf16x2(v.x, v.y), pack_bf16x2(v.z, v.w));
+                        if (exists) {
+#pragma unroll
+                            for (int x = 0; x < 4; ++x) {
+                                uint32_t w[4];
+#pragma unroll
+                                for (int y = 0; y < 4; ++y) w[y] = pack_bf16x2(__uint_as_float(o[8 * x + 2 * y]), __uint_as_float(o[8 * x + 2 * y + 1]));
+                                *reinterpret_cast<uint4*>(out + 32u * c + 8 * x) = make_uint4(w[0], w[1], w[2], w[3]);
+                            }
                         }
-                    } else {
-#pragma unroll 4
-                        for (uint32_t x = 0; x < 16u; ++x) {   // two rows of 64 f32 at a time
-                            const uint32_t from = 2u * x + (lane >> 4), piece = lane & 15u;
-                            *reinterpret_cast<float4*>(slot + (q * kTileRows + (r & 96u) + from) * 128u + 64u * c + 4u * piece) = *reinterpret_cast<const float4*>(mine + from * 256u + ((piece ^ (from & 15u)) << 4));
-                        }
+                    } else if (limit != 0u) {
+#pragma unroll
+                        for (int x = 0; x < 8; ++x) *reinterpret_cast<uint4*>(part + 32u * c + 4 * x) = make_uint4(o[4 * x], o[4 * x + 1], o[4 * x + 2], o[4 * x + 3]);
                     }
-                    __syncwarp();
                 }
                 if (whole) {
-                    if (exists && p.lse != nullptr) p.lse[(static_cast<size_t>(done.b) * p.H + h) * p.S + i] = none ? -INFINITY : (m + lg2(l)) * kLn2;
+                    if (exists && p.lse != nullptr) p.lse[(static_cast<size_t>(seg.b) * p.H + h) * p.S + i] = none ? -INFINITY : (m + lg2(l)) * kLn2;
                 } else if (limit != 0u) {
                     *reinterpret_cast<float2*>(slot + kItemRows * 128u + 2u * (q * kTileRows + r)) = make_float2(m, l);
                 }
             }
-        } else if (warp < 12u) {
+        } else if (warp < kIssueWarp) {
             asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kConvertRegs));
-            // Thread r brings row r of K, and of V one half (64 elements) of the pair of tokens that r is one of: V's codes lie in pairs
-            const uint32_t r = threadIdx.x & 127u, half = r & 1u;
+            // Block by block, 16 bytes of K and of V a thread: 16 elements of one token, 8 elements of both tokens of a pair
+            const uint32_t t = threadIdx.x & 127u, k_row = t >> 3, k_piece = (t & 7u) ^ k_swap(k_row), v_row = 2u * (t >> 4), v_piece = (t & 15u) ^ v_swap(t >> 4);
+            // (of a row's eight lanes the upper four store their second half first, so that the eight meet different banks)
+            const uint32_t up = k_piece >> 2;
+            uint4 *const k_first = piece_at(sh.k[0], k_row, 2u * k_piece + up), *const k_second = piece_at(sh.k[0], k_row, 2u * k_piece + (up ^ 1u));
+            uint4 *const v_first = piece_at(sh.v[0], v_row, v_piece), *const v_second = piece_at(sh.v[0], v_row + 1u, v_piece);
+            constexpr uint32_t kBlockOfTile = kBlockTokens * 128u / 16u;   // from a block's place in a tile to the next one's, in pieces
             uint32_t step = 0;   // so far
+            Shared::Plan now;
+            now.left = 1u;
             bool ok = true;
-            while (left > 0u && ok) {
-                const Segment seg = next_segment(p, deal, at, left);
-                if (lane == 0u) sh.nan_from[++sh.converting[warp & 3u] % kNanSlots][warp & 3u] = 0xFFFFFFFFu;
-                __syncwarp();
-                uint32_t* nan_from = &sh.nan_from[sh.converting[warp & 3u] % kNanSlots][warp & 3u];
-                const uint32_t length = length_of(p.c, seg.b);
-                // the block of this thread's token in step j: its page, looked up a step ahead of its bytes. (The second token of a pair may lie behind the length)
-                long long page_ahead = -1;
-                auto token = [&](uint32_t j) { return (seg.first + j) * kStepTokens + r; };
-                auto look_up = [&](uint32_t j) {
-                    const uint32_t t = token(j) & ~1u;
-                    if (j < seg.steps && t < length) page_ahead = page_of(p.c, seg.b, t);
-                };
-                uint4 k[8], v[8], meta = make_uint4(0x3F800000u, 0x3F800000u, 0u, 0u);
-                bool lost = false, dead = true;   // dead: no token of the pair is below the length
-                auto fetch = [&](uint32_t j, bool values) {
-                    const uint32_t t = token(j);
-                    if (!values) {
-                        dead = j >= seg.steps || (t & ~1u) >= length, lost = !dead && page_ahead < 0;
-                        meta = make_uint4(0x3F800000u, 0x3F800000u, 0u, 0u);
-                    }
-                    if (dead || lost) return;
-                    const uint8_t* block = block_of(p.c, page_ahead, seg.head, t);
-                    const uint32_t in = t % kBlockTokens, pair = in >> 1;
-                    if (values) {
-#pragma unroll
-                        for (uint32_t x = 0; x < 8u; ++x) v[x] = ld_v4(block + kVCodes + 256u * pair + 16u * ((8u * half + (x ^ half)) ^ v_swap(pair)));
-                    } else {
-#pragma unroll
-                        for (uint32_t x = 0; x < 8u; ++x) k[x] = ld_v4(block + 128u * in + 16u * (x ^ k_swap(in)));
-                        meta = ld_v4(block + kMeta);
-                    }
-                };
-#pragma unroll
-                for (int x = 0; x < 8; ++x) k[x] = v[x] = make_uint4(0u, 0u, 0u, 0u);
-                look_up(0u);
-                fetch(0u, false);
-                fetch(0u, true);
-                look_up(1u);
+            while (now.left > 0u && ok) {
+                if (!next_plan(now)) break;
+                const Segment seg = now.seg;
+                const uint32_t length = now.length;
                 for (uint32_t j = 0; j < seg.steps; ++j, ++step) {
-                    const uint32_t st = step % kStages, parity = (step / kStages + 1u) & 1u, slot = step % kFactorSlots, t = token(j);
-                    if ((r & (kBlockTokens - 1u)) == 0u) sh.scales[slot][r / kBlockTokens] = make_float2(__uint_as_float(meta.x), __uint_as_float(meta.y));
-                    const bool empty = dead || t >= length, no_key = !empty && (lost || (meta.z >> (t % kBlockTokens) & 1u) != 0u);
-                    const bool no_value = !empty && !lost && (meta.z >> (16u + t % kBlockTokens) & 1u) != 0u;
-                    const uint32_t bad = __ballot_sync(0xFFFFFFFFu, no_value);
-                    if (bad != 0u && lane == 0u && *nan_from == 0xFFFFFFFFu) *nan_from = t + static_cast<uint32_t>(__ffs(static_cast<int>(bad))) - 1u;
-                    __syncwarp();
-                    if (lane == 0u) mbar_arrive(bar(kEFull + slot));
-                    // codes of tokens behind the length may be anything
-                    const bool pair_dead = dead || lost;
-                    const uint32_t keep = pair_dead ? 0u : (t | 1u) < length ? 0xFFFFFFFFu : 0x00FF00FFu;
-                    ok = __all_sync(0xFFFFFFFFu, mbar_wait(bar(kKEmpty + st), parity, failed));
+                    const uint32_t st = step % kStages, raw = step % kRawStages, slot = step % kScaleSlots, parity = (step / kStages + 1u) & 1u, to = st * (kStepBytes / 16u);
+                    ok = __all_sync(0xFFFFFFFFu, mbar_wait2(bar(kScales + slot), step / kScaleSlots & 1u, bar(kKEmpty + st), parity, failed));
                     if (!ok) break;
+                    const uint8_t *k_codes = sh.raw_k[raw][0] + 16u * t, *v_codes = sh.raw_v[raw][0] + 16u * t;
+                    const bool plain = sh.plain[slot] != 0u;
+                    // tokens of a block below the length, and whether they have numbers in K and V: codes of others may be anything
+                    const auto live = [&](uint32_t x) {
+                        const uint32_t t0 = (seg.first + j) * kStep + x * kBlockTokens;
+                        return t0 >= length ? 0u : 0xFFFFu >> (16u - min(length - t0, 16u));
+                    };
+                    uint4 codes[kBlocks];
+                    if (plain) {
 #pragma unroll
-                    for (uint32_t x = 0; x < 8u; ++x) {
-                        uint4 lo = to_f16(k[x].x, k[x].y), hi = to_f16(k[x].z, k[x].w);
-                        if (empty || no_key) lo = hi = empty ? make_uint4(0u, 0u, 0u, 0u) : make_uint4(0x7E007E00u, 0x7E007E00u, 0x7E007E00u, 0x7E007E00u);
-                        *piece_at(sh.k[st], r, 2u * x) = lo;
-                        *piece_at(sh.k[st], r, 2u * x + 1u) = hi;
+                        for (uint32_t x = 0; x < kBlocks; ++x) codes[x] = *reinterpret_cast<const uint4*>(k_codes + x * kVCodes);
+#pragma unroll
+                        for (uint32_t x = 0; x < kBlocks; ++x) {
+                            const uint4 w = codes[x];
+                            const uint32_t a = up ? w.z : w.x, b = up ? w.w : w.y, c = up ? w.x : w.z, d = up ? w.y : w.w;
+                            k_first[to + x * kBlockOfTile] = to_f16(a, b);
+                            k_second[to + x * kBlockOfTile] = to_f16(c, d);
+                        }
+                    } else {
+#pragma unroll 1
+                        for (uint32_t x = 0; x < kBlocks; ++x) {
+                            const uint4 w = *reinterpret_cast<const uint4*>(k_codes + x * kVCodes);
+                            const uint32_t here = live(x), masks = here != 0u ? sh.meta[raw][x].z : 0u;
+                            uint4 first = up ? to_f16(w.z, w.w) : to_f16(w.x, w.y), second = up ? to_f16(w.x, w.y) : to_f16(w.z, w.w);
+                            if (!(here >> k_row & 1u)) first = second = make_uint4(0u, 0u, 0u, 0u);
+                            else if (masks >> k_row & 1u) first = second = make_uint4(0x7E007E00u, 0x7E007E00u, 0x7E007E00u, 0x7E007E00u);
+                            k_first[to + x * kBlockOfTile] = first;
+                            k_second[to + x * kBlockOfTile] = second;
+                        }
                     }
                     fence_proxy_async_smem();
                     mbar_arrive(bar(kKFull + st));
-                    fetch(j + 1u, false);
                     ok = __all_sync(0xFFFFFFFFu, mbar_wait(bar(kVEmpty + st), parity, failed));
                     if (!ok) break;
+                    if (plain) {
 #pragma unroll
-                    for (uint32_t x = 0; x < 8u; ++x) {   // (the two threads of a pair at neighbouring pieces, so that they meet different banks)
-                        const uint32_t w[4] = {v[x].x & keep, v[x].y & keep, v[x].z & keep, v[x].w & keep}, piece = 8u * half + (x ^ half);
-                        *piece_at(sh.v[st], r & ~1u, piece) = to_f16(__byte_perm(w[0], w[1], 0x6420), __byte_perm(w[2], w[3], 0x6420));
-                        *piece_at(sh.v[st], r | 1u, piece) = to_f16(__byte_perm(w[0], w[1], 0x7531), __byte_perm(w[2], w[3], 0x7531));
+                        for (uint32_t x = 0; x < kBlocks; ++x) codes[x] = *reinterpret_cast<const uint4*>(v_codes + x * kVCodes);
+#pragma unroll
+                        for (uint32_t x = 0; x < kBlocks; ++x) {
+                            const uint4 w = codes[x];
+                            v_first[to + x * kBlockOfTile] = to_f16(__byte_perm(w.x, w.y, 0x6420), __byte_perm(w.z, w.w, 0x6420));
+                            v_second[to + x * kBlockOfTile] = to_f16(__byte_perm(w.x, w.y, 0x7531), __byte_perm(w.z, w.w, 0x7531));
+                        }
+                    } else {
+#pragma unroll 1
+                        for (uint32_t x = 0; x < kBlocks; ++x) {
+                            uint4 w = *reinterpret_cast<const uint4*>(v_codes + x * kVCodes);
+                            const uint32_t here = live(x), good = here != 0u ? here & ~(sh.meta[raw][x].z >> 16) : 0u;
+                            const uint32_t keep = (good >> v_row & 1u ? 0x00FF00FFu : 0u) | (good >> (v_row + 1u) & 1u ? 0xFF00FF00u : 0u);
+                            w.x &= keep, w.y &= keep, w.z &= keep, w.w &= keep;
+                            v_first[to + x * kBlockOfTile] = to_f16(__byte_perm(w.x, w.y, 0x6420), __byte_perm(w.z, w.w, 0x6420));
+                            v_second[to + x * kBlockOfTile] = to_f16(__byte_perm(w.x, w.y, 0x7531), __byte_perm(w.z, w.w, 0x7531));
+                        }
                     }
                     fence_proxy_async_smem();
                     mbar_arrive(bar(kVFull + st));
-                    fetch(j + 1u, true);
-                    look_up(j + 2u);
+                    __syncwarp();
+                    if (lane == 0u) mbar_arrive(bar(kRawEmpty + raw));
                 }
             }
         } else {
             asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kIssueRegs));
-            if (warp < 14u) {
+            if (warp < kCopyWarp) {
                 // All of this runs on values that are the same in the warp's 32 lanes. The compiler has to see that (they come out of votes and reductions, which have uniform
-                // results): the products' operands then stay in uniform registers and take few instructions to issue. A warp per tile: the two take turns with the tensor cores,
-                // and neither's waits hold the other's products up.
+                // results): the products' operands then stay in uniform registers and take few instructions to issue. A warp per tile: neither's waits hold the other's products up.
                 auto uniform = [](uint32_t x) { return __reduce_max_sync(0xFFFFFFFFu, x); };
-                const uint32_t q = uniform(warp - 12u), t_s = uniform(tmem) + kColS + 128u * q, t_o = uniform(tmem) + kColO + 128u * q;
-                constexpr uint32_t id_s = idesc_16bit(false, 128, 128, 0, 0), id_o = idesc_16bit(false, 128, 128, 0, 1);
+                const uint32_t q = uniform(warp - kIssueWarp), t_s = uniform(tmem) + kColTile * q, t_p = t_s + kColP, t_o = t_s + kColO;
+                constexpr uint32_t id_s = idesc_16bit(false, 128, kStep, 0, 0), id_o = idesc_16bit(false, 128, 128, 0, 1);
                 const uint64_t d_k = make_smem_desc(smem_u32(sh.q[0]), 16, 1024, kSwizzle128B), d_v = make_smem_desc(smem_u32(sh.v[0]), kAtomBytes, 1024, kSwizzle128B);
                 const uint32_t k_hi = static_cast<uint32_t>(d_k >> 32), v_hi = static_cast<uint32_t>(d_v >> 32);
                 const uint32_t q_lo = uniform(static_cast<uint32_t>(d_k)) + (q * kTileBytes >> 4), k_lo = uniform(static_cast<uint32_t>(d_k)) + (2u * kTileBytes >> 4), v_lo = uniform(static_cast<uint32_t>(d_v));
                 static_assert(offsetof(Shared, k) == 2u * kTileBytes, "K behind Q");
-                uint32_t step = 0, q_phase = 0, turn = q ^ 1u, p_phase = 0, o_phase = 1;   // (tile 0 goes first)
+                uint32_t step = 0, q_phase = 0, p_phase = 0, o_phase = 1, s_phase = 1;
                 bool ok = true;
                 auto wait = [&](uint32_t b, uint32_t parity) {
                     ok = ok && __all_sync(0xFFFFFFFFu, mbar_wait(b, parity, failed));
@@ -474,68 +471,147 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
                 auto commit = [&](uint32_t b) {
                     if (elect_one_sync()) tc_commit(b);
                 };
-                auto scores = [&](uint32_t st) {
-                    if (elect_one_sync()) {
-                        const uint32_t b = k_lo + (st * kTileBytes >> 4);
+                // the scores of a step that this tile takes part in, or not; the step's K is done with then
+                auto scores = [&](uint32_t at_step, bool taken, bool last) {
+                    const uint32_t st = at_step % kStages;
+                    if (!wait(bar(kKFull + st), at_step / kStages & 1u)) return;
+                    if (taken) {
+                        if (!wait(bar(kSFree + q), s_phase)) return;
+                        s_phase ^= 1u;
+                        tc_fence_after_sync();
+                        if (elect_one_sync()) {
+                            const uint32_t b = k_lo + (st * kStepBytes >> 4);
 #pragma unroll
-                        for (uint32_t x = 0; x < 8u; ++x) {
-                            const uint32_t off = ((x >> 2) * kAtomBytes + (x & 3u) * 32u) >> 4;
-                            mma_f16_ss(t_s, q_lo + off, k_hi, b + off, k_hi, id_s, x > 0u ? 1u : 0u);
+                            for (uint32_t x = 0; x < 8u; ++x) mma_f16_ss(t_s, q_lo + (((x >> 2) * kQAtom + (x & 3u) * 32u) >> 4), k_hi, b + (((x >> 2) * kAtomBytes + (x & 3u) * 32u) >> 4), k_hi, id_s, x > 0u ? 1u : 0u);
+                            tc_commit(bar(kSFull + q));
                         }
-                        tc_commit(bar(kSFull + q));
                     }
+                    commit(bar(kKEmpty + st));
+                    if (last) commit(bar(kQEmpty + q));
                 };
-                while (uniform(left) > 0u && ok) {
-                    const Segment seg = next_segment(p, deal, at, left);
-                    const uint32_t length = length_of(p.c, seg.b), n = count_of(p.counts, seg.b, p.S, length);
-                    const uint32_t steps = uniform(tile_steps(p, seg, q, length, n)), seg_steps = uniform(seg.steps);
+                Shared::Plan now;
+                now.left = 1u;
+                while (uniform(now.left) > 0u && ok) {
+                    if (!next_plan(now)) break;
+                    const uint32_t steps = uniform(q != 0u ? now.steps[1] : now.steps[0]), seg_steps = uniform(now.seg.steps);
                     if (!wait(bar(kQFull + q), q_phase)) break;
                     q_phase ^= 1u;
-                    if (!wait(bar(kKFull + step % kStages), step / kStages & 1u)) break;
-                    tc_fence_after_sync();
-                    if (steps > 0u) {
-                        scores(step % kStages);   // overwrites P of the step before, behind its products
-                        if (!wait(bar(kOFree + q), o_phase)) break;
-                        o_phase ^= 1u;
-                    }
-                    commit(bar(kKEmpty + step % kStages));
-                    if (seg_steps == 1u) commit(bar(kQEmpty + q));
-                    for (uint32_t j = 0; j < seg_steps; ++j, ++step) {
-                        const uint32_t st = step % kStages, next = (step + 1u) % kStages;
-                        const bool more = j + 1u < seg_steps;
-                        if (!wait(bar(kVFull + st), step / kStages & 1u)) break;
-                        // The tiles take turns, so that one's products run under the other's softmax: without, both do the same at the same time
-                        if (!wait(bar(kTurn + q), turn)) break;
-                        turn ^= 1u;
+                    scores(step, steps > 0u, seg_steps == 1u);
+                    for (uint32_t j = 0; j < seg_steps && ok; ++j, ++step) {
+                        const uint32_t st = step % kStages;
+                        if (j + 1u < seg_steps) scores(step + 1u, j + 1u < steps, j + 2u == seg_steps);
+                        if (!ok || !wait(bar(kVFull + st), step / kStages & 1u)) break;
                         if (j < steps) {
-#pragma unroll
-                            for (uint32_t h = 0; h < 2u; ++h) {
-                                if (!wait(bar(kPFull + 2u * q + h), p_phase)) break;
-                                tc_fence_after_sync();
-                                if (elect_one_sync()) {
-                                    const uint32_t b = v_lo + ((st * kTileBytes + h * kHalf * 128u) >> 4);
-#pragma unroll
-                                    for (uint32_t x = 0; x < 4u; ++x) mma_f16_ts(t_o, t_s + 32u * h + 8u * x, b + (x * 2048u >> 4), v_hi, id_o, (j > 0u || h + x > 0u) ? 1u : 0u);
-                                    if (h == 1u && j + 1u == steps) tc_commit(bar(kODone + q));
-                                }
+                            if (j == 0u) {   // O of the segment before has been taken
+                                if (!wait(bar(kOFree + q), o_phase)) break;
+                                o_phase ^= 1u;
                             }
+                            if (!wait(bar(kPFull + q), p_phase)) break;
                             p_phase ^= 1u;
-                        }
-                        if (!ok) break;
-                        commit(bar(kVEmpty + st));
-                        if (more) {
-                            if (!wait(bar(kKFull + next), (step + 1u) / kStages & 1u)) break;
                             tc_fence_after_sync();
-                            if (j + 1u < steps) scores(next);
-                            commit(bar(kKEmpty + next));
+                            if (elect_one_sync()) {
+                                const uint32_t b = v_lo + (st * kStepBytes >> 4);
+#pragma unroll
+                                for (uint32_t x = 0; x < kBlocks; ++x) mma_f16_ts(t_o, t_p + 8u * x, b + (x * 2048u >> 4), v_hi, id_o, (j > 0u || x > 0u) ? 1u : 0u);
+                                tc_commit(bar(kPFree + q));
+                            }
                         }
-                        if (lane == 0u) mbar_arrive(bar(kTurn + (q ^ 1u)));
-                        if (j + 2u == seg_steps) commit(bar(kQEmpty + q));
+                        commit(bar(kVEmpty + st));
                     }
                 }
                 if (!ok) {   // whatever was issued has to be over before the tensor memory goes back
                     commit(bar(kDrained + q));
                     (void)mbar_wait(bar(kDrained + q), 0u, &sh.not_drained);
+                }
+                __syncwarp();
+            } else if (warp == kCopyWarp) {
+                // The segments, for all roles, and the copies of a step: lane x brings block x
+                uint32_t step = 0, left = end - begin;
+                Place at = find_step(p, deal, begin);
+                bool ok = true;
+                while (left > 0u && ok) {
+                    const uint32_t pos = end - left;
+                    const Segment seg = next_segment(p, deal, at, left);
+                    const uint32_t length = length_of(p.c, seg.b), n = count_of(p.counts, seg.b, p.S, length);
+                    if (lane == 0u) {
+                        Shared::Plan& x = sh.plan[number % kSegmentSlots];
+                        x.seg = seg, x.length = length, x.n = n, x.left = left;
+                        for (uint32_t q = 0; q < 2u; ++q) x.steps[q] = tile_steps(p, seg, q, length, n);
+                        mbar_arrive(bar(kSegment + number % kSegmentSlots));
+                        begin_item(p, deal, seg, pos, all, n_work);
+                    }
+                    ++number;
+                    for (uint32_t r = lane; r < kItemRows; r += 32u) {
+                        const uint32_t row = seg.row0 + r, i = row / p.group, h = seg.head * p.group + row - i * p.group;
+                        const uint8_t* src = p.q.data + seg.b * p.q.stride_b + i * p.q.stride_s + h * p.q.stride_h;
+                        if (i < n) asm volatile("prefetch.global.L2 [%0];\n\tprefetch.global.L2 [%0 + 128];" ::"l"(src));
+                    }
+                    long long page = -1;   // of the lane's block in the next step
+                    auto look_up = [&](uint32_t j) {
+                        const uint32_t t = (seg.first + j) * kStep + lane * kBlockTokens;
+                        if (lane < kBlocks && j < seg.steps && t < length) page = page_of(p.c, seg.b, t);
+                    };
+                    look_up(0u);
+                    for (uint32_t j = 0; j < seg.steps; ++j, ++step) {
+                        const uint32_t t = (seg.first + j) * kStep + lane * kBlockTokens, raw = step % kRawStages;
+                        const bool live = lane < kBlocks && t < length, here = live && page >= 0;
+                        const uint8_t* block = here ? block_of(p.c, page, seg.head, t) : nullptr;
+                        const uint32_t blocks = static_cast<uint32_t>(__popc(__ballot_sync(0xFFFFFFFFu, here)));
+                        ok = __all_sync(0xFFFFFFFFu, mbar_wait(bar(kRawEmpty + raw), (step / kRawStages + 1u) & 1u, failed));
+                        if (!ok) break;
+                        if (live && !here) sh.meta[raw][lane] = make_uint4(0x3F800000u, 0x3F800000u, 0xFFFFFFFFu, 0u);   // a page that the pool does not have: no numbers
+                        __syncwarp();
+                        if (lane == 0u) mbar_arrive_expect_tx(bar(kRawFull + raw), blocks * (kMeta + 16u));
+                        __syncwarp();
+                        if (here) {
+                            bulk_load(smem_u32(&sh.meta[raw][lane]), block + kMeta, 16u, bar(kRawFull + raw));
+                            bulk_load(smem_u32(sh.raw_k[raw][lane]), block, kVCodes, bar(kRawFull + raw));
+                            bulk_load(smem_u32(sh.raw_v[raw][lane]), block + kVCodes, kMeta - kVCodes, bar(kRawFull + raw));
+                        }
+                        look_up(j + 1u);
+                    }
+                }
+                // after a failure: copies that are under way land before the CTA's shared memory is another's. (step: the one whose copies were not asked for)
+                if (!ok) {
+                    for (uint32_t i = 1; i <= kRawStages && i <= step; ++i) (void)mbar_wait(bar(kRawFull + (step - i) % kRawStages), (step - i) / kRawStages & 1u, &sh.not_drained, 20000000LL);
+                }
+                __syncwarp();
+            } else {
+                // The scales of a step, a lane a block: as the softmax wants them, and whether the step's tokens are all there and have numbers
+                uint32_t step = 0;
+                Shared::Plan now;
+                now.left = 1u;
+                bool ok = true;
+                while (now.left > 0u && ok) {
+                    if (!next_plan(now)) break;
+                    const Segment seg = now.seg;
+                    uint32_t* nan_from = &sh.nan_from[(number - 1u) % kSegmentSlots];
+                    if (lane == 0u) *nan_from = 0xFFFFFFFFu;
+                    const uint32_t length = now.length;
+                    for (uint32_t j = 0; j < seg.steps; ++j, ++step) {
+                        const uint32_t raw = step % kRawStages, slot = step % kScaleSlots, t0 = (seg.first + j) * kStep + lane * kBlockTokens;
+                        const uint32_t live = lane >= kBlocks || t0 >= length ? 0u : 0xFFFFu >> (16u - min(length - t0, 16u));   // (behind the length there are no scales or masks)
+                        ok = __all_sync(0xFFFFFFFFu, mbar_wait(bar(kRawFull + raw), step / kRawStages & 1u, failed));
+                        if (!ok) break;
+                        const uint4 meta = live != 0u ? sh.meta[raw][lane] : make_uint4(0x3F800000u, 0x3F800000u, 0u, 0u);
+                        const bool plain = !__any_sync(0xFFFFFFFFu, lane < kBlocks && (live != 0xFFFFu || meta.z != 0u));
+                        if (lane < kBlocks) {
+                            float* of = sh.scales[slot][0] + lane;
+                            const int e = exponent_of(meta.y);
+                            of[0] = __uint_as_float(meta.x), of[8] = static_cast<float>(e), of[16] = power_of(-e);
+                        }
+                        uint32_t first = 0xFFFFFFFFu;
+                        if (!plain) {
+                            const uint32_t no_value = meta.z >> 16 & live;
+                            first = __reduce_min_sync(0xFFFFFFFFu, no_value != 0u ? t0 + static_cast<uint32_t>(__ffs(static_cast<int>(no_value))) - 1u : 0xFFFFFFFFu);
+                        }
+                        __syncwarp();
+                        if (lane == 0u) {
+                            sh.plain[slot] = plain;
+                            if (first < *nan_from) *nan_from = first;
+                            mbar_arrive(bar(kScales + slot));
+                        }
+                    }
                 }
                 __syncwarp();
             }
@@ -544,7 +620,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
     tc_fence_before_sync();
     __syncthreads();
     if (threadIdx.x == 0u && sh.failed != 0u) atomicOr(p.status, 1u);
-    if (warp == 12u) {
+    if (warp == kIssueWarp) {
         tc_fence_after_sync();
         tmem_dealloc(tmem, 512u);
     }

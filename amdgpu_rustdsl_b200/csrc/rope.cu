@@ -46,33 +46,60 @@ __device__ __forceinline__ float2 turn(unsigned long long phase) {
     return quarter & 2ull ? make_float2(-c, -s) : make_float2(c, s);
 }
 
-template <typename T> __device__ __forceinline__ float to_f32(T x);
-template <> __device__ __forceinline__ float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
-template <> __device__ __forceinline__ float to_f32(__half x) { return __half2float(x); }
-template <> __device__ __forceinline__ float to_f32(float x) { return x; }
-template <typename T> __device__ __forceinline__ T of_f32(float x);
-template <> __device__ __forceinline__ __nv_bfloat16 of_f32(float x) { return __float2bfloat16_rn(x); }
-template <> __device__ __forceinline__ __half of_f32(float x) { return __float2half_rn(x); }
-template <> __device__ __forceinline__ float of_f32(float x) { return x; }
-
+// N elements of T in words. (Arrays of 16-bit elements would be kept in local memory.)
 template <typename T, int N>
-struct alignas(sizeof(T) * N) Piece {
-    T at[N];
+struct Piece {
+    static constexpr int kBytes = sizeof(T) * N, kWords = kBytes >= 4 ? kBytes / 4 : 1;
+    uint32_t w[kWords];
+    __device__ __forceinline__ void load(const uint8_t* p) {   // (volatile: behind the wait for the grid before)
+        if constexpr (kBytes == 16) asm volatile("ld.global.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "l"(p));
+        if constexpr (kBytes == 8) asm volatile("ld.global.v2.u32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "l"(p));
+        if constexpr (kBytes == 4) asm volatile("ld.global.u32 %0, [%1];" : "=r"(w[0]) : "l"(p));
+        if constexpr (kBytes == 2) asm volatile("{\n\t.reg .b16 h;\n\tld.global.b16 h, [%1];\n\tmov.b32 %0, {h, h};\n\t}" : "=r"(w[0]) : "l"(p));
+    }
+    __device__ __forceinline__ void store(uint8_t* p) const {
+        if constexpr (kBytes == 16) *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+        if constexpr (kBytes == 8) *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+        if constexpr (kBytes == 4) *reinterpret_cast<uint32_t*>(p) = w[0];
+        if constexpr (kBytes == 2) *reinterpret_cast<uint16_t*>(p) = static_cast<uint16_t>(w[0]);
+    }
 };
-// (volatile: behind the wait for the grid before)
-template <typename T, int N>
-__device__ __forceinline__ Piece<T, N> load(const uint8_t* p) {
-    constexpr int kBytes = sizeof(T) * N;
-    union {
-        Piece<T, N> piece;
-        uint32_t w[kBytes >= 4 ? kBytes / 4 : 1];
-        uint16_t h;
-    } u;
-    if constexpr (kBytes == 16) asm volatile("ld.global.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(u.w[0]), "=r"(u.w[1]), "=r"(u.w[2]), "=r"(u.w[3]) : "l"(p));
-    if constexpr (kBytes == 8) asm volatile("ld.global.v2.u32 {%0, %1}, [%2];" : "=r"(u.w[0]), "=r"(u.w[1]) : "l"(p));
-    if constexpr (kBytes == 4) asm volatile("ld.global.u32 %0, [%1];" : "=r"(u.w[0]) : "l"(p));
-    if constexpr (kBytes == 2) asm volatile("ld.global.u16 %0, [%1];" : "=h"(u.h) : "l"(p));
-    return u.piece;
+// a word's two elements, and back
+template <typename T> __device__ __forceinline__ float2 unpack(uint32_t w);
+template <> __device__ __forceinline__ float2 unpack<__nv_bfloat16>(uint32_t w) { return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u)); }
+template <> __device__ __forceinline__ float2 unpack<__half>(uint32_t w) { return kv4::f16x2_to_f32(w); }
+template <typename T> __device__ __forceinline__ uint32_t pack(float lo, float hi);
+template <> __device__ __forceinline__ uint32_t pack<__nv_bfloat16>(float lo, float hi) { return kv4::pack_bf16x2(lo, hi); }
+template <> __device__ __forceinline__ uint32_t pack<__half>(float lo, float hi) { return kv4::pack_f16x2(lo, hi); }
+
+__device__ __forceinline__ float2 turn_pair(float u, float v, float2 t) { return make_float2(fmaf(u, t.x, -(v * t.y)), fmaf(u, t.y, v * t.x)); }
+
+// the pairs of a piece, or of a piece and its partner
+template <typename T, int N, bool kNeighbours>
+__device__ __forceinline__ void turn_piece(Piece<T, N>& a, Piece<T, N>& c, const float2* t) {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int i = 0; i < (kNeighbours ? N / 2 : N); ++i) {
+            uint32_t &u = kNeighbours ? a.w[2 * i] : a.w[i], &v = kNeighbours ? a.w[2 * i + 1] : c.w[i];
+            const float2 r = turn_pair(__uint_as_float(u), __uint_as_float(v), t[i]);
+            u = __float_as_uint(r.x), v = __float_as_uint(r.y);
+        }
+    } else if constexpr (N == 1) {
+        const float2 r = turn_pair(unpack<T>(a.w[0]).x, unpack<T>(c.w[0]).x, t[0]);
+        a.w[0] = pack<T>(r.x, 0.0f), c.w[0] = pack<T>(r.y, 0.0f);
+    } else {
+#pragma unroll
+        for (int i = 0; i < N / 2; ++i) {
+            const float2 u = unpack<T>(a.w[i]);
+            if constexpr (kNeighbours) {
+                const float2 r = turn_pair(u.x, u.y, t[i]);
+                a.w[i] = pack<T>(r.x, r.y);
+            } else {
+                const float2 v = unpack<T>(c.w[i]), r = turn_pair(u.x, v.x, t[2 * i]), q = turn_pair(u.y, v.y, t[2 * i + 1]);
+                a.w[i] = pack<T>(r.x, q.x), c.w[i] = pack<T>(r.y, q.y);
+            }
+        }
+    }
 }
 
 constexpr uint32_t kFlight = 4;   // heads of a thread at a time
@@ -109,8 +136,8 @@ __global__ void __launch_bounds__(kThreads, 3) rope_kernel(const __grid_constant
             const uint32_t h = h0 + k * stride;
             if (h >= p.heads) continue;
             const uint8_t* src = (h < p.heads_x ? in_x + h * p.x.in_h : in_y + (h - p.heads_x) * p.y.in_h) + offset(item);
-            a[k] = load<T, N>(src);
-            if (!kNeighbours && turned(item)) c[k] = load<T, N>(src + partner);
+            a[k].load(src);
+            if (!kNeighbours && turned(item)) c[k].load(src + partner);
         }
     };
     if (active && item0 < p.items) fetch(item0, first);   // under way while the sines are worked out
@@ -140,17 +167,10 @@ __global__ void __launch_bounds__(kThreads, 3) rope_kernel(const __grid_constant
                 if (h >= p.heads) continue;
                 uint8_t* dst = (h < p.heads_x ? out_x + h * p.x.out_h : out_y + (h - p.heads_x) * p.y.out_h) + offset(item);
                 if (turned(item)) {
-#pragma unroll
-                    for (uint32_t i = 0; i < kPairs; ++i) {
-                        T& first_of = kNeighbours ? a[k].at[2 * i] : a[k].at[i];
-                        T& second_of = kNeighbours ? a[k].at[2 * i + 1] : c[k].at[i];
-                        const float u = to_f32(first_of), v = to_f32(second_of);
-                        first_of = of_f32<T>(fmaf(u, t[i].x, -(v * t[i].y)));
-                        second_of = of_f32<T>(fmaf(u, t[i].y, v * t[i].x));
-                    }
-                    if (!kNeighbours) *reinterpret_cast<Piece<T, N>*>(dst + partner) = c[k];
+                    turn_piece<T, N, kNeighbours>(a[k], c[k], t);
+                    if (!kNeighbours) c[k].store(dst + partner);
                 }
-                *reinterpret_cast<Piece<T, N>*>(dst) = a[k];
+                a[k].store(dst);
             }
         }
     }

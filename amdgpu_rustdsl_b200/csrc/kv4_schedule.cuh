@@ -130,12 +130,12 @@ __device__ __forceinline__ void begin_item(const Kv4AttendParams& p, const DealO
 __device__ __forceinline__ float* slot_of(float* ws, uint32_t grid, uint32_t w, uint32_t slot, uint32_t rows) { return ws + 4u * grid + (static_cast<size_t>(w) * 2u + slot) * rows * 130u; }
 constexpr float kLowest = -1e30f;   // M of a row that has seen nothing
 
-// Sequences' row tiles that no CTA has steps of: their rows see nothing. All threads of the grid.
+// Sequences' row tiles that no CTA has steps of: their rows see nothing. All threads of the grid. `entries`: whether the workspace has entries
 template <uint32_t kTokens>
-__device__ __forceinline__ void clear_empty_entries(const Kv4AttendParams& p, const DealOf<kTokens>& d) {
+__device__ __forceinline__ void clear_empty_entries(const Kv4AttendParams& p, const DealOf<kTokens>& d, bool entries = true) {
     for (uint32_t e = blockIdx.x; e < p.c.B * d.row_tiles; e += gridDim.x) {
         if (steps_of(p, d, e) != 0u) continue;
-        if (begun_by_item(p.c, d.row_tiles, gridDim.x)) {
+        if (entries && begun_by_item(p.c, d.row_tiles, gridDim.x)) {
             for (uint32_t h = threadIdx.x; h < p.c.HK; h += blockDim.x) *begun_at(p.ws, e * p.c.HK + h) = {0u, 0u, 0u, 0u};
         }
         const uint32_t b = e / d.row_tiles, row0 = (e - b * d.row_tiles) * d.rows, rows = min(d.rows, p.S * p.group - row0);

@@ -29,6 +29,7 @@ constexpr uint32_t kWarps = 4, kThreads = kWarps * 32;
 constexpr uint32_t kUnit = 32, kUnitBytes = kUnit / kBlockTokens * kBlockBytes;   // a warp's tokens at a time
 static_assert(kWarps * kUnit == kStepTokens, "a step is a unit of each warp");
 constexpr uint32_t kStages = 3;
+constexpr int kTogether = 3;                      // groups of eight rows up to which a unit's two blocks are worked on together
 constexpr float kUp = 10.0f, kSlack = 4.0f;
 constexpr float kLeast = 1e-37f;                  // of a row's factor: times a masked score it is still -inf
 constexpr float kLn2 = 0.69314718055994531f;
@@ -43,8 +44,12 @@ template <int NT>
 struct QueryRows {
     static constexpr bool kShared = NT >= 2;
     uint4 q[kShared ? 1 : NT][4];   // [group][8 elements: two of the products]
-    float factor[NT][2];            // of the columns 2 tig, 2 tig + 1: scale * log2(e) * the power of two taken out
-    uint32_t limit[NT][2];          // tokens that the columns see
+    static constexpr bool kAway = NT >= 4;   // so do these
+    float factors[kAway ? 1 : NT][2];        // of the columns 2 tig, 2 tig + 1: scale * log2(e) * the power of two taken out
+    uint32_t limits[kAway ? 1 : NT][2];      // tokens that the columns see
+    float* away;                             // [group][column of 8] factors, then limits
+    __device__ __forceinline__ float factor(int g, int j) const { return kAway ? away[8 * g + 2 * (threadIdx.x & 3u) + j] : factors[kAway ? 0 : g][j]; }
+    __device__ __forceinline__ uint32_t limit(int g, int j) const { return kAway ? __float_as_uint(away[8 * NT + 8 * g + 2 * (threadIdx.x & 3u) + j]) : limits[kAway ? 0 : g][j]; }
 };
 template <int NT>
 __device__ __forceinline__ void load_rows(QueryRows<NT>& x, uint4* q_shared, const Kv8AttendParams& p, uint32_t b, uint32_t head, uint32_t row0, uint32_t length, uint32_t n) {
@@ -80,8 +85,10 @@ __device__ __forceinline__ void load_rows(QueryRows<NT>& x, uint4* q_shared, con
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
             const int src = static_cast<int>(2u * tig + j) * 4;   // a lane that holds that row
-            x.factor[g][j] = __shfl_sync(0xFFFFFFFFu, f.y, src) * p.scale_log2;
-            x.limit[g][j] = __shfl_sync(0xFFFFFFFFu, lim, src);
+            const float factor = __shfl_sync(0xFFFFFFFFu, f.y, src) * p.scale_log2;
+            const uint32_t seen = __shfl_sync(0xFFFFFFFFu, lim, src);
+            if constexpr (QueryRows<NT>::kAway) x.away[8 * g + 2 * tig + j] = factor, x.away[8 * NT + 8 * g + 2 * tig + j] = __uint_as_float(seen);   // (all warps write the same)
+            else x.factors[g][j] = factor, x.limits[g][j] = seen;
         }
     }
     if (QueryRows<NT>::kShared) __syncwarp();
@@ -91,6 +98,7 @@ template <int NT>
 struct alignas(128) CtaShared {
     uint8_t ring[kWarps][kStages][kUnitBytes];
     uint4 q[QueryRows<NT>::kShared ? NT * 4 * 32 : 1];
+    float away[QueryRows<NT>::kAway ? 16 * NT : 1];
     float m[kWarps][8 * NT], l[kWarps][8 * NT];
     Sums part[kWarps];
     unsigned long long full[kWarps][kStages];
@@ -109,21 +117,22 @@ struct LostBlocks {
 };
 __device__ const LostBlocks kNowhere;
 
-// 32 tokens: scores, softmax, and their part of O: o[g][i][j], d = 16 gid + 2 i and, from [2 + j], the next, of the column 2 tig + j
-template <int NT, bool kEdge>
-__device__ __forceinline__ void attend_unit(float (&o)[NT][8][4], float (&m)[NT][2], float (&l)[NT][2], const QueryRows<NT>& x, const uint8_t* unit, uint32_t tok0, const uint4* q_shared, uint32_t length) {
+// G blocks of 16 tokens: scores, softmax, and their part of O: o[g][i][j], d = 16 gid + 2 i and, from [2 + j], the next, of the column 2 tig + j
+template <int NT, int G, bool kEdge>
+__device__ __forceinline__ void attend_blocks(float (&o)[NT][8][4], float (&m)[NT][2], float (&l)[NT][2], const QueryRows<NT>& x, const uint8_t* unit, uint32_t tok0, const uint4* q_shared, uint32_t length) {
+    constexpr int kSums = NT <= 2 ? 2 : 1;
     const unsigned lane = threadIdx.x & 31u, gid = lane >> 2, tig = lane & 3u;
-    float s[2][NT][4];
-    uint4 meta[2];
-    bool dead[2];   // a block behind the length: whatever it holds
+    float s[G][NT][4];
+    uint4 meta[G];
+    bool dead[G];   // a block behind the length: whatever it holds
 #pragma unroll
-    for (int gr = 0; gr < 2; ++gr) {
+    for (int gr = 0; gr < G; ++gr) {
         meta[gr] = *reinterpret_cast<const uint4*>(unit + gr * kBlockBytes + kMeta);
         dead[gr] = kEdge && tok0 + 16u * gr >= length;
         if (dead[gr]) meta[gr] = make_uint4(0x3F800000u, 0x3F800000u, 0u, 0u);
     }
 #pragma unroll
-    for (int gr = 0; gr < 2; ++gr) {
+    for (int gr = 0; gr < G; ++gr) {
         const uint8_t* row = unit + gr * kBlockBytes + 128u * gid;
         uint4 top[2], bot[2];
 #pragma unroll
@@ -132,11 +141,11 @@ __device__ __forceinline__ void attend_unit(float (&o)[NT][8][4], float (&m)[NT]
             top[h] = *reinterpret_cast<const uint4*>(row + at);
             bot[h] = *reinterpret_cast<const uint4*>(row + 1024u + at);
         }
-        float d[NT][2][4];   // two sums, of every other product
+        float d[NT][kSums][4];   // two sums, of every other product, where the registers allow it
 #pragma unroll
         for (int g = 0; g < NT; ++g) {
 #pragma unroll
-            for (int y = 0; y < 4; ++y) d[g][0][y] = d[g][1][y] = 0.0f;
+            for (int y = 0; y < 4; ++y) d[g][0][y] = d[g][kSums - 1][y] = 0.0f;
         }
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
@@ -148,29 +157,29 @@ __device__ __forceinline__ void attend_unit(float (&o)[NT][8][4], float (&m)[NT]
             for (int y = 0; y < 2; ++y) {
                 const uint32_t a0 = e4m3x2_lo(t[y]), a1 = e4m3x2_lo(u[y]), a2 = e4m3x2_hi(t[y]), a3 = e4m3x2_hi(u[y]);
 #pragma unroll
-                for (int g = 0; g < NT; ++g) mma_f16(d[g][y], a0, a1, a2, a3, y ? q[g].z : q[g].x, y ? q[g].w : q[g].y, d[g][y]);
+                for (int g = 0; g < NT; ++g) mma_f16(d[g][y % kSums], a0, a1, a2, a3, y ? q[g].z : q[g].x, y ? q[g].w : q[g].y, d[g][y % kSums]);
             }
         }
 #pragma unroll
         for (int g = 0; g < NT; ++g) {
 #pragma unroll
-            for (int y = 0; y < 4; ++y) s[gr][g][y] = d[g][0][y] + d[g][1][y];
+            for (int y = 0; y < 4; ++y) s[gr][g][y] = kSums == 2 ? d[g][0][y] + d[g][kSums - 1][y] : d[g][0][y];
         }
     }
-    if (meta[0].z | meta[1].z) {   // tokens without numbers (the same in all lanes)
+    if (meta[0].z | meta[G - 1].z) {   // tokens without numbers (the same in all lanes)
 #pragma unroll 1
-        for (uint32_t t = 0; t < kUnit; ++t) {
-            const uint32_t mask = (t < 16u ? meta[0].z : meta[1].z) >> (t & 15u);
+        for (uint32_t t = 0; t < G * kBlockTokens; ++t) {
+            const uint32_t mask = (t < 16u ? meta[0].z : meta[G - 1].z) >> (t & 15u);
 #pragma unroll
             for (int g = 0; g < NT; ++g) {
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
-                    if ((mask & 0x10000u) != 0u && tok0 + t < x.limit[g][j]) {
+                    if ((mask & 0x10000u) != 0u && tok0 + t < x.limit(g, j)) {
 #pragma unroll
                         for (int i = 0; i < 8; ++i) o[g][i][j] = o[g][i][2 + j] = __uint_as_float(0x7FC00000u);
                     }
 #pragma unroll
-                    for (int y = 0; y < 4; ++y) {
+                    for (int y = 0; y < 2 * G; ++y) {
                         if ((mask & 1u) != 0u && t == 8u * y + gid) s[y >> 1][g][2 * (y & 1) + j] = __uint_as_float(0x7FC00000u);
                     }
                 }
@@ -179,25 +188,25 @@ __device__ __forceinline__ void attend_unit(float (&o)[NT][8][4], float (&m)[NT]
     }
     if (kEdge) {
 #pragma unroll
-        for (int gr = 0; gr < 2; ++gr) {
+        for (int gr = 0; gr < G; ++gr) {
 #pragma unroll
             for (int g = 0; g < NT; ++g) {
 #pragma unroll
                 for (int y = 0; y < 4; ++y) {
-                    if (tok0 + 16u * gr + 8u * (y >> 1) + gid >= x.limit[g][y & 1]) s[gr][g][y] = -INFINITY;
+                    if (tok0 + 16u * gr + 8u * (y >> 1) + gid >= x.limit(g, y & 1)) s[gr][g][y] = -INFINITY;
                 }
             }
         }
     }
-    float c[2][NT][2], e[2], back[2];
+    float c[G][NT][2], e[G], back[G];
 #pragma unroll
-    for (int gr = 0; gr < 2; ++gr) {
+    for (int gr = 0; gr < G; ++gr) {
         const int exponent = exponent_of(meta[gr].y);
         e[gr] = static_cast<float>(exponent), back[gr] = power_of(-exponent);
 #pragma unroll
         for (int g = 0; g < NT; ++g) {
 #pragma unroll
-            for (int j = 0; j < 2; ++j) c[gr][g][j] = fmaxf(x.factor[g][j] * __uint_as_float(meta[gr].x), kLeast);
+            for (int j = 0; j < 2; ++j) c[gr][g][j] = fmaxf(x.factor(g, j) * __uint_as_float(meta[gr].x), kLeast);
         }
     }
     bool over = false;
@@ -206,7 +215,8 @@ __device__ __forceinline__ void attend_unit(float (&o)[NT][8][4], float (&m)[NT]
     for (int g = 0; g < NT; ++g) {
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-            top[g][j] = fmaxf(fmaf(fmaxf(s[0][g][j], s[0][g][2 + j]), c[0][g][j], e[0]), fmaf(fmaxf(s[1][g][j], s[1][g][2 + j]), c[1][g][j], e[1])) - kUp;
+            top[g][j] = fmaf(fmaxf(s[0][g][j], s[0][g][2 + j]), c[0][g][j], e[0]) - kUp;
+            if (G == 2) top[g][j] = fmaxf(top[g][j], fmaf(fmaxf(s[G - 1][g][j], s[G - 1][g][2 + j]), c[G - 1][g][j], e[G - 1]) - kUp);
             over |= top[g][j] > m[g][j] + kSlack;
         }
     }
@@ -229,7 +239,7 @@ __device__ __forceinline__ void attend_unit(float (&o)[NT][8][4], float (&m)[NT]
         }
     }
 #pragma unroll
-    for (int gr = 0; gr < 2; ++gr) {
+    for (int gr = 0; gr < G; ++gr) {
         if (dead[gr]) continue;
         uint32_t pt[NT][2];
 #pragma unroll
@@ -267,10 +277,21 @@ __device__ __forceinline__ void attend_unit(float (&o)[NT][8][4], float (&m)[NT]
     }
 }
 
+// a unit's 32 tokens: both blocks together, or with many groups one after the other, which takes fewer registers
+template <int NT, bool kEdge>
+__device__ __forceinline__ void attend_unit(float (&o)[NT][8][4], float (&m)[NT][2], float (&l)[NT][2], const QueryRows<NT>& x, const uint8_t* unit, uint32_t tok0, const uint4* q_shared, uint32_t length) {
+    if constexpr (NT <= kTogether) {
+        attend_blocks<NT, 2, kEdge>(o, m, l, x, unit, tok0, q_shared, length);
+    } else {
+#pragma unroll 1
+        for (uint32_t b = 0; b < 2u && (!kEdge || tok0 + b * kBlockTokens < length); ++b) attend_blocks<NT, 1, kEdge>(o, m, l, x, unit + b * kBlockBytes, tok0 + b * kBlockTokens, q_shared, length);
+    }
+}
+
 constexpr uint32_t ctas_per_sm(int groups) { return groups >= 1 ? 2u : 1u; }
 
 template <int NT>
-__global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) kv8_attend_kernel(const __grid_constant__ Kv8AttendParams p) {
+__global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) kv8_attend_kernel(const __grid_constant__ Kv8AttendParams p, bool whole_items) {
     extern __shared__ __align__(128) uint8_t smem_raw[];
     CtaShared<NT>& sh = *reinterpret_cast<CtaShared<NT>*>(smem_raw);
     const unsigned lane = threadIdx.x & 31u, warp = threadIdx.x >> 5, gid = lane >> 2, tig = lane & 3u;
@@ -284,22 +305,37 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) kv8_attend_kernel(c
     pdl_wait();
     __syncthreads();
     const Deal deal{8u * NT, 1u};
-    const uint32_t all = sum_steps(p, deal, 0u, sh.part).all;
-    const uint32_t n_work = workers(all, gridDim.x);
-    clear_empty_entries(p, deal);
-    if (threadIdx.x == 0u) begin_nothing(p, deal);
-    if (blockIdx.x >= n_work) return;
-    const uint32_t begin = run_begin(all, n_work, blockIdx.x), end = run_begin(all, n_work, blockIdx.x + 1u);
-    uint32_t left = end - begin;
-    Place at = find_step(p, deal, begin);
+    // Steps are dealt out evenly, or, where the host has found that no item can have many, items as they are: nothing has to be put together then
+    const uint32_t all = whole_items ? 0u : sum_steps(p, deal, 0u, sh.part).all, n_work = workers(all, gridDim.x), items = p.c.B * p.c.HK;
+    clear_empty_entries(p, deal, !whole_items);
+    if (!whole_items && threadIdx.x == 0u) begin_nothing(p, deal);
+    if (!whole_items && blockIdx.x >= n_work) return;
+    const uint32_t begin = whole_items ? 0u : run_begin(all, n_work, blockIdx.x), end = whole_items ? 0u : run_begin(all, n_work, blockIdx.x + 1u);
+    uint32_t left = end - begin, item = blockIdx.x;
+    Place at = {0u, 0u};
+    if (!whole_items) at = find_step(p, deal, begin);
+    const auto next = [&](Segment& seg) {
+        if (whole_items) {
+            for (; item < items; item += gridDim.x) {
+                const uint32_t b = item / p.c.HK, steps = steps_of(p, deal, b);
+                if (steps == 0u) continue;
+                seg = {b, item - b * p.c.HK, 0u, 0u, steps, steps};
+                item += gridDim.x;
+                return true;
+            }
+            return false;
+        }
+        if (left == 0u) return false;
+        const uint32_t pos = end - left;
+        seg = next_segment(p, deal, at, left);
+        if (threadIdx.x == 0u) begin_item(p, deal, seg, pos, all, n_work);
+        return true;
+    };
     const uint32_t page = 1u << p.c.page_log2, pages = static_cast<uint32_t>(p.c.pages);
     const bool small_pages = page < kUnit;
     uint32_t stage = 0, phase = 0;   // of the warp's next unit: its stage and the parity of the stage's barrier
 
-    while (left > 0u) {
-        const uint32_t pos = end - left;
-        const Segment seg = next_segment(p, deal, at, left);
-        if (threadIdx.x == 0u) begin_item(p, deal, seg, pos, all, n_work);
+    for (Segment seg; next(seg);) {
         const uint32_t b = seg.b, head = seg.head, row0 = seg.row0, first = seg.first;
         const uint32_t length = length_of(p.c, b), n_rows = count_of(p.counts, b, p.S, length);
         const int32_t* row_of_table = p.c.table + static_cast<size_t>(b) * p.c.table_width;
@@ -342,12 +378,13 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) kv8_attend_kernel(c
 #pragma unroll 1
         for (uint32_t k = 0; k < kStages && k < units; ++k) issue(k, (stage + k) % kStages);
         QueryRows<NT> x;
+        x.away = sh.away;
         load_rows<NT>(x, sh.q, p, b, head, row0, length, n_rows);
         uint32_t low = 0xFFFFFFFFu;   // tokens that every live column sees
 #pragma unroll
         for (int g = 0; g < NT; ++g) {
 #pragma unroll
-            for (int j = 0; j < 2; ++j) low = min(low, x.limit[g][j] == 0u ? 0xFFFFFFFFu : x.limit[g][j]);
+            for (int j = 0; j < 2; ++j) low = min(low, x.limit(g, j) == 0u ? 0xFFFFFFFFu : x.limit(g, j));
         }
         low = min(__reduce_min_sync(0xFFFFFFFFu, low), length);
 
@@ -451,9 +488,12 @@ constexpr uint32_t kMostFew = 32;
 
 uint32_t groups_of(uint32_t rows) { return (rows + 7u) / 8u; }
 
+// Items of up to so many steps, which is up to 512 tokens, are not cut: a launch and the way through memory are saved, 2 heads of 256 tokens 11.8 -> ~ us
+constexpr uint32_t kWholeSteps = 4;
+uint32_t most_steps(const Kv4View& c) { return static_cast<uint32_t>(((static_cast<unsigned long long>(c.table_width) << c.page_log2) + kStepTokens - 1u) / kStepTokens); }
 uint32_t attend_grid(const Kv4View& c, uint32_t groups) {
-    const unsigned long long steps = ((static_cast<unsigned long long>(c.table_width) << c.page_log2) + kStepTokens - 1u) / kStepTokens, per_sm = ctas_per_sm(static_cast<int>(groups));
-    const unsigned long long most = steps * c.B * c.HK, full = per_sm * static_cast<unsigned long long>(current_sm_count());
+    const unsigned long long per_sm = ctas_per_sm(static_cast<int>(groups)), steps = most_steps(c);
+    const unsigned long long most = (steps <= kWholeSteps ? 1ull : steps) * c.B * c.HK, full = per_sm * static_cast<unsigned long long>(current_sm_count());
     return static_cast<uint32_t>(most < full ? (most ? most : 1ull) : full);
 }
 
@@ -470,8 +510,9 @@ cudaError_t launch_rows(const Kv8AttendParams& p, cudaStream_t stream) {
         if (e != cudaSuccess) return e;
         if (dev >= 0 && dev < 64) set[dev].store(true, std::memory_order_relaxed);
     }
-    e = kv4_launch(kv8_attend_kernel<NT>, dim3(grid), kThreads, smem, stream, p);
-    return e != cudaSuccess ? e : launch_combine_few(p, 8u * NT, grid, stream);
+    const bool whole = most_steps(p.c) <= kWholeSteps;
+    e = kv4_launch(kv8_attend_kernel<NT>, dim3(grid), kThreads, smem, stream, p, whole);
+    return e != cudaSuccess || whole ? e : launch_combine_few(p, 8u * NT, grid, stream);
 }
 
 cudaError_t launch_many(const Kv8AttendParams& p, cudaStream_t stream) {

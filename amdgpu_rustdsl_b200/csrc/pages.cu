@@ -128,6 +128,7 @@ __global__ void __launch_bounds__(kThreads) pages_take_kernel(const __grid_const
     uint32_t start = sum_in_front(tokens, part32, all_tokens);
     const Range range = own_range(p);
     const uint32_t known = min(range.end + 1u, p.B);   // (the maps' rows may begin the sequence behind)
+    const bool alone = gridDim.x == 1u;
     upto = in_front;
     uint32_t taken = 0;
     for (uint32_t b = b0; b < b1; ++b) {
@@ -140,6 +141,7 @@ __global__ void __launch_bounds__(kThreads) pages_take_kernel(const __grid_const
             sm_length[b - range.begin] = length, sm_granted[b - range.begin] = granted, sm_before[b - range.begin] = static_cast<uint32_t>(min(upto - need, 0xFFFFFFFFull));
             if (b < range.end) {
                 p.granted[b] = static_cast<int32_t>(granted);
+                if (alone) p.lengths[b] = static_cast<int32_t>(length + granted);   // (each thread has read its own)
                 if (p.starts != nullptr) p.starts[b] = static_cast<int32_t>(start);
             }
         }
@@ -174,7 +176,9 @@ __global__ void __launch_bounds__(kThreads) pages_take_kernel(const __grid_const
         }
     }
     if (!is_last(p, &last_flag)) return;
-    for (uint32_t b = threadIdx.x; b < p.B; b += kThreads) p.lengths[b] = static_cast<int32_t>(length_at(p, b) + ld_now(p.granted + b));
+    if (!alone) {
+        for (uint32_t b = threadIdx.x; b < p.B; b += kThreads) p.lengths[b] = static_cast<int32_t>(length_at(p, b) + ld_now(p.granted + b));
+    }
     const uint32_t most = __reduce_max_sync(0xFFFFFFFFu, taken);
     if ((threadIdx.x & 31u) == 0u) part32[threadIdx.x >> 5] = most;
     __syncthreads();
@@ -194,18 +198,20 @@ __global__ void __launch_bounds__(kThreads) pages_cut_kernel(const __grid_consta
     kv4::pdl_wait();
     const uint32_t per = (p.B + kThreads - 1u) / kThreads, b0 = min(threadIdx.x * per, p.B), b1 = min(b0 + per, p.B), n_free = height(p);
     const uint32_t length0 = b0 < b1 ? length_at(p, b0) : 0u, asked0 = b0 < b1 ? asked_at(p, b0) : 0u;
+    uint32_t had, kept, length_now, keep_now;
     const auto look = [&](uint32_t b, uint32_t& had, uint32_t& kept) {
-        const uint32_t length = b == b0 ? length0 : length_at(p, b), keep = min(length, b == b0 ? asked0 : asked_at(p, b));
-        had = pages_of(p, length), kept = pages_of(p, keep);
+        length_now = b == b0 ? length0 : length_at(p, b), keep_now = b == b0 ? asked0 : asked_at(p, b);
+        had = pages_of(p, length_now), kept = pages_of(p, min(length_now, keep_now));
         return had - kept;
     };
-    uint32_t had, kept;
+    const bool alone = gridDim.x == 1u;
     unsigned long long mine = 0, all;
     for (uint32_t b = b0; b < b1; ++b) mine += look(b, had, kept);
     unsigned long long upto = sum_in_front(mine, part64, all);
     const Range range = own_range(p);
     for (uint32_t b = b0; b < b1; ++b) {
         upto += look(b, had, kept);
+        if (alone) p.lengths[b] = static_cast<int32_t>(min(length_now, keep_now));   // (each thread has read its own)
         if (b >= range.begin && b < range.end) sm_kept[b - range.begin] = kept, sm_pages[b - range.begin] = had, sm_behind[b - range.begin] = all - upto;
     }
     __syncthreads();
@@ -218,7 +224,9 @@ __global__ void __launch_bounds__(kThreads) pages_cut_kernel(const __grid_consta
             *entry = -1;
         });
     if (!is_last(p, &last_flag)) return;
-    for (uint32_t b = threadIdx.x; b < p.B; b += kThreads) p.lengths[b] = static_cast<int32_t>(min(length_at(p, b), asked_at(p, b)));
+    if (!alone) {
+        for (uint32_t b = threadIdx.x; b < p.B; b += kThreads) p.lengths[b] = static_cast<int32_t>(min(length_at(p, b), asked_at(p, b)));
+    }
     if (threadIdx.x == 0u) p.free[0] = static_cast<int32_t>(min(n_free + all, static_cast<unsigned long long>(p.pages)));
 }
 

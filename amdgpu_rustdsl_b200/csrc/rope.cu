@@ -13,7 +13,7 @@ namespace b200mx {
 
 namespace {
 
-constexpr uint32_t kThreads = 256, kMostTokens = 4, kMostPairs = FMHA_ROPE_MAX_HEAD_DIM / 2;
+constexpr uint32_t kMostTokens = 4, kMostPairs = FMHA_ROPE_MAX_HEAD_DIM / 2;
 
 struct Rows {
     const uint8_t* in;
@@ -102,11 +102,13 @@ __device__ __forceinline__ void turn_piece(Piece<T, N>& a, Piece<T, N>& c, const
     }
 }
 
-constexpr uint32_t kFlight = 4;   // heads of a thread at a time
+// heads of a thread at a time: ten loads of a piece and its partner, or eight of a piece alone
+template <bool kNeighbours>
+constexpr uint32_t kFlightOf = kNeighbours ? 8u : 5u;
 
 // N elements of T at a time. N = 1 takes both layouts, a pair's elements one by one.
-template <typename T, int N, bool kNeighbours>
-__global__ void __launch_bounds__(kThreads, 3) rope_kernel(const __grid_constant__ RopeParams p) {
+template <typename T, int N, bool kNeighbours, uint32_t kThreads>
+__global__ void __launch_bounds__(kThreads, kThreads == 128 ? 5 : 3) rope_kernel(const __grid_constant__ RopeParams p) {
     __shared__ float2 table[kMostTokens * kMostPairs];
     kv4::pdl_launch();
     kv4::pdl_wait();
@@ -118,6 +120,7 @@ __global__ void __launch_bounds__(kThreads, 3) rope_kernel(const __grid_constant
     const bool active = group < sharing * p.per_cta && mine < tokens;
     const uint32_t token = token0 + (active ? mine : 0u), b = token / p.S, s = token - b * p.S;
     const uint32_t first = blockIdx.y * sharing + group / p.per_cta;
+    constexpr uint32_t kFlight = kFlightOf<kNeighbours>;
     constexpr bool kScalar = N == 1;
     constexpr uint32_t kPairs = kScalar ? 1 : kNeighbours ? N / 2 : N;
     const uint32_t item0 = p.items < kThreads ? threadIdx.x - group * p.items : threadIdx.x, item_step = p.items < kThreads ? p.items : kThreads;
@@ -180,20 +183,28 @@ template <typename T, int N, bool kNeighbours>
 cudaError_t launch(RopeParams p, bool copies, cudaStream_t stream) {
     p.rotate = N == 1 ? p.n : kNeighbours ? 2u * p.n / N : p.n / N;
     p.items = p.rotate + (copies ? (p.head_dim - 2u * p.n) / N : 0u);
-    const uint32_t groups = p.items < kThreads ? kThreads / p.items : 1u, sms = static_cast<uint32_t>(current_sm_count());
-    // With many tokens as many of them a CTA, up to four, as give the most heads a thread in one round of loads; with few one each, their heads dealt out over up to four CTAs
+    const uint32_t sms = static_cast<uint32_t>(current_sm_count());
+    // Threads a CTA and, with many tokens, tokens a CTA: what gives the most threads the most heads in their rounds of loads; then the fewest rounds, the smaller CTA. With few tokens one
+    // each, their heads dealt out over up to four CTAs. (4 x 4096 tokens of 40 heads of 128, bf16 halves: 128 threads, 2 tokens 57.6 us, 256 and 4 62.2, 256 and 3 with one head less
+    // in flight 65.5. 3 x 1337 of 24 heads of 96, f32 neighbours, 40 turned: 256 and 3 16.4, 128 and 1 32.5)
+    uint32_t threads = 256u, best = 0u;
     p.per_cta = 1u;
     if (p.tokens >= 16u * sms) {
-        uint32_t best = 0;
-        for (uint32_t t = 1; t <= kMostTokens && t <= groups; ++t) {
-            const uint32_t rounds = (p.heads + groups / t * kFlight - 1u) / (groups / t * kFlight), busy = t * p.heads * 1024u / (rounds * kFlight);
-            if (busy > best) best = busy, p.per_cta = t;
+        for (uint32_t n = 128u; n <= 256u; n += 128u) {
+            const uint32_t groups = p.items < n ? n / p.items : 1u;
+            for (uint32_t t = 1; t <= kMostTokens && t <= groups; ++t) {
+                const uint32_t at_once = groups / t * kFlightOf<kNeighbours>, rounds = (p.heads + at_once - 1u) / at_once;
+                const uint32_t busy = static_cast<uint32_t>(static_cast<uint64_t>(t) * p.heads * (p.items < n ? p.items : n) * 1024u / (static_cast<uint64_t>(rounds) * kFlightOf<kNeighbours> * n));
+                const uint32_t score = 16u * (busy < 1024u ? busy : 1024u) + 16u - (rounds < 15u ? rounds : 15u);
+                if (score > best) best = score, threads = n, p.per_cta = t;
+            }
         }
     }
-    const uint32_t ctas = (p.tokens + p.per_cta - 1u) / p.per_cta, sharing = groups / p.per_cta;
+    const uint32_t groups = p.items < threads ? threads / p.items : 1u, ctas = (p.tokens + p.per_cta - 1u) / p.per_cta, sharing = groups / p.per_cta;
     uint32_t split = 1;
     while (split < 4u && 2u * split * ctas <= 2u * sms && 2u * split * sharing <= p.heads) split *= 2u;
-    return kv4_launch(rope_kernel<T, N, kNeighbours>, dim3(ctas, split), kThreads, 0, stream, p);
+    if (threads == 128u) return kv4_launch(rope_kernel<T, N, kNeighbours, 128u>, dim3(ctas, split), 128u, 0, stream, p);
+    return kv4_launch(rope_kernel<T, N, kNeighbours, 256u>, dim3(ctas, split), 256u, 0, stream, p);
 }
 
 template <typename T, int N>

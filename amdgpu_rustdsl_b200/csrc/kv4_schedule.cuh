@@ -10,27 +10,28 @@ namespace kv4 {
 
 constexpr uint32_t kStepTokens = 128;
 
-// (steps of kTokens: what the text above says of 128 tokens holds for them)
-template <uint32_t kTokens>
+// (steps of kTokens: what the text above says of 128 tokens holds for them. kExtra: what it costs a CTA to begin an item, in steps: an item is dealt out as that many more, which lie in front
+// of its steps and are not carried out. A CTA's run may then hold nothing else of an item)
+template <uint32_t kTokens, uint32_t kExtra = 0>
 struct DealOf {
     uint32_t rows, row_tiles;   // of an item, of a sequence
 };
 using Deal = DealOf<kStepTokens>;
 
-template <uint32_t kTokens>
-__device__ __forceinline__ uint32_t steps_of(const Kv4AttendParams& p, const DealOf<kTokens>& d, uint32_t entry) {
+template <uint32_t kTokens, uint32_t kExtra>
+__device__ __forceinline__ uint32_t steps_of(const Kv4AttendParams& p, const DealOf<kTokens, kExtra>& d, uint32_t entry) {
     const uint32_t b = entry / d.row_tiles, row0 = (entry - b * d.row_tiles) * d.rows, length = length_of(p.c, b), n = count_of(p.counts, b, p.S, length);
     if (row0 >= n * p.group) return 0u;
     const uint32_t last = (min(row0 + d.rows, n * p.group) - 1u) / p.group;
-    return ((p.causal ? length - n + last + 1u : length) + kTokens - 1u) / kTokens;
+    return ((p.causal ? length - n + last + 1u : length) + kTokens - 1u) / kTokens + kExtra;
 }
 
 struct Sums {
     uint32_t below, all;
 };
 // Steps of the entries below `upto`, and of all, times the heads (the host has checked that they stay below 2^32). All threads of the CTA; `part` has an element per warp.
-template <uint32_t kTokens>
-__device__ __forceinline__ Sums sum_steps(const Kv4AttendParams& p, const DealOf<kTokens>& d, uint32_t upto, Sums* part) {
+template <uint32_t kTokens, uint32_t kExtra>
+__device__ __forceinline__ Sums sum_steps(const Kv4AttendParams& p, const DealOf<kTokens, kExtra>& d, uint32_t upto, Sums* part) {
     uint32_t below = 0, all = 0;
     for (uint32_t e = threadIdx.x; e < p.c.B * d.row_tiles; e += blockDim.x) {
         const uint32_t t = steps_of(p, d, e);
@@ -60,8 +61,8 @@ struct Place {
     uint32_t entry;
     uint32_t in;   // step within the entry's items
 };
-template <uint32_t kTokens>
-__device__ __forceinline__ Place find_step(const Kv4AttendParams& p, const DealOf<kTokens>& d, uint32_t pos) {
+template <uint32_t kTokens, uint32_t kExtra>
+__device__ __forceinline__ Place find_step(const Kv4AttendParams& p, const DealOf<kTokens, kExtra>& d, uint32_t pos) {
     const unsigned lane = threadIdx.x & 31u;
     const uint32_t entries = p.c.B * d.row_tiles;
     uint32_t before = 0;
@@ -87,10 +88,11 @@ __device__ __forceinline__ Place find_step(const Kv4AttendParams& p, const DealO
 struct Segment {
     uint32_t b, head, row0;         // the item
     uint32_t first, steps, of;      // steps first .. first + steps - 1 of `of`
+    uint32_t before;                // of what the item is dealt out as, the part in front of the run
 };
 // The segment at the head of a CTA's run of `left` steps; moves on behind it
-template <uint32_t kTokens>
-__device__ __forceinline__ Segment next_segment(const Kv4AttendParams& p, const DealOf<kTokens>& d, Place& at, uint32_t& left) {
+template <uint32_t kTokens, uint32_t kExtra>
+__device__ __forceinline__ Segment next_segment(const Kv4AttendParams& p, const DealOf<kTokens, kExtra>& d, Place& at, uint32_t& left) {
     uint32_t of = steps_of(p, d, at.entry);
     while (at.in >= of * p.c.HK) {   // also where an entry has none
         at.in -= of * p.c.HK;
@@ -98,10 +100,11 @@ __device__ __forceinline__ Segment next_segment(const Kv4AttendParams& p, const 
     }
     Segment s;
     s.b = at.entry / d.row_tiles, s.row0 = (at.entry - s.b * d.row_tiles) * d.rows;
-    s.head = at.in / of, s.first = at.in - s.head * of, s.of = of;
-    s.steps = min(of - s.first, left);
-    at.in += s.steps;
-    left -= s.steps;
+    s.head = at.in / of, s.before = at.in - s.head * of, s.of = of - kExtra;
+    const uint32_t dealt = min(of - s.before, left);
+    s.first = max(s.before, kExtra) - kExtra, s.steps = max(s.before + dealt, kExtra) - kExtra - s.first;
+    at.in += dealt;
+    left -= dealt;
     return s;
 }
 
@@ -116,14 +119,14 @@ __host__ __device__ __forceinline__ bool begun_by_item(const Kv4View& c, uint32_
 __host__ __device__ __forceinline__ uint32_t begun_entries(const Kv4View& c, uint32_t row_tiles, uint32_t grid) { return begun_by_item(c, row_tiles, grid) ? c.B * c.HK * row_tiles : grid; }
 __device__ __forceinline__ Begun* begun_at(float* ws, uint32_t x) { return reinterpret_cast<Begun*>(ws) + x; }
 // by one thread of a CTA: at its start, and for each segment
-template <uint32_t kTokens>
-__device__ __forceinline__ void begin_nothing(const Kv4AttendParams& p, const DealOf<kTokens>& d) {
+template <uint32_t kTokens, uint32_t kExtra>
+__device__ __forceinline__ void begin_nothing(const Kv4AttendParams& p, const DealOf<kTokens, kExtra>& d) {
     if (!begun_by_item(p.c, d.row_tiles, gridDim.x)) *begun_at(p.ws, blockIdx.x) = {0u, blockIdx.x, blockIdx.x, 0u};
 }
-template <uint32_t kTokens>
-__device__ __forceinline__ void begin_item(const Kv4AttendParams& p, const DealOf<kTokens>& d, const Segment& s, uint32_t pos, uint32_t all, uint32_t n_work) {
-    if (s.first != 0u) return;
-    const uint32_t item = (s.b * d.row_tiles + s.row0 / d.rows) * p.c.HK + s.head, last = s.steps == s.of ? blockIdx.x : worker_at(all, n_work, pos + s.of - 1u);
+template <uint32_t kTokens, uint32_t kExtra>
+__device__ __forceinline__ void begin_item(const Kv4AttendParams& p, const DealOf<kTokens, kExtra>& d, const Segment& s, uint32_t pos, uint32_t all, uint32_t n_work) {
+    if (s.first != 0u || s.steps == 0u) return;
+    const uint32_t item = (s.b * d.row_tiles + s.row0 / d.rows) * p.c.HK + s.head, last = s.steps == s.of ? blockIdx.x : worker_at(all, n_work, pos - s.before + s.of + kExtra - 1u);
     const bool by_item = begun_by_item(p.c, d.row_tiles, gridDim.x);
     if (by_item || last != blockIdx.x) *begun_at(p.ws, by_item ? item : blockIdx.x) = {item, blockIdx.x, last, 0u};
 }
@@ -131,8 +134,8 @@ __device__ __forceinline__ float* slot_of(float* ws, uint32_t grid, uint32_t w, 
 constexpr float kLowest = -1e30f;   // M of a row that has seen nothing
 
 // Sequences' row tiles that no CTA has steps of: their rows see nothing. All threads of the grid. `entries`: whether the workspace has entries
-template <uint32_t kTokens>
-__device__ __forceinline__ void clear_empty_entries(const Kv4AttendParams& p, const DealOf<kTokens>& d, bool entries = true) {
+template <uint32_t kTokens, uint32_t kExtra>
+__device__ __forceinline__ void clear_empty_entries(const Kv4AttendParams& p, const DealOf<kTokens, kExtra>& d, bool entries = true) {
     for (uint32_t e = blockIdx.x; e < p.c.B * d.row_tiles; e += gridDim.x) {
         if (steps_of(p, d, e) != 0u) continue;
         if (entries && begun_by_item(p.c, d.row_tiles, gridDim.x)) {

@@ -54,7 +54,7 @@ int fmha_kv8_attend(const fmha_kv8_cache* cache, const fmha_kv8_attend_args* a, 
     if (static_cast<uint64_t>(p.c.B) * a->S * a->H > kMostRows) return refuse(err, cap, "attend: more than 2^30 query rows");
     // the kernels deal out steps of 80 tokens and 256 rows at least, counted in 32 bits
     const uint64_t tokens = static_cast<uint64_t>(p.c.table_width) << p.c.page_log2, row_tiles = (static_cast<uint64_t>(a->S) * (a->H / p.c.HK) + 255u) / 256u;
-    if (((tokens + 79u) / 80u) * p.c.B * p.c.HK > 0xFFFFFFFFull / row_tiles) return refuse(err, cap, "attend: more than 2^32 steps of 80 tokens and 256 query rows");
+    if (((tokens + 79u) / 80u + 5u) * p.c.B * p.c.HK > 0xFFFFFFFFull / row_tiles) return refuse(err, cap, "attend: more than 2^32 steps of 80 tokens and 256 query rows");
     if (!(a->scale > 0.0f) || a->scale > 2.3e38f) return refuse(err, cap, "attend: scale must be a positive number");
     if (a->workspace == nullptr || !aligned16(a->workspace) || a->workspace_bytes < fmha_kv8_attend_workspace(cache, a))
         return refuse(err, cap, "attend: the workspace must be 16-byte aligned and hold fmha_kv8_attend_workspace() bytes");

@@ -29,6 +29,7 @@ constexpr uint32_t kWarps = 4, kThreads = kWarps * 32;
 constexpr uint32_t kUnit = 32, kUnitBytes = kUnit / kBlockTokens * kBlockBytes;   // a warp's tokens at a time
 static_assert(kWarps * kUnit == kStepTokens, "a step is a unit of each warp");
 constexpr uint32_t kStages = 3;
+constexpr uint32_t kExtra = 4;   // what a CTA's change to another item costs, in steps (24 ragged drafts of 5 rows in pages of 16: 78 us without, 65, 59, 59 with 2, 4, 6)
 constexpr int kTogether = 3;                      // groups of eight rows up to which a unit's two blocks are worked on together
 constexpr float kUp = 10.0f, kSlack = 4.0f;
 constexpr float kLeast = 1e-37f;                  // of a row's factor: times a masked score it is still -inf
@@ -304,7 +305,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) kv8_attend_kernel(c
     pdl_launch();
     pdl_wait();
     __syncthreads();
-    const Deal deal{8u * NT, 1u};
+    const DealOf<kStepTokens, kExtra> deal{8u * NT, 1u};
     // Steps are dealt out evenly, or, where the host has found that no item can have many, items as they are: nothing has to be put together then
     const uint32_t all = whole_items ? 0u : sum_steps(p, deal, 0u, sh.part).all, n_work = workers(all, gridDim.x), items = p.c.B * p.c.HK;
     clear_empty_entries(p, deal, !whole_items);
@@ -317,19 +318,22 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) kv8_attend_kernel(c
     const auto next = [&](Segment& seg) {
         if (whole_items) {
             for (; item < items; item += gridDim.x) {
-                const uint32_t b = item / p.c.HK, steps = steps_of(p, deal, b);
+                const uint32_t b = item / p.c.HK, dealt = steps_of(p, deal, b), steps = max(dealt, kExtra) - kExtra;
                 if (steps == 0u) continue;
-                seg = {b, item - b * p.c.HK, 0u, 0u, steps, steps};
+                seg = {b, item - b * p.c.HK, 0u, 0u, steps, steps, 0u};
                 item += gridDim.x;
                 return true;
             }
             return false;
         }
-        if (left == 0u) return false;
-        const uint32_t pos = end - left;
-        seg = next_segment(p, deal, at, left);
-        if (threadIdx.x == 0u) begin_item(p, deal, seg, pos, all, n_work);
-        return true;
+        while (left > 0u) {
+            const uint32_t pos = end - left;
+            seg = next_segment(p, deal, at, left);
+            if (seg.steps == 0u) continue;
+            if (threadIdx.x == 0u) begin_item(p, deal, seg, pos, all, n_work);
+            return true;
+        }
+        return false;
     };
     const uint32_t page = 1u << p.c.page_log2, pages = static_cast<uint32_t>(p.c.pages);
     const bool small_pages = page < kUnit;

@@ -27,6 +27,7 @@ using namespace kv8;
 using namespace sm100;
 
 constexpr uint32_t kTileRows = 128, kItemRows = 256, kStep = 80, kBlocks = kStep / kBlockTokens, kStages = 3, kRawStages = 2;
+constexpr uint32_t kExtra = 5;   // what a CTA's change to another item costs, in steps (4 ragged chunks of 333 rows, 24 heads, 94 us without, 73, 71, 70 with 2, 4, 6)
 // Slots of the steps' scales. Those of step j are written when its codes have come, for which those of step j - 2 must have been taken: behind the scores of step j - 5 (three stages of K)
 // and so behind the softmax's reads of the scores of step j - 6
 constexpr uint32_t kScaleSlots = 8;
@@ -65,7 +66,7 @@ struct Shared {
     Sums part[kThreads / 32];
     struct Plan {
         Segment seg;
-        uint32_t length, n, left;      // left: steps of the CTA's run behind the segment
+        uint32_t length, n, more;      // more: whether the CTA has a segment behind this one. (One without steps: it has none at all)
         uint32_t steps[2];             // of the two tiles: those that their last live rows see
     } plan[kSegmentSlots];
     uint32_t tmem, failed, not_drained;
@@ -153,12 +154,12 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
     const uint32_t tmem = __shfl_sync(0xFFFFFFFFu, sh.tmem, 0);
     pdl_launch();
     pdl_wait();
-    const DealOf<kStep> deal{kItemRows, row_tiles};
+    const DealOf<kStep, kExtra> deal{kItemRows, row_tiles};
     const uint32_t all = sum_steps(p, deal, 0u, sh.part).all;
     const uint32_t n_work = workers(all, gridDim.x);
     volatile uint32_t* failed = &sh.failed;
     clear_empty_entries(p, deal);
-    if (threadIdx.x == 0u) begin_nothing(p, deal);
+    if (threadIdx.x == 0u && blockIdx.x >= n_work) begin_nothing(p, deal);
     if (blockIdx.x < n_work) {
         const uint32_t begin = run_begin(all, n_work, blockIdx.x);
         const uint32_t end = run_begin(all, n_work, blockIdx.x + 1u);
@@ -219,11 +220,11 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
             };
             float c_row = 0.0f;
             Shared::Plan now;
-            ok = next_plan(now) && load_rows(now.seg, now.n, c_row);
+            ok = next_plan(now) && now.seg.steps > 0u && load_rows(now.seg, now.n, c_row);
             for (bool more = true; more && ok;) {
                 const Segment seg = now.seg;
                 const uint32_t length = now.length, n = now.n, nan_slot = (number - 1u) % kSegmentSlots;
-                more = now.left > 0u;
+                more = now.more != 0u;
                 const uint32_t steps = q != 0u ? now.steps[1] : now.steps[0], row = seg.row0 + q * kTileRows + r, i = row / p.group;
                 const bool exists = row < p.S * p.group;
                 const uint32_t limit = !exists || i >= n ? 0u : p.causal ? length - n + i + 1u : length;
@@ -380,9 +381,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
             constexpr uint32_t kBlockOfTile = kBlockTokens * 128u / 16u;   // from a block's place in a tile to the next one's, in pieces
             uint32_t step = 0;   // so far
             Shared::Plan now;
-            now.left = 1u;
+            now.more = 1u;
             bool ok = true;
-            while (now.left > 0u && ok) {
+            while (now.more != 0u && ok) {
                 if (!next_plan(now)) break;
                 const Segment seg = now.seg;
                 const uint32_t length = now.length;
@@ -490,9 +491,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
                     if (last) commit(bar(kQEmpty + q));
                 };
                 Shared::Plan now;
-                now.left = 1u;
-                while (uniform(now.left) > 0u && ok) {
-                    if (!next_plan(now)) break;
+                now.more = 1u;
+                while (uniform(now.more) != 0u && ok) {
+                    if (!next_plan(now) || uniform(now.seg.steps) == 0u) break;
                     const uint32_t steps = uniform(q != 0u ? now.steps[1] : now.steps[0]), seg_steps = uniform(now.seg.steps);
                     if (!wait(bar(kQFull + q), q_phase)) break;
                     q_phase ^= 1u;
@@ -526,16 +527,36 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
                 __syncwarp();
             } else if (warp == kCopyWarp) {
                 // The segments, for all roles, and the copies of a step: lane x brings block x
-                uint32_t step = 0, left = end - begin;
+                uint32_t step = 0, left = end - begin, pos = begin, next_pos = begin;
                 Place at = find_step(p, deal, begin);
-                bool ok = true;
-                while (left > 0u && ok) {
-                    const uint32_t pos = end - left;
-                    const Segment seg = next_segment(p, deal, at, left);
+                bool ok = true, have = false, have_next = false;
+                Segment seg, next;
+                const auto look_ahead = [&]() {   // for the next segment of the run that has steps
+                    have_next = false;
+                    while (left > 0u && !have_next) {
+                        next_pos = end - left;
+                        next = next_segment(p, deal, at, left);
+                        have_next = next.steps > 0u;
+                    }
+                };
+                if (lane == 0u) {
+                    begin_nothing(p, deal);
+                    sh.plan[0].seg.steps = 0u;
+                }
+                look_ahead();
+                have = have_next;
+                if (!have && lane == 0u) {
+                    sh.plan[0].more = 0u;
+                    mbar_arrive(bar(kSegment));
+                }
+                while (have && ok) {
+                    seg = next, pos = next_pos;
+                    look_ahead();
+                    have = have_next;
                     const uint32_t length = length_of(p.c, seg.b), n = count_of(p.counts, seg.b, p.S, length);
                     if (lane == 0u) {
                         Shared::Plan& x = sh.plan[number % kSegmentSlots];
-                        x.seg = seg, x.length = length, x.n = n, x.left = left;
+                        x.seg = seg, x.length = length, x.n = n, x.more = have_next;
                         for (uint32_t q = 0; q < 2u; ++q) x.steps[q] = tile_steps(p, seg, q, length, n);
                         mbar_arrive(bar(kSegment + number % kSegmentSlots));
                         begin_item(p, deal, seg, pos, all, n_work);
@@ -580,9 +601,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
                 // The scales of a step, a lane a block: as the softmax wants them, and whether the step's tokens are all there and have numbers
                 uint32_t step = 0;
                 Shared::Plan now;
-                now.left = 1u;
+                now.more = 1u;
                 bool ok = true;
-                while (now.left > 0u && ok) {
+                while (now.more != 0u && ok) {
                     if (!next_plan(now)) break;
                     const Segment seg = now.seg;
                     uint32_t* nan_from = &sh.nan_from[(number - 1u) % kSegmentSlots];

@@ -98,7 +98,10 @@ __device__ __forceinline__ void load_rows(QueryRows<NT>& x, uint4* q_shared, con
 template <int NT>
 struct alignas(128) CtaShared {
     uint8_t ring[kWarps][kStages][kUnitBytes];
-    uint4 q[QueryRows<NT>::kShared ? NT * 4 * 32 : 1];
+    union {
+        uint4 q[QueryRows<NT>::kShared ? NT * 4 * 32 : 1];
+        float o[2][8 * 128];   // where the warps' parts of an item's O come together, when its rows are no longer needed
+    };
     float away[QueryRows<NT>::kAway ? 16 * NT : 1];
     float m[kWarps][8 * NT], l[kWarps][8 * NT];
     Sums part[kWarps];
@@ -339,48 +342,63 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) kv8_attend_kernel(c
     const bool small_pages = page < kUnit;
     uint32_t stage = 0, phase = 0;   // of the warp's next unit: its stage and the parity of the stage's barrier
 
-    for (Segment seg; next(seg);) {
-        const uint32_t b = seg.b, head = seg.head, row0 = seg.row0, first = seg.first;
-        const uint32_t length = length_of(p.c, b), n_rows = count_of(p.counts, b, p.S, length);
-        const int32_t* row_of_table = p.c.table + static_cast<size_t>(b) * p.c.table_width;
-        const uint8_t* blocks = p.c.pool + static_cast<uint64_t>(head) * (page / kBlockTokens) * kBlockBytes;
-        // the warp's units: tokens start + 128 k of the segment, as far as the sequence goes
-        const uint32_t start = first * kStepTokens + warp * kUnit, stop = min(length, (first + seg.steps) * kStepTokens);
-        const uint32_t units = start < stop ? (stop - start + kStepTokens - 1u) / kStepTokens : 0u;
-        // page numbers of 32 units at a time, one a lane (two where a unit has two pages), and those of the next 32 ahead
-        int id = -1, id_second = -1, next_id = -1, next_second = -1;
-        auto look_up = [&](uint32_t k) {
-            const uint32_t t = start + k * kStepTokens;
-            if (k < units) {
-                next_id = ld_i32(row_of_table + (t >> p.c.page_log2));
-                if (small_pages && t + kBlockTokens < length) next_second = ld_i32(row_of_table + (t >> p.c.page_log2) + 1);
+    // A warp's copies of a segment: its units are the tokens start + 128 k, as far as the sequence goes
+    struct Feed {
+        const int32_t* row_of_table;
+        const uint8_t* blocks;
+        uint32_t start, units, length;
+        int id, id_second, next_id, next_second;   // page numbers of 32 units at a time, one a lane (two where a unit has two pages), and those of the next 32 ahead
+    } feed = {};
+    const auto look_up = [&](uint32_t k) {
+        const uint32_t t = feed.start + k * kStepTokens;
+        if (k < feed.units) {
+            feed.next_id = ld_i32(feed.row_of_table + (t >> p.c.page_log2));
+            if (small_pages && t + kBlockTokens < feed.length) feed.next_second = ld_i32(feed.row_of_table + (t >> p.c.page_log2) + 1);
+        }
+    };
+    const auto issue = [&](uint32_t k, uint32_t into) {
+        if ((k & 31u) == 0u) {
+            feed.id = feed.next_id, feed.id_second = feed.next_second;
+            look_up(k + 32u + lane);
+        }
+        const uint32_t t = feed.start + k * kStepTokens, mine = __shfl_sync(0xFFFFFFFFu, feed.id, k & 31u), second = __shfl_sync(0xFFFFFFFFu, feed.id_second, k & 31u);
+        if (lane == 0u) {
+            auto source = [&](uint32_t number) {
+                return number < pages ? feed.blocks + number * p.c.page_bytes + (t & (page - 1u)) / kBlockTokens * kBlockBytes : kNowhere.bytes;
+            };
+            const uint32_t bar = full0 + 8u * into, dst = ring0 + into * kUnitBytes;
+            if (!small_pages) {
+                sm100::mbar_arrive_expect_tx(bar, kUnitBytes);
+                bulk_load(dst, source(mine), kUnitBytes, bar);
+            } else {
+                const bool two = t + kBlockTokens < feed.length;
+                sm100::mbar_arrive_expect_tx(bar, two ? kUnitBytes : kBlockBytes);
+                bulk_load(dst, source(mine), kBlockBytes, bar);
+                if (two) bulk_load(dst + kBlockBytes, source(second), kBlockBytes, bar);
             }
-        };
-        auto issue = [&](uint32_t k, uint32_t into) {
-            if ((k & 31u) == 0u) {
-                id = next_id, id_second = next_second;
-                look_up(k + 32u + lane);
-            }
-            const uint32_t t = start + k * kStepTokens, mine = __shfl_sync(0xFFFFFFFFu, id, k & 31u), second = __shfl_sync(0xFFFFFFFFu, id_second, k & 31u);
-            if (lane == 0u) {
-                auto source = [&](uint32_t number) {
-                    return number < pages ? blocks + number * p.c.page_bytes + (t & (page - 1u)) / kBlockTokens * kBlockBytes : kNowhere.bytes;
-                };
-                const uint32_t bar = full0 + 8u * into, dst = ring0 + into * kUnitBytes;
-                if (!small_pages) {
-                    sm100::mbar_arrive_expect_tx(bar, kUnitBytes);
-                    bulk_load(dst, source(mine), kUnitBytes, bar);
-                } else {
-                    const bool two = t + kBlockTokens < length;
-                    sm100::mbar_arrive_expect_tx(bar, two ? kUnitBytes : kBlockBytes);
-                    bulk_load(dst, source(mine), kBlockBytes, bar);
-                    if (two) bulk_load(dst + kBlockBytes, source(second), kBlockBytes, bar);
-                }
-            }
-        };
+        }
+    };
+    // the first copies of a segment, into a ring that the warp has emptied
+    const auto open = [&](const Segment& seg) {
+        feed.length = length_of(p.c, seg.b);
+        feed.row_of_table = p.c.table + static_cast<size_t>(seg.b) * p.c.table_width;
+        feed.blocks = p.c.pool + static_cast<uint64_t>(seg.head) * (page / kBlockTokens) * kBlockBytes;
+        feed.start = seg.first * kStepTokens + warp * kUnit;
+        const uint32_t stop = min(feed.length, (seg.first + seg.steps) * kStepTokens);
+        feed.units = feed.start < stop ? (stop - feed.start + kStepTokens - 1u) / kStepTokens : 0u;
+        feed.id = feed.id_second = feed.next_id = feed.next_second = -1;
         look_up(lane);
 #pragma unroll 1
-        for (uint32_t k = 0; k < kStages && k < units; ++k) issue(k, (stage + k) % kStages);
+        for (uint32_t k = 0; k < kStages && k < feed.units; ++k) issue(k, (stage + k) % kStages);
+    };
+
+    Segment coming;
+    bool have = next(coming);
+    if (have) open(coming);
+    while (have) {
+        const Segment seg = coming;
+        const uint32_t b = seg.b, head = seg.head, row0 = seg.row0, first = seg.first, start = feed.start, units = feed.units, length = feed.length;
+        const uint32_t n_rows = count_of(p.counts, b, p.S, length);
         QueryRows<NT> x;
         x.away = sh.away;
         load_rows<NT>(x, sh.q, p, b, head, row0, length, n_rows);
@@ -414,8 +432,10 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) kv8_attend_kernel(c
             if (++stage == kStages) stage = 0u, phase ^= 1u;
         }
         if (!ok && lane == 0u) atomicOr(p.status, 1u);
+        // the next segment's first copies are under way while this one's sums come together
+        have = ok && next(coming);
+        if (have) open(coming);
 
-        // the warps' sums of the item come together
 #pragma unroll
         for (int g = 0; g < NT; ++g) {
 #pragma unroll
@@ -433,31 +453,42 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) kv8_attend_kernel(c
         float* part = slot_of(p.ws, gridDim.x, blockIdx.x, slot, 8u * NT);
 #pragma unroll
         for (int g = 0; g < NT; ++g) {
-            float* mine_o = reinterpret_cast<float*>(sh.ring[warp][0]);   // [8 rows][128], the ring is empty
+            // warps 2 and 3 hand their O, relative to the item's reference, to 0 and 1, which leave the sums there
+            float* sums = sh.o[warp & 1u];   // [8 rows][128]
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                const int row = 8 * g + 2 * static_cast<int>(tig) + j;
-                const float top = fmaxf(fmaxf(sh.m[0][row], sh.m[1][row]), fmaxf(sh.m[2][row], sh.m[3][row]));
-                const float f = ex2(m[g][j] - top);
+            for (uint32_t turn = 0; turn < 2u; ++turn) {
+                if ((warp >> 1) != turn) {
 #pragma unroll
-                for (uint32_t i = 0; i < 4; ++i) {
-                    *reinterpret_cast<float4*>(mine_o + (2u * tig + j) * 128u + 16u * gid + 4u * i) =
-                        make_float4(o[g][2 * i][j] * f, o[g][2 * i][2 + j] * f, o[g][2 * i + 1][j] * f, o[g][2 * i + 1][2 + j] * f);
+                    for (int j = 0; j < 2; ++j) {
+                        const int row = 8 * g + 2 * static_cast<int>(tig) + j;
+                        const float top = fmaxf(fmaxf(sh.m[0][row], sh.m[1][row]), fmaxf(sh.m[2][row], sh.m[3][row]));
+                        const float f = ex2(m[g][j] - top);
+#pragma unroll
+                        for (uint32_t i = 0; i < 4; ++i) {
+                            // (pieces of 16 bytes change places within a row, so that the lanes of a column meet different banks)
+                            float4* at = reinterpret_cast<float4*>(sums + (2u * tig + j) * 128u) + ((4u * gid + i) ^ ((2u * tig + j) & 7u));
+                            float4 v = make_float4(o[g][2 * i][j] * f, o[g][2 * i][2 + j] * f, o[g][2 * i + 1][j] * f, o[g][2 * i + 1][2 + j] * f);
+                            if (turn == 1u) {
+                                const float4 more = *at;
+                                v.x += more.x, v.y += more.y, v.z += more.z, v.w += more.w;
+                            }
+                            *at = v;
+                        }
+                    }
                 }
+                __syncthreads();
             }
-            __syncthreads();
             {
                 const uint32_t r = threadIdx.x >> 4, d = (threadIdx.x & 15u) * 8u, row = row0 + 8u * g + r;
                 const float top = fmaxf(fmaxf(sh.m[0][8 * g + r], sh.m[1][8 * g + r]), fmaxf(sh.m[2][8 * g + r], sh.m[3][8 * g + r]));
                 float total = 0.0f, acc[8];
 #pragma unroll
-                for (int k = 0; k < 8; ++k) acc[k] = 0.0f;
+                for (unsigned w = 0; w < kWarps; ++w) total = fmaf(sh.l[w][8 * g + r], ex2(sh.m[w][8 * g + r] - top), total);
 #pragma unroll
-                for (unsigned w = 0; w < kWarps; ++w) {
-                    total = fmaf(sh.l[w][8 * g + r], ex2(sh.m[w][8 * g + r] - top), total);
-                    const float4* src = reinterpret_cast<const float4*>(reinterpret_cast<const float*>(sh.ring[w][0]) + r * 128u + d);
-                    const float4 a = src[0], c = src[1];
-                    acc[0] += a.x, acc[1] += a.y, acc[2] += a.z, acc[3] += a.w, acc[4] += c.x, acc[5] += c.y, acc[6] += c.z, acc[7] += c.w;
+                for (uint32_t y = 0; y < 2u; ++y) {
+                    const uint32_t piece = (2u * (threadIdx.x & 15u) + y) ^ (r & 7u);
+                    const float4 a = reinterpret_cast<const float4*>(sh.o[0] + r * 128u)[piece], c = reinterpret_cast<const float4*>(sh.o[1] + r * 128u)[piece];
+                    acc[4 * y] = a.x + c.x, acc[4 * y + 1] = a.y + c.y, acc[4 * y + 2] = a.z + c.z, acc[4 * y + 3] = a.w + c.w;
                 }
                 if (row < p.S * p.group) {
                     if (whole) {
@@ -477,9 +508,6 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) kv8_attend_kernel(c
             }
             __syncthreads();
         }
-        // what the generic proxy read and wrote in the ring is behind the next copies into it
-        sm100::fence_proxy_async_smem();
-        __syncwarp();
     }
     // after a failure: no copy may land in shared memory that is another CTA's by then. (A copy that was issued ends by itself; the wait for it has a limit.)
     if (sh.failed != 0u) {

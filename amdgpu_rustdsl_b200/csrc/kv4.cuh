@@ -51,9 +51,10 @@ cudaError_t launch_kv4_append(const Kv4View& c, const Kv4Rows& k, const Kv4Rows&
 cudaError_t launch_kv4_read(const Kv4View& c, const Kv4Rows& k, const Kv4Rows& v, uint32_t S, bool last, const int32_t* counts, cudaStream_t stream);
 uint64_t kv4_attend_workspace(const Kv4View& c, uint32_t S, uint32_t H, bool weights, bool lse);
 cudaError_t launch_kv4_attend(const Kv4AttendParams& p, cudaStream_t stream);
-// kv4_attend.cu: puts the items together that several CTAs worked on, of the 8-bit cache too
+// kv4_attend.cu: puts the items together that several CTAs worked on, of the 8-bit cache too. together: items of many parts have a CTA for each row, whose sums are added up in another order than
+// by a warp a row, the 4-bit cache's
 cudaError_t launch_combine_few(const Kv4AttendParams& p, uint32_t slots, uint32_t grid, cudaStream_t stream);
-cudaError_t launch_combine_many(const Kv4AttendParams& p, uint32_t per, uint32_t row_tiles, uint32_t grid, cudaStream_t stream);
+cudaError_t launch_combine_many(const Kv4AttendParams& p, uint32_t per, uint32_t row_tiles, uint32_t grid, cudaStream_t stream, bool together = false);
 // kv4_weigh.cu: the attention weights, from p.lse and, if there, p.scores
 cudaError_t launch_kv4_weigh(const Kv4AttendParams& p, cudaStream_t stream);
 // kv4_prefill.cu: one CTA per SM, items of kv4_prefill_rows() query rows, partials in p.ws as the decode kernels leave them

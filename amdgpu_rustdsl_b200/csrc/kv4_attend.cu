@@ -580,6 +580,55 @@ __global__ void __launch_bounds__(kTogether ? 32 * kTogether : 256) kv4_combine_
     if (p.lse != nullptr && lane == 0u) p.lse[(static_cast<size_t>(b) * p.H + h) * p.S + i] = none ? -INFINITY : (m + lg2(l)) * kLn2;
 }
 
+// The same for items of many rows that a few CTAs each have a part of: a warp has kRows rows, whose parts come in together, one CTA's behind the other's, in the same order and to the same bits.
+// (A warp a row took as many rounds of CTAs, each as long as three trips to memory one behind the other: prompts of 4096 rows, 8-bit cache, 459 us and 456 so, 4 ragged chunks of 333 rows 69.7 and
+// 68.4; 2, 4 and 8 rows a warp are alike. Bound by the trips, then by L2.)
+template <uint32_t kRows>
+__global__ void __launch_bounds__(256) kv4_combine_rows_kernel(const __grid_constant__ Kv4AttendParams p, uint32_t rows, uint32_t row_tiles, uint32_t grid) {
+    pdl_launch();
+    pdl_wait();
+    const uint32_t lane = threadIdx.x & 31u, r0 = (blockIdx.y * 8u + (threadIdx.x >> 5)) * kRows;
+    const uint4 begun = ld_v4(begun_at(p.ws, blockIdx.x));
+    const uint32_t entry = begun.x / p.c.HK, head = begun.x - entry * p.c.HK, b = entry / row_tiles, row0 = (entry - b * row_tiles) * rows + r0, from = begun.y, last = begun.z;
+    if (last == from || row0 >= p.S * p.group) return;
+    const uint32_t live = count_of(p.counts, b, p.S, length_of(p.c, b)) * p.group;   // rows that see something
+    float m[kRows], l[kRows];
+    float4 o[kRows];
+#pragma unroll
+    for (uint32_t y = 0; y < kRows; ++y) m[y] = kLowest, l[y] = 0.0f, o[y] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 1
+    for (uint32_t w = from; w <= last; ++w) {
+        const float* src = slot_of(p.ws, grid, w, w == from ? 1u : 0u, rows);
+        float pm[kRows], pl[kRows];
+        uint4 raw[kRows];
+#pragma unroll
+        for (uint32_t y = 0; y < kRows; ++y) {
+            pm[y] = kLowest, pl[y] = 0.0f, raw[y] = make_uint4(0u, 0u, 0u, 0u);
+            if (row0 + y < live) {
+                pm[y] = ld_f32(src + rows * 128u + 2u * (r0 + y)), pl[y] = ld_f32(src + rows * 128u + 2u * (r0 + y) + 1u);
+                raw[y] = ld_v4(src + (r0 + y) * 128u + 4u * lane);
+            }
+        }
+#pragma unroll
+        for (uint32_t y = 0; y < kRows; ++y) {
+            const float top = fmaxf(m[y], pm[y]), a = ex2(m[y] - top), c = ex2(pm[y] - top);
+            m[y] = top;
+            l[y] = fmaf(l[y], a, pl[y] * c);
+            o[y].x = fmaf(o[y].x, a, __uint_as_float(raw[y].x) * c), o[y].y = fmaf(o[y].y, a, __uint_as_float(raw[y].y) * c);
+            o[y].z = fmaf(o[y].z, a, __uint_as_float(raw[y].z) * c), o[y].w = fmaf(o[y].w, a, __uint_as_float(raw[y].w) * c);
+        }
+    }
+#pragma unroll
+    for (uint32_t y = 0; y < kRows; ++y) {
+        const uint32_t row = row0 + y, i = row / p.group, h = head * p.group + row - i * p.group;
+        if (row >= p.S * p.group || r0 + y >= rows) break;
+        const bool none = l[y] == 0.0f;
+        const float inv = none ? 0.0f : 1.0f / l[y];
+        *reinterpret_cast<uint2*>(p.out + ((static_cast<size_t>(b) * p.S + i) * p.H + h) * 128u + 4u * lane) = make_uint2(pack_bf16x2(o[y].x * inv, o[y].y * inv), pack_bf16x2(o[y].z * inv, o[y].w * inv));
+        if (p.lse != nullptr && lane == 0u) p.lse[(static_cast<size_t>(b) * p.H + h) * p.S + i] = none ? -INFINITY : (m[y] + lg2(l[y])) * kLn2;
+    }
+}
+
 }  // namespace
 
 // what a launch of `grid` CTAs with items of `slots` rows (8 to 32, one row tile a sequence) or of `per` rows left in p.ws
@@ -589,9 +638,14 @@ cudaError_t launch_combine_few(const Kv4AttendParams& p, uint32_t slots, uint32_
     if (grid / entries > 16u) return kv4_launch(kv4_combine_kernel<16>, dim3(entries, some), 512u, 0, stream, p, slots, 1u, grid);
     return kv4_launch(kv4_combine_kernel<4>, dim3(entries, some), 128u, 0, stream, p, slots, 1u, grid);
 }
-cudaError_t launch_combine_many(const Kv4AttendParams& p, uint32_t per, uint32_t row_tiles, uint32_t grid, cudaStream_t stream) {
-    const uint32_t rows = p.S * p.group, most = rows < per ? rows : per;
-    return kv4_launch(kv4_combine_kernel<0>, dim3(begun_entries(p.c, row_tiles, grid), (most + 7u) / 8u), 256u, 0, stream, p, per, row_tiles, grid);
+cudaError_t launch_combine_many(const Kv4AttendParams& p, uint32_t per, uint32_t row_tiles, uint32_t grid, cudaStream_t stream, bool together) {
+    constexpr uint32_t kRows = 4;
+    const uint32_t rows = p.S * p.group, most = rows < per ? rows : per, entries = begun_entries(p.c, row_tiles, grid), parts = grid / entries;
+    // up to 6 parts an item one behind the other (4 parts of 333 rows: 81.4 us, 85.5 with a CTA a row; 6 parts alike; 9 parts 60 and 54, 148 parts 69 and 34)
+    if (parts <= 6u) return kv4_launch(kv4_combine_rows_kernel<kRows>, dim3(entries, (most + 8u * kRows - 1u) / (8u * kRows)), 256u, 0, stream, p, per, row_tiles, grid);
+    if (!together) return kv4_launch(kv4_combine_kernel<0>, dim3(entries, (most + 7u) / 8u), 256u, 0, stream, p, per, row_tiles, grid);
+    if (parts > 16u) return kv4_launch(kv4_combine_kernel<16>, dim3(entries, most), 512u, 0, stream, p, per, row_tiles, grid);
+    return kv4_launch(kv4_combine_kernel<4>, dim3(entries, most), 128u, 0, stream, p, per, row_tiles, grid);
 }
 
 namespace {

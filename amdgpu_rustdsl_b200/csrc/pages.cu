@@ -281,6 +281,8 @@ int fmha_pages_take(const fmha_pages* pages, const int32_t* counts, int32_t* gra
     if (S == 0u) positions = nullptr, slots = nullptr;
     const bool maps = positions != nullptr || slots != nullptr;
     if (maps && static_cast<uint64_t>(p.B) * S > kMostRows) return refuse(err, cap, "take: more than 2^30 rows");
+    // (a page's tokens for each free page, and what fits the pages that the sequences have)
+    if (starts != nullptr && (static_cast<uint64_t>(p.pages) + p.B) << p.page_log2 > 0x7FFFFFFFull) return refuse(err, cap, "take: starts of up to 2^31 tokens and more");
     const uint64_t rows = maps ? static_cast<uint64_t>(p.B) * S : 0u;
     const Span s[] = {{granted, 4ull * p.B, "granted"}, {positions, (positions_64 ? 8u : 4u) * rows, "positions"}, {slots, 8u * rows, "slots"}, {starts, 4ull * (p.B + 1ull), "starts"}, {counts, 4ull * p.B, "counts"},
                       {p.free, 4ull * (p.pages + 4ull), "the stack"}, {p.table, 4ull * p.B * p.table_width, "the table"}, {p.lengths, 4ull * p.B, "the lengths"}};

@@ -39,9 +39,10 @@ def pages_take(free, cache, counts, granted, *, positions=None, slots=None, star
     in front of it are more than are free.
 
     granted    int32 [B]: counts[b] or 0; what ``kv8_append`` and the attention take as ``counts``
-    positions  int32 or int64 [B, S]: of row i < granted[b] the token it becomes, the length before plus i; -1 in other rows
+    positions  int32 or int64 [B, S]: of row i < granted[b] the token it becomes, the length before plus i; -1 in other rows. (``counts`` may go beyond S, the rows do not: tokens without a row are
+               whoever writes them's to look after)
     slots      int64 [B, S]: page number times tokens of a page, plus the place within it, of that token; -1 in other rows
-    starts     int32 [B + 1]: the sums of granted in front of each sequence, and of all
+    starts     int32 [B + 1]: the sums of granted in front of each sequence, and of all; for stacks of less than 2^31 tokens
     """
     import torch
     lib = _abi.load()

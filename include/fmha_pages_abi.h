@@ -31,7 +31,8 @@ typedef struct fmha_pages {
  *   aside) are more than are free. granted[b] = counts[b] or 0; the new pages go from the stack to the table, in order; lengths[b] grows by granted[b].
  *   positions: NULL or int32 [B][S] (int64 with positions_64): of row i < granted[b] the token it becomes, length (before) + i; -1 in other rows.
  *   slots: NULL or int64 [B][S]: page * (tokens of a page) + place within the page of that token; -1 in other rows and where the table names no page.
- *   starts: NULL or int32 [B + 1]: sums of granted in front of each sequence, and of all.
+ *     (Rows are all that the maps have: a sequence may be granted more than S tokens.)
+ *   starts: NULL or int32 [B + 1]: sums of granted in front of each sequence, and of all. (pages + B) * page is below 2^31 then.
  *   granted, positions, slots and starts share no memory with counts, the stack, the table, the lengths or one another.
  * cut: lengths[b] becomes min(length, max(keep[b], 0)); pages without tokens go back to the stack, their table entries become -1. The last sequence's last page goes onto it first: a cut
  *   to the lengths before a take leaves stack, table and lengths as they were before it. Pages that the stack has no room for are dropped. keep shares no memory with the others.

@@ -60,3 +60,11 @@ def test_only_caches_have_pages():
     for call in (lambda: pages_take(pages_stack(3, device="cpu"), one, one, one), lambda: pages_cut(pages_stack(3, device="cpu"), None, one)):
         with pytest.raises(ValueError, match="Kv4Cache or a Kv8Cache"):
             call()
+
+
+def test_starts_that_do_not_fit_are_refused(abi):
+    """Sums of granted tokens are 32 bits: a stack of 2^27 pages of 16 tokens is too many for them (and is taken without starts: the refusal is the next one)."""
+    rc, err = _take(abi, _pages(abi, pages=1 << 27, free=1 << 40), starts=8 * FAKE)
+    assert rc == 6 and "starts" in err
+    rc, err = _take(abi, _pages(abi, pages=1 << 27, free=1 << 40), starts=None, S=1 << 29)
+    assert rc == 6 and "2^30 rows" in err

@@ -75,14 +75,15 @@ def _rows(who, name, x, cache, S=None, heads=None):
     """bf16 [B, S, heads, 128] with a dense last dimension as the C struct."""
     import torch
     shape = x.shape
-    if x.dtype != torch.bfloat16 or len(shape) != 4 or shape[0] != cache.B or shape[3] != D or (S is not None and shape[1] != S) or (heads is not None and shape[2] != heads):
+    b, s, h, d = shape if len(shape) == 4 else (0, 0, 0, 0)
+    if x.dtype != torch.bfloat16 or b != cache.B or d != D or (S is not None and s != S) or (heads is not None and h != heads):
         raise ValueError(f"{who}: {name} must be bf16 [{cache.B}, {'S' if S is None else S}, {'H' if heads is None else heads}, 128], not {x.dtype} {tuple(shape)}")
     sb, ss, sh, sd = x.stride()
     ptr = x.data_ptr()
     if x.device != cache.device or sd != 1 or (sb | ss | sh) & 7 or ptr & 15:
         raise ValueError(f"{who}: {name} must be on the cache's device, its last dimension dense, its start and its strides multiples of 16 bytes")
-    if shape[1] > 0x7FFFFFFF:   # (a stride of 0 makes as many rows as you like; the library counts them in 32 bits)
-        raise ValueError(f"{who}: {name} has {shape[1]} rows, more than 2^31")
+    if s > 0x7FFFFFFF:   # (a stride of 0 makes as many rows as you like; the library counts them in 32 bits)
+        raise ValueError(f"{who}: {name} has {s} rows, more than 2^31")
     return _abi.Kv4Rows(ptr, sb, ss, sh)
 
 
@@ -90,7 +91,7 @@ def _i32(who, name, x, cache, shape):
     import torch
     if x is None:
         return None
-    if x.dtype != torch.int32 or tuple(x.shape) != shape or x.device != cache.device or not x.is_contiguous():
+    if x.dtype != torch.int32 or x.shape != shape or x.device != cache.device or not x.is_contiguous():
         raise ValueError(f"{who}: {name} must be a contiguous int32 tensor of shape {shape} on the cache's device")
     return x.data_ptr()
 

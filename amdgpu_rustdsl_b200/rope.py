@@ -21,7 +21,7 @@ from .ops import _raw_stream
 # 2 pi to 40 digits, of which 64-bit phases need 20
 _TWO_PI = Fraction(62831853071795864769252867665590057683943, 10 ** 40)
 MAX_HEAD_DIM = 512
-_NO_ROWS = (0,) * 8
+_NO_ROWS, _NO_STRIDES = (0,) * 8, (0,) * 4
 _ARGS = struct.Struct("@20q10If4x").pack
 assert struct.calcsize("@20q10If4x") == C.sizeof(_abi.RopeArgs)
 _kinds, _entry = {}, None
@@ -125,8 +125,8 @@ class Rope:
 
 def _rope_rows(name, x, rope, like):
     """(address, strides) of x, [B, S, heads, head size] of like's type and sizes but for the heads."""
-    shape, (sb, ss, sh, sd) = x.shape, x.stride()
-    if x.dtype != like.dtype or shape[0] != like.shape[0] or shape[1] != like.shape[1] or shape[3] != like.shape[3]:
+    shape, other, (sb, ss, sh, sd) = x.shape, like.shape, x.stride()
+    if x.dtype != like.dtype or shape[:2] != other[:2] or shape[3] != other[3]:
         raise ValueError(f"rope_rotate: {name} must have x's type, sequences, rows and head size")
     if x.get_device() != rope.index or (sd != 1 and shape[3] > 1):
         raise ValueError(f"rope_rotate: {name} must be on the Rope's device, its last dimension dense")
@@ -141,48 +141,59 @@ def rope_rotate(rope, x, positions, out=None, *, y=None, y_out=None, backward=Fa
     backward   the transposed matrix: x is the gradient of the results, and out becomes the gradient of what went in
     """
     import torch
-    kind = _types(torch).get(x.dtype)
+    dtype, shape, index = x.dtype, x.shape, rope.index
+    kind = _types(torch).get(dtype)
     if kind is None:
-        raise ValueError(f"rope_rotate: x must be bf16, f16 or f32, not {x.dtype}")
-    if x.dim() != 4 or not rope.rotary <= x.shape[3] <= MAX_HEAD_DIM:
-        raise ValueError(f"rope_rotate: x must be [B, S, heads, {rope.rotary} to {MAX_HEAD_DIM}], not {tuple(x.shape)}")
-    B, S, H, head = x.shape
+        raise ValueError(f"rope_rotate: x must be bf16, f16 or f32, not {dtype}")
+    if len(shape) != 4 or not rope.rotary <= shape[3] <= MAX_HEAD_DIM:
+        raise ValueError(f"rope_rotate: x must be [B, S, heads, {rope.rotary} to {MAX_HEAD_DIM}], not {tuple(shape)}")
+    B, S, H, head = shape
     rows = _rope_rows("x", x, rope, x)
     rows_out, heads_y, more = rows, 0, _NO_ROWS
     if out is None:
         out = x
     elif out is not x:
-        if out.dim() != 4 or out.shape[2] != H:
-            raise ValueError("rope_rotate: out must have x's heads")
-        rows_out = _rope_rows("out", out, rope, x)
+        sb, ss, sh, sd = out.stride() if out.shape == shape else _NO_STRIDES
+        if sd == 1 and out.dtype == dtype and out.get_device() == index:   # (as a rule, and the quickest way to know)
+            rows_out = out.data_ptr(), sb, ss, sh
+        else:
+            if out.dim() != 4 or out.shape[2] != H:
+                raise ValueError("rope_rotate: out must have x's heads")
+            rows_out = _rope_rows("out", out, rope, x)
     if y is not None:
-        if y.dim() != 4:
+        shape_y = y.shape
+        if len(shape_y) != 4:
             raise ValueError("rope_rotate: y must have x's type, sequences, rows and head size")
-        heads_y, first = y.shape[2], _rope_rows("y", y, rope, x)
+        heads_y, first = shape_y[2], _rope_rows("y", y, rope, x)
         if y_out is None or y_out is y:
             more = first + first
         else:
-            if y_out.dim() != 4 or y_out.shape[2] != heads_y:
-                raise ValueError("rope_rotate: y_out must have y's heads")
-            more = first + _rope_rows("y_out", y_out, rope, x)
+            sb, ss, sh, sd = y_out.stride() if y_out.shape == shape_y else _NO_STRIDES
+            if sd == 1 and y_out.dtype == dtype and y_out.get_device() == index:
+                more = first + (y_out.data_ptr(), sb, ss, sh)
+            else:
+                if y_out.dim() != 4 or y_out.shape[2] != heads_y:
+                    raise ValueError("rope_rotate: y_out must have y's heads")
+                more = first + _rope_rows("y_out", y_out, rope, x)
     elif y_out is not None:
         raise ValueError("rope_rotate: y_out without y")
     wide = positions.dtype == torch.int64
-    if not (wide or positions.dtype == torch.int32) or tuple(positions.shape) != (B, S) or positions.get_device() != rope.index:
+    if not (wide or positions.dtype == torch.int32) or positions.shape != (B, S) or positions.get_device() != index:
         raise ValueError(f"rope_rotate: positions must be int32 or int64 of shape {(B, S)} on the Rope's device")
-    if B * S > 1 << 30 or H > 1 << 30 or heads_y > 1 << 30:   # (here, in numbers of any size: the struct's have 32 bits)
+    tokens = B * S
+    if tokens > 1 << 30 or H > 1 << 30 or heads_y > 1 << 30:   # (here, in numbers of any size: the struct's have 32 bits)
         raise ValueError("rope_rotate: more than 2^30 tokens or heads")
-    if B * S == 0 or H + heads_y == 0:
+    if tokens == 0 or H + heads_y == 0:
         return out
     if H == 0:   # only y has heads
         rows, rows_out, more, H, heads_y = more[:4], more[4:], _NO_ROWS, heads_y, 0
-    if rope.index < 0:
+    if index < 0:
         raise ValueError("rope_rotate: the Rope must be on a CUDA device")
     # fmha_rope_args, as bytes: an eighth of the time that setting the fields one by one takes
     args = _ARGS(*rows, *rows_out, *more, rope.address, positions.data_ptr(), *positions.stride(), wide, B, S, H, heads_y, head, rope.rotary, kind, rope.interleaved, bool(backward), rope.factor)
     raw = stream if stream is not None else _raw_stream(torch, rope.device)
     rotate = _entry or _load()
-    if torch.cuda.current_device() == rope.index:
+    if torch.cuda.current_device() == index:
         rc = rotate(args, raw, _errors.text, 256)
     else:
         with torch.cuda.device(rope.device):

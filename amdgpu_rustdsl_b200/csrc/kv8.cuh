@@ -34,6 +34,11 @@ __device__ __forceinline__ uint8_t* block_of(const Kv4View& c, long long page, u
 __device__ __forceinline__ uint32_t k_swap(uint32_t t) { return t & 7u; }
 __device__ __forceinline__ uint32_t v_swap(uint32_t pair) { return (pair & 1u) | ((pair & 2u) << 1); }
 
+__device__ __forceinline__ uint2 ld_v2(const void* p) {
+    uint2 v;
+    asm volatile("ld.global.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
+    return v;
+}
 // two e4m3 codes of a word, the lower or the upper half, as f16
 __device__ __forceinline__ uint32_t e4m3x2_lo(uint32_t w) {
     uint32_t r;

@@ -4,7 +4,8 @@
 //   scale = 2^max(ceil(log2(amax / 448)), -90),   code = e4m3_rne_sat(x / scale),   value = code * scale;   a block that had tokens keeps a larger scale, or its codes move to the new one
 //
 // A warp has a block's K or its V: 16 tokens of 128 elements are 8 loads of 16 bytes a lane (half a warp a token), all in flight together, and stay in registers between the largest
-// element and the rounding. Bound by bytes (6 a bf16 pair and its code) where there are many blocks, by the chain length -> page -> block -> store where there is one.
+// element and the rounding. Where there is one block the chain length -> page -> block -> store is what takes the time (64 x 1 tokens of 8 heads: append 3.7 us, read 2.4 of the device), where there
+// are many the chain's few rounds of warps and bytes: 8 ragged prompts of up to 1337 tokens of 8 heads, append 7.6 us for 22 MB, read 8.8 for 51 MB (5.8 TB/s, 0.89 of the copy rate).
 #include "kv8.cuh"
 
 namespace b200mx {
@@ -35,7 +36,10 @@ __device__ __forceinline__ uint32_t pair_bytes(bool even, bool odd) { return (ev
 // codes times a power of two (f16, twice), rounded again
 __device__ __forceinline__ uint32_t shrink(uint32_t codes, uint32_t factor) { return e4m3x4_of_f16(mul_f16x2(e4m3x2_lo(codes), factor), mul_f16x2(e4m3x2_hi(codes), factor)); }
 
-__global__ void __launch_bounds__(kThreads) kv8_append_kernel(const __grid_constant__ StoreParams p) {
+// kCtas: that an SM is to have room for. Many blocks take 4 (8 ragged prompts of up to 1337 tokens, read back after: 18.0 us in place of 19.6 with 2, whose next launch finds less room to begin in); few
+// are quicker with 2 and the registers to have all loads in flight (64 x 1 tokens: 3.7 us of the device in place of 4.3)
+template <int kCtas>
+__global__ void __launch_bounds__(kThreads, kCtas) kv8_append_kernel(const __grid_constant__ StoreParams p) {
     pdl_launch();
     pdl_wait();
     const uint32_t lane = threadIdx.x & 31u, piece = lane & 15u, odd = lane >> 4;
@@ -128,52 +132,54 @@ __device__ __forceinline__ uint32_t value_pair(uint32_t two, unsigned long long 
     return pack_bf16x2(lo, hi);
 }
 
-// Half a warp a row, a warp kRows rows of one head, K and V
-constexpr uint32_t kRows = 8;
-__global__ void __launch_bounds__(kThreads) kv8_read_kernel(const __grid_constant__ StoreParams p) {
+// A warp has a block's K or its V as kv8_append does, of which it gives back the rows that are asked for; half a warp a row
+__global__ void __launch_bounds__(kThreads, 4) kv8_read_kernel(const __grid_constant__ StoreParams p) {
     pdl_launch();
     pdl_wait();
     const uint32_t lane = threadIdx.x & 31u, piece = lane & 15u, odd = lane >> 4;
-    const uint32_t unit = blockIdx.x * kWarps + (threadIdx.x >> 5), group = unit / p.c.HK, head = unit - group * p.c.HK;
+    const uint32_t unit = blockIdx.x * kWarps + (threadIdx.x >> 5), part = unit / p.c.HK, head = unit - part * p.c.HK, nth = part >> 1;
+    const bool is_v = part & 1u;
     for (uint32_t b = blockIdx.y; b < p.c.B; b += gridDim.y) {
-        const uint32_t L = length_of(p.c, b), n = p.last ? count_of(p.counts, b, p.S, L) : min(p.S, L), t0 = p.last ? L - n : 0u;
-        uint2 k[kRows / 2];
-        uint4 v[kRows / 2], meta[kRows / 2];
-        long long page[kRows / 2];
+        const uint32_t L = length_of(p.c, b), n = p.last ? count_of(p.counts, b, p.S, L) : min(p.S, L), t0 = p.last ? L - n : 0u, base = (t0 / kBlockTokens + nth) * kBlockTokens;
+        if (base >= t0 + p.S) continue;
+        const uint32_t stop = t0 + n;   // rows from there on stand for nothing
+        const long long page = base < stop ? page_of(p.c, b, base) : -1;
+        uint4 codes[4];   // V: of a pair of tokens, 8 elements; K: of two tokens, 8 elements each
+        uint32_t scale_bits = 0, mask = base < stop ? 0xFFFFu : 0u;   // (tokens of a page that the pool does not have are without numbers)
 #pragma unroll
-        for (uint32_t x = 0; x < kRows / 2; ++x) {
-            const uint32_t i = group * kRows + 2u * x + odd;
-            page[x] = i < n ? page_of(p.c, b, t0 + i) : -1;
-        }
+        for (uint32_t i = 0; i < 4u; ++i) codes[i] = make_uint4(0u, 0u, 0u, 0u);
+        if (page >= 0) {
+            const uint8_t* block = block_of(p.c, page, head, base);
 #pragma unroll
-        for (uint32_t x = 0; x < kRows / 2; ++x) {
-            const uint32_t i = group * kRows + 2u * x + odd, t = t0 + i, in = t % kBlockTokens, pair = in >> 1;
-            k[x] = make_uint2(0u, 0u), v[x] = meta[x] = make_uint4(0u, 0u, 0u, 0u);
-            if (page[x] >= 0) {
-                const uint8_t* block = block_of(p.c, page[x], head, t);
-                const uint8_t* at = block + 128u * in + 16u * ((piece >> 1) ^ k_swap(in)) + 8u * (piece & 1u);
-                k[x] = make_uint2(ld_u32(at), ld_u32(at + 4));
-                v[x] = ld_v4(block + kVCodes + 256u * pair + 16u * (piece ^ v_swap(pair)));
-                meta[x] = ld_v4(block + kMeta);
+            for (uint32_t i = 0; i < 4u; ++i) {
+                if (is_v) {
+                    const uint32_t pair = 2u * i + odd;
+                    codes[i] = ld_v4(block + kVCodes + 256u * pair + 16u * (piece ^ v_swap(pair)));
+                } else {
+                    const uint32_t t = 4u * i + odd;
+                    const uint2 x = ld_v2(block + 128u * t + 16u * ((piece >> 1) ^ k_swap(t)) + 8u * (piece & 1u)), y = ld_v2(block + 128u * (t + 2u) + 16u * ((piece >> 1) ^ k_swap(t + 2u)) + 8u * (piece & 1u));
+                    codes[i] = make_uint4(x.x, x.y, y.x, y.y);
+                }
             }
+            const uint4 meta = ld_v4(block + kMeta);
+            scale_bits = is_v ? meta.y : meta.x, mask = is_v ? meta.z >> 16 : meta.z;
         }
+        const Kv4Rows& rows = is_v ? p.v : p.k;
+        uint8_t* to = rows.data + b * rows.stride_b + head * rows.stride_h + 16u * piece;
+        unsigned long long scale;
+        asm("mov.b64 %0, {%1, %1};" : "=l"(scale) : "r"(scale_bits));
 #pragma unroll
-        for (uint32_t x = 0; x < kRows / 2; ++x) {
-            const uint32_t i = group * kRows + 2u * x + odd, in = (t0 + i) % kBlockTokens;
-            if (i >= p.S) continue;
-            const bool lost = i < n && page[x] < 0;   // (a row that stands for nothing: codes of 0 times 0)
-            const uint32_t pick = in & 1u ? 0x7531u : 0x6420u;
-            const uint32_t words[2][2] = {{k[x].x, k[x].y}, {__byte_perm(v[x].x, v[x].y, pick), __byte_perm(v[x].z, v[x].w, pick)}};
-#pragma unroll
-            for (int part = 0; part < 2; ++part) {
-                const Kv4Rows& rows = part ? p.v : p.k;
-                unsigned long long scale;
-                asm("mov.b64 %0, {%1, %1};" : "=l"(scale) : "r"(part ? meta[x].y : meta[x].x));
-                const uint32_t w0 = words[part][0], w1 = words[part][1];
-                uint4 out = make_uint4(value_pair(e4m3x2_lo(w0), scale), value_pair(e4m3x2_hi(w0), scale), value_pair(e4m3x2_lo(w1), scale), value_pair(e4m3x2_hi(w1), scale));
-                if (lost || (meta[x].z >> (16 * part + in) & 1u)) out = make_uint4(0x7FFF7FFFu, 0x7FFF7FFFu, 0x7FFF7FFFu, 0x7FFF7FFFu);
-                *reinterpret_cast<uint4*>(rows.data + b * rows.stride_b + static_cast<long long>(i) * rows.stride_s + head * rows.stride_h + 16u * piece) = out;
-            }
+        for (uint32_t i = 0; i < 8u; ++i) {
+            const uint4 c = codes[i >> 1];
+            // K: tokens 2 i and 2 i + 1 in the two halves of the warp; V: those of the pair i - i % 2 and the next, one after the other
+            const uint32_t t = is_v ? 4u * (i >> 1) + 2u * odd + (i & 1u) : 2u * i + odd, pick = i & 1u ? 0x7531u : 0x6420u;
+            const uint32_t w0 = is_v ? __byte_perm(c.x, c.y, pick) : i & 1u ? c.z : c.x, w1 = is_v ? __byte_perm(c.z, c.w, pick) : i & 1u ? c.w : c.y;
+            if (base + t < t0 || base + t >= t0 + p.S) continue;
+            const bool live = base + t < stop;
+            uint4 out = make_uint4(value_pair(e4m3x2_lo(w0), scale), value_pair(e4m3x2_hi(w0), scale), value_pair(e4m3x2_lo(w1), scale), value_pair(e4m3x2_hi(w1), scale));
+            if (mask >> t & 1u) out = make_uint4(0x7FFF7FFFu, 0x7FFF7FFFu, 0x7FFF7FFFu, 0x7FFF7FFFu);
+            if (!live) out = make_uint4(0u, 0u, 0u, 0u);
+            *reinterpret_cast<uint4*>(to + static_cast<long long>(base + t - t0) * rows.stride_s) = out;
         }
     }
 }
@@ -184,10 +190,12 @@ uint32_t grid_y(const Kv4View& c) { return c.B < 65535u ? c.B : 65535u; }
 
 cudaError_t launch_kv8_append(const Kv4View& c, const Kv4Rows& k, const Kv4Rows& v, uint32_t S, const int32_t* counts, cudaStream_t stream) {
     const uint32_t blocks = (S + 2u * kBlockTokens - 2u) / kBlockTokens, units = blocks * c.HK * 2u;   // blocks that S tokens may fall into
-    return kv4_launch(kv8_append_kernel, dim3((units + kWarps - 1u) / kWarps, grid_y(c)), kThreads, 0, stream, StoreParams{c, k, v, S, 1, counts});
+    const dim3 grid((units + kWarps - 1u) / kWarps, grid_y(c));
+    const StoreParams p{c, k, v, S, 1, counts};
+    return static_cast<uint64_t>(grid.x) * grid.y <= 2u * current_sm_count() ? kv4_launch(kv8_append_kernel<2>, grid, kThreads, 0, stream, p) : kv4_launch(kv8_append_kernel<4>, grid, kThreads, 0, stream, p);
 }
 cudaError_t launch_kv8_read(const Kv4View& c, const Kv4Rows& k, const Kv4Rows& v, uint32_t S, bool last, const int32_t* counts, cudaStream_t stream) {
-    const uint32_t units = (S + kRows - 1u) / kRows * c.HK;
+    const uint32_t units = (S + 2u * kBlockTokens - 2u) / kBlockTokens * c.HK * 2u;
     return kv4_launch(kv8_read_kernel, dim3((units + kWarps - 1u) / kWarps, grid_y(c)), kThreads, 0, stream, StoreParams{c, k, v, S, last ? 1 : 0, counts});
 }
 

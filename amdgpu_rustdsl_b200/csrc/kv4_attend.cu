@@ -641,8 +641,7 @@ cudaError_t launch_combine_few(const Kv4AttendParams& p, uint32_t slots, uint32_
 cudaError_t launch_combine_many(const Kv4AttendParams& p, uint32_t per, uint32_t row_tiles, uint32_t grid, cudaStream_t stream, bool together) {
     constexpr uint32_t kRows = 4;
     const uint32_t rows = p.S * p.group, most = rows < per ? rows : per, entries = begun_entries(p.c, row_tiles, grid), parts = grid / entries;
-    // up to 6 parts an item one behind the other (4 parts of 333 rows: 81.4 us, 85.5 with a CTA a row; 6 parts alike; 9 parts 60 and 54, 148 parts 69 and 34)
-    if (parts <= 6u) return kv4_launch(kv4_combine_rows_kernel<kRows>, dim3(entries, (most + 8u * kRows - 1u) / (8u * kRows)), 256u, 0, stream, p, per, row_tiles, grid);
+    if (few_parts(p.c, row_tiles, grid)) return kv4_launch(kv4_combine_rows_kernel<kRows>, dim3(entries, (most + 8u * kRows - 1u) / (8u * kRows)), 256u, 0, stream, p, per, row_tiles, grid);
     if (!together) return kv4_launch(kv4_combine_kernel<0>, dim3(entries, (most + 7u) / 8u), 256u, 0, stream, p, per, row_tiles, grid);
     if (parts > 16u) return kv4_launch(kv4_combine_kernel<16>, dim3(entries, most), 512u, 0, stream, p, per, row_tiles, grid);
     return kv4_launch(kv4_combine_kernel<4>, dim3(entries, most), 128u, 0, stream, p, per, row_tiles, grid);

@@ -117,6 +117,8 @@ struct Begun {
 // (4 items of 74 parts each: 28 us with the item's entries, 36 with an entry and a row of idle CTAs for each of the 296 CTAs; 192 items of up to 7 parts among 592 CTAs: 72.6 and 69.7)
 __host__ __device__ __forceinline__ bool begun_by_item(const Kv4View& c, uint32_t row_tiles, uint32_t grid) { return 4ull * c.B * c.HK * row_tiles <= grid; }
 __host__ __device__ __forceinline__ uint32_t begun_entries(const Kv4View& c, uint32_t row_tiles, uint32_t grid) { return begun_by_item(c, row_tiles, grid) ? c.B * c.HK * row_tiles : grid; }
+// Whether an item's parts are few, so that a warp goes over them one behind the other. (6 parts alike, 9 parts of 256 rows 60 us so and 54 with warps that share them)
+__host__ __device__ __forceinline__ bool few_parts(const Kv4View& c, uint32_t row_tiles, uint32_t grid) { return grid / begun_entries(c, row_tiles, grid) <= 6u; }
 __device__ __forceinline__ Begun* begun_at(float* ws, uint32_t x) { return reinterpret_cast<Begun*>(ws) + x; }
 // by one thread of a CTA: at its start, and for each segment
 template <uint32_t kTokens, uint32_t kExtra>

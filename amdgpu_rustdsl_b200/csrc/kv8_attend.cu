@@ -549,9 +549,58 @@ cudaError_t launch_rows(const Kv8AttendParams& p, cudaStream_t stream) {
     return e != cudaSuccess || whole ? e : launch_combine_few(p, 8u * NT, grid, stream);
 }
 
+// Puts the prefill kernel's items together that a few CTAs each have a part of, whose parts lie by columns: a warp has 32 rows, a lane's own, and 16 columns
+__global__ void __launch_bounds__(256) kv8_combine_columns_kernel(const __grid_constant__ Kv8AttendParams p, uint32_t rows, uint32_t row_tiles, uint32_t grid) {
+    pdl_launch();
+    pdl_wait();
+    const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5, r = blockIdx.y * 32u + lane;
+    const uint4 begun = ld_v4(begun_at(p.ws, blockIdx.x));
+    const uint32_t entry = begun.x / p.c.HK, head = begun.x - entry * p.c.HK, b = entry / row_tiles, row = (entry - b * row_tiles) * rows + r, from = begun.y, last = begun.z;
+    if (last == from || row >= p.S * p.group) return;
+    const uint32_t i = row / p.group, h = head * p.group + row - i * p.group;
+    const bool sees = i < count_of(p.counts, b, p.S, length_of(p.c, b));
+    float m = kLowest, l = 0.0f, o[16];
+#pragma unroll
+    for (int x = 0; x < 16; ++x) o[x] = 0.0f;
+    for (uint32_t w0 = from; sees && w0 <= last; w0 += 2u) {   // two parts in flight
+        uint2 ml[2];
+        uint4 raw[2][4];
+#pragma unroll
+        for (uint32_t k = 0; k < 2u; ++k) {
+            const uint32_t w = min(w0 + k, last);
+            const float* src = slot_of(p.ws, grid, w, w == from ? 1u : 0u, rows);
+            ml[k] = ld_v2(src + rows * 128u + 2u * r);
+#pragma unroll
+            for (uint32_t y = 0; y < 4u; ++y) raw[k][y] = ld_v4(src + ((4u * warp + y) * rows + r) * 4u);
+        }
+#pragma unroll
+        for (uint32_t k = 0; k < 2u; ++k) {
+            if (w0 + k > last) break;
+            const float pm = __uint_as_float(ml[k].x), top = fmaxf(m, pm), a = ex2(m - top), c = ex2(pm - top);
+            m = top;
+            l = fmaf(l, a, __uint_as_float(ml[k].y) * c);
+#pragma unroll
+            for (uint32_t y = 0; y < 4u; ++y) {
+                const uint4 v = raw[k][y];
+                o[4 * y] = fmaf(o[4 * y], a, __uint_as_float(v.x) * c), o[4 * y + 1] = fmaf(o[4 * y + 1], a, __uint_as_float(v.y) * c);
+                o[4 * y + 2] = fmaf(o[4 * y + 2], a, __uint_as_float(v.z) * c), o[4 * y + 3] = fmaf(o[4 * y + 3], a, __uint_as_float(v.w) * c);
+            }
+        }
+    }
+    const bool none = l == 0.0f;
+    const float inv = none ? 0.0f : 1.0f / l;
+    uint32_t y[8];
+#pragma unroll
+    for (int x = 0; x < 8; ++x) y[x] = pack_bf16x2(o[2 * x] * inv, o[2 * x + 1] * inv);
+    uint4* to = reinterpret_cast<uint4*>(p.out + ((static_cast<size_t>(b) * p.S + i) * p.H + h) * 128u + 16u * warp);
+    to[0] = make_uint4(y[0], y[1], y[2], y[3]), to[1] = make_uint4(y[4], y[5], y[6], y[7]);
+    if (p.lse != nullptr && warp == 0u) p.lse[(static_cast<size_t>(b) * p.H + h) * p.S + i] = none ? -INFINITY : (m + lg2(l)) * kLn2;
+}
+
 cudaError_t launch_many(const Kv8AttendParams& p, cudaStream_t stream) {
-    const uint32_t rows = p.S * p.group, per = kv8_prefill_rows(), row_tiles = (rows + per - 1u) / per;
+    const uint32_t rows = p.S * p.group, per = kv8_prefill_rows(), row_tiles = (rows + per - 1u) / per, grid = kv8_prefill_grid(), most = rows < per ? rows : per;
     const cudaError_t e = launch_kv8_prefill(p, row_tiles, stream);
+    if (e == cudaSuccess && few_parts(p.c, row_tiles, grid)) return kv4_launch(kv8_combine_columns_kernel, dim3(begun_entries(p.c, row_tiles, grid), (most + 31u) / 32u), 256u, 0, stream, p, per, row_tiles, grid);
     return e != cudaSuccess ? e : launch_combine_many(p, per, row_tiles, kv8_prefill_grid(), stream, /*together=*/true);   // (48 rows over 30000 tokens: 25.5 us, 105.8 with a warp a row)
 }
 

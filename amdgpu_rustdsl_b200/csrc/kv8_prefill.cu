@@ -40,7 +40,7 @@ constexpr uint32_t kThreads = 512;
 // Warps 0-3 and 4-7: softmax of tile 0 and 1; 8-11: codes to f16; 12 and 13: products of tile 0 and 1; 14: copies; 15: scales. The pools of setmaxnreg come out of the launch's 128
 // registers a thread.
 constexpr uint32_t kIssueWarp = 12, kCopyWarp = 14;
-constexpr int kSoftmaxRegs = 168, kConvertRegs = 96, kIssueRegs = 80;
+constexpr int kSoftmaxRegs = 184, kConvertRegs = 72, kIssueRegs = 72;
 static_assert(8 * kSoftmaxRegs + 4 * kConvertRegs + 4 * kIssueRegs <= 16 * 128, "register shares");
 constexpr uint32_t kColP = 80, kColO = 128, kColTile = 256;   // of a tile's 256 columns: S, P, O
 constexpr float kUpF = 6.0f, kSlack = 8.0f;   // (f16 has more room above 1 than a weight needs)
@@ -69,7 +69,7 @@ struct Shared {
         uint32_t length, n, more;      // more: whether the CTA has a segment behind this one. (One without steps: it has none at all)
         uint32_t steps[2];             // of the two tiles: those that their last live rows see
     } plan[kSegmentSlots];
-    uint32_t tmem, failed, not_drained;
+    uint32_t tmem, failed, not_drained, to_next;   // to_next: from four columns of a part to the next four
 };
 
 // a = a x + c, b = b x + c in one instruction
@@ -146,6 +146,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
         for (uint32_t i = 0; i < kSegmentSlots; ++i) mbar_init(bar(kSegment + i), 1u);
         fence_mbar_init();
         sh.failed = sh.not_drained = 0u;
+        sh.to_next = few_parts(p.c, row_tiles, gridDim.x) ? 4u * kItemRows : 4u;
     }
     if (warp == kIssueWarp) tmem_alloc(smem_u32(&sh.tmem), 512u);
     tc_fence_before_sync();
@@ -178,9 +179,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
             const uint32_t t_s = tmem + lanes + kColTile * q, t_p = t_s + kColP, t_o = t_s + kColO;
             uint32_t s_phase = 0, p_phase = 0, q_phase = 0, step0 = 0;   // step0: steps in front of the segment
             bool ok = true;
-            // The query rows, fetched into L2 when the segment is published: they go to their place as they come, once the scores of the segment before are done with its rows, and become f16 there, a
-            // thread its row's, so that the next scores are computed while that segment's last product runs and its O is stored. c_row: what the thread's row was multiplied by, taken out
-            auto load_rows = [&](const Segment& seg, uint32_t n, float& c_row) {
+            // The query rows, fetched into L2 when the segment is published: asked for when that segment's last weights are written, and made f16 in their place, a thread its row's,
+            // in the middle of storing its O: what is left of that the next scores' product runs beside.
+            auto ask_rows = [&](const Segment& seg, uint32_t n) {
                 if (!__all_sync(0xFFFFFFFFu, mbar_wait(bar(kQEmpty + q), q_phase ^ 1u, failed))) return false;
                 q_phase ^= 1u;
                 const uint32_t row = seg.row0 + q * kTileRows + r, i = row / p.group, chunk = lane & 15u;
@@ -193,37 +194,48 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
                     cp_async_16(smem_u32(sh.q[q] + (chunk >> 3) * kQAtom + to * 128u + (((chunk & 7u) ^ (to & 7u)) << 4)),
                                 at_row != 0ull ? reinterpret_cast<const uint8_t*>(at_row) + 16u * chunk : p.q.data, at_row != 0ull ? 16u : 0u);
                 }
+                return true;
+            };
+            // what the thread's row was multiplied by, taken out
+            auto take_rows = [&]() {
                 cp_async_wait_all();
                 __syncwarp();
                 uint4* const place = reinterpret_cast<uint4*>(sh.q[q] + r * 128u);
+                uint4 v[16];
+#pragma unroll
+                for (uint32_t x = 0; x < 16u; ++x) v[x] = place[(x >> 3) * (kQAtom / 16u) + ((x & 7u) ^ (r & 7u))];
                 uint32_t top = 0;   // sizes as bf16 bits
-#pragma unroll 8
-                for (uint32_t x = 0; x < 16u; ++x) {
-                    const uint4 v = place[(x >> 3) * (kQAtom / 16u) + ((x & 7u) ^ (r & 7u))];
-                    top = __vmaxu2(top, __vmaxu2(__vmaxu2(v.x & 0x7FFF7FFFu, v.y & 0x7FFF7FFFu), __vmaxu2(v.z & 0x7FFF7FFFu, v.w & 0x7FFF7FFFu)));
-                }
+#pragma unroll
+                for (uint32_t x = 0; x < 16u; ++x) top = __vmaxu2(top, __vmaxu2(__vmaxu2(v[x].x & 0x7FFF7FFFu, v[x].y & 0x7FFF7FFFu), __vmaxu2(v[x].z & 0x7FFF7FFFu, v[x].w & 0x7FFF7FFFu)));
                 const float2 f = row_factors(max(top << 16, top & 0xFFFF0000u));
-                c_row = p.scale_log2 * f.y;
-#pragma unroll 4
+#pragma unroll
                 for (uint32_t x = 0; x < 16u; ++x) {
-                    uint4* at_piece = place + (x >> 3) * (kQAtom / 16u) + ((x & 7u) ^ (r & 7u));
-                    const uint4 v = *at_piece;
-                    uint32_t w[4] = {v.x, v.y, v.z, v.w};
+                    uint32_t w[4] = {v[x].x, v[x].y, v[x].z, v[x].w};
 #pragma unroll
                     for (int y = 0; y < 4; ++y) w[y] = pack_f16x2(__uint_as_float(w[y] << 16) * f.x, __uint_as_float(w[y] & 0xFFFF0000u) * f.x);
-                    *at_piece = make_uint4(w[0], w[1], w[2], w[3]);
+                    place[(x >> 3) * (kQAtom / 16u) + ((x & 7u) ^ (r & 7u))] = make_uint4(w[0], w[1], w[2], w[3]);
                 }
                 fence_proxy_async_smem();
                 __syncwarp();
                 if (lane == 0u) mbar_arrive(bar(kQFull + q));
-                return true;
+                return p.scale_log2 * f.y;
+            };
+            // the next segment's number and rows; where its plan stands
+            auto ask_next = [&]() {
+                const uint32_t slot = number % kSegmentSlots;
+                if (!__all_sync(0xFFFFFFFFu, mbar_wait(bar(kSegment + slot), number / kSegmentSlots & 1u, failed))) return false;
+                ++number;
+                return sh.plan[slot].seg.steps > 0u && ask_rows(sh.plan[slot].seg, sh.plan[slot].n);
             };
             float c_row = 0.0f;
             Shared::Plan now;
-            ok = next_plan(now) && now.seg.steps > 0u && load_rows(now.seg, now.n, c_row);
+            ok = ask_next();
+            if (ok) c_row = take_rows();
             for (bool more = true; more && ok;) {
+                const uint32_t nan_slot = (number - 1u) % kSegmentSlots;
+                now = sh.plan[nan_slot];
                 const Segment seg = now.seg;
-                const uint32_t length = now.length, n = now.n, nan_slot = (number - 1u) % kSegmentSlots;
+                const uint32_t length = now.length, n = now.n;
                 more = now.more != 0u;
                 const uint32_t steps = q != 0u ? now.steps[1] : now.steps[0], row = seg.row0 + q * kTileRows + r, i = row / p.group;
                 const bool exists = row < p.S * p.group;
@@ -319,7 +331,10 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
                 }
                 step0 += seg.steps;
                 if (!ok) break;
-                if (more) ok = next_plan(now) && load_rows(now.seg, now.n, c_row);   // (the next segment's scores start while this one's O is stored)
+                if (more) {
+                    ok = ask_next();
+                    if (ok) c_row = take_rows();
+                }
                 if (steps > 0u) {
                     ok = ok && __all_sync(0xFFFFFFFFu, mbar_wait(bar(kPFree + q), p_phase, failed));
                     p_phase ^= 1u;
@@ -333,7 +348,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
                 if (steps > 0u && sh.nan_from[nan_slot] < limit) factor = __uint_as_float(0x7FC00000u);
                 __nv_bfloat16* out = p.out + ((static_cast<size_t>(seg.b) * p.S + i) * p.H + h) * 128u;
                 float* slot = slot_of(p.ws, gridDim.x, blockIdx.x, seg.first == 0u ? 1u : 0u, kItemRows);
-                float* part = slot + (q * kTileRows + r) * 128u;
+                const uint32_t to_next = sh.to_next;
+                // few parts: by four columns, then rows, so that a warp's stores are whole lines (a row a thread is 32 lines each); else by rows
+                float* part = slot + (q * kTileRows + r) * (to_next == 4u ? 128u : 4u);
 #pragma unroll 1
                 for (uint32_t c = 0; c < 4u; ++c) {   // 32 columns at a time, a thread its row's
                     uint32_t o[32];
@@ -361,7 +378,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
                         }
                     } else if (limit != 0u) {
 #pragma unroll
-                        for (int x = 0; x < 8; ++x) *reinterpret_cast<uint4*>(part + 32u * c + 4 * x) = make_uint4(o[4 * x], o[4 * x + 1], o[4 * x + 2], o[4 * x + 3]);
+                        for (int x = 0; x < 8; ++x) *reinterpret_cast<uint4*>(part + (8u * c + x) * to_next) = make_uint4(o[4 * x], o[4 * x + 1], o[4 * x + 2], o[4 * x + 3]);
                     }
                 }
                 if (whole) {
@@ -370,6 +387,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
                     *reinterpret_cast<float2*>(slot + kItemRows * 128u + 2u * (q * kTileRows + r)) = make_float2(m, l);
                 }
             }
+            if (!ok) cp_async_wait_all();   // (what was asked for has to have come before the CTA ends)
         } else if (warp < kIssueWarp) {
             asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kConvertRegs));
             // Block by block, 16 bytes of K and of V a thread: 16 elements of one token, 8 elements of both tokens of a pair
@@ -472,7 +490,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
                 auto commit = [&](uint32_t b) {
                     if (elect_one_sync()) tc_commit(b);
                 };
-                // the scores of a step that this tile takes part in, or not; the step's K is done with then
+                // the scores of a step that this tile takes part in, or not; the step's K is done with then, and behind the tile's last scores its query rows
                 auto scores = [&](uint32_t at_step, bool taken, bool last) {
                     const uint32_t st = at_step % kStages;
                     if (!wait(bar(kKFull + st), at_step / kStages & 1u)) return;
@@ -497,10 +515,10 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
                     const uint32_t steps = uniform(q != 0u ? now.steps[1] : now.steps[0]), seg_steps = uniform(now.seg.steps);
                     if (!wait(bar(kQFull + q), q_phase)) break;
                     q_phase ^= 1u;
-                    scores(step, steps > 0u, seg_steps == 1u);
+                    scores(step, steps > 0u, steps <= 1u);
                     for (uint32_t j = 0; j < seg_steps && ok; ++j, ++step) {
                         const uint32_t st = step % kStages;
-                        if (j + 1u < seg_steps) scores(step + 1u, j + 1u < steps, j + 2u == seg_steps);
+                        if (j + 1u < seg_steps) scores(step + 1u, j + 1u < steps, j + 2u == steps);
                         if (!ok || !wait(bar(kVFull + st), step / kStages & 1u)) break;
                         if (j < steps) {
                             if (j == 0u) {   // O of the segment before has been taken

@@ -135,21 +135,28 @@ __device__ __forceinline__ void begin_item(const Kv4AttendParams& p, const DealO
 __device__ __forceinline__ float* slot_of(float* ws, uint32_t grid, uint32_t w, uint32_t slot, uint32_t rows) { return ws + 4u * grid + (static_cast<size_t>(w) * 2u + slot) * rows * 130u; }
 constexpr float kLowest = -1e30f;   // M of a row that has seen nothing
 
-// Sequences' row tiles that no CTA has steps of: their rows see nothing. All threads of the grid. `entries`: whether the workspace has entries
+// Sequences' row tiles that no CTA has steps of: their rows see nothing. `threads` threads of every CTA of the grid; with few entries several CTAs share one's rows (4 tiles of 256 rows, 8 heads, by
+// a CTA each: 15 us, longer than those CTAs' own work). `entries`: whether the workspace has entries
 template <uint32_t kTokens, uint32_t kExtra>
-__device__ __forceinline__ void clear_empty_entries(const Kv4AttendParams& p, const DealOf<kTokens, kExtra>& d, bool entries = true) {
-    for (uint32_t e = blockIdx.x; e < p.c.B * d.row_tiles; e += gridDim.x) {
+__device__ __forceinline__ void clear_empty_entries(const Kv4AttendParams& p, const DealOf<kTokens, kExtra>& d, bool entries, uint32_t thread, uint32_t threads) {
+    const uint32_t n = p.c.B * d.row_tiles, share = n < gridDim.x ? gridDim.x / n : 1u, part = blockIdx.x % share;
+    for (uint32_t e = blockIdx.x / share; e < n; e += gridDim.x / share) {
         if (steps_of(p, d, e) != 0u) continue;
-        if (entries && begun_by_item(p.c, d.row_tiles, gridDim.x)) {
-            for (uint32_t h = threadIdx.x; h < p.c.HK; h += blockDim.x) *begun_at(p.ws, e * p.c.HK + h) = {0u, 0u, 0u, 0u};
+        if (part == 0u && entries && begun_by_item(p.c, d.row_tiles, gridDim.x)) {
+            for (uint32_t h = thread; h < p.c.HK; h += threads) *begun_at(p.ws, e * p.c.HK + h) = {0u, 0u, 0u, 0u};
         }
-        const uint32_t b = e / d.row_tiles, row0 = (e - b * d.row_tiles) * d.rows, rows = min(d.rows, p.S * p.group - row0);
-        for (uint32_t x = threadIdx.x; x < rows * p.c.HK * 16u; x += blockDim.x) {
-            const uint32_t part = x & 15u, row = row0 + (x >> 4) % rows, head = (x >> 4) / rows, i = row / p.group, h = head * p.group + row % p.group;
-            *reinterpret_cast<uint4*>(p.out + ((static_cast<size_t>(b) * p.S + i) * p.H + h) * 128u + 8u * part) = make_uint4(0u, 0u, 0u, 0u);
-            if (part == 0u && p.lse != nullptr) p.lse[(static_cast<size_t>(b) * p.H + h) * p.S + i] = -INFINITY;
+        const uint32_t b = e / d.row_tiles, row0 = (e - b * d.row_tiles) * d.rows, rows = min(d.rows, p.S * p.group - row0), all = rows * p.c.HK * 16u;
+        const uint32_t end = static_cast<uint32_t>(static_cast<unsigned long long>(all) * (part + 1u) / share);
+        for (uint32_t x = static_cast<uint32_t>(static_cast<unsigned long long>(all) * part / share) + thread; x < end; x += threads) {
+            const uint32_t piece = x & 15u, row = row0 + (x >> 4) % rows, head = (x >> 4) / rows, i = row / p.group, h = head * p.group + row % p.group;
+            *reinterpret_cast<uint4*>(p.out + ((static_cast<size_t>(b) * p.S + i) * p.H + h) * 128u + 8u * piece) = make_uint4(0u, 0u, 0u, 0u);
+            if (piece == 0u && p.lse != nullptr) p.lse[(static_cast<size_t>(b) * p.H + h) * p.S + i] = -INFINITY;
         }
     }
+}
+template <uint32_t kTokens, uint32_t kExtra>
+__device__ __forceinline__ void clear_empty_entries(const Kv4AttendParams& p, const DealOf<kTokens, kExtra>& d, bool entries = true) {
+    clear_empty_entries(p, d, entries, threadIdx.x, blockDim.x);
 }
 
 }  // namespace kv4

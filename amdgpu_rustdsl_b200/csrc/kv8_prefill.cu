@@ -159,8 +159,10 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
     const uint32_t all = sum_steps(p, deal, 0u, sh.part).all;
     const uint32_t n_work = workers(all, gridDim.x);
     volatile uint32_t* failed = &sh.failed;
-    clear_empty_entries(p, deal);
-    if (threadIdx.x == 0u && blockIdx.x >= n_work) begin_nothing(p, deal);
+    if (blockIdx.x >= n_work) {
+        if (threadIdx.x == 0u) begin_nothing(p, deal);
+        clear_empty_entries(p, deal);
+    }
     if (blockIdx.x < n_work) {
         const uint32_t begin = run_begin(all, n_work, blockIdx.x);
         const uint32_t end = run_begin(all, n_work, blockIdx.x + 1u);
@@ -469,6 +471,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
                     if (lane == 0u) mbar_arrive(bar(kRawEmpty + raw));
                 }
             }
+            clear_empty_entries(p, deal, true, t, 128u);   // (while the others are still at the last steps)
         } else {
             asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kIssueRegs));
             if (warp < kCopyWarp) {
@@ -545,46 +548,33 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
                 __syncwarp();
             } else if (warp == kCopyWarp) {
                 // The segments, for all roles, and the copies of a step: lane x brings block x
-                uint32_t step = 0, left = end - begin, pos = begin, next_pos = begin;
+                uint32_t step = 0, left = end - begin, pos = begin;
                 Place at = find_step(p, deal, begin);
-                bool ok = true, have = false, have_next = false;
-                Segment seg, next;
-                const auto look_ahead = [&]() {   // for the next segment of the run that has steps
-                    have_next = false;
-                    while (left > 0u && !have_next) {
-                        next_pos = end - left;
-                        next = next_segment(p, deal, at, left);
-                        have_next = next.steps > 0u;
-                    }
-                };
+                bool ok = true, have = false;
+                Segment seg;
+                // the first segment that has steps; those behind it begin an item, and have some if the run is longer than what a beginning counts as
+                while (left > 0u && !have) {
+                    pos = end - left;
+                    seg = next_segment(p, deal, at, left);
+                    have = seg.steps > 0u;
+                }
                 if (lane == 0u) {
                     begin_nothing(p, deal);
-                    sh.plan[0].seg.steps = 0u;
-                }
-                look_ahead();
-                have = have_next;
-                if (!have && lane == 0u) {
-                    sh.plan[0].more = 0u;
-                    mbar_arrive(bar(kSegment));
+                    if (!have) {
+                        sh.plan[0].seg.steps = sh.plan[0].more = 0u;
+                        mbar_arrive(bar(kSegment));
+                    }
                 }
                 while (have && ok) {
-                    seg = next, pos = next_pos;
-                    look_ahead();
-                    have = have_next;
-                    const uint32_t length = length_of(p.c, seg.b), n = count_of(p.counts, seg.b, p.S, length);
+                    const uint32_t length = length_of(p.c, seg.b), n = count_of(p.counts, seg.b, p.S, length), segment_pos = pos;
+                    have = left > kExtra;
                     if (lane == 0u) {
                         Shared::Plan& x = sh.plan[number % kSegmentSlots];
-                        x.seg = seg, x.length = length, x.n = n, x.more = have_next;
+                        x.seg = seg, x.length = length, x.n = n, x.more = have;
                         for (uint32_t q = 0; q < 2u; ++q) x.steps[q] = tile_steps(p, seg, q, length, n);
                         mbar_arrive(bar(kSegment + number % kSegmentSlots));
-                        begin_item(p, deal, seg, pos, all, n_work);
                     }
                     ++number;
-                    for (uint32_t r = lane; r < kItemRows; r += 32u) {
-                        const uint32_t row = seg.row0 + r, i = row / p.group, h = seg.head * p.group + row - i * p.group;
-                        const uint8_t* src = p.q.data + seg.b * p.q.stride_b + i * p.q.stride_s + h * p.q.stride_h;
-                        if (i < n) asm volatile("prefetch.global.L2 [%0];\n\tprefetch.global.L2 [%0 + 128];" ::"l"(src));
-                    }
                     long long page = -1;   // of the lane's block in the next step
                     auto look_up = [&](uint32_t j) {
                         const uint32_t t = (seg.first + j) * kStep + lane * kBlockTokens;
@@ -608,6 +598,18 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
                             bulk_load(smem_u32(sh.raw_v[raw][lane]), block + kVCodes, kMeta - kVCodes, bar(kRawFull + raw));
                         }
                         look_up(j + 1u);
+                        if (j == 0u) {   // (what is not needed for the first copies)
+                            if (lane == 0u) begin_item(p, deal, seg, segment_pos, all, n_work);
+                            for (uint32_t r = lane; r < kItemRows && number > 1u; r += 32u) {
+                                const uint32_t row = seg.row0 + r, i = row / p.group, h = seg.head * p.group + row - i * p.group;
+                                const uint8_t* src = p.q.data + seg.b * p.q.stride_b + i * p.q.stride_s + h * p.q.stride_h;
+                                if (i < n) asm volatile("prefetch.global.L2 [%0];\n\tprefetch.global.L2 [%0 + 128];" ::"l"(src));
+                            }
+                        }
+                    }
+                    if (have && ok) {
+                        pos = end - left;
+                        seg = next_segment(p, deal, at, left);
                     }
                 }
                 // after a failure: copies that are under way land before the CTA's shared memory is another's. (step: the one whose copies were not asked for)

@@ -11,6 +11,13 @@
 // the products, S from shared memory, P V with P from tensor memory, and two groups of four warps do the softmax, one tile each, a thread a row. m moves only when a row's maximum
 // exceeds it by 2^(kUp + kSlack), so O is hardly ever rescaled.
 //
+// Bound by a tile's chain of scores, softmax and product: a step takes 2850 clocks, of which the products of both tiles are 1280, the exponentials of both 1280 (they meet: two warps of a scheduler do
+// them at the same time, which takes 1600), loads from tensor memory 250, the maximum 400, waits and stores 500. 4096 rows of 32 heads over 8192 tokens: 459 us among other calls (431 in a row), 0.90
+// PFLOP/s, 0.55 of what a matrix product measures; a change of item is 9000 clocks, of which a CTA of 4 ragged chunks of 333 rows (50.5 us) has one or two to its 16 steps.
+// Slower: steps of 128 tokens with P over S (514 us in place of 464 then), of 64 (500), a quarter and three eighths of the exponentials by a polynomial (470 and 485 in place of 461), locks or turns between the two
+// groups at the exponentials (489 and more), K's and V's conversion by four warps each (504), query rows brought by the issuing warps (427 and 451 in place of 431, chunks 51.5 and 55 in place of 50.6),
+// O stored 64 columns at a time (507) or exchanged between four lanes first (441).
+//
 // Steps are dealt out to one CTA per SM as kv4_schedule.cuh says; items that several CTAs worked on go through f32 partials and the combine kernel.
 #include "kv4_schedule.cuh"
 #include "kv8.cuh"
@@ -27,7 +34,7 @@ using namespace kv8;
 using namespace sm100;
 
 constexpr uint32_t kTileRows = 128, kItemRows = 256, kStep = 80, kBlocks = kStep / kBlockTokens, kStages = 3, kRawStages = 2;
-constexpr uint32_t kExtra = 5;   // what a CTA's change to another item costs, in steps (4 ragged chunks of 333 rows, 24 heads, 94 us without, 73, 71, 70 with 2, 4, 6)
+constexpr uint32_t kExtra = 5;   // what a CTA's change to another item costs, in steps (4 ragged chunks of 333 rows, 24 heads: 52.4, 50.6, 50.6 us with 3, 4, 5; 8 x 512 rows over 600 tokens 82.0, 82.4, 79.9)
 // Slots of the steps' scales. Those of step j are written when its codes have come, for which those of step j - 2 must have been taken: behind the scores of step j - 5 (three stages of K)
 // and so behind the softmax's reads of the scores of step j - 6
 constexpr uint32_t kScaleSlots = 8;

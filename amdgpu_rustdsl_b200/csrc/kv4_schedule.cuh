@@ -145,10 +145,10 @@ __device__ __forceinline__ void clear_empty_entries(const Kv4AttendParams& p, co
         if (part == 0u && entries && begun_by_item(p.c, d.row_tiles, gridDim.x)) {
             for (uint32_t h = thread; h < p.c.HK; h += threads) *begun_at(p.ws, e * p.c.HK + h) = {0u, 0u, 0u, 0u};
         }
-        const uint32_t b = e / d.row_tiles, row0 = (e - b * d.row_tiles) * d.rows, rows = min(d.rows, p.S * p.group - row0), all = rows * p.c.HK * 16u;
-        const uint32_t end = static_cast<uint32_t>(static_cast<unsigned long long>(all) * (part + 1u) / share);
-        for (uint32_t x = static_cast<uint32_t>(static_cast<unsigned long long>(all) * part / share) + thread; x < end; x += threads) {
-            const uint32_t piece = x & 15u, row = row0 + (x >> 4) % rows, head = (x >> 4) / rows, i = row / p.group, h = head * p.group + row % p.group;
+        const uint32_t b = e / d.row_tiles, row0 = (e - b * d.row_tiles) * d.rows, rows = min(d.rows, p.S * p.group - row0), all = rows * p.c.HK;
+        const uint32_t begin = static_cast<uint32_t>(static_cast<unsigned long long>(all) * part / share), end = static_cast<uint32_t>(static_cast<unsigned long long>(all) * (part + 1u) / share);
+        for (uint32_t y = begin + (thread >> 4); y < end; y += threads >> 4) {   // 16 threads a row (rows and heads together are 2^30 at most)
+            const uint32_t piece = thread & 15u, row = row0 + y % rows, head = y / rows, i = row / p.group, h = head * p.group + row % p.group;
             *reinterpret_cast<uint4*>(p.out + ((static_cast<size_t>(b) * p.S + i) * p.H + h) * 128u + 8u * piece) = make_uint4(0u, 0u, 0u, 0u);
             if (piece == 0u && p.lse != nullptr) p.lse[(static_cast<size_t>(b) * p.H + h) * p.S + i] = -INFINITY;
         }

@@ -11,9 +11,9 @@
 // the products, S from shared memory, P V with P from tensor memory, and two groups of four warps do the softmax, one tile each, a thread a row. m moves only when a row's maximum
 // exceeds it by 2^(kUp + kSlack), so O is hardly ever rescaled.
 //
-// Bound by a tile's chain of scores, softmax and product: a step takes 2850 clocks, of which the products of both tiles are 1280, the exponentials of both 1280 (they meet: two warps of a scheduler do
-// them at the same time, which takes 1600), loads from tensor memory 250, the maximum 400, waits and stores 500. 4096 rows of 32 heads over 8192 tokens: 459 us among other calls (431 in a row), 0.90
-// PFLOP/s, 0.55 of what a matrix product measures; a change of item is 9000 clocks, of which a CTA of 4 ragged chunks of 333 rows (50.5 us) has one or two to its 16 steps.
+// Bound by a tile's chain of scores, softmax and product: a step takes 2750 clocks, of which the products of both tiles are 1280, the exponentials of both 1280 (they meet: two warps of a scheduler do
+// them at the same time, which takes 1600), loads from tensor memory 250, the maximum 400, waits and stores 500. 4096 rows of 32 heads over 8192 tokens: 452 us among other calls (418 in a row), 0.91
+// PFLOP/s, 0.56 of what a matrix product measures; a change of item is 9000 clocks, of which a CTA of 4 ragged chunks of 333 rows (49.7 us) has one or two to its 16 steps.
 // Slower: steps of 128 tokens with P over S (514 us in place of 464 then), of 64 (500), a quarter and three eighths of the exponentials by a polynomial (470 and 485 in place of 461), locks or turns between the two
 // groups at the exponentials (489 and more), K's and V's conversion by four warps each (504), query rows brought by the issuing warps (427 and 451 in place of 431, chunks 51.5 and 55 in place of 50.6),
 // O stored 64 columns at a time (507) or exchanged between four lanes first (441).
@@ -276,16 +276,16 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
                             if (y >= seen) s[y] = 0xFF800000u;
                         }
                     }
-                    float most = -INFINITY;
+                    float tops[kBlocks];
 #pragma unroll
                     for (int k = 0; k < static_cast<int>(kBlocks); ++k) {
                         const uint32_t* y = s + 16 * k;
-                        float top = fmaxf(__uint_as_float(y[0]), __uint_as_float(y[1])), more = fmaxf(__uint_as_float(y[2]), __uint_as_float(y[3]));
+                        float top = max3(__uint_as_float(y[0]), __uint_as_float(y[1]), __uint_as_float(y[2]));
 #pragma unroll
-                        for (int z = 4; z < 16; z += 4) top = max3(top, __uint_as_float(y[z]), __uint_as_float(y[z + 1])), more = max3(more, __uint_as_float(y[z + 2]), __uint_as_float(y[z + 3]));
-                        most = fmaxf(most, fmaf(fmaxf(top, more), c[k], shift[k]));
+                        for (int z = 3; z < 15; z += 2) top = max3(top, __uint_as_float(y[z]), __uint_as_float(y[z + 1]));
+                        tops[k] = fmaf(fmaxf(top, __uint_as_float(y[15])), c[k], shift[k]);
                     }
-                    most -= kUpF;
+                    const float most = max3(max3(tops[0], tops[1], tops[2]), tops[3], tops[4]) - kUpF;
                     const bool over = most > m + kSlack;
                     // once the product of the step before is over, O may be rescaled and P overwritten
                     bool waited = j == 0u;
@@ -329,10 +329,14 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
                             s[16 * k + z] = pack_f16x2(ea, eb);   // (behind what it overwrites)
                         }
                         l = fmaf(l0 + l1, back[k], l);
-                    }
-                    wait_product();
+                        if (k == 3) {   // (four blocks at once, beside the last one's exponentials: a prompt of 4096 rows 427 us, 431 with all at the end, 453 with three)
+                            wait_product();
 #pragma unroll
-                    for (int k = 0; k < static_cast<int>(kBlocks); ++k) tmem_st8(t_p + 8u * k, s + 16 * k);
+                            for (int x = 0; x < 4; ++x) tmem_st8(t_p + 8u * x, s + 16 * x);
+                        }
+                    }
+#pragma unroll
+                    for (int k = 4; k < static_cast<int>(kBlocks); ++k) tmem_st8(t_p + 8u * k, s + 16 * k);
                     tmem_wait_st();
                     tc_fence_before_sync();
                     __syncwarp();

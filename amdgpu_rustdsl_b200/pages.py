@@ -10,9 +10,25 @@ device (or ``stream``, a raw handle) and do not wait for it. Wrong arguments rai
 """
 from __future__ import annotations
 
+import ctypes as C
+import struct
+
 from . import _abi
 from .kv4 import PagedCache, _call, _check, _i32
 from .ops import _raw_stream
+
+
+_ARGS = struct.Struct("@3Q4I").pack   # fmha_pages, as bytes: half the time that a ctypes structure takes
+assert struct.calcsize("@3Q4I") == C.sizeof(_abi.PagesArgs)
+_entries = {}
+
+
+def _entry(name, *kinds):
+    """The C entry with its first argument as bytes."""
+    entry = _abi.load()[name]
+    entry.restype, entry.argtypes = C.c_int, [C.c_char_p, *kinds, C.c_void_p, C.c_char_p, C.c_size_t]
+    _entries[name] = entry
+    return entry
 
 
 def pages_stack(pages, device="cuda"):
@@ -27,9 +43,22 @@ def _pages(who, free, cache):
     import torch
     if not isinstance(cache, PagedCache):
         raise ValueError(f"{who}: cache must be a Kv4Cache or a Kv8Cache, not {type(cache).__name__}")
-    if free.dtype != torch.int32 or free.dim() != 1 or free.shape[0] < 5 or not free.is_contiguous() or free.device != cache.device:
+    shape = free.shape
+    if free.dtype != torch.int32 or len(shape) != 1 or shape[0] < 5 or not free.is_contiguous() or free.device != cache.device:
         raise ValueError(f"{who}: free must be a contiguous int32 tensor [4 + pages] on the cache's device")
-    return _abi.PagesArgs(free.data_ptr(), cache.c.table, cache.c.lengths, free.shape[0] - 4, cache.B, cache.page, cache.table.shape[1])
+    pages = shape[0] - 4
+    if pages > 0x7FFFFFFF:   # (here, in numbers of any size)
+        raise ValueError(f"{who}: a stack of {pages} pages, more than 2^31")
+    c = cache.c
+    return _ARGS(free.data_ptr(), c.table, c.lengths, pages, c.B, c.page, c.table_width)
+
+
+def _map(name, x, kind, cache):
+    """S of a map's [B, S]."""
+    shape = x.shape
+    if not kind or len(shape) != 2 or shape[0] != cache.B or x.device != cache.device or not x.is_contiguous():
+        raise ValueError(f"pages_take: {name} must be a contiguous {'torch.int32 or torch.int64' if name == 'positions' else 'torch.int64'} tensor [{cache.B}, S] on the cache's device")
+    return shape[1]
 
 
 def pages_take(free, cache, counts, granted, *, positions=None, slots=None, starts=None, stream=None):
@@ -45,25 +74,25 @@ def pages_take(free, cache, counts, granted, *, positions=None, slots=None, star
     starts     int32 [B + 1]: the sums of granted in front of each sequence, and of all; for stacks of less than 2^31 tokens
     """
     import torch
-    lib = _abi.load()
     p = _pages("pages_take", free, cache)
     if counts is None or granted is None:
         raise ValueError("pages_take: counts and granted must be given")
     n, g = _i32("pages_take", "counts", counts, cache, (cache.B,)), _i32("pages_take", "granted", granted, cache, (cache.B,))
-    S = 0
-    for name, x, kinds in (("positions", positions, (torch.int32, torch.int64)), ("slots", slots, (torch.int64,))):
-        if x is None:
-            continue
-        if x.dtype not in kinds or x.dim() != 2 or x.shape[0] != cache.B or (S and x.shape[1] != S) or x.device != cache.device or not x.is_contiguous():
-            raise ValueError(f"pages_take: {name} must be a contiguous {" or ".join(map(str, kinds))} tensor [{cache.B}, S] on the cache's device, positions and slots with the same S")
-        S = x.shape[1]
+    S, wide, at_positions, at_slots = 0, False, None, None
+    if positions is not None:
+        wide = positions.dtype == torch.int64
+        S, at_positions = _map("positions", positions, wide or positions.dtype == torch.int32, cache), positions.data_ptr()
+    if slots is not None:
+        rows, at_slots = _map("slots", slots, slots.dtype == torch.int64, cache), slots.data_ptr()
+        if positions is not None and rows != S:
+            raise ValueError("pages_take: positions and slots must have the same S")
+        S = rows
     if S > 0x7FFFFFFF:
         raise ValueError(f"pages_take: {S} rows, more than 2^31")
-    if positions is not None and slots is not None and positions.shape != slots.shape:
-        raise ValueError("pages_take: positions and slots must have the same S")
     s = _i32("pages_take", "starts", starts, cache, (cache.B + 1,))
     raw = stream if stream is not None else _raw_stream(torch, cache.device)
-    rc = _call(torch, cache, raw, lib.fmha_pages_take, p, n, g, None if positions is None else positions.data_ptr(), positions is not None and positions.dtype == torch.int64, None if slots is None else slots.data_ptr(), s, S)
+    take = _entries.get("fmha_pages_take") or _entry("fmha_pages_take", C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_void_p, C.c_void_p, C.c_uint32)
+    rc = _call(torch, cache, raw, take, p, n, g, at_positions, wide, at_slots, s, S)
     if rc:
         _check("pages_take", rc)
 
@@ -73,12 +102,11 @@ def pages_cut(free, cache, keep, *, stream=None):
 
     A cut to the lengths before a ``pages_take`` leaves stack, table and lengths as they were before it. ``keep`` of 0 ends a sequence."""
     import torch
-    lib = _abi.load()
     p = _pages("pages_cut", free, cache)
     if keep is None:
         raise ValueError("pages_cut: keep must be given")
     k = _i32("pages_cut", "keep", keep, cache, (cache.B,))
     raw = stream if stream is not None else _raw_stream(torch, cache.device)
-    rc = _call(torch, cache, raw, lib.fmha_pages_cut, p, k)
+    rc = _call(torch, cache, raw, _entries.get("fmha_pages_cut") or _entry("fmha_pages_cut", C.c_void_p), p, k)
     if rc:
         _check("pages_cut", rc)

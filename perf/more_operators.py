@@ -255,7 +255,7 @@ def _prepare_pages(case, g):
     pool[4:4 + free] = used + torch.randperm(free, generator=g, device="cuda").int()
     s = {"case": case, "table": table, "lengths": torch.tensor(lengths, dtype=torch.int32, device="cuda"), "counts": torch.tensor(_new(case), dtype=torch.int32, device="cuda"),
          "free": pool, "granted": torch.empty(B, dtype=torch.int32, device="cuda"), "starts": torch.empty(B + 1, dtype=torch.int32, device="cuda"),
-         "positions": torch.empty((B, S), dtype=torch.int64, device="cuda"), "slots": torch.empty((B, S), dtype=torch.int64, device="cuda")}
+         "positions": torch.empty((B, S), dtype=torch.int32, device="cuda"), "slots": torch.empty((B, S), dtype=torch.int64, device="cuda")}
     s["keep"] = s["lengths"].clone()
     if own:
         from amdgpu_rustdsl_b200 import Kv8Cache

@@ -261,6 +261,7 @@ def _prepare_pages(case, g):
         from amdgpu_rustdsl_b200 import Kv8Cache
         # (the cache's own memory is not looked at: one KV head, as small as it can be)
         s["cache"] = Kv8Cache(torch.zeros((used + max(1, free), 1, 257 * page), dtype=torch.uint8, device="cuda"), table, s["lengths"])
+        s["positions"] = torch.empty_like(s["slots"])   # (64 bits, which the plain form's sums come out in)
     return s
 
 

@@ -153,6 +153,14 @@ __device__ __forceinline__ float ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+// 2^d for a sum l that moves to a reference which is larger by -d, to be multiplied by. The references follow the weights times V, the sums are of weights alone: they may differ by more than f32's exponents
+// (V's scales by 2^209), and a factor that is no f32 number still leaves something. It is taken in two halves then, the first onto the sum at once.
+__device__ __forceinline__ float sum_factor(float& l, float d) {
+    const bool halves = d < -120.0f;
+    const float f = ex2(halves ? 0.5f * d : d);
+    l = halves ? l * f : l;
+    return f;
+}
 __device__ __forceinline__ float lg2(float x) {
     float y;
     asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));

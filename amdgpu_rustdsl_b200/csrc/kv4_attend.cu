@@ -538,9 +538,9 @@ __global__ void __launch_bounds__(kTogether ? 32 * kTogether : 256) kv4_combine_
         }
 #pragma unroll
         for (uint32_t k = 0; k < 4u; ++k) {
-            const float top = fmaxf(m, pm[k]), a = ex2(m - top), c = ex2(pm[k] - top);
+            const float top = fmaxf(m, pm[k]), a = ex2(m - top), c = ex2(pm[k] - top), al = sum_factor(l, m - top), cl = sum_factor(pl[k], pm[k] - top);
             m = top;
-            l = fmaf(l, a, pl[k] * c);
+            l = fmaf(l, al, pl[k] * cl);
             o.x = fmaf(o.x, a, __uint_as_float(raw[k].x) * c), o.y = fmaf(o.y, a, __uint_as_float(raw[k].y) * c);
             o.z = fmaf(o.z, a, __uint_as_float(raw[k].z) * c), o.w = fmaf(o.w, a, __uint_as_float(raw[k].w) * c);
         }
@@ -565,9 +565,10 @@ __global__ void __launch_bounds__(kTogether ? 32 * kTogether : 256) kv4_combine_
             if (warp == 0u) {
 #pragma unroll
                 for (uint32_t w = 0; w < 4u; ++w) {
-                    const float f = ex2(sm_m[w0 + w] - m);
+                    float l_w = sm_l[w0 + w];
+                    const float f = ex2(sm_m[w0 + w] - m), fl = sum_factor(l_w, sm_m[w0 + w] - m);
                     const float4 c = sm_o[w][lane];
-                    l = fmaf(sm_l[w0 + w], f, l);
+                    l = fmaf(l_w, fl, l);
                     o.x = fmaf(c.x, f, o.x), o.y = fmaf(c.y, f, o.y), o.z = fmaf(c.z, f, o.z), o.w = fmaf(c.w, f, o.w);
                 }
             }
@@ -611,9 +612,9 @@ __global__ void __launch_bounds__(256) kv4_combine_rows_kernel(const __grid_cons
         }
 #pragma unroll
         for (uint32_t y = 0; y < kRows; ++y) {
-            const float top = fmaxf(m[y], pm[y]), a = ex2(m[y] - top), c = ex2(pm[y] - top);
+            const float top = fmaxf(m[y], pm[y]), a = ex2(m[y] - top), c = ex2(pm[y] - top), al = sum_factor(l[y], m[y] - top), cl = sum_factor(pl[y], pm[y] - top);
             m[y] = top;
-            l[y] = fmaf(l[y], a, pl[y] * c);
+            l[y] = fmaf(l[y], al, pl[y] * cl);
             o[y].x = fmaf(o[y].x, a, __uint_as_float(raw[y].x) * c), o[y].y = fmaf(o[y].y, a, __uint_as_float(raw[y].y) * c);
             o[y].z = fmaf(o[y].z, a, __uint_as_float(raw[y].z) * c), o[y].w = fmaf(o[y].w, a, __uint_as_float(raw[y].w) * c);
         }

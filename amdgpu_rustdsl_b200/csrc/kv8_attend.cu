@@ -124,9 +124,16 @@ struct LostBlocks {
 };
 __device__ const LostBlocks kNowhere;
 
+// What a run of steps has met of V's exponents (kv8.cuh); the same in all lanes
+struct Exponents {
+    int first;
+    bool wide;
+};
+constexpr int kNone = 1 << 20;
+
 // G blocks of 16 tokens: scores, softmax, and their part of O: o[g][i][j], d = 16 gid + 2 i and, from [2 + j], the next, of the column 2 tig + j
 template <int NT, int G, bool kEdge>
-__device__ __forceinline__ void attend_blocks(float (&o)[NT][8][4], float (&m)[NT][2], float (&l)[NT][2], const QueryRows<NT>& x, const uint8_t* unit, uint32_t tok0, const uint4* q_shared, uint32_t length) {
+__device__ __forceinline__ void attend_blocks(float (&o)[NT][8][4], float (&m)[NT][2], float (&l)[NT][2], const QueryRows<NT>& x, const uint8_t* unit, uint32_t tok0, const uint4* q_shared, uint32_t length, Exponents& seen) {
     constexpr int kSums = NT <= 2 ? 2 : 1;
     const unsigned lane = threadIdx.x & 31u, gid = lane >> 2, tig = lane & 3u;
     float s[G][NT][4];
@@ -206,17 +213,20 @@ __device__ __forceinline__ void attend_blocks(float (&o)[NT][8][4], float (&m)[N
         }
     }
     float c[G][NT][2], e[G], back[G];
+    seen.first = seen.first == kNone ? exponent_of(meta[0].y) : seen.first;
+#pragma unroll
+    for (int gr = 0; gr < G; ++gr) seen.wide = seen.wide || !(dead[gr] || is_near(exponent_of(meta[gr].y), seen.first));
 #pragma unroll
     for (int gr = 0; gr < G; ++gr) {
         const int exponent = exponent_of(meta[gr].y);
-        e[gr] = static_cast<float>(exponent), back[gr] = power_of(-exponent);
+        e[gr] = static_cast<float>(exponent), back[gr] = seen.wide ? 0.0f : power_of(-exponent);
 #pragma unroll
         for (int g = 0; g < NT; ++g) {
 #pragma unroll
             for (int j = 0; j < 2; ++j) c[gr][g][j] = fmaxf(x.factor(g, j) * __uint_as_float(meta[gr].x), kLeast);
         }
     }
-    bool over = false;
+    bool over = seen.wide;
     float top[NT][2];
 #pragma unroll
     for (int g = 0; g < NT; ++g) {
@@ -237,11 +247,24 @@ __device__ __forceinline__ void attend_blocks(float (&o)[NT][8][4], float (&m)[N
                 t = fmaxf(t, __shfl_xor_sync(0xFFFFFFFFu, t, 8));
                 t = fmaxf(t, __shfl_xor_sync(0xFFFFFFFFu, t, 16));
                 t = fmaxf(t, m[g][j]);
-                const float f = ex2(m[g][j] - t);
+                const float f = ex2(m[g][j] - t), fl = sum_factor(l[g][j], m[g][j] - t);
                 m[g][j] = t;
-                l[g][j] *= f;
+                l[g][j] *= fl;
 #pragma unroll
                 for (int i = 0; i < 8; ++i) o[g][i][j] *= f, o[g][i][2 + j] *= f;
+            }
+        }
+        if (seen.wide) {
+#pragma unroll
+            for (int gr = 0; gr < G; ++gr) {
+#pragma unroll
+                for (int g = 0; g < NT; ++g) {
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        const float up = static_cast<float>(kWide) - m[g][j], more = ex2_wide(fmaf(s[gr][g][j], c[gr][g][j], up)) + ex2_wide(fmaf(s[gr][g][2 + j], c[gr][g][j], up));
+                        l[g][j] = fmaf(more, 1.0f / (1 << kWide), l[g][j]);
+                    }
+                }
             }
         }
     }
@@ -286,12 +309,12 @@ __device__ __forceinline__ void attend_blocks(float (&o)[NT][8][4], float (&m)[N
 
 // a unit's 32 tokens: both blocks together, or with many groups one after the other, which takes fewer registers
 template <int NT, bool kEdge>
-__device__ __forceinline__ void attend_unit(float (&o)[NT][8][4], float (&m)[NT][2], float (&l)[NT][2], const QueryRows<NT>& x, const uint8_t* unit, uint32_t tok0, const uint4* q_shared, uint32_t length) {
+__device__ __forceinline__ void attend_unit(float (&o)[NT][8][4], float (&m)[NT][2], float (&l)[NT][2], const QueryRows<NT>& x, const uint8_t* unit, uint32_t tok0, const uint4* q_shared, uint32_t length, Exponents& seen) {
     if constexpr (NT <= kTogether) {
-        attend_blocks<NT, 2, kEdge>(o, m, l, x, unit, tok0, q_shared, length);
+        attend_blocks<NT, 2, kEdge>(o, m, l, x, unit, tok0, q_shared, length, seen);
     } else {
 #pragma unroll 1
-        for (uint32_t b = 0; b < 2u && (!kEdge || tok0 + b * kBlockTokens < length); ++b) attend_blocks<NT, 1, kEdge>(o, m, l, x, unit + b * kBlockBytes, tok0 + b * kBlockTokens, q_shared, length);
+        for (uint32_t b = 0; b < 2u && (!kEdge || tok0 + b * kBlockTokens < length); ++b) attend_blocks<NT, 1, kEdge>(o, m, l, x, unit + b * kBlockBytes, tok0 + b * kBlockTokens, q_shared, length, seen);
     }
 }
 
@@ -422,14 +445,15 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) kv8_attend_kernel(c
             for (int i = 0; i < 8; ++i) o[g][i][0] = o[g][i][1] = o[g][i][2] = o[g][i][3] = 0.0f;
         }
         bool ok = true;
+        Exponents seen = {kNone, false};
 #pragma unroll 1
         for (uint32_t k = 0; k < units; ++k) {
             ok = __all_sync(0xFFFFFFFFu, sm100::mbar_wait(full0 + 8u * stage, phase, &sh.failed));
             if (!ok) break;
             const uint32_t tok0 = start + k * kStepTokens;
             const uint8_t* unit = sh.ring[warp][stage];
-            if (tok0 + kUnit <= low) attend_unit<NT, false>(o, m, l, x, unit, tok0, sh.q, length);
-            else attend_unit<NT, true>(o, m, l, x, unit, tok0, sh.q, length);
+            if (tok0 + kUnit <= low) attend_unit<NT, false>(o, m, l, x, unit, tok0, sh.q, length, seen);
+            else attend_unit<NT, true>(o, m, l, x, unit, tok0, sh.q, length, seen);
             __syncwarp();   // the warp is done with the stage
             if (k + kStages < units) issue(k + kStages, stage);
             if (++stage == kStages) stage = 0u, phase ^= 1u;
@@ -486,7 +510,11 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) kv8_attend_kernel(c
                 const float top = fmaxf(fmaxf(sh.m[0][8 * g + r], sh.m[1][8 * g + r]), fmaxf(sh.m[2][8 * g + r], sh.m[3][8 * g + r]));
                 float total = 0.0f, acc[8];
 #pragma unroll
-                for (unsigned w = 0; w < kWarps; ++w) total = fmaf(sh.l[w][8 * g + r], ex2(sh.m[w][8 * g + r] - top), total);
+                for (unsigned w = 0; w < kWarps; ++w) {
+                    float l_w = sh.l[w][8 * g + r];
+                    const float f = sum_factor(l_w, sh.m[w][8 * g + r] - top);
+                    total = fmaf(l_w, f, total);
+                }
 #pragma unroll
                 for (uint32_t y = 0; y < 2u; ++y) {
                     const uint32_t piece = (2u * (threadIdx.x & 15u) + y) ^ (r & 7u);
@@ -580,8 +608,10 @@ __global__ void __launch_bounds__(256) kv8_combine_columns_kernel(const __grid_c
         for (uint32_t k = 0; k < 2u; ++k) {
             if (w0 + k > last) break;
             const float pm = __uint_as_float(ml[k].x), top = fmaxf(m, pm), a = ex2(m - top), c = ex2(pm - top);
+            float pl = __uint_as_float(ml[k].y);
+            const float al = sum_factor(l, m - top), cl = sum_factor(pl, pm - top);
             m = top;
-            l = fmaf(l, a, __uint_as_float(ml[k].y) * c);
+            l = fmaf(l, al, pl * cl);
 #pragma unroll
             for (uint32_t y = 0; y < 4u; ++y) {
                 const uint4 v = raw[k][y];

@@ -67,7 +67,8 @@ struct Shared {
     uint8_t raw_k[kRawStages][kBlocks][kVCodes], raw_v[kRawStages][kBlocks][kMeta - kVCodes];   // a step's codes as they come
     uint4 meta[kRawStages][kBlocks];   // and its scales and masks
     uint32_t plain[kScaleSlots];       // whether every token of a step has numbers
-    alignas(16) float scales[kScaleSlots][3][8];   // of a step's blocks: scale of K, exponent e of V's, 2^-e
+    alignas(16) float scales[kScaleSlots][3][8];   // of a step's blocks: scale of K, exponent e of V's, 2^-e (0 in wide steps)
+    uint32_t wide[kScaleSlots];        // whether a step is (kv8.cuh)
     uint32_t nan_from[kSegmentSlots];  // of a segment: the first token that has NaN in its V, all ones where none has
     unsigned long long bars[kBars];
     Sums part[kThreads / 32];
@@ -134,6 +135,57 @@ __device__ __forceinline__ bool mbar_wait2(uint32_t a, uint32_t a_parity, uint32
 __device__ __forceinline__ uint4 to_f16(uint32_t lo, uint32_t hi) { return make_uint4(e4m3x2_lo(lo), e4m3x2_hi(lo), e4m3x2_lo(hi), e4m3x2_hi(hi)); }
 __device__ __forceinline__ uint4* piece_at(uint8_t* tile, uint32_t row, uint32_t piece) {   // 8 elements of a row of a tile
     return reinterpret_cast<uint4*>(tile + (piece >> 3) * kAtomBytes + row * 128u + (((piece & 7u) ^ (row & 7u)) << 4));
+}
+
+struct RowSums {
+    float m, l;
+};
+// A wide step's part of a row's sum (kv8.cuh): brings m to where the step will have it, O and l with it, and adds up the weights. All lanes, in front of the step, which does the rest; a function of its own,
+// since among the step's instructions it costs prompts that have no such steps another 2 us
+__device__ __noinline__ RowSums sum_wide(Shared& sh, uint32_t slot, uint32_t t_s, uint32_t t_o, float c_row, int seen, bool first, uint32_t product, uint32_t p_phase, RowSums now) {
+    float most = -INFINITY, m = now.m, l = now.l;
+#pragma unroll 1
+    for (uint32_t k = 0; k < 2u * kBlocks; ++k) {   // the largest, then the sums
+        const uint32_t b = k % kBlocks;
+        if (k == kBlocks) {
+            const bool over = most - kUpF > m + kSlack;
+            if (__any_sync(0xFFFFFFFFu, over)) {
+                const float next = over ? most - kUpF : m, f = ex2(m - next), fl = sum_factor(l, m - next);
+                m = next;
+                l *= fl;
+                if (!first) {
+                    (void)mbar_wait(product, p_phase, &sh.failed);   // (the step waits for it too: the parity stays)
+                    __syncwarp();
+                    tc_fence_after_sync();
+#pragma unroll 1
+                    for (uint32_t x = 0; x < 8u; ++x) {
+                        uint32_t o[16];
+                        tmem_ld16(t_o + 16u * x, o);
+                        tmem_wait_ld();
+                        reg_fence16(o);
+#pragma unroll
+                        for (int y = 0; y < 16; ++y) o[y] = __float_as_uint(__uint_as_float(o[y]) * f);
+                        tmem_st16(t_o + 16u * x, o);
+                    }
+                    tmem_wait_st();
+                }
+            }
+        }
+        uint32_t x[16];
+        tmem_ld16(t_s + 16u * b, x);
+        tmem_wait_ld();
+        reg_fence16(x);
+        const float c = fmaxf(c_row * sh.scales[slot][0][b], kLeast), up = static_cast<float>(kWide) - m;
+        float top = -INFINITY, sum = 0.0f;
+#pragma unroll
+        for (int z = 0; z < 16; ++z) {
+            const float y = z < seen - static_cast<int>(16u * b) ? __uint_as_float(x[z]) : -INFINITY;
+            top = fmaxf(top, y), sum += ex2_wide(fmaf(y, c, up));
+        }
+        if (k < kBlocks) most = fmaxf(most, fmaf(top, c, sh.scales[slot][1][b]));
+        else l = fmaf(sum, 1.0f / (1 << kWide), l);
+    }
+    return {m, l};
 }
 
 __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_constant__ Kv8AttendParams p, uint32_t row_tiles) {
@@ -237,6 +289,19 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
                 return sh.plan[slot].seg.steps > 0u && ask_rows(sh.plan[slot].seg, sh.plan[slot].n);
             };
             float c_row = 0.0f;
+            const auto rescale = [&](float f) {   // O
+#pragma unroll 1
+                for (uint32_t k = 0; k < 8u; ++k) {
+                    uint32_t o[16];
+                    tmem_ld16(t_o + 16u * k, o);
+                    tmem_wait_ld();
+                    reg_fence16(o);
+#pragma unroll
+                    for (int x = 0; x < 16; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * f);
+                    tmem_st16(t_o + 16u * k, o);
+                }
+                tmem_wait_st();
+            };
             Shared::Plan now;
             ok = ask_next();
             if (ok) c_row = take_rows();
@@ -258,9 +323,16 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
                     s_phase ^= 1u;
                     tc_fence_after_sync();
                     uint32_t s[kStep];
-                    tmem_ld32(t_s, *reinterpret_cast<uint32_t(*)[32]>(s));
-                    tmem_ld32(t_s + 32u, *reinterpret_cast<uint32_t(*)[32]>(s + 32));
-                    tmem_ld16(t_s + 64u, *reinterpret_cast<uint32_t(*)[16]>(s + 64));
+                    const auto load = [&]() {
+                        tmem_ld32(t_s, *reinterpret_cast<uint32_t(*)[32]>(s));
+                        tmem_ld32(t_s + 32u, *reinterpret_cast<uint32_t(*)[32]>(s + 32));
+                        tmem_ld16(t_s + 64u, *reinterpret_cast<uint32_t(*)[16]>(s + 64));
+                    };
+                    if (sh.wide[slot] != 0u) {
+                        const RowSums x = sum_wide(sh, slot, t_s, t_o, c_row, static_cast<int>(limit) - static_cast<int>((seg.first + j) * kStep), j == 0u, bar(kPFree + q), p_phase, {m, l});
+                        m = x.m, l = x.l;
+                    }
+                    load();
                     float c[kBlocks], shift[kBlocks], back[kBlocks];
 #pragma unroll
                     for (int k = 0; k < static_cast<int>(kBlocks); ++k) c[k] = fmaxf(c_row * sh.scales[slot][0][k], kLeast), shift[k] = sh.scales[slot][1][k], back[k] = sh.scales[slot][2][k];
@@ -302,19 +374,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
                         const float next = over ? most : m, f = ex2(m - next);
                         m = next;
                         l *= f;
-                        if (j > 0u) {
-#pragma unroll 1
-                            for (uint32_t k = 0; k < 8u; ++k) {
-                                uint32_t o[16];
-                                tmem_ld16(t_o + 16u * k, o);
-                                tmem_wait_ld();
-                                reg_fence16(o);
-#pragma unroll
-                                for (int x = 0; x < 16; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * f);
-                                tmem_st16(t_o + 16u * k, o);
-                            }
-                            tmem_wait_st();
-                        }
+                        if (j > 0u) rescale(f);
                     }
 #pragma unroll
                     for (int k = 0; k < static_cast<int>(kBlocks); ++k) {
@@ -639,6 +699,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
                     const Segment seg = now.seg;
                     uint32_t* nan_from = &sh.nan_from[(number - 1u) % kSegmentSlots];
                     if (lane == 0u) *nan_from = 0xFFFFFFFFu;
+                    int e_first = 0;   // of the segment's first block
+                    bool wide = false;
                     const uint32_t length = now.length;
                     for (uint32_t j = 0; j < seg.steps; ++j, ++step) {
                         const uint32_t raw = step % kRawStages, slot = step % kScaleSlots, t0 = (seg.first + j) * kStep + lane * kBlockTokens;
@@ -646,11 +708,13 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
                         ok = __all_sync(0xFFFFFFFFu, mbar_wait(bar(kRawFull + raw), step / kRawStages & 1u, failed));
                         if (!ok) break;
                         const uint4 meta = live != 0u ? sh.meta[raw][lane] : make_uint4(0x3F800000u, 0x3F800000u, 0u, 0u);
+                        const int e = exponent_of(meta.y);
+                        if (j == 0u) e_first = __shfl_sync(0xFFFFFFFFu, e, 0);
+                        wide |= __any_sync(0xFFFFFFFFu, live != 0u && !is_near(e, e_first));
                         const bool plain = !__any_sync(0xFFFFFFFFu, lane < kBlocks && (live != 0xFFFFu || meta.z != 0u));
                         if (lane < kBlocks) {
                             float* of = sh.scales[slot][0] + lane;
-                            const int e = exponent_of(meta.y);
-                            of[0] = __uint_as_float(meta.x), of[8] = static_cast<float>(e), of[16] = power_of(-e);
+                            of[0] = __uint_as_float(meta.x), of[8] = static_cast<float>(e), of[16] = wide ? 0.0f : power_of(-e);
                         }
                         uint32_t first = 0xFFFFFFFFu;
                         if (!plain) {
@@ -659,7 +723,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
                         }
                         __syncwarp();
                         if (lane == 0u) {
-                            sh.plain[slot] = plain;
+                            sh.plain[slot] = plain, sh.wide[slot] = wide;
                             if (first < *nan_from) *nan_from = first;
                             mbar_arrive(bar(kScales + slot));
                         }

@@ -239,41 +239,88 @@ Extent extent_of(const fmha_rope_rows& r, const fmha_rope_args& a, uint32_t head
     const uint64_t begin = reinterpret_cast<uintptr_t>(r.data);
     return {begin, begin + size * ((a.B - 1u) * static_cast<uint64_t>(r.stride_b) + (a.S - 1u) * static_cast<uint64_t>(r.stride_s) + (heads - 1u) * static_cast<uint64_t>(r.stride_h) + a.head_dim)};
 }
-// whether no element stands twice: each dimension's stride, in their order, is as long as what lies within it
-bool distinct(const fmha_rope_rows& r, const fmha_rope_args& a, uint32_t heads) {
-    struct {
-        uint64_t stride, size;
-    } d[3] = {{static_cast<uint64_t>(r.stride_b), a.B}, {static_cast<uint64_t>(r.stride_s), a.S}, {static_cast<uint64_t>(r.stride_h), heads}};
-    for (int i = 0; i < 2; ++i) {
-        for (int j = 0; j < 2 - i; ++j) {
-            if (d[j].stride > d[j + 1].stride) {
-                const auto t = d[j];
-                d[j] = d[j + 1], d[j + 1] = t;
+
+// Whether two rows of places have an element in common: count * stride, summed over the dimensions, comes within a row's length of `distance` for some counts of their ranges, in elements. From the longest stride
+// down, only counts that the shorter ones can make up for are looked at: one or two a dimension in layouts that are nested as usual. Layouts that take more steps than kMostLooks count as overlapping.
+struct Dimension {
+    int64_t stride, least, most;   // counts
+};
+constexpr uint32_t kMostLooks = 1u << 16;
+struct Places {
+    int64_t row;    // elements of a row - 1
+    bool itself;    // the places of one tensor, against themselves: counts of 0 throughout are no meeting
+    int n;
+    uint32_t looks;
+    Dimension d[6];
+    void add(int64_t stride, int64_t least, int64_t most) {
+        if (least == most || (stride == 0 && !itself)) return;
+        for (int i = 0; i < n && !itself; ++i) {
+            if (d[i].stride != stride) continue;
+            d[i].least += least, d[i].most += most;
+            return;
+        }
+        int at = n++;
+        for (; at > 0 && d[at - 1].stride < stride; --at) d[at] = d[at - 1];
+        d[at] = {stride, least, most};
+    }
+    bool meet(int64_t distance, int from = 0, bool moved = false) {
+        if (from == n) return (moved || !itself) && distance <= row && -distance <= row;
+        if (++looks > kMostLooks) return true;
+        int64_t low = -row, high = row;   // what the dimensions behind reach
+        for (int i = from + 1; i < n; ++i) low += d[i].stride * d[i].least, high += d[i].stride * d[i].most;
+        const Dimension& x = d[from];
+        int64_t begin = x.least, end = x.most;
+        if (x.stride != 0) {
+            const auto floor_div = [](int64_t a, int64_t b) { return a / b - (a % b < 0 ? 1 : 0); };
+            const int64_t first = -floor_div(high - distance, x.stride), last = floor_div(distance - low, x.stride);
+            begin = begin > first ? begin : first, end = end < last ? end : last;
+        }
+        for (int64_t k = begin; k <= end; ++k) {
+            if (meet(distance - k * x.stride, from + 1, moved || k != 0)) return true;
+        }
+        return false;
+    }
+};
+// whether each dimension's stride, from the shortest on, is as long as what lies within it: the usual layouts, known without the search (0.2 us of a call's host time)
+bool nested(Dimension (&d)[3], int n, uint64_t inner) {
+    for (int i = 0; i < n; ++i) {
+        for (int k = i + 1; k < n; ++k) {
+            if (d[k].stride < d[i].stride) {
+                const Dimension t = d[i];
+                d[i] = d[k], d[k] = t;
             }
         }
-    }
-    uint64_t inner = a.head_dim;
-    for (int i = 0; i < 3; ++i) {
-        if (d[i].size == 1u) continue;
-        if (d[i].stride < inner) return false;
-        inner = d[i].stride * (d[i].size - 1u) + inner;
+        if (d[i].most == 0) continue;
+        if (static_cast<uint64_t>(d[i].stride) < inner) return false;
+        inner += static_cast<uint64_t>(d[i].stride) * static_cast<uint64_t>(d[i].most);
     }
     return true;
 }
-// Whether two tensors' elements are kept apart, as far as it shows: they lie behind one another, or they are heads of the same tokens' rows that do
+// whether no element stands twice
+bool distinct(const fmha_rope_rows& r, const fmha_rope_args& a, uint32_t heads) {
+    Dimension d[3] = {{r.stride_b, 0, a.B - 1ll}, {r.stride_s, 0, a.S - 1ll}, {r.stride_h, 0, heads - 1ll}};
+    if (nested(d, 3, a.head_dim)) return true;
+    Places x = {};
+    x.row = a.head_dim - 1, x.itself = true;
+    for (const Dimension& y : d) x.add(y.stride, -y.most, y.most);
+    return !x.meet(0);
+}
+// whether two tensors have no element in common
 bool apart(const fmha_rope_rows& r, uint32_t r_heads, const fmha_rope_rows& q, uint32_t q_heads, const fmha_rope_args& a, uint64_t size) {
     const Extent x = extent_of(r, a, r_heads, size), y = extent_of(q, a, q_heads, size);
     if (x.end <= y.begin || y.end <= x.begin) return true;
-    if ((a.B > 1u && r.stride_b != q.stride_b) || (a.S > 1u && r.stride_s != q.stride_s)) return false;
-    const bool first = x.begin < y.begin;
-    const uint64_t ahead = first ? y.begin - x.begin : x.begin - y.begin;
-    const uint64_t front = size * ((first ? r_heads - 1u : q_heads - 1u) * static_cast<uint64_t>(first ? r.stride_h : q.stride_h) + a.head_dim);
-    const uint64_t back = size * ((first ? q_heads - 1u : r_heads - 1u) * static_cast<uint64_t>(first ? q.stride_h : r.stride_h) + a.head_dim);
-    // the token's part in front ends where the other begins, and that ends in front of the next token's
-    uint64_t next = ~0ull;
-    if (a.S > 1u) next = size * static_cast<uint64_t>(r.stride_s);
-    if (a.B > 1u && size * static_cast<uint64_t>(r.stride_b) < next) next = size * static_cast<uint64_t>(r.stride_b);
-    return ahead >= front && ahead + back <= next;
+    const int64_t distance = static_cast<int64_t>(y.begin - x.begin) / static_cast<int64_t>(size);
+    if (r.stride_b == q.stride_b && r.stride_s == q.stride_s) {   // a token's heads of both as one row
+        const uint64_t r_row = (r_heads - 1ull) * static_cast<uint64_t>(r.stride_h) + a.head_dim, q_row = (q_heads - 1ull) * static_cast<uint64_t>(q.stride_h) + a.head_dim;
+        const uint64_t ahead = static_cast<uint64_t>(distance < 0 ? -distance : distance);
+        Dimension d[3] = {{r.stride_b, 0, a.B - 1ll}, {r.stride_s, 0, a.S - 1ll}, {}};
+        if (ahead >= (distance < 0 ? q_row : r_row) && nested(d, 2, ahead + (distance < 0 ? r_row : q_row))) return true;
+    }
+    Places z = {};
+    z.row = a.head_dim - 1;
+    z.add(r.stride_b, 0, a.B - 1ll), z.add(r.stride_s, 0, a.S - 1ll), z.add(r.stride_h, 0, r_heads - 1ll);
+    z.add(q.stride_b, 1ll - a.B, 0), z.add(q.stride_s, 1ll - a.S, 0), z.add(q.stride_h, 1ll - q_heads, 0);
+    return !z.meet(distance);
 }
 
 int check_rows(const fmha_rope_rows& r, const fmha_rope_args& a, uint32_t heads, uint64_t size, const char* name, char* err, size_t cap) {

@@ -120,7 +120,8 @@ class RopeArgs(C.Structure):
 
 class PagesArgs(C.Structure):
     """fmha_pages"""
-    _fields_ = [("free", C.c_void_p), ("table", C.c_void_p), ("lengths", C.c_void_p), ("pages", C.c_uint32), ("B", C.c_uint32), ("page", C.c_uint32), ("table_width", C.c_uint32)]
+    _fields_ = [("free", C.c_void_p), ("table", C.c_void_p), ("lengths", C.c_void_p), ("pages", C.c_uint32), ("B", C.c_uint32), ("page", C.c_uint32), ("table_width", C.c_uint32),
+                ("pool_pages", C.c_uint32)]
 
 
 assert C.sizeof(AttnArgs) == 656 and C.sizeof(KvSplitArgs) == 648 and C.sizeof(CombineArgs) == 36

@@ -1,9 +1,9 @@
 // Page tables, lengths, positions and slot maps from the numbers of new tokens (include/fmha_pages_abi.h).
 //
-// Every CTA goes over all sequences' lengths and counts for itself, two sums over them (pages needed in front of a sequence, tokens granted in front of it), and then writes its share
+// Of a take every CTA goes over all sequences' lengths and counts for itself, two sums over them (pages needed in front of a sequence, tokens granted in front of it), and then writes its share
 // of the maps and of the table; what all of them read, the lengths and the stack's height, is written by the one that is done last. So a call is one launch in which nothing waits for
-// another CTA: a decode step is one CTA and a few trips to memory, the maps of whole prompts get as many CTAs as keep memory busy. Bound by these trips and the launch: on the device, taken and cut
-// back, 256 x 1 tokens 11.1 us (a cut of nothing 3.6), 64 prompts to 2048 tokens 14.1 for 1.6 MB of maps, four of a thread's rows in flight (14.5 one by one; 256 x 8 tokens 12.9 and 14.0).
+// another CTA: a decode step is one CTA and a few trips to memory, the maps of whole prompts get as many CTAs as keep memory busy. A cut is one CTA. Bound by these trips and the launch: on the device, taken and cut
+// back, 256 x 1 tokens 9.2 us (a cut of nothing 2.2), 256 x 8 11.3, 64 prompts to 2048 tokens 13.0 for 1.6 MB of maps, four of a thread's rows in flight.
 #include "../../include/fmha_pages_abi.h"
 #include "cache_args.cuh"
 
@@ -12,11 +12,12 @@ namespace b200mx {
 namespace {
 
 constexpr uint32_t kThreads = 512, kWarps = kThreads / 32, kMostRange = 1024;   // sequences of a CTA
-constexpr uint32_t kTogether = 4;                                               // rows of the maps of a thread at a time
+constexpr uint32_t kTogether = 4;                                               // rows of the maps, or entries of the table, of a thread at a time
+constexpr uint32_t kParts = 4;                                                  // of a warp, whose entries stay in registers
 
 struct PagesParams {
     int32_t *free, *table, *lengths;
-    uint32_t pages, B, page_log2, table_width;
+    uint32_t pages, pool_pages, B, page_log2, table_width;
     const int32_t* asked;   // counts, or what to keep
     int32_t *granted, *starts;
     void* positions;
@@ -197,45 +198,128 @@ __global__ void __launch_bounds__(kThreads) pages_take_kernel(const __grid_const
     }
 }
 
+// One CTA, from the last sequences to the first, a thread's one at a time. What goes back is counted first, since entries that name no page do not: a sequence's one page by its thread, more by warps.
 __global__ void __launch_bounds__(kThreads) pages_cut_kernel(const __grid_constant__ PagesParams p) {
-    __shared__ unsigned long long part64[kWarps];
-    __shared__ uint32_t sm_kept[kMostRange + 2], sm_pages[kMostRange + 2];   // pages that stay, pages that there were
-    __shared__ unsigned long long sm_behind[kMostRange + 2];                 // pages that the sequences behind give back
-    __shared__ uint32_t last_flag;
+    __shared__ unsigned long long part64[kWarps], sm_to[kThreads];   // sm_to: height at which a sequence's last page goes back
+    __shared__ uint32_t sm_kept[kThreads], sm_many[kThreads], sm_count[kThreads];
     kv4::pdl_launch();
     kv4::pdl_wait();
-    const uint32_t per = (p.B + kThreads - 1u) / kThreads, b0 = min(threadIdx.x * per, p.B), b1 = min(b0 + per, p.B), n_free = height(p);
-    const uint32_t length0 = b0 < b1 ? length_at(p, b0) : 0u, asked0 = b0 < b1 ? asked_at(p, b0) : 0u;
-    uint32_t had, kept, length_now, keep_now;
-    const auto look = [&](uint32_t b, uint32_t& had, uint32_t& kept) {
-        length_now = b == b0 ? length0 : length_at(p, b), keep_now = b == b0 ? asked0 : asked_at(p, b);
-        had = pages_of(p, length_now), kept = pages_of(p, min(length_now, keep_now));
-        return had - kept;
-    };
-    const bool alone = gridDim.x == 1u;
-    unsigned long long mine = 0, all;
-    for (uint32_t b = b0; b < b1; ++b) mine += look(b, had, kept);
-    unsigned long long upto = sum_in_front(mine, part64, all);
-    const Range range = own_range(p);
-    for (uint32_t b = b0; b < b1; ++b) {
-        upto += look(b, had, kept);
-        if (alone) p.lengths[b] = static_cast<int32_t>(min(length_now, keep_now));   // (each thread has read its own)
-        if (b >= range.begin && b < range.end) sm_kept[b - range.begin] = kept, sm_pages[b - range.begin] = had, sm_behind[b - range.begin] = all - upto;
+    const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5, n_free = height(p);
+    const auto names_page = [&](int entry) { return entry >= 0 && static_cast<uint32_t>(entry) < p.pool_pages; };
+    unsigned long long given = 0;   // pages of the sequences behind
+    for (uint32_t end = p.B, n; end > 0u; end -= n) {
+        n = min(end, kThreads);
+        const uint32_t first = end - n, x = threadIdx.x, b = first + x;
+        uint32_t kept = 0, many = 0, count = 0;
+        bool one = false;
+        int entry = -1;
+        if (x < n) {
+            const uint32_t length = length_at(p, b), keep = min(length, asked_at(p, b)), had = pages_of(p, length);
+            kept = pages_of(p, keep);
+            one = had - kept == 1u, many = one ? 0u : had - kept;
+            if (one) entry = ld_now(p.table + static_cast<size_t>(b) * p.table_width + kept);
+            p.lengths[b] = static_cast<int32_t>(keep);   // (each thread has read its own)
+            count = names_page(entry);
+        }
+        sm_kept[x] = kept, sm_many[x] = many;
+        // Sequences of more than one page are cut up into parts, a warp's every kWarps-th; a part's entries are looked at kTogether of a lane at a time. Where a warp has kParts parts of one such look at most,
+        // all of them are under way together and stay in registers until they are written (64 sequences of up to 128 pages taken and cut: 13.0 us of the device, 14.7 in the loop)
+        const uint32_t parts_log2 = n >= kWarps ? 0u : 31u - static_cast<uint32_t>(__clz(static_cast<int>(kWarps / n))), parts = 1u << parts_log2;
+        const bool any = __syncthreads_or(many != 0u) != 0, few = any && n * parts <= kParts * kWarps && __syncthreads_or(many > 32u * kTogether * parts) == 0;
+        struct Part {
+            int32_t* row;
+            uint32_t of, y;
+        };
+        const auto part_of = [&](uint32_t u) {
+            const uint32_t y = u < n * parts ? u >> parts_log2 : 0u, part = u - y * parts, of = u < n * parts ? sm_many[y] : 0u;
+            const auto at = [&](uint32_t k) { return static_cast<uint32_t>(static_cast<unsigned long long>(of) * k >> parts_log2); };
+            return Part{p.table + static_cast<size_t>(first + y) * p.table_width + sm_kept[y] + at(part), at(part + 1u) - at(part), y};
+        };
+        const auto look = [&](const Part& part, uint32_t k0, int (&e)[kTogether]) {
+#pragma unroll
+            for (uint32_t k = 0; k < kTogether; ++k) e[k] = k0 + 32u * k + lane < part.of ? ld_now(part.row + k0 + 32u * k + lane) : -1;
+        };
+        const auto pages_in = [&](const int (&e)[kTogether]) {
+            uint32_t pages = 0;
+#pragma unroll
+            for (uint32_t k = 0; k < kTogether; ++k) pages += static_cast<uint32_t>(__popc(__ballot_sync(0xFFFFFFFFu, names_page(e[k]))));
+            return pages;
+        };
+        // entries go back from the height `above` down
+        const auto give_back = [&](const Part& part, uint32_t k0, const int (&e)[kTogether], unsigned long long& above) {
+#pragma unroll
+            for (uint32_t k = 0; k < kTogether; ++k) {
+                const uint32_t pages = __ballot_sync(0xFFFFFFFFu, names_page(e[k]));
+                const unsigned long long at = above - 1u - static_cast<uint32_t>(__popc(pages & ((1u << lane) - 1u)));
+                if (names_page(e[k]) && at < p.pages) p.free[4u + at] = e[k];
+                if (k0 + 32u * k + lane < part.of) part.row[k0 + 32u * k + lane] = -1;
+                above -= static_cast<uint32_t>(__popc(pages));
+            }
+        };
+        const auto height_of = [&](const Part& part, uint32_t u) {   // behind the parts behind
+            unsigned long long above = sm_to[part.y];
+            for (uint32_t k = u; k < (part.y + 1u) * parts; ++k) above += sm_count[k];
+            return above;
+        };
+        int held[kParts][kTogether];
+        if (few) {
+#pragma unroll
+            for (uint32_t i = 0; i < kParts; ++i) look(part_of(warp + i * kWarps), 0u, held[i]);
+#pragma unroll
+            for (uint32_t i = 0; i < kParts; ++i) {
+                const uint32_t pages = pages_in(held[i]);
+                if (lane == 0u && warp + i * kWarps < n * parts) sm_count[warp + i * kWarps] = pages;
+            }
+        } else if (any) {
+            for (uint32_t u = warp; u < n * parts; u += kWarps) {
+                const Part part = part_of(u);
+                uint32_t pages = 0;
+                for (uint32_t k0 = 0; k0 < part.of; k0 += 32u * kTogether) {
+                    int e[kTogether];
+                    look(part, k0, e);
+                    pages += pages_in(e);
+                }
+                if (lane == 0u) sm_count[u] = pages;
+            }
+        }
+        if (any) {
+            __syncthreads();
+            for (uint32_t k = 0; k < parts && many != 0u; ++k) count += sm_count[x * parts + k];
+        }
+        unsigned long long all;
+        const unsigned long long in_front = sum_in_front<unsigned long long>(count, part64, all), to = n_free + given + (all - in_front - count);
+        if (one) {
+            if (count != 0u && to < p.pages) p.free[4u + to] = entry;
+            p.table[static_cast<size_t>(b) * p.table_width + kept] = -1;
+        }
+        if (any) {
+            sm_to[x] = to;
+            __syncthreads();
+        }
+        if (few) {
+#pragma unroll
+            for (uint32_t i = 0; i < kParts; ++i) {
+                const uint32_t u = warp + i * kWarps;
+                if (u >= n * parts) break;
+                const Part part = part_of(u);
+                unsigned long long above = height_of(part, u);
+                give_back(part, 0u, held[i], above);
+            }
+        } else if (any) {
+            for (uint32_t u = warp; u < n * parts; u += kWarps) {
+                const Part part = part_of(u);
+                unsigned long long above = height_of(part, u);
+                for (uint32_t k0 = 0; k0 < part.of; k0 += 32u * kTogether) {
+                    int e[kTogether];
+                    look(part, k0, e);
+                    give_back(part, k0, e, above);
+                }
+            }
+        }
+        given += all;
+        __syncthreads();   // (the tables are the next sequences')
     }
-    __syncthreads();
-    for_pages(
-        range.end - range.begin, [&](uint32_t x) { return sm_pages[x] - sm_kept[x]; },
-        [&](uint32_t x, uint32_t k) {
-            int32_t* entry = p.table + static_cast<size_t>(range.begin + x) * p.table_width + sm_kept[x] + k;
-            const unsigned long long to = n_free + sm_behind[x] + (sm_pages[x] - sm_kept[x] - 1u - k);
-            if (to < p.pages) p.free[4u + to] = ld_now(entry);
-            *entry = -1;
-        });
-    if (!is_last(p, &last_flag)) return;
-    if (!alone) {
-        for (uint32_t b = threadIdx.x; b < p.B; b += kThreads) p.lengths[b] = static_cast<int32_t>(min(length_at(p, b), asked_at(p, b)));
-    }
-    if (threadIdx.x == 0u) p.free[0] = static_cast<int32_t>(min(n_free + all, static_cast<unsigned long long>(p.pages)));
+    if (threadIdx.x == 0u) p.free[0] = static_cast<int32_t>(min(n_free + given, static_cast<unsigned long long>(p.pages)));
 }
 
 }  // namespace
@@ -251,7 +335,7 @@ int params_of(const fmha_pages* p, const char* name, PagesParams& r, char* err, 
     if (p->B == 0u || p->pages == 0u || p->table_width == 0u) return refuse(err, cap, "%s: no sequences, pages or table columns", name);
     if (p->pages > 0x7FFFFFF0u || p->B > kMostRows || static_cast<uint64_t>(p->table_width) * p->page > 0x7FFFFFFFull) return refuse(err, cap, "%s: more than 2^31 pages or tokens of a sequence, or 2^30 sequences", name);
     r.free = p->free, r.table = p->table, r.lengths = p->lengths;
-    r.pages = p->pages, r.B = p->B, r.table_width = p->table_width;
+    r.pages = p->pages, r.pool_pages = p->pool_pages != 0u ? p->pool_pages : 0x80000000u, r.B = p->B, r.table_width = p->table_width;
     r.page_log2 = p->page == 16u ? 4u : p->page == 32u ? 5u : p->page == 64u ? 6u : 7u;
     return 0;
 }
@@ -306,7 +390,7 @@ int fmha_pages_cut(const fmha_pages* pages, const int32_t* keep, void* stream, c
     const Span s[] = {{p.free, 4ull * (p.pages + 4ull), "the stack"}, {p.table, 4ull * p.B * p.table_width, "the table"}, {p.lengths, 4ull * p.B, "the lengths"}, {keep, 4ull * p.B, "keep"}};
     if (int r = check_apart(s, 4, 3, "cut", err, cap)) return r;
     p.asked = keep;
-    return done(b200mx::kv4_launch(b200mx::pages_cut_kernel, dim3(grid_of(p.B, 0u)), b200mx::kThreads, 0, static_cast<cudaStream_t>(stream), p), err, cap);
+    return done(b200mx::kv4_launch(b200mx::pages_cut_kernel, dim3(1), b200mx::kThreads, 0, static_cast<cudaStream_t>(stream), p), err, cap);
 }
 
 }  // extern "C"

@@ -18,8 +18,8 @@ from .kv4 import PagedCache, _call, _check, _i32
 from .ops import _raw_stream
 
 
-_ARGS = struct.Struct("@3Q4I").pack   # fmha_pages, as bytes: half the time that a ctypes structure takes
-assert struct.calcsize("@3Q4I") == C.sizeof(_abi.PagesArgs)
+_ARGS = struct.Struct("@3Q5I4x").pack   # fmha_pages, as bytes: half the time that a ctypes structure takes
+assert struct.calcsize("@3Q5I4x") == C.sizeof(_abi.PagesArgs)
 _entries = {}
 
 
@@ -50,7 +50,7 @@ def _pages(who, free, cache):
     if pages > 0x7FFFFFFF:   # (here, in numbers of any size)
         raise ValueError(f"{who}: a stack of {pages} pages, more than 2^31")
     c = cache.c
-    return _ARGS(free.data_ptr(), c.table, c.lengths, pages, c.B, c.page, c.table_width)
+    return _ARGS(free.data_ptr(), c.table, c.lengths, pages, c.B, c.page, c.table_width, c.pages)
 
 
 def _map(name, x, kind, cache):
@@ -98,7 +98,8 @@ def pages_take(free, cache, counts, granted, *, positions=None, slots=None, star
 
 
 def pages_cut(free, cache, keep, *, stream=None):
-    """Cuts every sequence to ``keep[b]`` (int32 [B]) tokens, if it has more; its pages without tokens go back to the stack, and their entries in the table become -1.
+    """Cuts every sequence to ``keep[b]`` (int32 [B]) tokens, if it has more; its pages without tokens go back to the stack, and their entries in the table become -1. (Entries that
+    name no page of the pool give none back.)
 
     A cut to the lengths before a ``pages_take`` leaves stack, table and lengths as they were before it. ``keep`` of 0 ends a sequence."""
     import torch

@@ -23,6 +23,7 @@ typedef struct fmha_pages {
     int32_t* lengths;    /* [B] */
     uint32_t pages;      /* that the stack has room for */
     uint32_t B, page, table_width;
+    uint32_t pool_pages; /* of the pool that the table's entries are pages of: others below 0 or from there on name none. 0: not known, all from 0 on do */
 } fmha_pages;
 
 /*
@@ -35,7 +36,8 @@ typedef struct fmha_pages {
  *   starts: NULL or int32 [B + 1]: sums of granted in front of each sequence, and of all. (pages + B) * page is below 2^31 then.
  *   granted, positions, slots and starts share no memory with counts, the stack, the table, the lengths or one another.
  * cut: lengths[b] becomes min(length, max(keep[b], 0)); pages without tokens go back to the stack, their table entries become -1. The last sequence's last page goes onto it first: a cut
- *   to the lengths before a take leaves stack, table and lengths as they were before it. Pages that the stack has no room for are dropped. keep shares no memory with the others.
+ *   to the lengths before a take leaves stack, table and lengths as they were before it. Entries that name no page give none back. Pages that the stack has no room for are dropped. keep shares
+ *   no memory with the others.
  */
 int fmha_pages_take(const fmha_pages* p, const int32_t* counts, int32_t* granted, void* positions, int positions_64, int64_t* slots, int32_t* starts, uint32_t S, void* stream, char* err, size_t cap);
 int fmha_pages_cut(const fmha_pages* p, const int32_t* keep, void* stream, char* err, size_t cap);

@@ -56,7 +56,8 @@ def kv8_append(cache, k, v, *, counts=None, stream=None):
     Row i of sequence b becomes token ``lengths[b] - n + i``, with n = S, or ``counts[b]`` (int32 [B]) of the S rows where the sequences have different numbers of
     new tokens, and never more than the length. The lengths are the caller's to raise, before this call (``pages_take`` does). Per 16 tokens and head one scale for K
     and one for V, the smallest power of two that leaves no element above 448 of it; elements e4m3, rounded to nearest, ties to even. A block that has tokens already keeps
-    its scale, or its tokens' codes move to a larger one, which costs bits only below 2^-6 of that. (Sequences may share pages that are full; a page that one of them still fills is its own.)
+    its scale, or its tokens' codes move to a larger one, which costs bits only below 2^-6 of that. (Sequences may share pages that are full, as long as nobody takes those back:
+    ``pages_cut`` does not count their users. A page that one of them still fills is its own.)
     A token with Inf or NaN in its K (V) reads as NaN there throughout."""
     import torch
     _is_kv8("kv8_append", cache)

@@ -101,7 +101,10 @@ def pages_cut(free, cache, keep, *, stream=None):
     """Cuts every sequence to ``keep[b]`` (int32 [B]) tokens, if it has more; its pages without tokens go back to the stack, and their entries in the table become -1. (Entries that
     name no page of the pool give none back.)
 
-    A cut to the lengths before a ``pages_take`` leaves stack, table and lengths as they were before it. ``keep`` of 0 ends a sequence."""
+    A cut to the lengths before a ``pages_take`` leaves stack, table and lengths as they were before it. ``keep`` of 0 ends a sequence.
+
+    Nobody counts a page's users: every page behind ``keep`` is handed out again. Pages that other sequences hold too (a prefix in common) have to lie in front of ``keep``: such a sequence ends with
+    ``keep`` at the prefix's end, and the prefix's pages are the caller's to give back when nobody holds them any more."""
     import torch
     p = _pages("pages_cut", free, cache)
     if keep is None:

@@ -38,6 +38,8 @@ typedef struct fmha_pages {
  * cut: lengths[b] becomes min(length, max(keep[b], 0)); pages without tokens go back to the stack, their table entries become -1. The last sequence's last page goes onto it first: a cut
  *   to the lengths before a take leaves stack, table and lengths as they were before it. Entries that name no page give none back. Pages that the stack has no room for are dropped. keep shares
  *   no memory with the others.
+ *   Nobody counts a page's users: every page behind keep goes back, and is handed out again. Pages that other sequences hold too (a prefix in common) have to lie in front of keep; they, and the
+ *   last sequence that holds them, are the caller's to look after.
  */
 int fmha_pages_take(const fmha_pages* p, const int32_t* counts, int32_t* granted, void* positions, int positions_64, int64_t* slots, int32_t* starts, uint32_t S, void* stream, char* err, size_t cap);
 int fmha_pages_cut(const fmha_pages* p, const int32_t* keep, void* stream, char* err, size_t cap);

@@ -46,6 +46,40 @@ class PagedBatch:
         pages_cut(self.free, self.caches[0], keep)
 
 
+class Requests:
+    """What the host knows of the sequences' requests: a list [tokens of the prompt, tokens in all] each, which ``new()`` makes, and how far each one is.
+
+    One that is put off for want of pages starts again, prompt and all, when another is over: at once it would take the pages that it was put off for."""
+
+    def __init__(self, sequences, new):
+        self.new, self.now = new, [new() for _ in range(sequences)]
+        self.lengths, self.waits = [0] * sequences, [False] * sequences
+        self.finished, self.put_off = [], 0
+
+    def ask(self, chunk):
+        """New tokens of each sequence: prompts a chunk at a time beside the others' single tokens."""
+        return [0 if wait else min(chunk, r[0] - n) if n < r[0] else 1 for n, r, wait in zip(self.lengths, self.now, self.waits)]
+
+    def step(self, granted):
+        """What becomes of the sequences: whether each is cut to nothing, or None where none is."""
+        self.lengths = [n + got for n, got in zip(self.lengths, granted)]
+        over = [n >= r[1] for n, r in zip(self.lengths, self.now)]
+        for b, done in enumerate(over):
+            if done:
+                self.finished.append(self.now[b])
+                self.lengths[b], self.now[b] = 0, self.new()
+        if any(over):
+            self.waits = [False] * len(over)
+            return over
+        if any(granted):
+            return None
+        # where nobody gets any further, the longest makes room
+        b = max(range(len(over)), key=self.lengths.__getitem__)
+        self.lengths[b], self.waits[b] = 0, True
+        self.put_off += 1
+        return [x == b for x in range(len(over))]
+
+
 def main(argv=None):
     import torch
     parser = argparse.ArgumentParser(description="Requests of random lengths served from a paged 8-bit cache")
@@ -53,18 +87,19 @@ def main(argv=None):
         parser.add_argument("--" + name, type=int, default=value)
     a = parser.parse_args(argv)
     B, longest = a.sequences, a.prompt + a.tokens
+    if a.pages < -(-longest // 64):
+        parser.error(f"{a.pages} pages are too few for one request of {longest} tokens")
     batch = PagedBatch(B, a.layers, a.kv_heads, a.pages, longest, Rope(128, scaling={"kind": "yarn", "factor": 4.0, "original": 4096}))
     g = torch.Generator().manual_seed(1)
-    # a request: tokens of its prompt, tokens in all. Both of the host's lists are what the host knows; the device's lengths say how far each one is
-    new = lambda: [int(torch.randint(1, a.prompt + 1, (1,), generator=g)), 0]
-    requests = [new() for _ in range(B)]
-    for r in requests:
-        r[1] = r[0] + int(torch.randint(1, a.tokens + 1, (1,), generator=g))
-    lengths, finished, served, waits, us = [0] * B, 0, 0, 0, []
+
+    def new():
+        prompt = int(torch.randint(1, a.prompt + 1, (1,), generator=g))
+        return [prompt, prompt + int(torch.randint(1, a.tokens + 1, (1,), generator=g))]
+
+    requests, served, waits, us = Requests(B, new), 0, 0, []
     projections = {rows: torch.randn(B, rows, a.heads + 2 * a.kv_heads, 128, device="cuda", dtype=torch.bfloat16) for rows in (1, a.chunk)}
     for step in range(a.steps):
-        # prompts a chunk at a time beside the others' single tokens
-        asked = [min(a.chunk, p - n) if n < p else 1 for n, (p, _) in zip(lengths, requests)]
+        asked = requests.ask(a.chunk)
         rows = 1 if max(asked) == 1 else a.chunk
         qkv, out = projections[rows], torch.empty(B, rows, a.heads, 128, device="cuda", dtype=torch.bfloat16)
         start, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
@@ -77,25 +112,16 @@ def main(argv=None):
         end.record()
         granted = batch.granted.tolist()
         us.append((rows, start.elapsed_time(end) * 1e3 / a.layers))
-        lengths = [n + got for n, got in zip(lengths, granted)]
         served += sum(granted)
         waits += sum(got < want for got, want in zip(granted, asked))
-        over = [n >= end_at for n, (_, end_at) in zip(lengths, requests)]
-        if any(over) or not any(granted):
-            # what is over goes; where nobody gets any further, the longest request starts again later
-            if not any(over):
-                over[max(range(B), key=lengths.__getitem__)] = True
+        over = requests.step(granted)
+        if over is not None:
             batch.cut(torch.tensor([0 if x else longest for x in over], dtype=torch.int32).cuda())
-            for b in range(B):
-                if over[b]:
-                    finished += lengths[b] >= requests[b][1]
-                    lengths[b], requests[b] = 0, new()
-                    requests[b][1] = requests[b][0] + int(torch.randint(1, a.tokens + 1, (1,), generator=g))
     for rows in projections:
         times = sorted(t for r, t in us if r == rows)
         if times:
             print(f"{len(times)} steps of {rows} rows: {times[len(times) // 2]:.1f} us a layer (median), projections' copy included")
-    print(f"{served} tokens, {finished} requests finished, {waits} times one waited for pages; {int(batch.free[0])} of {a.pages} pages free")
+    print(f"{served} tokens, {len(requests.finished)} requests finished, {waits} times one waited for pages, {requests.put_off} times one was put off; {int(batch.free[0])} of {a.pages} pages free")
 
 
 if __name__ == "__main__":

@@ -129,6 +129,11 @@ def _call(torch, cache, stream, fn, *args):
         return fn(*args, stream, _errors.text, 256)
 
 
+def _is_kv4(who, cache, name="cache"):
+    if not isinstance(cache, Kv4Cache):   # (the 8-bit cache has the same fields, and other contents)
+        raise ValueError(f"{who}: {name} must be a Kv4Cache, not {type(cache).__name__}")
+
+
 def kv4_append(cache, k, v, *, counts=None, stream=None):
     """Rounds the newest tokens' keys and values into the cache: k, v bf16 [B, S, HK, 128] (slices of a wider projection are fine).
 
@@ -136,6 +141,7 @@ def kv4_append(cache, k, v, *, counts=None, stream=None):
     new tokens, and never more than the length. The lengths are the caller's to raise, before this call. Per 32 elements one E8M0 scale,
     floor(log2 of the largest) - 2, elements e2m1 rounded to nearest, ties to even, saturating at 6 times the scale; a block with Inf or NaN reads as NaN."""
     import torch
+    _is_kv4("kv4_append", cache)
     lib = _abi.load()
     rk = _rows("kv4_append", "k", k, cache, heads=cache.HK)
     rv = _rows("kv4_append", "v", v, cache, k.shape[1], cache.HK)
@@ -150,6 +156,7 @@ def kv4_read(cache, k, v, *, last=False, counts=None, stream=None):
     """The values that the cache holds, exact in bf16, into k, v [B, S, HK, 128]: tokens 0 .. S - 1, or with ``last`` the newest ones, row for row as
     ``kv4_append`` took them (``counts`` as there). Rows that stand for no token become zeros."""
     import torch
+    _is_kv4("kv4_read", cache)
     lib = _abi.load()
     rk = _rows("kv4_read", "k", k, cache, heads=cache.HK)
     rv = _rows("kv4_read", "v", v, cache, k.shape[1], cache.HK)
@@ -173,6 +180,7 @@ def fmha_fwd_kv4(q, cache, out, *, causal=True, counts=None, scale=None, lse=Non
                 written behind the length. The sums are the same bits every time.
     """
     import torch
+    _is_kv4("fmha_fwd_kv4", cache)
     lib = _abi.load()
     a = _abi.Kv4AttendArgs()
     a.q = _rows("fmha_fwd_kv4", "q", q, cache)
@@ -215,6 +223,8 @@ def kv4_evict(cache, weights, into, *, keep, recent=0, first=0, kept=None, weigh
                  memory it must not share.
     """
     import torch
+    _is_kv4("kv4_evict", cache)
+    _is_kv4("kv4_evict", into, "into")
     lib = _abi.load()
     a = _abi.Kv4EvictArgs()
     if into.device != cache.device:

@@ -161,6 +161,29 @@ __device__ __forceinline__ float sum_factor(float& l, float d) {
     l = halves ? l * f : l;
     return f;
 }
+// Weights w = 2^(c s + e - M), e the exponent of what a group of tokens has taken out of V, go into the sum as w 2^-e. That loses the ones that are no f32 number, which matters where e lies far below the
+// largest that M may follow. As long as a run of steps has exponents within kNear of its first one, what gets lost is less than 2^-54 of the largest term: M lies at most 8 higher relative to the largest
+// c s + e than to any other (a slack of 8, or 14 less the 6 that M lies below it), so that a weight below 2^-126, or a sum that a change of M takes there, belongs to a c s that is lower by 126 - 8 - 2 kNear.
+// From the first exponent outside on the run is `wide`: 2^(c s - M) is summed up for itself, times 2^kWide, which keeps it within f32 (with e from -100 to 124 it is 2^116 at most, the largest term 2^-116 at
+// least), and changes of M take the sums along in halves.
+constexpr int kNear = 32, kWide = 8;
+constexpr float kWideDown = 1.0f / (1 << kWide);
+__device__ __forceinline__ bool is_near(int e, int first) { return static_cast<uint32_t>(e - first + kNear) <= 2u * kNear; }
+__device__ __forceinline__ float ex2_wide(float x) {   // with results below 2^-126
+    float y;
+    asm("ex2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// what a warp's run of steps has met of exponents; the same in all lanes
+struct Exponents {
+    static constexpr int kNone = 1 << 20;
+    int first = kNone;
+    bool wide = false;
+    __device__ __forceinline__ void add(int e) {
+        first = first == kNone ? e : first;
+        wide = wide || !is_near(e, first);
+    }
+};
 __device__ __forceinline__ float lg2(float x) {
     float y;
     asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));

@@ -202,12 +202,13 @@ __device__ const LostPages kNowhere;
 // 32 tokens: scores, softmax, and their part of O
 template <int NT, bool kEdge>
 __device__ __forceinline__ void attend_unit(float (&o)[NT][8][4], float (&m)[NT][2], float (&l)[NT][2], const QueryRows<NT>& x, const uint8_t* k_codes, const uint8_t* v_codes, uint32_t granule,
-                                            const TokenFactors& f, int e, uint32_t tok0, const uint4* q_shared, float* kept_scores, uint32_t kept_rows, uint32_t length) {
+                                            const TokenFactors& f, int e, uint32_t tok0, const uint4* q_shared, float* kept_scores, uint32_t kept_rows, uint32_t length, Exponents& seen) {
+    seen.add(e);
     const unsigned lane = threadIdx.x & 31u, gid = lane >> 2, tig = lane & 3u;
     const uint32_t row = row_token(gid);
     float s[2][NT][4];
     scores<NT>(s, k_codes, granule, f.k, x, q_shared);
-    const float ef = static_cast<float>(e), inv = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+    const float ef = static_cast<float>(e), inv = seen.wide ? 0.0f : __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
 #pragma unroll
     for (int gr = 0; gr < 2; ++gr) {
 #pragma unroll
@@ -229,7 +230,7 @@ __device__ __forceinline__ void attend_unit(float (&o)[NT][8][4], float (&m)[NT]
             }
         }
     }
-    bool over = false;
+    bool over = seen.wide;
     float top[NT][2];
 #pragma unroll
     for (int g = 0; g < NT; ++g) {
@@ -249,11 +250,24 @@ __device__ __forceinline__ void attend_unit(float (&o)[NT][8][4], float (&m)[NT]
                 t = fmaxf(t, __shfl_xor_sync(0xFFFFFFFFu, t, 8));
                 t = fmaxf(t, __shfl_xor_sync(0xFFFFFFFFu, t, 16));
                 t = fmaxf(t, m[g][j]);
-                const float c = ex2(m[g][j] - t);
+                const float c = ex2(m[g][j] - t), cl = sum_factor(l[g][j], m[g][j] - t);
                 m[g][j] = t;
-                l[g][j] *= c;
+                l[g][j] *= cl;
 #pragma unroll
                 for (int i = 0; i < 8; ++i) o[g][i][j] *= c, o[g][i][2 + j] *= c;
+            }
+        }
+        if (seen.wide) {
+#pragma unroll
+            for (int gr = 0; gr < 2; ++gr) {
+#pragma unroll
+                for (int g = 0; g < NT; ++g) {
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        const float up = static_cast<float>(kWide) - m[g][j];
+                        l[g][j] = fmaf(ex2_wide(fmaf(s[gr][g][j], x.factor[g][j], up)) + ex2_wide(fmaf(s[gr][g][2 + j], x.factor[g][j], up)), kWideDown, l[g][j]);
+                    }
+                }
             }
         }
     }
@@ -396,6 +410,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : NT == 2 ? 3 : 2) kv4_a
         }
         float* kept = p.scores == nullptr ? nullptr : p.scores + ((static_cast<size_t>(b) * p.c.HK + head) * (static_cast<size_t>(p.c.table_width) << p.c.page_log2) + first * kTile + in_tile) * kept_rows;
         bool ok = true;
+        Exponents seen;
         uint32_t tok0 = first * kTile + in_tile, my_turn = (warp + 2u * kWarps - (kStages - 1u)) % kWarps;   // tiles until this warp brings one
         for (uint32_t i = 0; i < n_tiles; ++i, tok0 += kTile) {
             if (!sm100::mbar_wait(full0 + 8u * stage, phase, &sh.failed)) {
@@ -408,9 +423,9 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : NT == 2 ? 3 : 2) kv4_a
                 __syncwarp();
                 const uint8_t* codes = raw + unit_at;
                 if (tok0 + kUnit <= low) {
-                    attend_unit<NT, false>(o, m, l, x, codes, codes + v_codes, granule, sh.f[warp], e, tok0, sh.q, kept == nullptr ? nullptr : kept + i * kTile * kept_rows, kept_rows, length);
+                    attend_unit<NT, false>(o, m, l, x, codes, codes + v_codes, granule, sh.f[warp], e, tok0, sh.q, kept == nullptr ? nullptr : kept + i * kTile * kept_rows, kept_rows, length, seen);
                 } else {
-                    attend_unit<NT, true>(o, m, l, x, codes, codes + v_codes, granule, sh.f[warp], e, tok0, sh.q, kept == nullptr ? nullptr : kept + i * kTile * kept_rows, kept_rows, length);
+                    attend_unit<NT, true>(o, m, l, x, codes, codes + v_codes, granule, sh.f[warp], e, tok0, sh.q, kept == nullptr ? nullptr : kept + i * kTile * kept_rows, kept_rows, length, seen);
                 }
             }
             __syncwarp();   // this warp is done with the stage and its factors
@@ -475,7 +490,9 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : NT == 2 ? 3 : 2) kv4_a
                 for (int k = 0; k < 8; ++k) acc[k] = 0.0f;
 #pragma unroll
                 for (unsigned w = 0; w < kWarps; ++w) {
-                    total = fmaf(sh.l[w][8 * g + r], ex2(sh.m[w][8 * g + r] - top), total);
+                    float l_w = sh.l[w][8 * g + r];
+                    const float f = sum_factor(l_w, sh.m[w][8 * g + r] - top);
+                    total = fmaf(l_w, f, total);
                     const float4* src = reinterpret_cast<const float4*>(reinterpret_cast<const float*>(sh.ring[0]) + w * 1024u + r * 128u + d);
                     const float4 a = src[0], c = src[1];
                     acc[0] += a.x, acc[1] += a.y, acc[2] += a.z, acc[3] += a.w, acc[4] += c.x, acc[5] += c.y, acc[6] += c.z, acc[7] += c.w;

@@ -120,6 +120,55 @@ __device__ __forceinline__ void note_nan(uint4& first, uint32_t nan, uint32_t fr
     }
 }
 
+struct RowSums {
+    float m, l;
+};
+// A wide step's part of a row's sum (kv4.cuh): brings m to where the step will have it, O and l with it, and adds up the weights. All lanes, in front of the step, which does the rest. seen: tokens of the
+// step that the row sees
+__device__ __noinline__ RowSums sum_wide(uint32_t t_s, uint32_t t_o, float c, float e, int seen, bool first, RowSums now) {
+    float most = -INFINITY, m = now.m, l = now.l;
+#pragma unroll 1
+    for (uint32_t k = 0; k < kStepTokens / 8u; ++k) {   // the largest, then the sums; 16 tokens at a time
+        const uint32_t b = k % (kStepTokens / 16u);
+        if (k == kStepTokens / 16u) {
+            most = fmaf(most, c, e);
+            const bool over = most > m + kSlack;
+            if (__any_sync(0xFFFFFFFFu, over)) {
+                const float next = over ? most : m, f = ex2(m - next), fl = sum_factor(l, m - next);
+                m = next;
+                l *= fl;
+                if (!first) {
+#pragma unroll 1
+                    for (uint32_t x = 0; x < 8u; ++x) {
+                        uint32_t o[16];
+                        tmem_ld16(t_o + 16u * x, o);
+                        tmem_wait_ld();
+                        reg_fence16(o);
+#pragma unroll
+                        for (int y = 0; y < 16; ++y) o[y] = __float_as_uint(__uint_as_float(o[y]) * f);
+                        tmem_st16(t_o + 16u * x, o);
+                    }
+                    tmem_wait_st();
+                }
+            }
+        }
+        uint32_t x[16];
+        tmem_ld16(t_s + 16u * b, x);
+        tmem_wait_ld();
+        reg_fence16(x);
+        const float up = static_cast<float>(kWide) - m;
+        float top = -INFINITY, sum = 0.0f;
+#pragma unroll
+        for (int z = 0; z < 16; ++z) {
+            const float y = z < seen - static_cast<int>(16u * b) ? __uint_as_float(x[z]) : -INFINITY;
+            top = fmaxf(top, y), sum += ex2_wide(fmaf(y, c, up));
+        }
+        if (k < kStepTokens / 16u) most = fmaxf(most, top);
+        else l = fmaf(sum, kWideDown, l);
+    }
+    return {m, l};
+}
+
 __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_constant__ Kv4AttendParams p, uint32_t row_tiles) {
     extern __shared__ uint8_t smem_raw[];
     Shared& sh = *reinterpret_cast<Shared*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023u) & ~static_cast<uintptr_t>(1023u));
@@ -236,6 +285,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
                 if (lane == 0u) mbar_arrive(bar(kQFull + q));
                 more = left > 0u;
                 if (more) plan_next();
+                Exponents seen;
                 for (uint32_t j = 0; j < steps && ok; ++j) {
                     // (not the K tile's barrier: while a group is still storing the rows of the segment before, that one may already be two steps on)
                     const uint32_t slot = (step0 + j) % kFactorSlots;
@@ -243,10 +293,15 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
                     const uint4 mk = sh.most[slot][0], mv = sh.most[slot][1];
                     const int ek = group_exponent(max(max(mk.x, mk.y), max(mk.z, mk.w))), e = group_exponent(max(max(mv.x, mv.y), max(mv.z, mv.w)));
                     const float c = fmaxf(c_row * __uint_as_float(static_cast<uint32_t>(127 + ek - kUp) << 23), kLeast), ef = static_cast<float>(e);
+                    seen.add(e);
                     ok = ok && mbar_wait(bar(kSFull + q), s_phase, failed);
                     if (!ok) break;
                     s_phase ^= 1u;
                     tc_fence_after_sync();
+                    if (seen.wide) {
+                        const RowSums x = sum_wide(t_s, t_o, c, ef, static_cast<int>(limit) - static_cast<int>((seg.first + j) * kStepTokens), j == 0u, {m, l});
+                        m = x.m, l = x.l;
+                    }
                     uint32_t s[4][32];
 #pragma unroll
                     for (int k = 0; k < 4; ++k) tmem_ld32(t_s + 32u * k, s[k]);
@@ -310,7 +365,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
                             if (lane == 0u) mbar_arrive(bar(kPFull + 2u * q + (k >> 1)));
                         }
                     }
-                    l = fmaf(l0 + l1, __uint_as_float(static_cast<uint32_t>(127 - e) << 23), l);
+                    l = fmaf(l0 + l1, seen.wide ? 0.0f : __uint_as_float(static_cast<uint32_t>(127 - e) << 23), l);
                 }
                 step0 += seg.steps;
                 const Segment done = seg;

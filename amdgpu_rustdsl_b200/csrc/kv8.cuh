@@ -64,17 +64,6 @@ __device__ __forceinline__ uint32_t e4m3x4_of_f16(uint32_t lo, uint32_t hi) {
 }
 // A scale's exponent, and 2 to minus that, from its bits. (Scales are powers of two from 2^-90 to 2^119: sums of weights up to 2^14 times 2^90 stay within f32.)
 __device__ __forceinline__ int exponent_of(uint32_t scale) { return min(max(static_cast<int>(scale >> 23) - 127, -90), 119); }
-// Weights w = 2^(c s + e - M) go into the sum as w 2^-e. That loses the ones that are no f32 number, which matters where e lies far below the largest that M may follow. As long as a run of steps has
-// exponents within kNear of its first one, what gets lost is less than 2^-54 of the largest term: M lies 6 below the largest c s + e at least and 14 below any at most, so that a weight below 2^-126, or a
-// sum that a change of M takes there, belongs to a c s that is lower by 126 + 6 - 14 - 2 kNear. From the first exponent outside on the run is `wide`: 2^(c s - M) is summed up for itself, times 2^kWide, which
-// keeps it within f32 (with e >= -90 it is 2^120 at most, the largest term, with e <= 119, 2^-97 at least), and changes of M take the sums along in halves.
-constexpr int kNear = 32, kWide = 16;
-__device__ __forceinline__ bool is_near(int e, int first) { return static_cast<uint32_t>(e - first + kNear) <= 2u * kNear; }
-__device__ __forceinline__ float ex2_wide(float x) {   // with results below 2^-126
-    float y;
-    asm("ex2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
 __device__ __forceinline__ float power_of(int e) { return __uint_as_float(static_cast<uint32_t>(127 + e) << 23); }
 
 }  // namespace kv8

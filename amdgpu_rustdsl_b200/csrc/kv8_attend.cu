@@ -124,13 +124,6 @@ struct LostBlocks {
 };
 __device__ const LostBlocks kNowhere;
 
-// What a run of steps has met of V's exponents (kv8.cuh); the same in all lanes
-struct Exponents {
-    int first;
-    bool wide;
-};
-constexpr int kNone = 1 << 20;
-
 // G blocks of 16 tokens: scores, softmax, and their part of O: o[g][i][j], d = 16 gid + 2 i and, from [2 + j], the next, of the column 2 tig + j
 template <int NT, int G, bool kEdge>
 __device__ __forceinline__ void attend_blocks(float (&o)[NT][8][4], float (&m)[NT][2], float (&l)[NT][2], const QueryRows<NT>& x, const uint8_t* unit, uint32_t tok0, const uint4* q_shared, uint32_t length, Exponents& seen) {
@@ -213,9 +206,10 @@ __device__ __forceinline__ void attend_blocks(float (&o)[NT][8][4], float (&m)[N
         }
     }
     float c[G][NT][2], e[G], back[G];
-    seen.first = seen.first == kNone ? exponent_of(meta[0].y) : seen.first;
 #pragma unroll
-    for (int gr = 0; gr < G; ++gr) seen.wide = seen.wide || !(dead[gr] || is_near(exponent_of(meta[gr].y), seen.first));
+    for (int gr = 0; gr < G; ++gr) {
+        if (!dead[gr]) seen.add(exponent_of(meta[gr].y));
+    }
 #pragma unroll
     for (int gr = 0; gr < G; ++gr) {
         const int exponent = exponent_of(meta[gr].y);
@@ -262,7 +256,7 @@ __device__ __forceinline__ void attend_blocks(float (&o)[NT][8][4], float (&m)[N
 #pragma unroll
                     for (int j = 0; j < 2; ++j) {
                         const float up = static_cast<float>(kWide) - m[g][j], more = ex2_wide(fmaf(s[gr][g][j], c[gr][g][j], up)) + ex2_wide(fmaf(s[gr][g][2 + j], c[gr][g][j], up));
-                        l[g][j] = fmaf(more, 1.0f / (1 << kWide), l[g][j]);
+                        l[g][j] = fmaf(more, kWideDown, l[g][j]);
                     }
                 }
             }
@@ -445,7 +439,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) kv8_attend_kernel(c
             for (int i = 0; i < 8; ++i) o[g][i][0] = o[g][i][1] = o[g][i][2] = o[g][i][3] = 0.0f;
         }
         bool ok = true;
-        Exponents seen = {kNone, false};
+        Exponents seen;
 #pragma unroll 1
         for (uint32_t k = 0; k < units; ++k) {
             ok = __all_sync(0xFFFFFFFFu, sm100::mbar_wait(full0 + 8u * stage, phase, &sh.failed));

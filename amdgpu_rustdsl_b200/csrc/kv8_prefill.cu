@@ -68,7 +68,7 @@ struct Shared {
     uint4 meta[kRawStages][kBlocks];   // and its scales and masks
     uint32_t plain[kScaleSlots];       // whether every token of a step has numbers
     alignas(16) float scales[kScaleSlots][3][8];   // of a step's blocks: scale of K, exponent e of V's, 2^-e (0 in wide steps)
-    uint32_t wide[kScaleSlots];        // whether a step is (kv8.cuh)
+    uint32_t wide[kScaleSlots];        // whether a step is (kv4.cuh)
     uint32_t nan_from[kSegmentSlots];  // of a segment: the first token that has NaN in its V, all ones where none has
     unsigned long long bars[kBars];
     Sums part[kThreads / 32];
@@ -140,8 +140,8 @@ __device__ __forceinline__ uint4* piece_at(uint8_t* tile, uint32_t row, uint32_t
 struct RowSums {
     float m, l;
 };
-// A wide step's part of a row's sum (kv8.cuh): brings m to where the step will have it, O and l with it, and adds up the weights. All lanes, in front of the step, which does the rest; a function of its own,
-// since among the step's instructions it costs prompts that have no such steps another 2 us
+// A wide step's part of a row's sum (kv4.cuh): brings m to where the step will have it, O and l with it, and adds up the weights. All lanes, in front of the step, which does the rest; a function of its own,
+// since among the step's instructions it costs prompts that have no such steps another 7 us
 __device__ __noinline__ RowSums sum_wide(Shared& sh, uint32_t slot, uint32_t t_s, uint32_t t_o, float c_row, int seen, bool first, uint32_t product, uint32_t p_phase, RowSums now) {
     float most = -INFINITY, m = now.m, l = now.l;
 #pragma unroll 1
@@ -183,7 +183,7 @@ __device__ __noinline__ RowSums sum_wide(Shared& sh, uint32_t slot, uint32_t t_s
             top = fmaxf(top, y), sum += ex2_wide(fmaf(y, c, up));
         }
         if (k < kBlocks) most = fmaxf(most, fmaf(top, c, sh.scales[slot][1][b]));
-        else l = fmaf(sum, 1.0f / (1 << kWide), l);
+        else l = fmaf(sum, kWideDown, l);
     }
     return {m, l};
 }

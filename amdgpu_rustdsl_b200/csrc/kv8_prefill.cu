@@ -318,7 +318,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
                 for (uint32_t j = 0; j < steps && ok; ++j) {
                     // (not the K tile's barrier: while a group is still storing the rows of the segment before, that one may already be two steps on)
                     const uint32_t slot = (step0 + j) % kScaleSlots;
-                    ok = __all_sync(0xFFFFFFFFu, mbar_wait2(bar(kScales + slot), (step0 + j) / kScaleSlots & 1u, bar(kSFull + q), s_phase, failed));
+                    ok = mbar_wait(bar(kScales + slot), (step0 + j) / kScaleSlots & 1u, failed);
+                    const bool wide = sh.wide[slot] != 0u;
+                    ok = __all_sync(0xFFFFFFFFu, ok && mbar_wait(bar(kSFull + q), s_phase, failed));
                     if (!ok) break;
                     s_phase ^= 1u;
                     tc_fence_after_sync();
@@ -328,7 +330,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
                         tmem_ld32(t_s + 32u, *reinterpret_cast<uint32_t(*)[32]>(s + 32));
                         tmem_ld16(t_s + 64u, *reinterpret_cast<uint32_t(*)[16]>(s + 64));
                     };
-                    if (sh.wide[slot] != 0u) {
+                    if (wide) {
                         const RowSums x = sum_wide(sh, slot, t_s, t_o, c_row, static_cast<int>(limit) - static_cast<int>((seg.first + j) * kStep), j == 0u, bar(kPFree + q), p_phase, {m, l});
                         m = x.m, l = x.l;
                     }

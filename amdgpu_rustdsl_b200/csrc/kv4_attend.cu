@@ -598,9 +598,9 @@ __global__ void __launch_bounds__(kTogether ? 32 * kTogether : 256) kv4_combine_
     if (p.lse != nullptr && lane == 0u) p.lse[(static_cast<size_t>(b) * p.H + h) * p.S + i] = none ? -INFINITY : (m + lg2(l)) * kLn2;
 }
 
-// The same for items of many rows that a few CTAs each have a part of: a warp has kRows rows, whose parts come in together, one CTA's behind the other's, in the same order and to the same bits.
-// (A warp a row took as many rounds of CTAs, each as long as three trips to memory one behind the other: prompts of 4096 rows, 8-bit cache, 459 us and 456 so, 4 ragged chunks of 333 rows 69.7 and
-// 68.4; 2, 4 and 8 rows a warp are alike. Bound by the trips, then by L2.)
+// The same for items of many rows of which most have one or two parts: a warp has kRows rows, whose parts come in together, one CTA's behind the other's, in the same order and to the same bits. With a warp a
+// row there are kRows times as many CTAs, most of which find nothing to do (4-bit cache, 4096 rows over 8192 tokens, 128 items: 437.2 us and 434.8 so; 4 x 333 ragged rows, 128 items too: alike). Items of more
+// parts have a warp a row, whose trips to memory are then under way beside one another (512 rows over 16384 tokens, 32 items: 97.7 us so and 92.7 with a warp a row, 4 x 100 ragged rows, 64 items: 89.3 and 85.6).
 template <uint32_t kRows>
 __global__ void __launch_bounds__(256) kv4_combine_rows_kernel(const __grid_constant__ Kv4AttendParams p, uint32_t rows, uint32_t row_tiles, uint32_t grid) {
     pdl_launch();
@@ -659,7 +659,8 @@ cudaError_t launch_combine_few(const Kv4AttendParams& p, uint32_t slots, uint32_
 cudaError_t launch_combine_many(const Kv4AttendParams& p, uint32_t per, uint32_t row_tiles, uint32_t grid, cudaStream_t stream, bool together) {
     constexpr uint32_t kRows = 4;
     const uint32_t rows = p.S * p.group, most = rows < per ? rows : per, entries = begun_entries(p.c, row_tiles, grid), parts = grid / entries;
-    if (few_parts(p.c, row_tiles, grid)) return kv4_launch(kv4_combine_rows_kernel<kRows>, dim3(entries, (most + 8u * kRows - 1u) / (8u * kRows)), 256u, 0, stream, p, per, row_tiles, grid);
+    const uint64_t items = static_cast<uint64_t>(p.c.B) * p.c.HK * row_tiles;
+    if (!together && 2u * items > grid) return kv4_launch(kv4_combine_rows_kernel<kRows>, dim3(entries, (most + 8u * kRows - 1u) / (8u * kRows)), 256u, 0, stream, p, per, row_tiles, grid);
     if (!together) return kv4_launch(kv4_combine_kernel<0>, dim3(entries, (most + 7u) / 8u), 256u, 0, stream, p, per, row_tiles, grid);
     if (parts > 16u) return kv4_launch(kv4_combine_kernel<16>, dim3(entries, most), 512u, 0, stream, p, per, row_tiles, grid);
     return kv4_launch(kv4_combine_kernel<4>, dim3(entries, most), 128u, 0, stream, p, per, row_tiles, grid);

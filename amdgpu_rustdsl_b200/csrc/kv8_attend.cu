@@ -312,10 +312,10 @@ __device__ __forceinline__ void attend_unit(float (&o)[NT][8][4], float (&m)[NT]
     }
 }
 
-constexpr uint32_t ctas_per_sm(int groups) { return groups >= 1 ? 2u : 1u; }
+constexpr uint32_t kCtasPerSm = 2;
 
 template <int NT>
-__global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) kv8_attend_kernel(const __grid_constant__ Kv8AttendParams p, bool whole_items) {
+__global__ void __launch_bounds__(kThreads, kCtasPerSm) kv8_attend_kernel(const __grid_constant__ Kv8AttendParams p, bool whole_items) {
     extern __shared__ __align__(128) uint8_t smem_raw[];
     CtaShared<NT>& sh = *reinterpret_cast<CtaShared<NT>*>(smem_raw);
     const unsigned lane = threadIdx.x & 31u, warp = threadIdx.x >> 5, gid = lane >> 2, tig = lane & 3u;
@@ -550,15 +550,15 @@ uint32_t groups_of(uint32_t rows) { return (rows + 7u) / 8u; }
 // Items of up to so many steps, which is up to 512 tokens, are not cut: a launch and the way through memory are saved, 2 heads of 256 tokens 9.7 us in place of 11.8
 constexpr uint32_t kWholeSteps = 4;
 uint32_t most_steps(const Kv4View& c) { return static_cast<uint32_t>(((static_cast<unsigned long long>(c.table_width) << c.page_log2) + kStepTokens - 1u) / kStepTokens); }
-uint32_t attend_grid(const Kv4View& c, uint32_t groups) {
-    const unsigned long long per_sm = ctas_per_sm(static_cast<int>(groups)), steps = most_steps(c);
-    const unsigned long long most = (steps <= kWholeSteps ? 1ull : steps) * c.B * c.HK, full = per_sm * static_cast<unsigned long long>(current_sm_count());
+uint32_t attend_grid(const Kv4View& c) {
+    const unsigned long long steps = most_steps(c);
+    const unsigned long long most = (steps <= kWholeSteps ? 1ull : steps) * c.B * c.HK, full = static_cast<unsigned long long>(kCtasPerSm) * static_cast<unsigned long long>(current_sm_count());
     return static_cast<uint32_t>(most < full ? (most ? most : 1ull) : full);
 }
 
 template <int NT>
 cudaError_t launch_rows(const Kv8AttendParams& p, cudaStream_t stream) {
-    const uint32_t grid = attend_grid(p.c, NT);
+    const uint32_t grid = attend_grid(p.c);
     const size_t smem = sizeof(CtaShared<NT>);
     static std::atomic<bool> set[64];
     int dev = 0;
@@ -636,7 +636,7 @@ cudaError_t launch_many(const Kv8AttendParams& p, cudaStream_t stream) {
 uint64_t kv8_attend_workspace(const Kv4View& c, uint32_t S, uint32_t H) {
     const uint32_t rows = S * (H / c.HK);
     if (rows > kMostFew) return kv4_partial_bytes(kv8_prefill_grid(), kv8_prefill_rows());
-    return kv4_partial_bytes(attend_grid(c, groups_of(rows)), 8u * groups_of(rows));
+    return kv4_partial_bytes(attend_grid(c), 8u * groups_of(rows));
 }
 
 cudaError_t launch_kv8_attend(const Kv8AttendParams& p, cudaStream_t stream) {

@@ -67,7 +67,7 @@ struct Shared {
     uint8_t raw_k[kRawStages][kBlocks][kVCodes], raw_v[kRawStages][kBlocks][kMeta - kVCodes];   // a step's codes as they come
     uint4 meta[kRawStages][kBlocks];   // and its scales and masks
     uint32_t plain[kScaleSlots];       // whether every token of a step has numbers
-    alignas(16) float scales[kScaleSlots][3][8];   // of a step's blocks: scale of K, exponent e of V's, 2^-e (0 in wide steps)
+    alignas(16) float scales[kScaleSlots][3][8];   // of a step's blocks: scale of K, exponent e of V's, 2^-e
     uint32_t wide[kScaleSlots];        // whether a step is (kv4.cuh)
     uint32_t nan_from[kSegmentSlots];  // of a segment: the first token that has NaN in its V, all ones where none has
     unsigned long long bars[kBars];
@@ -140,23 +140,24 @@ __device__ __forceinline__ uint4* piece_at(uint8_t* tile, uint32_t row, uint32_t
 struct RowSums {
     float m, l;
 };
-// A wide step's part of a row's sum (kv4.cuh): brings m to where the step will have it, O and l with it, and adds up the weights. All lanes, in front of the step, which does the rest; a function of its own,
-// since among the step's instructions it costs prompts that have no such steps another 7 us
-__device__ __noinline__ RowSums sum_wide(Shared& sh, uint32_t slot, uint32_t t_s, uint32_t t_o, float c_row, int seen, bool first, uint32_t product, uint32_t p_phase, RowSums now) {
+// A wide step (kv4.cuh) of a row, 16 tokens at a time: brings m to where the step has it, O and l with it, adds the weights up for themselves and leaves them to the product. All lanes. seen: tokens of
+// the step that the row sees; product: the barrier of the step before's, 0 where there is none
+__device__ __forceinline__ RowSums wide_step(Shared& sh, uint32_t slot, uint32_t t_s, float c_row, int seen, uint32_t product, uint32_t p_phase, uint32_t s_free, uint32_t p_full, RowSums now) {
+    const uint32_t t_p = t_s + kColP, t_o = t_s + kColO;
     float most = -INFINITY, m = now.m, l = now.l;
 #pragma unroll 1
-    for (uint32_t k = 0; k < 2u * kBlocks; ++k) {   // the largest, then the sums
+    for (uint32_t k = 0; k < 2u * kBlocks; ++k) {   // the largest, then the weights
         const uint32_t b = k % kBlocks;
         if (k == kBlocks) {
-            const bool over = most - kUpF > m + kSlack;
-            if (__any_sync(0xFFFFFFFFu, over)) {
-                const float next = over ? most - kUpF : m, f = ex2(m - next), fl = sum_factor(l, m - next);
-                m = next;
-                l *= fl;
-                if (!first) {
-                    (void)mbar_wait(product, p_phase, &sh.failed);   // (the step waits for it too: the parity stays)
-                    __syncwarp();
-                    tc_fence_after_sync();
+            most -= kUpF;
+            const float next = most > m + kSlack ? most : m, f = ex2(m - next), fl = sum_factor(l, m - next);
+            m = next;
+            l *= fl;
+            if (product != 0u) {
+                (void)mbar_wait(product, p_phase, &sh.failed);
+                __syncwarp();
+                tc_fence_after_sync();
+                if (__any_sync(0xFFFFFFFFu, f != 1.0f)) {
 #pragma unroll 1
                     for (uint32_t x = 0; x < 8u; ++x) {
                         uint32_t o[16];
@@ -167,7 +168,6 @@ __device__ __noinline__ RowSums sum_wide(Shared& sh, uint32_t slot, uint32_t t_s
                         for (int y = 0; y < 16; ++y) o[y] = __float_as_uint(__uint_as_float(o[y]) * f);
                         tmem_st16(t_o + 16u * x, o);
                     }
-                    tmem_wait_st();
                 }
             }
         }
@@ -175,16 +175,29 @@ __device__ __noinline__ RowSums sum_wide(Shared& sh, uint32_t slot, uint32_t t_s
         tmem_ld16(t_s + 16u * b, x);
         tmem_wait_ld();
         reg_fence16(x);
-        const float c = fmaxf(c_row * sh.scales[slot][0][b], kLeast), up = static_cast<float>(kWide) - m;
+        const float c = fmaxf(c_row * sh.scales[slot][0][b], kLeast), shift = sh.scales[slot][1][b], up = static_cast<float>(kWide) - m;
         float top = -INFINITY, sum = 0.0f;
 #pragma unroll
-        for (int z = 0; z < 16; ++z) {
-            const float y = z < seen - static_cast<int>(16u * b) ? __uint_as_float(x[z]) : -INFINITY;
-            top = fmaxf(top, y), sum += ex2_wide(fmaf(y, c, up));
+        for (int z = 0; z < 16; ++z) x[z] = z < seen - static_cast<int>(16u * b) ? x[z] : 0xFF800000u;
+        if (k < kBlocks) {
+#pragma unroll
+            for (int z = 0; z < 16; ++z) top = fmaxf(top, __uint_as_float(x[z]));
+            most = fmaxf(most, fmaf(top, c, shift));
+        } else {
+#pragma unroll
+            for (int z = 0; z < 8; ++z) {
+                const float u = __uint_as_float(x[2 * z]), v = __uint_as_float(x[2 * z + 1]);
+                sum += ex2_wide(fmaf(u, c, up)) + ex2_wide(fmaf(v, c, up));
+                x[z] = pack_f16x2(ex2(fmaf(u, c, shift - m)), ex2(fmaf(v, c, shift - m)));
+            }
+            l = fmaf(sum, kWideDown, l);
+            tmem_st8(t_p + 8u * b, x);
         }
-        if (k < kBlocks) most = fmaxf(most, fmaf(top, c, sh.scales[slot][1][b]));
-        else l = fmaf(sum, kWideDown, l);
     }
+    tmem_wait_st();
+    tc_fence_before_sync();
+    __syncwarp();
+    if ((threadIdx.x & 31u) == 0u) mbar_arrive(s_free), mbar_arrive(p_full);
     return {m, l};
 }
 
@@ -315,26 +328,23 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
                 const bool exists = row < p.S * p.group;
                 const uint32_t limit = !exists || i >= n ? 0u : p.causal ? length - n + i + 1u : length;
                 float m = kLowest, l = 0.0f;
-                for (uint32_t j = 0; j < steps && ok; ++j) {
+                uint32_t j = 0;
+                // the step's scales and scores; false: it is a wide one, or a wait has run out
+                const auto is_near_step = [&]() {
                     // (not the K tile's barrier: while a group is still storing the rows of the segment before, that one may already be two steps on)
                     const uint32_t slot = (step0 + j) % kScaleSlots;
-                    ok = mbar_wait(bar(kScales + slot), (step0 + j) / kScaleSlots & 1u, failed);
-                    const bool wide = sh.wide[slot] != 0u;
-                    ok = __all_sync(0xFFFFFFFFu, ok && mbar_wait(bar(kSFull + q), s_phase, failed));
-                    if (!ok) break;
+                    ok = __all_sync(0xFFFFFFFFu, mbar_wait2(bar(kScales + slot), (step0 + j) / kScaleSlots & 1u, bar(kSFull + q), s_phase, failed));
                     s_phase ^= 1u;
+                    return ok && sh.wide[slot] == 0u;
+                };
+                for (; j < steps && ok; ++j) {
+                    if (!is_near_step()) break;
+                    const uint32_t slot = (step0 + j) % kScaleSlots;
                     tc_fence_after_sync();
                     uint32_t s[kStep];
-                    const auto load = [&]() {
-                        tmem_ld32(t_s, *reinterpret_cast<uint32_t(*)[32]>(s));
-                        tmem_ld32(t_s + 32u, *reinterpret_cast<uint32_t(*)[32]>(s + 32));
-                        tmem_ld16(t_s + 64u, *reinterpret_cast<uint32_t(*)[16]>(s + 64));
-                    };
-                    if (wide) {
-                        const RowSums x = sum_wide(sh, slot, t_s, t_o, c_row, static_cast<int>(limit) - static_cast<int>((seg.first + j) * kStep), j == 0u, bar(kPFree + q), p_phase, {m, l});
-                        m = x.m, l = x.l;
-                    }
-                    load();
+                    tmem_ld32(t_s, *reinterpret_cast<uint32_t(*)[32]>(s));
+                    tmem_ld32(t_s + 32u, *reinterpret_cast<uint32_t(*)[32]>(s + 32));
+                    tmem_ld16(t_s + 64u, *reinterpret_cast<uint32_t(*)[16]>(s + 64));
                     float c[kBlocks], shift[kBlocks], back[kBlocks];
 #pragma unroll
                     for (int k = 0; k < static_cast<int>(kBlocks); ++k) c[k] = fmaxf(c_row * sh.scales[slot][0][k], kLeast), shift[k] = sh.scales[slot][1][k], back[k] = sh.scales[slot][2][k];
@@ -403,6 +413,18 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
                     tc_fence_before_sync();
                     __syncwarp();
                     if (lane == 0u) mbar_arrive(bar(kPFull + q));
+                }
+                // From the first wide step on all of them are. (Among the other steps' instructions, or as a call from there, this took 3 to 5 % of prompts that have none: 4096 rows over 8192 tokens 452 us without
+                // it, 457 so, 464 with the scales waited for in front of the scores)
+                for (bool here = true; j < steps && ok; ++j) {
+                    if (!here) (void)is_near_step();
+                    here = false;
+                    if (!ok) break;
+                    tc_fence_after_sync();
+                    const RowSums x = wide_step(sh, (step0 + j) % kScaleSlots, t_s, c_row, static_cast<int>(limit) - static_cast<int>((seg.first + j) * kStep), j > 0u ? bar(kPFree + q) : 0u, p_phase, bar(kSFree + q),
+                                                bar(kPFull + q), {m, l});
+                    m = x.m, l = x.l;
+                    p_phase ^= j > 0u;
                 }
                 step0 += seg.steps;
                 if (!ok) break;
@@ -716,7 +738,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
                         const bool plain = !__any_sync(0xFFFFFFFFu, lane < kBlocks && (live != 0xFFFFu || meta.z != 0u));
                         if (lane < kBlocks) {
                             float* of = sh.scales[slot][0] + lane;
-                            of[0] = __uint_as_float(meta.x), of[8] = static_cast<float>(e), of[16] = wide ? 0.0f : power_of(-e);
+                            of[0] = __uint_as_float(meta.x), of[8] = static_cast<float>(e), of[16] = power_of(-e);
                         }
                         uint32_t first = 0xFFFFFFFFu;
                         if (!plain) {

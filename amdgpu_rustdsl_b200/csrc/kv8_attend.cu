@@ -14,8 +14,9 @@
 // Softmax in base 2 with a running reference per row: w = 2^(c s + e - M), e the exponent of V's scale, goes into the second product, w 2^-e into the sum. M follows the largest c s + e,
 // less 2^kUp, since f16 has more room above 1 than a weight needs; it moves when a value exceeds it by another 2^kSlack, by a vote of the warp.
 //
-// Bound by bytes where sequences are long: 64 of 16384 tokens, 8 KV heads, 4 rows each, 343 us for 2.16 GB, 6.3 TB/s, 0.96 of the copy rate (16 of them: issue 29 %, tensor pipe 19 %, 8 warps an SM).
-// Ragged and short ones by what a change of item costs: 24 of up to 32768 tokens in pages of 16, 20 rows each, 60 us where the bytes take 32. Two CTAs an SM: three stages of four warps are 99 KB.
+// Bound by bytes where sequences are long: 64 of 16384 tokens, 8 KV heads, 4 rows each, 342 to 352 us by box for 2.16 GB, 6.1 to 6.3 TB/s, 0.94 to 0.96 of the copy rate (16 of them: issue 31 %, tensor pipe
+// 20 %, 8 warps an SM).
+// Ragged and short ones by what a change of item costs: 24 of up to 32768 tokens in pages of 16, 20 rows each, 61 us where the bytes take 32. Two CTAs an SM: three stages of four warps are 99 KB.
 #include "kv4_schedule.cuh"
 #include "kv8.cuh"
 #include "ptx_sm100.cuh"
@@ -541,8 +542,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv8_attend_kernel(const 
     }
 }
 
-// Rows of a KV head up to which this kernel is taken; more go to the tensor cores' tiles of 256 rows. (24 ragged sequences of up to 32768 tokens: 20, 24, 28 and 32 rows 60, 62, 94 and 96 us here and 115
-// there; of up to 8192 tokens 32 to 50 and 54; 64 of up to 2048 31 to 50 and 61. Above 24 rows registers spill, which is a part of the 94.)
+// Rows of a KV head up to which this kernel is taken; more go to the tensor cores' tiles of 256 rows. (24 ragged sequences of up to 32768 tokens: 20, 24, 28 and 32 rows 62, 64, 100 and 102 us here, 36
+// rows 120 there; of up to 8192 tokens 34 to 54 and 56; 64 of up to 2048 32 to 53 and 63. Above 24 rows registers spill, which is a part of the 100.)
 constexpr uint32_t kMostFew = 32;
 
 uint32_t groups_of(uint32_t rows) { return (rows + 7u) / 8u; }

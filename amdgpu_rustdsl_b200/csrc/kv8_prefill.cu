@@ -11,9 +11,9 @@
 // the products, S from shared memory, P V with P from tensor memory, and two groups of four warps do the softmax, one tile each, a thread a row. m moves only when a row's maximum
 // exceeds it by 2^(kUp + kSlack), so O is hardly ever rescaled.
 //
-// Bound by a tile's chain of scores, softmax and product: a step takes 2750 clocks, of which the products of both tiles are 1280, the exponentials of both 1280 (they meet: two warps of a scheduler do
-// them at the same time, which takes 1600), loads from tensor memory 250, the maximum 400, waits and stores 500. 4096 rows of 32 heads over 8192 tokens: 452 us among other calls (418 in a row), 0.91
-// PFLOP/s, 0.56 of what a matrix product measures; a change of item is 9000 clocks, of which a CTA of 4 ragged chunks of 333 rows (49.7 us) has one or two to its 16 steps.
+// Bound by a tile's chain of scores, softmax and product: a step takes 2780 clocks, of which the products of both tiles are 1280, the exponentials of both 1280 (they meet: two warps of a scheduler do
+// them at the same time, which takes 1600), loads from tensor memory 250, the maximum 400, waits and stores 500. 4096 rows of 32 heads over 8192 tokens: 455 us among other calls (425 in a row), 0.91
+// PFLOP/s, 0.56 of what a matrix product measures; a change of item is 9000 clocks, of which a CTA of 4 ragged chunks of 333 rows (50.4 us) has one or two to its 16 steps.
 // Slower: steps of 128 tokens with P over S (514 us in place of 464 then), of 64 (500), a quarter and three eighths of the exponentials by a polynomial (470 and 485 in place of 461), locks or turns between the two
 // groups at the exponentials (489 and more), K's and V's conversion by four warps each (504), query rows brought by the issuing warps (427 and 451 in place of 431, chunks 51.5 and 55 in place of 50.6),
 // O stored 64 columns at a time (507) or exchanged between four lanes first (441).

@@ -3,8 +3,8 @@
 // A CTA has one to four tokens. Its threads first work out the tokens' sines and cosines, one pair each, into shared memory: the phase is position * frequency in 64-bit integers, whole
 // turns fall out at the top, and the quarter turn is taken off before the rest becomes f32. Then a thread keeps those of the pairs that it has in every head and goes over the token's
 // heads, 16 bytes of both halves of a head (or of neighbours) at a time, four heads in flight.
-// Bound by bytes: each row once in and once out; with one token a sequence by the launch and one trip to memory. 4 x 4096 tokens of 40 heads of 128, bf16: 57.5 us for 336 MB, 5.8 TB/s, 0.89 of the
-// copy rate (16-bit elements in arrays of their own went through local memory: 108).
+// Bound by bytes: each row once in and once out; with one token a sequence by the launch and one trip to memory. 4 x 4096 tokens of 40 heads of 128, bf16: 57.5 to 59.7 us by box for 336 MB, 5.6 to 5.8 TB/s,
+// 0.86 to 0.89 of the copy rate (16-bit elements in arrays of their own went through local memory: 108).
 #include "../../include/fmha_rope_abi.h"
 #include "cache_args.cuh"
 
